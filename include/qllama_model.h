@@ -150,6 +150,155 @@ int ql_llama_generate(ql_llama* m, ql_kv* kv, int32_t seq, const int32_t* prompt
                       const ql_sampler_config* cfg, const double* uniforms, int32_t* out_tokens,
                       int32_t* n_out);
 
+/* ---- RMSNorm with the residual's addition, plain or 8-bit outputs ----------
+ * Per row: s = x + residual (f32; s = x without a residual),
+ *   y_i = s_i / sqrt(mean(s^2) + eps) * weight_i,
+ * the norm of TransformerBlock::forward_with_cache (layers.rs:615-631) with
+ * the residual's addition before it, in one pass, evaluated in f32 (the model
+ * host's f32 path keeps the reference's f64 order instead).  sum_out receives
+ * s rounded once to in_dtype; y is computed from the unrounded s.
+ *
+ * out_dtype F32, F16 or BF16: out [rows, hidden] holds y rounded once.
+ * out_dtype Q8_0: out [rows, hidden] holds int8 values and out_scale
+ * [rows, hidden/32] one f16 scale d per 32 columns, by the cache's rule:
+ * d = max|y| / 127, value = round(y / d) with ties away from zero, d stored
+ * as f16 (65504 at most; larger values saturate).  A block that holds a NaN or
+ * an infinity gets a NaN scale, so that it reads back as NaN.
+ *
+ * x and residual have x_stride / residual_stride elements from row to row
+ * (0 = hidden); sum_out, out and out_scale are contiguous.  sum_out may be x
+ * or residual itself, and out may be x, residual or neither, where the
+ * strides (and for out the types) are the same; any other overlap is not
+ * supported.  Device pointers, aligned to their element size. */
+typedef struct {
+  int32_t rows;          /* 0 is a no-op */
+  int32_t hidden;        /* a multiple of 32 for Q8_0 */
+  int32_t in_dtype;      /* x, residual, sum_out: F32, F16 or BF16 */
+  int32_t weight_dtype;  /* F32, F16 or BF16 */
+  int32_t out_dtype;     /* F32, F16, BF16 or Q8_0 */
+  float eps;             /* finite, not negative */
+  int64_t x_stride, residual_stride;
+  const void* x;
+  const void* residual;  /* may be NULL */
+  const void* weight;    /* [hidden] */
+  void* sum_out;         /* may be NULL; needs a residual */
+  void* out;
+  void* out_scale;       /* Q8_0 only */
+} ql_norm_args;
+
+int ql_rms_norm(ql_ctx* ctx, const ql_norm_args* args);
+
+/* ---- 4-bit weights ----------------------------------------------------------
+ * A weight matrix [out_features, in_features] of 4-bit codes with one f16
+ * scale per row and `group` (32, 64 or 128) consecutive columns:
+ *   w[n][k] = scale[n][k / group] * (code[n][k] - 8),  0 <= code <= 15.
+ * Group 32 is GGUF's Q4_0.  The handle holds the matrix on the context's
+ * device in the order the product kernel streams it (in_features is a
+ * multiple of the group; rows are padded to 16, columns to 64). */
+typedef struct ql_q4 ql_q4;
+int ql_q4_create(ql_ctx* ctx, int32_t out_features, int32_t in_features, int32_t group,
+                 ql_q4** out);
+int ql_q4_destroy(ql_q4* w);
+int ql_q4_shape(const ql_q4* w, int32_t* out_features, int32_t* in_features, int32_t* group);
+/* From codes [out_features, in_features/2] (byte j of a row: column 2j in the
+ * low four bits, 2j+1 in the high ones) and f16 scales
+ * [out_features, in_features/group].  mem: where both live.  From device
+ * memory the copy is queued on the context's stream; from host memory the call
+ * returns when it is done.  (The same holds for the two calls below.) */
+int ql_q4_set(ql_q4* w, const uint8_t* codes, const void* scales, int32_t mem);
+/* From GGUF Q4_0 blocks: in_features/32 blocks of 18 bytes per row (an f16
+ * scale, then 16 bytes whose low bits are columns 0-15 and high bits columns
+ * 16-31); `bytes` must be out_features * in_features/32 * 18.  Group 32 only. */
+int ql_q4_set_blocks(ql_q4* w, const void* blocks, int64_t bytes, int32_t mem);
+/* Quantises a dense matrix (F32, F16 or BF16, row_stride elements from row to
+ * row, 0 = in_features): with m the group's value of largest magnitude (the
+ * first of equals), scale = f16(m / -8) and
+ * code = clamp(round(w / scale) + 8, 0, 15), ties to even; a group of zeros (or
+ * whose scale underflows) gets scale 0, code 8.  A group that holds a NaN or an
+ * infinity, or whose scale exceeds f16, gets a NaN scale. */
+int ql_q4_quantize(ql_q4* w, const void* dense, int32_t dtype, int64_t row_stride, int32_t mem);
+/* The codes and scales back, in ql_q4_set's layout (either may be NULL). */
+int ql_q4_get(const ql_q4* w, uint8_t* codes, void* scales, int32_t mem);
+
+/* y = x W^T for a few rows x [rows, in_features] (Linear::forward,
+ * layers.rs:148-171): single tokens, drafted tokens, small batches.  The
+ * kernel is built for up to some 64 rows, where the weights' bytes are the cost;
+ * more rows are taken in passes of that size.
+ *   in_dtype F32, F16, BF16: x as given, every product with a code exact;
+ *   in_dtype Q8_0: int8 values with x_scale [rows, in_features/32] f16, the
+ *     output of ql_rms_norm (integer products, exact per block of 32).
+ * Sums are f32; y [rows, out_features] is rounded once to out_dtype.  A row's
+ * bits depend neither on the other rows' values nor on their number.  x_stride and y_stride are
+ * elements from row to row (0 = contiguous); x_scale is contiguous.  y must not
+ * overlap x.  Device pointers, aligned to their element size. */
+typedef struct {
+  int32_t rows;      /* 0 is a no-op */
+  int32_t in_dtype;  /* F32, F16, BF16 or Q8_0 */
+  int32_t out_dtype; /* F32, F16 or BF16 */
+  int64_t x_stride, y_stride;
+  const void* x;
+  const void* x_scale; /* Q8_0 only */
+  void* y;
+} ql_linear_args;
+
+int ql_linear_q4(ql_ctx* ctx, const ql_q4* w, const ql_linear_args* args);
+
+/* Turns a model's projections and lm_head (its own or the tied embedding) into
+ * 4-bit weights of `group` on the device and frees their f32 form; hidden_size
+ * and intermediate_size must be multiples of the group.  From then on
+ * ql_llama_forward and ql_llama_generate run ql_rms_norm (Q8_0) and ql_linear_q4
+ * in place of the f32 kernels, and ql_llama_set_tensor is refused.  Logits then
+ * differ from the reference's by the weights' and activations' rounding. */
+int ql_llama_quantize(ql_llama* m, int32_t group);
+
+/* ---- verification of drafted tokens -----------------------------------------
+ * Speculative sampling for a batch of sequences: sequence b brings n_b drafted
+ * tokens x_0 .. x_{n_b-1}, the target model's distributions p_0 .. p_{n_b} at
+ * their positions and the one after them, and the distributions q_i that x_i was
+ * drawn from.  Draft i is accepted while u_i * q_i(x_i) < p_i(x_i).  At the first
+ * rejected draft a the new token is drawn from max(p_a - q_a, 0), normalised; if
+ * none is rejected, a = n_b and it is drawn from p_a.  The draw at r = uniform
+ * n_b takes the first token in id order whose running sum reaches r times the
+ * whole, as ql_sample does.  Tokens so produced follow the target's distribution.
+ *   tokens [batch, drafts + 1]: the accepted drafts, the new token, then -1
+ *   accepted [batch]: a
+ * form QL_VERIFY_LOGITS: p and q are softmax(logits / temperature); with
+ * temperature <= 0 a draft is accepted while it is its row's largest logit (the
+ * first of equals), and the new token is the largest of row a (the draft's logits
+ * and the uniforms are not read).  Logits of -inf are probability 0.
+ * form QL_VERIFY_PROBS: target and draft hold the probabilities themselves, as
+ * the caller's own filters left them (temperature is not read).
+ * draft NULL: the drafts are certain (q_i(x_i) = 1), as those looked up in the
+ * text are.  n_draft NULL: every sequence has `drafts`; entries are clamped to
+ * [0, drafts], and what lies behind a sequence's drafts is not read.
+ * Sums over the vocabulary that decide a token are f64.
+ * A row that is reached and holds a NaN or +inf, or has no positive
+ * probability, or a drafted id outside the vocabulary ends the sequence: its
+ * new token is -1 and the context's status is raised (QL_ERR_DEVICE at the next
+ * synchronize).  ql_kv_truncate then drops the rejected drafts' cache rows.
+ * Device pointers, aligned to their element size. */
+#define QL_VERIFY_LOGITS 0
+#define QL_VERIFY_PROBS 1
+#define QL_VERIFY_MAX_DRAFTS 31
+typedef struct {
+  int32_t batch;       /* 0 is a no-op */
+  int32_t drafts;      /* most drafted tokens of a sequence, 0 .. QL_VERIFY_MAX_DRAFTS */
+  int32_t vocab;
+  int32_t dtype;       /* target and draft: F32, F16 or BF16 */
+  int32_t form;        /* QL_VERIFY_* */
+  float temperature;
+  int64_t target_stride, draft_stride; /* elements from row to row (0 = vocab) */
+  const void* target;       /* [batch, drafts + 1, vocab] */
+  const void* draft;        /* [batch, drafts, vocab] or NULL */
+  const int32_t* draft_ids; /* [batch, drafts] */
+  const int32_t* n_draft;   /* [batch] or NULL */
+  const double* uniforms;   /* [batch, drafts + 1], each in [0, 1) */
+  int32_t* tokens;
+  int32_t* accepted;
+} ql_verify_args;
+
+int ql_verify_drafts(ql_ctx* ctx, const ql_verify_args* args);
+
 #ifdef __cplusplus
 }
 #endif

@@ -46,6 +46,9 @@ EXPORTS = (
     "ql_llama_create", "ql_llama_destroy", "ql_llama_get_config", "ql_llama_set_tensor",
     "ql_llama_load_gguf", "ql_llama_forward", "ql_sample", "ql_llama_generate",
     "ql_qkv_rope_append", "ql_attn_forward_appended",
+    "ql_rms_norm", "ql_q4_create", "ql_q4_destroy", "ql_q4_shape", "ql_q4_set",
+    "ql_q4_set_blocks", "ql_q4_quantize", "ql_q4_get", "ql_linear_q4", "ql_llama_quantize",
+    "ql_verify_drafts",
 )
 
 COMM_P2P, COMM_NCCL = 0, 1

@@ -26,3 +26,26 @@ int ql_check_status(ql_ctx* c);
 // The context's reusable device workspace, grown to at least `bytes`
 // (growing synchronises the context's stream first).
 int ql_ctx_workspace(ql_ctx* c, size_t bytes, void** out);
+
+// Makes `device` current for one call and puts the caller's device back.
+class ql_device_guard {
+ public:
+  explicit ql_device_guard(int device) {
+    if (cudaGetDevice(&prev_) != cudaSuccess) prev_ = -1;
+    if (prev_ != device) {
+      err_ = cudaSetDevice(device);
+      moved_ = true;
+    }
+  }
+  ~ql_device_guard() {
+    if (moved_ && prev_ >= 0) cudaSetDevice(prev_);
+  }
+  ql_device_guard(const ql_device_guard&) = delete;
+  ql_device_guard& operator=(const ql_device_guard&) = delete;
+  cudaError_t error() const { return err_; }
+
+ private:
+  int prev_ = -1;
+  bool moved_ = false;
+  cudaError_t err_ = cudaSuccess;
+};

@@ -1,0 +1,578 @@
+// ql_linear.cu -- the layers of a decode step on 4-bit weights
+// (qllama_model.h): RMSNorm with the residual's addition and an optional Q8_0
+// output, the 4-bit weight matrices, and products of a few rows with them.
+#include <cuda_runtime.h>
+
+#include <algorithm>
+#include <cmath>
+#include <new>
+
+#include "../../include/qllama_model.h"
+#include "ql_device.cuh"
+#include "ql_internal.h"
+
+namespace {
+
+#define QLN_CUDA(call, what)                                                                   \
+  do {                                                                                         \
+    cudaError_t e_ = (call);                                                                   \
+    if (e_ != cudaSuccess)                                                                     \
+      return ql_fail(e_ == cudaErrorMemoryAllocation ? QL_ERR_OOM : QL_ERR_CUDA, "%s: %s",    \
+                     what, cudaGetErrorString(e_));                                            \
+  } while (0)
+
+bool float_type(int dt) { return dt == QL_F32 || dt == QL_F16 || dt == QL_BF16; }
+size_t type_bytes(int dt) { return dt == QL_F32 ? 4 : dt == QL_Q8_0 ? 1 : 2; }
+bool aligned(const void* p, size_t to) { return reinterpret_cast<uintptr_t>(p) % to == 0; }
+
+// ------------------------------------------------------------------ RMSNorm --
+
+struct NormArgs {
+  const void* x;
+  const void* residual;
+  const void* weight;
+  void* sum_out;
+  void* out;
+  __half* out_scale;
+  int64_t x_stride, residual_stride;
+  int rows, hidden, in_dtype, weight_dtype, out_dtype;
+  float eps;
+};
+
+constexpr int kNormThreads = 256;
+
+template <typename T>
+__device__ __forceinline__ T warp_sum(T v) {
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
+  return v;
+}
+
+__device__ float norm_block_sum(float v, float* red) {
+  v = warp_sum(v);
+  __syncthreads();
+  if ((threadIdx.x & 31) == 0) red[threadIdx.x >> 5] = v;
+  __syncthreads();
+  float t = 0.f;
+  for (int i = 0; i < static_cast<int>(blockDim.x >> 5); ++i) t += red[i];
+  return t;
+}
+
+// One CTA per row.
+__global__ void __launch_bounds__(kNormThreads) rms_norm_kernel(const NormArgs a) {
+  __shared__ float red[kNormThreads / 32];
+  const size_t row = blockIdx.x;
+  const size_t xo = row * static_cast<size_t>(a.x_stride);
+  const size_t ro = row * static_cast<size_t>(a.residual_stride);
+  const size_t oo = row * static_cast<size_t>(a.hidden);
+  auto value = [&](int i) {
+    float s = ql::load_elem(a.x, xo + i, a.in_dtype);
+    if (a.residual) s += ql::load_elem(a.residual, ro + i, a.in_dtype);
+    return s;
+  };
+  float ss = 0.f;
+  for (int i = threadIdx.x; i < a.hidden; i += kNormThreads) {
+    const float s = value(i);
+    ss += s * s;
+  }
+  ss = norm_block_sum(ss, red);
+  const float inv = 1.0f / sqrtf(ss / static_cast<float>(a.hidden) + a.eps);
+  const int n = (a.hidden + kNormThreads - 1) / kNormThreads * kNormThreads;
+  for (int i = threadIdx.x; i < n; i += kNormThreads) {  // whole warps: the shuffles below
+    float y = 0.f;
+    if (i < a.hidden) {
+      const float s = value(i);
+      if (a.sum_out) ql::store_elem(a.sum_out, oo + i, a.in_dtype, s);
+      y = s * inv * ql::load_elem(a.weight, i, a.weight_dtype);
+      if (a.out_dtype != ql::kQ8_0) ql::store_elem(a.out, oo + i, a.out_dtype, y);
+    }
+    if (a.out_dtype == ql::kQ8_0) {
+      float m = fabsf(y);
+      int bad = !isfinite(y);
+#pragma unroll
+      for (int o = 16; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
+      bad = __any_sync(0xffffffffu, bad);
+      if (i < a.hidden) {
+        const float d = fminf(m / 127.0f, 65504.0f);
+        const float id = d > 0.f ? 1.0f / d : 0.f;
+        const float q = fminf(fmaxf(roundf(y * id), -127.f), 127.f);
+        static_cast<int8_t*>(a.out)[oo + i] = bad ? 0 : static_cast<int8_t>(q);
+        if (i % 32 == 0)
+          a.out_scale[(oo + i) / 32] = bad ? __ushort_as_half(0x7fff) : __float2half_rn(d);
+      }
+    }
+  }
+}
+
+}  // namespace
+
+// ------------------------------------------------------------- 4-bit weights --
+// Device order.  Tiles of 16 rows x 64 columns, row tiles outermost, so that a
+// row tile is one contiguous stream along the columns.  Tile (tile, chunk) is
+// 32 lanes x 4 words: lane = 4 g + t, word i = 2 j + h holds row
+// 16 tile + g + 8 h, columns 64 chunk + 32 j + 8 t .. + 7 -- the lane that needs
+// them in the A fragment of an m16n8k16 / m16n8k32 product (any order of the
+// columns inside a fragment serves, if x follows it).  A word holds the eight
+// values (code - 8) as two's-complement nibbles in the order of kNibble.  Scales:
+// f16, per tile (g, j, h), 64 bytes, each read by the four lanes of a quad.
+struct ql_q4 {
+  ql_ctx* ctx = nullptr;
+  int n = 0, k = 0, group = 0;
+  int tiles = 0, chunks = 0;
+  uint32_t* codes = nullptr;   // [tiles][chunks][32][4]
+  __half* scales = nullptr;    // [tiles][chunks][8][2][2]
+};
+
+namespace {
+
+// Nibble that holds element e of a word's eight: (0,4) (2,6) (1,5) (3,7) are
+// the pairs that a mask of 0x000f000f leaves after shifts of 0, 8, 4 and 12.
+__host__ __device__ constexpr int nibble_of(int e) {
+  return (e & 1) * 4 + (e >> 1 & 1) * 2 + (e >> 2);
+}
+
+struct Q4View {
+  uint32_t* codes;
+  __half* scales;
+  int n, k, group, tiles, chunks;
+};
+
+Q4View view_of(const ql_q4* w) {
+  return {w->codes, w->scales, w->n, w->k, w->group, w->tiles, w->chunks};
+}
+
+size_t q4_words(const ql_q4* w) { return static_cast<size_t>(w->tiles) * w->chunks * 128; }
+size_t q4_scales(const ql_q4* w) { return static_cast<size_t>(w->tiles) * w->chunks * 32; }
+
+// Row and first column of word i of lane `lane` of tile (tile, chunk).
+__device__ __forceinline__ void word_place(size_t tile, int chunk, int lane, int i, int& row,
+                                           int& col) {
+  row = static_cast<int>(tile) * 16 + (lane >> 2) + 8 * (i & 1);
+  col = chunk * 64 + 32 * (i >> 1) + 8 * (lane & 3);
+}
+
+enum PackFrom : int { kPackCodes = 0, kPackBlocks = 1, kPackDense = 2 };
+
+struct PackArgs {
+  Q4View w;
+  const uint8_t* bytes;  // codes or blocks
+  const uint16_t* scales;
+  const void* dense;     // element (row, col) at row * row_stride + col * col_stride
+  int64_t row_stride, col_stride;
+  int dtype;
+};
+
+// One thread per word of the device order.
+template <int FROM>
+__global__ void __launch_bounds__(256) q4_pack_kernel(const PackArgs a) {
+  const size_t id = static_cast<size_t>(blockIdx.x) * 256 + threadIdx.x;
+  const size_t per_tile = static_cast<size_t>(a.w.chunks) * 128;
+  if (id >= per_tile * a.w.tiles) return;
+  const size_t tile = id / per_tile;
+  const int rest = static_cast<int>(id % per_tile);
+  const int chunk = rest >> 7, lane = rest >> 2 & 31, i = rest & 3;
+  int row, col;
+  word_place(tile, chunk, lane, i, row, col);
+  uint32_t word = 0;
+  uint16_t scale = 0;
+  if (row < a.w.n && col < a.w.k) {
+    if constexpr (FROM == kPackCodes) {
+      const uint8_t* p = a.bytes + (static_cast<size_t>(row) * a.w.k + col) / 2;
+      for (int e = 0; e < 8; ++e) {
+        const uint32_t c = (p[e >> 1] >> (4 * (e & 1))) & 15u;
+        word |= (c ^ 8u) << (4 * nibble_of(e));
+      }
+      scale = a.scales[static_cast<size_t>(row) * (a.w.k / a.w.group) + col / a.w.group];
+    } else if constexpr (FROM == kPackBlocks) {
+      const uint8_t* b = a.bytes + (static_cast<size_t>(row) * (a.w.k / 32) + col / 32) * 18;
+      const int first = col % 32;
+      for (int e = 0; e < 8; ++e) {
+        const uint32_t c = (b[2 + (first + e) % 16] >> (first + e >= 16 ? 4 : 0)) & 15u;
+        word |= (c ^ 8u) << (4 * nibble_of(e));
+      }
+      scale = static_cast<uint16_t>(b[0] | b[1] << 8);
+    } else {
+      const int g0 = col / a.w.group * a.w.group;
+      const size_t base = static_cast<size_t>(row) * a.row_stride;
+      float most = 0.f, mag = 0.f;
+      bool bad = false;
+      for (int c = g0; c < g0 + a.w.group; ++c) {
+        const float v = ql::load_elem(a.dense, base + static_cast<size_t>(c) * a.col_stride, a.dtype);
+        bad |= !isfinite(v);
+        if (fabsf(v) > mag) {
+          mag = fabsf(v);
+          most = v;
+        }
+      }
+      const __half hs = __float2half_rn(most / -8.0f);
+      const float d = __half2float(hs);
+      bad |= !isfinite(d);
+      if (!bad && d != 0.f) {
+        for (int e = 0; e < 8; ++e) {
+          const float v =
+              ql::load_elem(a.dense, base + static_cast<size_t>(col + e) * a.col_stride, a.dtype);
+          const float q = fminf(fmaxf(rintf(v / d), -8.f), 7.f);
+          word |= (static_cast<uint32_t>(static_cast<int>(q)) & 15u) << (4 * nibble_of(e));
+        }
+      }
+      scale = bad ? 0x7fff : d == 0.f ? 0 : __half_as_ushort(hs);
+    }
+  }
+  a.w.codes[id] = word;
+  if ((lane & 3) == 0)  // one lane of the quad writes (g, j, h)
+    reinterpret_cast<uint16_t*>(a.w.scales)[(tile * a.w.chunks + chunk) * 32 + (lane >> 2) * 4 + i] =
+        scale;
+}
+
+// The device order back to codes and scales (one thread per word).
+__global__ void __launch_bounds__(256) q4_unpack_kernel(Q4View w, uint8_t* codes, uint16_t* scales) {
+  const size_t id = static_cast<size_t>(blockIdx.x) * 256 + threadIdx.x;
+  const size_t per_tile = static_cast<size_t>(w.chunks) * 128;
+  if (id >= per_tile * w.tiles) return;
+  const size_t tile = id / per_tile;
+  const int rest = static_cast<int>(id % per_tile);
+  const int chunk = rest >> 7, lane = rest >> 2 & 31, i = rest & 3;
+  int row, col;
+  word_place(tile, chunk, lane, i, row, col);
+  if (row >= w.n || col >= w.k) return;
+  const uint32_t word = w.codes[id] ^ 0x88888888u;
+  if (codes) {
+    uint8_t* p = codes + (static_cast<size_t>(row) * w.k + col) / 2;
+    for (int b = 0; b < 4; ++b)
+      p[b] = static_cast<uint8_t>((word >> (4 * nibble_of(2 * b)) & 15u) |
+                                  (word >> (4 * nibble_of(2 * b + 1)) & 15u) << 4);
+  }
+  if (scales && col % w.group == 0)
+    scales[static_cast<size_t>(row) * (w.k / w.group) + col / w.group] =
+        reinterpret_cast<const uint16_t*>(
+            w.scales)[(tile * w.chunks + chunk) * 32 + (lane >> 2) * 4 + i];
+}
+
+template <int FROM>
+int launch_pack(ql_q4* w, PackArgs a) {
+  a.w = view_of(w);
+  const size_t blocks = (q4_words(w) + 255) / 256;
+  q4_pack_kernel<FROM><<<static_cast<unsigned>(blocks), 256, 0, w->ctx->stream>>>(a);
+  QLN_CUDA(cudaGetLastError(), "launch the 4-bit layout");
+  return QL_OK;
+}
+
+// Device copies of host buffers for the length of one call.
+struct Staged {
+  ql_ctx* c;
+  void* p[2] = {nullptr, nullptr};
+  explicit Staged(ql_ctx* ctx) : c(ctx) {}
+  ~Staged() {
+    if (p[0] || p[1]) cudaStreamSynchronize(c->stream);
+    for (void* q : p)
+      if (q) cudaFree(q);
+  }
+  int copy(int slot, const void* host, size_t bytes) {
+    QLN_CUDA(cudaMalloc(&p[slot], std::max<size_t>(bytes, 16)), "allocate a staging buffer");
+    if (host)
+      QLN_CUDA(cudaMemcpyAsync(p[slot], host, bytes, cudaMemcpyHostToDevice, c->stream),
+               "copy to the device");
+    return QL_OK;
+  }
+};
+
+int check_mem(int mem) {
+  if (mem != QL_MEM_DEVICE && mem != QL_MEM_HOST)
+    return ql_fail(QL_ERR_INVALID, "unknown memory kind %d", mem);
+  return QL_OK;
+}
+
+// ----------------------------------------------------------------- products --
+
+struct LinearArgs {
+  Q4View w;
+  const void* x;
+  const __half* x_scale;
+  void* y;
+  int64_t x_stride, y_stride;
+  int rows, in_dtype, out_dtype;
+};
+
+// One warp per output column: the words of its weight row, lane by lane.
+__global__ void __launch_bounds__(128) linear_q4_kernel(const LinearArgs a) {
+  const int lane = threadIdx.x & 31;
+  const size_t n = static_cast<size_t>(blockIdx.x) * 4 + (threadIdx.x >> 5);
+  if (n >= static_cast<size_t>(a.w.n)) return;
+  const size_t tile = n / 16;
+  const int g = static_cast<int>(n % 8), h = static_cast<int>(n / 8 % 2);
+  for (int r = 0; r < a.rows; ++r) {
+    float acc = 0.f;
+    const size_t xo = static_cast<size_t>(r) * a.x_stride;
+    for (int c8 = lane; c8 < a.w.k / 8; c8 += 32) {
+      const int chunk = c8 >> 3, j = c8 >> 2 & 1, t = c8 & 3;
+      const uint32_t word =
+          a.w.codes[((tile * a.w.chunks + chunk) * 32 + 4 * g + t) * 4 + 2 * j + h];
+      float s = 0.f;
+      for (int e = 0; e < 8; ++e) {
+        const int q = static_cast<int>(word << (28 - 4 * nibble_of(e))) >> 28;
+        const float xv = a.in_dtype == ql::kQ8_0
+                             ? static_cast<const int8_t*>(a.x)[xo + 8 * c8 + e]
+                             : ql::load_elem(a.x, xo + 8 * c8 + e, a.in_dtype);
+        s = fmaf(static_cast<float>(q), xv, s);
+      }
+      s *= __half2float(a.w.scales[(tile * a.w.chunks + chunk) * 32 + 4 * g + 2 * j + h]);
+      if (a.in_dtype == ql::kQ8_0)
+        s *= __half2float(a.x_scale[static_cast<size_t>(r) * (a.w.k / 32) + c8 / 4]);
+      acc += s;
+    }
+    acc = warp_sum(acc);
+    if (lane == 0) ql::store_elem(a.y, static_cast<size_t>(r) * a.y_stride + n, a.out_dtype, acc);
+  }
+}
+
+}  // namespace
+
+// Quantises element (row, col) = dense[row * row_stride + col * col_stride] on
+// the context's stream (ql_llama_quantize reads its transposed weights this way).
+int ql_q4_quantize_strided(ql_q4* w, const void* dense, int dtype, int64_t row_stride,
+                           int64_t col_stride) {
+  PackArgs a{};
+  a.dense = dense;
+  a.dtype = dtype;
+  a.row_stride = row_stride;
+  a.col_stride = col_stride;
+  return launch_pack<kPackDense>(w, a);
+}
+
+extern "C" {
+
+int ql_rms_norm(ql_ctx* c, const ql_norm_args* args) {
+  if (!c || !args) return ql_fail(QL_ERR_INVALID, "ql_rms_norm: NULL argument");
+  const ql_norm_args& f = *args;
+  if (f.rows < 0) return ql_fail(QL_ERR_INVALID, "row count %d is negative", f.rows);
+  if (f.hidden <= 0) return ql_fail(QL_ERR_INVALID, "hidden must be positive, got %d", f.hidden);
+  if (!float_type(f.in_dtype) || !float_type(f.weight_dtype) ||
+      !(float_type(f.out_dtype) || f.out_dtype == QL_Q8_0))
+    return ql_fail(QL_ERR_INVALID, "unsupported element types %d, %d -> %d", f.in_dtype,
+                   f.weight_dtype, f.out_dtype);
+  if (!std::isfinite(f.eps) || f.eps < 0.f)
+    return ql_fail(QL_ERR_INVALID, "RMSNorm eps must be finite and nonnegative");
+  if (f.out_dtype == QL_Q8_0 && f.hidden % 32 != 0)
+    return ql_fail(QL_ERR_INVALID, "a Q8_0 output needs hidden divisible by 32, got %d", f.hidden);
+  if (f.sum_out && !f.residual)
+    return ql_fail(QL_ERR_INVALID, "ql_rms_norm: sum_out needs a residual");
+  const int64_t xs = f.x_stride ? f.x_stride : f.hidden;
+  const int64_t rs = f.residual_stride ? f.residual_stride : f.hidden;
+  if (xs < f.hidden || (f.residual && rs < f.hidden))
+    return ql_fail(QL_ERR_INVALID, "a row stride is smaller than hidden %d", f.hidden);
+  if (f.rows == 0) return QL_OK;
+  if (!f.x || !f.weight || !f.out || (f.out_dtype == QL_Q8_0 && !f.out_scale))
+    return ql_fail(QL_ERR_INVALID, "ql_rms_norm: NULL buffer");
+  const size_t ib = type_bytes(f.in_dtype);
+  if (!aligned(f.x, ib) || !aligned(f.residual, ib) || !aligned(f.sum_out, ib) ||
+      !aligned(f.weight, type_bytes(f.weight_dtype)) || !aligned(f.out, type_bytes(f.out_dtype)) ||
+      !aligned(f.out_scale, 2))
+    return ql_fail(QL_ERR_INVALID, "ql_rms_norm: a buffer is not aligned to its element size");
+  ql_device_guard dev(c->device);
+  QLN_CUDA(dev.error(), "set device");
+  NormArgs a{};
+  a.x = f.x;
+  a.residual = f.residual;
+  a.weight = f.weight;
+  a.sum_out = f.sum_out;
+  a.out = f.out;
+  a.out_scale = static_cast<__half*>(f.out_scale);
+  a.x_stride = xs;
+  a.residual_stride = rs;
+  a.rows = f.rows;
+  a.hidden = f.hidden;
+  a.in_dtype = f.in_dtype;
+  a.weight_dtype = f.weight_dtype;
+  a.out_dtype = f.out_dtype;
+  a.eps = f.eps;
+  rms_norm_kernel<<<f.rows, kNormThreads, 0, c->stream>>>(a);
+  QLN_CUDA(cudaGetLastError(), "launch rms_norm");
+  return QL_OK;
+}
+
+int ql_q4_create(ql_ctx* c, int32_t out_features, int32_t in_features, int32_t group,
+                 ql_q4** out) {
+  if (!c || !out) return ql_fail(QL_ERR_INVALID, "ql_q4_create: NULL argument");
+  *out = nullptr;
+  if (out_features <= 0 || in_features <= 0)
+    return ql_fail(QL_ERR_INVALID, "weight dimensions must be positive, got [%d, %d]",
+                   out_features, in_features);
+  if (group != 32 && group != 64 && group != 128)
+    return ql_fail(QL_ERR_INVALID, "group %d must be 32, 64 or 128", group);
+  if (in_features % group != 0)
+    return ql_fail(QL_ERR_INVALID, "in_features %d must be divisible by the group %d", in_features,
+                   group);
+  if (out_features > (1 << 30) || in_features > (1 << 30))
+    return ql_fail(QL_ERR_UNSUPPORTED, "weight dimensions [%d, %d] are too large", out_features,
+                   in_features);
+  ql_device_guard dev(c->device);
+  QLN_CUDA(dev.error(), "set device");
+  ql_q4* w = new (std::nothrow) ql_q4;
+  if (!w) return ql_fail(QL_ERR_OOM, "ql_q4_create: out of host memory");
+  w->ctx = c;
+  w->n = out_features;
+  w->k = in_features;
+  w->group = group;
+  w->tiles = (out_features + 15) / 16;
+  w->chunks = (in_features + 63) / 64;
+  cudaError_t e = cudaMalloc(&w->codes, q4_words(w) * 4);
+  if (e == cudaSuccess) e = cudaMalloc(&w->scales, q4_scales(w) * 2);
+  // a handle without values yet multiplies by zero
+  if (e == cudaSuccess) e = cudaMemsetAsync(w->codes, 0, q4_words(w) * 4, c->stream);
+  if (e == cudaSuccess) e = cudaMemsetAsync(w->scales, 0, q4_scales(w) * 2, c->stream);
+  if (e != cudaSuccess) {
+    ql_q4_destroy(w);
+    return ql_fail(e == cudaErrorMemoryAllocation ? QL_ERR_OOM : QL_ERR_CUDA,
+                   "allocate a 4-bit weight: %s", cudaGetErrorString(e));
+  }
+  *out = w;
+  return QL_OK;
+}
+
+int ql_q4_destroy(ql_q4* w) {
+  if (!w) return QL_OK;
+  ql_device_guard dev(w->ctx->device);
+  cudaStreamSynchronize(w->ctx->stream);
+  if (w->codes) cudaFree(w->codes);
+  if (w->scales) cudaFree(w->scales);
+  delete w;
+  return QL_OK;
+}
+
+int ql_q4_shape(const ql_q4* w, int32_t* out_features, int32_t* in_features, int32_t* group) {
+  if (!w || !out_features || !in_features || !group)
+    return ql_fail(QL_ERR_INVALID, "ql_q4_shape: NULL argument");
+  *out_features = w->n;
+  *in_features = w->k;
+  *group = w->group;
+  return QL_OK;
+}
+
+int ql_q4_set(ql_q4* w, const uint8_t* codes, const void* scales, int32_t mem) {
+  if (!w || !codes || !scales) return ql_fail(QL_ERR_INVALID, "ql_q4_set: NULL argument");
+  if (int r = check_mem(mem)) return r;
+  if (!aligned(scales, 2)) return ql_fail(QL_ERR_INVALID, "ql_q4_set: scales are not aligned");
+  ql_device_guard dev(w->ctx->device);
+  QLN_CUDA(dev.error(), "set device");
+  PackArgs a{};
+  a.bytes = codes;
+  a.scales = static_cast<const uint16_t*>(scales);
+  if (mem == QL_MEM_DEVICE) return launch_pack<kPackCodes>(w, a);
+  Staged s(w->ctx);
+  const size_t nk = static_cast<size_t>(w->n) * w->k;
+  if (int r = s.copy(0, codes, nk / 2)) return r;
+  if (int r = s.copy(1, scales, nk / w->group * 2)) return r;
+  a.bytes = static_cast<const uint8_t*>(s.p[0]);
+  a.scales = static_cast<const uint16_t*>(s.p[1]);
+  return launch_pack<kPackCodes>(w, a);
+}
+
+int ql_q4_set_blocks(ql_q4* w, const void* blocks, int64_t bytes, int32_t mem) {
+  if (!w || !blocks) return ql_fail(QL_ERR_INVALID, "ql_q4_set_blocks: NULL argument");
+  if (int r = check_mem(mem)) return r;
+  if (w->group != 32)
+    return ql_fail(QL_ERR_INVALID, "Q4_0 blocks need a group of 32, the weight has %d", w->group);
+  const int64_t want = static_cast<int64_t>(w->n) * (w->k / 32) * 18;
+  if (bytes != want)
+    return ql_fail(QL_ERR_INVALID, "Q4_0 blocks of [%d, %d] take %lld bytes, got %lld", w->n, w->k,
+                   (long long)want, (long long)bytes);
+  ql_device_guard dev(w->ctx->device);
+  QLN_CUDA(dev.error(), "set device");
+  PackArgs a{};
+  a.bytes = static_cast<const uint8_t*>(blocks);
+  if (mem == QL_MEM_DEVICE) return launch_pack<kPackBlocks>(w, a);
+  Staged s(w->ctx);
+  if (int r = s.copy(0, blocks, static_cast<size_t>(bytes))) return r;
+  a.bytes = static_cast<const uint8_t*>(s.p[0]);
+  return launch_pack<kPackBlocks>(w, a);
+}
+
+int ql_q4_quantize(ql_q4* w, const void* dense, int32_t dtype, int64_t row_stride, int32_t mem) {
+  if (!w || !dense) return ql_fail(QL_ERR_INVALID, "ql_q4_quantize: NULL argument");
+  if (int r = check_mem(mem)) return r;
+  if (!float_type(dtype)) return ql_fail(QL_ERR_INVALID, "unsupported element type %d", dtype);
+  const int64_t rs = row_stride ? row_stride : w->k;
+  if (rs < w->k)
+    return ql_fail(QL_ERR_INVALID, "a row stride is smaller than in_features %d", w->k);
+  if (!aligned(dense, type_bytes(dtype)))
+    return ql_fail(QL_ERR_INVALID, "ql_q4_quantize: the matrix is not aligned to its element size");
+  ql_device_guard dev(w->ctx->device);
+  QLN_CUDA(dev.error(), "set device");
+  if (mem == QL_MEM_DEVICE) return ql_q4_quantize_strided(w, dense, dtype, rs, 1);
+  Staged s(w->ctx);
+  const size_t elems = static_cast<size_t>(rs) * (w->n - 1) + w->k;
+  if (int r = s.copy(0, dense, elems * type_bytes(dtype))) return r;
+  return ql_q4_quantize_strided(w, s.p[0], dtype, rs, 1);
+}
+
+int ql_q4_get(const ql_q4* w, uint8_t* codes, void* scales, int32_t mem) {
+  if (!w) return ql_fail(QL_ERR_INVALID, "ql_q4_get: NULL argument");
+  if (int r = check_mem(mem)) return r;
+  if (!aligned(scales, 2)) return ql_fail(QL_ERR_INVALID, "ql_q4_get: scales are not aligned");
+  ql_device_guard dev(w->ctx->device);
+  QLN_CUDA(dev.error(), "set device");
+  cudaStream_t st = w->ctx->stream;
+  const size_t cb = static_cast<size_t>(w->n) * w->k / 2;
+  const size_t sb = static_cast<size_t>(w->n) * (w->k / w->group) * 2;
+  Staged s(w->ctx);
+  uint8_t* dc = codes;
+  void* ds = scales;
+  if (mem == QL_MEM_HOST) {
+    if (codes) {
+      if (int r = s.copy(0, nullptr, cb)) return r;
+      dc = static_cast<uint8_t*>(s.p[0]);
+    }
+    if (scales) {
+      if (int r = s.copy(1, nullptr, sb)) return r;
+      ds = s.p[1];
+    }
+  }
+  const size_t blocks = (q4_words(w) + 255) / 256;
+  q4_unpack_kernel<<<static_cast<unsigned>(blocks), 256, 0, st>>>(view_of(w), dc,
+                                                                  static_cast<uint16_t*>(ds));
+  QLN_CUDA(cudaGetLastError(), "launch the 4-bit read-back");
+  if (mem == QL_MEM_HOST) {
+    if (codes) QLN_CUDA(cudaMemcpyAsync(codes, dc, cb, cudaMemcpyDeviceToHost, st), "copy codes");
+    if (scales)
+      QLN_CUDA(cudaMemcpyAsync(scales, ds, sb, cudaMemcpyDeviceToHost, st), "copy scales");
+  }
+  return QL_OK;
+}
+
+int ql_linear_q4(ql_ctx* c, const ql_q4* w, const ql_linear_args* args) {
+  if (!c || !w || !args) return ql_fail(QL_ERR_INVALID, "ql_linear_q4: NULL argument");
+  const ql_linear_args& f = *args;
+  if (w->ctx->device != c->device)
+    return ql_fail(QL_ERR_INVALID, "the weight lives on device %d, the context on device %d",
+                   w->ctx->device, c->device);
+  if (f.rows < 0) return ql_fail(QL_ERR_INVALID, "row count %d is negative", f.rows);
+  if (!(float_type(f.in_dtype) || f.in_dtype == QL_Q8_0) || !float_type(f.out_dtype))
+    return ql_fail(QL_ERR_INVALID, "unsupported element types %d -> %d", f.in_dtype, f.out_dtype);
+  const int64_t xs = f.x_stride ? f.x_stride : w->k, ys = f.y_stride ? f.y_stride : w->n;
+  if (xs < w->k || ys < w->n)
+    return ql_fail(QL_ERR_INVALID, "a row stride is smaller than the row (%d in, %d out)", w->k,
+                   w->n);
+  if (f.rows == 0) return QL_OK;
+  if (!f.x || !f.y || (f.in_dtype == QL_Q8_0 && !f.x_scale))
+    return ql_fail(QL_ERR_INVALID, "ql_linear_q4: NULL buffer");
+  if (!aligned(f.x, type_bytes(f.in_dtype)) || !aligned(f.y, type_bytes(f.out_dtype)) ||
+      !aligned(f.x_scale, 2))
+    return ql_fail(QL_ERR_INVALID, "ql_linear_q4: a buffer is not aligned to its element size");
+  ql_device_guard dev(c->device);
+  QLN_CUDA(dev.error(), "set device");
+  LinearArgs a{};
+  a.w = view_of(w);
+  a.x = f.x;
+  a.x_scale = static_cast<const __half*>(f.x_scale);
+  a.y = f.y;
+  a.x_stride = xs;
+  a.y_stride = ys;
+  a.rows = f.rows;
+  a.in_dtype = f.in_dtype;
+  a.out_dtype = f.out_dtype;
+  linear_q4_kernel<<<(w->n + 3) / 4, 128, 0, c->stream>>>(a);
+  QLN_CUDA(cudaGetLastError(), "launch the 4-bit product");
+  return QL_OK;
+}
+
+}  // extern "C"

@@ -50,6 +50,9 @@
 int ql_kv_append_prepare(ql_ctx* c, ql_kv* kv, const ql_attn_args* a, ql::CacheView* view,
                          const double2** rope, ql::SeqTable* st);
 void ql_kv_append_commit(ql_kv* kv, const ql_attn_args* a);
+// ql_linear.cu: 4-bit codes of element (row, col) = dense[row * row_stride + col * col_stride]
+int ql_q4_quantize_strided(ql_q4* w, const void* dense, int dtype, int64_t row_stride,
+                           int64_t col_stride);
 
 namespace {
 
@@ -199,6 +202,15 @@ cudaError_t launch_gemm(const GemmArgs& g, cudaStream_t s) {
     gemm_kernel<4, M><<<dim3(cols, (g.n + 3) / 4), kGemmThreads, 0, s>>>(g);
   }
   return cudaGetLastError();
+}
+
+// SwiGLU over the fused gate and up products [n, 2F]: silu(gate) * up.
+__global__ void __launch_bounds__(256) silu_mul_kernel(const float* gu, int F, float* out) {
+  const size_t row = blockIdx.y;
+  const int i = blockIdx.x * 256 + threadIdx.x;
+  if (i >= F) return;
+  const float* p = gu + row * 2 * static_cast<size_t>(F);
+  out[row * F + i] = __fmul_rn(silu_ref(p[i]), p[F + i]);
 }
 
 // ------------------------------------------------- fused projection + RoPE --
@@ -804,6 +816,16 @@ struct ql_llama {
     float* wd_t = nullptr;       // [F, E]
   };
   std::vector<Layer> layers;
+  // after ql_llama_quantize: the 4-bit forms, and the f32 matrices are gone
+  struct Q4Layer {
+    ql_q4* qkv = nullptr;      // [E + 2 kvd, E]
+    ql_q4* wo = nullptr;       // [E, E]
+    ql_q4* gate_up = nullptr;  // [2F, E]
+    ql_q4* down = nullptr;     // [E, F]
+  };
+  bool quantized = false;
+  std::vector<Q4Layer> q4;
+  ql_q4* q4_lm = nullptr;      // [V, E]
   // workspace for `rows` tokens
   // projections fused with RoPE and the append (ql_qkv_rope_append); off:
   // the Q/K/V GEMM, then ql_attn_forward appends (same results, bit for bit)
@@ -811,6 +833,10 @@ struct ql_llama {
   int rows = 0;
   float *x = nullptr, *h = nullptr, *q = nullptr, *k = nullptr, *v = nullptr, *att = nullptr,
         *g = nullptr, *logits = nullptr;
+  // quantized models: [rows, qkv_cols], [rows, E], [rows, 2F] and the norm's Q8_0 rows
+  float *qkv = nullptr, *t = nullptr, *gu = nullptr;
+  int8_t* xq = nullptr;
+  uint16_t* xs = nullptr;
   int32_t* ids = nullptr;   // [max_pos + 1] token ids of the call / the generated context
   char* sample_scratch = nullptr;
   std::vector<void*> allocations;
@@ -827,9 +853,13 @@ int alloc_dev(ql_llama* m, void** p, size_t bytes) {
 }
 
 void free_work(ql_llama* m) {
-  for (float* p : {m->x, m->h, m->q, m->k, m->v, m->att, m->g, m->logits})
+  for (float* p : {m->x, m->h, m->q, m->k, m->v, m->att, m->g, m->logits, m->qkv, m->t, m->gu})
     if (p) cudaFree(p);
-  m->x = m->h = m->q = m->k = m->v = m->att = m->g = m->logits = nullptr;
+  if (m->xq) cudaFree(m->xq);
+  if (m->xs) cudaFree(m->xs);
+  m->x = m->h = m->q = m->k = m->v = m->att = m->g = m->logits = m->qkv = m->t = m->gu = nullptr;
+  m->xq = nullptr;
+  m->xs = nullptr;
   m->rows = 0;
 }
 
@@ -839,13 +869,19 @@ int ensure_rows(ql_llama* m, int rows) {
   free_work(m);
   const size_t E = m->cfg.hidden_size, F = m->cfg.intermediate_size, V = m->cfg.vocab_size;
   const size_t R = static_cast<size_t>(rows);
+  const size_t Q = m->quantized ? R : 0;
   struct {
-    float** p;
-    size_t n;
-  } bufs[] = {{&m->x, R * E}, {&m->h, R * E}, {&m->q, R * E}, {&m->k, R * m->kvd},
-              {&m->v, R * m->kvd}, {&m->att, R * E}, {&m->g, R * F}, {&m->logits, R * V}};
+    void** p;
+    size_t bytes;
+  } bufs[] = {{(void**)&m->x, R * E * 4},      {(void**)&m->h, R * E * 4},
+              {(void**)&m->q, R * E * 4},      {(void**)&m->k, R * m->kvd * 4},
+              {(void**)&m->v, R * m->kvd * 4}, {(void**)&m->att, R * E * 4},
+              {(void**)&m->g, R * F * 4},      {(void**)&m->logits, R * V * 4},
+              {(void**)&m->qkv, Q * m->qkv_cols * 4}, {(void**)&m->t, Q * E * 4},
+              {(void**)&m->gu, Q * 2 * F * 4}, {(void**)&m->xq, Q * E},
+              {(void**)&m->xs, Q * (E / 32) * 2}};
   for (auto& b : bufs) {
-    cudaError_t e = cudaMalloc(b.p, std::max<size_t>(b.n * sizeof(float), 256));
+    cudaError_t e = cudaMalloc(b.p, std::max<size_t>(b.bytes, 256));
     if (e != cudaSuccess) {
       free_work(m);
       return ql_fail(e == cudaErrorMemoryAllocation ? QL_ERR_OOM : QL_ERR_CUDA,
@@ -854,6 +890,22 @@ int ensure_rows(ql_llama* m, int rows) {
   }
   m->rows = rows;
   return QL_OK;
+}
+
+void free_q4(ql_llama* m) {
+  for (ql_llama::Q4Layer& q : m->q4)
+    for (ql_q4* w : {q.qkv, q.wo, q.gate_up, q.down}) ql_q4_destroy(w);
+  m->q4.clear();
+  ql_q4_destroy(m->q4_lm);
+  m->q4_lm = nullptr;
+}
+
+// Frees one of the model's matrices ahead of the model itself.
+void release(ql_llama* m, float** p) {
+  auto it = std::find(m->allocations.begin(), m->allocations.end(), static_cast<void*>(*p));
+  if (it != m->allocations.end()) m->allocations.erase(it);
+  cudaFree(*p);
+  *p = nullptr;
 }
 
 // Uploads host [rows, cols] as the transposed [cols, rows] block at column
@@ -880,10 +932,106 @@ int upload_plain(ql_llama* m, float* dst, const float* src, size_t n) {
   return QL_OK;
 }
 
+// RMSNorm of rows x (after adding `add`, when given, into x) to the Q8_0 rows.
+int norm_q8(ql_llama* m, float* x, const float* add, const float* weight, int rows) {
+  ql_norm_args a{};
+  a.rows = rows;
+  a.hidden = m->cfg.hidden_size;
+  a.in_dtype = a.weight_dtype = QL_F32;
+  a.out_dtype = QL_Q8_0;
+  a.eps = m->cfg.rms_norm_eps;
+  a.x = x;
+  a.residual = add;
+  a.sum_out = add ? x : nullptr;
+  a.weight = weight;
+  a.out = m->xq;
+  a.out_scale = m->xs;
+  return ql_rms_norm(m->ctx, &a);
+}
+
+// y = rows x w^T; x NULL: the Q8_0 rows of the last norm.
+int linear(ql_llama* m, const ql_q4* w, const float* x, int rows, float* y) {
+  ql_linear_args a{};
+  a.rows = rows;
+  a.in_dtype = x ? QL_F32 : QL_Q8_0;
+  a.out_dtype = QL_F32;
+  a.x = x ? static_cast<const void*>(x) : m->xq;
+  a.x_scale = x ? nullptr : m->xs;
+  a.y = y;
+  return ql_linear_q4(m->ctx, w, &a);
+}
+
+// forward_device of a quantized model.  Each layer's two outputs stay in m->t
+// until the next norm adds them to the residual stream.
+int forward_q4(ql_llama* m, ql_kv* kv, int32_t seq, const int32_t* ids, int n, int64_t start_pos,
+               int logit_rows) {
+  ql_ctx* c = m->ctx;
+  cudaStream_t s = c->stream;
+  const ql_llama_config& cf = m->cfg;
+  const int E = cf.hidden_size, F = cf.intermediate_size, V = cf.vocab_size, kvd = m->kvd;
+  embed_kernel<<<n, 256, 0, s>>>(ids, n, m->embd, V, E, m->x, c->status);
+  QLM_CUDA(cudaGetLastError(), "launch embedding");
+  int r = QL_OK;
+  for (int l = 0; l < cf.num_layers; ++l) {
+    const ql_llama::Layer& L = m->layers[l];
+    const ql_llama::Q4Layer& Q = m->q4[l];
+    if ((r = norm_q8(m, m->x, l ? m->t : nullptr, L.attn_norm, n)) != QL_OK) return r;
+    if ((r = linear(m, Q.qkv, nullptr, n, m->qkv)) != QL_OK) return r;
+    ql_attn_args a{};
+    a.layer_idx = l;
+    a.batch = 1;
+    a.new_len = n;
+    a.seq_ids = &seq;
+    a.start_pos = &start_pos;
+    a.num_heads = cf.num_heads;
+    a.num_kv_heads = cf.num_kv_heads;
+    a.head_dim = m->hd;
+    a.rope_theta = cf.rope_theta;
+    a.in_dtype = QL_F32;
+    a.out_dtype = QL_F32;
+    a.mem = QL_MEM_DEVICE;
+    a.q = m->qkv;
+    a.k = m->qkv + E;
+    a.v = m->qkv + E + kvd;
+    a.out = m->att;
+    if (n > 1) {  // the operator takes q, k and v as three contiguous tensors
+      const size_t ld = static_cast<size_t>(m->qkv_cols) * 4;
+      const struct {
+        float* to;
+        int col, width;
+      } parts[] = {{m->q, 0, E}, {m->k, E, kvd}, {m->v, E + kvd, kvd}};
+      for (const auto& p : parts)
+        QLM_CUDA(cudaMemcpy2DAsync(p.to, static_cast<size_t>(p.width) * 4, m->qkv + p.col, ld,
+                                   static_cast<size_t>(p.width) * 4, n, cudaMemcpyDeviceToDevice,
+                                   s),
+                 "split the Q/K/V product");
+      a.q = m->q;
+      a.k = m->k;
+      a.v = m->v;
+    }
+    if ((r = ql_attn_forward(c, kv, &a)) != QL_OK) {
+      std::string msg = ql_last_error();
+      return ql_fail(r, "Layer %d failed: %s", l, msg.c_str());
+    }
+    if ((r = linear(m, Q.wo, m->att, n, m->t)) != QL_OK) return r;
+    if ((r = norm_q8(m, m->x, m->t, L.ffn_norm, n)) != QL_OK) return r;
+    if ((r = linear(m, Q.gate_up, nullptr, n, m->gu)) != QL_OK) return r;
+    silu_mul_kernel<<<dim3((F + 255) / 256, n), 256, 0, s>>>(m->gu, F, m->g);
+    QLM_CUDA(cudaGetLastError(), "launch SwiGLU");
+    if ((r = linear(m, Q.down, m->g, n, m->t)) != QL_OK) return r;
+  }
+  if (logit_rows <= 0) return QL_OK;
+  const size_t first = static_cast<size_t>(n - logit_rows) * E;
+  const float* add = cf.num_layers ? m->t + first : nullptr;
+  if ((r = norm_q8(m, m->x + first, add, m->out_norm, logit_rows)) != QL_OK) return r;
+  return linear(m, m->q4_lm, nullptr, logit_rows, m->logits);
+}
+
 // Transformer::forward_with_cache with the token ids already on the device
 // (ids[0..n)); logits of the last `logit_rows` rows go to m->logits.
 int forward_device(ql_llama* m, ql_kv* kv, int32_t seq, const int32_t* ids, int n,
                    int64_t start_pos, int logit_rows) {
+  if (m->quantized) return forward_q4(m, kv, seq, ids, n, start_pos, logit_rows);
   ql_ctx* c = m->ctx;
   cudaStream_t s = c->stream;
   const ql_llama_config& cf = m->cfg;
@@ -1060,6 +1208,7 @@ int ql_llama_destroy(ql_llama* m) {
   cudaSetDevice(m->ctx->device);
   cudaStreamSynchronize(m->ctx->stream);
   free_work(m);
+  free_q4(m);
   for (void* p : m->allocations) cudaFree(p);
   delete m;
   return QL_OK;
@@ -1071,8 +1220,67 @@ int ql_llama_get_config(const ql_llama* m, ql_llama_config* out) {
   return QL_OK;
 }
 
+int ql_llama_quantize(ql_llama* m, int32_t group) {
+  if (!m) return ql_fail(QL_ERR_INVALID, "ql_llama_quantize: NULL argument");
+  const ql_llama_config& f = m->cfg;
+  const int E = f.hidden_size, F = f.intermediate_size, V = f.vocab_size;
+  if (m->quantized) return ql_fail(QL_ERR_INVALID, "the model is quantized already");
+  if (group != 32 && group != 64 && group != 128)
+    return ql_fail(QL_ERR_INVALID, "group %d must be 32, 64 or 128", group);
+  if (E % group != 0 || F % group != 0)
+    return ql_fail(QL_ERR_INVALID, "hidden_size %d and intermediate_size %d must be divisible by "
+                   "the group %d", E, F, group);
+  QLM_CUDA(cudaSetDevice(m->ctx->device), "set device");
+  cudaStream_t s = m->ctx->stream;
+  float* pair = nullptr;  // gate | up side by side, [E, 2F]
+  // the device matrices are transposed: element (out, in) at in * ld + out
+  auto make = [&](ql_q4** w, const float* wt, int rows, int cols) {
+    int r = ql_q4_create(m->ctx, rows, cols, group, w);
+    return r != QL_OK ? r : ql_q4_quantize_strided(*w, wt, QL_F32, 1, rows);
+  };
+  auto build = [&]() -> int {
+    QLM_CUDA(cudaMalloc(&pair, static_cast<size_t>(E) * 2 * F * 4), "allocate model memory");
+    m->q4.resize(f.num_layers);
+    int r = QL_OK;
+    for (int l = 0; l < f.num_layers; ++l) {
+      const ql_llama::Layer& L = m->layers[l];
+      ql_llama::Q4Layer& Q = m->q4[l];
+      const size_t row = static_cast<size_t>(F) * 4;
+      QLM_CUDA(cudaMemcpy2DAsync(pair, 2 * row, L.wg_t, row, row, E, cudaMemcpyDeviceToDevice, s),
+               "join gate and up");
+      QLM_CUDA(cudaMemcpy2DAsync(pair + F, 2 * row, L.wu_t, row, row, E, cudaMemcpyDeviceToDevice,
+                                 s),
+               "join gate and up");
+      if ((r = make(&Q.qkv, L.wqkv_t, m->qkv_cols, E)) != QL_OK) return r;
+      if ((r = make(&Q.wo, L.wo_t, E, E)) != QL_OK) return r;
+      if ((r = make(&Q.gate_up, pair, 2 * F, E)) != QL_OK) return r;
+      if ((r = make(&Q.down, L.wd_t, E, F)) != QL_OK) return r;
+    }
+    if ((r = make(&m->q4_lm, m->lm_t, V, E)) != QL_OK) return r;
+    QLM_CUDA(cudaStreamSynchronize(s), "synchronize quantization");
+    return QL_OK;
+  };
+  const int r = build();
+  if (r != QL_OK) {  // the f32 model stays as it was
+    const std::string msg = ql_last_error();
+    cudaStreamSynchronize(s);
+    if (pair) cudaFree(pair);
+    free_q4(m);
+    return ql_fail(r, "%s", msg.c_str());
+  }
+  cudaFree(pair);
+  for (ql_llama::Layer& L : m->layers)
+    for (float** p : {&L.wqkv_t, &L.wo_t, &L.wg_t, &L.wu_t, &L.wd_t}) release(m, p);
+  release(m, &m->lm_t);
+  free_work(m);  // the next call allocates the quantized model's workspace
+  m->quantized = true;
+  return QL_OK;
+}
+
 int ql_llama_set_tensor(ql_llama* m, const char* name, const float* data, int64_t n) {
   if (!m || !name || !data) return ql_fail(QL_ERR_INVALID, "ql_llama_set_tensor: NULL argument");
+  if (m->quantized)
+    return ql_fail(QL_ERR_INVALID, "the model is quantized: its tensors cannot be set any more");
   QLM_CUDA(cudaSetDevice(m->ctx->device), "set device");
   const ql_llama_config& f = m->cfg;
   const int E = f.hidden_size, F = f.intermediate_size, V = f.vocab_size, kvd = m->kvd;

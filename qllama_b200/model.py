@@ -8,6 +8,18 @@ Mirrors the reference's interface for these pieces:
 * ``Llama.generate``   -- generate() of src/main.rs:387-429;
 * ``SamplerConfig`` / ``sample`` -- src/sampler/sampler.rs (the uniform draw
   is passed in: the reference draws it from its seeded generator).
+
+and, with no counterpart in the reference, the pieces of a decode step on 4-bit
+weights with drafted tokens:
+
+* ``rms_norm``         -- RMSNorm with the residual's addition, plain or Q8_0 out;
+* ``Q4Weight`` / ``linear_q4`` -- 4-bit weight matrices and products of a few
+  rows with them (``Llama.quantize`` moves a model onto them);
+* ``verify_drafts``    -- speculative sampling's acceptance and next token.
+
+These take CUDA tensors and queue their work on the context's stream
+(``Context.set_stream``); tensors written on another stream have to be ordered
+before it by the caller.
 """
 from __future__ import annotations
 
@@ -34,7 +46,35 @@ class SamplerConfig(ctypes.Structure):
                 ("top_p", ctypes.c_float), ("repeat_penalty", ctypes.c_float)]
 
 
+class NormArgs(ctypes.Structure):
+    _fields_ = [("rows", ctypes.c_int32), ("hidden", ctypes.c_int32),
+                ("in_dtype", ctypes.c_int32), ("weight_dtype", ctypes.c_int32),
+                ("out_dtype", ctypes.c_int32), ("eps", ctypes.c_float),
+                ("x_stride", ctypes.c_int64), ("residual_stride", ctypes.c_int64),
+                ("x", ctypes.c_void_p), ("residual", ctypes.c_void_p),
+                ("weight", ctypes.c_void_p), ("sum_out", ctypes.c_void_p),
+                ("out", ctypes.c_void_p), ("out_scale", ctypes.c_void_p)]
+
+
+class LinearArgs(ctypes.Structure):
+    _fields_ = [("rows", ctypes.c_int32), ("in_dtype", ctypes.c_int32),
+                ("out_dtype", ctypes.c_int32), ("x_stride", ctypes.c_int64),
+                ("y_stride", ctypes.c_int64), ("x", ctypes.c_void_p),
+                ("x_scale", ctypes.c_void_p), ("y", ctypes.c_void_p)]
+
+
+class VerifyArgs(ctypes.Structure):
+    _fields_ = [("batch", ctypes.c_int32), ("drafts", ctypes.c_int32),
+                ("vocab", ctypes.c_int32), ("dtype", ctypes.c_int32), ("form", ctypes.c_int32),
+                ("temperature", ctypes.c_float), ("target_stride", ctypes.c_int64),
+                ("draft_stride", ctypes.c_int64), ("target", ctypes.c_void_p),
+                ("draft", ctypes.c_void_p), ("draft_ids", ctypes.c_void_p),
+                ("n_draft", ctypes.c_void_p), ("uniforms", ctypes.c_void_p),
+                ("tokens", ctypes.c_void_p), ("accepted", ctypes.c_void_p)]
+
+
 GREEDY = (0.0, 0, 1.0, 1.0)
+VERIFY_LOGITS, VERIFY_PROBS, VERIFY_MAX_DRAFTS = 0, 1, 31
 
 
 def bind(L: ctypes.CDLL) -> None:
@@ -53,6 +93,17 @@ def bind(L: ctypes.CDLL) -> None:
     L.ql_llama_generate.argtypes = [vp, vp, i32, i32p, i32, i32, i32,
                                     ctypes.POINTER(SamplerConfig),
                                     ctypes.POINTER(ctypes.c_double), i32p, i32p]
+    L.ql_rms_norm.argtypes = [vp, ctypes.POINTER(NormArgs)]
+    L.ql_q4_create.argtypes = [vp, i32, i32, i32, ctypes.POINTER(vp)]
+    L.ql_q4_destroy.argtypes = [vp]
+    L.ql_q4_shape.argtypes = [vp, i32p, i32p, i32p]
+    L.ql_q4_set.argtypes = [vp, vp, vp, i32]
+    L.ql_q4_set_blocks.argtypes = [vp, vp, i64, i32]
+    L.ql_q4_quantize.argtypes = [vp, vp, i32, i64, i32]
+    L.ql_q4_get.argtypes = [vp, vp, vp, i32]
+    L.ql_linear_q4.argtypes = [vp, vp, ctypes.POINTER(LinearArgs)]
+    L.ql_llama_quantize.argtypes = [vp, i32]
+    L.ql_verify_drafts.argtypes = [vp, ctypes.POINTER(VerifyArgs)]
 
 
 def _qb():
@@ -89,6 +140,11 @@ class Llama:
         a = np.ascontiguousarray(data, dtype=np.float32)
         qb = _qb()
         qb._check(qb.load().ql_llama_set_tensor(self._h, name.encode(), a.ctypes.data, a.size))
+
+    def quantize(self, group: int = 32) -> None:
+        """Projections and lm_head to 4-bit weights of `group` (ql_llama_quantize)."""
+        qb = _qb()
+        qb._check(qb.load().ql_llama_quantize(self._h, group))
 
     def kv_cache(self, max_batch: int = 1, dtype: str = "f32"):
         """KvCache::new(num_layers, max_position_embeddings, num_kv_heads, head_dim)."""
@@ -198,3 +254,307 @@ def attention_forward_appended(kv, layer: int, q_rot, start_pos, num_heads: int,
                        qb.MEM_DEVICE, q_rot.data_ptr(), None, None, out.data_ptr())
     qb._check(qb.load().ql_attn_forward_appended(kv.ctx._h, kv._h, ctypes.byref(args)))
     return out
+
+
+# ------------------------------------ 4-bit decode step and drafted tokens --
+
+_codes = {}  # torch dtype -> QL element type, filled at the first call
+
+
+def _types():
+    if not _codes:
+        import torch
+
+        qb = _qb()
+        _codes.update({torch.float32: qb.F32, torch.float16: qb.F16, torch.bfloat16: qb.BF16})
+    return _codes
+
+
+def _invalid(message: str):
+    qb = _qb()
+    return qb.QllamaError(qb.ERR_INVALID, message)
+
+
+def _float_code(t, name: str) -> int:
+    code = _types().get(t.dtype)
+    if code is None:
+        raise _invalid(f"{name}: unsupported element type {t.dtype}")
+    return code
+
+
+def _on(ctx, t, name: str) -> int:
+    """The pointer of a tensor on the context's device."""
+    d = t.device
+    if d.type != "cuda" or d.index != ctx.device:
+        raise _invalid(f"{name} is on {d}, the context on cuda:{ctx.device}")
+    return t.data_ptr()
+
+
+def _rows_of(t, width: int, name: str):
+    """(rows, elements from row to row) of a tensor [..., width]: a matrix whose
+    rows are contiguous, or a contiguous tensor of any rank."""
+    shape = t.shape
+    if not shape or shape[-1] != width:
+        raise _invalid(f"{name} has shape {tuple(shape)}, its last dimension must be {width}")
+    if len(shape) == 2 and t.stride(1) == 1 and (t.stride(0) >= width or shape[0] <= 1):
+        return shape[0], (t.stride(0) if shape[0] > 1 else width)
+    if not t.is_contiguous():
+        raise _invalid(f"{name} must have contiguous rows")
+    return t.numel() // width, width
+
+
+def _output(ctx, t, shape, dtype, name: str):
+    """A given output checked (contiguous, of that shape and type), or a new one."""
+    if t is None:
+        import torch
+
+        return torch.empty(shape, dtype=dtype, device=f"cuda:{ctx.device}")
+    if tuple(t.shape) != tuple(shape) or t.dtype != dtype or not t.is_contiguous():
+        raise _invalid(f"{name} must be a contiguous {dtype} tensor of shape {tuple(shape)}")
+    return t
+
+
+def _out_type(out, out_dtype, default):
+    import torch
+
+    if out_dtype is None:
+        return out.dtype if out is not None else default
+    named = {"f32": torch.float32, "f16": torch.float16, "bf16": torch.bfloat16}
+    if out_dtype not in named:
+        raise _invalid(f"unknown element type {out_dtype}")
+    return named[out_dtype]
+
+
+def rms_norm(ctx, x, weight, eps: float, residual=None, sum_out=None, out=None, scale=None,
+             out_dtype: str | None = None):
+    """y = s / sqrt(mean(s^2) + eps) * weight over the last dimension, s = x + residual.
+
+    x [..., hidden] (f32, f16 or bf16); residual like x; sum_out receives s (it
+    may be x or residual).  out_dtype: None (x's, or out's), "f32", "f16",
+    "bf16", or "q8_0", also chosen by giving an int8 `out`.  Returns y, or for
+    Q8_0 (int8 values [..., hidden], f16 scales [..., hidden / 32]).
+    """
+    import torch
+
+    qb = _qb()
+    if not x.dim() or not x.shape[-1]:
+        raise _invalid("x needs a last dimension to normalise")
+    hidden = x.shape[-1]
+    rows, xs = _rows_of(x, hidden, "x")
+    in_dt = _float_code(x, "x")
+    if weight.shape != (hidden,) or not weight.is_contiguous():
+        raise _invalid(f"weight must be contiguous [{hidden}], got {tuple(weight.shape)}")
+    rs, rp, sp = 0, None, None
+    if residual is not None:
+        if residual.shape != x.shape or residual.dtype != x.dtype:
+            raise _invalid("residual must have x's shape and type")
+        rs = _rows_of(residual, hidden, "residual")[1]
+        rp = _on(ctx, residual, "residual")
+    if sum_out is not None:
+        _output(ctx, sum_out, x.shape, x.dtype, "sum_out")
+        sp = _on(ctx, sum_out, "sum_out")
+    q8 = out_dtype == "q8_0" or (out_dtype is None and out is not None and out.dtype == torch.int8)
+    if q8:
+        if hidden % 32:
+            raise _invalid(f"a Q8_0 output needs hidden divisible by 32, got {hidden}")
+        out = _output(ctx, out, x.shape, torch.int8, "out")
+        scale = _output(ctx, scale, x.shape[:-1] + (hidden // 32,), torch.float16, "scale")
+        out_dt, scp = qb.Q8_0, _on(ctx, scale, "scale")
+    else:
+        if scale is not None:
+            raise _invalid("scale belongs to a Q8_0 output")
+        t = _out_type(out, out_dtype, x.dtype)
+        out = _output(ctx, out, x.shape, t, "out")
+        out_dt, scp = _float_code(out, "out"), None
+    args = NormArgs(rows, hidden, in_dt, _float_code(weight, "weight"), out_dt, eps, xs, rs,
+                    _on(ctx, x, "x"), rp, _on(ctx, weight, "weight"), sp, _on(ctx, out, "out"),
+                    scp)
+    qb._check(qb.load().ql_rms_norm(ctx._h, ctypes.byref(args)))
+    return (out, scale) if q8 else out
+
+
+class Q4Weight:
+    """A 4-bit weight matrix [out_features, in_features] on the device (ql_q4).
+
+    Q4Weight(ctx, codes, scales): codes uint8 [out, in/2] (column 2j in the low
+    four bits of byte j), scales f16 [out, in/group]; CUDA tensors or numpy
+    arrays.  The group (32, 64 or 128) follows from the shapes.
+    """
+
+    def __init__(self, ctx, codes=None, scales=None, *, shape=None):
+        qb = _qb()
+        self.ctx, self._h = ctx, None
+        if shape is None:
+            if codes is None or scales is None or len(codes.shape) != 2 or \
+                    len(scales.shape) != 2 or codes.shape[0] != scales.shape[0] or \
+                    not scales.shape[1] or 2 * codes.shape[1] % scales.shape[1]:
+                raise _invalid("codes [out, in/2] and scales [out, in/group] are needed")
+            k = 2 * int(codes.shape[1])
+            shape = (int(codes.shape[0]), k, k // int(scales.shape[1]))
+        self.out_features, self.in_features, self.group = shape
+        h = ctypes.c_void_p()
+        qb._check(qb.load().ql_q4_create(ctx._h, *shape, ctypes.byref(h)))
+        self._h = h
+        if codes is not None:
+            self.set(codes, scales)
+
+    @classmethod
+    def from_dense(cls, ctx, w, group: int = 32) -> "Q4Weight":
+        """Quantises a dense [out, in] matrix (f32, f16 or bf16)."""
+        qb = _qb()
+        if len(w.shape) != 2:
+            raise _invalid("a dense weight has two dimensions")
+        q = cls(ctx, shape=(int(w.shape[0]), int(w.shape[1]), group))
+        p, mem, keep = q._buffer(w, None, "w")
+        stride = 0 if mem == qb.MEM_HOST else _rows_of(keep, int(w.shape[1]), "w")[1]
+        qb._check(qb.load().ql_q4_quantize(q._h, p, qb._dtype_code(keep), stride, mem))
+        return q
+
+    @classmethod
+    def from_gguf(cls, ctx, blocks, out_features: int, in_features: int) -> "Q4Weight":
+        """From GGUF Q4_0 blocks (bytes, a numpy uint8 array or a CUDA uint8 tensor)."""
+        qb = _qb()
+        q = cls(ctx, shape=(out_features, in_features, 32))
+        if isinstance(blocks, (bytes, bytearray, memoryview)):
+            blocks = np.frombuffer(blocks, np.uint8)
+        p, mem, keep = q._buffer(blocks, "uint8", "blocks")
+        n = int(keep.size if mem == qb.MEM_HOST else keep.numel())
+        qb._check(qb.load().ql_q4_set_blocks(q._h, p, n, mem))
+        return q
+
+    def _buffer(self, x, dtype, name: str):
+        """(pointer, memory kind, keep-alive) of an array or a CUDA tensor."""
+        qb = _qb()
+        if dtype and not str(x.dtype).endswith(dtype):
+            raise _invalid(f"{name} must be {dtype}, got {x.dtype}")
+        if not isinstance(x, np.ndarray):
+            if not x.is_cuda:
+                x = x.contiguous()
+                return x.data_ptr(), qb.MEM_HOST, x
+            if dtype and not x.is_contiguous():
+                raise _invalid(f"{name} must be contiguous")
+            return _on(self.ctx, x, name), qb.MEM_DEVICE, x
+        x = np.ascontiguousarray(x)
+        return x.ctypes.data, qb.MEM_HOST, x
+
+    def set(self, codes, scales) -> None:
+        """New codes and scales of the same shape (ql_q4_set)."""
+        qb = _qb()
+        n, k = self.out_features, self.in_features
+        if tuple(codes.shape) != (n, k // 2) or tuple(scales.shape) != (n, k // self.group):
+            raise _invalid(f"codes and scales must be [{n}, {k // 2}] and "
+                           f"[{n}, {k // self.group}]")
+        cp, mem, c = self._buffer(codes, "uint8", "codes")
+        sp, mem2, s = self._buffer(scales, "float16", "scales")
+        if mem != mem2:
+            raise _invalid("codes and scales must live in the same memory")
+        qb._check(qb.load().ql_q4_set(self._h, cp, sp, mem))
+
+    def get(self):
+        """(codes, scales) as numpy arrays in the constructor's layout."""
+        qb = _qb()
+        codes = np.empty((self.out_features, self.in_features // 2), np.uint8)
+        scales = np.empty((self.out_features, self.in_features // self.group), np.float16)
+        qb._check(qb.load().ql_q4_get(self._h, codes.ctypes.data, scales.ctypes.data,
+                                      qb.MEM_HOST))
+        return codes, scales
+
+    def close(self) -> None:
+        if getattr(self, "_h", None):
+            _qb().load().ql_q4_destroy(self._h)
+            self._h = None
+
+    def __del__(self):
+        try:
+            self.close()
+        except Exception:  # interpreter shutdown: the library may already be gone
+            pass
+
+
+def linear_q4(weight: Q4Weight, x, x_scale=None, out=None, out_dtype: str | None = None):
+    """x W^T of a few rows x [..., in_features] with 4-bit weights (ql_linear_q4).
+
+    x is f32, f16 or bf16, or int8 with x_scale f16 [..., in_features / 32] (the
+    Q8_0 output of rms_norm).  The result is [..., out_features] of out_dtype
+    (default: out's type, else x's, f32 for Q8_0); `out` may be a matrix with a
+    row stride.
+    """
+    import torch
+
+    qb = _qb()
+    ctx, k, n = weight.ctx, weight.in_features, weight.out_features
+    rows, xs = _rows_of(x, k, "x")
+    if x.dtype == torch.int8:
+        if x_scale is None:
+            raise _invalid("int8 x needs x_scale")
+        _output(ctx, x_scale, x.shape[:-1] + (k // 32,), torch.float16, "x_scale")
+        in_dt, scp, t = qb.Q8_0, _on(ctx, x_scale, "x_scale"), torch.float32
+    else:
+        if x_scale is not None:
+            raise _invalid("x_scale belongs to int8 x")
+        in_dt, scp, t = _float_code(x, "x"), None, x.dtype
+    t = _out_type(out, out_dtype, t)
+    shape = x.shape[:-1] + (n,)
+    if out is None:
+        out = torch.empty(shape, dtype=t, device=x.device)
+    elif out.shape != shape or out.dtype != t:
+        raise _invalid(f"out must be {t} of shape {tuple(shape)}")
+    ys = _rows_of(out, n, "out")[1]
+    args = LinearArgs(rows, in_dt, _float_code(out, "out"), xs, ys, _on(ctx, x, "x"), scp,
+                      _on(ctx, out, "out"))
+    qb._check(qb.load().ql_linear_q4(ctx._h, weight._h, ctypes.byref(args)))
+    return out
+
+
+def verify_drafts(ctx, target, draft, draft_ids, uniforms, temperature: float = 1.0,
+                  n_draft=None, probs: bool = False, tokens=None, accepted=None):
+    """Speculative sampling's acceptance and next token (ql_verify_drafts).
+
+    target [batch, drafts + 1, vocab] and draft [batch, drafts, vocab] (or None:
+    the drafts are certain) hold logits, or probabilities with probs=True;
+    draft_ids int32 [batch, drafts]; uniforms f64 [batch, drafts + 1] (None when
+    temperature <= 0); n_draft int32 [batch] or None.  Returns (tokens int32
+    [batch, drafts + 1], accepted int32 [batch]): the accepted drafts, the new
+    token, then -1.
+    """
+    import torch
+
+    qb = _qb()
+    if target.dim() != 3 or target.shape[1] < 1:
+        raise _invalid("target must be [batch, drafts + 1, vocab]")
+    batch, m, vocab = target.shape[0], target.shape[1] - 1, target.shape[2]
+
+    def rows(t, count, name):
+        if tuple(t.shape) != (batch, count, vocab) or t.dtype != target.dtype:
+            raise _invalid(f"{name} must be {target.dtype} [{batch}, {count}, {vocab}]")
+        if not t.numel():
+            return vocab
+        row = t.stride(1) if count > 1 else t.stride(0) if batch > 1 else vocab
+        if t.stride(2) != 1 and vocab > 1 or row < vocab or \
+                batch > 1 and t.stride(0) != count * row:
+            raise _invalid(f"{name} must have its rows at one stride")
+        return row
+
+    def ints(t, shape, dtype, name):
+        if tuple(t.shape) != shape or t.dtype != dtype or not t.is_contiguous():
+            raise _invalid(f"{name} must be contiguous {dtype} {list(shape)}")
+        return _on(ctx, t, name)
+
+    ts = rows(target, m + 1, "target")
+    ds = rows(draft, m, "draft") if draft is not None else 0
+    dp = _on(ctx, draft, "draft") if draft is not None and m else None
+    ip = ints(draft_ids, (batch, m), torch.int32, "draft_ids") if m else None
+    np_ = ints(n_draft, (batch,), torch.int32, "n_draft") if n_draft is not None else None
+    up = None
+    if probs or temperature > 0:
+        if uniforms is None:
+            raise _invalid("sampling needs uniforms")
+        up = ints(uniforms, (batch, m + 1), torch.float64, "uniforms")
+    tokens = _output(ctx, tokens, (batch, m + 1), torch.int32, "tokens")
+    accepted = _output(ctx, accepted, (batch,), torch.int32, "accepted")
+    args = VerifyArgs(batch, m, vocab, _float_code(target, "target"),
+                      VERIFY_PROBS if probs else VERIFY_LOGITS, temperature, ts, ds,
+                      _on(ctx, target, "target"), dp, ip, np_, up, _on(ctx, tokens, "tokens"),
+                      _on(ctx, accepted, "accepted"))
+    qb._check(qb.load().ql_verify_drafts(ctx._h, ctypes.byref(args)))
+    return tokens, accepted
