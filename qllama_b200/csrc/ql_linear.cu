@@ -5,7 +5,9 @@
 
 #include <algorithm>
 #include <cmath>
+#include <cstdlib>
 #include <new>
+#include <type_traits>
 
 #include "../../include/qllama_model.h"
 #include "ql_device.cuh"
@@ -39,8 +41,6 @@ struct NormArgs {
   float eps;
 };
 
-constexpr int kNormThreads = 256;
-
 template <typename T>
 __device__ __forceinline__ T warp_sum(T v) {
 #pragma unroll
@@ -48,23 +48,71 @@ __device__ __forceinline__ T warp_sum(T v) {
   return v;
 }
 
-__device__ float norm_block_sum(float v, float* red) {
+// Sum over the CTA (every thread gets it, in the same order of additions).
+template <typename T>
+__device__ __forceinline__ T block_sum(T v, T* red) {
   v = warp_sum(v);
   __syncthreads();
   if ((threadIdx.x & 31) == 0) red[threadIdx.x >> 5] = v;
   __syncthreads();
-  float t = 0.f;
-  for (int i = 0; i < static_cast<int>(blockDim.x >> 5); ++i) t += red[i];
-  return t;
+  const int l = threadIdx.x & 31;
+  return warp_sum(l < static_cast<int>(blockDim.x >> 5) ? red[l] : T(0));
 }
 
-// One CTA per row.
-__global__ void __launch_bounds__(kNormThreads) rms_norm_kernel(const NormArgs a) {
-  __shared__ float red[kNormThreads / 32];
+// Whether an f32 sum of squares can be used as it is: neither overflowed (or
+// NaN) nor so small that squares below f32's normal range were a part of it.
+__device__ __forceinline__ bool plain_square_sum(float ss) {
+  return ss >= 0x1p-80f && ss < 0x1p126f;
+}
+
+// round(v), ties away from zero, for |v| < 2^22: the largest f32 below 0.5 is
+// added away from zero and the sum is cut.  (With 0.5 itself, values just below
+// a tie would be carried over it; v = 0.5 still reaches 1, since the sum rounds.)
+__device__ __forceinline__ int round_away(float v) {
+  return __float2int_rz(v + copysignf(0x1.fffffep-2f, v));
+}
+
+// Magnitudes as integers: they order like the values, and a NaN or an infinity
+// is above every finite one, so that one maximum carries both.
+__device__ __forceinline__ uint32_t magnitude(float y) { return __float_as_uint(y) & 0x7fffffffu; }
+
+// Q8_0 block scale of a block whose largest magnitude is `most`; a value v has
+// the code round_away(v * inv), within [-limit, limit] once v is cut to
+// +-*limit (infinite unless the scale saturates).
+__device__ __forceinline__ __half q8_scale(uint32_t most, float& inv, float& limit) {
+  limit = INFINITY;
+  inv = 0.f;
+  if (most >= 0x7f800000u) {
+    limit = 0.f;
+    return __ushort_as_half(0x7fff);
+  }
+  float d = __uint_as_float(most) / 127.0f;
+  if (d > 65504.0f) {
+    d = 65504.0f;
+    limit = 127.0f * 65504.0f;
+  }
+  if (d > 0.f) inv = 1.0f / d;
+  return __float2half_rn(d);
+}
+
+__device__ __forceinline__ int q8_code(float y, float inv, float limit) {
+  if (limit != INFINITY) y = limit == 0.f ? 0.f : fminf(fmaxf(y, -limit), limit);
+  return round_away(y * inv);
+}
+
+// One CTA per row, element by element, reading the row twice: what the kernel
+// below cannot take (more columns than it holds, tensors that do not start on
+// 16 bytes, strides that break the groups of eight).
+constexpr int kNormThreads = 256;
+__global__ void __launch_bounds__(kNormThreads) rms_norm_loop_kernel(const NormArgs a) {
+  __shared__ float red[32];
+  __shared__ double red_d[32];
   const size_t row = blockIdx.x;
   const size_t xo = row * static_cast<size_t>(a.x_stride);
   const size_t ro = row * static_cast<size_t>(a.residual_stride);
   const size_t oo = row * static_cast<size_t>(a.hidden);
+  ql::griddep_wait();
+  ql::griddep_launch_dependents();
   auto value = [&](int i) {
     float s = ql::load_elem(a.x, xo + i, a.in_dtype);
     if (a.residual) s += ql::load_elem(a.residual, ro + i, a.in_dtype);
@@ -75,32 +123,280 @@ __global__ void __launch_bounds__(kNormThreads) rms_norm_kernel(const NormArgs a
     const float s = value(i);
     ss += s * s;
   }
-  ss = norm_block_sum(ss, red);
-  const float inv = 1.0f / sqrtf(ss / static_cast<float>(a.hidden) + a.eps);
+  ss = block_sum(ss, red);
+  const bool plain = plain_square_sum(ss);
+  float inv = 1.0f / sqrtf(ss / static_cast<float>(a.hidden) + a.eps);
+  double inv_d = 0.0;
+  if (!plain) {
+    double sd = 0.0;
+    for (int i = threadIdx.x; i < a.hidden; i += kNormThreads) {
+      const double s = value(i);
+      sd += s * s;
+    }
+    inv_d = 1.0 / sqrt(block_sum(sd, red_d) / a.hidden + static_cast<double>(a.eps));
+  }
   const int n = (a.hidden + kNormThreads - 1) / kNormThreads * kNormThreads;
   for (int i = threadIdx.x; i < n; i += kNormThreads) {  // whole warps: the shuffles below
     float y = 0.f;
     if (i < a.hidden) {
       const float s = value(i);
+      const float w = ql::load_elem(a.weight, i, a.weight_dtype);
       if (a.sum_out) ql::store_elem(a.sum_out, oo + i, a.in_dtype, s);
-      y = s * inv * ql::load_elem(a.weight, i, a.weight_dtype);
+      y = plain ? s * inv * w : static_cast<float>(s * inv_d * w);
       if (a.out_dtype != ql::kQ8_0) ql::store_elem(a.out, oo + i, a.out_dtype, y);
     }
     if (a.out_dtype == ql::kQ8_0) {
-      float m = fabsf(y);
-      int bad = !isfinite(y);
-#pragma unroll
-      for (int o = 16; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
-      bad = __any_sync(0xffffffffu, bad);
+      const uint32_t m = __reduce_max_sync(0xffffffffu, magnitude(y));
       if (i < a.hidden) {
-        const float d = fminf(m / 127.0f, 65504.0f);
-        const float id = d > 0.f ? 1.0f / d : 0.f;
-        const float q = fminf(fmaxf(roundf(y * id), -127.f), 127.f);
-        static_cast<int8_t*>(a.out)[oo + i] = bad ? 0 : static_cast<int8_t>(q);
-        if (i % 32 == 0)
-          a.out_scale[(oo + i) / 32] = bad ? __ushort_as_half(0x7fff) : __float2half_rn(d);
+        float id, limit;
+        const __half d = q8_scale(m, id, limit);
+        static_cast<int8_t*>(a.out)[oo + i] = static_cast<int8_t>(q8_code(y, id, limit));
+        if (i % 32 == 0) a.out_scale[(oo + i) / 32] = d;
       }
     }
+  }
+}
+
+// Eight consecutive elements: 16 bytes, or 32 for f32.
+template <int DT>
+struct Raw8 {
+  static constexpr int kWords = DT == ql::kF32 ? 8 : 4;
+  uint32_t w[kWords];
+  __device__ __forceinline__ void load(const void* base, size_t i) {
+    const uint4* p = reinterpret_cast<const uint4*>(static_cast<const char*>(base) +
+                                                    i * (DT == ql::kF32 ? 4 : 2));
+#pragma unroll
+    for (int j = 0; j < kWords / 4; ++j) {
+      const uint4 v = p[j];
+      w[4 * j] = v.x;
+      w[4 * j + 1] = v.y;
+      w[4 * j + 2] = v.z;
+      w[4 * j + 3] = v.w;
+    }
+  }
+  // elements [lo, hi) of the eight one by one, zeros for the others
+  __device__ __forceinline__ void load_part(const void* base, size_t i, int lo, int hi) {
+#pragma unroll
+    for (int j = 0; j < kWords; ++j) w[j] = 0;
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+      if (e < lo || e >= hi) continue;
+      if constexpr (DT == ql::kF32)
+        w[e] = static_cast<const uint32_t*>(base)[i + e];
+      else
+        w[e / 2] |= static_cast<uint32_t>(static_cast<const uint16_t*>(base)[i + e])
+                    << (16 * (e & 1));
+    }
+  }
+  __device__ __forceinline__ void get(float (&x)[8]) const {
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+      if constexpr (DT == ql::kF32) {
+        x[e] = __uint_as_float(w[e]);
+      } else {
+        const uint16_t h = static_cast<uint16_t>(w[e / 2] >> (16 * (e & 1)));
+        if constexpr (DT == ql::kF16) x[e] = __half2float(__ushort_as_half(h));
+        else x[e] = __uint_as_float(static_cast<uint32_t>(h) << 16);
+      }
+    }
+  }
+};
+
+__device__ __forceinline__ void store_part(void* base, size_t i, int dt, const float (&x)[8],
+                                           int lo, int hi) {
+  if (lo == 0 && hi == 8) return ql::store8(base, i, dt, x, true);
+#pragma unroll
+  for (int e = 0; e < 8; ++e)
+    if (e >= lo && e < hi) ql::store_elem(base, i + e, dt, x[e]);
+}
+
+// One CTA per row; a thread holds NV groups of eight columns in registers, so
+// that x and the residual are read once, all loads of a row in flight together,
+// and the row's sum and result are written once.  Bound by those bytes for many
+// rows and by one round trip to memory plus the reduction for a few; launch_norm
+// says how NV is chosen.
+// LEAD: the row length is no multiple of eight, so a row starts `lead` elements
+// into an aligned group of eight.  Groups keep that alignment -- it is the same
+// in every contiguous tensor, whatever its type -- and only the row's first and
+// last go element by element (2000 rows of 4101 bf16 columns: 52.8 us with
+// element-wise loads throughout).
+constexpr int kNormMax = 16384;  // 512 threads x 32 columns
+template <int DT, int WT, int NV, bool LEAD>
+__global__ void __launch_bounds__(NV == 1 ? 1024 : 512, NV == 1 ? 1 : 2)
+    rms_norm_kernel(const NormArgs a) {
+  __shared__ float red[32];
+  __shared__ double red_d[32];
+  const size_t row = blockIdx.x;
+  const size_t oo = row * static_cast<size_t>(a.hidden);
+  const int lead = LEAD ? static_cast<int>(oo % 8) : 0;
+  ql::griddep_wait();
+  ql::griddep_launch_dependents();
+  // where x and the residual fill the registers, the weight is left for later
+  constexpr bool kEarly = NV * (DT == ql::kF32 ? 2 : 1) < 4;
+  Raw8<DT> xr[NV], rr[NV];
+  Raw8<WT> wr[NV];
+  auto column = [&](int j) { return 8 * static_cast<int>(threadIdx.x + j * blockDim.x) - lead; };
+  auto read = [&](auto& r, const void* base, size_t at, int c, bool whole) {
+    if (!LEAD || whole) r.load(base, at + c);
+    else r.load_part(base, at + c, c < 0 ? -c : 0, min(8, a.hidden - c));
+  };
+#pragma unroll
+  for (int j = 0; j < NV; ++j) {
+    const int c = column(j);
+    if (c < a.hidden) {
+      const bool whole = c >= 0 && c + 8 <= a.hidden;
+      read(xr[j], a.x, row * static_cast<size_t>(a.x_stride), c, whole);
+      if (a.residual) read(rr[j], a.residual, row * static_cast<size_t>(a.residual_stride), c, whole);
+    }
+  }
+  if constexpr (kEarly) {
+#pragma unroll
+    for (int j = 0; j < NV; ++j)
+      if (column(j) < a.hidden) read(wr[j], a.weight, 0, column(j), lead == 0 && column(j) + 8 <= a.hidden);
+  }
+  float s[NV][8];
+  float ss = 0.f;
+#pragma unroll
+  for (int j = 0; j < NV; ++j) {
+    const int c = column(j);
+    if (c < a.hidden) {
+      xr[j].get(s[j]);
+      if (a.residual) {
+        float r[8];
+        rr[j].get(r);
+#pragma unroll
+        for (int e = 0; e < 8; ++e) s[j][e] += r[e];
+        if (a.sum_out)
+          store_part(a.sum_out, oo + c, DT, s[j], LEAD && c < 0 ? -c : 0,
+                     LEAD ? min(8, a.hidden - c) : 8);
+      }
+#pragma unroll
+      for (int e = 0; e < 8; ++e) ss += s[j][e] * s[j][e];
+    } else {
+#pragma unroll
+      for (int e = 0; e < 8; ++e) s[j][e] = 0.f;
+    }
+  }
+  ss = block_sum(ss, red);
+  float inv = 1.0f / sqrtf(ss / static_cast<float>(a.hidden) + a.eps);
+  if (!plain_square_sum(ss)) {
+    // the same for every thread: 64 bits, and s becomes s * inv here
+    double sd = 0.0;
+#pragma unroll
+    for (int j = 0; j < NV; ++j)
+#pragma unroll
+      for (int e = 0; e < 8; ++e) sd += static_cast<double>(s[j][e]) * s[j][e];
+    const double id =
+        1.0 / sqrt(block_sum(sd, red_d) / a.hidden + static_cast<double>(a.eps));
+#pragma unroll
+    for (int j = 0; j < NV; ++j)
+#pragma unroll
+      for (int e = 0; e < 8; ++e) s[j][e] = static_cast<float>(s[j][e] * id);
+    inv = 1.f;
+  }
+#pragma unroll
+  for (int j = 0; j < NV; ++j) {
+    const int c = column(j);
+    const bool in = c < a.hidden;
+    float y[8];
+#pragma unroll
+    for (int e = 0; e < 8; ++e) y[e] = 0.f;
+    if (in) {
+      float w[8];
+      if constexpr (!kEarly) read(wr[j], a.weight, 0, c, lead == 0 && c + 8 <= a.hidden);
+      wr[j].get(w);
+#pragma unroll
+      for (int e = 0; e < 8; ++e) y[e] = s[j][e] * inv * w[e];
+    }
+    if (LEAD || a.out_dtype != ql::kQ8_0) {
+      if (in)
+        store_part(a.out, oo + c, a.out_dtype, y, LEAD && c < 0 ? -c : 0,
+                   LEAD ? min(8, a.hidden - c) : 8);
+      continue;
+    }
+    // a block of 32 columns is four neighbouring lanes' (hidden % 32 == 0:
+    // all four inside the row, or none)
+    uint32_t m = 0;
+#pragma unroll
+    for (int e = 0; e < 8; ++e) m = max(m, magnitude(y[e]));
+    m = max(m, __shfl_xor_sync(0xffffffffu, m, 1));
+    m = max(m, __shfl_xor_sync(0xffffffffu, m, 2));
+    float id, limit;
+    const __half d = q8_scale(m, id, limit);
+    uint32_t q[8];
+#pragma unroll
+    for (int e = 0; e < 8; ++e) q[e] = static_cast<uint32_t>(q8_code(y[e], id, limit));
+    if (in) {
+      uint2 w;
+      w.x = __byte_perm(__byte_perm(q[0], q[1], 0x0040), __byte_perm(q[2], q[3], 0x0040), 0x5410);
+      w.y = __byte_perm(__byte_perm(q[4], q[5], 0x0040), __byte_perm(q[6], q[7], 0x0040), 0x5410);
+      *reinterpret_cast<uint2*>(static_cast<int8_t*>(a.out) + oo + c) = w;
+      if ((threadIdx.x & 3) == 0) a.out_scale[(oo + c) / 32] = d;
+    }
+  }
+}
+
+// A launch that may begin while the kernel before it in the stream drains
+// (every kernel here waits for that kernel's end before it touches a tensor).
+template <typename... P, typename... A>
+cudaError_t launch_pdl(void (*kernel)(P...), dim3 grid, dim3 block, size_t smem, cudaStream_t s,
+                       bool pdl, A... args) {
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = grid;
+  cfg.blockDim = block;
+  cfg.dynamicSmemBytes = smem;
+  cfg.stream = s;
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = pdl ? 1 : 0;
+  return cudaLaunchKernelEx(&cfg, kernel, args...);
+}
+
+// NV: a few rows go over as many threads as they have groups (one round trip,
+// the shortest reduction); with two rows or more for every SM, twice as many
+// columns a thread (fewer threads wait in a reduction).
+cudaError_t launch_norm(const NormArgs& a, int num_sms, cudaStream_t s) {
+  auto fits = [](const void* p, int dt, int64_t stride) {
+    const size_t to = dt == QL_Q8_0 ? 8 : 16;
+    return aligned(p, to) && (stride * type_bytes(dt)) % to == 0;
+  };
+  const bool bases = aligned(a.x, 16) && aligned(a.residual, 16) && aligned(a.sum_out, 16) &&
+                     aligned(a.weight, 16) && aligned(a.out, a.out_dtype == QL_Q8_0 ? 8 : 16);
+  const bool even = a.hidden % 8 == 0 && fits(a.x, a.in_dtype, a.x_stride) &&
+                    (!a.residual || fits(a.residual, a.in_dtype, a.residual_stride));
+  const bool lead = !even && a.hidden % 8 != 0 && a.x_stride == a.hidden &&
+                    (!a.residual || a.residual_stride == a.hidden);
+  if (!bases || !(even || lead) || a.hidden > kNormMax - 8)
+    return launch_pdl(rms_norm_loop_kernel, dim3(a.rows), dim3(kNormThreads), 0, s, true, a);
+  const int groups = (a.hidden + 7) / 8 + lead;
+  int nv = groups <= 1024 ? 1 : 4;
+  if (nv == 1 && a.rows >= 2 * num_sms && groups >= 256) nv = 2;
+  if (const char* e = getenv("QLNV")) nv = atoi(e);
+  const int threads = ((groups + nv - 1) / nv + 31) / 32 * 32;
+  const dim3 grid(a.rows), block(threads);
+  auto go = [&](auto dt, auto wt, auto ld) {
+    constexpr int DT = decltype(dt)::value, WT = decltype(wt)::value;
+    constexpr bool LEAD = decltype(ld)::value;
+    if (nv == 1) return launch_pdl(rms_norm_kernel<DT, WT, 1, LEAD>, grid, block, 0, s, true, a);
+    if (nv == 2) return launch_pdl(rms_norm_kernel<DT, WT, 2, LEAD>, grid, block, 0, s, true, a);
+    return launch_pdl(rms_norm_kernel<DT, WT, 4, LEAD>, grid, block, 0, s, true, a);
+  };
+  auto by_lead = [&](auto dt, auto wt) {
+    return lead ? go(dt, wt, std::true_type()) : go(dt, wt, std::false_type());
+  };
+  auto by_weight = [&](auto dt) {
+    switch (a.weight_dtype) {
+      case QL_F32: return by_lead(dt, std::integral_constant<int, ql::kF32>());
+      case QL_F16: return by_lead(dt, std::integral_constant<int, ql::kF16>());
+      default: return by_lead(dt, std::integral_constant<int, ql::kBF16>());
+    }
+  };
+  switch (a.in_dtype) {
+    case QL_F32: return by_weight(std::integral_constant<int, ql::kF32>());
+    case QL_F16: return by_weight(std::integral_constant<int, ql::kF16>());
+    default: return by_weight(std::integral_constant<int, ql::kBF16>());
   }
 }
 
@@ -385,8 +681,7 @@ int ql_rms_norm(ql_ctx* c, const ql_norm_args* args) {
   a.weight_dtype = f.weight_dtype;
   a.out_dtype = f.out_dtype;
   a.eps = f.eps;
-  rms_norm_kernel<<<f.rows, kNormThreads, 0, c->stream>>>(a);
-  QLN_CUDA(cudaGetLastError(), "launch rms_norm");
+  QLN_CUDA(launch_norm(a, c->num_sms, c->stream), "launch rms_norm");
   return QL_OK;
 }
 
