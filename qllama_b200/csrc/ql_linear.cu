@@ -373,7 +373,6 @@ cudaError_t launch_norm(const NormArgs& a, int num_sms, cudaStream_t s) {
   const int groups = (a.hidden + 7) / 8 + lead;
   int nv = groups <= 1024 ? 1 : 4;
   if (nv == 1 && a.rows >= 2 * num_sms && groups >= 256) nv = 2;
-  if (const char* e = getenv("QLNV")) nv = atoi(e);
   const int threads = ((groups + nv - 1) / nv + 31) / 32 * 32;
   const dim3 grid(a.rows), block(threads);
   auto go = [&](auto dt, auto wt, auto ld) {
@@ -409,14 +408,19 @@ cudaError_t launch_norm(const NormArgs& a, int num_sms, cudaStream_t s) {
 // 16 tile + g + 8 h, columns 64 chunk + 32 j + 8 t .. + 7 -- the lane that needs
 // them in the A fragment of an m16n8k16 / m16n8k32 product (any order of the
 // columns inside a fragment serves, if x follows it).  A word holds the eight
-// values (code - 8) as two's-complement nibbles in the order of kNibble.  Scales:
-// f16, per tile (g, j, h), 64 bytes, each read by the four lanes of a quad.
+// values (code - 8) as two's-complement nibbles in the order of nibble_of.  Scales:
+// f16, one for each row and group of 32 columns (64 bytes a tile, [g][j][h]), of
+// 64 (32 bytes a tile, [g][h]) or of 128 (32 bytes for two tiles along the columns);
+// the four lanes of a quad read the same.
 struct ql_q4 {
   ql_ctx* ctx = nullptr;
   int n = 0, k = 0, group = 0;
   int tiles = 0, chunks = 0;
   uint32_t* codes = nullptr;   // [tiles][chunks][32][4]
-  __half* scales = nullptr;    // [tiles][chunks][8][2][2]
+  __half* scales = nullptr;    // [tiles][chunks][8][2][2], [tiles][chunks or chunks/2][8][2]
+  // Written since the last product: the next one starts only when all work
+  // queued before it is done, and may not read the weights ahead.
+  mutable bool fresh = true;
 };
 
 namespace {
@@ -438,7 +442,18 @@ Q4View view_of(const ql_q4* w) {
 }
 
 size_t q4_words(const ql_q4* w) { return static_cast<size_t>(w->tiles) * w->chunks * 128; }
-size_t q4_scales(const ql_q4* w) { return static_cast<size_t>(w->tiles) * w->chunks * 32; }
+size_t q4_scales(const ql_q4* w) {
+  const size_t tiles = static_cast<size_t>(w->tiles) * w->chunks;
+  return w->group == 32 ? tiles * 32 : w->group == 64 ? tiles * 16 : tiles * 8;
+}
+
+// Place of the scale of row g + 8 h and 32 columns j of tile (tile, chunk).
+__host__ __device__ __forceinline__ size_t scale_at(int group, int chunks, size_t tile, int chunk,
+                                                    int g, int j, int h) {
+  if (group == 32) return ((tile * chunks + chunk) * 8 + g) * 4 + 2 * j + h;
+  if (group == 64) return ((tile * chunks + chunk) * 8 + g) * 2 + h;
+  return ((tile * (chunks / 2) + chunk / 2) * 8 + g) * 2 + h;
+}
 
 // Row and first column of word i of lane `lane` of tile (tile, chunk).
 __device__ __forceinline__ void word_place(size_t tile, int chunk, int lane, int i, int& row,
@@ -515,9 +530,10 @@ __global__ void __launch_bounds__(256) q4_pack_kernel(const PackArgs a) {
     }
   }
   a.w.codes[id] = word;
-  if ((lane & 3) == 0)  // one lane of the quad writes (g, j, h)
-    reinterpret_cast<uint16_t*>(a.w.scales)[(tile * a.w.chunks + chunk) * 32 + (lane >> 2) * 4 + i] =
-        scale;
+  // one lane of the quad writes, where the group (or its padding) starts
+  if ((lane & 3) == 0 && col % a.w.group == 0)
+    reinterpret_cast<uint16_t*>(
+        a.w.scales)[scale_at(a.w.group, a.w.chunks, tile, chunk, lane >> 2, i >> 1, i & 1)] = scale;
 }
 
 // The device order back to codes and scales (one thread per word).
@@ -541,12 +557,13 @@ __global__ void __launch_bounds__(256) q4_unpack_kernel(Q4View w, uint8_t* codes
   if (scales && col % w.group == 0)
     scales[static_cast<size_t>(row) * (w.k / w.group) + col / w.group] =
         reinterpret_cast<const uint16_t*>(
-            w.scales)[(tile * w.chunks + chunk) * 32 + (lane >> 2) * 4 + i];
+            w.scales)[scale_at(w.group, w.chunks, tile, chunk, lane >> 2, i >> 1, i & 1)];
 }
 
 template <int FROM>
 int launch_pack(ql_q4* w, PackArgs a) {
   a.w = view_of(w);
+  w->fresh = true;
   const size_t blocks = (q4_words(w) + 255) / 256;
   q4_pack_kernel<FROM><<<static_cast<unsigned>(blocks), 256, 0, w->ctx->stream>>>(a);
   QLN_CUDA(cudaGetLastError(), "launch the 4-bit layout");
@@ -589,35 +606,394 @@ struct LinearArgs {
   int rows, in_dtype, out_dtype;
 };
 
-// One warp per output column: the words of its weight row, lane by lane.
-__global__ void __launch_bounds__(128) linear_q4_kernel(const LinearArgs a) {
-  const int lane = threadIdx.x & 31;
-  const size_t n = static_cast<size_t>(blockIdx.x) * 4 + (threadIdx.x >> 5);
-  if (n >= static_cast<size_t>(a.w.n)) return;
-  const size_t tile = n / 16;
-  const int g = static_cast<int>(n % 8), h = static_cast<int>(n / 8 % 2);
-  for (int r = 0; r < a.rows; ++r) {
-    float acc = 0.f;
-    const size_t xo = static_cast<size_t>(r) * a.x_stride;
-    for (int c8 = lane; c8 < a.w.k / 8; c8 += 32) {
-      const int chunk = c8 >> 3, j = c8 >> 2 & 1, t = c8 & 3;
-      const uint32_t word =
-          a.w.codes[((tile * a.w.chunks + chunk) * 32 + 4 * g + t) * 4 + 2 * j + h];
-      float s = 0.f;
-      for (int e = 0; e < 8; ++e) {
-        const int q = static_cast<int>(word << (28 - 4 * nibble_of(e))) >> 28;
-        const float xv = a.in_dtype == ql::kQ8_0
-                             ? static_cast<const int8_t*>(a.x)[xo + 8 * c8 + e]
-                             : ql::load_elem(a.x, xo + 8 * c8 + e, a.in_dtype);
-        s = fmaf(static_cast<float>(q), xv, s);
-      }
-      s *= __half2float(a.w.scales[(tile * a.w.chunks + chunk) * 32 + 4 * g + 2 * j + h]);
-      if (a.in_dtype == ql::kQ8_0)
-        s *= __half2float(a.x_scale[static_cast<size_t>(r) * (a.w.k / 32) + c8 / 4]);
-      acc += s;
+// ---- the tensor-core product ----
+// Formula: y[r][n] = sum over blocks of 32 columns of scale * (sum of (code - 8) x).
+// The weights' bytes (0.53-0.56 of them per weight) are the cost of a few rows, so
+// they stream straight from HBM into the registers of the lanes that multiply them,
+// 16 bytes a lane, with the next ones in flight while one set is multiplied.
+// A warp owns MT tiles of 16 weight rows and every 8th chunk of 64 columns; the
+// weights are the A operand (16 rows of W), x the B operand (8 columns), so one
+// row of x costs as much as eight.  Codes turn into f16 / bf16 exactly (a nibble
+// in the mantissa of 1024 or 128, less an offset), or into int8 (a two's-complement
+// nibble in the high half of a byte: 16 times its value).  Blocks of 32 sum on the
+// tensor cores in f32 (int32 for Q8_0: exact), are scaled in f32 and added to f32
+// sums.  f32 rows: three bf16 parts of 8 significand bits each carry a value's 24
+// exactly; the parts are three columns of B, whose sums are added at the end.
+// The split of the columns over the warps and every order of additions are the
+// same for all MT, NT and row counts, so a row's bits depend only on it and W.
+constexpr int kLinWarps = 8;
+constexpr int kLinThreads = 32 * kLinWarps;
+
+// D = A B (no addend)
+template <bool BF>
+__device__ __forceinline__ void mma16816_first(float (&d)[4], const uint32_t (&a)[4], uint32_t b0,
+                                               uint32_t b1) {
+  if constexpr (BF) {
+    asm volatile(
+        "mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, "
+        "{%8,%9}, {%10,%10,%10,%10};"
+        : "=f"(d[0]), "=f"(d[1]), "=f"(d[2]), "=f"(d[3])
+        : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1), "f"(0.f));
+  } else {
+    asm volatile(
+        "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, "
+        "{%8,%9}, {%10,%10,%10,%10};"
+        : "=f"(d[0]), "=f"(d[1]), "=f"(d[2]), "=f"(d[3])
+        : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1), "f"(0.f));
+  }
+}
+
+__device__ __forceinline__ uint4 ld_weights(const void* p) {
+  uint4 v;
+  asm volatile("ld.global.nc.L1::no_allocate.v4.u32 {%0,%1,%2,%3}, [%4];"
+               : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w)
+               : "l"(p));
+  return v;
+}
+
+// (a & b) ^ c
+__device__ __forceinline__ uint32_t and_xor(uint32_t a, uint32_t b, uint32_t c) {
+  uint32_t d;
+  asm("lop3.b32 %0, %1, %2, %3, 0x6a;" : "=r"(d) : "r"(a), "r"(b), "r"(c));
+  return d;
+}
+
+// A word's eight values as four pairs in x's order, exactly.
+template <bool BF>
+__device__ __forceinline__ void unpack_word(uint32_t w, uint32_t (&p)[4]) {
+  if constexpr (BF) {
+    const uint32_t in[4] = {w, w >> 8, w >> 4, w >> 12};
+    const __nv_bfloat162 off = __halves2bfloat162(__ushort_as_bfloat16(0x4308),
+                                                  __ushort_as_bfloat16(0x4308));  // 136
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const uint32_t h = and_xor(in[i], 0x000f000fu, 0x43084308u);  // 128 + (value + 8)
+      const __nv_bfloat162 v = __hsub2(*reinterpret_cast<const __nv_bfloat162*>(&h), off);
+      p[i] = *reinterpret_cast<const uint32_t*>(&v);
     }
-    acc = warp_sum(acc);
-    if (lane == 0) ql::store_elem(a.y, static_cast<size_t>(r) * a.y_stride + n, a.out_dtype, acc);
+  } else {
+    const __half2 off = __halves2half2(__ushort_as_half(0x6408), __ushort_as_half(0x6408));  // 1032
+    const __half2 s16 = __halves2half2(__ushort_as_half(0x2c00), __ushort_as_half(0x2c00));  // 1/16
+    const __half2 m72 = __halves2half2(__ushort_as_half(0xd480), __ushort_as_half(0xd480));  // -72
+    const uint32_t in[2] = {w, w >> 8};
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      const uint32_t lo = and_xor(in[i], 0x000f000fu, 0x64086408u);  // 1024 + (value + 8)
+      const uint32_t hi = and_xor(in[i], 0x00f000f0u, 0x64806480u);  // 1024 + 16 (value + 8)
+      const __half2 a = __hsub2(*reinterpret_cast<const __half2*>(&lo), off);
+      const __half2 b = __hfma2(*reinterpret_cast<const __half2*>(&hi), s16, m72);
+      p[i] = *reinterpret_cast<const uint32_t*>(&a);
+      p[i + 2] = *reinterpret_cast<const uint32_t*>(&b);
+    }
+  }
+}
+
+template <int IN, int NT, int MT, int G>
+struct LinCfg {
+  static constexpr bool kQ8 = IN == ql::kQ8_0;
+  static constexpr bool kBF = IN == ql::kBF16 || IN == ql::kF32;
+  static constexpr int kParts = IN == ql::kF32 ? 3 : 1;
+  static constexpr int kRows = 8 * NT / kParts;  // rows of x in one pass
+  static constexpr int kU = MT >= 4 ? 1 : 4 / MT;  // chunks of one set
+  static constexpr int kXWords = kQ8 ? 2 : 4;      // words of a block of 32 in a lane
+  static constexpr int kPitch = 16 * MT + 4;
+  static constexpr int kSmem = kLinWarps * 8 * NT * kPitch * 4;
+};
+
+// One set of loads: U chunks of MT tiles, with x.
+template <int IN, int NT, int MT, int G>
+struct LinSet {
+  using C = LinCfg<IN, NT, MT, G>;
+  uint4 w[C::kU][MT];
+  uint2 s[C::kU][MT];  // f16: rows g, g + 8 of block j in .x / .y; G >= 64: .x alone
+  uint32_t x[C::kU][NT][2][C::kXWords];
+  float sx[C::kQ8 ? C::kU : 1][C::kQ8 ? NT : 1][2][2];  // [block][column 2t, 2t + 1]
+};
+
+template <int IN, int NT, int MT, int G>
+__global__ void __launch_bounds__(kLinThreads) linear_q4_kernel(const LinearArgs a) {
+  using C = LinCfg<IN, NT, MT, G>;
+  extern __shared__ float red[];
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
+  const int tile0 = blockIdx.x * MT;
+  const int r0 = blockIdx.y * C::kRows;
+  const int rows = min(a.rows - r0, C::kRows);
+  const int chunks = a.w.chunks, steps = (chunks + kLinWarps - 1) / kLinWarps;
+
+  using Set = LinSet<IN, NT, MT, G>;
+  auto load_w = [&](Set& z, int step) {
+#pragma unroll
+    for (int u = 0; u < C::kU; ++u) {
+      const int chunk = (step + u) * kLinWarps + warp;
+      const bool ok = chunk < chunks;
+#pragma unroll
+      for (int m = 0; m < MT; ++m) {
+        const size_t tile = min(tile0 + m, a.w.tiles - 1);  // past the end: not stored
+        z.w[u][m] = make_uint4(0, 0, 0, 0);
+        z.s[u][m] = make_uint2(0, 0);
+        if (ok) {
+          z.w[u][m] = ld_weights(a.w.codes + ((tile * chunks + chunk) * 32 + lane) * 4);
+          const __half* sp = a.w.scales + scale_at(G, chunks, tile, chunk, g, 0, 0);
+          if constexpr (G == 32) z.s[u][m] = __ldg(reinterpret_cast<const uint2*>(sp));
+          else z.s[u][m].x = __ldg(reinterpret_cast<const uint32_t*>(sp));
+        }
+      }
+    }
+  };
+  // this lane's column of each B tile: a row of x (and a part of it)
+  const char* xrow[NT];
+  bool live[NT];
+  constexpr int kBytes = IN == ql::kF32 ? 4 : C::kQ8 ? 1 : 2;
+  const bool vec = (reinterpret_cast<uintptr_t>(a.x) | static_cast<uintptr_t>(a.x_stride * kBytes)) %
+                       (C::kQ8 ? 8 : 16) == 0;
+  uint32_t m1[NT], m2[NT];  // f32: the bits that parts 1 and 2 take off first
+#pragma unroll
+  for (int n = 0; n < NT; ++n) {
+    const int col = 8 * n + g;
+    const int r = col / C::kParts, part = col % C::kParts;
+    live[n] = r < rows;
+    xrow[n] = static_cast<const char*>(a.x) +
+              static_cast<size_t>(r0 + (live[n] ? r : 0)) * a.x_stride * kBytes;
+    m1[n] = part >= 1 ? 0xffff0000u : 0u;
+    m2[n] = part == 2 ? 0xffff0000u : 0u;
+  }
+  auto load_x = [&](Set& z, int step) {
+#pragma unroll
+    for (int u = 0; u < C::kU; ++u) {
+      const int chunk = (step + u) * kLinWarps + warp;
+#pragma unroll
+      for (int j = 0; j < 2; ++j) {
+        const int k = 64 * chunk + 32 * j;
+        const bool ok = k < a.w.k;
+#pragma unroll
+        for (int n = 0; n < NT; ++n) {
+          uint32_t(&o)[C::kXWords] = z.x[u][n][j];
+#pragma unroll
+          for (int i = 0; i < C::kXWords; ++i) o[i] = 0;
+          if (ok && live[n]) {
+            const char* p = xrow[n] + static_cast<size_t>(k + 8 * t) * kBytes;
+            if constexpr (C::kQ8) {
+              if (vec) {
+                const uint2 v = *reinterpret_cast<const uint2*>(p);
+                o[0] = v.x;
+                o[1] = v.y;
+              } else {
+#pragma unroll
+                for (int e = 0; e < 8; ++e)
+                  o[e / 4] |= static_cast<uint32_t>(reinterpret_cast<const uint8_t*>(p)[e])
+                              << (8 * (e % 4));
+              }
+            } else if constexpr (IN == ql::kF32) {
+              uint32_t f[8];
+              if (vec) {
+                const uint4 v = reinterpret_cast<const uint4*>(p)[0];
+                const uint4 q = reinterpret_cast<const uint4*>(p)[1];
+                f[0] = v.x; f[1] = v.y; f[2] = v.z; f[3] = v.w;
+                f[4] = q.x; f[5] = q.y; f[6] = q.z; f[7] = q.w;
+              } else {
+#pragma unroll
+                for (int e = 0; e < 8; ++e) f[e] = reinterpret_cast<const uint32_t*>(p)[e];
+              }
+#pragma unroll
+              for (int e = 0; e < 8; ++e) {
+                float v = __uint_as_float(f[e]);
+                v -= __uint_as_float(__float_as_uint(v) & m1[n]);
+                v -= __uint_as_float(__float_as_uint(v) & m2[n]);
+                f[e] = __float_as_uint(v);
+              }
+#pragma unroll
+              for (int i = 0; i < 4; ++i) o[i] = __byte_perm(f[2 * i], f[2 * i + 1], 0x7632);
+            } else {
+              if (vec) {
+                const uint4 v = *reinterpret_cast<const uint4*>(p);
+                o[0] = v.x; o[1] = v.y; o[2] = v.z; o[3] = v.w;
+              } else {
+#pragma unroll
+                for (int e = 0; e < 8; ++e)
+                  o[e / 2] |= static_cast<uint32_t>(reinterpret_cast<const uint16_t*>(p)[e])
+                              << (16 * (e % 2));
+              }
+            }
+          }
+          if constexpr (C::kQ8) {
+#pragma unroll
+            for (int c = 0; c < 2; ++c) {
+              const int r = 8 * n + 2 * t + c;
+              z.sx[u][n][j][c] = 0.f;
+              if (ok && r < rows)  // 1/16: the codes are 16 times their values
+                z.sx[u][n][j][c] =
+                    0.0625f * __half2float(a.x_scale[static_cast<size_t>(r0 + r) * (a.w.k / 32) +
+                                                     k / 32]);
+            }
+          }
+        }
+      }
+    }
+  };
+
+  float acc[MT][NT][4];
+#pragma unroll
+  for (int m = 0; m < MT; ++m)
+#pragma unroll
+    for (int n = 0; n < NT; ++n)
+#pragma unroll
+      for (int i = 0; i < 4; ++i) acc[m][n][i] = 0.f;
+
+  auto multiply = [&](const Set& z) {
+#pragma unroll
+    for (int u = 0; u < C::kU; ++u) {
+#pragma unroll
+      for (int m = 0; m < MT; ++m) {
+        const uint32_t w[4] = {z.w[u][m].x, z.w[u][m].y, z.w[u][m].z, z.w[u][m].w};
+        if constexpr (C::kQ8) {
+#pragma unroll
+          for (int j = 0; j < 2; ++j) {
+            const uint32_t sw = G == 32 && j == 1 ? z.s[u][m].y : z.s[u][m].x;
+            const float2 s = __half22float2(*reinterpret_cast<const __half2*>(&sw));
+            const uint4 A = make_uint4((w[2 * j] << 4) & 0xf0f0f0f0u, (w[2 * j + 1] << 4) & 0xf0f0f0f0u,
+                                       w[2 * j] & 0xf0f0f0f0u, w[2 * j + 1] & 0xf0f0f0f0u);
+#pragma unroll
+            for (int n = 0; n < NT; ++n) {
+              // sums start at the bits of 1.5 * 2^23: below 2^22 they are the
+              // mantissa of a float, and a subtraction converts them
+              int d[4] = {0x4b400000, 0x4b400000, 0x4b400000, 0x4b400000};
+              ql::mma16832_s8(d, A, __byte_perm(z.x[u][n][j][0], 0, 0x3120),
+                              __byte_perm(z.x[u][n][j][1], 0, 0x3120));
+#pragma unroll
+              for (int i = 0; i < 4; ++i)
+                acc[m][n][i] = fmaf(__int_as_float(d[i]) - 12582912.0f,
+                                    (i < 2 ? s.x : s.y) * z.sx[u][n][j][i & 1], acc[m][n][i]);
+            }
+          }
+        } else {
+          uint32_t lo[2][4], hi[2][4];  // rows g and g + 8 of both blocks
+#pragma unroll
+          for (int j = 0; j < 2; ++j) {
+            unpack_word<C::kBF>(w[2 * j], lo[j]);
+            unpack_word<C::kBF>(w[2 * j + 1], hi[j]);
+          }
+#pragma unroll
+          for (int n = 0; n < NT; ++n) {
+            float d[4];
+#pragma unroll
+            for (int j = 0; j < 2; ++j) {
+              const uint32_t A0[4] = {lo[j][0], hi[j][0], lo[j][1], hi[j][1]};
+              const uint32_t A1[4] = {lo[j][2], hi[j][2], lo[j][3], hi[j][3]};
+              if (G == 32 || j == 0)
+                mma16816_first<C::kBF>(d, A0, z.x[u][n][j][0], z.x[u][n][j][1]);
+              else
+                ql::mma16816<C::kBF>(d, A0, z.x[u][n][j][0], z.x[u][n][j][1]);
+              ql::mma16816<C::kBF>(d, A1, z.x[u][n][j][2], z.x[u][n][j][3]);
+              if (G == 32 || j == 1) {
+                const uint32_t sw = G == 32 && j == 1 ? z.s[u][m].y : z.s[u][m].x;
+                const float2 s = __half22float2(*reinterpret_cast<const __half2*>(&sw));
+                acc[m][n][0] = fmaf(d[0], s.x, acc[m][n][0]);
+                acc[m][n][1] = fmaf(d[1], s.x, acc[m][n][1]);
+                acc[m][n][2] = fmaf(d[2], s.y, acc[m][n][2]);
+                acc[m][n][3] = fmaf(d[3], s.y, acc[m][n][3]);
+              }
+            }
+          }
+        }
+      }
+    }
+  };
+
+  // The first weights do not depend on the kernel before this one (a product
+  // after a write of the weights is launched without the overlap).
+  Set z0, z1;
+  load_w(z0, 0);
+  ql::griddep_wait();
+  ql::griddep_launch_dependents();
+  load_x(z0, 0);
+  for (int step = 0; step < steps; step += 2 * C::kU) {
+    if (step + C::kU < steps) {
+      load_w(z1, step + C::kU);
+      load_x(z1, step + C::kU);
+    }
+    multiply(z0);
+    if (step + C::kU >= steps) break;
+    if (step + 2 * C::kU < steps) {
+      load_w(z0, step + 2 * C::kU);
+      load_x(z0, step + 2 * C::kU);
+    }
+    multiply(z1);
+  }
+
+  // join the warps: red[warp][column][row]
+  float* mine = red + static_cast<size_t>(warp) * 8 * NT * C::kPitch;
+#pragma unroll
+  for (int m = 0; m < MT; ++m)
+#pragma unroll
+    for (int n = 0; n < NT; ++n)
+#pragma unroll
+      for (int i = 0; i < 4; ++i)
+        mine[(8 * n + 2 * t + (i & 1)) * C::kPitch + 16 * m + g + 8 * (i >> 1)] = acc[m][n][i];
+  __syncthreads();
+  for (int i = threadIdx.x; i < 16 * MT * rows; i += kLinThreads) {
+    const int row = i % (16 * MT), r = i / (16 * MT);
+    const int n = tile0 * 16 + row;
+    if (n >= a.w.n) continue;
+    float y = 0.f;
+#pragma unroll
+    for (int p = C::kParts - 1; p >= 0; --p) {  // the small parts first
+      float v = 0.f;
+#pragma unroll
+      for (int w = 0; w < kLinWarps; ++w)
+        v += red[(static_cast<size_t>(w) * 8 * NT + r * C::kParts + p) * C::kPitch + row];
+      y += v;
+    }
+    ql::store_elem(a.y, static_cast<size_t>(r0 + r) * a.y_stride + n, a.out_dtype, y);
+  }
+}
+
+template <int IN, int NT, int MT, int G>
+cudaError_t launch_linear_as(const LinearArgs& a, bool pdl, cudaStream_t s) {
+  using C = LinCfg<IN, NT, MT, G>;
+  const int kern_smem = C::kSmem;
+  if constexpr (C::kSmem > 48 * 1024) {
+    const cudaError_t e =
+        cudaFuncSetAttribute(linear_q4_kernel<IN, NT, MT, G>,
+                             cudaFuncAttributeMaxDynamicSharedMemorySize, C::kSmem);
+    if (e != cudaSuccess) return e;
+  }
+  for (int r = 0; r < a.rows; r += 65535 * C::kRows) {  // grid.y holds 65535 passes
+    LinearArgs b = a;
+    b.rows = std::min(a.rows - r, 65535 * C::kRows);
+    const size_t xb = type_bytes(a.in_dtype), yb = type_bytes(a.out_dtype);
+    b.x = static_cast<const char*>(a.x) + static_cast<size_t>(r) * a.x_stride * xb;
+    b.x_scale = a.x_scale ? a.x_scale + static_cast<size_t>(r) * (a.w.k / 32) : nullptr;
+    b.y = static_cast<char*>(a.y) + static_cast<size_t>(r) * a.y_stride * yb;
+    const dim3 grid((a.w.tiles + MT - 1) / MT, (b.rows + C::kRows - 1) / C::kRows);
+    const cudaError_t e =
+        launch_pdl(linear_q4_kernel<IN, NT, MT, G>, grid, dim3(kLinThreads), kern_smem, s, pdl, b);
+    if (e != cudaSuccess) return e;
+  }
+  return cudaSuccess;
+}
+
+template <int IN, int G>
+cudaError_t launch_linear_in(const LinearArgs& a, bool pdl, cudaStream_t s) {
+  const int columns = a.rows * (IN == QL_F32 ? 3 : 1);
+  int mt = columns <= 8 ? 1 : columns <= 16 ? 2 : 4;
+  if (const char* e = getenv("QLMT")) mt = atoi(e);
+  if (columns <= 8) return mt == 1 ? launch_linear_as<IN, 1, 1, G>(a, pdl, s) : launch_linear_as<IN, 1, 2, G>(a, pdl, s);
+  if (columns <= 16) return mt == 1 ? launch_linear_as<IN, 2, 1, G>(a, pdl, s) : mt == 2 ? launch_linear_as<IN, 2, 2, G>(a, pdl, s) : launch_linear_as<IN, 2, 4, G>(a, pdl, s);
+  return mt == 2 ? launch_linear_as<IN, 4, 2, G>(a, pdl, s) : launch_linear_as<IN, 4, 4, G>(a, pdl, s);
+}
+
+cudaError_t launch_linear(const LinearArgs& a, bool pdl, cudaStream_t s) {
+  auto by_group = [&](auto in) {
+    constexpr int IN = decltype(in)::value;
+    if (a.w.group == 32) return launch_linear_in<IN, 32>(a, pdl, s);
+    if (a.w.group == 64) return launch_linear_in<IN, 64>(a, pdl, s);
+    return launch_linear_in<IN, 128>(a, pdl, s);
+  };
+  switch (a.in_dtype) {
+    case QL_F32: return by_group(std::integral_constant<int, ql::kF32>());
+    case QL_F16: return by_group(std::integral_constant<int, ql::kF16>());
+    case QL_BF16: return by_group(std::integral_constant<int, ql::kBF16>());
+    default: return by_group(std::integral_constant<int, ql::kQ8_0>());
   }
 }
 
@@ -865,8 +1241,8 @@ int ql_linear_q4(ql_ctx* c, const ql_q4* w, const ql_linear_args* args) {
   a.rows = f.rows;
   a.in_dtype = f.in_dtype;
   a.out_dtype = f.out_dtype;
-  linear_q4_kernel<<<(w->n + 3) / 4, 128, 0, c->stream>>>(a);
-  QLN_CUDA(cudaGetLastError(), "launch the 4-bit product");
+  QLN_CUDA(launch_linear(a, !w->fresh, c->stream), "launch the 4-bit product");
+  w->fresh = false;
   return QL_OK;
 }
 
