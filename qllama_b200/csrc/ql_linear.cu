@@ -5,7 +5,6 @@
 
 #include <algorithm>
 #include <cmath>
-#include <cstdlib>
 #include <new>
 #include <type_traits>
 
@@ -608,47 +607,98 @@ struct LinearArgs {
 
 // ---- the tensor-core product ----
 // Formula: y[r][n] = sum over blocks of 32 columns of scale * (sum of (code - 8) x).
-// The weights' bytes (0.53-0.56 of them per weight) are the cost of a few rows, so
-// they stream straight from HBM into the registers of the lanes that multiply them,
-// 16 bytes a lane, with the next ones in flight while one set is multiplied.
-// A warp owns MT tiles of 16 weight rows and every 8th chunk of 64 columns; the
-// weights are the A operand (16 rows of W), x the B operand (8 columns), so one
-// row of x costs as much as eight.  Codes turn into f16 / bf16 exactly (a nibble
-// in the mantissa of 1024 or 128, less an offset), or into int8 (a two's-complement
-// nibble in the high half of a byte: 16 times its value).  Blocks of 32 sum on the
-// tensor cores in f32 (int32 for Q8_0: exact), are scaled in f32 and added to f32
-// sums.  f32 rows: three bf16 parts of 8 significand bits each carry a value's 24
-// exactly; the parts are three columns of B, whose sums are added at the end.
-// The split of the columns over the warps and every order of additions are the
-// same for all MT, NT and row counts, so a row's bits depend only on it and W.
-constexpr int kLinWarps = 8;
-constexpr int kLinThreads = 32 * kLinWarps;
+// The weights' bytes (0.52-0.56 of them per weight) are the cost of a few rows, so
+// each goes from HBM to the lane that multiplies it once, through a ring in shared
+// memory that every warp keeps for itself (cp.async, kD sets deep; a __syncwarp is
+// the only barrier of the loop).  Codes turn into f16 / bf16 exactly (a nibble in the
+// mantissa of 1024 or 128, less an offset), or into int8 (a two's-complement nibble in
+// the high half of a byte: 16 times its value).  The weights are the A operand (16
+// rows of W), x the B operand (8 columns), so one row of x costs as much as eight.
+// Blocks of 32 are summed on the tensor cores in f32 (int32 for Q8_0: exact), scaled
+// in f32 and added to f32 sums.  f32 rows: three bf16 parts of 8 significand bits
+// carry a value's 24 exactly; the parts are three columns of B, whose sums are added
+// at the end.
+// One CTA an SM, each with an equal share of W's row tiles (an even share matters
+// more than anything else: CTAs of a few tiles, several an SM, left a third of the
+// time to the last of them).  The columns are cut into 8 ranges, one for each warp of
+// a team; WR teams take every WR-th tile.  The loads of the next tiles are under way
+// while the ranges are joined, in order.  Every order of additions is the same for
+// all variants and row counts, so a row's bits depend only on it and W.
+constexpr int kRanges = 8;
 
-// D = A B (no addend)
-template <bool BF>
-__device__ __forceinline__ void mma16816_first(float (&d)[4], const uint32_t (&a)[4], uint32_t b0,
-                                               uint32_t b1) {
-  if constexpr (BF) {
-    asm volatile(
-        "mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, "
-        "{%8,%9}, {%10,%10,%10,%10};"
+// D = A B + C of one m16n8k16 (FIRST: D = A B).  Not volatile: the compiler
+// interleaves the independent products of a chunk, which hides their latency.
+template <bool BF, bool FIRST>
+__device__ __forceinline__ void mma_f(float (&d)[4], const uint32_t (&a)[4], uint32_t b0,
+                                      uint32_t b1) {
+  const float c0 = FIRST ? 0.f : d[0], c1 = FIRST ? 0.f : d[1], c2 = FIRST ? 0.f : d[2],
+              c3 = FIRST ? 0.f : d[3];
+  if constexpr (BF)
+    asm("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, "
+        "{%8,%9}, {%10,%11,%12,%13};"
         : "=f"(d[0]), "=f"(d[1]), "=f"(d[2]), "=f"(d[3])
-        : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1), "f"(0.f));
-  } else {
-    asm volatile(
-        "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, "
-        "{%8,%9}, {%10,%10,%10,%10};"
+        : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1), "f"(c0), "f"(c1), "f"(c2),
+          "f"(c3));
+  else
+    asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, "
+        "{%8,%9}, {%10,%11,%12,%13};"
         : "=f"(d[0]), "=f"(d[1]), "=f"(d[2]), "=f"(d[3])
-        : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1), "f"(0.f));
-  }
+        : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1), "f"(c0), "f"(c1), "f"(c2),
+          "f"(c3));
 }
 
-__device__ __forceinline__ uint4 ld_weights(const void* p) {
-  uint4 v;
-  asm volatile("ld.global.nc.L1::no_allocate.v4.u32 {%0,%1,%2,%3}, [%4];"
-               : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w)
-               : "l"(p));
-  return v;
+// Asynchronous copies of this lane's bytes into shared memory; the first `bytes`
+// of them are read, the rest are zeros.
+__device__ __forceinline__ void cp16_stream(uint32_t dst, const void* src, int bytes) {
+  asm volatile("cp.async.cg.shared.global.L2::128B [%0], [%1], 16, %2;" ::"r"(dst), "l"(src),
+               "r"(bytes)
+               : "memory");
+}
+template <int N>
+__device__ __forceinline__ void cp_cached(uint32_t dst, const void* src, int bytes) {
+  asm volatile("cp.async.ca.shared.global [%0], [%1], %2, %3;" ::"r"(dst), "l"(src), "n"(N),
+               "r"(bytes)
+               : "memory");
+}
+__device__ __forceinline__ void cp_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+template <int N>
+__device__ __forceinline__ void cp_wait() {
+  asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory");
+}
+template <int N>
+__device__ __forceinline__ void lds(uint32_t (&v)[N], uint32_t a) {
+  static_assert(N == 1 || N == 2 || N == 4, "one access");
+  if constexpr (N == 4)
+    asm volatile("ld.shared.v4.u32 {%0,%1,%2,%3}, [%4];"
+                 : "=r"(v[0]), "=r"(v[1]), "=r"(v[2]), "=r"(v[3])
+                 : "r"(a));
+  else if constexpr (N == 2)
+    asm volatile("ld.shared.v2.u32 {%0,%1}, [%2];" : "=r"(v[0]), "=r"(v[1]) : "r"(a));
+  else
+    asm volatile("ld.shared.u32 %0, [%1];" : "=r"(v[0]) : "r"(a));
+}
+// Two f32 operations in one instruction, each rounded as by itself.
+__device__ __forceinline__ uint64_t bits2(float2 v) {
+  return static_cast<uint64_t>(__float_as_uint(v.y)) << 32 | __float_as_uint(v.x);
+}
+__device__ __forceinline__ float2 pair2(uint64_t v) {
+  return make_float2(__uint_as_float(static_cast<uint32_t>(v)),
+                     __uint_as_float(static_cast<uint32_t>(v >> 32)));
+}
+__device__ __forceinline__ float2 add2(float2 a, float2 b) {
+  uint64_t d;
+  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(bits2(a)), "l"(bits2(b)));
+  return pair2(d);
+}
+__device__ __forceinline__ float2 mul2(float2 a, float2 b) {
+  uint64_t d;
+  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(bits2(a)), "l"(bits2(b)));
+  return pair2(d);
+}
+__device__ __forceinline__ float2 fma2(float2 a, float2 b, float2 c) {
+  uint64_t d;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(d) : "l"(bits2(a)), "l"(bits2(b)), "l"(bits2(c)));
+  return pair2(d);
 }
 
 // (a & b) ^ c
@@ -688,211 +738,232 @@ __device__ __forceinline__ void unpack_word(uint32_t w, uint32_t (&p)[4]) {
   }
 }
 
-template <int IN, int NT, int MT, int G>
+template <int IN, int NT, int MT, int WR, int G>
 struct LinCfg {
   static constexpr bool kQ8 = IN == ql::kQ8_0;
   static constexpr bool kBF = IN == ql::kBF16 || IN == ql::kF32;
   static constexpr int kParts = IN == ql::kF32 ? 3 : 1;
-  static constexpr int kRows = 8 * NT / kParts;  // rows of x in one pass
-  static constexpr int kU = MT >= 4 ? 1 : 4 / MT;  // chunks of one set
-  static constexpr int kXWords = kQ8 ? 2 : 4;      // words of a block of 32 in a lane
-  static constexpr int kPitch = 16 * MT + 4;
-  static constexpr int kSmem = kLinWarps * 8 * NT * kPitch * 4;
+  static constexpr int kTileRows = IN == ql::kF32 ? 2 : 8;  // rows of x in 8 columns of B
+  static constexpr int kRows = NT * kTileRows;              // and in one pass
+  static constexpr int kWarps = kRanges * WR, kThreads = 32 * kWarps;
+  static constexpr int kGroup = MT * WR;  // tiles that the CTA works on at a time
+  // one set of a warp: MT tiles of codes, their scales, 64 columns of x's rows
+  static constexpr int kScaleTile = G == 32 ? 64 : 32;
+  static constexpr int kXRow = kQ8 ? 64 : IN == ql::kF32 ? 256 : 128;
+  static constexpr int kScales = MT * 512;
+  static constexpr int kX = kScales + MT * kScaleTile;
+  static constexpr int kXScales = kX + kRows * kXRow;  // Q8_0: two f16 a row
+  static constexpr int kSet = kXScales + (kQ8 ? kRows * 4 : 0);
+  static constexpr int kPitch = 16 * kGroup + 4;  // of a column in the join
+  static constexpr int kJoin = 8 * kPitch * 4;    // a range's 8 columns
+  static constexpr int kRoom = 227 * 1024 - kRanges * kJoin;
+  static constexpr int kD = 4 * kWarps * kSet <= kRoom ? 4 : 3 * kWarps * kSet <= kRoom ? 3 : 2;
+  static constexpr int kRing = kWarps * kD * kSet;
+  static constexpr int kSmem = kRing + kRanges * kJoin;
 };
 
-// One set of loads: U chunks of MT tiles, with x.
-template <int IN, int NT, int MT, int G>
-struct LinSet {
-  using C = LinCfg<IN, NT, MT, G>;
-  uint4 w[C::kU][MT];
-  uint2 s[C::kU][MT];  // f16: rows g, g + 8 of block j in .x / .y; G >= 64: .x alone
-  uint32_t x[C::kU][NT][2][C::kXWords];
-  float sx[C::kQ8 ? C::kU : 1][C::kQ8 ? NT : 1][2][2];  // [block][column 2t, 2t + 1]
-};
-
-template <int IN, int NT, int MT, int G>
-__global__ void __launch_bounds__(kLinThreads) linear_q4_kernel(const LinearArgs a) {
-  using C = LinCfg<IN, NT, MT, G>;
-  extern __shared__ float red[];
+template <int IN, int NT, int MT, int WR, int G>
+__global__ void __launch_bounds__(kRanges* WR * 32, 1) linear_q4_kernel(const LinearArgs a) {
+  using C = LinCfg<IN, NT, MT, WR, G>;
+  extern __shared__ __align__(16) char smem[];
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
-  const int tile0 = blockIdx.x * MT;
+  const int range = warp % kRanges, team = warp / kRanges;
   const int r0 = blockIdx.y * C::kRows;
   const int rows = min(a.rows - r0, C::kRows);
-  const int chunks = a.w.chunks, steps = (chunks + kLinWarps - 1) / kLinWarps;
+  const int chunks = a.w.chunks, K = a.w.k;
+  // this CTA's tiles [t0, t1) and this warp's chunks [c0, c0 + nc)
+  const int t0 = static_cast<int>(static_cast<long long>(a.w.tiles) * blockIdx.x / gridDim.x);
+  const int t1 = static_cast<int>(static_cast<long long>(a.w.tiles) * (blockIdx.x + 1) / gridDim.x);
+  const int groups = (t1 - t0 + C::kGroup - 1) / C::kGroup;
+  const int c0 = static_cast<int>(static_cast<long long>(chunks) * range / kRanges);
+  const int nc = static_cast<int>(static_cast<long long>(chunks) * (range + 1) / kRanges) - c0;
 
-  using Set = LinSet<IN, NT, MT, G>;
-  auto load_w = [&](Set& z, int step) {
+  const uint32_t ring = ql::smem_u32(smem) + warp * C::kD * C::kSet;
+  const uint32_t join = ql::smem_u32(smem) + C::kRing;
+  // tiles of this team in a group: first, first + WR, ... below t1
+  auto live_tiles = [&](int group) {
+    const int left = t1 - (t0 + group * C::kGroup + team);
+    return left <= 0 ? 0 : min(MT, (left + WR - 1) / WR);
+  };
+  // ---- loads: where the next set's weights lie (advanced chunk by chunk)
+  const uint32_t wstep = static_cast<uint32_t>(WR) * chunks * 512u;  // tile to tile of the team
+  constexpr int kLanes = C::kScaleTile / 16;  // lanes that copy a tile's scales, 16 bytes each
+  const char* wp;
+  const char* sp;
+  int lg = 0, lc = c0, llive = 0;  // group and chunk of the next set
+  auto start_group = [&](int group) {
+    const size_t tile = t0 + group * C::kGroup + team;
+    wp = reinterpret_cast<const char*>(a.w.codes) + (tile * chunks + c0) * 512 + lane * 16;
+    sp = reinterpret_cast<const char*>(a.w.scales) +
+         scale_at(G, chunks, tile + lane / kLanes * WR, 0, 0, 0, 0) * 2 + lane % kLanes * 16;
+    llive = live_tiles(group);
+  };
+  start_group(0);
+  auto copy_w = [&](uint32_t set) {
 #pragma unroll
-    for (int u = 0; u < C::kU; ++u) {
-      const int chunk = (step + u) * kLinWarps + warp;
-      const bool ok = chunk < chunks;
+    for (int m = 0; m < MT; ++m)
+      if (m < llive) cp16_stream(set + m * 512 + lane * 16, wp + m * wstep, 16);
+    if (lane < llive * kLanes)
+      cp_cached<16>(set + C::kScales + lane * 16,
+                    sp + (G == 32 ? lc * 64 : G == 64 ? lc * 32 : (lc >> 1) * 32), 16);
+  };
+  auto next = [&]() {
+    wp += 512;
+    if (++lc == c0 + nc) {
+      lc = c0;
+      start_group(++lg);
+    }
+  };
+  // x: 16-byte units of a row's 64 columns, spread so that the lanes of a fragment
+  // read from different banks.  Rows past the call's are left as they are: their
+  // columns of the product are not stored.
+  constexpr int kBytes = IN == ql::kF32 ? 4 : C::kQ8 ? 1 : 2;
+  constexpr int kUnits = C::kXRow / 16;  // of a row: 4, 8 or 16
+  constexpr int kXU = (C::kRows * kUnits + 31) / 32;
+  const bool vec =
+      (reinterpret_cast<uintptr_t>(a.x) | static_cast<uintptr_t>(a.x_stride * kBytes)) % 16 == 0;
+  auto unit_at = [](int r, int u) {
+    if constexpr (C::kQ8) return r * C::kXRow + (u ^ (r & 2)) * 16;
+    else if constexpr (IN == ql::kF32) return r * C::kXRow + (u ^ (r & 1)) * 16;
+    else return r * C::kXRow + (u ^ (r & 1) * 4) * 16;
+  };
+  // this lane's units: column xcol of rows xr, xr + 32 / kUnits, ...
+  const int xr = lane / kUnits, xcol = lane % kUnits * (16 / kBytes);
+  const char* const xp = static_cast<const char*>(a.x) +
+                         (static_cast<size_t>(r0 + xr) * a.x_stride + xcol) * kBytes;
+  const size_t xstep = static_cast<size_t>(32 / kUnits) * a.x_stride * kBytes;
+  uint32_t xdst[kXU];
 #pragma unroll
-      for (int m = 0; m < MT; ++m) {
-        const size_t tile = min(tile0 + m, a.w.tiles - 1);  // past the end: not stored
-        z.w[u][m] = make_uint4(0, 0, 0, 0);
-        z.s[u][m] = make_uint2(0, 0);
-        if (ok) {
-          z.w[u][m] = ld_weights(a.w.codes + ((tile * chunks + chunk) * 32 + lane) * 4);
-          const __half* sp = a.w.scales + scale_at(G, chunks, tile, chunk, g, 0, 0);
-          if constexpr (G == 32) z.s[u][m] = __ldg(reinterpret_cast<const uint2*>(sp));
-          else z.s[u][m].x = __ldg(reinterpret_cast<const uint32_t*>(sp));
+  for (int i = 0; i < kXU; ++i) xdst[i] = C::kX + unit_at(xr + i * (32 / kUnits), lane % kUnits);
+  // Q8_0: the scales of x's row `lane`, two of a chunk at a time
+  const uint16_t* const xsp =
+      reinterpret_cast<const uint16_t*>(a.x_scale) + static_cast<size_t>(r0 + lane) * (K / 32);
+  const bool xs_vec = C::kQ8 && (reinterpret_cast<uintptr_t>(a.x_scale) | (K / 32 * 2)) % 4 == 0;
+  auto copy_x = [&](uint32_t set, int c) {
+    const int k = 64 * c + xcol;
+#pragma unroll
+    for (int i = 0; i < kXU; ++i) {
+      if (xr + i * (32 / kUnits) >= rows) continue;
+      const char* p = xp + i * xstep + c * (64 * kBytes);
+      if (vec) {
+        cp_cached<16>(set + xdst[i], k < K ? p : xp, k < K ? 16 : 0);
+      } else {
+        uint32_t v[4] = {0, 0, 0, 0};
+        if (k < K) {
+#pragma unroll
+          for (int e = 0; e < 16 / kBytes; ++e) {
+            if constexpr (IN == ql::kF32) v[e] = reinterpret_cast<const uint32_t*>(p)[e];
+            else if constexpr (C::kQ8)
+              v[e / 4] |= static_cast<uint32_t>(reinterpret_cast<const uint8_t*>(p)[e])
+                          << (8 * (e % 4));
+            else
+              v[e / 2] |= static_cast<uint32_t>(reinterpret_cast<const uint16_t*>(p)[e])
+                          << (16 * (e % 2));
+          }
+        }
+        asm volatile("st.shared.v4.u32 [%0], {%1,%2,%3,%4};" ::"r"(set + xdst[i]), "r"(v[0]),
+                     "r"(v[1]), "r"(v[2]), "r"(v[3])
+                     : "memory");
+      }
+    }
+    if constexpr (C::kQ8) {
+      if (lane < rows) {
+        if (xs_vec) {
+          cp_cached<4>(set + C::kXScales + lane * 4, xsp + 2 * c, 4);
+        } else {
+          const uint32_t v =
+              xsp[2 * c] | (64 * c + 32 < K ? static_cast<uint32_t>(xsp[2 * c + 1]) << 16 : 0u);
+          asm volatile("st.shared.u32 [%0], %1;" ::"r"(set + C::kXScales + lane * 4), "r"(v)
+                       : "memory");
         }
       }
     }
   };
-  // this lane's column of each B tile: a row of x (and a part of it)
-  const char* xrow[NT];
-  bool live[NT];
-  constexpr int kBytes = IN == ql::kF32 ? 4 : C::kQ8 ? 1 : 2;
-  const bool vec = (reinterpret_cast<uintptr_t>(a.x) | static_cast<uintptr_t>(a.x_stride * kBytes)) %
-                       (C::kQ8 ? 8 : 16) == 0;
-  uint32_t m1[NT], m2[NT];  // f32: the bits that parts 1 and 2 take off first
+  // ---- products
+  // f32: this lane's column is part g % 3 of row g / 3; the bits that parts 1 and 2
+  // take off first
+  const int part = g % 3;
+  const uint32_t m1 = part >= 1 ? 0xffff0000u : 0u, m2 = part == 2 ? 0xffff0000u : 0u;
+  // The fragment of block j in B tile q: eight values of this lane's column.
+  auto fragment = [&](uint32_t set, int q, int j, uint32_t (&o)[C::kQ8 ? 2 : 4]) {
+    if constexpr (IN == ql::kF32) {
+      const int r = 2 * q + min(g / 3, 1);
+      uint32_t f[2][4];
+      lds(f[0], set + C::kX + unit_at(r, 8 * j + 2 * t));
+      lds(f[1], set + C::kX + unit_at(r, 8 * j + 2 * t + 1));
 #pragma unroll
-  for (int n = 0; n < NT; ++n) {
-    const int col = 8 * n + g;
-    const int r = col / C::kParts, part = col % C::kParts;
-    live[n] = r < rows;
-    xrow[n] = static_cast<const char*>(a.x) +
-              static_cast<size_t>(r0 + (live[n] ? r : 0)) * a.x_stride * kBytes;
-    m1[n] = part >= 1 ? 0xffff0000u : 0u;
-    m2[n] = part == 2 ? 0xffff0000u : 0u;
-  }
-  auto load_x = [&](Set& z, int step) {
+      for (int h = 0; h < 2; ++h) {
 #pragma unroll
-    for (int u = 0; u < C::kU; ++u) {
-      const int chunk = (step + u) * kLinWarps + warp;
+        for (int e = 0; e < 4; ++e) {
+          float v = __uint_as_float(f[h][e]);
+          v -= __uint_as_float(__float_as_uint(v) & m1);
+          v -= __uint_as_float(__float_as_uint(v) & m2);
+          f[h][e] = __float_as_uint(v);
+        }
+        o[2 * h] = __byte_perm(f[h][0], f[h][1], 0x7632);
+        o[2 * h + 1] = __byte_perm(f[h][2], f[h][3], 0x7632);
+      }
+    } else if constexpr (C::kQ8) {
+      lds(o, set + C::kX + unit_at(8 * q + g, 2 * j + t / 2) + t % 2 * 8);
+      o[0] = __byte_perm(o[0], 0, 0x3120);  // the order of the codes' bytes
+      o[1] = __byte_perm(o[1], 0, 0x3120);
+    } else {
+      lds(o, set + C::kX + unit_at(8 * q + g, 4 * j + t));
+    }
+  };
+  float2 acc[MT][NT][2];  // [rows g, g + 8]: columns 2t, 2t + 1
+  uint32_t x[NT][2][C::kQ8 ? 2 : 4];
+  float2 xs[C::kQ8 ? NT : 1][2];  // Q8_0: [block], of columns 2t, 2t + 1
+  auto product = [&](uint32_t set, int m) {
+    uint32_t w[4], sr[G == 32 ? 2 : 1];
+    lds(w, set + m * 512 + lane * 16);
+    lds(sr, set + C::kScales + m * C::kScaleTile + g * (C::kScaleTile / 8));
+    float2 s[2];  // rows g, g + 8
+    s[0] = __half22float2(*reinterpret_cast<const __half2*>(&sr[0]));
+    s[1] = __half22float2(*reinterpret_cast<const __half2*>(&sr[G == 32 ? 1 : 0]));
+    if constexpr (C::kQ8) {
 #pragma unroll
       for (int j = 0; j < 2; ++j) {
-        const int k = 64 * chunk + 32 * j;
-        const bool ok = k < a.w.k;
+        const uint4 A = make_uint4((w[2 * j] << 4) & 0xf0f0f0f0u, (w[2 * j + 1] << 4) & 0xf0f0f0f0u,
+                                   w[2 * j] & 0xf0f0f0f0u, w[2 * j + 1] & 0xf0f0f0f0u);
 #pragma unroll
-        for (int n = 0; n < NT; ++n) {
-          uint32_t(&o)[C::kXWords] = z.x[u][n][j];
+        for (int q = 0; q < NT; ++q) {
+          // sums start at the bits of 1.5 * 2^23: below 2^22 they are the
+          // mantissa of a float, and a subtraction converts them
+          int d[4] = {0x4b400000, 0x4b400000, 0x4b400000, 0x4b400000};
+          ql::mma16832_s8(d, A, x[q][j][0], x[q][j][1]);
 #pragma unroll
-          for (int i = 0; i < C::kXWords; ++i) o[i] = 0;
-          if (ok && live[n]) {
-            const char* p = xrow[n] + static_cast<size_t>(k + 8 * t) * kBytes;
-            if constexpr (C::kQ8) {
-              if (vec) {
-                const uint2 v = *reinterpret_cast<const uint2*>(p);
-                o[0] = v.x;
-                o[1] = v.y;
-              } else {
-#pragma unroll
-                for (int e = 0; e < 8; ++e)
-                  o[e / 4] |= static_cast<uint32_t>(reinterpret_cast<const uint8_t*>(p)[e])
-                              << (8 * (e % 4));
-              }
-            } else if constexpr (IN == ql::kF32) {
-              uint32_t f[8];
-              if (vec) {
-                const uint4 v = reinterpret_cast<const uint4*>(p)[0];
-                const uint4 q = reinterpret_cast<const uint4*>(p)[1];
-                f[0] = v.x; f[1] = v.y; f[2] = v.z; f[3] = v.w;
-                f[4] = q.x; f[5] = q.y; f[6] = q.z; f[7] = q.w;
-              } else {
-#pragma unroll
-                for (int e = 0; e < 8; ++e) f[e] = reinterpret_cast<const uint32_t*>(p)[e];
-              }
-#pragma unroll
-              for (int e = 0; e < 8; ++e) {
-                float v = __uint_as_float(f[e]);
-                v -= __uint_as_float(__float_as_uint(v) & m1[n]);
-                v -= __uint_as_float(__float_as_uint(v) & m2[n]);
-                f[e] = __float_as_uint(v);
-              }
-#pragma unroll
-              for (int i = 0; i < 4; ++i) o[i] = __byte_perm(f[2 * i], f[2 * i + 1], 0x7632);
-            } else {
-              if (vec) {
-                const uint4 v = *reinterpret_cast<const uint4*>(p);
-                o[0] = v.x; o[1] = v.y; o[2] = v.z; o[3] = v.w;
-              } else {
-#pragma unroll
-                for (int e = 0; e < 8; ++e)
-                  o[e / 2] |= static_cast<uint32_t>(reinterpret_cast<const uint16_t*>(p)[e])
-                              << (16 * (e % 2));
-              }
-            }
-          }
-          if constexpr (C::kQ8) {
-#pragma unroll
-            for (int c = 0; c < 2; ++c) {
-              const int r = 8 * n + 2 * t + c;
-              z.sx[u][n][j][c] = 0.f;
-              if (ok && r < rows)  // 1/16: the codes are 16 times their values
-                z.sx[u][n][j][c] =
-                    0.0625f * __half2float(a.x_scale[static_cast<size_t>(r0 + r) * (a.w.k / 32) +
-                                                     k / 32]);
-            }
+          for (int h = 0; h < 2; ++h) {
+            const float sh = h ? s[j].y : s[j].x;
+            const float2 f = add2(make_float2(__int_as_float(d[2 * h]), __int_as_float(d[2 * h + 1])),
+                                  make_float2(-12582912.0f, -12582912.0f));
+            acc[m][q][h] = fma2(f, mul2(make_float2(sh, sh), xs[q][j]), acc[m][q][h]);
           }
         }
       }
-    }
-  };
-
-  float acc[MT][NT][4];
+    } else {
+      float d[NT][4];
 #pragma unroll
-  for (int m = 0; m < MT; ++m)
+      for (int j = 0; j < 2; ++j) {
+        uint32_t lo[4], hi[4];  // rows g and g + 8
+        unpack_word<C::kBF>(w[2 * j], lo);
+        unpack_word<C::kBF>(w[2 * j + 1], hi);
+        const uint32_t A0[4] = {lo[0], hi[0], lo[1], hi[1]};
+        const uint32_t A1[4] = {lo[2], hi[2], lo[3], hi[3]};
 #pragma unroll
-    for (int n = 0; n < NT; ++n)
+        for (int q = 0; q < NT; ++q) {
+          if (G == 32 || j == 0) mma_f<C::kBF, true>(d[q], A0, x[q][j][0], x[q][j][1]);
+          else mma_f<C::kBF, false>(d[q], A0, x[q][j][0], x[q][j][1]);
+        }
 #pragma unroll
-      for (int i = 0; i < 4; ++i) acc[m][n][i] = 0.f;
-
-  auto multiply = [&](const Set& z) {
+        for (int q = 0; q < NT; ++q) mma_f<C::kBF, false>(d[q], A1, x[q][j][2], x[q][j][3]);
+        if (G == 32 || j == 1) {
 #pragma unroll
-    for (int u = 0; u < C::kU; ++u) {
-#pragma unroll
-      for (int m = 0; m < MT; ++m) {
-        const uint32_t w[4] = {z.w[u][m].x, z.w[u][m].y, z.w[u][m].z, z.w[u][m].w};
-        if constexpr (C::kQ8) {
-#pragma unroll
-          for (int j = 0; j < 2; ++j) {
-            const uint32_t sw = G == 32 && j == 1 ? z.s[u][m].y : z.s[u][m].x;
-            const float2 s = __half22float2(*reinterpret_cast<const __half2*>(&sw));
-            const uint4 A = make_uint4((w[2 * j] << 4) & 0xf0f0f0f0u, (w[2 * j + 1] << 4) & 0xf0f0f0f0u,
-                                       w[2 * j] & 0xf0f0f0f0u, w[2 * j + 1] & 0xf0f0f0f0u);
-#pragma unroll
-            for (int n = 0; n < NT; ++n) {
-              // sums start at the bits of 1.5 * 2^23: below 2^22 they are the
-              // mantissa of a float, and a subtraction converts them
-              int d[4] = {0x4b400000, 0x4b400000, 0x4b400000, 0x4b400000};
-              ql::mma16832_s8(d, A, __byte_perm(z.x[u][n][j][0], 0, 0x3120),
-                              __byte_perm(z.x[u][n][j][1], 0, 0x3120));
-#pragma unroll
-              for (int i = 0; i < 4; ++i)
-                acc[m][n][i] = fmaf(__int_as_float(d[i]) - 12582912.0f,
-                                    (i < 2 ? s.x : s.y) * z.sx[u][n][j][i & 1], acc[m][n][i]);
-            }
-          }
-        } else {
-          uint32_t lo[2][4], hi[2][4];  // rows g and g + 8 of both blocks
-#pragma unroll
-          for (int j = 0; j < 2; ++j) {
-            unpack_word<C::kBF>(w[2 * j], lo[j]);
-            unpack_word<C::kBF>(w[2 * j + 1], hi[j]);
-          }
-#pragma unroll
-          for (int n = 0; n < NT; ++n) {
-            float d[4];
-#pragma unroll
-            for (int j = 0; j < 2; ++j) {
-              const uint32_t A0[4] = {lo[j][0], hi[j][0], lo[j][1], hi[j][1]};
-              const uint32_t A1[4] = {lo[j][2], hi[j][2], lo[j][3], hi[j][3]};
-              if (G == 32 || j == 0)
-                mma16816_first<C::kBF>(d, A0, z.x[u][n][j][0], z.x[u][n][j][1]);
-              else
-                ql::mma16816<C::kBF>(d, A0, z.x[u][n][j][0], z.x[u][n][j][1]);
-              ql::mma16816<C::kBF>(d, A1, z.x[u][n][j][2], z.x[u][n][j][3]);
-              if (G == 32 || j == 1) {
-                const uint32_t sw = G == 32 && j == 1 ? z.s[u][m].y : z.s[u][m].x;
-                const float2 s = __half22float2(*reinterpret_cast<const __half2*>(&sw));
-                acc[m][n][0] = fmaf(d[0], s.x, acc[m][n][0]);
-                acc[m][n][1] = fmaf(d[1], s.x, acc[m][n][1]);
-                acc[m][n][2] = fmaf(d[2], s.y, acc[m][n][2]);
-                acc[m][n][3] = fmaf(d[3], s.y, acc[m][n][3]);
-              }
-            }
+          for (int q = 0; q < NT; ++q) {
+            acc[m][q][0] =
+                fma2(make_float2(d[q][0], d[q][1]), make_float2(s[j].x, s[j].x), acc[m][q][0]);
+            acc[m][q][1] =
+                fma2(make_float2(d[q][2], d[q][3]), make_float2(s[j].y, s[j].y), acc[m][q][1]);
           }
         }
       }
@@ -901,93 +972,157 @@ __global__ void __launch_bounds__(kLinThreads) linear_q4_kernel(const LinearArgs
 
   // The first weights do not depend on the kernel before this one (a product
   // after a write of the weights is launched without the overlap).
-  Set z0, z1;
-  load_w(z0, 0);
+  const int total = groups * nc;
+#pragma unroll
+  for (int i = 0; i < C::kD - 1; ++i)
+    if (i < total) {
+      copy_w(ring + i * C::kSet);
+      next();
+    }
   ql::griddep_wait();
   ql::griddep_launch_dependents();
-  load_x(z0, 0);
-  for (int step = 0; step < steps; step += 2 * C::kU) {
-    if (step + C::kU < steps) {
-      load_w(z1, step + C::kU);
-      load_x(z1, step + C::kU);
-    }
-    multiply(z0);
-    if (step + C::kU >= steps) break;
-    if (step + 2 * C::kU < steps) {
-      load_w(z0, step + 2 * C::kU);
-      load_x(z0, step + 2 * C::kU);
-    }
-    multiply(z1);
+#pragma unroll
+  for (int i = 0; i < C::kD - 1; ++i) {
+    if (i < total) copy_x(ring + i * C::kSet, c0 + i % nc);
+    cp_commit();
   }
-
-  // join the warps: red[warp][column][row]
-  float* mine = red + static_cast<size_t>(warp) * 8 * NT * C::kPitch;
+  uint32_t set = ring, load_set = ring + (C::kD - 1) * C::kSet;
+  const uint32_t ring_end = ring + C::kD * C::kSet;
+  int to_load = total - (C::kD - 1);
+  for (int group = 0; group < groups; ++group) {
+    const int live = live_tiles(group);
 #pragma unroll
-  for (int m = 0; m < MT; ++m)
+    for (int m = 0; m < MT; ++m)
 #pragma unroll
-    for (int n = 0; n < NT; ++n)
+      for (int q = 0; q < NT; ++q) acc[m][q][0] = acc[m][q][1] = make_float2(0.f, 0.f);
+    for (int i = 0; i < nc; ++i) {
+      cp_wait<C::kD - 2>();
+      __syncwarp();  // the set has arrived for every lane, and the one before is read
+      if (to_load > 0) {
+        copy_w(load_set);
+        copy_x(load_set, lc);
+        next();
+      }
+      --to_load;
+      cp_commit();
+      load_set = load_set + C::kSet == ring_end ? ring : load_set + C::kSet;
 #pragma unroll
-      for (int i = 0; i < 4; ++i)
-        mine[(8 * n + 2 * t + (i & 1)) * C::kPitch + 16 * m + g + 8 * (i >> 1)] = acc[m][n][i];
-  __syncthreads();
-  for (int i = threadIdx.x; i < 16 * MT * rows; i += kLinThreads) {
-    const int row = i % (16 * MT), r = i / (16 * MT);
-    const int n = tile0 * 16 + row;
-    if (n >= a.w.n) continue;
-    float y = 0.f;
+      for (int q = 0; q < NT; ++q)
 #pragma unroll
-    for (int p = C::kParts - 1; p >= 0; --p) {  // the small parts first
-      float v = 0.f;
+        for (int j = 0; j < 2; ++j) fragment(set, q, j, x[q][j]);
+      if constexpr (C::kQ8) {
 #pragma unroll
-      for (int w = 0; w < kLinWarps; ++w)
-        v += red[(static_cast<size_t>(w) * 8 * NT + r * C::kParts + p) * C::kPitch + row];
-      y += v;
+        for (int q = 0; q < NT; ++q) {
+          uint32_t v[2];  // rows 8q + 2t and the next
+          lds(v, set + C::kXScales + (8 * q + 2 * t) * 4);
+          const float2 even = __half22float2(*reinterpret_cast<const __half2*>(&v[0]));
+          const float2 odd = __half22float2(*reinterpret_cast<const __half2*>(&v[1]));
+          xs[q][0] = make_float2(even.x, odd.x);
+          xs[q][1] = make_float2(even.y, odd.y);
+        }
+      }
+      if (live == MT) {
+#pragma unroll
+        for (int m = 0; m < MT; ++m) product(set, m);
+      } else {
+#pragma unroll
+        for (int m = 0; m < MT - 1; ++m)
+          if (m < live) product(set, m);
+      }
+      set = set + C::kSet == ring_end ? ring : set + C::kSet;
     }
-    ql::store_elem(a.y, static_cast<size_t>(r0 + r) * a.y_stride + n, a.out_dtype, y);
+    // Join the ranges, eight columns of B at a time: [range][column][row].
+    const int n0 = (t0 + group * C::kGroup) * 16;
+    const int n1 = min(min(C::kGroup * 16, t1 * 16 - n0), a.w.n - n0);
+#pragma unroll
+    for (int q = 0; q < NT; ++q) {
+      if (q * C::kTileRows >= rows) break;
+      if (group > 0 || q > 0) __syncthreads();  // the sums before have been read
+#pragma unroll
+      for (int m = 0; m < MT; ++m) {
+        if (m >= live) continue;
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+          asm volatile("st.shared.f32 [%0], %1;" ::"r"(
+                           join + range * C::kJoin +
+                           ((2 * t + (i & 1)) * C::kPitch + 16 * (m * WR + team) + g +
+                            8 * (i >> 1)) * 4),
+                       "f"(i & 1 ? acc[m][q][i >> 1].y : acc[m][q][i >> 1].x)
+                       : "memory");
+      }
+      __syncthreads();
+      const int left = min(C::kTileRows, rows - q * C::kTileRows);
+      for (int i = threadIdx.x; i < 16 * C::kGroup * left; i += C::kThreads) {
+        const int row = i % (16 * C::kGroup), r = i / (16 * C::kGroup);
+        if (row >= n1) continue;
+        float y = 0.f;
+#pragma unroll
+        for (int p = C::kParts - 1; p >= 0; --p) {  // the small parts first
+          float v = 0.f;
+#pragma unroll
+          for (int w = 0; w < kRanges; ++w) {
+            float z;
+            asm volatile("ld.shared.f32 %0, [%1];"
+                         : "=f"(z)
+                         : "r"(join + w * C::kJoin + ((r * C::kParts + p) * C::kPitch + row) * 4)
+                         : "memory");
+            v += z;
+          }
+          y += v;
+        }
+        if (C::kQ8) y *= 0.0625f;  // the codes were 16 times their values
+        ql::store_elem(a.y, static_cast<size_t>(r0 + q * C::kTileRows + r) * a.y_stride + n0 + row,
+                       a.out_dtype, y);
+      }
+    }
   }
 }
 
-template <int IN, int NT, int MT, int G>
-cudaError_t launch_linear_as(const LinearArgs& a, bool pdl, cudaStream_t s) {
-  using C = LinCfg<IN, NT, MT, G>;
-  const int kern_smem = C::kSmem;
-  if constexpr (C::kSmem > 48 * 1024) {
-    const cudaError_t e =
-        cudaFuncSetAttribute(linear_q4_kernel<IN, NT, MT, G>,
-                             cudaFuncAttributeMaxDynamicSharedMemorySize, C::kSmem);
-    if (e != cudaSuccess) return e;
-  }
-  for (int r = 0; r < a.rows; r += 65535 * C::kRows) {  // grid.y holds 65535 passes
+template <int IN, int NT, int MT, int WR, int G>
+cudaError_t launch_linear_as(const LinearArgs& a, int num_sms, bool pdl, cudaStream_t s) {
+  using C = LinCfg<IN, NT, MT, WR, G>;
+  static_assert(C::kSmem <= 227 * 1024, "shared memory");
+  auto* const kernel = linear_q4_kernel<IN, NT, MT, WR, G>;
+  cudaError_t e =
+      cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, C::kSmem);
+  for (int r = 0; e == cudaSuccess && r < a.rows; r += 65535 * C::kRows) {  // grid.y's limit
     LinearArgs b = a;
     b.rows = std::min(a.rows - r, 65535 * C::kRows);
     const size_t xb = type_bytes(a.in_dtype), yb = type_bytes(a.out_dtype);
     b.x = static_cast<const char*>(a.x) + static_cast<size_t>(r) * a.x_stride * xb;
     b.x_scale = a.x_scale ? a.x_scale + static_cast<size_t>(r) * (a.w.k / 32) : nullptr;
     b.y = static_cast<char*>(a.y) + static_cast<size_t>(r) * a.y_stride * yb;
-    const dim3 grid((a.w.tiles + MT - 1) / MT, (b.rows + C::kRows - 1) / C::kRows);
-    const cudaError_t e =
-        launch_pdl(linear_q4_kernel<IN, NT, MT, G>, grid, dim3(kLinThreads), kern_smem, s, pdl, b);
-    if (e != cudaSuccess) return e;
+    const dim3 grid(std::min(num_sms, a.w.tiles), (b.rows + C::kRows - 1) / C::kRows);
+    e = launch_pdl(kernel, grid, dim3(C::kThreads), C::kSmem, s, pdl, b);
   }
-  return cudaSuccess;
+  return e;
 }
 
+// B tiles by the rows of x.  Two teams of warps (16 warps hide more latency: 1 x 8192 ->
+// 57344 f16 55 us, 59 us with one) unless the SMs have no second tile for the second
+// team (1 x 2048 -> 2048 Q8_0 2.8 us with one team, 3.2 us with two).  With four B
+// tiles the sums fill the registers of one team, eight tiles at a time where a CTA has
+// that many.
 template <int IN, int G>
-cudaError_t launch_linear_in(const LinearArgs& a, bool pdl, cudaStream_t s) {
-  const int columns = a.rows * (IN == QL_F32 ? 3 : 1);
-  int mt = columns <= 8 ? 1 : columns <= 16 ? 2 : 4;
-  if (const char* e = getenv("QLMT")) mt = atoi(e);
-  if (columns <= 8) return mt == 1 ? launch_linear_as<IN, 1, 1, G>(a, pdl, s) : launch_linear_as<IN, 1, 2, G>(a, pdl, s);
-  if (columns <= 16) return mt == 1 ? launch_linear_as<IN, 2, 1, G>(a, pdl, s) : mt == 2 ? launch_linear_as<IN, 2, 2, G>(a, pdl, s) : launch_linear_as<IN, 2, 4, G>(a, pdl, s);
-  return mt == 2 ? launch_linear_as<IN, 4, 2, G>(a, pdl, s) : launch_linear_as<IN, 4, 4, G>(a, pdl, s);
+cudaError_t launch_linear_in(const LinearArgs& a, int num_sms, bool pdl, cudaStream_t s) {
+  const int b = (a.rows - 1) / LinCfg<IN, 1, 1, 1, G>::kTileRows + 1;
+  if (b > 2)
+    return a.w.tiles <= 4 * num_sms ? launch_linear_as<IN, 4, 4, 1, G>(a, num_sms, pdl, s)
+                                    : launch_linear_as<IN, 4, 8, 1, G>(a, num_sms, pdl, s);
+  const bool one = a.w.tiles <= num_sms;
+  if (b == 1)
+    return one ? launch_linear_as<IN, 1, 1, 1, G>(a, num_sms, pdl, s)
+               : launch_linear_as<IN, 1, 4, 2, G>(a, num_sms, pdl, s);
+  return one ? launch_linear_as<IN, 2, 1, 1, G>(a, num_sms, pdl, s)
+             : launch_linear_as<IN, 2, 4, 2, G>(a, num_sms, pdl, s);
 }
 
-cudaError_t launch_linear(const LinearArgs& a, bool pdl, cudaStream_t s) {
+cudaError_t launch_linear(const LinearArgs& a, int num_sms, bool pdl, cudaStream_t s) {
   auto by_group = [&](auto in) {
     constexpr int IN = decltype(in)::value;
-    if (a.w.group == 32) return launch_linear_in<IN, 32>(a, pdl, s);
-    if (a.w.group == 64) return launch_linear_in<IN, 64>(a, pdl, s);
-    return launch_linear_in<IN, 128>(a, pdl, s);
+    if (a.w.group == 32) return launch_linear_in<IN, 32>(a, num_sms, pdl, s);
+    if (a.w.group == 64) return launch_linear_in<IN, 64>(a, num_sms, pdl, s);
+    return launch_linear_in<IN, 128>(a, num_sms, pdl, s);
   };
   switch (a.in_dtype) {
     case QL_F32: return by_group(std::integral_constant<int, ql::kF32>());
@@ -1241,7 +1376,7 @@ int ql_linear_q4(ql_ctx* c, const ql_q4* w, const ql_linear_args* args) {
   a.rows = f.rows;
   a.in_dtype = f.in_dtype;
   a.out_dtype = f.out_dtype;
-  QLN_CUDA(launch_linear(a, !w->fresh, c->stream), "launch the 4-bit product");
+  QLN_CUDA(launch_linear(a, c->num_sms, !w->fresh, c->stream), "launch the 4-bit product");
   w->fresh = false;
   return QL_OK;
 }
