@@ -275,7 +275,8 @@ int ql_llama_quantize(ql_llama* m, int32_t group);
  * A row that is reached and holds a NaN or +inf, or has no positive
  * probability, or a drafted id outside the vocabulary ends the sequence: its
  * new token is -1 and the context's status is raised (QL_ERR_DEVICE at the next
- * synchronize).  ql_kv_truncate then drops the rejected drafts' cache rows.
+ * synchronize).  (Of probabilities, an accepted draft's rows are read at its id
+ * alone.)  ql_kv_truncate then drops the rejected drafts' cache rows.
  * Device pointers, aligned to their element size. */
 #define QL_VERIFY_LOGITS 0
 #define QL_VERIFY_PROBS 1

@@ -2,6 +2,7 @@
 // sampling's acceptance and the draw of the next token, beside ql_sample.
 #include <cuda_runtime.h>
 
+#include <climits>
 #include <cmath>
 
 #include "../../include/qllama_model.h"
@@ -31,173 +32,546 @@ struct VerifyArgs {
   double inv_t;  // 1 / temperature; 0: greedy
 };
 
+// One cluster of CTAs per sequence, each CTA with its share of every row.
+//   1. f32 (maximum, sum of exponentials) of all of the sequence's rows at once --
+//      the one pass over the logits, bound by their bytes -- joined over the cluster
+//      through distributed shared memory.  (Greedy: largest logit and its id.)
+//   2. Every draft is decided from its two logits and those sums.  A decision whose
+//      two sides are within 2^-14 of each other, far more than the f32 sums' error, is
+//      taken again from f64 sums of its rows.
+//   3. The rows at the first rejection (or the last row) are summed again in f64: the
+//      draw compares running sums over the whole vocabulary with a threshold, where an
+//      error of 1e-7 would change one token in some thousands.  The CTA, the warp and
+//      the lane where the running sum of the draw passes the threshold are found in
+//      turn.
+// All CTAs compute the same decisions from the same numbers, so the cluster's
+// barriers are met by all.  Nothing is kept outside shared memory.
 constexpr int kVerifyThreads = 512;
+constexpr int kVerifyWarps = kVerifyThreads / 32;
+constexpr int kVerifyRows = 2 * QL_VERIFY_MAX_DRAFTS + 1;
+constexpr int kMaxCluster = 16;
 
-__device__ double vsum(double v, double* red) {
-  for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
-  __syncthreads();
-  if ((threadIdx.x & 31) == 0) red[threadIdx.x >> 5] = v;
-  __syncthreads();
-  double t = 0;
-  for (int i = 0; i < static_cast<int>(blockDim.x >> 5); ++i) t += red[i];
-  return t;
+__device__ __forceinline__ uint32_t cluster_rank() {
+  uint32_t r;
+  asm("mov.u32 %0, %%cluster_ctarank;" : "=r"(r));
+  return r;
+}
+__device__ __forceinline__ uint32_t cluster_size() {
+  uint32_t r;
+  asm("mov.u32 %0, %%cluster_nctarank;" : "=r"(r));
+  return r;
+}
+__device__ __forceinline__ void cluster_sync() {
+  asm volatile("barrier.cluster.arrive.release;" ::: "memory");
+  asm volatile("barrier.cluster.wait.acquire;" ::: "memory");
+}
+__device__ __forceinline__ float2 ld_cluster_f2(const void* p, uint32_t rank) {
+  float2 v;
+  asm volatile("ld.shared::cluster.v2.f32 {%0, %1}, [%2];"
+               : "=f"(v.x), "=f"(v.y)
+               : "r"(ql::mapa_shared(ql::smem_u32(p), rank))
+               : "memory");
+  return v;
+}
+__device__ __forceinline__ double ld_cluster_f64(const void* p, uint32_t rank) {
+  double v;
+  asm volatile("ld.shared::cluster.f64 %0, [%1];"
+               : "=d"(v)
+               : "r"(ql::mapa_shared(ql::smem_u32(p), rank))
+               : "memory");
+  return v;
+}
+__device__ __forceinline__ float exp2_fast(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
 }
 
-__device__ float vmax(float v, float* red) {
-  for (int o = 16; o > 0; o >>= 1) v = fmaxf(v, __shfl_xor_sync(0xffffffffu, v, o));
-  __syncthreads();
-  if ((threadIdx.x & 31) == 0) red[threadIdx.x >> 5] = v;
-  __syncthreads();
-  float t = red[0];
-  for (int i = 1; i < static_cast<int>(blockDim.x >> 5); ++i) t = fmaxf(t, red[i]);
-  return t;
-}
-
-// One row as a distribution: value(i) is its unnormalised weight, z the sum.
-struct Row {
-  const void* base;
-  size_t at;
-  int dtype;
-  bool probs;
-  float m;
-  double inv_t, z;
-  __device__ float raw(int i) const { return ql::load_elem(base, at + i, dtype); }
-  __device__ double value(int i) const {
-    const float x = raw(i);
-    return probs ? x : exp((static_cast<double>(x) - m) * inv_t);
+// exp(d / T) in f64 for d <= 0 by the table method (P. T. P. Tang, 1989):
+// d / T = (k + r) ln2 / 32 with |r| <= 1/2, k = 32 e + j; the result is
+// 2^e 2^(j/32) exp(r ln2 / 32), the last by five terms of its series (the sixth is
+// below 3e-15).  Lane j holds 2^(j/32), read by shuffles: whole warps call this.
+struct Exp64 {
+  double table, scale, least;
+  __device__ explicit Exp64(double inv_t) {
+    constexpr double ln2 = 0.693147180559945309417232;
+    table = exp2(static_cast<double>(threadIdx.x & 31) / 32.0);
+    scale = inv_t * (32.0 / ln2);
+    least = -690.0 / inv_t;  // below it the result is taken as 0 (it is under 1e-299)
+  }
+  __device__ __forceinline__ double operator()(double d) const {
+    constexpr double L = 0.693147180559945309417232 / 32.0;
+    constexpr double magic = 6755399441055744.0;  // 1.5 * 2^52
+    const bool in = d >= least;
+    if (!in) d = 0.0;
+    const double t = fma(d, scale, magic);
+    const int k = __double2loint(t);
+    const double r = fma(d, scale, magic - t);
+    double p = fma(r, L * L * L * L * L / 120, L * L * L * L / 24);
+    p = fma(p, r, L * L * L / 6);
+    p = fma(p, r, L * L / 2);
+    p = fma(p, r, L);
+    p = fma(p, r, 1.0);
+    const int hi = __shfl_sync(0xffffffffu, __double2hiint(table), k & 31) + ((k >> 5) << 20);
+    const int lo = __shfl_sync(0xffffffffu, __double2loint(table), k & 31);
+    return in ? p * __hiloint2double(hi, lo) : 0.0;
   }
 };
 
-// One CTA per sequence.
-__global__ void __launch_bounds__(kVerifyThreads) verify_kernel(const VerifyArgs a) {
-  __shared__ double red[kVerifyThreads / 32];
-  __shared__ double part[kVerifyThreads];
-  __shared__ float redf[kVerifyThreads / 32];
-  __shared__ int found_s;
-  const int b = blockIdx.x, V = a.vocab, tid = threadIdx.x;
-  const int n = a.n_draft ? min(max(a.n_draft[b], 0), a.drafts) : a.drafts;
-  int32_t* tok = a.tokens + static_cast<size_t>(b) * (a.drafts + 1);
-  const int32_t* ids = a.ids + static_cast<size_t>(b) * a.drafts;
-  const double* u = a.uniforms ? a.uniforms + static_cast<size_t>(b) * (a.drafts + 1) : nullptr;
-  for (int i = tid; i <= a.drafts; i += kVerifyThreads) tok[i] = -1;
-  __syncthreads();
-  auto open = [&](const void* base, size_t row, int64_t stride, bool& bad) {
-    Row r{base, row * static_cast<size_t>(stride), a.dtype, a.probs != 0, 0.f, a.inv_t, 1.0};
-    float m = -INFINITY;
-    int wrong = 0;
-    for (int i = tid; i < V; i += kVerifyThreads) {
-      const float x = r.raw(i);
-      wrong |= !(x < INFINITY);
-      m = fmaxf(m, x);
-    }
-    wrong = __syncthreads_or(wrong);
-    r.m = vmax(m, redf);
-    bad = wrong || (a.probs ? !(r.m > 0.f) : r.m == -INFINITY);
-    if (!a.probs && !bad && a.inv_t > 0) {
-      double s = 0;
-      for (int i = tid; i < V; i += kVerifyThreads) s += r.value(i);
-      r.z = vsum(s, red);
-    }
-    return r;
-  };
-  int pos = 0;
-  bool bad = false, rejected = false;
-  Row p{}, q{};
-  for (;; ++pos) {
-    p = open(a.target, static_cast<size_t>(b) * (a.drafts + 1) + pos, a.target_stride, bad);
-    if (bad || pos == n) break;
-    const int x = ids[pos];
-    bad = x < 0 || x >= V;
-    if (bad) break;
-    if (a.inv_t == 0) {
-      if (tid == 0) found_s = V;
-      __syncthreads();
-      for (int i = tid; i < V; i += kVerifyThreads)
-        if (p.raw(i) == p.m) {
-          atomicMin(&found_s, i);
-          break;
+// A row's 16-byte groups: element e of the row is element (e + shift) of the groups.
+template <int DT>
+struct Groups {
+  static constexpr int kN = DT == ql::kF32 ? 4 : 8;
+  const uint4* base;
+  int shift, count;
+  __device__ Groups(const void* p, size_t at, int vocab) {
+    const uintptr_t a = reinterpret_cast<uintptr_t>(p) + at * (16 / kN);
+    shift = static_cast<int>(a % 16) / (16 / kN);
+    base = reinterpret_cast<const uint4*>(a - a % 16);
+    count = (vocab + shift + kN - 1) / kN;
+  }
+  // Elements of group i; those outside the row are `fill` (their memory is not read).
+  __device__ __forceinline__ void load(int i, int vocab, float fill, float (&x)[kN]) const {
+    const int e0 = i * kN - shift;
+    if (e0 >= 0 && e0 + kN <= vocab) {
+      const uint4 v = base[i];
+      const uint32_t w[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+      for (int e = 0; e < kN; ++e) {
+        if constexpr (DT == ql::kF32) x[e] = __uint_as_float(w[e]);
+        else {
+          const uint16_t h = static_cast<uint16_t>(w[e / 2] >> (16 * (e & 1)));
+          if constexpr (DT == ql::kF16) x[e] = __half2float(__ushort_as_half(h));
+          else x[e] = __uint_as_float(static_cast<uint32_t>(h) << 16);
         }
-      __syncthreads();
-      rejected = found_s != x;
-      __syncthreads();
-      if (rejected) break;
+      }
     } else {
-      double qx = 1.0;
-      if (a.draft) {
-        q = open(a.draft, static_cast<size_t>(b) * a.drafts + pos, a.draft_stride, bad);
-        if (bad) break;
-        qx = q.value(x) / q.z;
-      }
-      rejected = !(u[pos] * qx < p.value(x) / p.z);
-      if (rejected) break;
+#pragma unroll
+      for (int e = 0; e < kN; ++e)
+        x[e] = e0 + e >= 0 && e0 + e < vocab ? ql::load_elem(base, static_cast<size_t>(i) * kN + e, DT)
+                                             : fill;
     }
-    if (tid == 0) tok[pos] = x;
   }
-  if (tid == 0) a.accepted[b] = pos;
-  if (bad) {
-    if (tid == 0) {
-      const bool id = pos < n && (ids[pos] < 0 || ids[pos] >= V);
-      atomicOr(a.status, id ? ql::kStatusBadToken : ql::kStatusBadLogits);
-    }
-    return;
-  }
-  if (a.inv_t == 0) {
-    if (tid == 0) found_s = V;
-    __syncthreads();
-    for (int i = tid; i < V; i += kVerifyThreads)
-      if (p.raw(i) == p.m) {
-        atomicMin(&found_s, i);
-        break;
-      }
-    __syncthreads();
-    if (tid == 0) tok[pos] = found_s;
-    return;
-  }
-  const int x = rejected ? ids[pos] : -1;
-  auto weight = [&](int i, bool less) {
-    double w = p.value(i) / p.z;
-    if (less) w = a.draft ? w - q.value(i) / q.z : (i == x ? 0.0 : w);
-    return w > 0 ? w : 0.0;
+};
+
+// A row as a distribution: weight(i) / z.
+struct Row {
+  size_t at;
+  float m;
+  double z;
+};
+
+template <int DT>
+__global__ void __launch_bounds__(kVerifyThreads, 1) verify_kernel(const VerifyArgs a) {
+  __shared__ float2 part[kVerifyRows][kVerifyWarps];  // a row's (m, s) or (best, id) by warp
+  __shared__ float2 mine[kVerifyRows];                // of this CTA
+  __shared__ float2 row_stat[kVerifyRows];            // of the cluster
+  __shared__ double sums[kVerifyWarps][2];
+  __shared__ double share[2][2];  // this CTA's sums, for the cluster (two turns)
+  __shared__ int pos_s, exact_s;
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, V = a.vocab;
+  const int rank = static_cast<int>(cluster_rank()), ctas = static_cast<int>(cluster_size());
+  const int b = blockIdx.x / ctas;
+  ql::griddep_wait();
+  ql::griddep_launch_dependents();
+  const int n = a.n_draft ? min(max(a.n_draft[b], 0), a.drafts) : a.drafts;
+  const int32_t* ids = a.ids + static_cast<size_t>(b) * a.drafts;
+  const double* u = a.uniforms + static_cast<size_t>(b) * (a.drafts + 1);
+  const bool greedy = a.inv_t == 0, stats = !a.probs;
+  const bool has_q = a.draft != nullptr && !greedy;
+  auto target_at = [&](int i) {
+    return (static_cast<size_t>(b) * (a.drafts + 1) + i) * static_cast<size_t>(a.target_stride);
   };
-  // thread t sums the contiguous ids [t * per, (t + 1) * per)
-  const int per = (V + kVerifyThreads - 1) / kVerifyThreads;
-  for (int pass = 0; pass < 2; ++pass) {
-    const bool less = rejected && pass == 0;
-    double s = 0;
-    for (int i = tid * per; i < min(V, (tid + 1) * per); ++i) s += weight(i, less);
-    __syncthreads();
-    part[tid] = s;
-    __syncthreads();
-    double total = 0;
-    for (int t = 0; t < kVerifyThreads; ++t) total += part[t];
-    if (!(total > 0) && less) continue;  // nothing left of the difference: the target itself
-    if (tid == 0) {
-      const double th = u[n] * total;
-      double cum = 0;
-      int last = -1, hit = -1;
-      for (int t = 0; t < kVerifyThreads && hit < 0; ++t) {
-        if (cum + part[t] < th && t + 1 < kVerifyThreads) {
-          cum += part[t];
-          continue;
+  auto draft_at = [&](int i) {
+    return (static_cast<size_t>(b) * a.drafts + i) * static_cast<size_t>(a.draft_stride);
+  };
+  // ---- 1. rows 0 .. n: the target's, n + 1 .. 2n: the draft's
+  const int nrows = stats ? n + 1 + (has_q ? n : 0) : 0;
+  const float c = static_cast<float>(fmin(a.inv_t * 1.4426950408889634, 3e38));
+  for (int i = tid; i < nrows * kVerifyWarps; i += kVerifyThreads)
+    part[i / kVerifyWarps][i % kVerifyWarps] =
+        greedy ? make_float2(-INFINITY, __int_as_float(INT_MAX)) : make_float2(-INFINITY, 0.f);
+  __syncthreads();
+  if (stats) {
+    using G = Groups<DT>;
+    constexpr int kLoads = 8;  // groups of a lane in flight
+    // items: pieces of 32 * kLoads groups of this CTA's share of a row
+    const int most = (V + 2 * G::kN - 2) / G::kN;
+    const int span = (most + ctas - 1) / ctas;
+    const int pieces = (span + 32 * kLoads - 1) / (32 * kLoads);
+    const long long items = static_cast<long long>(pieces) * nrows;
+    long long it = items * warp / kVerifyWarps;
+    const long long end = items * (warp + 1) / kVerifyWarps;
+    int row = static_cast<int>(it / pieces), piece = static_cast<int>(it % pieces);
+    while (it < end) {
+      const G g(row <= n ? a.target : a.draft, row <= n ? target_at(row) : draft_at(row - n - 1), V);
+      const int stop = min(g.count, (rank + 1) * span);
+      float m = -INFINITY, s = 0.f;
+      int best = INT_MAX, bad = 0;
+      for (; it < end && piece < pieces; ++it, ++piece) {
+        const int i0 = rank * span + piece * 32 * kLoads + lane;
+        float x[kLoads][G::kN];
+#pragma unroll
+        for (int j = 0; j < kLoads; ++j) {
+          if (i0 + 32 * j < stop) {
+            g.load(i0 + 32 * j, V, -INFINITY, x[j]);
+          } else {
+#pragma unroll
+            for (int e = 0; e < G::kN; ++e) x[j][e] = -INFINITY;
+          }
         }
-        for (int i = t * per; i < min(V, (t + 1) * per); ++i) {
-          const double w = weight(i, less);
-          if (w <= 0) continue;
-          last = i;
-          cum += w;
-          if (cum >= th) {
-            hit = i;
-            break;
+        if (greedy) {
+#pragma unroll
+          for (int j = 0; j < kLoads; ++j)
+#pragma unroll
+            for (int e = 0; e < G::kN; ++e) {  // ascending ids: the first of equals stays
+              bad |= !(x[j][e] < INFINITY);
+              if (x[j][e] > m) {
+                m = x[j][e];
+                best = (i0 + 32 * j) * G::kN - g.shift + e;
+              }
+            }
+        } else {
+          float top = m;
+#pragma unroll
+          for (int j = 0; j < kLoads; ++j)
+#pragma unroll
+            for (int e = 0; e < G::kN; ++e) top = fmaxf(top, x[j][e]);
+          if (top == -INFINITY) {  // nothing yet, unless a NaN hides among the -inf
+#pragma unroll
+            for (int j = 0; j < kLoads; ++j)
+#pragma unroll
+              for (int e = 0; e < G::kN; ++e) bad |= x[j][e] != x[j][e];
+          } else {
+            s *= m == -INFINITY ? 0.f : exp2_fast((m - top) * c);
+            m = top;
+            float add = 0.f;
+#pragma unroll
+            for (int j = 0; j < kLoads; ++j)
+#pragma unroll
+              for (int e = 0; e < G::kN; ++e) add += exp2_fast((x[j][e] - top) * c);
+            s += add;
           }
         }
       }
-      if (hit < 0)
-        for (int i = V - 1; i >= 0 && last < 0; --i)
-          if (weight(i, less) > 0) last = i;
-      tok[pos] = hit >= 0 ? hit : last;
+      // this warp's part of the row
+      if (greedy) {
+#pragma unroll
+        for (int o = 16; o > 0; o >>= 1) {
+          const float m2 = __shfl_xor_sync(0xffffffffu, m, o);
+          const int b2 = __shfl_xor_sync(0xffffffffu, best, o);
+          if (m2 > m || (m2 == m && b2 < best)) {
+            m = m2;
+            best = b2;
+          }
+        }
+        if (__any_sync(0xffffffffu, bad)) m = NAN;
+        if (lane == 0) part[row][warp] = make_float2(m, __int_as_float(best));
+      } else {
+        float top = m;
+#pragma unroll
+        for (int o = 16; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
+        s = m == -INFINITY ? 0.f : s * exp2_fast((m - top) * c);
+#pragma unroll
+        for (int o = 16; o > 0; o >>= 1) s += __shfl_xor_sync(0xffffffffu, s, o);
+        if (__any_sync(0xffffffffu, bad)) s = NAN;
+        if (lane == 0) part[row][warp] = make_float2(top, s);
+      }
+      ++row;
+      piece = 0;
     }
+    __syncthreads();
+    auto join = [&](auto at, int count) {  // (m, s) or (best, id) of `count` parts
+      float2 r = at(0);
+      for (int i = 1; i < count; ++i) {
+        const float2 v = at(i);
+        if (greedy) {
+          const int vi = __float_as_int(v.y), ri = __float_as_int(r.y);
+          if (r.x != r.x) continue;  // NaN: the row is bad
+          if (v.x != v.x || v.x > r.x || (v.x == r.x && vi < ri)) r = v;
+        } else {
+          const float top = fmaxf(r.x, v.x);
+          if (top == -INFINITY) {
+            r.y += v.y;  // zeros, or a NaN that marks the row
+          } else {
+            r.y = (r.x == -INFINITY ? r.y * 0.f : r.y * exp2_fast((r.x - top) * c)) +
+                  (v.x == -INFINITY ? v.y * 0.f : v.y * exp2_fast((v.x - top) * c));
+            r.x = top;
+          }
+        }
+      }
+      return r;
+    };
+    if (tid < nrows) mine[tid] = join([&](int w) { return part[tid][w]; }, kVerifyWarps);
+    cluster_sync();
+    if (tid < nrows)
+      row_stat[tid] = join([&](int k) { return ld_cluster_f2(&mine[tid], k); }, ctas);
+    __syncthreads();
+  }
+
+  // ---- f64 sums over the cluster: every CTA's two sums, added in rank order
+  int turn = 0;
+  auto cluster_sums = [&](double& v0, double& v1, double (*all)[2]) {
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) {
+      v0 += __shfl_xor_sync(0xffffffffu, v0, o);
+      v1 += __shfl_xor_sync(0xffffffffu, v1, o);
+    }
+    __syncthreads();
+    if (lane == 0) {
+      sums[warp][0] = v0;
+      sums[warp][1] = v1;
+    }
+    __syncthreads();
+    if (tid < 2) {
+      double s = 0;
+      for (int w = 0; w < kVerifyWarps; ++w) s += sums[w][tid];
+      share[turn][tid] = s;
+    }
+    cluster_sync();
+    v0 = v1 = 0;
+    for (int k = 0; k < ctas; ++k) {
+      const double p0 = ld_cluster_f64(&share[turn][0], k), p1 = ld_cluster_f64(&share[turn][1], k);
+      v0 += p0;
+      v1 += p1;
+      if (all) {
+        all[k][0] = p0;
+        all[k][1] = p1;
+      }
+    }
+    turn ^= 1;  // the other pair next: this one is read until the next barrier
+  };
+  // this CTA's ids, and this warp's of them
+  const int lo = static_cast<int>(static_cast<long long>(V) * rank / ctas);
+  const int hi = static_cast<int>(static_cast<long long>(V) * (rank + 1) / ctas);
+  auto warp_part = [&](int from, int to, int w) {
+    return from + static_cast<int>(static_cast<long long>(to - from) * w / kVerifyWarps);
+  };
+  const Exp64 ex(greedy ? 1.0 : a.inv_t);
+  auto weight = [&](const void* base, const Row& r, int i) {  // whole warps
+    const float x = ql::load_elem(base, r.at + i, DT);
+    return a.probs ? static_cast<double>(x) : ex(static_cast<double>(x) - r.m);
+  };
+  auto exact_sums = [&](Row& p, Row& q, bool with_q) {
+    if (a.probs) {
+      p.z = q.z = 1.0;
+      return;
+    }
+    double sp = 0, sq = 0;
+    const int from = warp_part(lo, hi, warp), to = warp_part(lo, hi, warp + 1);
+    for (int i0 = from; i0 < to; i0 += 32) {
+      const int i = min(i0 + lane, to - 1);
+      const double wp = weight(a.target, p, i);
+      const double wq = with_q ? weight(a.draft, q, i) : 0.0;
+      if (i0 + lane < to) {
+        sp += wp;
+        sq += wq;
+      }
+    }
+    cluster_sums(sp, sq, nullptr);
+    p.z = sp;
+    q.z = sq;
+  };
+
+  // ---- 2. the first draft that is not accepted
+  // of[i]: 0 accepted, 1 rejected, 2 too close for the f32 sums, 3 cannot be decided
+  auto usable = [&](float2 st) { return st.y > 0.f && st.y < INFINITY && st.x > -INFINITY; };
+  auto decide = [&](int i, double zp, double zq, bool exact) {
+    const int x = ids[i];
+    if (x < 0 || x >= V) return 3;
+    if (greedy) {
+      const float2 st = row_stat[i];
+      if (!(st.x > -INFINITY)) return 3;
+      return __float_as_int(st.y) == x ? 0 : 1;
+    }
+    double px = ql::load_elem(a.target, target_at(i) + x, DT), qx = 1.0;
+    if (stats) {
+      if (!usable(row_stat[i]) || (has_q && !usable(row_stat[n + 1 + i]))) return 3;
+      px = exp((px - row_stat[i].x) * a.inv_t) / zp;
+    } else if (!(px < INFINITY)) {
+      return 3;
+    }
+    if (has_q) {
+      qx = ql::load_elem(a.draft, draft_at(i) + x, DT);
+      if (stats) qx = exp((qx - row_stat[n + 1 + i].x) * a.inv_t) / zq;
+      else if (!(qx < INFINITY)) return 3;
+    }
+    const double uq = u[i] * qx;
+    if (stats && !exact && fabs(uq - px) <= 0x1p-14 * px) return 2;
+    return uq < px ? 0 : 1;
+  };
+  int pos = 0, how = 0;
+  for (;;) {
+    if (warp == 0) {
+      const int i = pos + lane;
+      const int d = i < n ? decide(i, row_stat[min(i, kVerifyRows - 1)].y,
+                                   row_stat[min(n + 1 + i, kVerifyRows - 1)].y, false)
+                          : 1;
+      const unsigned stop = __ballot_sync(0xffffffffu, d != 0);
+      const int first = __ffs(stop) - 1;  // n - pos <= 31, so there is one
+      const int what = __shfl_sync(0xffffffffu, d, first);
+      if (lane == 0) {
+        pos_s = pos + first;
+        exact_s = what;
+      }
+    }
+    __syncthreads();
+    pos = pos_s;
+    how = pos < n ? exact_s : 0;
+    __syncthreads();
+    if (how != 2) break;
+    Row p{target_at(pos), row_stat[pos].x, 1.0};
+    Row q{has_q ? draft_at(pos) : 0, has_q ? row_stat[n + 1 + pos].x : 0.f, 1.0};
+    exact_sums(p, q, has_q);
+    how = decide(pos, p.z, q.z, true);
+    if (how != 0) break;
+    ++pos;
+  }
+  // how: 0 all accepted (pos = n), 1 rejected at pos, 3 undecidable there
+  const bool rejected = how == 1;
+  bool bad = how == 3;
+  if (stats && !bad) bad = greedy ? !(row_stat[pos].x > -INFINITY) : !usable(row_stat[pos]);
+  if (rank == 0) {
+    int32_t* tok = a.tokens + static_cast<size_t>(b) * (a.drafts + 1);
+    for (int i = tid; i <= a.drafts; i += kVerifyThreads)
+      if (i != pos || bad || greedy)
+        tok[i] = i < pos ? ids[i]
+                 : i == pos && greedy && !bad ? __float_as_int(row_stat[pos].y) : -1;
+    if (tid == 0) a.accepted[b] = pos;
+  }
+  auto raise = [&]() {
+    if (rank == 0 && tid == 0) {
+      const bool id = pos < n && (ids[pos] < 0 || ids[pos] >= V);
+      atomicOr(a.status, id ? ql::kStatusBadToken : ql::kStatusBadLogits);
+    }
+  };
+  if (bad || greedy) {
+    if (bad) raise();
+    cluster_sync();  // nobody leaves while its shared memory may still be read
     return;
   }
+
+  // ---- 3. the draw from the target's row, less the draft's after a rejection
+  Row p{target_at(pos), stats ? row_stat[pos].x : 0.f, 1.0};
+  const bool less_q = rejected && has_q;
+  Row q{less_q ? draft_at(pos) : 0, less_q && stats ? row_stat[n + 1 + pos].x : 0.f, 1.0};
+  exact_sums(p, q, less_q);
+  const double rp = 1.0 / p.z, rq = 1.0 / q.z;
+  const int out = rejected && !has_q ? ids[pos] : -1;  // a certain draft: its id is taken out
+  bool less = rejected;
+  auto left = [&](int i) {  // whole warps
+    double w = weight(a.target, p, i) * rp;
+    if (less) w = less_q ? w - weight(a.draft, q, i) * rq : i == out ? 0.0 : w;
+    return w < 0 ? 0.0 : w;  // NaN stays
+  };
+  // this lane's sum over its warp's part of [from, to)
+  auto part_sum = [&](int from, int to) {
+    double s = 0;
+    const int f = warp_part(from, to, warp), e = warp_part(from, to, warp + 1);
+    for (int i0 = f; i0 < e; i0 += 32) {
+      const double w = left(min(i0 + lane, e - 1));
+      if (i0 + lane < e) s += w;
+    }
+    return s;
+  };
+  double all[kMaxCluster][2];
+  double total = part_sum(lo, hi), unused = 0;
+  cluster_sums(total, unused, all);
+  if (less && total <= 0) {  // nothing left of the difference: the target itself
+    less = false;
+    total = part_sum(lo, hi);
+    unused = 0;
+    cluster_sums(total, unused, all);
+  }
+  if (!(total > 0 && total < INFINITY)) {  // probabilities that are none
+    raise();
+    if (rank == 0 && tid == 0) a.tokens[static_cast<size_t>(b) * (a.drafts + 1) + pos] = -1;
+    cluster_sync();
+    return;
+  }
+  const double th = u[n] * total;
+  // The first of `count` shares where the running sum reaches th, else the last
+  // that is not empty; `before` becomes the sum before it.
+  auto find = [&](auto at, int count, double& before) {
+    int last = 0;
+    double cum = before, at_last = before;
+    for (int k = 0; k < count; ++k) {
+      const double v = at(k);
+      if (v > 0) {
+        last = k;
+        at_last = cum;
+        if (cum + v >= th) break;
+      }
+      cum += v;
+    }
+    before = at_last;
+    return last;
+  };
+  double before = 0;
+  const int owner = find([&](int k) { return all[k][0]; }, ctas, before);
+  cluster_sync();
+  if (owner != rank) return;
+  // sums[w][0] holds this CTA's warps' sums of the last part_sum
+  int from = lo, to = hi;
+  for (;;) {
+    const int w = find([&](int k) { return sums[k][0]; }, kVerifyWarps, before);
+    const int f = warp_part(from, to, w), e = warp_part(from, to, w + 1);
+    from = f;
+    to = e;
+    if (to - from <= 32) break;
+    double s = part_sum(from, to);
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) s += __shfl_xor_sync(0xffffffffu, s, o);
+    __syncthreads();
+    if (lane == 0) sums[warp][0] = s;
+    __syncthreads();
+  }
+  if (warp == 0) {
+    const int i = min(min(from + lane, max(to - 1, from)), V - 1);
+    const double w = from + lane < to ? left(i) : 0.0 * left(i);
+    double cum = w;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const double v = __shfl_up_sync(0xffffffffu, cum, o);
+      if (lane >= o) cum += v;
+    }
+    const unsigned some = __ballot_sync(0xffffffffu, w > 0);
+    const unsigned hit = __ballot_sync(0xffffffffu, w > 0 && before + cum >= th);
+    const int k = hit ? __ffs(hit) - 1 : 31 - __clz(some);
+    if (lane == 0)
+      a.tokens[static_cast<size_t>(b) * (a.drafts + 1) + pos] = some ? from + k : -1;
+  }
+}
+
+// CTAs of a cluster: up to 16 while the clusters together have an SM for each CTA, and
+// a CTA has 1024 ids or more of its rows.
+int cluster_ctas(int batch, int vocab, int num_sms) {
+  int c = kMaxCluster;
+  while (c > 1 && (static_cast<long long>(batch) * c > num_sms || vocab / c < 1024)) c /= 2;
+  return c;
+}
+
+template <int DT>
+cudaError_t launch_verify(const VerifyArgs& a, int batch, int num_sms, cudaStream_t s) {
+  const int ctas = cluster_ctas(batch, a.vocab, num_sms);
+  cudaError_t e = cudaSuccess;
+  if (ctas > 8)
+    e = cudaFuncSetAttribute(verify_kernel<DT>, cudaFuncAttributeNonPortableClusterSizeAllowed, 1);
+  if (e != cudaSuccess) return e;
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3(static_cast<unsigned>(batch) * ctas);
+  cfg.blockDim = dim3(kVerifyThreads);
+  cfg.stream = s;
+  cudaLaunchAttribute attr[2];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  attr[1].id = cudaLaunchAttributeClusterDimension;
+  attr[1].val.clusterDim.x = ctas;
+  attr[1].val.clusterDim.y = 1;
+  attr[1].val.clusterDim.z = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = 2;
+  return cudaLaunchKernelEx(&cfg, verify_kernel<DT>, a);
 }
 
 }  // namespace
@@ -252,7 +626,10 @@ extern "C" int ql_verify_drafts(ql_ctx* c, const ql_verify_args* args) {
   a.dtype = f.dtype;
   a.probs = probs;
   a.inv_t = probs ? 1.0 : greedy ? 0.0 : 1.0 / static_cast<double>(f.temperature);
-  verify_kernel<<<f.batch, kVerifyThreads, 0, c->stream>>>(a);
-  QLV_CUDA(cudaGetLastError(), "launch the draft verification");
+  cudaError_t e;
+  if (f.dtype == QL_F32) e = launch_verify<ql::kF32>(a, f.batch, c->num_sms, c->stream);
+  else if (f.dtype == QL_F16) e = launch_verify<ql::kF16>(a, f.batch, c->num_sms, c->stream);
+  else e = launch_verify<ql::kBF16>(a, f.batch, c->num_sms, c->stream);
+  QLV_CUDA(e, "launch the draft verification");
   return QL_OK;
 }
