@@ -166,7 +166,7 @@ __global__ void __launch_bounds__(kVerifyThreads, 1) verify_kernel(const VerifyA
   __shared__ float2 part[kVerifyRows][kVerifyWarps];  // a row's (m, s) or (best, id) by warp
   __shared__ float2 mine[kVerifyRows];                // of this CTA
   __shared__ float2 row_stat[kVerifyRows];            // of the cluster
-  __shared__ double sums[kVerifyWarps][2];
+  __shared__ double sums[2][kVerifyWarps];
   __shared__ double share[2][2];  // this CTA's sums, for the cluster (two turns)
   __shared__ int pos_s, exact_s;
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, V = a.vocab;
@@ -281,65 +281,69 @@ __global__ void __launch_bounds__(kVerifyThreads, 1) verify_kernel(const VerifyA
       piece = 0;
     }
     __syncthreads();
-    auto join = [&](auto at, int count) {  // (m, s) or (best, id) of `count` parts
-      float2 r = at(0);
-      for (int i = 1; i < count; ++i) {
-        const float2 v = at(i);
-        if (greedy) {
-          const int vi = __float_as_int(v.y), ri = __float_as_int(r.y);
-          if (r.x != r.x) continue;  // NaN: the row is bad
-          if (v.x != v.x || v.x > r.x || (v.x == r.x && vi < ri)) r = v;
+    // (m, s) or (best, id) of the parts that the lanes of a warp hold
+    auto join = [&](float2 r) {
+#pragma unroll
+      for (int o = 16; o > 0; o >>= 1) {
+        const float2 v = make_float2(__shfl_xor_sync(0xffffffffu, r.x, o),
+                                     __shfl_xor_sync(0xffffffffu, r.y, o));
+        if (greedy) {  // NaN: the row is bad
+          if (r.x != r.x) continue;
+          if (v.x != v.x || v.x > r.x ||
+              (v.x == r.x && __float_as_int(v.y) < __float_as_int(r.y)))
+            r = v;
         } else {
           const float top = fmaxf(r.x, v.x);
-          if (top == -INFINITY) {
-            r.y += v.y;  // zeros, or a NaN that marks the row
-          } else {
-            r.y = (r.x == -INFINITY ? r.y * 0.f : r.y * exp2_fast((r.x - top) * c)) +
-                  (v.x == -INFINITY ? v.y * 0.f : v.y * exp2_fast((v.x - top) * c));
-            r.x = top;
-          }
+          // sums under a maximum of -inf are zeros, or a NaN that marks the row
+          const float f = r.x == top ? 1.f : r.x == -INFINITY ? 0.f : exp2_fast((r.x - top) * c);
+          const float h = v.x == top ? 1.f : v.x == -INFINITY ? 0.f : exp2_fast((v.x - top) * c);
+          r.y = r.y * f + v.y * h;
+          r.x = top;
         }
       }
       return r;
     };
-    if (tid < nrows) mine[tid] = join([&](int w) { return part[tid][w]; }, kVerifyWarps);
+    const float2 none =
+        greedy ? make_float2(-INFINITY, __int_as_float(INT_MAX)) : make_float2(-INFINITY, 0.f);
+    for (int r = warp; r < nrows; r += kVerifyWarps) {
+      const float2 v = join(lane < kVerifyWarps ? part[r][lane] : none);
+      if (lane == 0) mine[r] = v;
+    }
     cluster_sync();
-    if (tid < nrows)
-      row_stat[tid] = join([&](int k) { return ld_cluster_f2(&mine[tid], k); }, ctas);
+    for (int r = warp; r < nrows; r += kVerifyWarps) {
+      const float2 v = join(lane < ctas ? ld_cluster_f2(&mine[r], lane) : none);
+      if (lane == 0) row_stat[r] = v;
+    }
     __syncthreads();
   }
 
-  // ---- f64 sums over the cluster: every CTA's two sums, added in rank order
+  // ---- f64 sums over the cluster; lane k of every warp gets CTA k's first sum
   int turn = 0;
-  auto cluster_sums = [&](double& v0, double& v1, double (*all)[2]) {
+  auto warp_total = [&](double v) {
 #pragma unroll
-    for (int o = 16; o > 0; o >>= 1) {
-      v0 += __shfl_xor_sync(0xffffffffu, v0, o);
-      v1 += __shfl_xor_sync(0xffffffffu, v1, o);
-    }
-    __syncthreads();
+    for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
+    return v;
+  };
+  auto cluster_sums = [&](double& v0, double& v1) -> double {
+    v0 = warp_total(v0);
+    v1 = warp_total(v1);
+    __syncthreads();  // the warps' sums before have been read
     if (lane == 0) {
-      sums[warp][0] = v0;
-      sums[warp][1] = v1;
+      sums[0][warp] = v0;
+      sums[1][warp] = v1;
     }
     __syncthreads();
-    if (tid < 2) {
-      double s = 0;
-      for (int w = 0; w < kVerifyWarps; ++w) s += sums[w][tid];
-      share[turn][tid] = s;
+    if (warp < 2) {
+      const double s = warp_total(lane < kVerifyWarps ? sums[warp][lane] : 0.0);
+      if (lane == 0) share[turn][warp] = s;
     }
     cluster_sync();
-    v0 = v1 = 0;
-    for (int k = 0; k < ctas; ++k) {
-      const double p0 = ld_cluster_f64(&share[turn][0], k), p1 = ld_cluster_f64(&share[turn][1], k);
-      v0 += p0;
-      v1 += p1;
-      if (all) {
-        all[k][0] = p0;
-        all[k][1] = p1;
-      }
-    }
+    const double p0 = lane < ctas ? ld_cluster_f64(&share[turn][0], lane) : 0.0;
+    const double p1 = lane < ctas ? ld_cluster_f64(&share[turn][1], lane) : 0.0;
+    v0 = warp_total(p0);
+    v1 = warp_total(p1);
     turn ^= 1;  // the other pair next: this one is read until the next barrier
+    return p0;
   };
   // this CTA's ids, and this warp's of them
   const int lo = static_cast<int>(static_cast<long long>(V) * rank / ctas);
@@ -348,9 +352,25 @@ __global__ void __launch_bounds__(kVerifyThreads, 1) verify_kernel(const VerifyA
     return from + static_cast<int>(static_cast<long long>(to - from) * w / kVerifyWarps);
   };
   const Exp64 ex(greedy ? 1.0 : a.inv_t);
-  auto weight = [&](const void* base, const Row& r, int i) {  // whole warps
-    const float x = ql::load_elem(base, r.at + i, DT);
-    return a.probs ? static_cast<double>(x) : ex(static_cast<double>(x) - r.m);
+  // Weights of a row at four ids of a lane (their loads, and then the steps of four
+  // exponentials, in flight together); whole warps.
+  auto weights = [&](const void* base, const Row& r, const int (&i)[4], double (&w)[4]) {
+    float x[4];
+#pragma unroll
+    for (int e = 0; e < 4; ++e) x[e] = ql::load_elem(base, r.at + i[e], DT);
+#pragma unroll
+    for (int e = 0; e < 4; ++e)
+      w[e] = a.probs ? static_cast<double>(x[e]) : ex(static_cast<double>(x[e]) - r.m);
+  };
+  // add(ids, of) over this warp's part of [from, to), 128 ids at a time; ids past the
+  // part repeat its last, and `of` says how many of the lane's four are inside
+  auto each = [&](int from, int to, auto add) {
+    const int f = warp_part(from, to, warp), e = warp_part(from, to, warp + 1);
+    for (int i0 = f + lane; i0 - lane < e; i0 += 128) {
+      const int i[4] = {min(i0, e - 1), min(i0 + 32, e - 1), min(i0 + 64, e - 1),
+                        min(i0 + 96, e - 1)};
+      add(i, i0 < e ? min(4, (e - i0 + 31) / 32) : 0);
+    }
   };
   auto exact_sums = [&](Row& p, Row& q, bool with_q) {
     if (a.probs) {
@@ -358,17 +378,18 @@ __global__ void __launch_bounds__(kVerifyThreads, 1) verify_kernel(const VerifyA
       return;
     }
     double sp = 0, sq = 0;
-    const int from = warp_part(lo, hi, warp), to = warp_part(lo, hi, warp + 1);
-    for (int i0 = from; i0 < to; i0 += 32) {
-      const int i = min(i0 + lane, to - 1);
-      const double wp = weight(a.target, p, i);
-      const double wq = with_q ? weight(a.draft, q, i) : 0.0;
-      if (i0 + lane < to) {
-        sp += wp;
-        sq += wq;
+    each(lo, hi, [&](const int(&i)[4], int of) {
+      double w[4];
+      weights(a.target, p, i, w);
+#pragma unroll
+      for (int e = 0; e < 4; ++e) sp += e < of ? w[e] : 0.0;
+      if (with_q) {
+        weights(a.draft, q, i, w);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) sq += e < of ? w[e] : 0.0;
       }
-    }
-    cluster_sums(sp, sq, nullptr);
+    });
+    cluster_sums(sp, sq);
     p.z = sp;
     q.z = sq;
   };
@@ -459,29 +480,35 @@ __global__ void __launch_bounds__(kVerifyThreads, 1) verify_kernel(const VerifyA
   const double rp = 1.0 / p.z, rq = 1.0 / q.z;
   const int out = rejected && !has_q ? ids[pos] : -1;  // a certain draft: its id is taken out
   bool less = rejected;
-  auto left = [&](int i) {  // whole warps
-    double w = weight(a.target, p, i) * rp;
-    if (less) w = less_q ? w - weight(a.draft, q, i) * rq : i == out ? 0.0 : w;
-    return w < 0 ? 0.0 : w;  // NaN stays
+  auto left = [&](const int(&i)[4], double (&w)[4]) {  // whole warps
+    weights(a.target, p, i, w);
+    double v[4];
+    if (less && less_q) weights(a.draft, q, i, v);
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      w[e] *= rp;
+      if (less) w[e] = less_q ? w[e] - v[e] * rq : i[e] == out ? 0.0 : w[e];
+      w[e] = w[e] < 0 ? 0.0 : w[e];  // NaN stays
+    }
   };
   // this lane's sum over its warp's part of [from, to)
   auto part_sum = [&](int from, int to) {
     double s = 0;
-    const int f = warp_part(from, to, warp), e = warp_part(from, to, warp + 1);
-    for (int i0 = f; i0 < e; i0 += 32) {
-      const double w = left(min(i0 + lane, e - 1));
-      if (i0 + lane < e) s += w;
-    }
+    each(from, to, [&](const int(&i)[4], int of) {
+      double w[4];
+      left(i, w);
+#pragma unroll
+      for (int e = 0; e < 4; ++e) s += e < of ? w[e] : 0.0;
+    });
     return s;
   };
-  double all[kMaxCluster][2];
   double total = part_sum(lo, hi), unused = 0;
-  cluster_sums(total, unused, all);
+  double of_cta = cluster_sums(total, unused);
   if (less && total <= 0) {  // nothing left of the difference: the target itself
     less = false;
     total = part_sum(lo, hi);
     unused = 0;
-    cluster_sums(total, unused, all);
+    of_cta = cluster_sums(total, unused);
   }
   if (!(total > 0 && total < INFINITY)) {  // probabilities that are none
     raise();
@@ -490,54 +517,46 @@ __global__ void __launch_bounds__(kVerifyThreads, 1) verify_kernel(const VerifyA
     return;
   }
   const double th = u[n] * total;
-  // The first of `count` shares where the running sum reaches th, else the last
-  // that is not empty; `before` becomes the sum before it.
-  auto find = [&](auto at, int count, double& before) {
-    int last = 0;
-    double cum = before, at_last = before;
-    for (int k = 0; k < count; ++k) {
-      const double v = at(k);
-      if (v > 0) {
-        last = k;
-        at_last = cum;
-        if (cum + v >= th) break;
-      }
-      cum += v;
+  // Of the lanes' shares (in lane order), the first where the running sum reaches
+  // th, else the last that is not empty; `before` becomes the sum before it.
+  auto find = [&](double v, double& before) {
+    double cum = v;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const double w = __shfl_up_sync(0xffffffffu, cum, o);
+      if (lane >= o) cum += w;
     }
-    before = at_last;
-    return last;
+    const unsigned some = __ballot_sync(0xffffffffu, v > 0);
+    const unsigned hit = __ballot_sync(0xffffffffu, v > 0 && before + cum >= th);
+    const int k = hit ? __ffs(hit) - 1 : some ? 31 - __clz(some) : 0;
+    before += __shfl_sync(0xffffffffu, cum - v, k);
+    return k;
   };
   double before = 0;
-  const int owner = find([&](int k) { return all[k][0]; }, ctas, before);
+  const int owner = find(of_cta, before);
   cluster_sync();
   if (owner != rank) return;
-  // sums[w][0] holds this CTA's warps' sums of the last part_sum
+  // sums[0] holds this CTA's warps' sums of the last part_sum
   int from = lo, to = hi;
   for (;;) {
-    const int w = find([&](int k) { return sums[k][0]; }, kVerifyWarps, before);
+    const int w = find(lane < kVerifyWarps ? sums[0][lane] : 0.0, before);
     const int f = warp_part(from, to, w), e = warp_part(from, to, w + 1);
     from = f;
     to = e;
     if (to - from <= 32) break;
-    double s = part_sum(from, to);
-#pragma unroll
-    for (int o = 16; o > 0; o >>= 1) s += __shfl_xor_sync(0xffffffffu, s, o);
+    const double s = warp_total(part_sum(from, to));
     __syncthreads();
-    if (lane == 0) sums[warp][0] = s;
+    if (lane == 0) sums[0][warp] = s;
     __syncthreads();
   }
   if (warp == 0) {
-    const int i = min(min(from + lane, max(to - 1, from)), V - 1);
-    const double w = from + lane < to ? left(i) : 0.0 * left(i);
-    double cum = w;
-#pragma unroll
-    for (int o = 1; o < 32; o <<= 1) {
-      const double v = __shfl_up_sync(0xffffffffu, cum, o);
-      if (lane >= o) cum += v;
-    }
-    const unsigned some = __ballot_sync(0xffffffffu, w > 0);
-    const unsigned hit = __ballot_sync(0xffffffffu, w > 0 && before + cum >= th);
-    const int k = hit ? __ffs(hit) - 1 : 31 - __clz(some);
+    const int at = min(min(from + lane, max(to - 1, from)), V - 1);
+    const int i[4] = {at, at, at, at};
+    double w[4];
+    left(i, w);
+    const double v = from + lane < to ? w[0] : 0.0;
+    const unsigned some = __ballot_sync(0xffffffffu, v > 0);
+    const int k = find(v, before);
     if (lane == 0)
       a.tokens[static_cast<size_t>(b) * (a.drafts + 1) + pos] = some ? from + k : -1;
   }
