@@ -34,19 +34,25 @@ struct VerifyArgs {
 
 // One cluster of CTAs per sequence, each CTA with its share of every row.
 //   1. f32 (maximum, sum of exponentials) of all of the sequence's rows at once --
-//      the one pass over the logits, bound by their bytes -- joined over the cluster
-//      through distributed shared memory.  (Greedy: largest logit and its id.)
+//      the one pass over the logits, bound by their bytes.  (Greedy: largest logit and
+//      its id.)
 //   2. Every draft is decided from its two logits and those sums.  A decision whose
-//      two sides are within 2^-14 of each other, far more than the f32 sums' error, is
+//      two sides are within 2^-14 of each other, far more than the f32 error, is
 //      taken again from f64 sums of its rows.
-//   3. The rows at the first rejection (or the last row) are summed again in f64: the
-//      draw compares running sums over the whole vocabulary with a threshold, where an
-//      error of 1e-7 would change one token in some thousands.  The CTA, the warp and
-//      the lane where the running sum of the draw passes the threshold are found in
-//      turn.
-// All CTAs compute the same decisions from the same numbers, so the cluster's
-// barriers are met by all.  Nothing is kept outside shared memory.
-constexpr int kVerifyThreads = 512;
+//   3. The draw compares running sums over the whole vocabulary with a threshold,
+//      where an error of 1e-7 would change one token in some thousands: its sums are
+//      f64.  A rejected draft's two rows are summed first, for their ratio; then the
+//      sum of what is left of the target gives the threshold, and the CTA, the warps
+//      and the lane where the running sum passes it are found in turn.
+// The CTAs of a cluster tell each other their sums by stores into one another's
+// shared memory that count on an mbarrier there; all make the same decisions from the
+// same numbers.  Nothing is kept outside shared memory.
+// A small call is bound by its instructions, not its bytes (32 sequences, one row of
+// 32000: 24 us when every warp followed every decision): only the sums themselves are
+// every warp's work, one loop for all of them, and warp 0 alone decides what is next.
+// Greedy, logits and probabilities are kernels of their own, and rows are read in
+// whole aligned groups with the odd ends on the side.
+constexpr int kVerifyThreads = 256;
 constexpr int kVerifyWarps = kVerifyThreads / 32;
 constexpr int kVerifyRows = 2 * QL_VERIFY_MAX_DRAFTS + 1;
 constexpr int kMaxCluster = 16;
@@ -61,201 +67,188 @@ __device__ __forceinline__ uint32_t cluster_size() {
   asm("mov.u32 %0, %%cluster_nctarank;" : "=r"(r));
   return r;
 }
-__device__ __forceinline__ void cluster_sync() {
-  asm volatile("barrier.cluster.arrive.release;" ::: "memory");
-  asm volatile("barrier.cluster.wait.acquire;" ::: "memory");
-}
-__device__ __forceinline__ float2 ld_cluster_f2(const void* p, uint32_t rank) {
-  float2 v;
-  asm volatile("ld.shared::cluster.v2.f32 {%0, %1}, [%2];"
-               : "=f"(v.x), "=f"(v.y)
-               : "r"(ql::mapa_shared(ql::smem_u32(p), rank))
-               : "memory");
-  return v;
-}
-__device__ __forceinline__ double ld_cluster_f64(const void* p, uint32_t rank) {
-  double v;
-  asm volatile("ld.shared::cluster.f64 %0, [%1];"
-               : "=d"(v)
-               : "r"(ql::mapa_shared(ql::smem_u32(p), rank))
-               : "memory");
-  return v;
-}
 __device__ __forceinline__ float exp2_fast(float x) {
   float y;
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
   return y;
 }
+__device__ __forceinline__ double warp_total(double v) {
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
+  return v;
+}
 
-// exp(d / T) in f64 for d <= 0 by the table method (P. T. P. Tang, 1989):
-// d / T = (k + r) ln2 / 32 with |r| <= 1/2, k = 32 e + j; the result is
-// 2^e 2^(j/32) exp(r ln2 / 32), the last by five terms of its series (the sixth is
-// below 3e-15).  Lane j holds 2^(j/32), read by shuffles: whole warps call this.
+// exp((x - m) / T) in f64 for x <= m by the table method (P. T. P. Tang, 1989):
+// (x - m) / T = (k + r) ln2 / 32 with |r| <= 1/2, k = 32 e + j; the result is
+// 2^e 2^(j/32) exp(r ln2 / 32), the last by four terms of its series (the fifth is
+// below 1.3e-12).  Lane j holds 2^(j/32), read by shuffles: whole warps call this.
 struct Exp64 {
-  double table, scale, least;
+  double table, scale;
+  float span;
   __device__ explicit Exp64(double inv_t) {
     constexpr double ln2 = 0.693147180559945309417232;
     table = exp2(static_cast<double>(threadIdx.x & 31) / 32.0);
     scale = inv_t * (32.0 / ln2);
-    least = -690.0 / inv_t;  // below it the result is taken as 0 (it is under 1e-299)
+    span = static_cast<float>(fmin(690.0 / inv_t, 3e38));
   }
-  __device__ __forceinline__ double operator()(double d) const {
+  // Below it an exponential (under 1e-299) is taken as 0.
+  __device__ __forceinline__ float least(float m) const { return m - span; }
+  __device__ __forceinline__ double operator()(float x, double m, float least) const {
     constexpr double L = 0.693147180559945309417232 / 32.0;
     constexpr double magic = 6755399441055744.0;  // 1.5 * 2^52
-    const bool in = d >= least;
-    if (!in) d = 0.0;
+    const double d = static_cast<double>(x) - m;
     const double t = fma(d, scale, magic);
     const int k = __double2loint(t);
     const double r = fma(d, scale, magic - t);
-    double p = fma(r, L * L * L * L * L / 120, L * L * L * L / 24);
-    p = fma(p, r, L * L * L / 6);
+    double p = fma(r, L * L * L * L / 24, L * L * L / 6);
     p = fma(p, r, L * L / 2);
     p = fma(p, r, L);
     p = fma(p, r, 1.0);
-    const int hi = __shfl_sync(0xffffffffu, __double2hiint(table), k & 31) + ((k >> 5) << 20);
-    const int lo = __shfl_sync(0xffffffffu, __double2loint(table), k & 31);
-    return in ? p * __hiloint2double(hi, lo) : 0.0;
+    const int hi = __shfl_sync(0xffffffffu, __double2hiint(table), k) + ((k & ~31) << 15);
+    const int lo = __shfl_sync(0xffffffffu, __double2loint(table), k);
+    return x < least ? 0.0 : p * __hiloint2double(hi, lo);
   }
 };
 
-// A row's 16-byte groups: element e of the row is element (e + shift) of the groups.
-template <int DT>
-struct Groups {
-  static constexpr int kN = DT == ql::kF32 ? 4 : 8;
-  const uint4* base;
-  int shift, count;
-  __device__ Groups(const void* p, size_t at, int vocab) {
-    const uintptr_t a = reinterpret_cast<uintptr_t>(p) + at * (16 / kN);
-    shift = static_cast<int>(a % 16) / (16 / kN);
-    base = reinterpret_cast<const uint4*>(a - a % 16);
-    count = (vocab + shift + kN - 1) / kN;
-  }
-  // Elements of group i; those outside the row are `fill` (their memory is not read).
-  __device__ __forceinline__ void load(int i, int vocab, float fill, float (&x)[kN]) const {
-    const int e0 = i * kN - shift;
-    if (e0 >= 0 && e0 + kN <= vocab) {
-      const uint4 v = base[i];
-      const uint32_t w[4] = {v.x, v.y, v.z, v.w};
-#pragma unroll
-      for (int e = 0; e < kN; ++e) {
-        if constexpr (DT == ql::kF32) x[e] = __uint_as_float(w[e]);
-        else {
-          const uint16_t h = static_cast<uint16_t>(w[e / 2] >> (16 * (e & 1)));
-          if constexpr (DT == ql::kF16) x[e] = __half2float(__ushort_as_half(h));
-          else x[e] = __uint_as_float(static_cast<uint32_t>(h) << 16);
-        }
-      }
-    } else {
-#pragma unroll
-      for (int e = 0; e < kN; ++e)
-        x[e] = e0 + e >= 0 && e0 + e < vocab ? ql::load_elem(base, static_cast<size_t>(i) * kN + e, DT)
-                                             : fill;
-    }
-  }
-};
-
-// A row as a distribution: weight(i) / z.
-struct Row {
-  size_t at;
-  float m;
-  double z;
-};
+enum VerifyMode : int { kGreedy = 0, kLogits = 1, kProbs = 2 };
 
 template <int DT>
-__global__ void __launch_bounds__(kVerifyThreads, 1) verify_kernel(const VerifyArgs a) {
-  __shared__ float2 part[kVerifyRows][kVerifyWarps];  // a row's (m, s) or (best, id) by warp
-  __shared__ float2 mine[kVerifyRows];                // of this CTA
-  __shared__ float2 row_stat[kVerifyRows];            // of the cluster
+__device__ __forceinline__ float half_word(uint32_t w, int upper) {
+  if constexpr (DT == ql::kF16)
+    return __half2float(__ushort_as_half(static_cast<uint16_t>(w >> (16 * upper))));
+  return __uint_as_float(upper ? w & 0xffff0000u : w << 16);
+}
+
+// What the CTA does next: set by warp 0, read by all.
+struct VerifyStep {
+  int what;       // the sums to take, or kDone
+  int from, to;   // over these ids
+  int pos;        // of these rows
+  int out;        // a certain draft's id that is taken out of the row, or -1
+  double fp, fq;  // of max(wp fp - wq fq, 0)
+};
+enum : int { kTotals = 0, kAtDraft = 1, kLeft = 2, kNarrow = 3, kDone = 4 };
+
+template <int DT, int MODE>
+__global__ void __launch_bounds__(kVerifyThreads, 4) verify_kernel(const VerifyArgs a) {
+  constexpr int kN = DT == ql::kF32 ? 4 : 8;  // elements of a 16-byte group
+  constexpr int kLoads = 4;                   // groups of a lane in a piece
+  constexpr uint32_t kNone = DT == ql::kF32 ? 0xff800000u : DT == ql::kF16 ? 0xfc00fc00u : 0xff80ff80u;
+  __shared__ float2 part[kVerifyRows][kVerifyWarps];     // a row's (m, s) or (best, id) by warp
+  __shared__ __align__(16) float2 from_cta[kVerifyRows][kMaxCluster];  // by CTA of the cluster
+  __shared__ float2 row_stat[kVerifyRows];               // of the whole row
   __shared__ double sums[2][kVerifyWarps];
-  __shared__ double share[2][2];  // this CTA's sums, for the cluster (two turns)
-  __shared__ int pos_s, exact_s;
+  __shared__ __align__(16) float4 sums_of[2][kMaxCluster];  // two f64 of each CTA (two turns)
+  __shared__ VerifyStep next_step;
+  __shared__ __align__(8) uint64_t bars[3];
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, V = a.vocab;
   const int rank = static_cast<int>(cluster_rank()), ctas = static_cast<int>(cluster_size());
   const int b = blockIdx.x / ctas;
+  if (tid == 0) {
+    for (uint64_t& bar : bars) ql::mbar_init(&bar, 1);
+    ql::fence_mbar_init();
+  }
+  __syncthreads();
+  ql::cluster_arrive_relaxed();
   ql::griddep_wait();
   ql::griddep_launch_dependents();
   const int n = a.n_draft ? min(max(a.n_draft[b], 0), a.drafts) : a.drafts;
   const int32_t* ids = a.ids + static_cast<size_t>(b) * a.drafts;
   const double* u = a.uniforms + static_cast<size_t>(b) * (a.drafts + 1);
-  const bool greedy = a.inv_t == 0, stats = !a.probs;
-  const bool has_q = a.draft != nullptr && !greedy;
-  auto target_at = [&](int i) {
-    return (static_cast<size_t>(b) * (a.drafts + 1) + i) * static_cast<size_t>(a.target_stride);
+  const bool has_q = MODE != kGreedy && a.draft != nullptr;
+  // Row r: 0 .. n the target's, n + 1 .. 2n the draft's.
+  constexpr size_t kBytes = DT == ql::kF32 ? 4 : 2;
+  auto row_at = [&](int r) {
+    return r <= n ? static_cast<const char*>(a.target) +
+                        (static_cast<size_t>(b) * (a.drafts + 1) + r) * a.target_stride * kBytes
+                  : static_cast<const char*>(a.draft) +
+                        (static_cast<size_t>(b) * a.drafts + r - n - 1) * a.draft_stride * kBytes;
   };
-  auto draft_at = [&](int i) {
-    return (static_cast<size_t>(b) * a.drafts + i) * static_cast<size_t>(a.draft_stride);
-  };
-  // ---- 1. rows 0 .. n: the target's, n + 1 .. 2n: the draft's
-  const int nrows = stats ? n + 1 + (has_q ? n : 0) : 0;
+  // ---- 1.
   const float c = static_cast<float>(fmin(a.inv_t * 1.4426950408889634, 3e38));
-  for (int i = tid; i < nrows * kVerifyWarps; i += kVerifyThreads)
-    part[i / kVerifyWarps][i % kVerifyWarps] =
-        greedy ? make_float2(-INFINITY, __int_as_float(INT_MAX)) : make_float2(-INFINITY, 0.f);
-  __syncthreads();
-  if (stats) {
-    using G = Groups<DT>;
-    constexpr int kLoads = 8;  // groups of a lane in flight
-    // items: pieces of 32 * kLoads groups of this CTA's share of a row
-    const int most = (V + 2 * G::kN - 2) / G::kN;
-    const int span = (most + ctas - 1) / ctas;
-    const int pieces = (span + 32 * kLoads - 1) / (32 * kLoads);
-    const long long items = static_cast<long long>(pieces) * nrows;
-    long long it = items * warp / kVerifyWarps;
-    const long long end = items * (warp + 1) / kVerifyWarps;
-    int row = static_cast<int>(it / pieces), piece = static_cast<int>(it % pieces);
+  if constexpr (MODE != kProbs) {
+    const int nrows = n + 1 + (has_q ? n : 0);
+    const float2 none = make_float2(-INFINITY, MODE == kGreedy ? __int_as_float(INT_MAX) : 0.f);
+    for (int i = tid; i < nrows * kVerifyWarps; i += kVerifyThreads) part[0][i] = none;
+    __syncthreads();
+    // pieces of 32 * kLoads groups of this CTA's share of each row, by warps in turn
+    const int span = (V / kN + ctas - 1) / ctas;
+    const int pieces = max(1, (span + 32 * kLoads - 1) / (32 * kLoads));
+    const int items = pieces * nrows;
+    int it = static_cast<int>(static_cast<long long>(items) * warp / kVerifyWarps);
+    const int end = static_cast<int>(static_cast<long long>(items) * (warp + 1) / kVerifyWarps);
+    int row = it / pieces, piece = it % pieces;  // of the next piece to load
+    uint4 now[kLoads], next[kLoads];
+    int first = 0;  // id of the lane's first element of `next`
+    float end_x = -INFINITY;  // an element outside the row's whole groups
+    int end_id = 0;
+    auto load = [&]() {
+      const char* p = row_at(row);
+      const int lead = static_cast<int>((16 - reinterpret_cast<uintptr_t>(p) % 16) % 16 / kBytes);
+      const int head = min(lead, V), groups = (V - head) / kN;
+      const int g0 = rank * span + piece * 32 * kLoads + lane;
+      const int stop = min(groups, (rank + 1) * span);
+      const uint4* gp = reinterpret_cast<const uint4*>(p + head * kBytes);
+#pragma unroll
+      for (int j = 0; j < kLoads; ++j)
+        next[j] = g0 + 32 * j < stop ? gp[g0 + 32 * j] : make_uint4(kNone, kNone, kNone, kNone);
+      first = head + g0 * kN;
+      end_x = -INFINITY;
+      if (rank == 0 && piece == 0) {  // the ends: lanes 0-15 before, 16-31 behind
+        end_id = lane < 16 ? lane : head + groups * kN + lane - 16;
+        if (lane < 16 ? lane < head : end_id < V) end_x = ql::load_elem(p, end_id, DT);
+      }
+    };
+    if (it < end) load();
     while (it < end) {
-      const G g(row <= n ? a.target : a.draft, row <= n ? target_at(row) : draft_at(row - n - 1), V);
-      const int stop = min(g.count, (rank + 1) * span);
+      const int at = row;
       float m = -INFINITY, s = 0.f;
       int best = INT_MAX, bad = 0;
-      for (; it < end && piece < pieces; ++it, ++piece) {
-        const int i0 = rank * span + piece * 32 * kLoads + lane;
-        float x[kLoads][G::kN];
+      do {
 #pragma unroll
-        for (int j = 0; j < kLoads; ++j) {
-          if (i0 + 32 * j < stop) {
-            g.load(i0 + 32 * j, V, -INFINITY, x[j]);
-          } else {
-#pragma unroll
-            for (int e = 0; e < G::kN; ++e) x[j][e] = -INFINITY;
-          }
+        for (int j = 0; j < kLoads; ++j) now[j] = next[j];
+        const float ex = end_x;
+        const int eid = end_id, id0 = first;
+        if (++piece == pieces) {
+          piece = 0;
+          ++row;
         }
-        if (greedy) {
-#pragma unroll
-          for (int j = 0; j < kLoads; ++j)
-#pragma unroll
-            for (int e = 0; e < G::kN; ++e) {  // ascending ids: the first of equals stays
-              bad |= !(x[j][e] < INFINITY);
-              if (x[j][e] > m) {
-                m = x[j][e];
-                best = (i0 + 32 * j) * G::kN - g.shift + e;
-              }
+        if (++it < end) load();  // in flight while this piece is summed
+        auto element = [&](int k) {
+          const uint4 v = now[k / kN];
+          const int e = k % kN, w = DT == ql::kF32 ? e : e / 2;
+          const uint32_t x = w == 0 ? v.x : w == 1 ? v.y : w == 2 ? v.z : v.w;
+          if constexpr (DT == ql::kF32) return __uint_as_float(x);
+          else return half_word<DT>(x, e & 1);
+        };
+        if constexpr (MODE == kGreedy) {
+          auto take = [&](float x, int id) {
+            bad |= !(x < INFINITY);
+            if (x > m || (x == m && id < best)) {
+              m = x;
+              best = id;
             }
+          };
+#pragma unroll
+          for (int k = 0; k < kLoads * kN; ++k)
+            take(element(k), id0 + k / kN * (32 * kN) + k % kN);
+          take(ex, eid);
         } else {
-          float top = m;
+          float top = fmaxf(m, ex);
 #pragma unroll
-          for (int j = 0; j < kLoads; ++j)
+          for (int k = 0; k < kLoads * kN; ++k) top = fmaxf(top, element(k));
+          // nothing above -inf yet: 0 for the maximum leaves zeros, and NaN a NaN
+          const float ref = top == -INFINITY ? 0.f : top;
+          s = s * exp2_fast((m == -INFINITY ? 0.f : m - ref) * c) + exp2_fast((ex - ref) * c);
+          m = top;
+          float add[4] = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-            for (int e = 0; e < G::kN; ++e) top = fmaxf(top, x[j][e]);
-          if (top == -INFINITY) {  // nothing yet, unless a NaN hides among the -inf
-#pragma unroll
-            for (int j = 0; j < kLoads; ++j)
-#pragma unroll
-              for (int e = 0; e < G::kN; ++e) bad |= x[j][e] != x[j][e];
-          } else {
-            s *= m == -INFINITY ? 0.f : exp2_fast((m - top) * c);
-            m = top;
-            float add = 0.f;
-#pragma unroll
-            for (int j = 0; j < kLoads; ++j)
-#pragma unroll
-              for (int e = 0; e < G::kN; ++e) add += exp2_fast((x[j][e] - top) * c);
-            s += add;
-          }
+          for (int k = 0; k < kLoads * kN; ++k) add[k % 4] += exp2_fast((element(k) - ref) * c);
+          s += (add[0] + add[1]) + (add[2] + add[3]);
         }
-      }
+      } while (it < end && row == at);
       // this warp's part of the row
-      if (greedy) {
+      if constexpr (MODE == kGreedy) {
 #pragma unroll
         for (int o = 16; o > 0; o >>= 1) {
           const float m2 = __shfl_xor_sync(0xffffffffu, m, o);
@@ -266,316 +259,301 @@ __global__ void __launch_bounds__(kVerifyThreads, 1) verify_kernel(const VerifyA
           }
         }
         if (__any_sync(0xffffffffu, bad)) m = NAN;
-        if (lane == 0) part[row][warp] = make_float2(m, __int_as_float(best));
+        if (lane == 0) part[at][warp] = make_float2(m, __int_as_float(best));
       } else {
         float top = m;
 #pragma unroll
         for (int o = 16; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
-        s = m == -INFINITY ? 0.f : s * exp2_fast((m - top) * c);
+        s *= m == top ? 1.f : m == -INFINITY ? 0.f * s : exp2_fast((m - top) * c);
 #pragma unroll
         for (int o = 16; o > 0; o >>= 1) s += __shfl_xor_sync(0xffffffffu, s, o);
-        if (__any_sync(0xffffffffu, bad)) s = NAN;
-        if (lane == 0) part[row][warp] = make_float2(top, s);
+        if (lane == 0) part[at][warp] = make_float2(top, s);
       }
-      ++row;
-      piece = 0;
     }
+    // (m, s) or (best, id) of the parts of a row that a warp's lanes hold: first of
+    // the CTA's warps, told to every CTA, then of the CTAs
+    if (tid == 0) ql::mbar_arrive_expect_tx(&bars[0], static_cast<uint32_t>(nrows * ctas * 8));
     __syncthreads();
-    // (m, s) or (best, id) of the parts that the lanes of a warp hold
-    auto join = [&](float2 r) {
-#pragma unroll
-      for (int o = 16; o > 0; o >>= 1) {
-        const float2 v = make_float2(__shfl_xor_sync(0xffffffffu, r.x, o),
-                                     __shfl_xor_sync(0xffffffffu, r.y, o));
-        if (greedy) {  // NaN: the row is bad
-          if (r.x != r.x) continue;
-          if (v.x != v.x || v.x > r.x ||
-              (v.x == r.x && __float_as_int(v.y) < __float_as_int(r.y)))
-            r = v;
-        } else {
-          const float top = fmaxf(r.x, v.x);
-          // sums under a maximum of -inf are zeros, or a NaN that marks the row
-          const float f = r.x == top ? 1.f : r.x == -INFINITY ? 0.f : exp2_fast((r.x - top) * c);
-          const float h = v.x == top ? 1.f : v.x == -INFINITY ? 0.f : exp2_fast((v.x - top) * c);
-          r.y = r.y * f + v.y * h;
-          r.x = top;
+    ql::cluster_wait();  // every CTA's barriers are there
+#pragma unroll 1
+    for (int turn = 0; turn < 2; ++turn) {
+      if (turn == 1) ql::mbar_wait_cluster(&bars[0], 0, a.status);
+#pragma unroll 1
+      for (int r = warp; r < nrows; r += kVerifyWarps) {
+        float2 z = none;
+        if (turn == 0 && lane < kVerifyWarps) z = part[r][lane];
+        if (turn == 1 && lane < ctas) z = from_cta[r][lane];
+#pragma unroll 1
+        for (int o = 8; o > 0; o >>= 1) {
+          const float2 v = make_float2(__shfl_xor_sync(0xffffffffu, z.x, o),
+                                       __shfl_xor_sync(0xffffffffu, z.y, o));
+          if constexpr (MODE == kGreedy) {  // a NaN marks the row
+            if (z.x == z.x && (v.x != v.x || v.x > z.x ||
+                               (v.x == z.x && __float_as_int(v.y) < __float_as_int(z.y))))
+              z = v;
+          } else {  // sums under a maximum of -inf are zeros, or a NaN that marks the row
+            const float top = fmaxf(z.x, v.x);
+            const float f = z.x == top ? 1.f : z.x == -INFINITY ? 0.f : exp2_fast((z.x - top) * c);
+            const float h = v.x == top ? 1.f : v.x == -INFINITY ? 0.f : exp2_fast((v.x - top) * c);
+            z = make_float2(top, z.y * f + v.y * h);
+          }
+        }
+        if (turn == 0) {
+          if (lane < ctas)
+            ql::st_async_v2(ql::mapa_shared(ql::smem_u32(&from_cta[r][rank]), lane), z,
+                            ql::mapa_shared(ql::smem_u32(&bars[0]), lane));
+        } else if (lane == 0) {
+          row_stat[r] = z;
         }
       }
-      return r;
-    };
-    const float2 none =
-        greedy ? make_float2(-INFINITY, __int_as_float(INT_MAX)) : make_float2(-INFINITY, 0.f);
-    for (int r = warp; r < nrows; r += kVerifyWarps) {
-      const float2 v = join(lane < kVerifyWarps ? part[r][lane] : none);
-      if (lane == 0) mine[r] = v;
-    }
-    cluster_sync();
-    for (int r = warp; r < nrows; r += kVerifyWarps) {
-      const float2 v = join(lane < ctas ? ld_cluster_f2(&mine[r], lane) : none);
-      if (lane == 0) row_stat[r] = v;
     }
     __syncthreads();
+  } else {
+    ql::cluster_wait();
   }
 
-  // ---- f64 sums over the cluster; lane k of every warp gets CTA k's first sum
-  int turn = 0;
-  auto warp_total = [&](double v) {
-#pragma unroll
-    for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
-    return v;
+  // ---- 2. Warp 0: the first draft that is not accepted, from `pos` on.
+  // verdict: 0 none (pos = n), 1 rejected, 2 too close for f32 sums, 3 cannot be decided
+  int pos = 0, verdict = 0;
+  // whether a row's numbers are those of a distribution
+  auto usable = [&](int r) {
+    if (MODE == kProbs) return true;
+    const float2 st = row_stat[r];
+    return MODE == kGreedy ? st.x > -INFINITY
+                           : st.y > 0.f && st.y < INFINITY && st.x > -INFINITY;
   };
-  auto cluster_sums = [&](double& v0, double& v1) -> double {
-    v0 = warp_total(v0);
-    v1 = warp_total(v1);
-    __syncthreads();  // the warps' sums before have been read
-    if (lane == 0) {
-      sums[0][warp] = v0;
-      sums[1][warp] = v1;
-    }
-    __syncthreads();
-    if (warp < 2) {
-      const double s = warp_total(lane < kVerifyWarps ? sums[warp][lane] : 0.0);
-      if (lane == 0) share[turn][warp] = s;
-    }
-    cluster_sync();
-    const double p0 = lane < ctas ? ld_cluster_f64(&share[turn][0], lane) : 0.0;
-    const double p1 = lane < ctas ? ld_cluster_f64(&share[turn][1], lane) : 0.0;
-    v0 = warp_total(p0);
-    v1 = warp_total(p1);
-    turn ^= 1;  // the other pair next: this one is read until the next barrier
-    return p0;
-  };
-  // this CTA's ids, and this warp's of them
-  const int lo = static_cast<int>(static_cast<long long>(V) * rank / ctas);
-  const int hi = static_cast<int>(static_cast<long long>(V) * (rank + 1) / ctas);
-  auto warp_part = [&](int from, int to, int w) {
-    return from + static_cast<int>(static_cast<long long>(to - from) * w / kVerifyWarps);
-  };
-  const Exp64 ex(greedy ? 1.0 : a.inv_t);
-  // Weights of a row at four ids of a lane (their loads, and then the steps of four
-  // exponentials, in flight together); whole warps.
-  auto weights = [&](const void* base, const Row& r, const int (&i)[4], double (&w)[4]) {
-    float x[4];
-#pragma unroll
-    for (int e = 0; e < 4; ++e) x[e] = ql::load_elem(base, r.at + i[e], DT);
-#pragma unroll
-    for (int e = 0; e < 4; ++e)
-      w[e] = a.probs ? static_cast<double>(x[e]) : ex(static_cast<double>(x[e]) - r.m);
-  };
-  // add(ids, of) over this warp's part of [from, to), 128 ids at a time; ids past the
-  // part repeat its last, and `of` says how many of the lane's four are inside
-  auto each = [&](int from, int to, auto add) {
-    const int f = warp_part(from, to, warp), e = warp_part(from, to, warp + 1);
-    for (int i0 = f + lane; i0 - lane < e; i0 += 128) {
-      const int i[4] = {min(i0, e - 1), min(i0 + 32, e - 1), min(i0 + 64, e - 1),
-                        min(i0 + 96, e - 1)};
-      add(i, i0 < e ? min(4, (e - i0 + 31) / 32) : 0);
-    }
-  };
-  auto exact_sums = [&](Row& p, Row& q, bool with_q) {
-    if (a.probs) {
-      p.z = q.z = 1.0;
-      return;
-    }
-    double sp = 0, sq = 0;
-    each(lo, hi, [&](const int(&i)[4], int of) {
-      double w[4];
-      weights(a.target, p, i, w);
-#pragma unroll
-      for (int e = 0; e < 4; ++e) sp += e < of ? w[e] : 0.0;
-      if (with_q) {
-        weights(a.draft, q, i, w);
-#pragma unroll
-        for (int e = 0; e < 4; ++e) sq += e < of ? w[e] : 0.0;
-      }
-    });
-    cluster_sums(sp, sq);
-    p.z = sp;
-    q.z = sq;
-  };
-
-  // ---- 2. the first draft that is not accepted
-  // of[i]: 0 accepted, 1 rejected, 2 too close for the f32 sums, 3 cannot be decided
-  auto usable = [&](float2 st) { return st.y > 0.f && st.y < INFINITY && st.x > -INFINITY; };
-  auto decide = [&](int i, double zp, double zq, bool exact) {
-    const int x = ids[i];
-    if (x < 0 || x >= V) return 3;
-    if (greedy) {
-      const float2 st = row_stat[i];
-      if (!(st.x > -INFINITY)) return 3;
-      return __float_as_int(st.y) == x ? 0 : 1;
-    }
-    double px = ql::load_elem(a.target, target_at(i) + x, DT), qx = 1.0;
-    if (stats) {
-      if (!usable(row_stat[i]) || (has_q && !usable(row_stat[n + 1 + i]))) return 3;
-      px = exp((px - row_stat[i].x) * a.inv_t) / zp;
-    } else if (!(px < INFINITY)) {
-      return 3;
-    }
-    if (has_q) {
-      qx = ql::load_elem(a.draft, draft_at(i) + x, DT);
-      if (stats) qx = exp((qx - row_stat[n + 1 + i].x) * a.inv_t) / zq;
-      else if (!(qx < INFINITY)) return 3;
-    }
-    const double uq = u[i] * qx;
-    if (stats && !exact && fabs(uq - px) <= 0x1p-14 * px) return 2;
-    return uq < px ? 0 : 1;
-  };
-  int pos = 0, how = 0;
-  for (;;) {
-    if (warp == 0) {
-      const int i = pos + lane;
-      const int d = i < n ? decide(i, row_stat[min(i, kVerifyRows - 1)].y,
-                                   row_stat[min(n + 1 + i, kVerifyRows - 1)].y, false)
-                          : 1;
-      const unsigned stop = __ballot_sync(0xffffffffu, d != 0);
-      const int first = __ffs(stop) - 1;  // n - pos <= 31, so there is one
-      const int what = __shfl_sync(0xffffffffu, d, first);
-      if (lane == 0) {
-        pos_s = pos + first;
-        exact_s = what;
+  auto decide = [&]() {
+    const int i = pos + lane;
+    int d = i < n ? 3 : 1;
+    const int x = i < n ? ids[i] : -1;
+    if (x >= 0 && x < V && usable(i) && (!has_q || usable(n + 1 + i))) {
+      if constexpr (MODE == kGreedy) {
+        d = __float_as_int(row_stat[i].y) == x ? 0 : 1;
+      } else {
+        const float lp = ql::load_elem(row_at(i), x, DT);
+        const float lq = has_q ? ql::load_elem(row_at(n + 1 + i), x, DT) : 0.f;
+        double px = lp, qx = has_q ? lq : 1.0;
+        if constexpr (MODE == kLogits) {
+          px = exp2_fast((lp - row_stat[i].x) * c) / row_stat[i].y;
+          if (has_q) qx = exp2_fast((lq - row_stat[n + 1 + i].x) * c) / row_stat[n + 1 + i].y;
+        }
+        const double uq = u[i] * qx;
+        d = uq < px ? 0 : 1;
+        if (MODE == kLogits && !(fabs(uq - px) > 0x1p-14 * px)) d = 2;
+        if (MODE == kProbs && !(px < INFINITY && qx < INFINITY)) d = 3;
       }
     }
-    __syncthreads();
-    pos = pos_s;
-    how = pos < n ? exact_s : 0;
-    __syncthreads();
-    if (how != 2) break;
-    Row p{target_at(pos), row_stat[pos].x, 1.0};
-    Row q{has_q ? draft_at(pos) : 0, has_q ? row_stat[n + 1 + pos].x : 0.f, 1.0};
-    exact_sums(p, q, has_q);
-    how = decide(pos, p.z, q.z, true);
-    if (how != 0) break;
-    ++pos;
-  }
-  // how: 0 all accepted (pos = n), 1 rejected at pos, 3 undecidable there
-  const bool rejected = how == 1;
-  bool bad = how == 3;
-  if (stats && !bad) bad = greedy ? !(row_stat[pos].x > -INFINITY) : !usable(row_stat[pos]);
-  if (rank == 0) {
-    int32_t* tok = a.tokens + static_cast<size_t>(b) * (a.drafts + 1);
-    for (int i = tid; i <= a.drafts; i += kVerifyThreads)
-      if (i != pos || bad || greedy)
-        tok[i] = i < pos ? ids[i]
-                 : i == pos && greedy && !bad ? __float_as_int(row_stat[pos].y) : -1;
-    if (tid == 0) a.accepted[b] = pos;
-  }
-  auto raise = [&]() {
-    if (rank == 0 && tid == 0) {
+    const int k = __ffs(__ballot_sync(0xffffffffu, d != 0)) - 1;  // n - pos <= 31: there is one
+    d = __shfl_sync(0xffffffffu, d, k);
+    pos += k;
+    verdict = pos < n ? d : 0;
+    if (verdict != 3 && !usable(pos)) verdict = 3;
+  };
+  int32_t* const tok = a.tokens + static_cast<size_t>(b) * (a.drafts + 1);
+  // Everything but the new token, which is `token` if that is known already.
+  auto write = [&](bool known, int token) {
+    if (rank != 0) return;
+    for (int i = lane; i <= a.drafts; i += 32)
+      if (i != pos || known) tok[i] = i < pos ? ids[i] : i == pos ? token : -1;
+    if (lane == 0) a.accepted[b] = pos;
+  };
+  auto give_up = [&]() {
+    write(true, -1);
+    if (rank == 0 && lane == 0) {
       const bool id = pos < n && (ids[pos] < 0 || ids[pos] >= V);
       atomicOr(a.status, id ? ql::kStatusBadToken : ql::kStatusBadLogits);
     }
   };
-  if (bad || greedy) {
-    if (bad) raise();
-    cluster_sync();  // nobody leaves while its shared memory may still be read
-    return;
-  }
-
-  // ---- 3. the draw from the target's row, less the draft's after a rejection
-  Row p{target_at(pos), stats ? row_stat[pos].x : 0.f, 1.0};
-  const bool less_q = rejected && has_q;
-  Row q{less_q ? draft_at(pos) : 0, less_q && stats ? row_stat[n + 1 + pos].x : 0.f, 1.0};
-  exact_sums(p, q, less_q);
-  const double rp = 1.0 / p.z, rq = 1.0 / q.z;
-  const int out = rejected && !has_q ? ids[pos] : -1;  // a certain draft: its id is taken out
-  bool less = rejected;
-  auto left = [&](const int(&i)[4], double (&w)[4]) {  // whole warps
-    weights(a.target, p, i, w);
-    double v[4];
-    if (less && less_q) weights(a.draft, q, i, v);
+  if constexpr (MODE == kGreedy) {
+    if (warp != 0) return;
+    decide();
+    if (verdict == 3) give_up();
+    else write(true, __float_as_int(row_stat[pos].y));
+  } else {
+    // ---- 3.
+    const int lo = static_cast<int>(static_cast<long long>(V) * rank / ctas);
+    const int hi = static_cast<int>(static_cast<long long>(V) * (rank + 1) / ctas);
+    const Exp64 ex(MODE == kLogits ? a.inv_t : 1.0);
+    // warp 0's: sums of the rows at pos, the threshold, the sum before [from, to)
+    double zp = 1.0, zq = 1.0, th = 0.0, before = 0.0;
+    int turn = 0;
+    auto go = [&](int what, int from, int to, int out, double fp, double fq) {
+      if (lane == 0) next_step = {what, from, to, pos, out, fp, fq};
+    };
+    // After a verdict: a rejected draft's row is taken off the target's, both divided
+    // by their sums; without one the target's weights serve as they are.
+    auto draw = [&]() {
+      const bool less = verdict == 1;
+      go(kLeft, lo, hi, less && !has_q ? ids[pos] : -1, less && has_q ? 1.0 / zp : 1.0,
+         !less ? 0.0 : has_q ? 1.0 / zq : 1.0);
+    };
+    auto begin = [&]() {
+      decide();
+      if (verdict == 3) {
+        give_up();
+        go(kDone, 0, 0, 0, 0, 0);
+      } else if (MODE == kLogits && (verdict == 2 || (verdict == 1 && has_q))) {
+        go(kTotals, lo, hi, -1, 1.0, 0.0);
+      } else {
+        draw();
+      }
+    };
+    // Of the lanes' shares (in lane order), the first where the running sum reaches
+    // th, else the last that is not empty; `before` becomes the sum before it.
+    auto find = [&](double v) {
+      double cum = v;
+#pragma unroll 1
+      for (int o = 1; o < 32; o <<= 1) {
+        const double w = __shfl_up_sync(0xffffffffu, cum, o);
+        if (lane >= o) cum += w;
+      }
+      const unsigned some = __ballot_sync(0xffffffffu, v > 0);
+      const unsigned hit = __ballot_sync(0xffffffffu, v > 0 && before + cum >= th);
+      const int k = hit ? __ffs(hit) - 1 : some ? 31 - __clz(some) : 0;
+      before += __shfl_sync(0xffffffffu, cum - v, k);
+      return k;
+    };
+    if (warp == 0) begin();
+#pragma unroll 1
+    for (;;) {
+      __syncthreads();
+      const VerifyStep z = next_step;
+      if (z.what == kDone) break;
+      auto share = [&](int w) {
+        return z.from + static_cast<int>(static_cast<long long>(z.to - z.from) * w / kVerifyWarps);
+      };
+      // s0 = sum of max(wp fp - wq fq, 0), s1 = sum of wq, with wp, wq the weights
+      // exp((logit - maximum) / T), or the probabilities, of the rows at pos
+      const bool with_q = has_q && z.pos < n;
+      const bool narrow = z.to - z.from <= 32 && z.what == kNarrow;
+      const char* const prow = row_at(z.pos);
+      const char* const qrow = row_at(with_q ? n + 1 + z.pos : z.pos);
+      const float pm = MODE == kLogits ? row_stat[z.pos].x : 0.f;
+      const float qm = MODE == kLogits && with_q ? row_stat[n + 1 + z.pos].x : 0.f;
+      const float pl = ex.least(pm), ql_ = ex.least(qm);
+      const int f = narrow ? z.from : share(warp), e = narrow ? z.to : share(warp + 1);
+      double s0 = 0, s1 = 0;
+      constexpr int kIds = 4;  // of a lane at a time
+#pragma unroll 1
+      for (int i0 = f; i0 < e; i0 += 32 * kIds) {
+        float xp[kIds], xq[kIds];
 #pragma unroll
-    for (int e = 0; e < 4; ++e) {
-      w[e] *= rp;
-      if (less) w[e] = less_q ? w[e] - v[e] * rq : i[e] == out ? 0.0 : w[e];
-      w[e] = w[e] < 0 ? 0.0 : w[e];  // NaN stays
+        for (int k = 0; k < kIds; ++k) {
+          const int i = min(i0 + 32 * k + lane, e - 1);
+          xp[k] = ql::load_elem(prow, i, DT);
+          xq[k] = with_q ? ql::load_elem(qrow, i, DT) : i == z.out ? 3e38f : 0.f;
+        }
+#pragma unroll
+        for (int k = 0; k < kIds; ++k) {
+          double wp = xp[k], wq = xq[k];
+          if constexpr (MODE == kLogits) {
+            wp = ex(xp[k], pm, pl);
+            if (with_q) wq = ex(xq[k], qm, ql_);
+          }
+          const double w = wp * z.fp - wq * z.fq;
+          if (i0 + 32 * k + lane < e) {
+            s0 += w < 0 ? 0.0 : w;  // NaN stays
+            s1 += wq;
+          }
+        }
+      }
+      if (!narrow) {
+        s0 = warp_total(s0);
+        s1 = warp_total(s1);
+        if (lane == 0) {
+          sums[0][warp] = s0;
+          sums[1][warp] = s1;
+        }
+      }
+      __syncthreads();
+      if (warp != 0) continue;
+      // ---- warp 0: what these sums mean, and what is next
+      if (narrow) {  // at most 32 ids are left, one to a lane
+        const unsigned some = __ballot_sync(0xffffffffu, s0 > 0);
+        const int k = find(s0);
+        if (lane == 0) tok[pos] = some ? z.from + k : -1;
+        go(kDone, 0, 0, 0, 0, 0);
+        continue;
+      }
+      double c0 = lane < kVerifyWarps ? sums[0][lane] : 0.0;
+      double c1 = lane < kVerifyWarps ? sums[1][lane] : 0.0;
+      if (z.what == kNarrow) {
+        const int w = find(c0);
+        go(kNarrow, share(w), share(w + 1), z.out, z.fp, z.fq);
+        continue;
+      }
+      const double of_warp = c0;
+      c0 = warp_total(c0);
+      c1 = warp_total(c1);
+      if (z.what == kAtDraft) {  // every CTA has looked at the id itself
+        if (u[pos] * (has_q ? c1 / zq : 1.0) < c0 / zp) {
+          ++pos;
+          begin();
+        } else {
+          verdict = 1;
+          draw();
+        }
+        continue;
+      }
+      // the cluster's sums: a rank that is one exchange ahead writes the other turn's
+      if (lane == 0)
+        ql::mbar_arrive_expect_tx(&bars[1 + (turn & 1)], static_cast<uint32_t>(16 * ctas));
+      __syncwarp();
+      if (lane < ctas) {
+        const double2 v = make_double2(c0, c1);
+        ql::st_async_v4(ql::mapa_shared(ql::smem_u32(&sums_of[turn & 1][rank]), lane),
+                        *reinterpret_cast<const float4*>(&v),
+                        ql::mapa_shared(ql::smem_u32(&bars[1 + (turn & 1)]), lane));
+      }
+      ql::mbar_wait_cluster(&bars[1 + (turn & 1)], turn >> 1 & 1, a.status);
+      const double2 of =
+          lane < ctas ? *reinterpret_cast<const double2*>(&sums_of[turn & 1][lane])
+                      : make_double2(0.0, 0.0);
+      ++turn;
+      const double t0 = warp_total(of.x);
+      if (z.what == kTotals) {
+        zp = t0;
+        zq = warp_total(of.y);
+        if (verdict == 2) go(kAtDraft, ids[pos], ids[pos] + 1, -1, 1.0, 0.0);
+        else draw();
+        continue;
+      }
+      if (t0 <= 0 && z.fq != 0) {  // nothing left of the difference: the target itself
+        go(kLeft, lo, hi, -1, z.fp, 0.0);
+        continue;
+      }
+      if (!(t0 > 0 && t0 < INFINITY)) {  // probabilities that are none
+        give_up();
+        go(kDone, 0, 0, 0, 0, 0);
+        continue;
+      }
+      th = u[n] * t0;
+      write(false, 0);
+      if (find(of.x) == rank) {
+        const int w = find(of_warp);
+        go(kNarrow, share(w), share(w + 1), z.out, z.fp, z.fq);
+      } else {
+        go(kDone, 0, 0, 0, 0, 0);
+      }
     }
-  };
-  // this lane's sum over its warp's part of [from, to)
-  auto part_sum = [&](int from, int to) {
-    double s = 0;
-    each(from, to, [&](const int(&i)[4], int of) {
-      double w[4];
-      left(i, w);
-#pragma unroll
-      for (int e = 0; e < 4; ++e) s += e < of ? w[e] : 0.0;
-    });
-    return s;
-  };
-  double total = part_sum(lo, hi), unused = 0;
-  double of_cta = cluster_sums(total, unused);
-  if (less && total <= 0) {  // nothing left of the difference: the target itself
-    less = false;
-    total = part_sum(lo, hi);
-    unused = 0;
-    of_cta = cluster_sums(total, unused);
-  }
-  if (!(total > 0 && total < INFINITY)) {  // probabilities that are none
-    raise();
-    if (rank == 0 && tid == 0) a.tokens[static_cast<size_t>(b) * (a.drafts + 1) + pos] = -1;
-    cluster_sync();
-    return;
-  }
-  const double th = u[n] * total;
-  // Of the lanes' shares (in lane order), the first where the running sum reaches
-  // th, else the last that is not empty; `before` becomes the sum before it.
-  auto find = [&](double v, double& before) {
-    double cum = v;
-#pragma unroll
-    for (int o = 1; o < 32; o <<= 1) {
-      const double w = __shfl_up_sync(0xffffffffu, cum, o);
-      if (lane >= o) cum += w;
-    }
-    const unsigned some = __ballot_sync(0xffffffffu, v > 0);
-    const unsigned hit = __ballot_sync(0xffffffffu, v > 0 && before + cum >= th);
-    const int k = hit ? __ffs(hit) - 1 : some ? 31 - __clz(some) : 0;
-    before += __shfl_sync(0xffffffffu, cum - v, k);
-    return k;
-  };
-  double before = 0;
-  const int owner = find(of_cta, before);
-  cluster_sync();
-  if (owner != rank) return;
-  // sums[0] holds this CTA's warps' sums of the last part_sum
-  int from = lo, to = hi;
-  for (;;) {
-    const int w = find(lane < kVerifyWarps ? sums[0][lane] : 0.0, before);
-    const int f = warp_part(from, to, w), e = warp_part(from, to, w + 1);
-    from = f;
-    to = e;
-    if (to - from <= 32) break;
-    const double s = warp_total(part_sum(from, to));
-    __syncthreads();
-    if (lane == 0) sums[0][warp] = s;
-    __syncthreads();
-  }
-  if (warp == 0) {
-    const int at = min(min(from + lane, max(to - 1, from)), V - 1);
-    const int i[4] = {at, at, at, at};
-    double w[4];
-    left(i, w);
-    const double v = from + lane < to ? w[0] : 0.0;
-    const unsigned some = __ballot_sync(0xffffffffu, v > 0);
-    const int k = find(v, before);
-    if (lane == 0)
-      a.tokens[static_cast<size_t>(b) * (a.drafts + 1) + pos] = some ? from + k : -1;
   }
 }
 
-// CTAs of a cluster: up to 16 while the clusters together have an SM for each CTA, and
-// a CTA has 1024 ids or more of its rows.
+// CTAs of a cluster: up to 16 while all CTAs run at once (four to an SM), and a CTA has
+// 1024 ids or more of its rows.
 int cluster_ctas(int batch, int vocab, int num_sms) {
   int c = kMaxCluster;
-  while (c > 1 && (static_cast<long long>(batch) * c > num_sms || vocab / c < 1024)) c /= 2;
+  while (c > 1 && (static_cast<long long>(batch) * c > 4LL * num_sms || vocab / c < 1024)) c /= 2;
   return c;
 }
 
-template <int DT>
-cudaError_t launch_verify(const VerifyArgs& a, int batch, int num_sms, cudaStream_t s) {
+template <int DT, int MODE>
+cudaError_t launch_verify_as(const VerifyArgs& a, int batch, int num_sms, cudaStream_t s) {
   const int ctas = cluster_ctas(batch, a.vocab, num_sms);
   cudaError_t e = cudaSuccess;
   if (ctas > 8)
-    e = cudaFuncSetAttribute(verify_kernel<DT>, cudaFuncAttributeNonPortableClusterSizeAllowed, 1);
+    e = cudaFuncSetAttribute(verify_kernel<DT, MODE>,
+                             cudaFuncAttributeNonPortableClusterSizeAllowed, 1);
   if (e != cudaSuccess) return e;
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3(static_cast<unsigned>(batch) * ctas);
@@ -590,7 +568,14 @@ cudaError_t launch_verify(const VerifyArgs& a, int batch, int num_sms, cudaStrea
   attr[1].val.clusterDim.z = 1;
   cfg.attrs = attr;
   cfg.numAttrs = 2;
-  return cudaLaunchKernelEx(&cfg, verify_kernel<DT>, a);
+  return cudaLaunchKernelEx(&cfg, verify_kernel<DT, MODE>, a);
+}
+
+template <int DT>
+cudaError_t launch_verify(const VerifyArgs& a, int batch, int num_sms, cudaStream_t s) {
+  if (a.probs) return launch_verify_as<DT, kProbs>(a, batch, num_sms, s);
+  return a.inv_t == 0 ? launch_verify_as<DT, kGreedy>(a, batch, num_sms, s)
+                      : launch_verify_as<DT, kLogits>(a, batch, num_sms, s);
 }
 
 }  // namespace
