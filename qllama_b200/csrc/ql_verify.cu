@@ -2,6 +2,7 @@
 // sampling's acceptance and the draw of the next token, beside ql_sample.
 #include <cuda_runtime.h>
 
+#include <algorithm>
 #include <climits>
 #include <cmath>
 
@@ -30,6 +31,9 @@ struct VerifyArgs {
   int64_t target_stride, draft_stride;
   int drafts, vocab, dtype, probs;
   double inv_t;  // 1 / temperature; 0: greedy
+  double exp_scale;  // 32 / (T ln2)
+  float exp_span;    // (x - m) / T is taken as -infinity below -690
+  float exp2_scale;  // 1 / (T ln2)
 };
 
 // One cluster of CTAs per sequence, each CTA with its share of every row.
@@ -52,8 +56,6 @@ struct VerifyArgs {
 // every warp's work, one loop for all of them, and warp 0 alone decides what is next.
 // Greedy, logits and probabilities are kernels of their own, and rows are read in
 // whole aligned groups with the odd ends on the side.
-constexpr int kVerifyThreads = 256;
-constexpr int kVerifyWarps = kVerifyThreads / 32;
 constexpr int kVerifyRows = 2 * QL_VERIFY_MAX_DRAFTS + 1;
 constexpr int kMaxCluster = 16;
 
@@ -72,6 +74,11 @@ __device__ __forceinline__ float exp2_fast(float x) {
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
   return y;
 }
+__device__ __forceinline__ float warp_max(float v) {  // NaN only of NaNs
+  float m;
+  asm("redux.sync.max.f32 %0, %1, 0xffffffff;" : "=f"(m) : "f"(v));
+  return m;
+}
 __device__ __forceinline__ double warp_total(double v) {
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
@@ -85,12 +92,6 @@ __device__ __forceinline__ double warp_total(double v) {
 struct Exp64 {
   double table, scale;
   float span;
-  __device__ explicit Exp64(double inv_t) {
-    constexpr double ln2 = 0.693147180559945309417232;
-    table = exp2(static_cast<double>(threadIdx.x & 31) / 32.0);
-    scale = inv_t * (32.0 / ln2);
-    span = static_cast<float>(fmin(690.0 / inv_t, 3e38));
-  }
   // Below it an exponential (under 1e-299) is taken as 0.
   __device__ __forceinline__ float least(float m) const { return m - span; }
   __device__ __forceinline__ double operator()(float x, double m, float least) const {
@@ -129,8 +130,10 @@ struct VerifyStep {
 };
 enum : int { kTotals = 0, kAtDraft = 1, kLeft = 2, kNarrow = 3, kDone = 4 };
 
-template <int DT, int MODE>
-__global__ void __launch_bounds__(kVerifyThreads, 4) verify_kernel(const VerifyArgs a) {
+// T threads: 1024 where a cluster's CTAs have an SM each, 256 where four share one.
+template <int DT, int MODE, int T>
+__global__ void __launch_bounds__(T, 1024 / T) verify_kernel(const VerifyArgs a) {
+  constexpr int kVerifyThreads = T, kVerifyWarps = T / 32;
   constexpr int kN = DT == ql::kF32 ? 4 : 8;  // elements of a 16-byte group
   constexpr int kLoads = 4;                   // groups of a lane in a piece
   constexpr uint32_t kNone = DT == ql::kF32 ? 0xff800000u : DT == ql::kF16 ? 0xfc00fc00u : 0xff80ff80u;
@@ -141,6 +144,9 @@ __global__ void __launch_bounds__(kVerifyThreads, 4) verify_kernel(const VerifyA
   __shared__ __align__(16) float4 sums_of[2][kMaxCluster];  // two f64 of each CTA (two turns)
   __shared__ VerifyStep next_step;
   __shared__ __align__(8) uint64_t bars[3];
+  __shared__ double pow2_32[32];                         // 2^(j/32)
+  __shared__ int32_t id_of[QL_VERIFY_MAX_DRAFTS + 1];    // the drafts
+  __shared__ double u_of[QL_VERIFY_MAX_DRAFTS + 1];
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, V = a.vocab;
   const int rank = static_cast<int>(cluster_rank()), ctas = static_cast<int>(cluster_size());
   const int b = blockIdx.x / ctas;
@@ -148,13 +154,15 @@ __global__ void __launch_bounds__(kVerifyThreads, 4) verify_kernel(const VerifyA
     for (uint64_t& bar : bars) ql::mbar_init(&bar, 1);
     ql::fence_mbar_init();
   }
+  if (MODE == kLogits && warp == 1) pow2_32[lane] = exp2(lane / 32.0);
   __syncthreads();
   ql::cluster_arrive_relaxed();
+  ql::cluster_wait();  // every CTA's barriers are there
   ql::griddep_wait();
   ql::griddep_launch_dependents();
   const int n = a.n_draft ? min(max(a.n_draft[b], 0), a.drafts) : a.drafts;
-  const int32_t* ids = a.ids + static_cast<size_t>(b) * a.drafts;
-  const double* u = a.uniforms + static_cast<size_t>(b) * (a.drafts + 1);
+  const int32_t* const ids = id_of;
+  const double* const u = u_of;
   const bool has_q = MODE != kGreedy && a.draft != nullptr;
   // Row r: 0 .. n the target's, n + 1 .. 2n the draft's.
   constexpr size_t kBytes = DT == ql::kF32 ? 4 : 2;
@@ -164,8 +172,21 @@ __global__ void __launch_bounds__(kVerifyThreads, 4) verify_kernel(const VerifyA
                   : static_cast<const char*>(a.draft) +
                         (static_cast<size_t>(b) * a.drafts + r - n - 1) * a.draft_stride * kBytes;
   };
+  // Warp 0's lane i: the logits (probabilities) of draft i, ready when the rows' sums are.
+  float drafted_p = 0.f, drafted_q = 0.f;
+  if (warp == 0) {
+    const int x = lane < n ? a.ids[static_cast<size_t>(b) * a.drafts + lane] : -1;
+    if (lane < n) id_of[lane] = x;
+    if (MODE != kGreedy && lane <= n)
+      u_of[lane] = a.uniforms[static_cast<size_t>(b) * (a.drafts + 1) + lane];
+    if (MODE != kGreedy && x >= 0 && x < V) {
+      drafted_p = ql::load_elem(row_at(lane), x, DT);
+      if (has_q) drafted_q = ql::load_elem(row_at(n + 1 + lane), x, DT);
+    }
+    __syncwarp();
+  }
   // ---- 1.
-  const float c = static_cast<float>(fmin(a.inv_t * 1.4426950408889634, 3e38));
+  const float c = a.exp2_scale;
   if constexpr (MODE != kProbs) {
     const int nrows = n + 1 + (has_q ? n : 0);
     const float2 none = make_float2(-INFINITY, MODE == kGreedy ? __int_as_float(INT_MAX) : 0.f);
@@ -249,21 +270,13 @@ __global__ void __launch_bounds__(kVerifyThreads, 4) verify_kernel(const VerifyA
       } while (it < end && row == at);
       // this warp's part of the row
       if constexpr (MODE == kGreedy) {
-#pragma unroll
-        for (int o = 16; o > 0; o >>= 1) {
-          const float m2 = __shfl_xor_sync(0xffffffffu, m, o);
-          const int b2 = __shfl_xor_sync(0xffffffffu, best, o);
-          if (m2 > m || (m2 == m && b2 < best)) {
-            m = m2;
-            best = b2;
-          }
-        }
+        const float top = warp_max(m);
+        best = __reduce_min_sync(0xffffffffu, m == top ? best : INT_MAX);
+        m = top;
         if (__any_sync(0xffffffffu, bad)) m = NAN;
         if (lane == 0) part[at][warp] = make_float2(m, __int_as_float(best));
       } else {
-        float top = m;
-#pragma unroll
-        for (int o = 16; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
+        const float top = warp_max(m);
         s *= m == top ? 1.f : m == -INFINITY ? 0.f * s : exp2_fast((m - top) * c);
 #pragma unroll
         for (int o = 16; o > 0; o >>= 1) s += __shfl_xor_sync(0xffffffffu, s, o);
@@ -274,7 +287,6 @@ __global__ void __launch_bounds__(kVerifyThreads, 4) verify_kernel(const VerifyA
     // the CTA's warps, told to every CTA, then of the CTAs
     if (tid == 0) ql::mbar_arrive_expect_tx(&bars[0], static_cast<uint32_t>(nrows * ctas * 8));
     __syncthreads();
-    ql::cluster_wait();  // every CTA's barriers are there
 #pragma unroll 1
     for (int turn = 0; turn < 2; ++turn) {
       if (turn == 1) ql::mbar_wait_cluster(&bars[0], 0, a.status);
@@ -283,20 +295,17 @@ __global__ void __launch_bounds__(kVerifyThreads, 4) verify_kernel(const VerifyA
         float2 z = none;
         if (turn == 0 && lane < kVerifyWarps) z = part[r][lane];
         if (turn == 1 && lane < ctas) z = from_cta[r][lane];
-#pragma unroll 1
-        for (int o = 8; o > 0; o >>= 1) {
-          const float2 v = make_float2(__shfl_xor_sync(0xffffffffu, z.x, o),
-                                       __shfl_xor_sync(0xffffffffu, z.y, o));
-          if constexpr (MODE == kGreedy) {  // a NaN marks the row
-            if (z.x == z.x && (v.x != v.x || v.x > z.x ||
-                               (v.x == z.x && __float_as_int(v.y) < __float_as_int(z.y))))
-              z = v;
-          } else {  // sums under a maximum of -inf are zeros, or a NaN that marks the row
-            const float top = fmaxf(z.x, v.x);
-            const float f = z.x == top ? 1.f : z.x == -INFINITY ? 0.f : exp2_fast((z.x - top) * c);
-            const float h = v.x == top ? 1.f : v.x == -INFINITY ? 0.f : exp2_fast((v.x - top) * c);
-            z = make_float2(top, z.y * f + v.y * h);
-          }
+        if constexpr (MODE == kGreedy) {  // a NaN marks the row
+          const bool bad = __any_sync(0xffffffffu, z.x != z.x);
+          const float top = warp_max(z.x);
+          const int id = __reduce_min_sync(0xffffffffu, z.x == top ? __float_as_int(z.y) : INT_MAX);
+          z = make_float2(bad ? NAN : top, __int_as_float(id));
+        } else {  // sums under a maximum of -inf are zeros, or a NaN that marks the row
+          const float top = warp_max(z.x);
+          float s = z.x == top ? z.y : z.x == -INFINITY ? 0.f * z.y : z.y * exp2_fast((z.x - top) * c);
+#pragma unroll
+          for (int o = 16; o > 0; o >>= 1) s += __shfl_xor_sync(0xffffffffu, s, o);
+          z = make_float2(top, s);
         }
         if (turn == 0) {
           if (lane < ctas)
@@ -308,8 +317,6 @@ __global__ void __launch_bounds__(kVerifyThreads, 4) verify_kernel(const VerifyA
       }
     }
     __syncthreads();
-  } else {
-    ql::cluster_wait();
   }
 
   // ---- 2. Warp 0: the first draft that is not accepted, from `pos` on.
@@ -323,15 +330,14 @@ __global__ void __launch_bounds__(kVerifyThreads, 4) verify_kernel(const VerifyA
                            : st.y > 0.f && st.y < INFINITY && st.x > -INFINITY;
   };
   auto decide = [&]() {
-    const int i = pos + lane;
-    int d = i < n ? 3 : 1;
-    const int x = i < n ? ids[i] : -1;
+    const int i = lane;  // drafts before pos are accepted already
+    int d = i < pos ? 0 : i < n ? 3 : 1;
+    const int x = i >= pos && i < n ? ids[i] : -1;
     if (x >= 0 && x < V && usable(i) && (!has_q || usable(n + 1 + i))) {
       if constexpr (MODE == kGreedy) {
         d = __float_as_int(row_stat[i].y) == x ? 0 : 1;
       } else {
-        const float lp = ql::load_elem(row_at(i), x, DT);
-        const float lq = has_q ? ql::load_elem(row_at(n + 1 + i), x, DT) : 0.f;
+        const float lp = drafted_p, lq = drafted_q;
         double px = lp, qx = has_q ? lq : 1.0;
         if constexpr (MODE == kLogits) {
           px = exp2_fast((lp - row_stat[i].x) * c) / row_stat[i].y;
@@ -343,9 +349,8 @@ __global__ void __launch_bounds__(kVerifyThreads, 4) verify_kernel(const VerifyA
         if (MODE == kProbs && !(px < INFINITY && qx < INFINITY)) d = 3;
       }
     }
-    const int k = __ffs(__ballot_sync(0xffffffffu, d != 0)) - 1;  // n - pos <= 31: there is one
-    d = __shfl_sync(0xffffffffu, d, k);
-    pos += k;
+    pos = __ffs(__ballot_sync(0xffffffffu, d != 0)) - 1;  // n <= 31: lane n has one
+    d = __shfl_sync(0xffffffffu, d, pos);
     verdict = pos < n ? d : 0;
     if (verdict != 3 && !usable(pos)) verdict = 3;
   };
@@ -373,7 +378,7 @@ __global__ void __launch_bounds__(kVerifyThreads, 4) verify_kernel(const VerifyA
     // ---- 3.
     const int lo = static_cast<int>(static_cast<long long>(V) * rank / ctas);
     const int hi = static_cast<int>(static_cast<long long>(V) * (rank + 1) / ctas);
-    const Exp64 ex(MODE == kLogits ? a.inv_t : 1.0);
+    const Exp64 ex{pow2_32[lane], a.exp_scale, a.exp_span};
     // warp 0's: sums of the rows at pos, the threshold, the sum before [from, to)
     double zp = 1.0, zq = 1.0, th = 0.0, before = 0.0;
     int turn = 0;
@@ -385,7 +390,7 @@ __global__ void __launch_bounds__(kVerifyThreads, 4) verify_kernel(const VerifyA
     auto draw = [&]() {
       const bool less = verdict == 1;
       go(kLeft, lo, hi, less && !has_q ? ids[pos] : -1, less && has_q ? 1.0 / zp : 1.0,
-         !less ? 0.0 : has_q ? 1.0 / zq : 1.0);
+         less && has_q ? 1.0 / zq : 0.0);
     };
     auto begin = [&]() {
       decide();
@@ -433,29 +438,35 @@ __global__ void __launch_bounds__(kVerifyThreads, 4) verify_kernel(const VerifyA
       const float pl = ex.least(pm), ql_ = ex.least(qm);
       const int f = narrow ? z.from : share(warp), e = narrow ? z.to : share(warp + 1);
       double s0 = 0, s1 = 0;
-      constexpr int kIds = 4;  // of a lane at a time
+      constexpr int kIds = 4;  // of a lane at a time, their loads in flight together
+      constexpr float kEmpty = MODE == kLogits ? -INFINITY : 0.f;
 #pragma unroll 1
-      for (int i0 = f; i0 < e; i0 += 32 * kIds) {
+      for (int i0 = f + lane; i0 - lane < e; i0 += 32 * kIds) {
         float xp[kIds], xq[kIds];
 #pragma unroll
-        for (int k = 0; k < kIds; ++k) {
-          const int i = min(i0 + 32 * k + lane, e - 1);
-          xp[k] = ql::load_elem(prow, i, DT);
-          xq[k] = with_q ? ql::load_elem(qrow, i, DT) : i == z.out ? 3e38f : 0.f;
+        for (int k = 0; k < kIds; ++k) xp[k] = ql::load_elem(prow, min(i0 + 32 * k, e - 1), DT);
+        if (with_q) {
+#pragma unroll
+          for (int k = 0; k < kIds; ++k) xq[k] = ql::load_elem(qrow, min(i0 + 32 * k, e - 1), DT);
         }
+        double w[kIds];
 #pragma unroll
         for (int k = 0; k < kIds; ++k) {
-          double wp = xp[k], wq = xq[k];
-          if constexpr (MODE == kLogits) {
-            wp = ex(xp[k], pm, pl);
-            if (with_q) wq = ex(xq[k], qm, ql_);
-          }
-          const double w = wp * z.fp - wq * z.fq;
-          if (i0 + 32 * k + lane < e) {
-            s0 += w < 0 ? 0.0 : w;  // NaN stays
+          const float x = i0 + 32 * k < e ? xp[k] : kEmpty;
+          w[k] = z.fp * (MODE == kLogits ? ex(x, pm, pl) : static_cast<double>(x));
+        }
+        if (with_q) {
+#pragma unroll
+          for (int k = 0; k < kIds; ++k) {
+            const float x = i0 + 32 * k < e ? xq[k] : kEmpty;
+            const double wq = MODE == kLogits ? ex(x, qm, ql_) : static_cast<double>(x);
             s1 += wq;
+            w[k] = fma(-wq, z.fq, w[k]);
           }
         }
+#pragma unroll
+        for (int k = 0; k < kIds; ++k)  // NaN stays
+          s0 += w[k] < 0 || i0 + 32 * k == z.out ? 0.0 : w[k];
       }
       if (!narrow) {
         s0 = warp_total(s0);
@@ -518,7 +529,7 @@ __global__ void __launch_bounds__(kVerifyThreads, 4) verify_kernel(const VerifyA
         else draw();
         continue;
       }
-      if (t0 <= 0 && z.fq != 0) {  // nothing left of the difference: the target itself
+      if (t0 <= 0 && (z.fq != 0 || z.out >= 0)) {  // nothing left: the target itself
         go(kLeft, lo, hi, -1, z.fp, 0.0);
         continue;
       }
@@ -539,25 +550,30 @@ __global__ void __launch_bounds__(kVerifyThreads, 4) verify_kernel(const VerifyA
   }
 }
 
-// CTAs of a cluster: up to 16 while all CTAs run at once (four to an SM), and a CTA has
-// 1024 ids or more of its rows.
+// CTAs of a cluster: up to 16, in powers of two, with an equal share of the GPU's
+// places (four CTAs to an SM) for every sequence; 1024 ids or more each, or 4096 when
+// most of the places are taken and the CTAs slow one another down (32 sequences, one
+// row of 32000: 12.8 us with 8, 16.3 us with 16; 8 sequences: 21.5 us and 17.2 us).
 int cluster_ctas(int batch, int vocab, int num_sms) {
   int c = kMaxCluster;
-  while (c > 1 && (static_cast<long long>(batch) * c > 4LL * num_sms || vocab / c < 1024)) c /= 2;
+  while (c > 1) {
+    const long long all = static_cast<long long>(batch) * c;
+    if (all <= 4LL * num_sms && vocab / c >= (all > 2LL * num_sms ? 4096 : 1024)) break;
+    c /= 2;
+  }
   return c;
 }
 
-template <int DT, int MODE>
-cudaError_t launch_verify_as(const VerifyArgs& a, int batch, int num_sms, cudaStream_t s) {
-  const int ctas = cluster_ctas(batch, a.vocab, num_sms);
+template <int DT, int MODE, int T>
+cudaError_t launch_verify_as(const VerifyArgs& a, int batch, int ctas, cudaStream_t s) {
   cudaError_t e = cudaSuccess;
   if (ctas > 8)
-    e = cudaFuncSetAttribute(verify_kernel<DT, MODE>,
+    e = cudaFuncSetAttribute(verify_kernel<DT, MODE, T>,
                              cudaFuncAttributeNonPortableClusterSizeAllowed, 1);
   if (e != cudaSuccess) return e;
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3(static_cast<unsigned>(batch) * ctas);
-  cfg.blockDim = dim3(kVerifyThreads);
+  cfg.blockDim = dim3(T);
   cfg.stream = s;
   cudaLaunchAttribute attr[2];
   attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
@@ -568,14 +584,24 @@ cudaError_t launch_verify_as(const VerifyArgs& a, int batch, int num_sms, cudaSt
   attr[1].val.clusterDim.z = 1;
   cfg.attrs = attr;
   cfg.numAttrs = 2;
-  return cudaLaunchKernelEx(&cfg, verify_kernel<DT, MODE>, a);
+  return cudaLaunchKernelEx(&cfg, verify_kernel<DT, MODE, T>, a);
+}
+
+template <int DT, int MODE>
+cudaError_t launch_verify_mode(const VerifyArgs& a, int batch, int num_sms, cudaStream_t s) {
+  const int ctas = cluster_ctas(batch, a.vocab, num_sms);
+  // a few clusters with long shares: four times the warps (one sequence of 8 rows of
+  // 128000 f32 28.7 us, 35.2 us with 256 threads; of 5 rows of 32000 19.8 us and 15.6 us)
+  return batch * ctas <= num_sms / 2 && a.vocab / ctas >= 4096
+             ? launch_verify_as<DT, MODE, 1024>(a, batch, ctas, s)
+             : launch_verify_as<DT, MODE, 256>(a, batch, ctas, s);
 }
 
 template <int DT>
 cudaError_t launch_verify(const VerifyArgs& a, int batch, int num_sms, cudaStream_t s) {
-  if (a.probs) return launch_verify_as<DT, kProbs>(a, batch, num_sms, s);
-  return a.inv_t == 0 ? launch_verify_as<DT, kGreedy>(a, batch, num_sms, s)
-                      : launch_verify_as<DT, kLogits>(a, batch, num_sms, s);
+  if (a.probs) return launch_verify_mode<DT, kProbs>(a, batch, num_sms, s);
+  return a.inv_t == 0 ? launch_verify_mode<DT, kGreedy>(a, batch, num_sms, s)
+                      : launch_verify_mode<DT, kLogits>(a, batch, num_sms, s);
 }
 
 }  // namespace
@@ -630,6 +656,9 @@ extern "C" int ql_verify_drafts(ql_ctx* c, const ql_verify_args* args) {
   a.dtype = f.dtype;
   a.probs = probs;
   a.inv_t = probs ? 1.0 : greedy ? 0.0 : 1.0 / static_cast<double>(f.temperature);
+  a.exp_scale = a.inv_t * (32.0 / 0.693147180559945309417232);
+  a.exp_span = static_cast<float>(std::fmin(690.0 / a.inv_t, 3e38));
+  a.exp2_scale = static_cast<float>(std::fmin(a.inv_t / 0.693147180559945309417232, 3e38));
   cudaError_t e;
   if (f.dtype == QL_F32) e = launch_verify<ql::kF32>(a, f.batch, c->num_sms, c->stream);
   else if (f.dtype == QL_F16) e = launch_verify<ql::kF16>(a, f.batch, c->num_sms, c->stream);
