@@ -6,6 +6,8 @@
 #include <stddef.h>
 #include <stdint.h>
 
+#include <atomic>
+
 struct ql_ctx {
   int device = 0;
   int num_sms = 0;
@@ -49,3 +51,17 @@ class ql_device_guard {
   bool moved_ = false;
   cudaError_t err_ = cudaSuccess;
 };
+
+// Runs `set` once for each device (kernel attributes belong to a device's context).
+// Two first calls at once both run it, with the same effect.
+template <typename F>
+cudaError_t ql_once_per_device(std::atomic<uint64_t>& done, F set) {
+  int device = 0;
+  cudaError_t e = cudaGetDevice(&device);
+  if (e != cudaSuccess) return e;
+  const uint64_t bit = 1ull << (device & 63);
+  if (device < 64 && (done.load(std::memory_order_acquire) & bit)) return cudaSuccess;
+  e = set();
+  if (e == cudaSuccess && device < 64) done.fetch_or(bit, std::memory_order_release);
+  return e;
+}

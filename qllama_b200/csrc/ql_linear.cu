@@ -1083,8 +1083,10 @@ cudaError_t launch_linear_as(const LinearArgs& a, int num_sms, bool pdl, cudaStr
   using C = LinCfg<IN, NT, MT, WR, G>;
   static_assert(C::kSmem <= 227 * 1024, "shared memory");
   auto* const kernel = linear_q4_kernel<IN, NT, MT, WR, G>;
-  cudaError_t e =
-      cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, C::kSmem);
+  static std::atomic<uint64_t> done{0};
+  cudaError_t e = ql_once_per_device(done, [&] {
+    return cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, C::kSmem);
+  });
   for (int r = 0; e == cudaSuccess && r < a.rows; r += 65535 * C::kRows) {  // grid.y's limit
     LinearArgs b = a;
     b.rows = std::min(a.rows - r, 65535 * C::kRows);

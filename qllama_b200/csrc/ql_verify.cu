@@ -566,10 +566,11 @@ int cluster_ctas(int batch, int vocab, int num_sms) {
 
 template <int DT, int MODE, int T>
 cudaError_t launch_verify_as(const VerifyArgs& a, int batch, int ctas, cudaStream_t s) {
-  cudaError_t e = cudaSuccess;
-  if (ctas > 8)
-    e = cudaFuncSetAttribute(verify_kernel<DT, MODE, T>,
-                             cudaFuncAttributeNonPortableClusterSizeAllowed, 1);
+  static std::atomic<uint64_t> done{0};
+  const cudaError_t e = ql_once_per_device(done, [] {
+    return cudaFuncSetAttribute(verify_kernel<DT, MODE, T>,
+                                cudaFuncAttributeNonPortableClusterSizeAllowed, 1);
+  });
   if (e != cudaSuccess) return e;
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3(static_cast<unsigned>(batch) * ctas);

@@ -75,6 +75,7 @@ class VerifyArgs(ctypes.Structure):
 
 GREEDY = (0.0, 0, 1.0, 1.0)
 VERIFY_LOGITS, VERIFY_PROBS, VERIFY_MAX_DRAFTS = 0, 1, 31
+_Q8_0 = 3  # the package's Q8_0
 
 
 def bind(L: ctypes.CDLL) -> None:
@@ -258,16 +259,20 @@ def attention_forward_appended(kv, layer: int, q_rot, start_pos, num_heads: int,
 
 # ------------------------------------ 4-bit decode step and drafted tokens --
 
-_codes = {}  # torch dtype -> QL element type, filled at the first call
+# The calls below are a few microseconds of GPU work each, so their own path is
+# kept short: these are filled at the first call.
+_codes = {}  # torch dtype -> QL element type
+_L = None    # the library
 
 
-def _types():
-    if not _codes:
-        import torch
+def _start():
+    global _L
+    import torch
 
-        qb = _qb()
-        _codes.update({torch.float32: qb.F32, torch.float16: qb.F16, torch.bfloat16: qb.BF16})
-    return _codes
+    qb = _qb()
+    _codes.update({torch.float32: qb.F32, torch.float16: qb.F16, torch.bfloat16: qb.BF16})
+    _L = qb.load()
+    return _L
 
 
 def _invalid(message: str):
@@ -275,32 +280,32 @@ def _invalid(message: str):
     return qb.QllamaError(qb.ERR_INVALID, message)
 
 
+def _raise(rc: int):
+    raise _qb().QllamaError(rc, _L.ql_last_error().decode())
+
+
 def _float_code(t, name: str) -> int:
-    code = _types().get(t.dtype)
+    code = _codes.get(t.dtype)
     if code is None:
         raise _invalid(f"{name}: unsupported element type {t.dtype}")
     return code
 
 
-def _on(ctx, t, name: str) -> int:
+def _on(device: int, t, name: str) -> int:
     """The pointer of a tensor on the context's device."""
-    d = t.device
-    if d.type != "cuda" or d.index != ctx.device:
-        raise _invalid(f"{name} is on {d}, the context on cuda:{ctx.device}")
+    if t.get_device() != device:
+        raise _invalid(f"{name} is on {t.device}, the context on cuda:{device}")
     return t.data_ptr()
 
 
-def _rows_of(t, width: int, name: str):
-    """(rows, elements from row to row) of a tensor [..., width]: a matrix whose
-    rows are contiguous, or a contiguous tensor of any rank."""
-    shape = t.shape
-    if not shape or shape[-1] != width:
-        raise _invalid(f"{name} has shape {tuple(shape)}, its last dimension must be {width}")
-    if len(shape) == 2 and t.stride(1) == 1 and (t.stride(0) >= width or shape[0] <= 1):
-        return shape[0], (t.stride(0) if shape[0] > 1 else width)
-    if not t.is_contiguous():
-        raise _invalid(f"{name} must have contiguous rows")
-    return t.numel() // width, width
+def _stride_of(t, width: int, name: str) -> int:
+    """Elements from row to row (0: contiguous) of a tensor [..., width]: a matrix
+    whose rows are contiguous, or a contiguous tensor of any rank."""
+    if t.is_contiguous():
+        return 0
+    if t.dim() == 2 and t.stride(1) == 1 and t.stride(0) >= width:
+        return t.stride(0)
+    raise _invalid(f"{name} must have contiguous rows")
 
 
 def _output(ctx, t, shape, dtype, name: str):
@@ -309,20 +314,18 @@ def _output(ctx, t, shape, dtype, name: str):
         import torch
 
         return torch.empty(shape, dtype=dtype, device=f"cuda:{ctx.device}")
-    if tuple(t.shape) != tuple(shape) or t.dtype != dtype or not t.is_contiguous():
+    if t.shape != shape or t.dtype is not dtype or not t.is_contiguous():
         raise _invalid(f"{name} must be a contiguous {dtype} tensor of shape {tuple(shape)}")
     return t
 
 
-def _out_type(out, out_dtype, default):
+def _named_type(name: str):
     import torch
 
-    if out_dtype is None:
-        return out.dtype if out is not None else default
     named = {"f32": torch.float32, "f16": torch.float16, "bf16": torch.bfloat16}
-    if out_dtype not in named:
-        raise _invalid(f"unknown element type {out_dtype}")
-    return named[out_dtype]
+    if name not in named:
+        raise _invalid(f"unknown element type {name}")
+    return named[name]
 
 
 def rms_norm(ctx, x, weight, eps: float, residual=None, sum_out=None, out=None, scale=None,
@@ -334,43 +337,42 @@ def rms_norm(ctx, x, weight, eps: float, residual=None, sum_out=None, out=None, 
     "bf16", or "q8_0", also chosen by giving an int8 `out`.  Returns y, or for
     Q8_0 (int8 values [..., hidden], f16 scales [..., hidden / 32]).
     """
-    import torch
-
-    qb = _qb()
-    if not x.dim() or not x.shape[-1]:
+    L = _L or _start()
+    shape, dtype, dev = x.shape, x.dtype, ctx.device
+    if not shape or not shape[-1]:
         raise _invalid("x needs a last dimension to normalise")
-    hidden = x.shape[-1]
-    rows, xs = _rows_of(x, hidden, "x")
+    hidden = shape[-1]
     in_dt = _float_code(x, "x")
     if weight.shape != (hidden,) or not weight.is_contiguous():
         raise _invalid(f"weight must be contiguous [{hidden}], got {tuple(weight.shape)}")
     rs, rp, sp = 0, None, None
     if residual is not None:
-        if residual.shape != x.shape or residual.dtype != x.dtype:
+        if residual.shape != shape or residual.dtype is not dtype:
             raise _invalid("residual must have x's shape and type")
-        rs = _rows_of(residual, hidden, "residual")[1]
-        rp = _on(ctx, residual, "residual")
+        rs = _stride_of(residual, hidden, "residual")
+        rp = _on(dev, residual, "residual")
     if sum_out is not None:
-        _output(ctx, sum_out, x.shape, x.dtype, "sum_out")
-        sp = _on(ctx, sum_out, "sum_out")
-    q8 = out_dtype == "q8_0" or (out_dtype is None and out is not None and out.dtype == torch.int8)
-    if q8:
+        sp = _on(dev, _output(ctx, sum_out, shape, dtype, "sum_out"), "sum_out")
+    if out_dtype == "q8_0" or scale is not None or (
+            out is not None and out_dtype is None and out.dtype not in _codes):
+        import torch
+
         if hidden % 32:
             raise _invalid(f"a Q8_0 output needs hidden divisible by 32, got {hidden}")
-        out = _output(ctx, out, x.shape, torch.int8, "out")
-        scale = _output(ctx, scale, x.shape[:-1] + (hidden // 32,), torch.float16, "scale")
-        out_dt, scp = qb.Q8_0, _on(ctx, scale, "scale")
+        out = _output(ctx, out, shape, torch.int8, "out")
+        scale = _output(ctx, scale, shape[:-1] + (hidden // 32,), torch.float16, "scale")
+        out_dt, scp = _Q8_0, _on(dev, scale, "scale")
     else:
-        if scale is not None:
-            raise _invalid("scale belongs to a Q8_0 output")
-        t = _out_type(out, out_dtype, x.dtype)
-        out = _output(ctx, out, x.shape, t, "out")
-        out_dt, scp = _float_code(out, "out"), None
-    args = NormArgs(rows, hidden, in_dt, _float_code(weight, "weight"), out_dt, eps, xs, rs,
-                    _on(ctx, x, "x"), rp, _on(ctx, weight, "weight"), sp, _on(ctx, out, "out"),
-                    scp)
-    qb._check(qb.load().ql_rms_norm(ctx._h, ctypes.byref(args)))
-    return (out, scale) if q8 else out
+        t = _named_type(out_dtype) if out_dtype else dtype if out is None else out.dtype
+        out = _output(ctx, out, shape, t, "out")
+        out_dt, scp = _codes[t], None
+    rc = L.ql_rms_norm(ctx._h, ctypes.byref(NormArgs(
+        x.numel() // hidden, hidden, in_dt, _float_code(weight, "weight"), out_dt, eps,
+        _stride_of(x, hidden, "x"), rs, _on(dev, x, "x"), rp, _on(dev, weight, "weight"), sp,
+        _on(dev, out, "out"), scp)))
+    if rc:
+        _raise(rc)
+    return out if scp is None else (out, scale)
 
 
 class Q4Weight:
@@ -406,7 +408,7 @@ class Q4Weight:
             raise _invalid("a dense weight has two dimensions")
         q = cls(ctx, shape=(int(w.shape[0]), int(w.shape[1]), group))
         p, mem, keep = q._buffer(w, None, "w")
-        stride = 0 if mem == qb.MEM_HOST else _rows_of(keep, int(w.shape[1]), "w")[1]
+        stride = 0 if mem == qb.MEM_HOST else _stride_of(keep, int(w.shape[1]), "w")
         qb._check(qb.load().ql_q4_quantize(q._h, p, qb._dtype_code(keep), stride, mem))
         return q
 
@@ -433,7 +435,7 @@ class Q4Weight:
                 return x.data_ptr(), qb.MEM_HOST, x
             if dtype and not x.is_contiguous():
                 raise _invalid(f"{name} must be contiguous")
-            return _on(self.ctx, x, name), qb.MEM_DEVICE, x
+            return _on(self.ctx.device, x, name), qb.MEM_DEVICE, x
         x = np.ascontiguousarray(x)
         return x.ctypes.data, qb.MEM_HOST, x
 
@@ -479,30 +481,43 @@ def linear_q4(weight: Q4Weight, x, x_scale=None, out=None, out_dtype: str | None
     (default: out's type, else x's, f32 for Q8_0); `out` may be a matrix with a
     row stride.
     """
-    import torch
+    L = _L or _start()
+    ctx, k, n, dtype, lead = (weight.ctx, weight.in_features, weight.out_features, x.dtype,
+                              x.shape[:-1])
+    dev = ctx.device
+    if not x.dim() or x.shape[-1] != k:
+        raise _invalid(f"x has shape {tuple(x.shape)}, its last dimension must be {k}")
+    in_dt = _codes.get(dtype)
+    if in_dt is None or x_scale is not None:
+        import torch
 
-    qb = _qb()
-    ctx, k, n = weight.ctx, weight.in_features, weight.out_features
-    rows, xs = _rows_of(x, k, "x")
-    if x.dtype == torch.int8:
+        if dtype is not torch.int8:
+            raise _invalid(f"x: unsupported element type {dtype}" if in_dt is None else
+                           "x_scale belongs to int8 x")
         if x_scale is None:
             raise _invalid("int8 x needs x_scale")
-        _output(ctx, x_scale, x.shape[:-1] + (k // 32,), torch.float16, "x_scale")
-        in_dt, scp, t = qb.Q8_0, _on(ctx, x_scale, "x_scale"), torch.float32
+        _output(ctx, x_scale, lead + (k // 32,), torch.float16, "x_scale")
+        in_dt, scp, dtype = _Q8_0, _on(dev, x_scale, "x_scale"), torch.float32
     else:
-        if x_scale is not None:
-            raise _invalid("x_scale belongs to int8 x")
-        in_dt, scp, t = _float_code(x, "x"), None, x.dtype
-    t = _out_type(out, out_dtype, t)
-    shape = x.shape[:-1] + (n,)
+        scp = None
+    if out_dtype is not None:
+        dtype = _named_type(out_dtype)
+    elif out is not None:
+        dtype = out.dtype
+    shape = lead + (n,)
     if out is None:
-        out = torch.empty(shape, dtype=t, device=x.device)
-    elif out.shape != shape or out.dtype != t:
-        raise _invalid(f"out must be {t} of shape {tuple(shape)}")
-    ys = _rows_of(out, n, "out")[1]
-    args = LinearArgs(rows, in_dt, _float_code(out, "out"), xs, ys, _on(ctx, x, "x"), scp,
-                      _on(ctx, out, "out"))
-    qb._check(qb.load().ql_linear_q4(ctx._h, weight._h, ctypes.byref(args)))
+        import torch
+
+        out, ys = torch.empty(shape, dtype=dtype, device=x.device), 0
+    else:
+        if out.shape != shape or out.dtype is not dtype:
+            raise _invalid(f"out must be {dtype} of shape {tuple(shape)}")
+        ys = _stride_of(out, n, "out")
+    rc = L.ql_linear_q4(ctx._h, weight._h, ctypes.byref(LinearArgs(
+        x.numel() // k, in_dt, _float_code(out, "out"), _stride_of(x, k, "x"), ys,
+        _on(dev, x, "x"), scp, _on(dev, out, "out"))))
+    if rc:
+        _raise(rc)
     return out
 
 
@@ -519,42 +534,47 @@ def verify_drafts(ctx, target, draft, draft_ids, uniforms, temperature: float = 
     """
     import torch
 
-    qb = _qb()
+    L = _L or _start()
+    dev, dtype = ctx.device, target.dtype
     if target.dim() != 3 or target.shape[1] < 1:
         raise _invalid("target must be [batch, drafts + 1, vocab]")
-    batch, m, vocab = target.shape[0], target.shape[1] - 1, target.shape[2]
+    batch, m, vocab = target.shape
+    m -= 1
+    dt = _float_code(target, "target")
 
     def rows(t, count, name):
-        if tuple(t.shape) != (batch, count, vocab) or t.dtype != target.dtype:
-            raise _invalid(f"{name} must be {target.dtype} [{batch}, {count}, {vocab}]")
-        if not t.numel():
-            return vocab
-        row = t.stride(1) if count > 1 else t.stride(0) if batch > 1 else vocab
-        if t.stride(2) != 1 and vocab > 1 or row < vocab or \
-                batch > 1 and t.stride(0) != count * row:
+        if t.shape != (batch, count, vocab) or t.dtype is not dtype:
+            raise _invalid(f"{name} must be {dtype} [{batch}, {count}, {vocab}]")
+        if t.is_contiguous():
+            return 0
+        row = t.stride(1) if count > 1 else t.stride(0)
+        if (t.stride(2) != 1 and vocab > 1) or row < vocab or (
+                batch > 1 and t.stride(0) != count * row):
             raise _invalid(f"{name} must have its rows at one stride")
         return row
 
-    def ints(t, shape, dtype, name):
-        if tuple(t.shape) != shape or t.dtype != dtype or not t.is_contiguous():
-            raise _invalid(f"{name} must be contiguous {dtype} {list(shape)}")
-        return _on(ctx, t, name)
+    def plain(t, shape, kind, name):
+        if t.shape != shape or t.dtype is not kind or not t.is_contiguous():
+            raise _invalid(f"{name} must be contiguous {kind} {list(shape)}")
+        return _on(dev, t, name)
 
-    ts = rows(target, m + 1, "target")
-    ds = rows(draft, m, "draft") if draft is not None else 0
-    dp = _on(ctx, draft, "draft") if draft is not None and m else None
-    ip = ints(draft_ids, (batch, m), torch.int32, "draft_ids") if m else None
-    np_ = ints(n_draft, (batch,), torch.int32, "n_draft") if n_draft is not None else None
-    up = None
+    ts, ds, dp, ip, up = rows(target, m + 1, "target"), 0, None, None, None
+    if draft is not None:
+        ds = rows(draft, m, "draft")
+        dp = _on(dev, draft, "draft") if m else None
+    if m:
+        ip = plain(draft_ids, (batch, m), torch.int32, "draft_ids")
+    np_ = plain(n_draft, (batch,), torch.int32, "n_draft") if n_draft is not None else None
     if probs or temperature > 0:
         if uniforms is None:
             raise _invalid("sampling needs uniforms")
-        up = ints(uniforms, (batch, m + 1), torch.float64, "uniforms")
+        up = plain(uniforms, (batch, m + 1), torch.float64, "uniforms")
     tokens = _output(ctx, tokens, (batch, m + 1), torch.int32, "tokens")
     accepted = _output(ctx, accepted, (batch,), torch.int32, "accepted")
-    args = VerifyArgs(batch, m, vocab, _float_code(target, "target"),
-                      VERIFY_PROBS if probs else VERIFY_LOGITS, temperature, ts, ds,
-                      _on(ctx, target, "target"), dp, ip, np_, up, _on(ctx, tokens, "tokens"),
-                      _on(ctx, accepted, "accepted"))
-    qb._check(qb.load().ql_verify_drafts(ctx._h, ctypes.byref(args)))
+    rc = L.ql_verify_drafts(ctx._h, ctypes.byref(VerifyArgs(
+        batch, m, vocab, dt, VERIFY_PROBS if probs else VERIFY_LOGITS, temperature, ts, ds,
+        _on(dev, target, "target"), dp, ip, np_, up, _on(dev, tokens, "tokens"),
+        _on(dev, accepted, "accepted"))))
+    if rc:
+        _raise(rc)
     return tokens, accepted
