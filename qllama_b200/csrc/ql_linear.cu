@@ -832,36 +832,38 @@ __global__ void __launch_bounds__(kRanges* WR * 32, 1) linear_q4_kernel(const Li
   const char* const xp = static_cast<const char*>(a.x) +
                          (static_cast<size_t>(r0 + xr) * a.x_stride + xcol) * kBytes;
   const size_t xstep = static_cast<size_t>(32 / kUnits) * a.x_stride * kBytes;
-  uint32_t xdst[kXU];
-#pragma unroll
-  for (int i = 0; i < kXU; ++i) xdst[i] = C::kX + unit_at(xr + i * (32 / kUnits), lane % kUnits);
+  // (rows 32 / kUnits apart are spread alike: their places are 512 bytes apart)
+  const uint32_t xdst = C::kX + unit_at(xr, lane % kUnits);
   // Q8_0: the scales of x's row `lane`, two of a chunk at a time
   const uint16_t* const xsp =
       reinterpret_cast<const uint16_t*>(a.x_scale) + static_cast<size_t>(r0 + lane) * (K / 32);
   const bool xs_vec = C::kQ8 && (reinterpret_cast<uintptr_t>(a.x_scale) | (K / 32 * 2)) % 4 == 0;
   auto copy_x = [&](uint32_t set, int c) {
-    const int k = 64 * c + xcol;
+    const char* const p = xp + c * (64 * kBytes);
+    if (vec && 64 * c + 64 <= K) {
 #pragma unroll
-    for (int i = 0; i < kXU; ++i) {
-      if (xr + i * (32 / kUnits) >= rows) continue;
-      const char* p = xp + i * xstep + c * (64 * kBytes);
-      if (vec) {
-        cp_cached<16>(set + xdst[i], k < K ? p : xp, k < K ? 16 : 0);
-      } else {
+      for (int i = 0; i < kXU; ++i)
+        if (xr + i * (32 / kUnits) < rows) cp_cached<16>(set + xdst + 512 * i, p + i * xstep, 16);
+    } else {  // the last half chunk, or rows that do not start on 16 bytes
+      const bool in = 64 * c + xcol < K;
+#pragma unroll 1
+      for (int i = 0; i < kXU; ++i) {
+        if (xr + i * (32 / kUnits) >= rows) break;
+        const char* const q = p + i * xstep;
         uint32_t v[4] = {0, 0, 0, 0};
-        if (k < K) {
+        if (in) {
 #pragma unroll
           for (int e = 0; e < 16 / kBytes; ++e) {
-            if constexpr (IN == ql::kF32) v[e] = reinterpret_cast<const uint32_t*>(p)[e];
+            if constexpr (IN == ql::kF32) v[e] = reinterpret_cast<const uint32_t*>(q)[e];
             else if constexpr (C::kQ8)
-              v[e / 4] |= static_cast<uint32_t>(reinterpret_cast<const uint8_t*>(p)[e])
+              v[e / 4] |= static_cast<uint32_t>(reinterpret_cast<const uint8_t*>(q)[e])
                           << (8 * (e % 4));
             else
-              v[e / 2] |= static_cast<uint32_t>(reinterpret_cast<const uint16_t*>(p)[e])
+              v[e / 2] |= static_cast<uint32_t>(reinterpret_cast<const uint16_t*>(q)[e])
                           << (16 * (e % 2));
           }
         }
-        asm volatile("st.shared.v4.u32 [%0], {%1,%2,%3,%4};" ::"r"(set + xdst[i]), "r"(v[0]),
+        asm volatile("st.shared.v4.u32 [%0], {%1,%2,%3,%4};" ::"r"(set + xdst + 512 * i), "r"(v[0]),
                      "r"(v[1]), "r"(v[2]), "r"(v[3])
                      : "memory");
       }
@@ -1103,8 +1105,9 @@ cudaError_t launch_linear_as(const LinearArgs& a, int num_sms, bool pdl, cudaStr
 // B tiles by the rows of x.  Two teams of warps (16 warps hide more latency: 1 x 8192 ->
 // 57344 f16 55 us, 59 us with one) unless the SMs have no second tile for the second
 // team (1 x 2048 -> 2048 Q8_0 2.8 us with one team, 3.2 us with two).  With four B
-// tiles the sums fill the registers of one team, eight tiles at a time where a CTA has
-// that many.
+// tiles the sums fill the registers of one team (32 x 8192 -> 28672 f16 64 us, 116 us
+// with two teams of half the tiles), eight tiles at a time where a CTA has more than
+// four (86 us with four at a time).
 template <int IN, int G>
 cudaError_t launch_linear_in(const LinearArgs& a, int num_sms, bool pdl, cudaStream_t s) {
   const int b = (a.rows - 1) / LinCfg<IN, 1, 1, 1, G>::kTileRows + 1;
