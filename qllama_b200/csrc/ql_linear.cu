@@ -355,7 +355,8 @@ cudaError_t launch_pdl(void (*kernel)(P...), dim3 grid, dim3 block, size_t smem,
 
 // NV: a few rows go over as many threads as they have groups (one round trip,
 // the shortest reduction); with two rows or more for every SM, twice as many
-// columns a thread (fewer threads wait in a reduction).
+// columns a thread (fewer threads wait in a reduction: 4099 x 4096 bf16 22.1 us, 30.7 us
+// with one group a thread).
 cudaError_t launch_norm(const NormArgs& a, int num_sms, cudaStream_t s) {
   auto fits = [](const void* p, int dt, int64_t stride) {
     const size_t to = dt == QL_Q8_0 ? 8 : 16;

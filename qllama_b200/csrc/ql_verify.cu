@@ -45,17 +45,22 @@ struct VerifyArgs {
 //      taken again from f64 sums of its rows.
 //   3. The draw compares running sums over the whole vocabulary with a threshold,
 //      where an error of 1e-7 would change one token in some thousands: its sums are
-//      f64.  A rejected draft's two rows are summed first, for their ratio; then the
-//      sum of what is left of the target gives the threshold, and the CTA, the warps
-//      and the lane where the running sum passes it are found in turn.
+//      f64, of the rows' weights wp, wq = exp((logit - maximum) / T).  After a rejected
+//      draft the ids with wp / sum wp > wq / sum wq keep the difference.  Which they
+//      are is decided with the f32 sums: an id that these misjudge has a difference of
+//      1e-6 of its probability or less.  So one pass gives the whole sums and those of
+//      the ids that count, and from them the sum of what is left; its threshold is
+//      then looked for in the CTAs, the warps and the lanes in turn.
 // The CTAs of a cluster tell each other their sums by stores into one another's
 // shared memory that count on an mbarrier there; all make the same decisions from the
 // same numbers.  Nothing is kept outside shared memory.
-// A small call is bound by its instructions, not its bytes (32 sequences, one row of
-// 32000: 24 us when every warp followed every decision): only the sums themselves are
-// every warp's work, one loop for all of them, and warp 0 alone decides what is next.
-// Greedy, logits and probabilities are kernels of their own, and rows are read in
-// whole aligned groups with the odd ends on the side.
+// A small call is bound by the latencies of its steps, one after the other (32
+// sequences, one row of 32000: 24 us with every warp following every decision, 17 us
+// with the weights computed anew at every turn of the search).  So one loop takes all
+// f64 sums, warp 0 alone decides what is next, and where a CTA's share is small
+// enough its weights stay in shared memory for the search.  Greedy, logits and
+// probabilities are kernels of their own, and rows are read in whole aligned groups
+// with the odd ends on the side.
 constexpr int kVerifyRows = 2 * QL_VERIFY_MAX_DRAFTS + 1;
 constexpr int kMaxCluster = 16;
 
@@ -74,15 +79,51 @@ __device__ __forceinline__ float exp2_fast(float x) {
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
   return y;
 }
+__device__ __forceinline__ float max_nan(float a, float b) {  // NaN if either is
+  float m;
+  asm("max.NaN.f32 %0, %1, %2;" : "=f"(m) : "f"(a), "f"(b));
+  return m;
+}
 __device__ __forceinline__ float warp_max(float v) {  // NaN only of NaNs
   float m;
   asm("redux.sync.max.f32 %0, %1, 0xffffffff;" : "=f"(m) : "f"(v));
   return m;
 }
-__device__ __forceinline__ double warp_total(double v) {
-#pragma unroll
-  for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
-  return v;
+__device__ __forceinline__ double shfl_xor(double v, int o) {
+  return __shfl_xor_sync(0xffffffffu, v, o);
+}
+// Sums of four values over the warp, each step halving what a lane still carries:
+// lanes 8 i .. 8 i + 7 get the sum of v[i].
+__device__ __forceinline__ double warp_totals(const double (&v)[4]) {
+  const int lane = threadIdx.x & 31;
+  const bool hi = lane & 16, up = lane & 8;
+  const double a = (hi ? v[2] : v[0]) + shfl_xor(hi ? v[0] : v[2], 16);
+  const double b = (hi ? v[3] : v[1]) + shfl_xor(hi ? v[1] : v[3], 16);
+  double t = (up ? b : a) + shfl_xor(up ? a : b, 8);
+  t += shfl_xor(t, 4);
+  t += shfl_xor(t, 2);
+  return t + shfl_xor(t, 1);
+}
+// A wait that looks often before it looks at the clock.
+__device__ __forceinline__ void await(uint64_t* bar, uint32_t parity, uint32_t* status) {
+  for (int i = 0; i < 64; ++i) {
+    uint32_t ok;
+    asm volatile(
+        "{\n\t.reg .pred p;\n\t"
+        "mbarrier.test_wait.parity.acquire.cluster.shared::cta.b64 p, [%1], %2;\n\t"
+        "selp.u32 %0, 1, 0, p;\n\t}"
+        : "=r"(ok)
+        : "r"(ql::smem_u32(bar)), "r"(parity)
+        : "memory");
+    if (ok) return;
+  }
+  ql::mbar_wait_cluster(bar, parity, status);
+}
+__device__ __forceinline__ void st_async_f64(uint32_t remote_addr, double v, uint32_t remote_bar) {
+  asm volatile("st.async.shared::cluster.mbarrier::complete_tx::bytes.b64 [%0], %1, [%2];" ::"r"(
+                   remote_addr),
+               "l"(__double_as_longlong(v)), "r"(remote_bar)
+               : "memory");
 }
 
 // exp((x - m) / T) in f64 for x <= m by the table method (P. T. P. Tang, 1989):
@@ -126,13 +167,16 @@ struct VerifyStep {
   int from, to;   // over these ids
   int pos;        // of these rows
   int out;        // a certain draft's id that is taken out of the row, or -1
-  double fp, fq;  // of max(wp fp - wq fq, 0)
+  double ratio;   // ids count where wp > ratio wq
+  double fp, fq;  // and weigh wp fp - wq fq
 };
-enum : int { kTotals = 0, kAtDraft = 1, kLeft = 2, kNarrow = 3, kDone = 4 };
+// With sums: of the rows at a close decision, of its draft alone, of what is left, of a
+// part of it; without: the decisions from pos on, the end.
+enum : int { kTotals = 0, kAtDraft, kLeft, kNarrow, kBegin, kGiveUp, kDone };
 
 // T threads: 1024 where a cluster's CTAs have an SM each, 256 where four share one.
 template <int DT, int MODE, int T>
-__global__ void __launch_bounds__(T, 1024 / T) verify_kernel(const VerifyArgs a) {
+__global__ void __launch_bounds__(T, T == 1024 ? 1 : 3) verify_kernel(const VerifyArgs a) {
   constexpr int kVerifyThreads = T, kVerifyWarps = T / 32;
   constexpr int kN = DT == ql::kF32 ? 4 : 8;  // elements of a 16-byte group
   constexpr int kLoads = 4;                   // groups of a lane in a piece
@@ -140,8 +184,10 @@ __global__ void __launch_bounds__(T, 1024 / T) verify_kernel(const VerifyArgs a)
   __shared__ float2 part[kVerifyRows][kVerifyWarps];     // a row's (m, s) or (best, id) by warp
   __shared__ __align__(16) float2 from_cta[kVerifyRows][kMaxCluster];  // by CTA of the cluster
   __shared__ float2 row_stat[kVerifyRows];               // of the whole row
-  __shared__ double sums[2][kVerifyWarps];
-  __shared__ __align__(16) float4 sums_of[2][kMaxCluster];  // two f64 of each CTA (two turns)
+  __shared__ double sums[4][kVerifyWarps];
+  __shared__ double sums_of[2][4][kMaxCluster];  // of each CTA, two turns
+  constexpr int kKeep = T == 1024 ? 2048 : 4096;
+  __shared__ double kept[MODE == kGreedy ? 1 : kKeep];  // weights of a share's ids
   __shared__ VerifyStep next_step;
   __shared__ __align__(8) uint64_t bars[3];
   __shared__ double pow2_32[32];                         // 2^(j/32)
@@ -242,25 +288,35 @@ __global__ void __launch_bounds__(T, 1024 / T) verify_kernel(const VerifyArgs a)
           if constexpr (DT == ql::kF32) return __uint_as_float(x);
           else return half_word<DT>(x, e & 1);
         };
+        float top = ex;
+#pragma unroll
+        for (int k = 0; k < kLoads * kN; ++k) top = max_nan(top, element(k));
         if constexpr (MODE == kGreedy) {
-          auto take = [&](float x, int id) {
-            bad |= !(x < INFINITY);
-            if (x > m || (x == m && id < best)) {
-              m = x;
-              best = id;
+          // a piece that matters is looked through again for its first largest
+          bad |= !(top < INFINITY);
+          if (top > m || (top == m && top > -INFINITY)) {
+            int id = ex == top ? eid : INT_MAX;
+#pragma unroll 1
+            for (int j = kLoads - 1; j >= 0; --j) {
+              const uint4 v = j == 0 ? now[0] : j == 1 ? now[1] : j == 2 ? now[2] : now[3];
+              const uint32_t w[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+              for (int e = kN - 1; e >= 0; --e) {
+                float x;
+                if constexpr (DT == ql::kF32) x = __uint_as_float(w[e]);
+                else x = half_word<DT>(w[e / 2], e & 1);
+                const int i = id0 + j * (32 * kN) + e;
+                if (x == top && i < id) id = i;
+              }
             }
-          };
-#pragma unroll
-          for (int k = 0; k < kLoads * kN; ++k)
-            take(element(k), id0 + k / kN * (32 * kN) + k % kN);
-          take(ex, eid);
+            best = top > m ? id : min(best, id);
+            m = top;
+          }
         } else {
-          float top = fmaxf(m, ex);
-#pragma unroll
-          for (int k = 0; k < kLoads * kN; ++k) top = fmaxf(top, element(k));
+          top = fmaxf(top, m);  // a NaN is met again below
           // nothing above -inf yet: 0 for the maximum leaves zeros, and NaN a NaN
-          const float ref = top == -INFINITY ? 0.f : top;
-          s = s * exp2_fast((m == -INFINITY ? 0.f : m - ref) * c) + exp2_fast((ex - ref) * c);
+          const float ref = top > -INFINITY ? top : 0.f;
+          s = s * exp2_fast(m == -INFINITY ? 0.f : (m - ref) * c) + exp2_fast((ex - ref) * c);
           m = top;
           float add[4] = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
@@ -289,7 +345,7 @@ __global__ void __launch_bounds__(T, 1024 / T) verify_kernel(const VerifyArgs a)
     __syncthreads();
 #pragma unroll 1
     for (int turn = 0; turn < 2; ++turn) {
-      if (turn == 1) ql::mbar_wait_cluster(&bars[0], 0, a.status);
+      if (turn == 1) await(&bars[0], 0, a.status);
 #pragma unroll 1
       for (int r = warp; r < nrows; r += kVerifyWarps) {
         float2 z = none;
@@ -362,8 +418,7 @@ __global__ void __launch_bounds__(T, 1024 / T) verify_kernel(const VerifyArgs a)
       if (i != pos || known) tok[i] = i < pos ? ids[i] : i == pos ? token : -1;
     if (lane == 0) a.accepted[b] = pos;
   };
-  auto give_up = [&]() {
-    write(true, -1);
+  auto raise = [&]() {
     if (rank == 0 && lane == 0) {
       const bool id = pos < n && (ids[pos] < 0 || ids[pos] >= V);
       atomicOr(a.status, id ? ql::kStatusBadToken : ql::kStatusBadLogits);
@@ -372,8 +427,8 @@ __global__ void __launch_bounds__(T, 1024 / T) verify_kernel(const VerifyArgs a)
   if constexpr (MODE == kGreedy) {
     if (warp != 0) return;
     decide();
-    if (verdict == 3) give_up();
-    else write(true, __float_as_int(row_stat[pos].y));
+    write(true, verdict == 3 ? -1 : __float_as_int(row_stat[pos].y));
+    if (verdict == 3) raise();
   } else {
     // ---- 3.
     const int lo = static_cast<int>(static_cast<long long>(V) * rank / ctas);
@@ -382,170 +437,221 @@ __global__ void __launch_bounds__(T, 1024 / T) verify_kernel(const VerifyArgs a)
     // warp 0's: sums of the rows at pos, the threshold, the sum before [from, to)
     double zp = 1.0, zq = 1.0, th = 0.0, before = 0.0;
     int turn = 0;
-    auto go = [&](int what, int from, int to, int out, double fp, double fq) {
-      if (lane == 0) next_step = {what, from, to, pos, out, fp, fq};
-    };
-    // After a verdict: a rejected draft's row is taken off the target's, both divided
-    // by their sums; without one the target's weights serve as they are.
-    auto draw = [&]() {
-      const bool less = verdict == 1;
-      go(kLeft, lo, hi, less && !has_q ? ids[pos] : -1, less && has_q ? 1.0 / zp : 1.0,
-         less && has_q ? 1.0 / zq : 0.0);
-    };
-    auto begin = [&]() {
-      decide();
-      if (verdict == 3) {
-        give_up();
-        go(kDone, 0, 0, 0, 0, 0);
-      } else if (MODE == kLogits && (verdict == 2 || (verdict == 1 && has_q))) {
-        go(kTotals, lo, hi, -1, 1.0, 0.0);
-      } else {
-        draw();
-      }
-    };
-    // Of the lanes' shares (in lane order), the first where the running sum reaches
-    // th, else the last that is not empty; `before` becomes the sum before it.
-    auto find = [&](double v) {
-      double cum = v;
-#pragma unroll 1
-      for (int o = 1; o < 32; o <<= 1) {
-        const double w = __shfl_up_sync(0xffffffffu, cum, o);
-        if (lane >= o) cum += w;
-      }
-      const unsigned some = __ballot_sync(0xffffffffu, v > 0);
-      const unsigned hit = __ballot_sync(0xffffffffu, v > 0 && before + cum >= th);
-      const int k = hit ? __ffs(hit) - 1 : some ? 31 - __clz(some) : 0;
-      before += __shfl_sync(0xffffffffu, cum - v, k);
-      return k;
-    };
-    if (warp == 0) begin();
+    if (tid == 0) next_step = {kBegin, lo, hi, 0, -1, 0.0, 1.0, 0.0};
 #pragma unroll 1
     for (;;) {
       __syncthreads();
-      const VerifyStep z = next_step;
+      VerifyStep z = next_step;
       if (z.what == kDone) break;
       auto share = [&](int w) {
         return z.from + static_cast<int>(static_cast<long long>(z.to - z.from) * w / kVerifyWarps);
       };
-      // s0 = sum of max(wp fp - wq fq, 0), s1 = sum of wq, with wp, wq the weights
-      // exp((logit - maximum) / T), or the probabilities, of the rows at pos
       const bool with_q = has_q && z.pos < n;
-      const bool narrow = z.to - z.from <= 32 && z.what == kNarrow;
-      const char* const prow = row_at(z.pos);
-      const char* const qrow = row_at(with_q ? n + 1 + z.pos : z.pos);
-      const float pm = MODE == kLogits ? row_stat[z.pos].x : 0.f;
-      const float qm = MODE == kLogits && with_q ? row_stat[n + 1 + z.pos].x : 0.f;
-      const float pl = ex.least(pm), ql_ = ex.least(qm);
-      const int f = narrow ? z.from : share(warp), e = narrow ? z.to : share(warp + 1);
-      double s0 = 0, s1 = 0;
-      constexpr int kIds = 4;  // of a lane at a time, their loads in flight together
-      constexpr float kEmpty = MODE == kLogits ? -INFINITY : 0.f;
+      const bool keep = z.to - z.from <= (with_q ? kKeep / 2 : kKeep);
+      // of the ids that count: sums of wp, wq; of all
+      if (z.what < kBegin) {
+        double s[4] = {0.0, 0.0, 0.0, 0.0};
+        const char* const prow = row_at(z.pos);
+        const char* const qrow = row_at(with_q ? n + 1 + z.pos : z.pos);
+        const float pm = MODE == kLogits ? row_stat[z.pos].x : 0.f;
+        const float qm = MODE == kLogits && with_q ? row_stat[n + 1 + z.pos].x : 0.f;
+        const float pl = ex.least(pm), ql_ = ex.least(qm);
+        const int f = share(warp), e = share(warp + 1);
+        constexpr int kIds = 4;  // of a lane at a time, their loads in flight together
+        constexpr float kEmpty = MODE == kLogits ? -INFINITY : 0.f;
 #pragma unroll 1
-      for (int i0 = f + lane; i0 - lane < e; i0 += 32 * kIds) {
-        float xp[kIds], xq[kIds];
+        for (int i0 = f + lane; i0 - lane < e; i0 += 32 * kIds) {
+          float xp[kIds], xq[kIds];
 #pragma unroll
-        for (int k = 0; k < kIds; ++k) xp[k] = ql::load_elem(prow, min(i0 + 32 * k, e - 1), DT);
-        if (with_q) {
+          for (int k = 0; k < kIds; ++k) xp[k] = ql::load_elem(prow, min(i0 + 32 * k, e - 1), DT);
+          if (with_q) {
 #pragma unroll
-          for (int k = 0; k < kIds; ++k) xq[k] = ql::load_elem(qrow, min(i0 + 32 * k, e - 1), DT);
-        }
-        double w[kIds];
-#pragma unroll
-        for (int k = 0; k < kIds; ++k) {
-          const float x = i0 + 32 * k < e ? xp[k] : kEmpty;
-          w[k] = z.fp * (MODE == kLogits ? ex(x, pm, pl) : static_cast<double>(x));
-        }
-        if (with_q) {
+            for (int k = 0; k < kIds; ++k) xq[k] = ql::load_elem(qrow, min(i0 + 32 * k, e - 1), DT);
+          }
+          double wp[kIds], wq[kIds];
 #pragma unroll
           for (int k = 0; k < kIds; ++k) {
-            const float x = i0 + 32 * k < e ? xq[k] : kEmpty;
-            const double wq = MODE == kLogits ? ex(x, qm, ql_) : static_cast<double>(x);
-            s1 += wq;
-            w[k] = fma(-wq, z.fq, w[k]);
+            const float x = i0 + 32 * k < e ? xp[k] : kEmpty;
+            wp[k] = MODE == kLogits ? ex(x, pm, pl) : static_cast<double>(x);
+            wq[k] = 0.0;
+          }
+          if (with_q) {
+#pragma unroll
+            for (int k = 0; k < kIds; ++k) {
+              const float x = i0 + 32 * k < e ? xq[k] : kEmpty;
+              wq[k] = MODE == kLogits ? ex(x, qm, ql_) : static_cast<double>(x);
+            }
+          }
+#pragma unroll
+          for (int k = 0; k < kIds; ++k) {
+            const bool counts = wp[k] > z.ratio * wq[k] && i0 + 32 * k != z.out;
+            s[2] += wp[k];
+            s[3] += wq[k];
+            if (!counts) wp[k] = wq[k] = 0.0;
+            s[0] += wp[k];
+            s[1] += wq[k];
+            if (keep && i0 + 32 * k < e) {
+              kept[i0 + 32 * k - z.from] = wp[k];
+              if (with_q) kept[kKeep / 2 + i0 + 32 * k - z.from] = wq[k];
+            }
           }
         }
-#pragma unroll
-        for (int k = 0; k < kIds; ++k)  // NaN stays
-          s0 += w[k] < 0 || i0 + 32 * k == z.out ? 0.0 : w[k];
-      }
-      if (!narrow) {
-        s0 = warp_total(s0);
-        s1 = warp_total(s1);
-        if (lane == 0) {
-          sums[0][warp] = s0;
-          sums[1][warp] = s1;
-        }
+        const double t = warp_totals(s);
+        if (lane % 8 == 0) sums[lane / 8][warp] = t;
       }
       __syncthreads();
       if (warp != 0) continue;
+
       // ---- warp 0: what these sums mean, and what is next
-      if (narrow) {  // at most 32 ids are left, one to a lane
-        const unsigned some = __ballot_sync(0xffffffffu, s0 > 0);
-        const int k = find(s0);
-        if (lane == 0) tok[pos] = some ? z.from + k : -1;
-        go(kDone, 0, 0, 0, 0, 0);
-        continue;
-      }
-      double c0 = lane < kVerifyWarps ? sums[0][lane] : 0.0;
-      double c1 = lane < kVerifyWarps ? sums[1][lane] : 0.0;
-      if (z.what == kNarrow) {
-        const int w = find(c0);
-        go(kNarrow, share(w), share(w + 1), z.out, z.fp, z.fq);
-        continue;
-      }
-      const double of_warp = c0;
-      c0 = warp_total(c0);
-      c1 = warp_total(c1);
-      if (z.what == kAtDraft) {  // every CTA has looked at the id itself
-        if (u[pos] * (has_q ? c1 / zq : 1.0) < c0 / zp) {
-          ++pos;
-          begin();
-        } else {
+      bool draw = false, search = z.what == kNarrow;
+      int what = kDone;
+      if (z.what == kBegin) {
+        decide();
+        z.pos = pos;
+        if (verdict == 2) what = kTotals;
+        else if (verdict == 3) what = kGiveUp;
+        else draw = true;
+      } else if (z.what < kNarrow) {
+        // lanes 8 i ..: sum i of the CTA
+        double t = 0.0;
+#pragma unroll
+        for (int w = 0; w < kVerifyWarps; w += 8) t += sums[lane / 8][w + lane % 8];
+        t += shfl_xor(t, 4);
+        t += shfl_xor(t, 2);
+        t += shfl_xor(t, 1);
+        if (z.what == kAtDraft) {  // every CTA has looked at the id itself
+          const double wp = __shfl_sync(0xffffffffu, t, 16), wq = __shfl_sync(0xffffffffu, t, 24);
+          draw = !(u[pos] * (has_q ? wq / zq : 1.0) < wp / zp);
           verdict = 1;
-          draw();
+          if (!draw) {
+            ++pos;
+            what = kBegin;
+          }
+        } else {
+          // the cluster's sums: a rank one exchange ahead writes the other turn's
+          uint64_t* const bar = &bars[1 + (turn & 1)];
+          if (lane == 0) ql::mbar_arrive_expect_tx(bar, static_cast<uint32_t>(32 * ctas));
+          __syncwarp();
+          const uint32_t mine = ql::smem_u32(&sums_of[turn & 1][lane / 8][rank]);
+#pragma unroll
+          for (int h = 0; h < kMaxCluster; h += 8)
+            if (h + lane % 8 < ctas)
+              st_async_f64(ql::mapa_shared(mine, h + lane % 8), t,
+                           ql::mapa_shared(ql::smem_u32(bar), h + lane % 8));
+          await(bar, turn >> 1 & 1, a.status);
+          t = 0.0;
+#pragma unroll
+          for (int h = 0; h < kMaxCluster; h += 8)
+            if (h + lane % 8 < ctas) t += sums_of[turn & 1][lane / 8][h + lane % 8];
+          t += shfl_xor(t, 4);
+          t += shfl_xor(t, 2);
+          t += shfl_xor(t, 1);  // lanes 8 i ..: sum i of the cluster
+          const double inv = 1.0 / t;
+          const double t2 = __shfl_sync(0xffffffffu, t, 16), t3 = __shfl_sync(0xffffffffu, t, 24);
+          if (z.what == kTotals) {
+            zp = t2;
+            zq = t3;
+            what = kAtDraft;
+            z.from = ids[pos];
+            z.to = z.from + 1;
+          } else {
+            const bool less = z.fq != 0;
+            if (less && MODE == kLogits) {
+              z.fp = __shfl_sync(0xffffffffu, inv, 16);
+              z.fq = __shfl_sync(0xffffffffu, inv, 24);
+            }
+            const double left = __shfl_sync(0xffffffffu, t, 0) * z.fp -
+                                __shfl_sync(0xffffffffu, t, 8) * z.fq;
+            th = u[n] * left;
+            search = left > 0 && t2 < INFINITY && t3 < INFINITY;
+            if (!search) {
+              what = kGiveUp;  // probabilities that are none, unless
+              if ((less || z.out >= 0) && left <= 0) {  // the draft's took all: the target
+                what = kLeft;
+                z.out = -1;
+                z.ratio = z.fq = 0.0;
+                z.fp = 1.0;
+              }
+            }
+          }
         }
-        continue;
       }
-      // the cluster's sums: a rank that is one exchange ahead writes the other turn's
-      if (lane == 0)
-        ql::mbar_arrive_expect_tx(&bars[1 + (turn & 1)], static_cast<uint32_t>(16 * ctas));
-      __syncwarp();
-      if (lane < ctas) {
-        const double2 v = make_double2(c0, c1);
-        ql::st_async_v4(ql::mapa_shared(ql::smem_u32(&sums_of[turn & 1][rank]), lane),
-                        *reinterpret_cast<const float4*>(&v),
-                        ql::mapa_shared(ql::smem_u32(&bars[1 + (turn & 1)]), lane));
+      // Of the lanes' parts (in lane order), the first where the running sum reaches th,
+      // else the last that is not empty; `before` becomes the sum before it.
+      unsigned some = 0;
+      auto find = [&](double part) {
+        double cum = part;
+#pragma unroll
+        for (int o = 1; o < 32; o <<= 1) {
+          const double v = __shfl_up_sync(0xffffffffu, cum, o);
+          if (lane >= o) cum += v;
+        }
+        some = __ballot_sync(0xffffffffu, part > 0);
+        const unsigned hit = __ballot_sync(0xffffffffu, part > 0 && before + cum >= th);
+        const int k = hit ? __ffs(hit) - 1 : some ? 31 - __clz(some) : 0;
+        before += __shfl_sync(0xffffffffu, cum - part, k);
+        return k;
+      };
+      if (search) {
+        auto weigh = [&](double wp, double wq) { return wp * z.fp - wq * z.fq; };
+        bool here = true;
+        if (z.what == kLeft) {  // the CTA
+          write(false, 0);
+          const int at = (turn & 1) * 4 * kMaxCluster + lane;
+          const double* const of = &sums_of[0][0][0];
+          here = find(lane < ctas ? weigh(of[at], of[at + kMaxCluster]) : 0.0) == rank;
+        }
+        if (here) {  // its warp
+          const int w = find(lane < kVerifyWarps ? weigh(sums[0][lane], sums[1][lane]) : 0.0);
+          const int f = share(w), e = share(w + 1);
+          if (keep) {  // the lane's ids of that warp, then the id
+            auto kept_at = [&](int i) {
+              return weigh(kept[i - z.from], with_q ? kept[kKeep / 2 + i - z.from] : 0.0);
+            };
+            const int len = ((e - f + 31) / 32) | 1;  // odd: no two lanes on one bank
+            double v = 0.0;
+            for (int j = 0; j < len; ++j) {
+              const int i = f + lane * len + j;
+              if (i < e) v += kept_at(i);
+            }
+            const int i0 = f + find(v) * len;
+            const int k = find(lane < len && i0 + lane < e ? kept_at(i0 + lane) : 0.0);
+            if (lane == 0) tok[pos] = some ? i0 + k : -1;
+          } else {
+            what = kNarrow;
+            z.from = f;
+            z.to = e;
+          }
+        }
       }
-      ql::mbar_wait_cluster(&bars[1 + (turn & 1)], turn >> 1 & 1, a.status);
-      const double2 of =
-          lane < ctas ? *reinterpret_cast<const double2*>(&sums_of[turn & 1][lane])
-                      : make_double2(0.0, 0.0);
-      ++turn;
-      const double t0 = warp_total(of.x);
-      if (z.what == kTotals) {
-        zp = t0;
-        zq = warp_total(of.y);
-        if (verdict == 2) go(kAtDraft, ids[pos], ids[pos] + 1, -1, 1.0, 0.0);
-        else draw();
-        continue;
+      turn += z.what == kTotals || z.what == kLeft;
+      // What a rejected draft leaves of the target's row, or all of it.
+      if (draw) {
+        const bool less = verdict == 1 && has_q;
+        what = kLeft;
+        z.from = lo;
+        z.to = hi;
+        z.out = verdict == 1 && !has_q ? ids[pos] : -1;
+        z.ratio = !less ? 0.0 : MODE == kProbs ? 1.0 : row_stat[pos].y / row_stat[n + 1 + pos].y;
+        z.fp = 1.0;
+        z.fq = less ? 1.0 : 0.0;
       }
-      if (t0 <= 0 && (z.fq != 0 || z.out >= 0)) {  // nothing left: the target itself
-        go(kLeft, lo, hi, -1, z.fp, 0.0);
-        continue;
+      if (what == kGiveUp) {
+        write(true, -1);
+        raise();
+        what = kDone;
       }
-      if (!(t0 > 0 && t0 < INFINITY)) {  // probabilities that are none
-        give_up();
-        go(kDone, 0, 0, 0, 0, 0);
-        continue;
+      z.what = what;
+      z.pos = pos;
+      if (what == kTotals || what == kBegin) {
+        z.from = lo;
+        z.to = hi;
       }
-      th = u[n] * t0;
-      write(false, 0);
-      if (find(of.x) == rank) {
-        const int w = find(of_warp);
-        go(kNarrow, share(w), share(w + 1), z.out, z.fp, z.fq);
-      } else {
-        go(kDone, 0, 0, 0, 0, 0);
+      if (what == kTotals || what == kAtDraft) {
+        z.out = -1;
+        z.ratio = 0.0;
       }
+      if (lane == 0) next_step = z;
     }
   }
 }
