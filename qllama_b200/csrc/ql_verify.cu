@@ -47,10 +47,12 @@ struct VerifyArgs {
 //      where an error of 1e-7 would change one token in some thousands: its sums are
 //      f64, of the rows' weights wp, wq = exp((logit - maximum) / T).  After a rejected
 //      draft the ids with wp / sum wp > wq / sum wq keep the difference.  Which they
-//      are is decided with the f32 sums: an id that these misjudge has a difference of
-//      1e-6 of its probability or less.  So one pass gives the whole sums and those of
-//      the ids that count, and from them the sum of what is left; its threshold is
-//      then looked for in the CTAs, the warps and the lanes in turn.
+//      are is decided with the f32 sums, so that one pass gives the whole sums and
+//      those of the ids that count, and from them the sum of what is left: an id that
+//      the f32 sums misjudge has a difference of 1e-6 of its probability or less, and
+//      few have (when less than 1/32 is left, more may: a second pass then goes by the
+//      f64 sums).  The threshold is looked for in the CTAs, the warps and the lanes in
+//      turn.
 // The CTAs of a cluster tell each other their sums by stores into one another's
 // shared memory that count on an mbarrier there; all make the same decisions from the
 // same numbers.  Nothing is kept outside shared memory.
@@ -174,7 +176,7 @@ struct VerifyStep {
 // part of it; without: the decisions from pos on, the end.
 enum : int { kTotals = 0, kAtDraft, kLeft, kNarrow, kBegin, kGiveUp, kDone };
 
-// T threads: 1024 where a cluster's CTAs have an SM each, 256 where four share one.
+// T threads: 1024 where a cluster's CTAs have an SM each, 256 where three share one.
 template <int DT, int MODE, int T>
 __global__ void __launch_bounds__(T, T == 1024 ? 1 : 3) verify_kernel(const VerifyArgs a) {
   constexpr int kVerifyThreads = T, kVerifyWarps = T / 32;
@@ -401,7 +403,9 @@ __global__ void __launch_bounds__(T, T == 1024 ? 1 : 3) verify_kernel(const Veri
         }
         const double uq = u[i] * qx;
         d = uq < px ? 0 : 1;
-        if (MODE == kLogits && !(fabs(uq - px) > 0x1p-14 * px)) d = 2;
+        if (MODE == kLogits &&  // close, or so small that f32 may have lost it
+            (!(fabs(uq - px) > 0x1p-14 * px) || px < 1e-30 || qx < 1e-30))
+          d = 2;
         if (MODE == kProbs && !(px < INFINITY && qx < INFINITY)) d = 3;
       }
     }
@@ -564,7 +568,12 @@ __global__ void __launch_bounds__(T, T == 1024 ? 1 : 3) verify_kernel(const Veri
                                 __shfl_sync(0xffffffffu, t, 8) * z.fq;
             th = u[n] * left;
             search = left > 0 && t2 < INFINITY && t3 < INFINITY;
-            if (!search) {
+            if (search && less && MODE == kLogits && left < 0.03125 && z.ratio != t2 / t3) {
+              search = false;
+              what = kLeft;
+              z.ratio = t2 / t3;
+              z.fp = z.fq = 1.0;
+            } else if (!search) {
               what = kGiveUp;  // probabilities that are none, unless
               if ((less || z.out >= 0) && left <= 0) {  // the draft's took all: the target
                 what = kLeft;
@@ -632,7 +641,10 @@ __global__ void __launch_bounds__(T, T == 1024 ? 1 : 3) verify_kernel(const Veri
         z.from = lo;
         z.to = hi;
         z.out = verdict == 1 && !has_q ? ids[pos] : -1;
-        z.ratio = !less ? 0.0 : MODE == kProbs ? 1.0 : row_stat[pos].y / row_stat[n + 1 + pos].y;
+        z.ratio = !less ? 0.0
+                  : MODE == kProbs
+                      ? 1.0
+                      : static_cast<double>(row_stat[pos].y) / row_stat[n + 1 + pos].y;
         z.fp = 1.0;
         z.fq = less ? 1.0 : 0.0;
       }
@@ -656,10 +668,10 @@ __global__ void __launch_bounds__(T, T == 1024 ? 1 : 3) verify_kernel(const Veri
   }
 }
 
-// CTAs of a cluster: up to 16, in powers of two, with an equal share of the GPU's
-// places (four CTAs to an SM) for every sequence; 1024 ids or more each, or 4096 when
-// most of the places are taken and the CTAs slow one another down (32 sequences, one
-// row of 32000: 12.8 us with 8, 16.3 us with 16; 8 sequences: 21.5 us and 17.2 us).
+// CTAs of a cluster: up to 16, in powers of two, while all sequences' CTAs are not many
+// more than run at once (three to an SM); 1024 ids or more each, or 4096 when the SMs
+// are shared and the CTAs slow one another down (32 sequences, one row of 32000: 12.4 us
+// with 8, 15.8 us with 16; 8 sequences of 6 rows: 15.9 us and 13.0 us).
 int cluster_ctas(int batch, int vocab, int num_sms) {
   int c = kMaxCluster;
   while (c > 1) {
@@ -697,8 +709,8 @@ cudaError_t launch_verify_as(const VerifyArgs& a, int batch, int ctas, cudaStrea
 template <int DT, int MODE>
 cudaError_t launch_verify_mode(const VerifyArgs& a, int batch, int num_sms, cudaStream_t s) {
   const int ctas = cluster_ctas(batch, a.vocab, num_sms);
-  // a few clusters with long shares: four times the warps (one sequence of 8 rows of
-  // 128000 f32 28.7 us, 35.2 us with 256 threads; of 5 rows of 32000 19.8 us and 15.6 us)
+  // a few clusters with long shares: four times the warps (two sequences of 8 rows of
+  // 128000 f32 23.7 us, 26.1 us with 256 threads; one of 5 rows of 32000 16.0 us, 10.9 us)
   return batch * ctas <= num_sms / 2 && a.vocab / ctas >= 4096
              ? launch_verify_as<DT, MODE, 1024>(a, batch, ctas, s)
              : launch_verify_as<DT, MODE, 256>(a, batch, ctas, s);

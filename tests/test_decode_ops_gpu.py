@@ -525,6 +525,37 @@ def test_verify_accepts_equal_distributions(ctx):
     assert (a == 6).all()
 
 
+@pytest.mark.parametrize("V, near", [(5000, 1e-5), (128000, 1e-3), (32000, 3e-2)])
+def test_verify_rejects_from_nearly_equal_distributions(ctx, V, near):
+    """Little is left of a target that its draft nearly equals: the few ids that keep a
+    difference, and how much, are those of the definition."""
+    g = gen(V)
+    torch.manual_seed(V)
+    target, draft, ids, un = drafted(g, 6, 2, V, "f32", near=near)
+    # a drafted id whose draft probability is the larger, and a uniform that rejects it
+    p, q = torch.softmax(target.double(), -1)[:, :2], torch.softmax(draft.double(), -1)
+    ids = ((q - p) / q).argmax(-1).int()
+    un[:, :2] = 1 - 2.0 ** -53
+    t, a = check_verify(ctx, target, draft, ids, un)
+    assert (a == 0).all()
+
+
+def test_verify_probabilities_below_f32(ctx):
+    """A decision between probabilities that are no f32 numbers any more."""
+    target = torch.zeros(2, 2, 50, device="cuda")
+    draft = torch.zeros(2, 1, 50, device="cuda")
+    target[:, 0, 7], draft[:, 0, 7] = -120.0, -118.0  # e^-120 and e^-118 of some 49
+    ids = torch.full((2, 1), 7, dtype=torch.int32, device="cuda")
+    un = torch.tensor([[0.13, 0.5], [0.14, 0.5]], dtype=torch.float64, device="cuda")
+    tokens, accepted = qm.verify_drafts(ctx, target, draft, ids, un)
+    ctx.synchronize()
+    assert accepted.tolist() == [1, 0]  # e^-2 = 0.1353
+    assert tokens[0].tolist() == [7, 24]
+    # what is left of the other rows (the 49 ids' shares of e^-118 - e^-120) is below
+    # f64's resolution, the definition's as well: any of the 49
+    assert tokens[1, 0].item() != 7 and tokens[1, 0].item() >= 0
+
+
 def test_verify_masked_and_bad_rows(ctx):
     g = gen(9)
     torch.manual_seed(9)
