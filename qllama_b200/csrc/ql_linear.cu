@@ -37,7 +37,7 @@ struct NormArgs {
   __half* out_scale;
   int64_t x_stride, residual_stride;
   int rows, hidden, in_dtype, weight_dtype, out_dtype;
-  float eps;
+  float eps, inv_hidden;
 };
 
 template <typename T>
@@ -75,28 +75,33 @@ __device__ __forceinline__ int round_away(float v) {
 // is above every finite one, so that one maximum carries both.
 __device__ __forceinline__ uint32_t magnitude(float y) { return __float_as_uint(y) & 0x7fffffffu; }
 
-// Q8_0 block scale of a block whose largest magnitude is `most`; a value v has
-// the code round_away(v * inv), within [-limit, limit] once v is cut to
-// +-*limit (infinite unless the scale saturates).
+__device__ __forceinline__ float rcp_fast(float v) {  // within 1 ulp
+  float r;
+  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(v));
+  return r;
+}
+
+// Q8_0 scale d of a block whose largest magnitude is `most`, and inv = 1 / d.  The two
+// divisions of the rule are a product with 1/127 and an approximate reciprocal, each
+// within an ulp (they were a tenth of the instructions).  `limit` is where values are
+// cut: finite only if the scale saturates, 0 for a block with a NaN or an infinity.
 __device__ __forceinline__ __half q8_scale(uint32_t most, float& inv, float& limit) {
+  float d = __uint_as_float(most) * (1.0f / 127.0f);
   limit = INFINITY;
-  inv = 0.f;
   if (most >= 0x7f800000u) {
-    limit = 0.f;
+    limit = inv = 0.f;
     return __ushort_as_half(0x7fff);
   }
-  float d = __uint_as_float(most) / 127.0f;
   if (d > 65504.0f) {
     d = 65504.0f;
     limit = 127.0f * 65504.0f;
   }
-  if (d > 0.f) inv = 1.0f / d;
+  inv = d > 1e-30f ? rcp_fast(d) : 0.f;  // (as f16 it is 0 long before)
   return __float2half_rn(d);
 }
 
-__device__ __forceinline__ int q8_code(float y, float inv, float limit) {
-  if (limit != INFINITY) y = limit == 0.f ? 0.f : fminf(fmaxf(y, -limit), limit);
-  return round_away(y * inv);
+__device__ __forceinline__ float q8_cut(float y, float limit) {
+  return limit == 0.f ? 0.f : fminf(fmaxf(y, -limit), limit);
 }
 
 // One CTA per row, element by element, reading the row twice: what the kernel
@@ -124,7 +129,7 @@ __global__ void __launch_bounds__(kNormThreads) rms_norm_loop_kernel(const NormA
   }
   ss = block_sum(ss, red);
   const bool plain = plain_square_sum(ss);
-  float inv = 1.0f / sqrtf(ss / static_cast<float>(a.hidden) + a.eps);
+  float inv = rsqrtf(fmaf(ss, a.inv_hidden, a.eps));  // within 2 ulp
   double inv_d = 0.0;
   if (!plain) {
     double sd = 0.0;
@@ -149,7 +154,8 @@ __global__ void __launch_bounds__(kNormThreads) rms_norm_loop_kernel(const NormA
       if (i < a.hidden) {
         float id, limit;
         const __half d = q8_scale(m, id, limit);
-        static_cast<int8_t*>(a.out)[oo + i] = static_cast<int8_t>(q8_code(y, id, limit));
+        if (limit != INFINITY) y = q8_cut(y, limit);
+        static_cast<int8_t*>(a.out)[oo + i] = static_cast<int8_t>(round_away(y * id));
         if (i % 32 == 0) a.out_scale[(oo + i) / 32] = d;
       }
     }
@@ -277,7 +283,7 @@ __global__ void __launch_bounds__(NV == 1 ? 1024 : 512, NV == 1 ? 1 : 2)
     }
   }
   ss = block_sum(ss, red);
-  float inv = 1.0f / sqrtf(ss / static_cast<float>(a.hidden) + a.eps);
+  float inv = rsqrtf(fmaf(ss, a.inv_hidden, a.eps));  // within 2 ulp
   if (!plain_square_sum(ss)) {
     // the same for every thread: 64 bits, and s becomes s * inv here
     double sd = 0.0;
@@ -322,9 +328,13 @@ __global__ void __launch_bounds__(NV == 1 ? 1024 : 512, NV == 1 ? 1 : 2)
     m = max(m, __shfl_xor_sync(0xffffffffu, m, 2));
     float id, limit;
     const __half d = q8_scale(m, id, limit);
+    if (limit != INFINITY) {
+#pragma unroll
+      for (int e = 0; e < 8; ++e) y[e] = q8_cut(y[e], limit);
+    }
     uint32_t q[8];
 #pragma unroll
-    for (int e = 0; e < 8; ++e) q[e] = static_cast<uint32_t>(q8_code(y[e], id, limit));
+    for (int e = 0; e < 8; ++e) q[e] = static_cast<uint32_t>(round_away(y[e] * id));
     if (in) {
       uint2 w;
       w.x = __byte_perm(__byte_perm(q[0], q[1], 0x0040), __byte_perm(q[2], q[3], 0x0040), 0x5410);
@@ -1194,6 +1204,7 @@ int ql_rms_norm(ql_ctx* c, const ql_norm_args* args) {
   a.residual_stride = rs;
   a.rows = f.rows;
   a.hidden = f.hidden;
+  a.inv_hidden = 1.0f / static_cast<float>(f.hidden);
   a.in_dtype = f.in_dtype;
   a.weight_dtype = f.weight_dtype;
   a.out_dtype = f.out_dtype;
