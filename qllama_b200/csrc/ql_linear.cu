@@ -225,22 +225,30 @@ __device__ __forceinline__ void store_part(void* base, size_t i, int dt, const f
 // in every contiguous tensor, whatever its type -- and only the row's first and
 // last go element by element (2000 rows of 4101 bf16 columns: 52.8 us with
 // element-wise loads throughout).
+// WARP: a warp per row, kNormRows rows to a CTA, for many short rows (8000 x 128 bf16
+// 8.6 us with a CTA for each, 4.8 us so; 8000 x 1000 12.7 us and 15.4 us).
 constexpr int kNormMax = 16384;  // 512 threads x 32 columns
-template <int DT, int WT, int NV, bool LEAD>
-__global__ void __launch_bounds__(NV == 1 ? 1024 : 512, NV == 1 ? 1 : 2)
+constexpr int kNormRows = 8;
+template <int DT, int WT, int NV, bool LEAD, bool WARP>
+__global__ void __launch_bounds__(WARP ? 32 * kNormRows : NV == 1 ? 1024 : 512,
+                                  !WARP && NV > 1 ? 2 : 1)
     rms_norm_kernel(const NormArgs a) {
   __shared__ float red[32];
   __shared__ double red_d[32];
-  const size_t row = blockIdx.x;
+  const size_t row = WARP ? blockIdx.x * static_cast<size_t>(kNormRows) + threadIdx.x / 32
+                          : blockIdx.x;
+  const int thread = WARP ? threadIdx.x % 32 : threadIdx.x;
+  const int threads = WARP ? 32 : blockDim.x;
   const size_t oo = row * static_cast<size_t>(a.hidden);
   const int lead = LEAD ? static_cast<int>(oo % 8) : 0;
   ql::griddep_wait();
   ql::griddep_launch_dependents();
+  if (WARP && row >= static_cast<size_t>(a.rows)) return;
   // where x and the residual fill the registers, the weight is left for later
   constexpr bool kEarly = NV * (DT == ql::kF32 ? 2 : 1) < 4;
   Raw8<DT> xr[NV], rr[NV];
   Raw8<WT> wr[NV];
-  auto column = [&](int j) { return 8 * static_cast<int>(threadIdx.x + j * blockDim.x) - lead; };
+  auto column = [&](int j) { return 8 * (thread + j * threads) - lead; };
   auto read = [&](auto& r, const void* base, size_t at, int c, bool whole) {
     if (!LEAD || whole) r.load(base, at + c);
     else r.load_part(base, at + c, c < 0 ? -c : 0, min(8, a.hidden - c));
@@ -282,7 +290,7 @@ __global__ void __launch_bounds__(NV == 1 ? 1024 : 512, NV == 1 ? 1 : 2)
       for (int e = 0; e < 8; ++e) s[j][e] = 0.f;
     }
   }
-  ss = block_sum(ss, red);
+  ss = WARP ? warp_sum(ss) : block_sum(ss, red);
   float inv = rsqrtf(fmaf(ss, a.inv_hidden, a.eps));  // within 2 ulp
   if (!plain_square_sum(ss)) {
     // the same for every thread: 64 bits, and s becomes s * inv here
@@ -291,8 +299,8 @@ __global__ void __launch_bounds__(NV == 1 ? 1024 : 512, NV == 1 ? 1 : 2)
     for (int j = 0; j < NV; ++j)
 #pragma unroll
       for (int e = 0; e < 8; ++e) sd += static_cast<double>(s[j][e]) * s[j][e];
-    const double id =
-        1.0 / sqrt(block_sum(sd, red_d) / a.hidden + static_cast<double>(a.eps));
+    sd = WARP ? warp_sum(sd) : block_sum(sd, red_d);
+    const double id = 1.0 / sqrt(sd / a.hidden + static_cast<double>(a.eps));
 #pragma unroll
     for (int j = 0; j < NV; ++j)
 #pragma unroll
@@ -381,16 +389,20 @@ cudaError_t launch_norm(const NormArgs& a, int num_sms, cudaStream_t s) {
   if (!bases || !(even || lead) || a.hidden > kNormMax - 8)
     return launch_pdl(rms_norm_loop_kernel, dim3(a.rows), dim3(kNormThreads), 0, s, true, a);
   const int groups = (a.hidden + 7) / 8 + lead;
-  int nv = groups <= 1024 ? 1 : 4;
+  const bool warp = groups <= 64 && a.rows >= 4 * num_sms;
+  int nv = warp ? (groups <= 32 ? 1 : 2) : groups <= 1024 ? 1 : 4;
   if (nv == 1 && a.rows >= 2 * num_sms && groups >= 256) nv = 2;
-  const int threads = ((groups + nv - 1) / nv + 31) / 32 * 32;
-  const dim3 grid(a.rows), block(threads);
+  const dim3 block(warp ? 32 * kNormRows : ((groups + nv - 1) / nv + 31) / 32 * 32);
+  const dim3 grid(warp ? (a.rows - 1) / kNormRows + 1 : a.rows);
   auto go = [&](auto dt, auto wt, auto ld) {
     constexpr int DT = decltype(dt)::value, WT = decltype(wt)::value;
     constexpr bool LEAD = decltype(ld)::value;
-    if (nv == 1) return launch_pdl(rms_norm_kernel<DT, WT, 1, LEAD>, grid, block, 0, s, true, a);
-    if (nv == 2) return launch_pdl(rms_norm_kernel<DT, WT, 2, LEAD>, grid, block, 0, s, true, a);
-    return launch_pdl(rms_norm_kernel<DT, WT, 4, LEAD>, grid, block, 0, s, true, a);
+    auto* const kernel = warp ? (nv == 1 ? rms_norm_kernel<DT, WT, 1, LEAD, true>
+                                         : rms_norm_kernel<DT, WT, 2, LEAD, true>)
+                         : nv == 1 ? rms_norm_kernel<DT, WT, 1, LEAD, false>
+                         : nv == 2 ? rms_norm_kernel<DT, WT, 2, LEAD, false>
+                                   : rms_norm_kernel<DT, WT, 4, LEAD, false>;
+    return launch_pdl(kernel, grid, block, 0, s, true, a);
   };
   auto by_lead = [&](auto dt, auto wt) {
     return lead ? go(dt, wt, std::true_type()) : go(dt, wt, std::false_type());
@@ -656,6 +668,15 @@ __device__ __forceinline__ void mma_f(float (&d)[4], const uint32_t (&a)[4], uin
         : "=f"(d[0]), "=f"(d[1]), "=f"(d[2]), "=f"(d[3])
         : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1), "f"(c0), "f"(c1), "f"(c2),
           "f"(c3));
+}
+
+// D = A B + c of one m16n8k32 with the same addend everywhere.
+__device__ __forceinline__ void mma_s8(int (&d)[4], const uint4& a, uint32_t b0, uint32_t b1,
+                                       int c) {
+  asm("mma.sync.aligned.m16n8k32.row.col.s32.s8.s8.s32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, "
+      "{%8,%9}, {%10,%10,%10,%10};"
+      : "=r"(d[0]), "=r"(d[1]), "=r"(d[2]), "=r"(d[3])
+      : "r"(a.x), "r"(a.y), "r"(a.z), "r"(a.w), "r"(b0), "r"(b1), "r"(c));
 }
 
 // Asynchronous copies of this lane's bytes into shared memory; the first `bytes`
@@ -943,8 +964,8 @@ __global__ void __launch_bounds__(kRanges* WR * 32, 1) linear_q4_kernel(const Li
         for (int q = 0; q < NT; ++q) {
           // sums start at the bits of 1.5 * 2^23: below 2^22 they are the
           // mantissa of a float, and a subtraction converts them
-          int d[4] = {0x4b400000, 0x4b400000, 0x4b400000, 0x4b400000};
-          ql::mma16832_s8(d, A, x[q][j][0], x[q][j][1]);
+          int d[4];
+          mma_s8(d, A, x[q][j][0], x[q][j][1], 0x4b400000);
 #pragma unroll
           for (int h = 0; h < 2; ++h) {
             const float sh = h ? s[j].y : s[j].x;

@@ -128,6 +128,26 @@ def test_norm_q8(ctx, rows, hidden, dt, residual):
     check_q8(q, d, norm_f64(x, r, w, 1e-6)[0], norm_tol(hidden))
 
 
+@pytest.mark.parametrize("hidden", [1, 7, 64, 96, 300, 512])
+@pytest.mark.parametrize("dt", ["f32", "f16", "bf16"])
+def test_norm_many_short_rows(ctx, hidden, dt):
+    """Rows that share a CTA, the last CTA not full."""
+    g = gen(hidden)
+    x, r = randn(g, 1201, hidden).to(DT[dt]), randn(g, 1201, hidden).to(DT[dt])
+    x[5] *= 1e-3 if dt == "f16" else 1e-30
+    w = 1 + 0.2 * randn(g, hidden)
+    total = torch.empty_like(x)
+    y = qm.rms_norm(ctx, x, w, 1e-5, residual=r, sum_out=total)
+    ctx.synchronize()
+    ref, s = norm_f64(x, r, w, 1e-5)
+    assert ((y.double() - ref).abs() <= ref.abs() * (norm_tol(hidden) + u(dt)) + least(dt)).all()
+    assert ((total.double() - s).abs() <= s.abs() * (u(dt) + 2 * U32) + least(dt)).all()
+    if hidden % 32 == 0:
+        q, d = qm.rms_norm(ctx, x, w, 1e-5, out_dtype="q8_0")
+        ctx.synchronize()
+        check_q8(q, d, norm_f64(x, None, w, 1e-5)[0], norm_tol(hidden))
+
+
 @pytest.mark.parametrize("hidden", [64, 4096, 4100])
 def test_norm_strides_and_in_place(ctx, hidden):
     g = gen(hidden)
