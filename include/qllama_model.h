@@ -167,9 +167,9 @@ int ql_llama_generate(ql_llama* m, ql_kv* kv, int32_t seq, const int32_t* prompt
  *
  * x and residual have x_stride / residual_stride elements from row to row
  * (0 = hidden); sum_out, out and out_scale are contiguous.  sum_out may be x
- * or residual itself, and out may be x, residual or neither, where the
- * strides (and for out the types) are the same; any other overlap is not
- * supported.  Device pointers, aligned to their element size. */
+ * or residual itself, and so may out, where the strides (and for out the types)
+ * are the same; any other overlap of an output is refused.  Device pointers,
+ * aligned to their element size. */
 typedef struct {
   int32_t rows;          /* 0 is a no-op */
   int32_t hidden;        /* a multiple of 32 for Q8_0 */
@@ -194,7 +194,7 @@ int ql_rms_norm(ql_ctx* ctx, const ql_norm_args* args);
  *   w[n][k] = scale[n][k / group] * (code[n][k] - 8),  0 <= code <= 15.
  * Group 32 is GGUF's Q4_0.  The handle holds the matrix on the context's
  * device in the order the product kernel streams it (in_features is a
- * multiple of the group; rows are padded to 16, columns to 64). */
+ * multiple of the group, at most 2^24; rows are padded to 16, columns to 64). */
 typedef struct ql_q4 ql_q4;
 int ql_q4_create(ql_ctx* ctx, int32_t out_features, int32_t in_features, int32_t group,
                  ql_q4** out);
@@ -224,7 +224,8 @@ int ql_q4_get(const ql_q4* w, uint8_t* codes, void* scales, int32_t mem);
  * layers.rs:148-171): single tokens, drafted tokens, small batches.  The
  * kernel is built for up to some 64 rows, where the weights' bytes are the cost;
  * more rows are taken in passes of that size.
- *   in_dtype F32, F16, BF16: x as given, every product with a code exact;
+ *   in_dtype F32, F16, BF16: x as given, every product with a code exact (an
+ *     infinity in an F32 row gives NaN);
  *   in_dtype Q8_0: int8 values with x_scale [rows, in_features/32] f16, the
  *     output of ql_rms_norm (integer products, exact per block of 32).
  * Sums are f32; y [rows, out_features] is rounded once to out_dtype.  A row's

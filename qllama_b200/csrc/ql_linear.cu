@@ -1121,9 +1121,9 @@ cudaError_t launch_linear_as(const LinearArgs& a, int num_sms, bool pdl, cudaStr
   cudaError_t e = ql_once_per_device(done, [&] {
     return cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, C::kSmem);
   });
-  for (int r = 0; e == cudaSuccess && r < a.rows; r += 65535 * C::kRows) {  // grid.y's limit
+  for (int64_t r = 0; e == cudaSuccess && r < a.rows; r += 65535 * C::kRows) {  // grid.y's limit
     LinearArgs b = a;
-    b.rows = std::min(a.rows - r, 65535 * C::kRows);
+    b.rows = static_cast<int>(std::min<int64_t>(a.rows - r, 65535 * C::kRows));
     const size_t xb = type_bytes(a.in_dtype), yb = type_bytes(a.out_dtype);
     b.x = static_cast<const char*>(a.x) + static_cast<size_t>(r) * a.x_stride * xb;
     b.x_scale = a.x_scale ? a.x_scale + static_cast<size_t>(r) * (a.w.k / 32) : nullptr;
@@ -1135,7 +1135,7 @@ cudaError_t launch_linear_as(const LinearArgs& a, int num_sms, bool pdl, cudaStr
 }
 
 // B tiles by the rows of x.  Two teams of warps (16 warps hide more latency: 1 x 8192 ->
-// 57344 f16 55 us, 59 us with one) unless the SMs have no second tile for the second
+// 57344 f16 55 us, 59 us with one, both before later steps brought it to 52) unless the SMs have no second tile for the second
 // team (1 x 2048 -> 2048 Q8_0 2.8 us with one team, 3.2 us with two).  With four B
 // tiles the sums fill the registers of one team (32 x 8192 -> 28672 f16 64 us, 116 us
 // with two teams of half the tiles), eight tiles at a time where a CTA has more than
@@ -1190,6 +1190,7 @@ int ql_rms_norm(ql_ctx* c, const ql_norm_args* args) {
   const ql_norm_args& f = *args;
   if (f.rows < 0) return ql_fail(QL_ERR_INVALID, "row count %d is negative", f.rows);
   if (f.hidden <= 0) return ql_fail(QL_ERR_INVALID, "hidden must be positive, got %d", f.hidden);
+  if (f.hidden > (1 << 30)) return ql_fail(QL_ERR_UNSUPPORTED, "hidden %d is too large", f.hidden);
   if (!float_type(f.in_dtype) || !float_type(f.weight_dtype) ||
       !(float_type(f.out_dtype) || f.out_dtype == QL_Q8_0))
     return ql_fail(QL_ERR_INVALID, "unsupported element types %d, %d -> %d", f.in_dtype,
@@ -1212,6 +1213,31 @@ int ql_rms_norm(ql_ctx* c, const ql_norm_args* args) {
       !aligned(f.weight, type_bytes(f.weight_dtype)) || !aligned(f.out, type_bytes(f.out_dtype)) ||
       !aligned(f.out_scale, 2))
     return ql_fail(QL_ERR_INVALID, "ql_rms_norm: a buffer is not aligned to its element size");
+  // Outputs may be inputs, element on element, and nothing else may overlap.
+  struct Span {
+    const char* p;
+    size_t bytes;
+    int64_t stride;
+    int dtype;
+  };
+  auto span = [&](const void* p, int64_t stride, int dt) {
+    const size_t n = static_cast<size_t>(stride) * (f.rows - 1) + f.hidden;
+    return Span{static_cast<const char*>(p), p ? n * type_bytes(dt) : 0, f.rows > 1 ? stride : 0, dt};
+  };
+  auto clash = [](const Span& a, const Span& b, bool same) {
+    if (!a.bytes || !b.bytes || a.p >= b.p + b.bytes || b.p >= a.p + a.bytes) return false;
+    return !(same && a.p == b.p && a.stride == b.stride && a.dtype == b.dtype);
+  };
+  const Span in[] = {span(f.x, xs, f.in_dtype), span(f.residual, rs, f.in_dtype)};
+  const Span w{static_cast<const char*>(f.weight), f.hidden * type_bytes(f.weight_dtype), 0, -1};
+  const Span outs[] = {span(f.sum_out, f.hidden, f.in_dtype), span(f.out, f.hidden, f.out_dtype),
+                       Span{static_cast<const char*>(f.out_scale),
+                            f.out_dtype == QL_Q8_0 ? static_cast<size_t>(f.rows) * (f.hidden / 32) * 2 : 0,
+                            0, -1}};
+  bool bad = clash(outs[0], outs[1], false) || clash(outs[0], outs[2], false) ||
+             clash(outs[1], outs[2], false);
+  for (const Span& o : outs) bad |= clash(o, w, false) || clash(o, in[0], true) || clash(o, in[1], true);
+  if (bad) return ql_fail(QL_ERR_INVALID, "ql_rms_norm: an output overlaps another buffer");
   ql_device_guard dev(c->device);
   QLN_CUDA(dev.error(), "set device");
   NormArgs a{};
@@ -1246,7 +1272,7 @@ int ql_q4_create(ql_ctx* c, int32_t out_features, int32_t in_features, int32_t g
   if (in_features % group != 0)
     return ql_fail(QL_ERR_INVALID, "in_features %d must be divisible by the group %d", in_features,
                    group);
-  if (out_features > (1 << 30) || in_features > (1 << 30))
+  if (out_features > (1 << 30) || in_features > (1 << 24))
     return ql_fail(QL_ERR_UNSUPPORTED, "weight dimensions [%d, %d] are too large", out_features,
                    in_features);
   ql_device_guard dev(c->device);

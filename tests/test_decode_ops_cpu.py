@@ -36,7 +36,7 @@ def refused(rc, text, code=qb.ERR_INVALID):
 
 
 NORM = dict(rows=2, hidden=64, in_dtype=qb.F32, weight_dtype=qb.F32, out_dtype=qb.F32, eps=1e-5,
-            x=P, weight=P, out=P)
+            x=P, weight=P + 512, out=P)
 
 
 @pytest.mark.parametrize("change, text", [
@@ -47,7 +47,12 @@ NORM = dict(rows=2, hidden=64, in_dtype=qb.F32, weight_dtype=qb.F32, out_dtype=q
     (dict(residual=P, residual_stride=8), "stride"), (dict(x=None), "NULL"),
     (dict(weight=None), "NULL"), (dict(out=None), "NULL"), (dict(out_dtype=qb.Q8_0), "NULL"),
     (dict(x=P + 2), "aligned"), (dict(residual=P + 1), "aligned"), (dict(out=P + 2), "aligned"),
-    (dict(out_dtype=qb.Q8_0, out_scale=P + 1), "aligned")])
+    (dict(out_dtype=qb.Q8_0, out_scale=P + 1), "aligned"),
+    (dict(out=P + 4), "overlaps"), (dict(residual=P, sum_out=P), "overlaps"),
+    (dict(x_stride=128), "overlaps"), (dict(out=P + 1024, weight=P + 1200), "overlaps"),
+    (dict(in_dtype=qb.F16), "overlaps"),
+    (dict(out_dtype=qb.Q8_0, out=P + 1024, out_scale=P + 1024), "overlaps"),
+    (dict(residual=P, sum_out=P + 1024, out=P + 1024), "overlaps")])
 def test_norm_refusals(change, text):
     a = qm.NormArgs(**{**NORM, **change})
     refused(qb.load().ql_rms_norm(ctypes.byref(CTX), ctypes.byref(a)), text)
@@ -65,6 +70,14 @@ def test_weight_refusals(n, k, group, text):
     h = ctypes.c_void_p()
     refused(qb.load().ql_q4_create(ctypes.byref(CTX), n, k, group, ctypes.byref(h)), text)
     assert not h.value
+
+
+def test_sizes_beyond_the_kernels_are_refused():
+    L, h = qb.load(), ctypes.c_void_p()
+    refused(L.ql_q4_create(ctypes.byref(CTX), 8, (1 << 24) + 32, 32, ctypes.byref(h)), "too large",
+            qb.ERR_UNSUPPORTED)
+    a = qm.NormArgs(**{**NORM, "hidden": (1 << 30) + 32})
+    refused(L.ql_rms_norm(ctypes.byref(CTX), ctypes.byref(a)), "too large", qb.ERR_UNSUPPORTED)
 
 
 def test_weight_value_refusals():
