@@ -427,7 +427,7 @@ class Q4Weight:
     def _buffer(self, x, dtype, name: str):
         """(pointer, memory kind, keep-alive) of an array or a CUDA tensor."""
         qb = _qb()
-        if dtype and not str(x.dtype).endswith(dtype):
+        if dtype and str(x.dtype).split(".")[-1] != dtype:  # bfloat16 ends in float16
             raise _invalid(f"{name} must be {dtype}, got {x.dtype}")
         if not isinstance(x, np.ndarray):
             if not x.is_cuda:

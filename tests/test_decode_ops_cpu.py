@@ -80,6 +80,16 @@ def test_sizes_beyond_the_kernels_are_refused():
     refused(L.ql_rms_norm(ctypes.byref(CTX), ctypes.byref(a)), "too large", qb.ERR_UNSUPPORTED)
 
 
+@pytest.mark.parametrize("dtype", ["bfloat16", "float32", "int16"])
+def test_scales_of_another_type_are_refused(dtype):
+    torch = pytest.importorskip("torch")
+    q = object.__new__(qm.Q4Weight)
+    with pytest.raises(qb.QllamaError, match="scales must be float16"):
+        q._buffer(torch.zeros(4, 2, dtype=getattr(torch, dtype)), "float16", "scales")
+    p, mem, keep = q._buffer(torch.zeros(4, 2, dtype=torch.float16), "float16", "scales")
+    assert p == keep.data_ptr() and mem == qb.MEM_HOST
+
+
 def test_weight_value_refusals():
     L, w, w64 = qb.load(), q4(), q4(group=64)
     refused(L.ql_q4_set(ctypes.byref(w), None, P, 0), "NULL")
