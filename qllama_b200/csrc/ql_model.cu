@@ -994,7 +994,9 @@ int forward_q4(ql_llama* m, ql_kv* kv, int32_t seq, const int32_t* ids, int n, i
     a.k = m->qkv + E;
     a.v = m->qkv + E + kvd;
     a.out = m->att;
-    if (n > 1) {  // the operator takes q, k and v as three contiguous tensors
+    // the operator takes q, k and v as three contiguous tensors (k and v of one row
+    // lie on 16 bytes if kvd is a multiple of four)
+    if (n > 1 || kvd % 4 != 0) {
       const size_t ld = static_cast<size_t>(m->qkv_cols) * 4;
       const struct {
         float* to;
