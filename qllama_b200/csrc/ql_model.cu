@@ -206,8 +206,8 @@ cudaError_t launch_gemm(const GemmArgs& g, cudaStream_t s) {
 
 // SwiGLU over the fused gate and up products [n, 2F]: silu(gate) * up.
 __global__ void __launch_bounds__(256) silu_mul_kernel(const float* gu, int F, float* out) {
-  const size_t row = blockIdx.y;
-  const int i = blockIdx.x * 256 + threadIdx.x;
+  const size_t row = blockIdx.x;  // not y: a prompt may have more than 65535 tokens
+  const int i = blockIdx.y * 256 + threadIdx.x;
   if (i >= F) return;
   const float* p = gu + row * 2 * static_cast<size_t>(F);
   out[row * F + i] = __fmul_rn(silu_ref(p[i]), p[F + i]);
@@ -1018,7 +1018,7 @@ int forward_q4(ql_llama* m, ql_kv* kv, int32_t seq, const int32_t* ids, int n, i
     if ((r = linear(m, Q.wo, m->att, n, m->t)) != QL_OK) return r;
     if ((r = norm_q8(m, m->x, m->t, L.ffn_norm, n)) != QL_OK) return r;
     if ((r = linear(m, Q.gate_up, nullptr, n, m->gu)) != QL_OK) return r;
-    silu_mul_kernel<<<dim3((F + 255) / 256, n), 256, 0, s>>>(m->gu, F, m->g);
+    silu_mul_kernel<<<dim3(n, (F + 255) / 256), 256, 0, s>>>(m->gu, F, m->g);
     QLM_CUDA(cudaGetLastError(), "launch SwiGLU");
     if ((r = linear(m, Q.down, m->g, n, m->t)) != QL_OK) return r;
   }

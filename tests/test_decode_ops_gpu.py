@@ -858,6 +858,27 @@ def test_quantized_model_refusals(ctx):
         c.close()
 
 
+def test_quantized_model_takes_a_prompt_of_more_than_65535_tokens(ctx):
+    """Without an attention output each row's logits are those of its token alone."""
+    n, V = 65537, 32
+    cfg = dict(vocab=V, dim=64, ff=96, heads=1, kv_heads=1, layers=1, max_pos=n, eps=1e-5,
+               theta=10000.0)
+    tensors = mu.c1_weights(seed=5, cfg=cfg)
+    m = qm.Llama(ctx, qm.LlamaConfig(V, 64, 96, 1, 1, 1, n, 1e-5, 10000.0))
+    for name, a in tensors.items():
+        m.set_tensor(name, np.zeros_like(a) if name.endswith("attn_output.weight") else a)
+    m.quantize(32)
+    ids = np.arange(n) % V
+    kv = m.kv_cache(dtype="f16")
+    got = np.asarray(m.forward_with_cache(ids, 0, kv)).reshape(-1, V)
+    for row in {0, len(got) // 2, len(got) - 1}:
+        kv.clear()
+        alone = np.asarray(m.forward_with_cache([ids[n - len(got) + row]], 0, kv)).reshape(V)
+        assert np.array_equal(got[row].view(np.uint32), alone.view(np.uint32))
+    for c in (kv, m):
+        c.close()
+
+
 @pytest.mark.parametrize("sampled", [False, True])
 def test_drafted_generation_on_a_quantized_model(ctx, sampled):
     """Drafts, some right and some wrong, verified step by step with the rejected
