@@ -17,9 +17,11 @@ namespace {
 #define QLN_CUDA(call, what)                                                                   \
   do {                                                                                         \
     cudaError_t e_ = (call);                                                                   \
-    if (e_ != cudaSuccess)                                                                     \
+    if (e_ != cudaSuccess) {                                                                   \
+      cudaGetLastError(); /* a refused allocation is not the next launch's error */            \
       return ql_fail(e_ == cudaErrorMemoryAllocation ? QL_ERR_OOM : QL_ERR_CUDA, "%s: %s",    \
                      what, cudaGetErrorString(e_));                                            \
+    }                                                                                          \
   } while (0)
 
 bool float_type(int dt) { return dt == QL_F32 || dt == QL_F16 || dt == QL_BF16; }
@@ -1292,6 +1294,7 @@ int ql_q4_create(ql_ctx* c, int32_t out_features, int32_t in_features, int32_t g
   if (e == cudaSuccess) e = cudaMemsetAsync(w->scales, 0, q4_scales(w) * 2, c->stream);
   if (e != cudaSuccess) {
     ql_q4_destroy(w);
+    cudaGetLastError();
     return ql_fail(e == cudaErrorMemoryAllocation ? QL_ERR_OOM : QL_ERR_CUDA,
                    "allocate a 4-bit weight: %s", cudaGetErrorString(e));
   }

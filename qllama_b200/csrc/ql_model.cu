@@ -1268,6 +1268,7 @@ int ql_llama_quantize(ql_llama* m, int32_t group) {
     cudaStreamSynchronize(s);
     if (pair) cudaFree(pair);
     free_q4(m);
+    cudaGetLastError();  // a refused allocation is not the next launch's error
     return ql_fail(r, "%s", msg.c_str());
   }
   cudaFree(pair);

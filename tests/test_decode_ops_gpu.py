@@ -879,6 +879,18 @@ def test_quantized_model_takes_a_prompt_of_more_than_65535_tokens(ctx):
         c.close()
 
 
+def test_a_refused_allocation_is_not_the_next_calls_error(ctx):
+    with pytest.raises(qb.QllamaError) as e:  # 2^53 bytes of codes
+        qm.Q4Weight(ctx, shape=(1 << 30, 1 << 24, 32))
+    assert e.value.code == qb.ERR_OOM
+    codes, scales = random_weight(gen(2), 8, 64, 32)
+    w = qm.Q4Weight(ctx, codes, scales)  # its launch check reads the last error
+    got = w.get()
+    ctx.synchronize()
+    assert np.array_equal(got[0], codes.cpu().numpy())
+    w.close()
+
+
 @pytest.mark.parametrize("sampled", [False, True])
 def test_drafted_generation_on_a_quantized_model(ctx, sampled):
     """Drafts, some right and some wrong, verified step by step with the rejected
