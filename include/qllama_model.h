@@ -278,7 +278,8 @@ int ql_llama_quantize(ql_llama* m, int32_t group);
  * new token is -1 and the context's status is raised (QL_ERR_DEVICE at the next
  * synchronize).  (Of probabilities, an accepted draft's rows are read at its id
  * alone.)  ql_kv_truncate then drops the rejected drafts' cache rows.
- * Device pointers, aligned to their element size. */
+ * tokens and accepted must not overlap each other or an input.  Device pointers,
+ * aligned to their element size. */
 #define QL_VERIFY_LOGITS 0
 #define QL_VERIFY_PROBS 1
 #define QL_VERIFY_MAX_DRAFTS 31
