@@ -44,6 +44,7 @@ int fail(int code, const char* fmt, ...) {
 }
 
 int cuda_fail(cudaError_t e, const char* what) {
+  cudaGetLastError();  // a refused allocation is not the next launch's error
   return fail(e == cudaErrorMemoryAllocation ? QL_ERR_OOM : QL_ERR_CUDA, "%s: %s", what,
               cudaGetErrorString(e));
 }

@@ -59,9 +59,11 @@ namespace {
 #define QLM_CUDA(call, what)                                                                   \
   do {                                                                                         \
     cudaError_t e_ = (call);                                                                   \
-    if (e_ != cudaSuccess)                                                                     \
+    if (e_ != cudaSuccess) {                                                                   \
+      cudaGetLastError(); /* a refused allocation is not the next launch's error */            \
       return ql_fail(e_ == cudaErrorMemoryAllocation ? QL_ERR_OOM : QL_ERR_CUDA, "%s: %s",    \
                      what, cudaGetErrorString(e_));                                            \
+    }                                                                                          \
   } while (0)
 
 // ------------------------------------------------------------------ kernels --
@@ -884,8 +886,7 @@ int ensure_rows(ql_llama* m, int rows) {
     cudaError_t e = cudaMalloc(b.p, std::max<size_t>(b.bytes, 256));
     if (e != cudaSuccess) {
       free_work(m);
-      return ql_fail(e == cudaErrorMemoryAllocation ? QL_ERR_OOM : QL_ERR_CUDA,
-                     "allocate the model workspace: %s", cudaGetErrorString(e));
+      QLM_CUDA(e, "allocate the model workspace");
     }
   }
   m->rows = rows;
@@ -1268,7 +1269,6 @@ int ql_llama_quantize(ql_llama* m, int32_t group) {
     cudaStreamSynchronize(s);
     if (pair) cudaFree(pair);
     free_q4(m);
-    cudaGetLastError();  // a refused allocation is not the next launch's error
     return ql_fail(r, "%s", msg.c_str());
   }
   cudaFree(pair);

@@ -15,8 +15,10 @@ namespace {
 #define QLV_CUDA(call, what)                                                      \
   do {                                                                            \
     cudaError_t e_ = (call);                                                      \
-    if (e_ != cudaSuccess)                                                        \
+    if (e_ != cudaSuccess) {                                                      \
+      cudaGetLastError(); /* not the next launch's error */                       \
       return ql_fail(QL_ERR_CUDA, "%s: %s", what, cudaGetErrorString(e_));        \
+    }                                                                             \
   } while (0)
 
 struct VerifyArgs {

@@ -6,6 +6,8 @@ them on a quantized model.
 Tolerances count roundings: u(t) = eps(t) / 2 is the most that one rounding to t
 moves a value, relative to it.
 """
+import ctypes
+
 import numpy as np
 import pytest
 import torch
@@ -889,6 +891,31 @@ def test_a_refused_allocation_is_not_the_next_calls_error(ctx):
     ctx.synchronize()
     assert np.array_equal(got[0], codes.cpu().numpy())
     w.close()
+
+
+def test_a_refused_workspace_or_cache_is_not_the_next_calls_error(ctx):
+    """A forward whose workspace (210 GB of logits) is refused, and a cache that is, leave
+    the next calls as they were."""
+    n, V = 1 << 17, 400000
+    m = qm.Llama(ctx, qm.LlamaConfig(V, 64, 96, 1, 1, 1, n, 1e-5, 10000.0))
+    kv = m.kv_cache(dtype="f16")
+    L, ids = qb.load(), (ctypes.c_int32 * n)()
+
+    def forward(tokens):
+        rc = L.ql_llama_forward(m._h, kv._h, 0, ids, tokens, kv.seq_len(), None, qb.MEM_HOST)
+        return rc, L.ql_last_error().decode()
+
+    rc, message = forward(n)
+    assert rc == qb.ERR_OOM and "workspace" in message
+    rc, message = forward(3)
+    assert rc == qb.OK, message
+    with pytest.raises(qb.QllamaError) as e:  # 2^45 bytes a layer
+        qb.KvCache(ctx, 1, 1 << 30, 64, 128, "f32")
+    assert e.value.code == qb.ERR_OOM
+    rc, message = forward(3)
+    assert rc == qb.OK, message
+    for c in (kv, m):
+        c.close()
 
 
 @pytest.mark.parametrize("sampled", [False, True])
