@@ -34,7 +34,7 @@ struct VerifyArgs {
   int drafts, vocab, dtype, probs;
   double inv_t;  // 1 / temperature; 0: greedy
   double exp_scale;  // 32 / (T ln2)
-  float exp_span;    // (x - m) / T is taken as -infinity below -690
+  double exp_least;  // -690 T: an exponential below exp(-690) is taken as 0
   float exp2_scale;  // 1 / (T ln2)
 };
 
@@ -136,10 +136,11 @@ __device__ __forceinline__ void st_async_f64(uint32_t remote_addr, double v, uin
 // below 1.3e-12).  Lane j holds 2^(j/32), read by shuffles: whole warps call this.
 struct Exp64 {
   double table, scale;
-  float span;
-  // Below it an exponential (under 1e-299) is taken as 0.
-  __device__ __forceinline__ float least(float m) const { return m - span; }
-  __device__ __forceinline__ double operator()(float x, double m, float least) const {
+  // Differences x - m below it (an exponential under 1e-299) give 0.  They are compared
+  // as they are, in f64: m + least in f32 may be a step of the logits too low, where
+  // 2^e no longer is a number of the type.
+  double least;
+  __device__ __forceinline__ double operator()(float x, double m) const {
     constexpr double L = 0.693147180559945309417232 / 32.0;
     constexpr double magic = 6755399441055744.0;  // 1.5 * 2^52
     const double d = static_cast<double>(x) - m;
@@ -152,7 +153,7 @@ struct Exp64 {
     p = fma(p, r, 1.0);
     const int hi = __shfl_sync(0xffffffffu, __double2hiint(table), k) + ((k & ~31) << 15);
     const int lo = __shfl_sync(0xffffffffu, __double2loint(table), k);
-    return x < least ? 0.0 : p * __hiloint2double(hi, lo);
+    return d < least ? 0.0 : p * __hiloint2double(hi, lo);
   }
 };
 
@@ -439,7 +440,7 @@ __global__ void __launch_bounds__(T, T == 1024 ? 1 : 3) verify_kernel(const Veri
     // ---- 3.
     const int lo = static_cast<int>(static_cast<long long>(V) * rank / ctas);
     const int hi = static_cast<int>(static_cast<long long>(V) * (rank + 1) / ctas);
-    const Exp64 ex{pow2_32[lane], a.exp_scale, a.exp_span};
+    const Exp64 ex{pow2_32[lane], a.exp_scale, a.exp_least};
     // warp 0's: sums of the rows at pos, the threshold, the sum before [from, to)
     double zp = 1.0, zq = 1.0, th = 0.0, before = 0.0;
     int turn = 0;
@@ -461,7 +462,6 @@ __global__ void __launch_bounds__(T, T == 1024 ? 1 : 3) verify_kernel(const Veri
         const char* const qrow = row_at(with_q ? n + 1 + z.pos : z.pos);
         const float pm = MODE == kLogits ? row_stat[z.pos].x : 0.f;
         const float qm = MODE == kLogits && with_q ? row_stat[n + 1 + z.pos].x : 0.f;
-        const float pl = ex.least(pm), ql_ = ex.least(qm);
         const int f = share(warp), e = share(warp + 1);
         constexpr int kIds = 4;  // of a lane at a time, their loads in flight together
         constexpr float kEmpty = MODE == kLogits ? -INFINITY : 0.f;
@@ -478,14 +478,14 @@ __global__ void __launch_bounds__(T, T == 1024 ? 1 : 3) verify_kernel(const Veri
 #pragma unroll
           for (int k = 0; k < kIds; ++k) {
             const float x = i0 + 32 * k < e ? xp[k] : kEmpty;
-            wp[k] = MODE == kLogits ? ex(x, pm, pl) : static_cast<double>(x);
+            wp[k] = MODE == kLogits ? ex(x, pm) : static_cast<double>(x);
             wq[k] = 0.0;
           }
           if (with_q) {
 #pragma unroll
             for (int k = 0; k < kIds; ++k) {
               const float x = i0 + 32 * k < e ? xq[k] : kEmpty;
-              wq[k] = MODE == kLogits ? ex(x, qm, ql_) : static_cast<double>(x);
+              wq[k] = MODE == kLogits ? ex(x, qm) : static_cast<double>(x);
             }
           }
 #pragma unroll
@@ -778,7 +778,7 @@ extern "C" int ql_verify_drafts(ql_ctx* c, const ql_verify_args* args) {
   a.probs = probs;
   a.inv_t = probs ? 1.0 : greedy ? 0.0 : 1.0 / static_cast<double>(f.temperature);
   a.exp_scale = a.inv_t * (32.0 / 0.693147180559945309417232);
-  a.exp_span = static_cast<float>(std::fmin(690.0 / a.inv_t, 3e38));
+  a.exp_least = -690.0 / a.inv_t;
   a.exp2_scale = static_cast<float>(std::fmin(a.inv_t / 0.693147180559945309417232, 3e38));
   cudaError_t e;
   if (f.dtype == QL_F32) e = launch_verify<ql::kF32>(a, f.batch, c->num_sms, c->stream);

@@ -562,6 +562,26 @@ def test_verify_rejects_from_nearly_equal_distributions(ctx, V, near):
     assert (a == 0).all()
 
 
+@pytest.mark.parametrize("base, T", [(30.0, 1.6e-9), (30.0, 2.65e-8), (300.0, 3.5e-8),
+                                     (300.0, 4.24e-7), (30.0, 1e-6)])
+def test_verify_temperatures_near_a_step_of_the_logits(ctx, base, T):
+    """Logits some f32 steps below the largest, at temperatures that make their weights
+    too small for 64 bits: they weigh nothing."""
+    g = gen(11)
+    V, B, m = 500, 24, 2
+    step = 2.0 ** -19 if base < 32 else 2.0 ** -15
+
+    def below(*shape):
+        n = torch.randint(0, 14, shape, device="cuda", generator=g)
+        return (base - n.double() * step).float()
+
+    target, draft = below(B, m + 1, V), below(B, m, V)
+    ids = draft.argmax(-1).int()  # (the first of the largest: mostly rejected)
+    un = torch.rand(B, m + 1, dtype=torch.float64, device="cuda", generator=g)
+    a = check_verify(ctx, target, draft, ids, un, T)[1]
+    assert (a < m).any()
+
+
 def test_verify_probabilities_below_f32(ctx):
     """A decision between probabilities that are no f32 numbers any more."""
     target = torch.zeros(2, 2, 50, device="cuda")
