@@ -266,7 +266,8 @@ int ql_llama_quantize(ql_llama* m, int32_t group);
  * form QL_VERIFY_LOGITS: p and q are softmax(logits / temperature); with
  * temperature <= 0 a draft is accepted while it is its row's largest logit (the
  * first of equals), and the new token is the largest of row a (the draft's logits
- * and the uniforms are not read).  Logits of -inf are probability 0.
+ * and the uniforms are not read).  Logits of -inf are probability 0.  A positive
+ * temperature below f32's normal range (1.18e-38) is refused.
  * form QL_VERIFY_PROBS: target and draft hold the probabilities themselves, as
  * the caller's own filters left them (temperature is not read).
  * draft NULL: the drafts are certain (q_i(x_i) = 1), as those looked up in the

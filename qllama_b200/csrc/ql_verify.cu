@@ -3,6 +3,7 @@
 #include <cuda_runtime.h>
 
 #include <algorithm>
+#include <cfloat>
 #include <climits>
 #include <cmath>
 
@@ -745,6 +746,10 @@ extern "C" int ql_verify_drafts(ql_ctx* c, const ql_verify_args* args) {
   if (!probs && !std::isfinite(f.temperature))
     return ql_fail(QL_ERR_INVALID, "Sampler temperature must be finite, got %g",
                    static_cast<double>(f.temperature));
+  // (1 / (T ln2) of a smaller one is no f32 number)
+  if (!probs && f.temperature > 0.f && f.temperature < FLT_MIN)
+    return ql_fail(QL_ERR_UNSUPPORTED, "temperature %g is positive, but below f32's normal range",
+                   static_cast<double>(f.temperature));
   const int64_t ts = f.target_stride ? f.target_stride : f.vocab;
   const int64_t ds = f.draft_stride ? f.draft_stride : f.vocab;
   if (ts < f.vocab || ds < f.vocab)
@@ -779,7 +784,7 @@ extern "C" int ql_verify_drafts(ql_ctx* c, const ql_verify_args* args) {
   a.inv_t = probs ? 1.0 : greedy ? 0.0 : 1.0 / static_cast<double>(f.temperature);
   a.exp_scale = a.inv_t * (32.0 / 0.693147180559945309417232);
   a.exp_least = -690.0 / a.inv_t;
-  a.exp2_scale = static_cast<float>(std::fmin(a.inv_t / 0.693147180559945309417232, 3e38));
+  a.exp2_scale = static_cast<float>(a.inv_t / 0.693147180559945309417232);
   cudaError_t e;
   if (f.dtype == QL_F32) e = launch_verify<ql::kF32>(a, f.batch, c->num_sms, c->stream);
   else if (f.dtype == QL_F16) e = launch_verify<ql::kF16>(a, f.batch, c->num_sms, c->stream);

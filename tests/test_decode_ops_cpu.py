@@ -148,6 +148,18 @@ def test_verify_refusals(change, text, code):
     refused(qb.load().ql_verify_drafts(ctypes.byref(CTX), ctypes.byref(a)), text, code)
 
 
+@pytest.mark.parametrize("T, refuse", [(1e-39, True), (1e-45, True), (1.2e-38, False),
+                                       (0.0, False), (-1e-39, False)])
+def test_verify_temperatures_below_the_normal_range(T, refuse):
+    """(A batch of no sequences shows which ones pass the checks.)"""
+    a = qm.VerifyArgs(**{**VERIFY, "batch": 0, "temperature": T})
+    rc = qb.load().ql_verify_drafts(ctypes.byref(CTX), ctypes.byref(a))
+    if refuse:
+        refused(rc, "temperature", qb.ERR_UNSUPPORTED)
+    else:
+        assert rc == qb.OK
+
+
 def test_verify_of_no_sequences_is_a_no_op():
     a = qm.VerifyArgs(**{**VERIFY, "batch": 0, "target": None})
     assert qb.load().ql_verify_drafts(ctypes.byref(CTX), ctypes.byref(a)) == qb.OK
