@@ -356,10 +356,11 @@ __global__ void __launch_bounds__(WARP ? 32 * kNormRows : NV == 1 ? 1024 : 512,
 }
 
 // A launch that may begin while the kernel before it in the stream drains
-// (every kernel here waits for that kernel's end before it touches a tensor).
+// (every kernel here waits for that kernel's end before it touches a tensor; only a
+// product's weights are read ahead).
 template <typename... P, typename... A>
 cudaError_t launch_pdl(void (*kernel)(P...), dim3 grid, dim3 block, size_t smem, cudaStream_t s,
-                       bool pdl, A... args) {
+                       A... args) {
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = grid;
   cfg.blockDim = block;
@@ -369,7 +370,7 @@ cudaError_t launch_pdl(void (*kernel)(P...), dim3 grid, dim3 block, size_t smem,
   attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
   attr[0].val.programmaticStreamSerializationAllowed = 1;
   cfg.attrs = attr;
-  cfg.numAttrs = pdl ? 1 : 0;
+  cfg.numAttrs = 1;
   return cudaLaunchKernelEx(&cfg, kernel, args...);
 }
 
@@ -389,7 +390,7 @@ cudaError_t launch_norm(const NormArgs& a, int num_sms, cudaStream_t s) {
   const bool lead = !even && a.hidden % 8 != 0 && a.x_stride == a.hidden &&
                     (!a.residual || a.residual_stride == a.hidden);
   if (!bases || !(even || lead) || a.hidden > kNormMax - 8)
-    return launch_pdl(rms_norm_loop_kernel, dim3(a.rows), dim3(kNormThreads), 0, s, true, a);
+    return launch_pdl(rms_norm_loop_kernel, dim3(a.rows), dim3(kNormThreads), 0, s, a);
   const int groups = (a.hidden + 7) / 8 + lead;
   const bool warp = groups <= 64 && a.rows >= 4 * num_sms;
   int nv = warp ? (groups <= 32 ? 1 : 2) : groups <= 1024 ? 1 : 4;
@@ -404,7 +405,7 @@ cudaError_t launch_norm(const NormArgs& a, int num_sms, cudaStream_t s) {
                          : nv == 1 ? rms_norm_kernel<DT, WT, 1, LEAD, false>
                          : nv == 2 ? rms_norm_kernel<DT, WT, 2, LEAD, false>
                                    : rms_norm_kernel<DT, WT, 4, LEAD, false>;
-    return launch_pdl(kernel, grid, block, 0, s, true, a);
+    return launch_pdl(kernel, grid, block, 0, s, a);
   };
   auto by_lead = [&](auto dt, auto wt) {
     return lead ? go(dt, wt, std::true_type()) : go(dt, wt, std::false_type());
@@ -442,9 +443,6 @@ struct ql_q4 {
   int tiles = 0, chunks = 0;
   uint32_t* codes = nullptr;   // [tiles][chunks][32][4]
   __half* scales = nullptr;    // [tiles][chunks][8][2][2], [tiles][chunks or chunks/2][8][2]
-  // Written since the last product: the next one starts only when all work
-  // queued before it is done, and may not read the weights ahead.
-  mutable bool fresh = true;
 };
 
 namespace {
@@ -584,14 +582,26 @@ __global__ void __launch_bounds__(256) q4_unpack_kernel(Q4View w, uint8_t* codes
             w.scales)[scale_at(w.group, w.chunks, tile, chunk, lane >> 2, i >> 1, i & 1)];
 }
 
+// An empty launch behind every write of a weight.  A product reads weights ahead of its
+// griddepcontrol.wait, so that a write must have ended, its bytes visible, before the
+// launch in front of the product begins.  This one, an ordinary launch, begins then; and
+// whatever else stands between the write and a product (an event on another stream, a
+// captured graph's edge, another kernel) waits for it in the same way.
+__global__ void q4_written_kernel() {}
+
+int close_write(ql_q4* w) {
+  q4_written_kernel<<<1, 1, 0, w->ctx->stream>>>();
+  QLN_CUDA(cudaGetLastError(), "launch behind the 4-bit layout");
+  return QL_OK;
+}
+
 template <int FROM>
 int launch_pack(ql_q4* w, PackArgs a) {
   a.w = view_of(w);
-  w->fresh = true;
   const size_t blocks = (q4_words(w) + 255) / 256;
   q4_pack_kernel<FROM><<<static_cast<unsigned>(blocks), 256, 0, w->ctx->stream>>>(a);
   QLN_CUDA(cudaGetLastError(), "launch the 4-bit layout");
-  return QL_OK;
+  return close_write(w);
 }
 
 // Device copies of host buffers for the length of one call.
@@ -1006,8 +1016,8 @@ __global__ void __launch_bounds__(kRanges* WR * 32, 1) linear_q4_kernel(const Li
     }
   };
 
-  // The first weights do not depend on the kernel before this one (a product
-  // after a write of the weights is launched without the overlap).
+  // The first weights do not depend on the kernel before this one (an empty launch
+  // stands between a write of them and any product).
   const int total = groups * nc;
 #pragma unroll
   for (int i = 0; i < C::kD - 1; ++i)
@@ -1115,7 +1125,7 @@ __global__ void __launch_bounds__(kRanges* WR * 32, 1) linear_q4_kernel(const Li
 }
 
 template <int IN, int NT, int MT, int WR, int G>
-cudaError_t launch_linear_as(const LinearArgs& a, int num_sms, bool pdl, cudaStream_t s) {
+cudaError_t launch_linear_as(const LinearArgs& a, int num_sms, cudaStream_t s) {
   using C = LinCfg<IN, NT, MT, WR, G>;
   static_assert(C::kSmem <= 227 * 1024, "shared memory");
   auto* const kernel = linear_q4_kernel<IN, NT, MT, WR, G>;
@@ -1131,7 +1141,7 @@ cudaError_t launch_linear_as(const LinearArgs& a, int num_sms, bool pdl, cudaStr
     b.x_scale = a.x_scale ? a.x_scale + static_cast<size_t>(r) * (a.w.k / 32) : nullptr;
     b.y = static_cast<char*>(a.y) + static_cast<size_t>(r) * a.y_stride * yb;
     const dim3 grid(std::min(num_sms, a.w.tiles), (b.rows + C::kRows - 1) / C::kRows);
-    e = launch_pdl(kernel, grid, dim3(C::kThreads), C::kSmem, s, pdl, b);
+    e = launch_pdl(kernel, grid, dim3(C::kThreads), C::kSmem, s, b);
   }
   return e;
 }
@@ -1143,25 +1153,25 @@ cudaError_t launch_linear_as(const LinearArgs& a, int num_sms, bool pdl, cudaStr
 // with two teams of half the tiles), eight tiles at a time where a CTA has more than
 // four (86 us with four at a time).
 template <int IN, int G>
-cudaError_t launch_linear_in(const LinearArgs& a, int num_sms, bool pdl, cudaStream_t s) {
+cudaError_t launch_linear_in(const LinearArgs& a, int num_sms, cudaStream_t s) {
   const int b = (a.rows - 1) / LinCfg<IN, 1, 1, 1, G>::kTileRows + 1;
   if (b > 2)
-    return a.w.tiles <= 4 * num_sms ? launch_linear_as<IN, 4, 4, 1, G>(a, num_sms, pdl, s)
-                                    : launch_linear_as<IN, 4, 8, 1, G>(a, num_sms, pdl, s);
+    return a.w.tiles <= 4 * num_sms ? launch_linear_as<IN, 4, 4, 1, G>(a, num_sms, s)
+                                    : launch_linear_as<IN, 4, 8, 1, G>(a, num_sms, s);
   const bool one = a.w.tiles <= num_sms;
   if (b == 1)
-    return one ? launch_linear_as<IN, 1, 1, 1, G>(a, num_sms, pdl, s)
-               : launch_linear_as<IN, 1, 4, 2, G>(a, num_sms, pdl, s);
-  return one ? launch_linear_as<IN, 2, 1, 1, G>(a, num_sms, pdl, s)
-             : launch_linear_as<IN, 2, 4, 2, G>(a, num_sms, pdl, s);
+    return one ? launch_linear_as<IN, 1, 1, 1, G>(a, num_sms, s)
+               : launch_linear_as<IN, 1, 4, 2, G>(a, num_sms, s);
+  return one ? launch_linear_as<IN, 2, 1, 1, G>(a, num_sms, s)
+             : launch_linear_as<IN, 2, 4, 2, G>(a, num_sms, s);
 }
 
-cudaError_t launch_linear(const LinearArgs& a, int num_sms, bool pdl, cudaStream_t s) {
+cudaError_t launch_linear(const LinearArgs& a, int num_sms, cudaStream_t s) {
   auto by_group = [&](auto in) {
     constexpr int IN = decltype(in)::value;
-    if (a.w.group == 32) return launch_linear_in<IN, 32>(a, num_sms, pdl, s);
-    if (a.w.group == 64) return launch_linear_in<IN, 64>(a, num_sms, pdl, s);
-    return launch_linear_in<IN, 128>(a, num_sms, pdl, s);
+    if (a.w.group == 32) return launch_linear_in<IN, 32>(a, num_sms, s);
+    if (a.w.group == 64) return launch_linear_in<IN, 64>(a, num_sms, s);
+    return launch_linear_in<IN, 128>(a, num_sms, s);
   };
   switch (a.in_dtype) {
     case QL_F32: return by_group(std::integral_constant<int, ql::kF32>());
@@ -1297,6 +1307,10 @@ int ql_q4_create(ql_ctx* c, int32_t out_features, int32_t in_features, int32_t g
     cudaGetLastError();
     return ql_fail(e == cudaErrorMemoryAllocation ? QL_ERR_OOM : QL_ERR_CUDA,
                    "allocate a 4-bit weight: %s", cudaGetErrorString(e));
+  }
+  if (int r = close_write(w)) {
+    ql_q4_destroy(w);
+    return r;
   }
   *out = w;
   return QL_OK;
@@ -1443,8 +1457,7 @@ int ql_linear_q4(ql_ctx* c, const ql_q4* w, const ql_linear_args* args) {
   a.rows = f.rows;
   a.in_dtype = f.in_dtype;
   a.out_dtype = f.out_dtype;
-  QLN_CUDA(launch_linear(a, c->num_sms, !w->fresh, c->stream), "launch the 4-bit product");
-  w->fresh = false;
+  QLN_CUDA(launch_linear(a, c->num_sms, c->stream), "launch the 4-bit product");
   return QL_OK;
 }
 

@@ -384,6 +384,53 @@ def test_linear_large_and_tiny_values(ctx):
     w.close()
 
 
+@pytest.mark.parametrize("where", ["captured", "another context"])
+def test_linear_after_new_weights_wherever_the_last_product_was(ctx, stream, where):
+    """New weights, a product of them that has not run or ran on another stream, and at
+    once a product on the stream that wrote them."""
+    g = gen(31)
+    n, k = 4096, 4096
+    old, new = random_weight(g, n, k, 32), random_weight(g, n, k, 32)
+    x = randn(g, 1, k).half()
+    w = qm.Q4Weight(ctx, *new)
+    want = qm.linear_q4(w, x)
+    y, y2 = torch.empty_like(want), torch.empty_like(want)
+    other, s2 = qb.Context(0), torch.cuda.Stream()
+    other.set_stream(s2.cuda_stream)
+    graph = torch.cuda.CUDAGraph()
+    # a context's handle of the same weight, for calls on the other stream
+    view = object.__new__(qm.Q4Weight)
+    view.__dict__.update(w.__dict__)
+    view.ctx = other
+    for _ in range(10):
+        w.set(*old)
+        qm.linear_q4(w, x, out=y)
+        stream.synchronize()
+        assert not torch.equal(y, want)
+        w.set(*new)
+        if where == "captured":
+            stream.synchronize()
+            graph.reset()
+            with torch.cuda.graph(graph, stream=stream):
+                qm.linear_q4(w, x, out=y2)
+            w.set(*new)
+        else:
+            s2.wait_stream(stream)
+            with torch.cuda.stream(s2):
+                qm.linear_q4(view, x, out=y2)
+        qm.linear_q4(w, x, out=y)
+        stream.synchronize()
+        s2.synchronize()
+        assert torch.equal(y, want)
+        if where == "captured":
+            graph.replay()
+            stream.synchronize()
+        assert torch.equal(y2, want)
+    graph.reset()
+    view._h = None  # the handle is w's
+    w.close()
+
+
 def test_empty_calls(ctx):
     codes, scales = random_weight(gen(1), 8, 64, 32)
     w = qm.Q4Weight(ctx, codes, scales)
