@@ -67,6 +67,12 @@ int ql_ctx_create(int device, ql_ctx** out);
 int ql_ctx_destroy(ql_ctx* ctx);
 /* Use `stream` (a cudaStream_t; NULL = the context's own stream) for later calls. */
 int ql_ctx_set_stream(ql_ctx* ctx, void* stream);
+/* Order between the context's stream and `stream` (a cudaStream_t of the same device; NULL =
+ * the legacy default stream), without waiting on the host: later work of the context starts
+ * when what `stream` holds now is done (wait), and the other way round (join).  A pair of
+ * them around a call lets it use buffers that belong to `stream`. */
+int ql_ctx_wait_stream(ql_ctx* ctx, void* stream);
+int ql_ctx_join_stream(ql_ctx* ctx, void* stream);
 /* Wait for all work queued by this context; returns QL_ERR_DEVICE if a
  * kernel set its status word since the last call. */
 int ql_ctx_synchronize(ql_ctx* ctx);

@@ -38,7 +38,7 @@ OK, ERR_INVALID, ERR_CUDA, ERR_OOM, ERR_NO_DEVICE, ERR_UNSUPPORTED, ERR_DEVICE =
 # Every symbol include/qllama_attn.h declares.
 EXPORTS = (
     "ql_version", "ql_last_error", "ql_ctx_create", "ql_ctx_destroy", "ql_ctx_set_stream",
-    "ql_ctx_synchronize", "ql_kv_create", "ql_kv_destroy", "ql_kv_clear", "ql_kv_clear_seq",
+    "ql_ctx_wait_stream", "ql_ctx_join_stream", "ql_ctx_synchronize", "ql_kv_create", "ql_kv_destroy", "ql_kv_clear", "ql_kv_clear_seq",
     "ql_kv_seq_len", "ql_kv_layer_len", "ql_kv_update", "ql_kv_get", "ql_attn_forward",
     "ql_attn_decode_noalloc", "ql_kv_truncate", "ql_comm_unique_id", "ql_comm_create",
     "ql_comm_destroy", "ql_comm_buffer", "ql_attn_forward_sharded",
@@ -112,6 +112,8 @@ def load(build_if_missing: bool = True) -> ctypes.CDLL:
     L.ql_ctx_create.argtypes = [ctypes.c_int, ctypes.POINTER(vp)]
     L.ql_ctx_destroy.argtypes = [vp]
     L.ql_ctx_set_stream.argtypes = [vp, vp]
+    L.ql_ctx_wait_stream.argtypes = [vp, vp]
+    L.ql_ctx_join_stream.argtypes = [vp, vp]
     L.ql_ctx_synchronize.argtypes = [vp]
     L.ql_kv_create.argtypes = [vp, ctypes.POINTER(KvConfig), ctypes.POINTER(vp)]
     L.ql_kv_destroy.argtypes = [vp]
@@ -179,9 +181,12 @@ class Context:
         _check(L.ql_ctx_create(device, ctypes.byref(h)))
         self._h = h
         self.device = device
+        self._stream = None  # the context's own
 
     def set_stream(self, stream_handle: int | None) -> None:
         _check(load().ql_ctx_set_stream(self._h, stream_handle))
+        # as torch names it: 0 is the legacy default stream, cudaStreamLegacy (1) here
+        self._stream = (0 if stream_handle == 1 else stream_handle) if stream_handle else None
 
     def synchronize(self) -> None:
         _check(load().ql_ctx_synchronize(self._h))

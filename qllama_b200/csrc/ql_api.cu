@@ -502,6 +502,8 @@ int ql_ctx_destroy(ql_ctx* c) {
   if (c->ws) cudaFree(c->ws);
   if (c->counters) cudaFree(c->counters);
   if (c->status) cudaFree(c->status);
+  for (cudaEvent_t e : c->order)
+    if (e) cudaEventDestroy(e);
   if (c->own) cudaStreamDestroy(c->own);
   delete c;
   return QL_OK;
@@ -511,6 +513,27 @@ int ql_ctx_set_stream(ql_ctx* c, void* stream) {
   if (!c) return fail(QL_ERR_INVALID, "ql_ctx_set_stream: ctx is NULL");
   c->stream = stream ? static_cast<cudaStream_t>(stream) : c->own;
   return QL_OK;
+}
+
+// `after` waits for what `before` holds now.
+static int order_streams(ql_ctx* c, int which, cudaStream_t before, cudaStream_t after) {
+  ql_device_guard dev(c->device);
+  QL_CUDA(dev.error(), "set device");
+  cudaEvent_t& e = c->order[which];
+  if (!e) QL_CUDA(cudaEventCreateWithFlags(&e, cudaEventDisableTiming), "create an event");
+  QL_CUDA(cudaEventRecord(e, before), "record an event");
+  QL_CUDA(cudaStreamWaitEvent(after, e, 0), "wait for an event");
+  return QL_OK;
+}
+
+int ql_ctx_wait_stream(ql_ctx* c, void* stream) {
+  if (!c) return fail(QL_ERR_INVALID, "ql_ctx_wait_stream: ctx is NULL");
+  return order_streams(c, 0, static_cast<cudaStream_t>(stream), c->stream);
+}
+
+int ql_ctx_join_stream(ql_ctx* c, void* stream) {
+  if (!c) return fail(QL_ERR_INVALID, "ql_ctx_join_stream: ctx is NULL");
+  return order_streams(c, 1, c->stream, static_cast<cudaStream_t>(stream));
 }
 
 int ql_ctx_synchronize(ql_ctx* c) {

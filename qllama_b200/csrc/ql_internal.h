@@ -18,6 +18,7 @@ struct ql_ctx {
   size_t ws_bytes = 0;
   int32_t* counters = nullptr;  // split-merge arrival counters, kept at zero
   size_t counters_n = 0;
+  cudaEvent_t order[2] = {nullptr, nullptr};  // of ql_ctx_wait_stream and ql_ctx_join_stream
 };
 
 // Records the message of a failed call (ql_last_error) and returns `code`.

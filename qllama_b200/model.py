@@ -18,8 +18,10 @@ weights with drafted tokens:
 * ``verify_drafts``    -- speculative sampling's acceptance and next token.
 
 These take CUDA tensors and queue their work on the context's stream
-(``Context.set_stream``); tensors written on another stream have to be ordered
-before it by the caller.
+(``Context.set_stream``).  Where torch's current stream is another one, they make
+the context's stream wait for it first and it for the context's afterwards, so
+that tensors of the current stream may be passed, used and dropped as with any
+torch call; tensors of a third stream have to be ordered by the caller.
 """
 from __future__ import annotations
 
@@ -263,13 +265,16 @@ def attention_forward_appended(kv, layer: int, q_rot, start_pos, num_heads: int,
 # kept short: these are filled at the first call.
 _codes = {}  # torch dtype -> QL element type
 _L = None    # the library
+_current = None  # a device's current stream in torch, as a handle
 
 
 def _start():
-    global _L
+    global _L, _current
     import torch
 
     qb = _qb()
+    # (torch.cuda.current_stream makes an object of it: a microsecond and more a call)
+    _current = torch._C._cuda_getCurrentRawStream
     _codes.update({torch.float32: qb.F32, torch.float16: qb.F16, torch.bfloat16: qb.BF16})
     _L = qb.load()
     return _L
@@ -282,6 +287,24 @@ def _invalid(message: str):
 
 def _raise(rc: int):
     raise _qb().QllamaError(rc, _L.ql_last_error().decode())
+
+
+def _fork(ctx):
+    """Where torch's current stream is not the context's: the context waits for it.
+    Returns its handle for _join, or None."""
+    s = _current(ctx.device)
+    if s == ctx._stream:
+        return None
+    if rc := _L.ql_ctx_wait_stream(ctx._h, s):
+        _raise(rc)
+    return s
+
+
+def _join(ctx, s) -> None:
+    """The current stream waits for the call: its tensors may be used, or dropped and
+    their memory taken by the next ones."""
+    if s is not None and (rc := _L.ql_ctx_join_stream(ctx._h, s)):
+        _raise(rc)
 
 
 def _float_code(t, name: str) -> int:
@@ -366,12 +389,16 @@ def rms_norm(ctx, x, weight, eps: float, residual=None, sum_out=None, out=None, 
         t = _named_type(out_dtype) if out_dtype else dtype if out is None else out.dtype
         out = _output(ctx, out, shape, t, "out")
         out_dt, scp = _codes[t], None
-    rc = L.ql_rms_norm(ctx._h, ctypes.byref(NormArgs(
+    args = NormArgs(
         x.numel() // hidden, hidden, in_dt, _float_code(weight, "weight"), out_dt, eps,
         _stride_of(x, hidden, "x"), rs, _on(dev, x, "x"), rp, _on(dev, weight, "weight"), sp,
-        _on(dev, out, "out"), scp)))
+        _on(dev, out, "out"), scp)
+    side = _fork(ctx)
+    rc = L.ql_rms_norm(ctx._h, ctypes.byref(args))
     if rc:
         _raise(rc)
+    if side is not None:
+        _join(ctx, side)
     return out if scp is None else (out, scale)
 
 
@@ -409,7 +436,7 @@ class Q4Weight:
         q = cls(ctx, shape=(int(w.shape[0]), int(w.shape[1]), group))
         p, mem, keep = q._buffer(w, None, "w")
         stride = 0 if mem == qb.MEM_HOST else _stride_of(keep, int(w.shape[1]), "w")
-        qb._check(qb.load().ql_q4_quantize(q._h, p, qb._dtype_code(keep), stride, mem))
+        q._write(mem, qb.load().ql_q4_quantize, p, qb._dtype_code(keep), stride, mem)
         return q
 
     @classmethod
@@ -421,8 +448,18 @@ class Q4Weight:
             blocks = np.frombuffer(blocks, np.uint8)
         p, mem, keep = q._buffer(blocks, "uint8", "blocks")
         n = int(keep.size if mem == qb.MEM_HOST else keep.numel())
-        qb._check(qb.load().ql_q4_set_blocks(q._h, p, n, mem))
+        q._write(mem, qb.load().ql_q4_set_blocks, p, n, mem)
         return q
+
+    def _write(self, mem: int, call, *args) -> None:
+        """One of the calls that write the weight, from tensors of the current stream."""
+        qb = _qb()
+        side = None
+        if mem == qb.MEM_DEVICE:
+            _L or _start()
+            side = _fork(self.ctx)
+        qb._check(call(self._h, *args))
+        _join(self.ctx, side)
 
     def _buffer(self, x, dtype, name: str):
         """(pointer, memory kind, keep-alive) of an array or a CUDA tensor."""
@@ -450,7 +487,7 @@ class Q4Weight:
         sp, mem2, s = self._buffer(scales, "float16", "scales")
         if mem != mem2:
             raise _invalid("codes and scales must live in the same memory")
-        qb._check(qb.load().ql_q4_set(self._h, cp, sp, mem))
+        self._write(mem, qb.load().ql_q4_set, cp, sp, mem)
 
     def get(self):
         """(codes, scales) as numpy arrays in the constructor's layout."""
@@ -513,11 +550,14 @@ def linear_q4(weight: Q4Weight, x, x_scale=None, out=None, out_dtype: str | None
         if out.shape != shape or out.dtype is not dtype:
             raise _invalid(f"out must be {dtype} of shape {tuple(shape)}")
         ys = _stride_of(out, n, "out")
-    rc = L.ql_linear_q4(ctx._h, weight._h, ctypes.byref(LinearArgs(
-        x.numel() // k, in_dt, _float_code(out, "out"), _stride_of(x, k, "x"), ys,
-        _on(dev, x, "x"), scp, _on(dev, out, "out"))))
+    args = LinearArgs(x.numel() // k, in_dt, _float_code(out, "out"), _stride_of(x, k, "x"), ys,
+                      _on(dev, x, "x"), scp, _on(dev, out, "out"))
+    side = _fork(ctx)
+    rc = L.ql_linear_q4(ctx._h, weight._h, ctypes.byref(args))
     if rc:
         _raise(rc)
+    if side is not None:
+        _join(ctx, side)
     return out
 
 
@@ -571,10 +611,14 @@ def verify_drafts(ctx, target, draft, draft_ids, uniforms, temperature: float = 
         up = plain(uniforms, (batch, m + 1), torch.float64, "uniforms")
     tokens = _output(ctx, tokens, (batch, m + 1), torch.int32, "tokens")
     accepted = _output(ctx, accepted, (batch,), torch.int32, "accepted")
-    rc = L.ql_verify_drafts(ctx._h, ctypes.byref(VerifyArgs(
+    args = VerifyArgs(
         batch, m, vocab, dt, VERIFY_PROBS if probs else VERIFY_LOGITS, temperature, ts, ds,
         _on(dev, target, "target"), dp, ip, np_, up, _on(dev, tokens, "tokens"),
-        _on(dev, accepted, "accepted"))))
+        _on(dev, accepted, "accepted"))
+    side = _fork(ctx)
+    rc = L.ql_verify_drafts(ctx._h, ctypes.byref(args))
     if rc:
         _raise(rc)
+    if side is not None:
+        _join(ctx, side)
     return tokens, accepted

@@ -165,6 +165,47 @@ def test_verify_of_no_sequences_is_a_no_op():
     assert qb.load().ql_verify_drafts(ctypes.byref(CTX), ctypes.byref(a)) == qb.OK
 
 
+@pytest.mark.parametrize("current, own, ordered", [(7, 7, False), (0, 0, False), (7, None, True),
+                                                   (0, None, True), (7, 9, True)])
+def test_calls_are_ordered_with_the_current_stream(monkeypatch, current, own, ordered):
+    """Around a call whose context has another stream than torch's current one: the context
+    waits for that stream before it, and that stream for the context after it."""
+    class Context:
+        device, _stream, _h = 0, own, 5
+
+    class Library:
+        log = []
+
+        def __getattr__(self, name):
+            def call(handle, *args):
+                self.log.append(name if name == "ql_q4_set" else (name, handle, *args))
+                return 0
+            return call
+
+    lib = Library()
+    monkeypatch.setattr(qm, "_L", lib)
+    monkeypatch.setattr(qm, "_current", lambda device: current)
+    w = object.__new__(qm.Q4Weight)
+    w.ctx, w._h = Context(), 6
+    w._write(qb.MEM_DEVICE, lib.ql_q4_set, P, P, 0)
+    w._h = None
+    around = [("ql_ctx_wait_stream", 5, current), "ql_q4_set", ("ql_ctx_join_stream", 5, current)]
+    assert lib.log == (around if ordered else ["ql_q4_set"])
+
+
+def test_a_contexts_stream_as_torch_names_it(monkeypatch):
+    class Library:
+        def ql_ctx_set_stream(self, handle, stream):
+            return 0
+
+    monkeypatch.setattr(qb, "load", Library)
+    c = object.__new__(qb.Context)
+    c._h = None
+    for handle, name in ((None, None), (0, None), (1, 0), (0x7f00, 0x7f00)):
+        c.set_stream(handle)
+        assert c._stream == name
+
+
 def test_null_arguments():
     L = qb.load()
     for rc in (L.ql_rms_norm(None, None), L.ql_q4_create(None, 1, 32, 32, None),

@@ -832,6 +832,86 @@ def test_two_contexts_on_two_streams(stream):
         run[2].close()
 
 
+@pytest.fixture
+def own():
+    """A context on its own stream, as it comes."""
+    c = qb.Context(0)
+    yield c
+    c.synchronize()
+    c.close()
+
+
+def busy():
+    torch.cuda._sleep(2_000_000)  # about a millisecond of the current stream
+
+
+def spoil(n):
+    """Fills memory that was just dropped on the current stream."""
+    for _ in range(4):
+        torch.full((n,), 0x7f, dtype=torch.uint8, device="cuda")
+
+
+def test_tensors_of_the_current_stream_on_a_context_of_its_own(ctx, own):
+    """Inputs that the current stream is still writing, dropped and overwritten at once, and
+    results used there, without a synchronisation."""
+    g = gen(40)
+    torch.manual_seed(40)
+    rows, k, n = 6, 4096, 2048
+    x, r, wt = randn(g, rows, k), randn(g, rows, k), 1 + 0.1 * randn(g, k)
+    a = randn(g, n, k) * 0.02
+    target, draft, ids, un = drafted(g, 3, 3, 5000, "f32")
+
+    def run(c):
+        out = []
+        busy()
+        w = qm.Q4Weight.from_dense(c, a.half() * 1, 64)
+        spoil(2 * n * k)
+        y = qm.linear_q4(w, x + r)
+        spoil(4 * rows * k)
+        out += [y * 1]
+        busy()
+        q, d = qm.rms_norm(c, x * 1, wt * 1, 1e-5, residual=r * 1, out_dtype="q8_0")
+        spoil(4 * rows * k)
+        out += [q * 1, d * 1, qm.linear_q4(w, q * 1, d * 1) * 1]
+        del q, d, y
+        busy()
+        codes, scales = (torch.from_numpy(t).cuda() for t in w.get())
+        busy()
+        w.set(codes * 1, scales * 1)
+        spoil(n * k // 2)
+        out += [qm.linear_q4(w, x * 1) * 1]
+        busy()
+        out += [t * 1 for t in qm.verify_drafts(c, target * 1, draft * 1, ids * 1, un * 1)]
+        spoil(4 * target.numel())
+        return out
+
+    want = run(ctx)
+    torch.cuda.synchronize()
+    for _ in range(3):
+        got = run(own)
+        assert all(torch.equal(s, t) for s, t in zip(want, got))
+
+
+def test_a_context_of_its_own_in_a_captured_stream(ctx, own, stream):
+    """Calls of a context on its own stream are part of a graph that torch's current
+    stream captures."""
+    g = gen(41)
+    k, n = 512, 300
+    w = qm.Q4Weight(own, *random_weight(g, n, k, 32))
+    x, wt = randn(g, 3, k), 1 + 0.1 * randn(g, k)
+    graph = torch.cuda.CUDAGraph()
+    stream.synchronize()
+    with torch.cuda.graph(graph, stream=stream):
+        y = qm.linear_q4(w, *qm.rms_norm(own, x, wt, 1e-5, out_dtype="q8_0"))
+    for seed in (42, 43):
+        x.copy_(randn(gen(seed), 3, k))
+        graph.replay()
+        got = y.clone()
+        assert torch.equal(got, qm.linear_q4(w, *qm.rms_norm(own, x, wt, 1e-5, out_dtype="q8_0")))
+    stream.synchronize()
+    w.close()
+
+
 # --------------------------------------------------------- a quantized model --
 
 def small_model(ctx, layers=2):
