@@ -441,14 +441,13 @@ class Q4Weight:
 
     @classmethod
     def from_gguf(cls, ctx, blocks, out_features: int, in_features: int) -> "Q4Weight":
-        """From GGUF Q4_0 blocks (bytes, a numpy uint8 array or a CUDA uint8 tensor)."""
+        """From GGUF Q4_0 blocks (bytes, a numpy uint8 array or a uint8 tensor)."""
         qb = _qb()
         q = cls(ctx, shape=(out_features, in_features, 32))
         if isinstance(blocks, (bytes, bytearray, memoryview)):
             blocks = np.frombuffer(blocks, np.uint8)
         p, mem, keep = q._buffer(blocks, "uint8", "blocks")
-        n = int(keep.size if mem == qb.MEM_HOST else keep.numel())
-        q._write(mem, qb.load().ql_q4_set_blocks, p, n, mem)
+        q._write(mem, qb.load().ql_q4_set_blocks, p, int(keep.nbytes), mem)
         return q
 
     def _write(self, mem: int, call, *args) -> None:

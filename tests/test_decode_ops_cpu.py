@@ -90,6 +90,31 @@ def test_scales_of_another_type_are_refused(dtype):
     assert p == keep.data_ptr() and mem == qb.MEM_HOST
 
 
+@pytest.mark.parametrize("kind", ["bytes", "numpy", "torch", "torch, every other byte"])
+def test_gguf_blocks_in_host_memory(monkeypatch, kind):
+    """Blocks as bytes, an array or a CPU tensor reach the library with their byte count."""
+    torch = pytest.importorskip("torch")
+    raw = torch.arange(2 * 3 * 2 * 18, dtype=torch.uint8).view(3, -1)
+    blocks = raw[:, ::2] if "every" in kind else raw[:, :36].contiguous()
+    plain = blocks.numpy().tobytes()
+    blocks = {"bytes": plain, "numpy": blocks.numpy()}.get(kind, blocks)
+
+    class Library:
+        got = None
+
+        def ql_q4_create(self, *args):
+            return 0
+
+        def ql_q4_set_blocks(self, handle, p, n, mem):
+            Library.got = (ctypes.string_at(p, n), mem)
+            return 0
+
+    monkeypatch.setattr(qb, "load", Library)
+    monkeypatch.setattr(CTX, "_h", None, raising=False)
+    qm.Q4Weight.from_gguf(CTX, blocks, 3, 64)
+    assert Library.got == (plain, qb.MEM_HOST)
+
+
 def test_weight_value_refusals():
     L, w, w64 = qb.load(), q4(), q4(group=64)
     refused(L.ql_q4_set(ctypes.byref(w), None, P, 0), "NULL")
