@@ -225,7 +225,8 @@ int ql_q4_get(const ql_q4* w, uint8_t* codes, void* scales, int32_t mem);
  * kernel is built for up to some 64 rows, where the weights' bytes are the cost;
  * more rows are taken in passes of that size.
  *   in_dtype F32, F16, BF16: x as given, every product with a code exact (an
- *     infinity in an F32 row gives NaN);
+ *     infinity in an F32 row gives NaN; F32 magnitudes below 2^-110 count in
+ *     steps of 2^-133);
  *   in_dtype Q8_0: int8 values with x_scale [rows, in_features/32] f16, the
  *     output of ql_rms_norm (integer products, exact per block of 32).
  * Sums are f32; y [rows, out_features] is rounded once to out_dtype.  A row's

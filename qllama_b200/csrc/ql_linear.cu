@@ -646,13 +646,13 @@ struct LinearArgs {
 // each goes from HBM to the lane that multiplies it once, through a ring in shared
 // memory that every warp keeps for itself (cp.async, kD sets deep; a __syncwarp is
 // the only barrier of the loop).  Codes turn into f16 / bf16 exactly (a nibble in the
-// mantissa of 1024 or 128, less an offset), or into int8 (a two's-complement nibble in
+// mantissa of 1024 or 1/4, less an offset), or into int8 (a two's-complement nibble in
 // the high half of a byte: 16 times its value).  The weights are the A operand (16
 // rows of W), x the B operand (8 columns), so one row of x costs as much as eight.
 // Blocks of 32 are summed on the tensor cores in f32 (int32 for Q8_0: exact), scaled
 // in f32 and added to f32 sums.  f32 rows: three bf16 parts of 8 significand bits
-// carry a value's 24 exactly; the parts are three columns of B, whose sums are added
-// at the end.
+// carry a value's 24 exactly (down to 2^-110, where the last part meets bf16's smallest
+// step, 2^-133); the parts are three columns of B, whose sums are added at the end.
 // One CTA an SM, each with an equal share of W's row tiles (an even share matters
 // more than anything else: CTAs of a few tiles, several an SM, left a third of the
 // time to the last of them).  The columns are cut into 8 ranges, one for each warp of
@@ -752,16 +752,19 @@ __device__ __forceinline__ uint32_t and_xor(uint32_t a, uint32_t b, uint32_t c) 
   return d;
 }
 
-// A word's eight values as four pairs in x's order, exactly.
+// A word's eight values as four pairs in x's order, exactly; in bf16 2^-9 of them (an
+// exponent is free to choose), so that a sum of 64 columns is no larger than the largest
+// |x|: f32 and bf16 rows reach f32's largest numbers.
+constexpr float kBfCodes = 512.f;
 template <bool BF>
 __device__ __forceinline__ void unpack_word(uint32_t w, uint32_t (&p)[4]) {
   if constexpr (BF) {
     const uint32_t in[4] = {w, w >> 8, w >> 4, w >> 12};
-    const __nv_bfloat162 off = __halves2bfloat162(__ushort_as_bfloat16(0x4308),
-                                                  __ushort_as_bfloat16(0x4308));  // 136
+    const __nv_bfloat162 off = __halves2bfloat162(__ushort_as_bfloat16(0x3e88),
+                                                  __ushort_as_bfloat16(0x3e88));  // 136 / 512
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
-      const uint32_t h = and_xor(in[i], 0x000f000fu, 0x43084308u);  // 128 + (value + 8)
+      const uint32_t h = and_xor(in[i], 0x000f000fu, 0x3e883e88u);  // (128 + (value + 8)) / 512
       const __nv_bfloat162 v = __hsub2(*reinterpret_cast<const __nv_bfloat162*>(&h), off);
       p[i] = *reinterpret_cast<const uint32_t*>(&v);
     }
@@ -1117,6 +1120,7 @@ __global__ void __launch_bounds__(kRanges* WR * 32, 1) linear_q4_kernel(const Li
           y += v;
         }
         if (C::kQ8) y *= 0.0625f;  // the codes were 16 times their values
+        if (C::kBF) y *= kBfCodes;
         ql::store_elem(a.y, static_cast<size_t>(r0 + q * C::kTileRows + r) * a.y_stride + n0 + row,
                        a.out_dtype, y);
       }

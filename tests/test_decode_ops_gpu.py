@@ -384,6 +384,24 @@ def test_linear_large_and_tiny_values(ctx):
     w.close()
 
 
+@pytest.mark.parametrize("group", [32, 64, 128])
+@pytest.mark.parametrize("dt", ["f32", "bf16"])
+def test_linear_rows_near_the_types_largest(ctx, dt, group):
+    """Sums of a block's products with its codes, before the scale makes them smaller, are
+    beyond f32's range; the results are not."""
+    g = gen(7)
+    codes, scales = random_weight(g, 70, 256, group)
+    scales = (scales.float() * 2.0 ** -10).half()
+    w, wd = qm.Q4Weight(ctx, codes, scales), dense(codes, scales)
+    for rows in (1, 9, 33):
+        x = (torch.sign(randn(g, rows, 256)) * 3e38).to(DT[dt])
+        y = qm.linear_q4(w, x)
+        ctx.synchronize()
+        assert y.isfinite().all()
+        check_linear(y, x.double(), wd, dt)
+    w.close()
+
+
 @pytest.mark.parametrize("where", ["captured", "another context"])
 def test_linear_after_new_weights_wherever_the_last_product_was(ctx, stream, where):
     """New weights, a product of them that has not run or ran on another stream, and at
