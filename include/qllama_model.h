@@ -279,7 +279,8 @@ int ql_llama_quantize(ql_llama* m, int32_t group);
  * probability, or a drafted id outside the vocabulary ends the sequence: its
  * new token is -1 and the context's status is raised (QL_ERR_DEVICE at the next
  * synchronize).  (Of probabilities, an accepted draft's rows are read at its id
- * alone.)  ql_kv_truncate then drops the rejected drafts' cache rows.
+ * alone.  Should the GPU not run a sequence's blocks side by side within a second, its
+ * tokens are -1 and the status is raised too.)  ql_kv_truncate then drops the rejected drafts' cache rows.
  * tokens and accepted must not overlap each other or an input.  Device pointers,
  * aligned to their element size. */
 #define QL_VERIFY_LOGITS 0

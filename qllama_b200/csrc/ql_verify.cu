@@ -58,7 +58,10 @@ struct VerifyArgs {
 //      turn.
 // The CTAs of a cluster tell each other their sums by stores into one another's
 // shared memory that count on an mbarrier there; all make the same decisions from the
-// same numbers.  Nothing is kept outside shared memory.
+// same numbers.  Nothing is kept outside shared memory.  A CTA whose wait for the others
+// runs out writes -1 for the sequence and stays until they are at their end, so that no
+// store of theirs meets shared memory that is no longer its own; the others have all
+// that was sent to them when they leave.
 // A small call is bound by the latencies of its steps, one after the other (32
 // sequences, one row of 32000: 24 us with every warp following every decision, 17 us
 // with the weights computed anew at every turn of the search).  So one loop takes all
@@ -109,8 +112,9 @@ __device__ __forceinline__ double warp_totals(const double (&v)[4]) {
   t += shfl_xor(t, 2);
   return t + shfl_xor(t, 1);
 }
-// A wait that looks often before it looks at the clock.
-__device__ __forceinline__ void await(uint64_t* bar, uint32_t parity, uint32_t* status) {
+// A wait that looks often before it looks at the clock.  False, with the status raised,
+// when the time ran out.
+__device__ __forceinline__ bool await(uint64_t* bar, uint32_t parity, uint32_t* status) {
   for (int i = 0; i < 64; ++i) {
     uint32_t ok;
     asm volatile(
@@ -120,9 +124,9 @@ __device__ __forceinline__ void await(uint64_t* bar, uint32_t parity, uint32_t* 
         : "=r"(ok)
         : "r"(ql::smem_u32(bar)), "r"(parity)
         : "memory");
-    if (ok) return;
+    if (ok) return true;
   }
-  ql::mbar_wait_cluster(bar, parity, status);
+  return ql::mbar_wait_cluster(bar, parity, status);
 }
 __device__ __forceinline__ void st_async_f64(uint32_t remote_addr, double v, uint32_t remote_bar) {
   asm volatile("st.async.shared::cluster.mbarrier::complete_tx::bytes.b64 [%0], %1, [%2];" ::"r"(
@@ -199,10 +203,12 @@ __global__ void __launch_bounds__(T, T == 1024 ? 1 : 3) verify_kernel(const Veri
   __shared__ double pow2_32[32];                         // 2^(j/32)
   __shared__ int32_t id_of[QL_VERIFY_MAX_DRAFTS + 1];    // the drafts
   __shared__ double u_of[QL_VERIFY_MAX_DRAFTS + 1];
+  __shared__ int lost;  // a wait for the other CTAs ran out
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, V = a.vocab;
   const int rank = static_cast<int>(cluster_rank()), ctas = static_cast<int>(cluster_size());
   const int b = blockIdx.x / ctas;
   if (tid == 0) {
+    lost = 0;
     for (uint64_t& bar : bars) ql::mbar_init(&bar, 1);
     ql::fence_mbar_init();
   }
@@ -351,7 +357,10 @@ __global__ void __launch_bounds__(T, T == 1024 ? 1 : 3) verify_kernel(const Veri
     __syncthreads();
 #pragma unroll 1
     for (int turn = 0; turn < 2; ++turn) {
-      if (turn == 1) await(&bars[0], 0, a.status);
+      if (turn == 1 && !__all_sync(0xffffffffu, await(&bars[0], 0, a.status))) {
+        lost = 1;
+        break;
+      }
 #pragma unroll 1
       for (int r = warp; r < nrows; r += kVerifyWarps) {
         float2 z = none;
@@ -380,6 +389,7 @@ __global__ void __launch_bounds__(T, T == 1024 ? 1 : 3) verify_kernel(const Veri
     }
     __syncthreads();
   }
+  int32_t* const tok = a.tokens + static_cast<size_t>(b) * (a.drafts + 1);
 
   // ---- 2. Warp 0: the first draft that is not accepted, from `pos` on.
   // verdict: 0 none (pos = n), 1 rejected, 2 too close for f32 sums, 3 cannot be decided
@@ -418,7 +428,6 @@ __global__ void __launch_bounds__(T, T == 1024 ? 1 : 3) verify_kernel(const Veri
     verdict = pos < n ? d : 0;
     if (verdict != 3 && !usable(pos)) verdict = 3;
   };
-  int32_t* const tok = a.tokens + static_cast<size_t>(b) * (a.drafts + 1);
   // Everything but the new token, which is `token` if that is known already.
   auto write = [&](bool known, int token) {
     if (rank != 0) return;
@@ -433,11 +442,12 @@ __global__ void __launch_bounds__(T, T == 1024 ? 1 : 3) verify_kernel(const Veri
     }
   };
   if constexpr (MODE == kGreedy) {
-    if (warp != 0) return;
-    decide();
-    write(true, verdict == 3 ? -1 : __float_as_int(row_stat[pos].y));
-    if (verdict == 3) raise();
-  } else {
+    if (warp == 0 && !lost) {
+      decide();
+      write(true, verdict == 3 ? -1 : __float_as_int(row_stat[pos].y));
+      if (verdict == 3) raise();
+    }
+  } else if (MODE == kProbs || !lost) {
     // ---- 3.
     const int lo = static_cast<int>(static_cast<long long>(V) * rank / ctas);
     const int hi = static_cast<int>(static_cast<long long>(V) * (rank + 1) / ctas);
@@ -545,7 +555,13 @@ __global__ void __launch_bounds__(T, T == 1024 ? 1 : 3) verify_kernel(const Veri
             if (h + lane % 8 < ctas)
               st_async_f64(ql::mapa_shared(mine, h + lane % 8), t,
                            ql::mapa_shared(ql::smem_u32(bar), h + lane % 8));
-          await(bar, turn >> 1 & 1, a.status);
+          if (!__all_sync(0xffffffffu, await(bar, turn >> 1 & 1, a.status))) {
+            if (lane == 0) {
+              lost = 1;
+              next_step.what = kDone;
+            }
+            continue;
+          }
           t = 0.0;
 #pragma unroll
           for (int h = 0; h < kMaxCluster; h += 8)
@@ -669,6 +685,12 @@ __global__ void __launch_bounds__(T, T == 1024 ? 1 : 3) verify_kernel(const Veri
       if (lane == 0) next_step = z;
     }
   }
+  if (lost && warp == 0) {
+    for (int i = lane; i <= a.drafts; i += 32) tok[i] = -1;
+    if (lane == 0) a.accepted[b] = 0;
+  }
+  ql::cluster_arrive_relaxed();
+  if (lost) ql::cluster_wait();
 }
 
 // CTAs of a cluster: up to 16, in powers of two, while all sequences' CTAs are not many
