@@ -70,7 +70,9 @@ int ql_ctx_set_stream(ql_ctx* ctx, void* stream);
 /* Order between the context's stream and `stream` (a cudaStream_t of the same device; NULL =
  * the legacy default stream), without waiting on the host: later work of the context starts
  * when what `stream` holds now is done (wait), and the other way round (join).  A pair of
- * them around a call lets it use buffers that belong to `stream`. */
+ * them around a call lets it use buffers that belong to `stream`.  They do nothing while
+ * the context's stream is being captured and `stream` is not; if only `stream` is, the
+ * context's work between them becomes part of its graph. */
 int ql_ctx_wait_stream(ql_ctx* ctx, void* stream);
 int ql_ctx_join_stream(ql_ctx* ctx, void* stream);
 /* Wait for all work queued by this context; returns QL_ERR_DEVICE if a

@@ -21,6 +21,7 @@
 #include <atomic>
 #include <cstring>
 #include <memory>
+#include <mutex>
 #include <string>
 #include <vector>
 
@@ -515,11 +516,25 @@ int ql_ctx_set_stream(ql_ctx* c, void* stream) {
   return QL_OK;
 }
 
-// `after` waits for what `before` holds now.
-static int order_streams(ql_ctx* c, int which, cudaStream_t before, cudaStream_t after) {
+static bool is_capturing(cudaStream_t s) {
+  if (!s || s == cudaStreamLegacy) return false;  // cannot be
+  cudaStreamCaptureStatus st = cudaStreamCaptureStatusNone;
+  if (cudaStreamIsCapturing(s, &st) != cudaSuccess) cudaGetLastError();
+  return st == cudaStreamCaptureStatusActive;
+}
+
+// The context's stream waits for what `stream` holds now, or (join) the other way round.
+static int order_streams(ql_ctx* c, cudaStream_t stream, bool join) {
   ql_device_guard dev(c->device);
   QL_CUDA(dev.error(), "set device");
-  cudaEvent_t& e = c->order[which];
+  // Recorded into a graph of its own, the context's work takes place when that graph is
+  // launched, ordered by whoever launches it.
+  if (is_capturing(c->stream) && !is_capturing(stream)) return QL_OK;
+  const cudaStream_t before = join ? c->stream : stream, after = join ? stream : c->stream;
+  // two threads with calls on one context: an event's record and its wait belong together
+  static std::mutex mutex;
+  std::lock_guard<std::mutex> lock(mutex);
+  cudaEvent_t& e = c->order[join];
   if (!e) QL_CUDA(cudaEventCreateWithFlags(&e, cudaEventDisableTiming), "create an event");
   QL_CUDA(cudaEventRecord(e, before), "record an event");
   QL_CUDA(cudaStreamWaitEvent(after, e, 0), "wait for an event");
@@ -528,12 +543,12 @@ static int order_streams(ql_ctx* c, int which, cudaStream_t before, cudaStream_t
 
 int ql_ctx_wait_stream(ql_ctx* c, void* stream) {
   if (!c) return fail(QL_ERR_INVALID, "ql_ctx_wait_stream: ctx is NULL");
-  return order_streams(c, 0, static_cast<cudaStream_t>(stream), c->stream);
+  return order_streams(c, static_cast<cudaStream_t>(stream), false);
 }
 
 int ql_ctx_join_stream(ql_ctx* c, void* stream) {
   if (!c) return fail(QL_ERR_INVALID, "ql_ctx_join_stream: ctx is NULL");
-  return order_streams(c, 1, c->stream, static_cast<cudaStream_t>(stream));
+  return order_streams(c, static_cast<cudaStream_t>(stream), true);
 }
 
 int ql_ctx_synchronize(ql_ctx* c) {

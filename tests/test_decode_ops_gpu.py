@@ -7,6 +7,7 @@ Tolerances count roundings: u(t) = eps(t) / 2 is the most that one rounding to t
 moves a value, relative to it.
 """
 import ctypes
+import threading
 
 import numpy as np
 import pytest
@@ -927,6 +928,51 @@ def test_a_context_of_its_own_in_a_captured_stream(ctx, own, stream):
         got = y.clone()
         assert torch.equal(got, qm.linear_q4(w, *qm.rms_norm(own, x, wt, 1e-5, out_dtype="q8_0")))
     stream.synchronize()
+    w.close()
+
+
+def test_a_captured_context_called_from_another_stream(ctx, stream):
+    """A context whose stream is being captured, while torch's current stream is not: the
+    call is part of the graph, and nothing orders it with the current stream."""
+    g = gen(44)
+    k = 256
+    x, wt, y = randn(g, 3, k), 1 + 0.1 * randn(g, k), torch.empty(3, k, device="cuda")
+    want = qm.rms_norm(ctx, x, wt, 1e-5)
+    graph, other = torch.cuda.CUDAGraph(), torch.cuda.Stream()
+    stream.synchronize()
+    with torch.cuda.graph(graph, stream=stream, capture_error_mode="thread_local"):
+        with torch.cuda.stream(other):
+            qm.rms_norm(ctx, x, wt, 1e-5, out=y)
+    y.zero_()
+    graph.replay()
+    stream.synchronize()
+    assert torch.equal(y, want)
+
+
+def test_two_threads_on_a_context_of_its_own(own):
+    """Calls of one context from two threads with streams of their own: each is ordered
+    with its own stream."""
+    g = gen(45)
+    k, n = 2048, 512
+    w = qm.Q4Weight(own, *random_weight(g, n, k, 32))
+    xs = [randn(g, 4, k) for _ in range(2)]
+    want = [qm.linear_q4(w, x) for x in xs]
+    torch.cuda.synchronize()
+    bad = []
+
+    def work(i):
+        with torch.cuda.stream(torch.cuda.Stream()):
+            for _ in range(100):
+                torch.cuda._sleep(20_000)
+                if not torch.equal(qm.linear_q4(w, xs[i] * 1), want[i]):
+                    bad.append(i)
+
+    threads = [threading.Thread(target=work, args=(i,)) for i in range(2)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    assert not bad
     w.close()
 
 
