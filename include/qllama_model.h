@@ -162,7 +162,9 @@ int ql_llama_generate(ql_llama* m, ql_kv* kv, int32_t seq, const int32_t* prompt
  * out_dtype Q8_0: out [rows, hidden] holds int8 values and out_scale
  * [rows, hidden/32] one f16 scale d per 32 columns, by the cache's rule:
  * d = max|y| / 127, value = round(y / d) with ties away from zero, d stored
- * as f16 (65504 at most; larger values saturate).  A block that holds a NaN or
+ * as f16 (65504 at most; larger values saturate).  Quotients are f32 within some
+ * units in the last place, so that a value within 1e-4 of a tie, or a d that close
+ * (relative to f16's step) to one, may be the neighbouring one.  A block that holds a NaN or
  * an infinity gets a NaN scale, so that it reads back as NaN.
  *
  * x and residual have x_stride / residual_stride elements from row to row
@@ -198,6 +200,8 @@ int ql_rms_norm(ql_ctx* ctx, const ql_norm_args* args);
 typedef struct ql_q4 ql_q4;
 int ql_q4_create(ql_ctx* ctx, int32_t out_features, int32_t in_features, int32_t group,
                  ql_q4** out);
+/* Waits for the stream of the context that the handle was made with; products that
+ * other contexts have queued must be done. */
 int ql_q4_destroy(ql_q4* w);
 int ql_q4_shape(const ql_q4* w, int32_t* out_features, int32_t* in_features, int32_t* group);
 /* From codes [out_features, in_features/2] (byte j of a row: column 2j in the
@@ -222,8 +226,9 @@ int ql_q4_get(const ql_q4* w, uint8_t* codes, void* scales, int32_t mem);
 
 /* y = x W^T for a few rows x [rows, in_features] (Linear::forward,
  * layers.rs:148-171): single tokens, drafted tokens, small batches.  The
- * kernel is built for up to some 64 rows, where the weights' bytes are the cost;
- * more rows are taken in passes of that size.
+ * kernel is built for a few rows, where the weights' bytes are the cost: a pass
+ * over the weights takes up to 32 rows (F16, BF16, Q8_0) or 8 (F32), and more
+ * rows are taken in that many passes.
  *   in_dtype F32, F16, BF16: x as given, every product with a code exact (an
  *     infinity in an F32 row gives NaN; F32 magnitudes below 2^-110 count in
  *     steps of 2^-133);

@@ -85,7 +85,8 @@ __device__ __forceinline__ float rcp_fast(float v) {  // within 1 ulp
 
 // Q8_0 scale d of a block whose largest magnitude is `most`, and inv = 1 / d.  The two
 // divisions of the rule are a product with 1/127 and an approximate reciprocal, each
-// within an ulp (they were a tenth of the instructions).  `limit` is where values are
+// within an ulp (they were a tenth of the instructions).  A value y / d, 127 at most, is
+// then off by 127 * 3 * 2^-23 or less: next to a tie it may go to the other side.  `limit` is where values are
 // cut: finite only if the scale saturates, 0 for a block with a NaN or an infinity.
 __device__ __forceinline__ __half q8_scale(uint32_t most, float& inv, float& limit) {
   float d = __uint_as_float(most) * (1.0f / 127.0f);
@@ -225,10 +226,11 @@ __device__ __forceinline__ void store_part(void* base, size_t i, int dt, const f
 // LEAD: the row length is no multiple of eight, so a row starts `lead` elements
 // into an aligned group of eight.  Groups keep that alignment -- it is the same
 // in every contiguous tensor, whatever its type -- and only the row's first and
-// last go element by element (2000 rows of 4101 bf16 columns: 52.8 us with
-// element-wise loads throughout).
-// WARP: a warp per row, kNormRows rows to a CTA, for many short rows (8000 x 128 bf16
-// 8.6 us with a CTA for each, 4.8 us so; 8000 x 1000 12.7 us and 15.4 us).
+// last go element by element (2000 rows of 4101 bf16 columns 19.2 us, 52.8 us
+// with element-wise loads throughout).
+// WARP: a warp per row, kNormRows rows to a CTA, for many short rows (8000 x 128 bf16 with
+// a residual 8.6 us with a CTA for each, 2.9 us so; 8000 x 512 9.0 us and 6.3 us; 8000 x
+// 1000 12.5 us and 15.4 us).
 constexpr int kNormMax = 16384;  // 512 threads x 32 columns
 constexpr int kNormRows = 8;
 template <int DT, int WT, int NV, bool LEAD, bool WARP>
@@ -645,7 +647,8 @@ struct LinearArgs {
 // The weights' bytes (0.52-0.56 of them per weight) are the cost of a few rows, so
 // each goes from HBM to the lane that multiplies it once, through a ring in shared
 // memory that every warp keeps for itself (cp.async, kD sets deep; a __syncwarp is
-// the only barrier of the loop).  Codes turn into f16 / bf16 exactly (a nibble in the
+// the only barrier of the loop).  More than 32 rows (8 of f32) are passes, each with all
+// of the weights.  Codes turn into f16 / bf16 exactly (a nibble in the
 // mantissa of 1024 or 1/4, less an offset), or into int8 (a two's-complement nibble in
 // the high half of a byte: 16 times its value).  The weights are the A operand (16
 // rows of W), x the B operand (8 columns), so one row of x costs as much as eight.
@@ -653,9 +656,8 @@ struct LinearArgs {
 // in f32 and added to f32 sums.  f32 rows: three bf16 parts of 8 significand bits
 // carry a value's 24 exactly (down to 2^-110, where the last part meets bf16's smallest
 // step, 2^-133); the parts are three columns of B, whose sums are added at the end.
-// One CTA an SM, each with an equal share of W's row tiles (an even share matters
-// more than anything else: CTAs of a few tiles, several an SM, left a third of the
-// time to the last of them).  The columns are cut into 8 ranges, one for each warp of
+// One CTA an SM, each with an equal share of W's row tiles (with CTAs of a few tiles,
+// several an SM, the last of them worked alone).  The columns are cut into 8 ranges, one for each warp of
 // a team; WR teams take every WR-th tile.  The loads of the next tiles are under way
 // while the ranges are joined, in order.  Every order of additions is the same for
 // all variants and row counts, so a row's bits depend only on it and W.
