@@ -279,7 +279,9 @@ int ql_llama_quantize(ql_llama* m, int32_t group);
  * draft NULL: the drafts are certain (q_i(x_i) = 1), as those looked up in the
  * text are.  n_draft NULL: every sequence has `drafts`; entries are clamped to
  * [0, drafts], and what lies behind a sequence's drafts is not read.
- * Sums over the vocabulary that decide a token are f64.
+ * Sums over the vocabulary that decide a token are f64, as are p_i(x_i) and q_i(x_i) in
+ * a decision that f32 leaves open (below f64's smallest number they are 0); an id of
+ * less than 1e-299 times its row's most probable counts as nothing in the sums.
  * A row that is reached and holds a NaN or +inf, or has no positive
  * probability, or a drafted id outside the vocabulary ends the sequence: its
  * new token is -1 and the context's status is raised (QL_ERR_DEVICE at the next

@@ -44,8 +44,8 @@ struct VerifyArgs {
 //      the one pass over the logits, bound by their bytes.  (Greedy: largest logit and
 //      its id.)
 //   2. Every draft is decided from its two logits and those sums.  A decision whose
-//      two sides are within 2^-14 of each other, far more than the f32 error, is
-//      taken again from f64 sums of its rows.
+//      two sides are within 2^-14 of each other, far more than the f32 error, or below
+//      f32's range is taken again from f64 sums of its rows, p and q being f64 numbers.
 //   3. The draw compares running sums over the whole vocabulary with a threshold,
 //      where an error of 1e-7 would change one token in some thousands: its sums are
 //      f64, of the rows' weights wp, wq = exp((logit - maximum) / T).  After a rejected
@@ -146,9 +146,16 @@ struct Exp64 {
   // 2^e no longer is a number of the type.
   double least;
   __device__ __forceinline__ double operator()(float x, double m) const {
+    return at(static_cast<double>(x) - m);
+  }
+  // the square of half the exponent's: down to f64's smallest numbers
+  __device__ __forceinline__ double all(float x, double m) const {
+    const double h = at(0.5 * (static_cast<double>(x) - m));
+    return h * h;
+  }
+  __device__ __forceinline__ double at(double d) const {
     constexpr double L = 0.693147180559945309417232 / 32.0;
     constexpr double magic = 6755399441055744.0;  // 1.5 * 2^52
-    const double d = static_cast<double>(x) - m;
     const double t = fma(d, scale, magic);
     const int k = __double2loint(t);
     const double r = fma(d, scale, magic - t);
@@ -180,8 +187,8 @@ struct VerifyStep {
   double ratio;   // ids count where wp > ratio wq
   double fp, fq;  // and weigh wp fp - wq fq
 };
-// With sums: of the rows at a close decision, of its draft alone, of what is left, of a
-// part of it; without: the decisions from pos on, the end.
+// With sums: of the rows at a close decision, of what is left, of a part of it; without:
+// that decision by its sums, the decisions from pos on, the end.
 enum : int { kTotals = 0, kAtDraft, kLeft, kNarrow, kBegin, kGiveUp, kDone };
 
 // T threads: 1024 where a cluster's CTAs have an SM each, 256 where three share one.
@@ -528,6 +535,17 @@ __global__ void __launch_bounds__(T, T == 1024 ? 1 : 3) verify_kernel(const Veri
         if (verdict == 2) what = kTotals;
         else if (verdict == 3) what = kGiveUp;
         else draw = true;
+      } else if (z.what == kAtDraft) {  // (its own turn: 11.0 us for one sequence, 11.3 in the
+        // branch that has the sums, where more values are held)
+        double uq = u[pos];
+        if (has_q)
+          uq *= ex.all(__shfl_sync(0xffffffffu, drafted_q, pos), row_stat[n + 1 + pos].x) / zq;
+        draw = !(uq < ex.all(__shfl_sync(0xffffffffu, drafted_p, pos), row_stat[pos].x) / zp);
+        verdict = 1;
+        if (!draw) {
+          ++pos;
+          what = kBegin;
+        }
       } else if (z.what < kNarrow) {
         // lanes 8 i ..: sum i of the CTA
         double t = 0.0;
@@ -536,70 +554,59 @@ __global__ void __launch_bounds__(T, T == 1024 ? 1 : 3) verify_kernel(const Veri
         t += shfl_xor(t, 4);
         t += shfl_xor(t, 2);
         t += shfl_xor(t, 1);
-        if (z.what == kAtDraft) {  // every CTA has looked at the id itself
-          const double wp = __shfl_sync(0xffffffffu, t, 16), wq = __shfl_sync(0xffffffffu, t, 24);
-          draw = !(u[pos] * (has_q ? wq / zq : 1.0) < wp / zp);
-          verdict = 1;
-          if (!draw) {
-            ++pos;
-            what = kBegin;
+        // the cluster's sums: a rank one exchange ahead writes the other turn's
+        uint64_t* const bar = &bars[1 + (turn & 1)];
+        if (lane == 0) ql::mbar_arrive_expect_tx(bar, static_cast<uint32_t>(32 * ctas));
+        __syncwarp();
+        const uint32_t mine = ql::smem_u32(&sums_of[turn & 1][lane / 8][rank]);
+#pragma unroll
+        for (int h = 0; h < kMaxCluster; h += 8)
+          if (h + lane % 8 < ctas)
+            st_async_f64(ql::mapa_shared(mine, h + lane % 8), t,
+                         ql::mapa_shared(ql::smem_u32(bar), h + lane % 8));
+        if (!__all_sync(0xffffffffu, await(bar, turn >> 1 & 1, a.status))) {
+          if (lane == 0) {
+            lost = 1;
+            next_step.what = kDone;
           }
+          continue;
+        }
+        t = 0.0;
+#pragma unroll
+        for (int h = 0; h < kMaxCluster; h += 8)
+          if (h + lane % 8 < ctas) t += sums_of[turn & 1][lane / 8][h + lane % 8];
+        t += shfl_xor(t, 4);
+        t += shfl_xor(t, 2);
+        t += shfl_xor(t, 1);  // lanes 8 i ..: sum i of the cluster
+        const double inv = 1.0 / t;
+        const double t2 = __shfl_sync(0xffffffffu, t, 16), t3 = __shfl_sync(0xffffffffu, t, 24);
+        if (z.what == kTotals) {
+          zp = t2;
+          zq = t3;
+          what = kAtDraft;
+          z.to = z.from;
         } else {
-          // the cluster's sums: a rank one exchange ahead writes the other turn's
-          uint64_t* const bar = &bars[1 + (turn & 1)];
-          if (lane == 0) ql::mbar_arrive_expect_tx(bar, static_cast<uint32_t>(32 * ctas));
-          __syncwarp();
-          const uint32_t mine = ql::smem_u32(&sums_of[turn & 1][lane / 8][rank]);
-#pragma unroll
-          for (int h = 0; h < kMaxCluster; h += 8)
-            if (h + lane % 8 < ctas)
-              st_async_f64(ql::mapa_shared(mine, h + lane % 8), t,
-                           ql::mapa_shared(ql::smem_u32(bar), h + lane % 8));
-          if (!__all_sync(0xffffffffu, await(bar, turn >> 1 & 1, a.status))) {
-            if (lane == 0) {
-              lost = 1;
-              next_step.what = kDone;
-            }
-            continue;
+          const bool less = z.fq != 0;
+          if (less && MODE == kLogits) {
+            z.fp = __shfl_sync(0xffffffffu, inv, 16);
+            z.fq = __shfl_sync(0xffffffffu, inv, 24);
           }
-          t = 0.0;
-#pragma unroll
-          for (int h = 0; h < kMaxCluster; h += 8)
-            if (h + lane % 8 < ctas) t += sums_of[turn & 1][lane / 8][h + lane % 8];
-          t += shfl_xor(t, 4);
-          t += shfl_xor(t, 2);
-          t += shfl_xor(t, 1);  // lanes 8 i ..: sum i of the cluster
-          const double inv = 1.0 / t;
-          const double t2 = __shfl_sync(0xffffffffu, t, 16), t3 = __shfl_sync(0xffffffffu, t, 24);
-          if (z.what == kTotals) {
-            zp = t2;
-            zq = t3;
-            what = kAtDraft;
-            z.from = ids[pos];
-            z.to = z.from + 1;
-          } else {
-            const bool less = z.fq != 0;
-            if (less && MODE == kLogits) {
-              z.fp = __shfl_sync(0xffffffffu, inv, 16);
-              z.fq = __shfl_sync(0xffffffffu, inv, 24);
-            }
-            const double left = __shfl_sync(0xffffffffu, t, 0) * z.fp -
-                                __shfl_sync(0xffffffffu, t, 8) * z.fq;
-            th = u[n] * left;
-            search = left > 0 && t2 < INFINITY && t3 < INFINITY;
-            if (search && less && MODE == kLogits && left < 0.03125 && z.ratio != t2 / t3) {
-              search = false;
+          const double left = __shfl_sync(0xffffffffu, t, 0) * z.fp -
+                              __shfl_sync(0xffffffffu, t, 8) * z.fq;
+          th = u[n] * left;
+          search = left > 0 && t2 < INFINITY && t3 < INFINITY;
+          if (search && less && MODE == kLogits && left < 0.03125 && z.ratio != t2 / t3) {
+            search = false;
+            what = kLeft;
+            z.ratio = t2 / t3;
+            z.fp = z.fq = 1.0;
+          } else if (!search) {
+            what = kGiveUp;  // probabilities that are none, unless
+            if ((less || z.out >= 0) && left <= 0) {  // the draft's took all: the target
               what = kLeft;
-              z.ratio = t2 / t3;
-              z.fp = z.fq = 1.0;
-            } else if (!search) {
-              what = kGiveUp;  // probabilities that are none, unless
-              if ((less || z.out >= 0) && left <= 0) {  // the draft's took all: the target
-                what = kLeft;
-                z.out = -1;
-                z.ratio = z.fq = 0.0;
-                z.fp = 1.0;
-              }
+              z.out = -1;
+              z.ratio = z.fq = 0.0;
+              z.fp = 1.0;
             }
           }
         }
@@ -678,7 +685,7 @@ __global__ void __launch_bounds__(T, T == 1024 ? 1 : 3) verify_kernel(const Veri
         z.from = lo;
         z.to = hi;
       }
-      if (what == kTotals || what == kAtDraft) {
+      if (what == kTotals) {
         z.out = -1;
         z.ratio = 0.0;
       }

@@ -664,6 +664,30 @@ def test_verify_probabilities_below_f32(ctx):
     assert tokens[1, 0].item() != 7 and tokens[1, 0].item() >= 0
 
 
+@pytest.mark.parametrize("depth, T", [(702.0, 1.0), (7.0, 0.01), (690.5, 1.0), (725.0, 1.0)])
+def test_verify_probabilities_near_f64s_smallest(ctx, depth, T):
+    """A decision between probabilities of 1e-300 to 1e-317, and a probability that is not
+    0 against a uniform of 0 or a draft's probability of 0."""
+    inf = float("inf")
+    target = torch.zeros(5, 2, 50, device="cuda")
+    draft = torch.zeros(5, 1, 50, device="cuda")
+    target[:, 0, 7], draft[:, 0, 7] = -depth - 2 * T, -depth
+    target[2, 0, 7] = -inf
+    draft[3, 0, 7] = -inf
+    ids = torch.full((5, 1), 7, dtype=torch.int32, device="cuda")
+    un = torch.full((5, 2), 0.5, dtype=torch.float64, device="cuda")
+    # e^-2 = 0.135; at e^-727 / 50 a step of f64's smallest numbers is 2e-6 of p
+    un[:, 0] = torch.tensor([0.13, 0.14, 0.0, 0.5, 0.0])
+    tokens, accepted = qm.verify_drafts(ctx, target, draft, ids, un, T)
+    ctx.synchronize()
+    assert accepted.tolist() == [1, 0, 0, 1, 1]
+    assert tokens[:, 0].tolist()[3:] == [7, 7] and not {7, -1} & set(tokens[1:3, 0].tolist())
+    assert accepted.tolist() == verify_f64(target, draft, ids, un, T, None, False)[1].tolist()
+    certain, accepted = qm.verify_drafts(ctx, target, None, ids, un, T)
+    ctx.synchronize()
+    assert accepted.tolist() == [0, 0, 0, 0, 1]
+
+
 def test_verify_masked_and_bad_rows(ctx):
     g = gen(9)
     torch.manual_seed(9)
