@@ -49,6 +49,8 @@ extern "C" {
 #define QL_BF16 2
 #define QL_Q8_0 3 /* GGUF Q8_0: blocks of 32 int8 values with one f16 scale (cache only) */
 
+#define QL_Q4_0 4 /* blocks of 32 4-bit codes with one f16 scale (cache only) */
+
 /* ---- memory kinds for the buffers of one call ---- */
 #define QL_MEM_DEVICE 0
 #define QL_MEM_HOST 1
@@ -86,15 +88,22 @@ int ql_ctx_synchronize(ql_ctx* ctx);
  * Layout per layer: pages of `page_size` positions, each page holding
  * [num_kv_heads][page_size][head_dim] elements of K (post-RoPE, cache.rs:3-6)
  * and the same of V.  Q8_0 keeps the int8 values and the f16 block scales in
- * two planes with the same page geometry.  Sequence `s` owns pages through a
- * block table shared by all layers.
+ * two planes with the same page geometry, Q4_0 the codes (half a byte each) and the
+ * scales.  Sequence `s` owns pages through a block table shared by all layers.
+ *
+ * Q4_0: 32 values as codes 0..15 and a scale d, each standing for d * (code - 8): with m
+ * the block's value of largest magnitude (the first of equals), d = f16(m / -8) and
+ * code = clamp(round(x / d) + 8, 0, 15), ties to even; d == 0 gives code 8.  A block that
+ * holds a NaN or an infinity, or whose d leaves f16's range, gets a NaN scale and reads back
+ * as NaN.  The order of a row's codes in memory is the library's own (ql_kv_read and
+ * ql_kv_get give the values).
  */
 typedef struct {
   int32_t num_layers;
   int32_t max_seq_len;  /* positions per sequence (capacity, cache.rs:138-143) */
   int32_t num_kv_heads;
   int32_t head_dim;     /* even; the fast kernels take 64 or 128 */
-  int32_t dtype;        /* QL_F32, QL_F16, QL_BF16 or QL_Q8_0 */
+  int32_t dtype;        /* QL_F32, QL_F16, QL_BF16, QL_Q8_0 or QL_Q4_0 */
   int32_t page_size;    /* positions per page, a multiple of 64 (0 = 64) */
   int32_t max_batch;    /* sequence slots (0 = 1) */
   int32_t num_pages;    /* pages in the pool (0 = max_batch * ceil(max_seq_len/page_size)) */
@@ -112,6 +121,10 @@ int ql_kv_clear_seq(ql_kv* kv, int32_t seq);
  * new_len.  No counterpart in the reference, whose cache only appends or
  * clears; it serves roll-back (a rejected speculative draft, a replayed step). */
 int ql_kv_truncate(ql_kv* kv, int32_t seq, int64_t new_len);
+/* ql_kv_truncate for `batch` sequences at once, such as a batch whose drafts have been
+ * verified: every length is checked before any moves.  seq_ids, new_len: host arrays. */
+int ql_kv_truncate_batch(ql_kv* kv, int32_t batch, const int32_t* seq_ids,
+                         const int64_t* new_len);
 /* KvCache::seq_len (cache.rs:245-247): written prefix of layer 0 of `seq`. */
 int ql_kv_seq_len(const ql_kv* kv, int32_t seq, int64_t* out_len);
 /* Written prefix of one layer of one sequence. */
@@ -133,6 +146,51 @@ int ql_kv_update(ql_ctx* ctx, ql_kv* kv, int32_t layer, int32_t seq, const void*
 int ql_kv_get(ql_ctx* ctx, const ql_kv* kv, int32_t layer, int32_t seq,
               const int32_t* positions, int64_t n_positions, float* k_out, float* v_out,
               int32_t mem);
+
+/* ---- rows of several sequences at once -------------------------------------
+ * Appends the new rows of a batch of sequences, each with its own number of them, and
+ * rotates K (and the queries, if given) on the way: steps 3-4 of
+ * Attention::forward_with_cache (layers.rs:397-413) without the attention.  What follows is
+ * ql_attn_forward_appended or ql_attn_forward_sparse with the rotated queries, per group of
+ * sequences of one length, or whatever else reads the cache.  The rows are packed: sequence
+ * 0's tokens first, then sequence 1's; a token's row is heads x head_dim values, and
+ * *_stride elements lie from one token to the next (0 = contiguous), so that the columns of
+ * a fused projection can be given as they are.
+ * start_pos[b] must equal the current length ("must continue"); new_len[b] may be 0.  The
+ * rotation is ql_attn_forward's, in f64 and rounded once to f32, and the rows are then
+ * converted to the cache's type; q_out gets the rotated queries rounded to q_out_dtype.
+ * q_out [tokens, num_heads, head_dim] is contiguous and may be q itself (of the same type,
+ * contiguous); any other overlap with an input is refused.  Device pointers, aligned to
+ * their element size. */
+typedef struct {
+  int32_t layer_idx;
+  int32_t batch;             /* sequences, each slot once (0 is a no-op) */
+  const int32_t* seq_ids;    /* host array [batch] */
+  const int64_t* start_pos;  /* host array [batch] */
+  const int32_t* new_len;    /* host array [batch]: new tokens of each sequence, >= 0 */
+  int32_t num_heads;         /* of q; 0: no queries */
+  int32_t num_kv_heads;
+  int32_t head_dim;
+  float rope_theta;
+  int32_t in_dtype;          /* q, k, v: QL_F32, QL_F16 or QL_BF16 */
+  int32_t q_out_dtype;
+  int64_t q_stride, k_stride, v_stride;
+  const void* q;
+  const void* k;
+  const void* v;
+  void* q_out;
+} ql_append_args;
+
+int ql_kv_append(ql_ctx* ctx, ql_kv* kv, const ql_append_args* args);
+
+/* Rows of several sequences out of the cache in stream order, on the device: positions
+ * start_pos[b] .. start_pos[b] + lens[b] - 1 (inside the written prefix) of each listed
+ * sequence, packed into k_out and v_out [tokens, num_kv_heads, head_dim], dequantised and
+ * rounded once to out_dtype (QL_F32, QL_F16 or QL_BF16).  A sequence may be listed more
+ * than once.  (ql_kv_get copies to f32 and waits.) */
+int ql_kv_read(ql_ctx* ctx, const ql_kv* kv, int32_t layer, int32_t batch,
+               const int32_t* seq_ids, const int64_t* start_pos, const int32_t* lens,
+               int32_t out_dtype, void* k_out, void* v_out);
 
 /* ---- the attention operator ----------------------------------------------
  * Steps 3-7 of Attention::forward_with_cache (layers.rs:397-455) for a

@@ -104,17 +104,43 @@ int ql_llama_forward(ql_llama* m, ql_kv* kv, int32_t seq, const int32_t* ids, in
  * wqkv_t: device f32 [in_features, (num_heads + 2*num_kv_heads)*head_dim],
  * the transposed weights of q, k and v side by side; q_rot: device f32
  * [batch, new_len, num_heads, head_dim], the rotated queries.  The cache
- * must store f32, f16 or bf16; positions must continue each sequence
- * ("must continue"), and the sequences' lengths advance.  Every product is an
- * f32 sequential sum in the reference's order. */
+ * must store f32, f16 or bf16 (others take ql_kv_append or ql_attn_forward);
+ * positions must continue each sequence ("must continue"), and the sequences'
+ * lengths advance.  Every product is an f32 sequential sum in the reference's
+ * order. */
 int ql_qkv_rope_append(ql_ctx* ctx, ql_kv* kv, const ql_attn_args* args, const float* x,
                        int32_t in_features, const float* wqkv_t, float* q_rot);
 
 /* Steps 5-7 of forward_with_cache (layers.rs:425-455) over rows that
- * ql_qkv_rope_append has just written: args as for ql_attn_forward with
- * q = the rotated queries (in_dtype f32) and k, v unused; start_pos[b] +
+ * ql_qkv_rope_append or ql_kv_append has just written: args as for ql_attn_forward with
+ * q = the rotated queries and k, v unused; start_pos[b] +
  * new_len must equal the sequence's current length. */
 int ql_attn_forward_appended(ql_ctx* ctx, ql_kv* kv, const ql_attn_args* args);
+
+/* ql_attn_forward_appended over a part of a long cache: each token's KV heads attend to
+ * `blocks` blocks of 64 positions (positions 64 j .. 64 j + 63) of those up to the token's
+ * own: the first `first`, the newest `last`, and of the others those of the largest scores,
+ * the lower block of equal ones.  A token that sees no more than `blocks` blocks attends to
+ * all of them, as ql_attn_forward_appended does.
+ * Block j's score for a KV head bounds from above what any of its keys can score, summed
+ * over the head's group of queries:
+ *   sum_h sum_d max(q_hd * lo_jd, q_hd * hi_jd),
+ * with lo and hi the least and the largest value of channel d among the block's stored keys
+ * (dequantised; rounded to f16 for an f16 cache, else to bf16), evaluated in f64.  A score
+ * that is NaN counts as the largest.
+ * The bounds belong to the cache: a layer's first call allocates them (1/32 of an f16
+ * cache's keys; make it before a capture), and a call adds those of the blocks that have
+ * filled up since.  selected (may be NULL) receives each list in ascending order, -1 behind
+ * its end.  args->mem must be QL_MEM_DEVICE; batch * new_len is at most 65535. */
+typedef struct {
+  int32_t blocks;     /* >= first + last */
+  int32_t first;      /* >= 0 */
+  int32_t last;       /* >= 1: the newest block is the token's own */
+  int32_t* selected;  /* device [batch, new_len, num_kv_heads, blocks] or NULL */
+} ql_sparse_args;
+
+int ql_attn_forward_sparse(ql_ctx* ctx, ql_kv* kv, const ql_attn_args* args,
+                           const ql_sparse_args* sparse);
 
 /* SamplerConfig (src/sampler/sampler.rs:15-25).  temperature <= 0 is greedy
  * (argmax after the repeat penalty, ties to the smaller id). */

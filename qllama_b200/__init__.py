@@ -29,8 +29,8 @@ import numpy as np
 
 from . import build as _build
 
-F32, F16, BF16, Q8_0 = 0, 1, 2, 3
-DTYPES = {"f32": F32, "f16": F16, "bf16": BF16, "q8_0": Q8_0}
+F32, F16, BF16, Q8_0, Q4_0 = 0, 1, 2, 3, 4
+DTYPES = {"f32": F32, "f16": F16, "bf16": BF16, "q8_0": Q8_0, "q4_0": Q4_0}
 MEM_DEVICE, MEM_HOST = 0, 1
 
 OK, ERR_INVALID, ERR_CUDA, ERR_OOM, ERR_NO_DEVICE, ERR_UNSUPPORTED, ERR_DEVICE = range(7)
@@ -40,12 +40,13 @@ EXPORTS = (
     "ql_version", "ql_last_error", "ql_ctx_create", "ql_ctx_destroy", "ql_ctx_set_stream",
     "ql_ctx_wait_stream", "ql_ctx_join_stream", "ql_ctx_synchronize", "ql_kv_create", "ql_kv_destroy", "ql_kv_clear", "ql_kv_clear_seq",
     "ql_kv_seq_len", "ql_kv_layer_len", "ql_kv_update", "ql_kv_get", "ql_attn_forward",
-    "ql_attn_decode_noalloc", "ql_kv_truncate", "ql_comm_unique_id", "ql_comm_create",
+    "ql_attn_decode_noalloc", "ql_kv_truncate", "ql_kv_truncate_batch", "ql_kv_append",
+    "ql_kv_read", "ql_comm_unique_id", "ql_comm_create",
     "ql_comm_destroy", "ql_comm_buffer", "ql_attn_forward_sharded",
     # include/qllama_model.h
     "ql_llama_create", "ql_llama_destroy", "ql_llama_get_config", "ql_llama_set_tensor",
     "ql_llama_load_gguf", "ql_llama_forward", "ql_sample", "ql_llama_generate",
-    "ql_qkv_rope_append", "ql_attn_forward_appended",
+    "ql_qkv_rope_append", "ql_attn_forward_appended", "ql_attn_forward_sparse",
     "ql_rms_norm", "ql_q4_create", "ql_q4_destroy", "ql_q4_shape", "ql_q4_set",
     "ql_q4_set_blocks", "ql_q4_quantize", "ql_q4_get", "ql_linear_q4", "ql_llama_quantize",
     "ql_verify_drafts",
@@ -81,6 +82,19 @@ class AttnArgs(ctypes.Structure):
                 ("out_dtype", ctypes.c_int32), ("mem", ctypes.c_int32),
                 ("q", ctypes.c_void_p), ("k", ctypes.c_void_p), ("v", ctypes.c_void_p),
                 ("out", ctypes.c_void_p)]
+
+
+class AppendArgs(ctypes.Structure):
+    _fields_ = [("layer_idx", ctypes.c_int32), ("batch", ctypes.c_int32),
+                ("seq_ids", ctypes.POINTER(ctypes.c_int32)),
+                ("start_pos", ctypes.POINTER(ctypes.c_int64)),
+                ("new_len", ctypes.POINTER(ctypes.c_int32)), ("num_heads", ctypes.c_int32),
+                ("num_kv_heads", ctypes.c_int32), ("head_dim", ctypes.c_int32),
+                ("rope_theta", ctypes.c_float), ("in_dtype", ctypes.c_int32),
+                ("q_out_dtype", ctypes.c_int32), ("q_stride", ctypes.c_int64),
+                ("k_stride", ctypes.c_int64), ("v_stride", ctypes.c_int64),
+                ("q", ctypes.c_void_p), ("k", ctypes.c_void_p), ("v", ctypes.c_void_p),
+                ("q_out", ctypes.c_void_p)]
 
 
 class CommId(ctypes.Structure):
@@ -120,6 +134,9 @@ def load(build_if_missing: bool = True) -> ctypes.CDLL:
     L.ql_kv_clear.argtypes = [vp]
     L.ql_kv_clear_seq.argtypes = [vp, i32]
     L.ql_kv_truncate.argtypes = [vp, i32, i64]
+    L.ql_kv_truncate_batch.argtypes = [vp, i32, vp, vp]
+    L.ql_kv_append.argtypes = [vp, vp, ctypes.POINTER(AppendArgs)]
+    L.ql_kv_read.argtypes = [vp, vp, i32, i32, vp, vp, vp, i32, vp, vp]
     L.ql_kv_seq_len.argtypes = [vp, i32, i64p]
     L.ql_kv_layer_len.argtypes = [vp, i32, i32, i64p]
     L.ql_kv_update.argtypes = [vp, vp, i32, i32, vp, i64p, i32, vp, i64p, i32, i32, i32p, i64,
@@ -206,7 +223,7 @@ class Context:
 class KvCache:
     """KvCache::new(num_layers, max_seq_len, num_kv_heads, head_dim) on the device.
 
-    Extra arguments: storage dtype ("f32", "f16", "bf16", "q8_0"), page_size,
+    Extra arguments: storage dtype ("f32", "f16", "bf16", "q8_0", "q4_0"), page_size,
     max_batch (sequence slots), num_pages (0 = enough for every slot).
     """
 
@@ -214,7 +231,7 @@ class KvCache:
                  head_dim: int, dtype: str = "f16", page_size: int = 64, max_batch: int = 1,
                  num_pages: int = 0):
         self.ctx = ctx
-        self.num_kv_heads, self.head_dim = num_kv_heads, head_dim
+        self.num_kv_heads, self.head_dim, self.dtype = num_kv_heads, head_dim, dtype
         cfg = KvConfig(num_layers, max_seq_len, num_kv_heads, head_dim, DTYPES[dtype], page_size,
                        max_batch, num_pages)
         h = ctypes.c_void_p()
@@ -252,9 +269,109 @@ class KvCache:
     def clear_seq(self, seq: int) -> None:
         _check(load().ql_kv_clear_seq(self._h, seq))
 
-    def truncate(self, seq: int, new_len: int) -> None:
-        """Roll sequence `seq` back to `new_len` positions in every layer (pages kept)."""
-        _check(load().ql_kv_truncate(self._h, seq, new_len))
+    def truncate(self, seq, new_len) -> None:
+        """Roll sequence `seq` back to `new_len` positions in every layer (pages kept);
+        lists of sequences and of their lengths roll back a batch at once."""
+        if np.ndim(seq) == 0:
+            _check(load().ql_kv_truncate(self._h, seq, new_len))
+            return
+        n = len(seq)
+        if len(new_len) != n:
+            raise QllamaError(ERR_INVALID, f"{n} sequence(s) but {len(new_len)} length(s)")
+        _check(load().ql_kv_truncate_batch(self._h, n, (ctypes.c_int32 * n)(*seq),
+                                           (ctypes.c_int64 * n)(*new_len)))
+
+    def append(self, layer: int, k, v, start_pos, new_len, rope_theta: float, seq_ids=None,
+               q=None, q_out=None):
+        """Appends the new rows of several sequences, rotated on the way (ql_kv_append).
+
+        k, v [tokens, num_kv_heads, head_dim] and q [tokens, heads, head_dim] (f32, f16
+        or bf16 CUDA tensors; the tokens may have a stride) hold the sequences' rows one
+        after the other: new_len[b] tokens of sequence seq_ids[b] (default b) from
+        position start_pos[b] on.  Returns the rotated queries (q_out, or a new tensor
+        of q's type), None without q.
+        """
+        from . import model as m
+
+        L = m._L or m._start()
+        ctx, shape = self.ctx, (self.num_kv_heads, self.head_dim)
+        batch, total, rows = self._ragged(seq_ids, start_pos, new_len)
+        dev = ctx.device
+
+        def tokens(t, name, heads):
+            if t.dim() != 3 or t.shape[0] != total or t.shape[2] != shape[1] or \
+                    (heads and t.shape[1] != heads):
+                raise m._invalid(f"{name} has shape {tuple(t.shape)}, expected [{total}, "
+                                 f"{heads or 'heads'}, {shape[1]}]")
+            if t.dtype is not k.dtype:
+                raise m._invalid(f"{name} must have k's type")
+            width = t.shape[1] * t.shape[2]
+            if t.is_contiguous() or total < 2 and t[:1].is_contiguous():
+                return 0, m._on(dev, t, name)
+            if t.stride(2) != 1 or t.stride(0) < width or \
+                    (t.shape[1] > 1 and t.stride(1) != t.shape[2]):
+                raise m._invalid(f"{name} must have a token's heads contiguous")
+            return t.stride(0), m._on(dev, t, name)
+
+        dt = m._float_code(k, "k")
+        ks, kp = tokens(k, "k", shape[0])
+        vs, vp = tokens(v, "v", shape[0])
+        hq, qs, qp, op, od = 0, 0, None, None, F32
+        if q is not None:
+            qs, qp = tokens(q, "q", 0)
+            hq = q.shape[1]
+            q_out = m._output(ctx, q_out, q.shape, q.dtype if q_out is None else q_out.dtype,
+                              "q_out")
+            od, op = m._float_code(q_out, "q_out"), m._on(dev, q_out, "q_out")
+        args = AppendArgs(layer, batch, *rows, hq, *shape, rope_theta, dt, od, qs, ks, vs, qp, kp,
+                          vp, op)
+        side = m._fork(ctx)
+        rc = L.ql_kv_append(ctx._h, self._h, ctypes.byref(args))
+        if rc:
+            m._raise(rc)
+        if side is not None:
+            m._join(ctx, side)
+        return q_out
+
+    def read(self, layer: int, start_pos, lens, seq_ids=None, out=None, out_dtype=None):
+        """Rows of several sequences on the device, in stream order (ql_kv_read): lens[b]
+        positions of sequence seq_ids[b] (default b) from start_pos[b] on, packed into
+        (k, v), each [tokens, num_kv_heads, head_dim] of out_dtype (default: the cache's
+        type, f32 for Q8_0 and Q4_0); `out`: the two tensors to write."""
+        from . import model as m
+
+        L = m._L or m._start()
+        ctx = self.ctx
+        batch, total, rows = self._ragged(seq_ids, start_pos, lens)
+        shape = (total, self.num_kv_heads, self.head_dim)
+        k, v = out if out is not None else (None, None)
+        if out is None:
+            t = m._named_type(out_dtype or (self.dtype if self.dtype[0] != "q" else "f32"))
+        else:
+            t = k.dtype
+        k = m._output(ctx, k, shape, t, "k")
+        v = m._output(ctx, v, shape, t, "v")
+        code, kp, vp = m._float_code(k, "out"), m._on(ctx.device, k, "k"), m._on(ctx.device, v, "v")
+        side = m._fork(ctx)
+        rc = L.ql_kv_read(ctx._h, self._h, layer, batch, *rows, code, kp, vp)
+        if rc:
+            m._raise(rc)
+        if side is not None:
+            m._join(ctx, side)
+        return k, v
+
+    @staticmethod
+    def _ragged(seq_ids, start_pos, lens):
+        """(sequences, tokens, (seq_ids, start_pos, lens) as C arrays)."""
+        batch = len(lens)
+        if seq_ids is None:
+            seq_ids = range(batch)
+        if len(start_pos) != batch or len(seq_ids) != batch:
+            raise QllamaError(ERR_INVALID, f"{batch} length(s) but {len(start_pos)} position(s) "
+                                           f"and {len(seq_ids)} sequence(s)")
+        return batch, int(sum(lens)), ((ctypes.c_int32 * batch)(*seq_ids),
+                                       (ctypes.c_int64 * batch)(*start_pos),
+                                       (ctypes.c_int32 * batch)(*lens))
 
     def seq_len(self, seq: int = 0) -> int:
         out = ctypes.c_int64()

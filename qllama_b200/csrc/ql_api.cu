@@ -26,6 +26,7 @@
 #include <vector>
 
 #include "../../include/qllama_attn.h"
+#include "../../include/qllama_model.h"
 #include "ql_device.cuh"
 #include "ql_internal.h"
 #include "ql_kernels.cuh"
@@ -57,6 +58,12 @@ int cuda_fail(cudaError_t e, const char* what) {
   } while (0)
 
 size_t elem_bytes(int dt) { return dt == QL_F32 ? 4 : (dt == QL_Q8_0 ? 1 : 2); }
+
+// Bytes of `n` values in a cache's value plane (a whole number of rows).
+size_t plane_bytes(int dt, size_t n) { return dt == QL_Q4_0 ? n / 2 : n * elem_bytes(dt); }
+
+// Storage types whose blocks of 32 values have their scales in a plane of their own.
+bool block_dtype(int dt) { return dt == QL_Q8_0 || dt == QL_Q4_0; }
 
 bool valid_io_dtype(int dt) { return dt == QL_F32 || dt == QL_F16 || dt == QL_BF16; }
 
@@ -106,7 +113,7 @@ struct ql_kv {
   ql_kv_config cfg{};
   int pages_per_seq = 0;
   std::vector<void*> k, v;             // per layer
-  std::vector<uint16_t*> ks, vs;       // per layer, Q8_0 scales
+  std::vector<uint16_t*> ks, vs;       // per layer, Q8_0 and Q4_0 scales
   std::vector<CUtensorMap> kmap, vmap;  // per layer, split-KV kernel descriptors
   bool have_maps = false;
   int32_t* d_table = nullptr;          // [max_batch][pages_per_seq]
@@ -126,14 +133,37 @@ struct ql_kv {
   // uploads.  Reserved to the table's size at creation, so a call never
   // grows it.
   std::vector<int32_t> patch_idx;
+  // Bounds of whole blocks for attention over selected ones, made by a layer's first such call
+  // (BoundsArgs::bounds), and how many leading blocks of each sequence have theirs.
+  std::vector<uint16_t*> bounds;   // per layer, null until then
+  std::vector<int32_t> bounded;    // [layer][seq]
 };
 
 namespace {
 
+bool is_capturing(cudaStream_t s) {
+  if (!s || s == cudaStreamLegacy) return false;  // cannot be
+  cudaStreamCaptureStatus st = cudaStreamCaptureStatusNone;
+  if (cudaStreamIsCapturing(s, &st) != cudaSuccess) cudaGetLastError();
+  return st == cudaStreamCaptureStatusActive;
+}
+
 int ensure_ws(ql_ctx* c, size_t bytes) {
-  if (bytes <= c->ws_bytes) return QL_OK;
+  const bool capturing = bytes > 0 && is_capturing(c->stream);
+  if (bytes <= c->ws_bytes) {
+    c->ws_captured |= capturing;
+    return QL_OK;
+  }
+  if (capturing)
+    return fail(QL_ERR_INVALID, "the workspace has to grow to %zu bytes: make the call once before "
+                "its capture", bytes);
   QL_CUDA(cudaStreamSynchronize(c->stream), "synchronize before growing workspace");
-  if (c->ws) cudaFree(c->ws);
+  if (c->ws && c->ws_captured) {
+    c->retired.push_back(c->ws);  // a captured graph goes on using it
+    c->ws_captured = false;
+  } else if (c->ws) {
+    cudaFree(c->ws);
+  }
   c->ws = nullptr;
   c->ws_bytes = 0;
   size_t want = bytes + bytes / 4 + (1 << 20);
@@ -143,9 +173,21 @@ int ensure_ws(ql_ctx* c, size_t bytes) {
 }
 
 int ensure_counters(ql_ctx* c, size_t n) {
-  if (n <= c->counters_n) return QL_OK;
+  const bool capturing = is_capturing(c->stream);
+  if (n <= c->counters_n) {
+    c->counters_captured |= capturing;
+    return QL_OK;
+  }
+  if (capturing)
+    return fail(QL_ERR_INVALID, "the split counters have to grow: make the call once before its "
+                "capture");
   QL_CUDA(cudaStreamSynchronize(c->stream), "synchronize before growing counters");
-  if (c->counters) cudaFree(c->counters);
+  if (c->counters && c->counters_captured) {
+    c->retired.push_back(c->counters);
+    c->counters_captured = false;
+  } else if (c->counters) {
+    cudaFree(c->counters);
+  }
   c->counters = nullptr;
   c->counters_n = 0;
   size_t want = n + n / 2 + 1024;
@@ -161,8 +203,8 @@ ql::CacheView view_of(const ql_kv* kv, int layer) {
   ql::CacheView c;
   c.k = kv->k[layer];
   c.v = kv->v[layer];
-  c.k_scale = kv->cfg.dtype == QL_Q8_0 ? kv->ks[layer] : nullptr;
-  c.v_scale = kv->cfg.dtype == QL_Q8_0 ? kv->vs[layer] : nullptr;
+  c.k_scale = block_dtype(kv->cfg.dtype) ? kv->ks[layer] : nullptr;
+  c.v_scale = block_dtype(kv->cfg.dtype) ? kv->vs[layer] : nullptr;
   c.block_table = kv->d_table;
   c.pages_per_seq = kv->pages_per_seq;
   c.num_pages = kv->cfg.num_pages;
@@ -205,10 +247,30 @@ int encode_q_map(CUtensorMap* m, void* base, int hd, uint64_t rows) {
   return QL_OK;
 }
 
+// The identity rotation (cos 1, sin 0 leaves a pair exactly as it is), for queries that arrive
+// rotated.
+int ensure_identity(ql_kv* kv) {
+  if (kv->d_rope_id) return QL_OK;
+  std::vector<double2> id(std::max(1, kv->cfg.head_dim / 2), make_double2(1.0, 0.0));
+  double2* p = nullptr;
+  QL_CUDA(cudaMalloc(&p, id.size() * sizeof(double2)), "allocate rope table");
+  cudaError_t e = cudaMemcpyAsync(p, id.data(), id.size() * sizeof(double2),
+                                  cudaMemcpyHostToDevice, kv->ctx->stream);
+  if (e == cudaSuccess) e = cudaStreamSynchronize(kv->ctx->stream);
+  if (e != cudaSuccess) {
+    cudaFree(p);
+    return cuda_fail(e, "upload the identity rotation");
+  }
+  kv->d_rope_id = p;
+  return QL_OK;
+}
+
 // Builds (once per theta) the f64 (cos, sin) table of every position with the
 // reference formula: freq_i = theta^(-2i/hd) via pow, angle = pos * freq_i
 // (src/tensor/ops.rs:193-207), evaluated by the host libm as the reference does.
 int ensure_rope(ql_kv* kv, float theta) {
+  const int r = ensure_identity(kv);
+  if (r != QL_OK) return r;
   if (kv->d_rope && kv->rope_theta == theta) return QL_OK;
   const int hd = kv->cfg.head_dim, pairs = hd / 2, n = kv->cfg.max_seq_len;
   std::vector<double> freq(pairs);
@@ -223,13 +285,6 @@ int ensure_rope(ql_kv* kv, float theta) {
   if (!kv->d_rope) {
     QL_CUDA(cudaMalloc(&kv->d_rope, std::max<size_t>(1, tab.size()) * sizeof(double2)),
             "allocate rope table");
-    // the identity rotation (cos 1, sin 0 leaves a pair exactly as it is)
-    std::vector<double2> id(std::max(1, pairs), make_double2(1.0, 0.0));
-    QL_CUDA(cudaMalloc(&kv->d_rope_id, id.size() * sizeof(double2)), "allocate rope table");
-    QL_CUDA(cudaMemcpyAsync(kv->d_rope_id, id.data(), id.size() * sizeof(double2),
-                            cudaMemcpyHostToDevice, kv->ctx->stream),
-            "upload the identity rotation");
-    QL_CUDA(cudaStreamSynchronize(kv->ctx->stream), "wait for the identity rotation");
   }
   // On the context's stream (the kernels that read the table run there), and
   // waited for before the host vector goes away.
@@ -313,6 +368,17 @@ int64_t& len_at(ql_kv* kv, int layer, int seq) {
   return kv->len[static_cast<size_t>(layer) * kv->cfg.max_batch + seq];
 }
 
+int32_t& bounded_at(ql_kv* kv, int layer, int seq) {
+  return kv->bounded[static_cast<size_t>(layer) * kv->cfg.max_batch + seq];
+}
+
+// A sequence goes back to `len` positions: what later appends rewrite has no bounds.
+void shorten(ql_kv* kv, int layer, int seq, int64_t len) {
+  len_at(kv, layer, seq) = len;
+  int32_t& n = bounded_at(kv, layer, seq);
+  n = static_cast<int32_t>(std::min<int64_t>(n, len / ql::kTile));
+}
+
 }  // namespace
 
 int ql_ctx_workspace(ql_ctx* c, size_t bytes, void** out) {
@@ -339,6 +405,38 @@ int ql_check_status(ql_ctx* c) {
 }
 
 namespace {
+
+// Brings the bounds of a layer's whole blocks up to date for the listed sequences: the blocks
+// that have filled up since the last call (a launch for one call in 64 of a decode loop).
+int ensure_bounds(ql_ctx* c, ql_kv* kv, int layer, const int32_t* seqs, int batch) {
+  if (!kv->bounds[layer]) {
+    if (is_capturing(c->stream))
+      return fail(QL_ERR_INVALID, "a layer's first call over selected blocks allocates their "
+                  "bounds: make it before the capture");
+    const size_t bytes = static_cast<size_t>(kv->cfg.num_pages) * (kv->cfg.page_size / ql::kTile) *
+                         kv->cfg.num_kv_heads * 2 * kv->cfg.head_dim * sizeof(uint16_t);
+    QL_CUDA(cudaMalloc(&kv->bounds[layer], std::max<size_t>(bytes, 256)), "allocate block bounds");
+  }
+  ql::BoundsArgs a{};
+  int64_t total = 0;
+  for (int b = 0; b < batch; ++b) {
+    const int whole = static_cast<int>(len_at(kv, layer, seqs[b]) / ql::kTile);
+    a.blocks.seq[b] = seqs[b];
+    a.blocks.start[b] = bounded_at(kv, layer, seqs[b]);
+    a.blocks.first[b] = static_cast<int32_t>(total);
+    total += whole - a.blocks.start[b];
+  }
+  a.blocks.first[batch] = static_cast<int32_t>(total);
+  if (total == 0) return QL_OK;
+  a.bounds = kv->bounds[layer];
+  a.cache = view_of(kv, layer);
+  a.batch = batch;
+  a.status = c->status;
+  QL_CUDA(ql::launch_bounds(a, c->stream), "launch block bounds");
+  for (int b = 0; b < batch; ++b)
+    bounded_at(kv, layer, seqs[b]) = static_cast<int32_t>(len_at(kv, layer, seqs[b]) / ql::kTile);
+  return QL_OK;
+}
 
 // Split plan of the split-KV decode kernel: the 64-position tiles each CTA
 // streams, and the most splits any (token, KV head) job is cut into.
@@ -501,6 +599,7 @@ int ql_ctx_destroy(ql_ctx* c) {
   cudaSetDevice(c->device);
   if (c->own) cudaStreamSynchronize(c->own);
   if (c->ws) cudaFree(c->ws);
+  for (void* p : c->retired) cudaFree(p);
   if (c->counters) cudaFree(c->counters);
   if (c->status) cudaFree(c->status);
   for (cudaEvent_t e : c->order)
@@ -514,13 +613,6 @@ int ql_ctx_set_stream(ql_ctx* c, void* stream) {
   if (!c) return fail(QL_ERR_INVALID, "ql_ctx_set_stream: ctx is NULL");
   c->stream = stream ? static_cast<cudaStream_t>(stream) : c->own;
   return QL_OK;
-}
-
-static bool is_capturing(cudaStream_t s) {
-  if (!s || s == cudaStreamLegacy) return false;  // cannot be
-  cudaStreamCaptureStatus st = cudaStreamCaptureStatusNone;
-  if (cudaStreamIsCapturing(s, &st) != cudaSuccess) cudaGetLastError();
-  return st == cudaStreamCaptureStatusActive;
 }
 
 // The context's stream waits for what `stream` holds now, or (join) the other way round.
@@ -568,14 +660,14 @@ int ql_kv_create(ql_ctx* c, const ql_kv_config* cfg_in, ql_kv** out) {
       cfg.max_batch < 0 || cfg.num_pages < 0)
     return fail(QL_ERR_INVALID,
                 "KV cache needs num_layers >= 0, max_seq_len >= 0, num_kv_heads > 0, head_dim > 0");
-  if (cfg.dtype < QL_F32 || cfg.dtype > QL_Q8_0)
+  if (cfg.dtype < QL_F32 || cfg.dtype > QL_Q4_0)
     return fail(QL_ERR_INVALID, "unknown KV cache dtype %d", cfg.dtype);
   if (cfg.page_size % ql::kTile != 0)
     return fail(QL_ERR_INVALID, "page_size %d must be a positive multiple of %d", cfg.page_size,
                 ql::kTile);
-  if (cfg.dtype == QL_Q8_0 && cfg.head_dim % 32 != 0)
-    return fail(QL_ERR_INVALID, "Q8_0 storage needs head_dim divisible by 32, got %d",
-                cfg.head_dim);
+  if (block_dtype(cfg.dtype) && cfg.head_dim % 32 != 0)
+    return fail(QL_ERR_INVALID, "%s storage needs head_dim divisible by 32, got %d",
+                cfg.dtype == QL_Q8_0 ? "Q8_0" : "Q4_0", cfg.head_dim);
   QL_CUDA(cudaSetDevice(c->device), "set device");
   ql_kv* kv = new ql_kv;
   kv->ctx = c;
@@ -583,7 +675,7 @@ int ql_kv_create(ql_ctx* c, const ql_kv_config* cfg_in, ql_kv** out) {
   if (cfg.num_pages == 0) cfg.num_pages = cfg.max_batch * std::max(1, kv->pages_per_seq);
   kv->cfg = cfg;
   const size_t rows = static_cast<size_t>(cfg.num_pages) * cfg.num_kv_heads * cfg.page_size;
-  const size_t bytes = rows * cfg.head_dim * elem_bytes(cfg.dtype);
+  const size_t bytes = plane_bytes(cfg.dtype, rows * cfg.head_dim);
   auto cleanup = [&](int code) {
     ql_kv_destroy(kv);
     return code;
@@ -597,7 +689,7 @@ int ql_kv_create(ql_ctx* c, const ql_kv_config* cfg_in, ql_kv** out) {
     kv->k.push_back(kp);
     kv->v.push_back(vp);
     if (e != cudaSuccess) return cleanup(cuda_fail(e, "allocate KV pool"));
-    if (cfg.dtype == QL_Q8_0) {
+    if (block_dtype(cfg.dtype)) {
       const size_t sb = std::max<size_t>(rows * (cfg.head_dim / 32) * 2, 256);
       uint16_t *a = nullptr, *b = nullptr;
       e = cudaMalloc(&a, sb);
@@ -606,7 +698,7 @@ int ql_kv_create(ql_ctx* c, const ql_kv_config* cfg_in, ql_kv** out) {
       if (e == cudaSuccess) e = cudaMemset(b, 0, sb);
       kv->ks.push_back(a);
       kv->vs.push_back(b);
-      if (e != cudaSuccess) return cleanup(cuda_fail(e, "allocate Q8_0 scales"));
+      if (e != cudaSuccess) return cleanup(cuda_fail(e, "allocate block scales"));
     }
   }
   kv->table.assign(static_cast<size_t>(cfg.max_batch) * std::max(1, kv->pages_per_seq), -1);
@@ -616,6 +708,8 @@ int ql_kv_create(ql_ctx* c, const ql_kv_config* cfg_in, ql_kv** out) {
   kv->free_pages.reserve(cfg.num_pages);
   for (int p = cfg.num_pages - 1; p >= 0; --p) kv->free_pages.push_back(p);
   kv->len.assign(static_cast<size_t>(std::max(1, cfg.num_layers)) * cfg.max_batch, 0);
+  kv->bounds.assign(cfg.num_layers, nullptr);
+  kv->bounded.assign(kv->len.size(), 0);
   cudaError_t e = cudaMalloc(&kv->d_table, kv->table.size() * sizeof(int32_t));
   // Every entry -1 (all bytes 0xff).  The pool memsets above ran on the legacy
   // stream, which the context's non-blocking stream does not wait for: the
@@ -645,6 +739,7 @@ int ql_kv_destroy(ql_kv* kv) {
   for (void* p : kv->v) cudaFree(p);
   for (void* p : kv->ks) cudaFree(p);
   for (void* p : kv->vs) cudaFree(p);
+  for (void* p : kv->bounds) cudaFree(p);
   if (kv->d_table) cudaFree(kv->d_table);
   if (kv->d_rope) cudaFree(kv->d_rope);
   if (kv->d_rope_id) cudaFree(kv->d_rope_id);
@@ -656,6 +751,7 @@ int ql_kv_clear(ql_kv* kv) {
   if (!kv) return fail(QL_ERR_INVALID, "ql_kv_clear: kv is NULL");
   // Lengths back to zero; buffers (and pages) stay, as in cache.rs:231-239.
   std::fill(kv->len.begin(), kv->len.end(), 0);
+  std::fill(kv->bounded.begin(), kv->bounded.end(), 0);
   return QL_OK;
 }
 
@@ -665,7 +761,7 @@ int ql_kv_clear_seq(ql_kv* kv, int32_t seq) {
     return fail(QL_ERR_INVALID, "sequence %d out of range (cache has %d slots)", seq,
                 kv->cfg.max_batch);
   // Stale rows stay in the pages; lengths make them unreachable (cache.rs:231-234).
-  for (int l = 0; l < kv->cfg.num_layers; ++l) len_at(kv, l, seq) = 0;
+  for (int l = 0; l < kv->cfg.num_layers; ++l) shorten(kv, l, seq, 0);
   const int pps = kv->pages_per_seq;
   if (kv->seq_pages[seq] > 0) {
     QL_CUDA(cudaSetDevice(kv->ctx->device), "set device");
@@ -688,14 +784,30 @@ int ql_kv_clear_seq(ql_kv* kv, int32_t seq) {
 
 int ql_kv_truncate(ql_kv* kv, int32_t seq, int64_t new_len) {
   if (!kv) return fail(QL_ERR_INVALID, "ql_kv_truncate: kv is NULL");
-  if (seq < 0 || seq >= kv->cfg.max_batch)
-    return fail(QL_ERR_INVALID, "sequence %d out of range (cache has %d slots)", seq,
-                kv->cfg.max_batch);
-  for (int l = 0; l < kv->cfg.num_layers; ++l)
-    if (new_len < 0 || new_len > len_at(kv, l, seq))
-      return fail(QL_ERR_INVALID, "cannot truncate layer %d of sequence %d to %lld positions "
-                  "(it holds %lld)", l, seq, (long long)new_len, (long long)len_at(kv, l, seq));
-  for (int l = 0; l < kv->cfg.num_layers; ++l) len_at(kv, l, seq) = new_len;
+  return ql_kv_truncate_batch(kv, 1, &seq, &new_len);
+}
+
+int ql_kv_truncate_batch(ql_kv* kv, int32_t batch, const int32_t* seq_ids,
+                         const int64_t* new_len) {
+  if (!kv) return fail(QL_ERR_INVALID, "ql_kv_truncate_batch: kv is NULL");
+  if (batch < 0) return fail(QL_ERR_INVALID, "batch must be >= 0 (got %d)", batch);
+  if (batch > 0 && (!seq_ids || !new_len))
+    return fail(QL_ERR_INVALID, "ql_kv_truncate_batch: NULL argument");
+  for (int i = 0; i < batch; ++i) {
+    const int32_t seq = seq_ids[i];
+    if (seq < 0 || seq >= kv->cfg.max_batch)
+      return fail(QL_ERR_INVALID, "sequence %d out of range (cache has %d slots)", seq,
+                  kv->cfg.max_batch);
+    for (int l = 0; l < kv->cfg.num_layers; ++l)
+      if (new_len[i] < 0 || new_len[i] > len_at(kv, l, seq))
+        return fail(QL_ERR_INVALID, "cannot truncate layer %d of sequence %d to %lld positions "
+                    "(it holds %lld)", l, seq, (long long)new_len[i],
+                    (long long)len_at(kv, l, seq));
+  }
+  // (a sequence named twice ends at the smaller of its lengths)
+  for (int i = 0; i < batch; ++i)
+    for (int l = 0; l < kv->cfg.num_layers; ++l)
+      shorten(kv, l, seq_ids[i], std::min(new_len[i], len_at(kv, l, seq_ids[i])));
   return QL_OK;
 }
 
@@ -841,13 +953,194 @@ int ql_kv_get(ql_ctx* c, const ql_kv* kv, int32_t layer, int32_t seq, const int3
   return QL_OK;
 }
 
+}  // extern "C"
+
+namespace {
+
+// The sequences of a call on rows packed one after the other: each slot once, its rows
+// [start, start + n) inside the cache's capacity (appended ones continue its prefix, read ones
+// lie in it).  Fills the launch's table and, per sequence, where its rows end.
+int ragged_rows(ql_kv* kv, const char* who, int layer, int batch, const int32_t* seq_ids,
+                const int64_t* start_pos, const int32_t* lens, bool append, ql::RaggedTable* t,
+                int64_t* ends) {
+  if (layer < 0 || layer >= kv->cfg.num_layers)
+    return fail(QL_ERR_INVALID, "KV cache layer index %d out of range (cache has %d layers)",
+                layer, kv->cfg.num_layers);
+  if (batch < 0 || batch > ql::kMaxBatch)
+    return fail(QL_ERR_INVALID, "batch %d is outside 0..%d", batch, ql::kMaxBatch);
+  if (batch > 0 && (!seq_ids || !start_pos || !lens))
+    return fail(QL_ERR_INVALID, "%s: seq_ids, start_pos or the lengths are NULL", who);
+  const uint32_t mark = next_seen_epoch(kv);
+  int64_t total = 0;
+  for (int b = 0; b < batch; ++b) {
+    const int s = seq_ids[b];
+    if (s < 0 || s >= kv->cfg.max_batch)
+      return fail(QL_ERR_INVALID, "sequence %d out of range (cache has %d slots)", s,
+                  kv->cfg.max_batch);
+    if (append && kv->seen_mark[s] == mark)
+      return fail(QL_ERR_INVALID, "sequence %d appears twice in one call", s);
+    kv->seen_mark[s] = mark;
+    const int64_t start = start_pos[b], n = lens[b], cur = len_at(kv, layer, s);
+    if (n < 0) return fail(QL_ERR_INVALID, "sequence %d has %lld rows", s, (long long)n);
+    if (start < 0) return fail(QL_ERR_INVALID, "start_pos %lld is negative", (long long)start);
+    if (append) {
+      if (start != cur)
+        return fail(QL_ERR_INVALID,
+                    "positions[0] = %lld must continue from current_len (expected %lld); "
+                    "skipping, backward, or double writes are not allowed",
+                    (long long)start, (long long)cur);
+      if (start + n > kv->cfg.max_seq_len)
+        return fail(QL_ERR_INVALID, "positions[%lld] = %lld exceeds cache capacity %d",
+                    (long long)(kv->cfg.max_seq_len - start), (long long)kv->cfg.max_seq_len,
+                    kv->cfg.max_seq_len);
+    } else if (start > cur || n > cur - start) {
+      return fail(QL_ERR_INVALID,
+                  "positions %lld..%lld of sequence %d reach beyond the written prefix "
+                  "(current_len %lld)", (long long)start, (long long)(start + n - 1), s,
+                  (long long)cur);
+    }
+    t->seq[b] = s;
+    t->start[b] = static_cast<int32_t>(start);
+    t->first[b] = static_cast<int32_t>(total);
+    ends[b] = start + n;
+    total += n;
+    if (total > INT32_MAX / 2)
+      return fail(QL_ERR_INVALID, "%s: more than %d tokens in one call", who, INT32_MAX / 2);
+  }
+  t->first[batch] = static_cast<int32_t>(total);
+  return QL_OK;
+}
+
+// A row stride in elements: 0 stands for contiguous rows.
+bool row_stride(int64_t& stride, int64_t width) {
+  if (stride == 0) stride = width;
+  return stride >= width;
+}
+
+bool aligned_to(const void* p, size_t bytes) {
+  return reinterpret_cast<uintptr_t>(p) % bytes == 0;
+}
+
+}  // namespace
+
+extern "C" {
+
+int ql_kv_append(ql_ctx* c, ql_kv* kv, const ql_append_args* a) {
+  if (!c || !kv || !a) return fail(QL_ERR_INVALID, "ql_kv_append: NULL argument");
+  const int hq = a->num_heads, hkv = a->num_kv_heads, hd = a->head_dim;
+  if (hq < 0 || hkv <= 0 || hd <= 0)
+    return fail(QL_ERR_INVALID, "Attention head counts and head_dim must be positive");
+  if ((hd & 1) != 0)
+    return fail(QL_ERR_INVALID,
+                "RoPE requires shape [seq_len, ..., head_dim] with a positive even head_dim");
+  if (!std::isfinite(a->rope_theta) || a->rope_theta <= 0.f)
+    return fail(QL_ERR_INVALID, "RoPE theta must be finite and positive");
+  if (!valid_io_dtype(a->in_dtype) || (hq > 0 && !valid_io_dtype(a->q_out_dtype)))
+    return fail(QL_ERR_INVALID, "unknown input/output dtype (%d, %d)", a->in_dtype,
+                a->q_out_dtype);
+  if (hkv != kv->cfg.num_kv_heads || hd != kv->cfg.head_dim)
+    return fail(QL_ERR_INVALID, "K shape [_, %d, %d] does not match cache [_, %d, %d]", hkv, hd,
+                kv->cfg.num_kv_heads, kv->cfg.head_dim);
+  ql::RaggedAppendArgs k{};
+  k.q_stride = a->q_stride;
+  k.k_stride = a->k_stride;
+  k.v_stride = a->v_stride;
+  if (!row_stride(k.q_stride, static_cast<int64_t>(hq) * hd) ||
+      !row_stride(k.k_stride, static_cast<int64_t>(hkv) * hd) ||
+      !row_stride(k.v_stride, static_cast<int64_t>(hkv) * hd))
+    return fail(QL_ERR_INVALID, "strides (%lld, %lld, %lld) are below a token's width",
+                (long long)a->q_stride, (long long)a->k_stride, (long long)a->v_stride);
+  int64_t ends[ql::kMaxBatch];
+  int r = ragged_rows(kv, "ql_kv_append", a->layer_idx, a->batch, a->seq_ids, a->start_pos,
+                      a->new_len, true, &k.rows, ends);
+  if (r != QL_OK) return r;
+  const int64_t total = k.rows.first[a->batch];
+  if (total == 0) return QL_OK;
+  if (!a->k || !a->v || (hq > 0 && (!a->q || !a->q_out)))
+    return fail(QL_ERR_INVALID, "ql_kv_append: NULL data");
+  const size_t ib = elem_bytes(a->in_dtype), ob = hq > 0 ? elem_bytes(a->q_out_dtype) : 1;
+  if (!aligned_to(a->k, ib) || !aligned_to(a->v, ib) || !aligned_to(a->q, ib) ||
+      !aligned_to(a->q_out, ob))
+    return fail(QL_ERR_INVALID, "ql_kv_append: a buffer is not aligned to its element size");
+  if (hq > 0) {  // q_out may be q itself; no other overlap
+    const char* o0 = static_cast<const char*>(a->q_out);
+    const char* o1 = o0 + static_cast<size_t>(total) * hq * hd * ob;
+    auto hits = [&](const void* p, int64_t stride, int heads) {
+      const char* p0 = static_cast<const char*>(p);
+      const char* p1 = p0 + (static_cast<size_t>(total - 1) * stride +
+                             static_cast<size_t>(heads) * hd) * ib;
+      return p0 < o1 && o0 < p1;
+    };
+    const bool in_place = a->q_out == a->q && a->q_out_dtype == a->in_dtype &&
+                          k.q_stride == static_cast<int64_t>(hq) * hd;
+    if ((!in_place && hits(a->q, k.q_stride, hq)) || hits(a->k, k.k_stride, hkv) ||
+        hits(a->v, k.v_stride, hkv))
+      return fail(QL_ERR_INVALID, "ql_kv_append: q_out overlaps an input");
+  }
+  ql_device_guard dev(c->device);
+  QL_CUDA(dev.error(), "set device");
+  bool patched = false;  // the append is an ordinary launch: it sees the patch
+  r = reserve_pages(kv, k.rows.seq, ends, a->batch, &patched);
+  if (r == QL_OK) r = ensure_rope(kv, a->rope_theta);
+  if (r != QL_OK) return r;
+  k.q = hq > 0 ? a->q : nullptr;
+  k.k = a->k;
+  k.v = a->v;
+  k.q_out = a->q_out;
+  k.in_dtype = a->in_dtype;
+  k.q_out_dtype = a->q_out_dtype;
+  k.hq = hq;
+  k.batch = a->batch;
+  k.rope = kv->d_rope;
+  k.cache = view_of(kv, a->layer_idx);
+  k.status = c->status;
+  QL_CUDA(ql::launch_ragged_append(k, c->stream), "launch append");
+  for (int b = 0; b < a->batch; ++b) len_at(kv, a->layer_idx, k.rows.seq[b]) = ends[b];
+  return QL_OK;
+}
+
+int ql_kv_read(ql_ctx* c, const ql_kv* kv_in, int32_t layer, int32_t batch,
+               const int32_t* seq_ids, const int64_t* start_pos, const int32_t* lens,
+               int32_t out_dtype, void* k_out, void* v_out) {
+  if (!c || !kv_in) return fail(QL_ERR_INVALID, "ql_kv_read: NULL argument");
+  ql_kv* kv = const_cast<ql_kv*>(kv_in);  // only the marks of the checks are written
+  if (!valid_io_dtype(out_dtype)) return fail(QL_ERR_INVALID, "unknown output dtype %d", out_dtype);
+  ql::RaggedReadArgs k{};
+  int64_t ends[ql::kMaxBatch];
+  const int r = ragged_rows(kv, "ql_kv_read", layer, batch, seq_ids, start_pos, lens, false,
+                            &k.rows, ends);
+  if (r != QL_OK) return r;
+  if (k.rows.first[batch] == 0) return QL_OK;
+  if (!k_out || !v_out) return fail(QL_ERR_INVALID, "ql_kv_read: NULL output");
+  const size_t ob = elem_bytes(out_dtype);
+  if (!aligned_to(k_out, ob) || !aligned_to(v_out, ob))
+    return fail(QL_ERR_INVALID, "ql_kv_read: a buffer is not aligned to its element size");
+  const char *k0 = static_cast<const char*>(k_out), *v0 = static_cast<const char*>(v_out);
+  const size_t bytes = static_cast<size_t>(k.rows.first[batch]) * kv->cfg.num_kv_heads *
+                       kv->cfg.head_dim * ob;
+  if (k0 < v0 + bytes && v0 < k0 + bytes)
+    return fail(QL_ERR_INVALID, "ql_kv_read: k_out and v_out overlap");
+  ql_device_guard dev(c->device);
+  QL_CUDA(dev.error(), "set device");
+  k.k_out = k_out;
+  k.v_out = v_out;
+  k.out_dtype = out_dtype;
+  k.batch = batch;
+  k.cache = view_of(kv, layer);
+  k.status = c->status;
+  QL_CUDA(ql::launch_ragged_read(k, c->stream), "launch read");
+  return QL_OK;
+}
+
 // The operator.  With `peer` (a head-sharded single-token decode), the
 // split-KV kernel stores its rows into every rank's output instead of a->out.
 // appended: the call's K/V rows are already in the cache (written by
 // ql_qkv_rope_append at positions start_pos .. start_pos+new_len-1) and q
 // arrives rotated, so nothing is appended and q is not rotated again.
+// sparse: attention over selected blocks (with `appended`).
 static int attn_forward_impl(ql_ctx* c, ql_kv* kv, const ql_attn_args* a,
-                             const ql::PeerOut* peer, bool appended = false) {
+                             const ql::PeerOut* peer, bool appended = false,
+                             const ql_sparse_args* sparse = nullptr) {
   if (!c || !kv || !a) return fail(QL_ERR_INVALID, "ql_attn_forward: NULL argument");
   const int hq = a->num_heads, hkv = a->num_kv_heads, hd = a->head_dim;
   // Attention::new (layers.rs:254-261)
@@ -927,6 +1220,9 @@ static int attn_forward_impl(ql_ctx* c, ql_kv* kv, const ql_attn_args* a,
     return fail(QL_ERR_INVALID, "q/k/v/out is NULL");
   if (appended && peer)
     return fail(QL_ERR_UNSUPPORTED, "a head-sharded call appends its own rows");
+  if (sparse && 1LL * a->batch * n > 65535)
+    return fail(QL_ERR_UNSUPPORTED, "attention over selected blocks takes up to 65535 tokens a "
+                "call, got %lld", 1LL * a->batch * n);
   if (peer && !(n == 1 && a->mem == QL_MEM_DEVICE && kv->have_maps &&
                 ql::splitkv_supported(hd, kv->cfg.dtype, hq / hkv, kv->cfg.page_size)))
     return fail(QL_ERR_UNSUPPORTED, "the fused head-sharded exchange needs a single-token "
@@ -935,16 +1231,20 @@ static int attn_forward_impl(ql_ctx* c, ql_kv* kv, const ql_attn_args* a,
   bool patched = false;
   int r = appended ? QL_OK : reserve_pages(kv, seqs, ends, a->batch, &patched);
   if (r != QL_OK) return r;
-  r = ensure_rope(kv, a->rope_theta);
+  // rows that are in the cache were rotated when they were appended
+  r = appended ? ensure_identity(kv) : ensure_rope(kv, a->rope_theta);
   if (r != QL_OK) return r;
-
+  if (sparse) {
+    r = ensure_bounds(c, kv, layer, seqs, a->batch);
+    if (r != QL_OK) return r;
+  }
   const int group = hq / hkv;
   const int jobs = a->batch * n;
   const size_t qn = static_cast<size_t>(jobs) * hq * hd, kn = static_cast<size_t>(jobs) * hkv * hd;
   const size_t ib = elem_bytes(a->in_dtype), obb = elem_bytes(a->out_dtype);
-  const bool fast = kv->have_maps && ql::splitkv_supported(hd, kv->cfg.dtype, group,
-                                                          kv->cfg.page_size);
-  const bool tc_prefill = kv->have_maps && n > 1 &&
+  const bool fast = !sparse && kv->have_maps &&
+                    ql::splitkv_supported(hd, kv->cfg.dtype, group, kv->cfg.page_size);
+  const bool tc_prefill = !sparse && (kv->have_maps || kv->cfg.dtype == QL_Q4_0) && n > 1 &&
                           ql::prefill_tc_supported(hd, kv->cfg.dtype, n);
   // split planning for the tensor-core kernel
   int max_tiles = 0;
@@ -956,6 +1256,14 @@ static int attn_forward_impl(ql_ctx* c, ql_kv* kv, const ql_attn_args* a,
     row_tiles[b] = static_cast<int>((end + ql::kTile - 1) / ql::kTile);
     max_tiles = std::max(max_tiles, row_tiles[b]);
   }
+  const int max_blocks = max_tiles;  // of any sequence
+  if (sparse) {
+    max_tiles = std::min(max_tiles, sparse->blocks);
+    for (int b = 0; b < a->batch; ++b) row_tiles[b] = std::min(row_tiles[b], max_tiles);
+    max_len = std::min<int64_t>(max_len, static_cast<int64_t>(max_tiles) * ql::kTile);
+  }
+  // the lists' rows: as the caller asked for them, or as long as they can get
+  const int sel_max = !sparse ? 0 : sparse->selected ? sparse->blocks : max_tiles;
   int tps = max_tiles, max_splits = 1;
   // Too few (token, KV head) jobs to fill half the SMs: the wide kernel, whose
   // consumer groups share each split's tiles, one CTA per SM (latency).
@@ -1013,8 +1321,8 @@ static int attn_forward_impl(ql_ctx* c, ql_kv* kv, const ql_attn_args* a,
   if (tc_prefill) off += align256(static_cast<size_t>(a->batch) * hq * q_rows * hd * 2);
   const size_t o_qs = off;
   if (tc_prefill) off += align256(static_cast<size_t>(a->batch) * hq * q_rows * sizeof(float));
-  // bf16 and Q8_0: every key the call sees, per (sequence, KV head), padded to 128
-  const bool bf_copy = tc_prefill && (kv->cfg.dtype == QL_BF16 || kv->cfg.dtype == QL_Q8_0);
+  // bf16, Q8_0 and Q4_0: every key the call sees, per (sequence, KV head), padded to 128
+  const bool bf_copy = tc_prefill && kv->cfg.dtype != QL_F16;
   const size_t kv_rows = static_cast<size_t>((max_len + 127) / 128) * 128;
   const size_t copy_bytes = static_cast<size_t>(a->batch) * hkv * kv_rows * hd * 2;
   const size_t o_kc = off;
@@ -1028,6 +1336,11 @@ static int attn_forward_impl(ql_ctx* c, ql_kv* kv, const ql_attn_args* a,
   if (!fast) off += align256(static_cast<size_t>(gjobs) * hq * max_len * sizeof(float));
   const size_t o_gd = off;
   if (!fast) off += align256(static_cast<size_t>(gjobs) * hq * max_len * sizeof(double));
+  const size_t o_sc = off;
+  if (sparse) off += align256(static_cast<size_t>(jobs) * hkv * max_blocks * sizeof(double));
+  const size_t o_sel = off;
+  if (sparse && !sparse->selected)
+    off += align256(static_cast<size_t>(jobs) * hkv * sel_max * sizeof(int32_t));
   r = ensure_ws(c, off);
   if (r != QL_OK) return r;
   if (fast && max_splits > 1) {
@@ -1097,9 +1410,9 @@ static int attn_forward_impl(ql_ctx* c, ql_kv* kv, const ql_attn_args* a,
     CUtensorMap qmap;
     r = encode_q_map(&qmap, w + o_qr, hd, static_cast<uint64_t>(a->batch) * hq * q_rows);
     if (r != QL_OK) return r;
-    const CUtensorMap* kmap = &kv->kmap[layer];
-    const CUtensorMap* vmap = &kv->vmap[layer];
-    CUtensorMap kcm, vcm;  // bf16 / Q8_0: the attention kernel reads the f16 copies
+    const CUtensorMap* kmap = kv->have_maps ? &kv->kmap[layer] : nullptr;
+    const CUtensorMap* vmap = kv->have_maps ? &kv->vmap[layer] : nullptr;
+    CUtensorMap kcm, vcm;  // bf16, Q8_0, Q4_0: the attention kernel reads the f16 copies
     if (bf_copy) {
       pa.k_copy = reinterpret_cast<__half*>(w + o_kc);
       pa.v_copy = reinterpret_cast<__half*>(w + o_vc);
@@ -1151,6 +1464,28 @@ static int attn_forward_impl(ql_ctx* c, ql_kv* kv, const ql_attn_args* a,
   at.cluster = cluster;
   at.status = c->status;
   at.seqs = st;
+  if (sparse) {
+    ql::SelectArgs se{};
+    se.q = q;
+    se.in_dtype = a->in_dtype;
+    se.hq = hq;
+    se.group = group;
+    se.batch = a->batch;
+    se.new_len = n;
+    se.take = sel_max;
+    se.first = sparse->first;
+    se.last = sparse->last;
+    se.max_blocks = max_blocks;
+    se.score = reinterpret_cast<double*>(w + o_sc);
+    se.bounds = kv->bounds[layer];
+    se.sel = sparse->selected ? sparse->selected : reinterpret_cast<int32_t*>(w + o_sel);
+    se.cache = cv;
+    se.status = c->status;
+    se.seqs = st;
+    QL_CUDA(ql::launch_select(se, c->stream), "launch the choice of blocks");
+    at.sel = se.sel;
+    at.sel_max = sel_max;
+  }
   if (peer) {
     at.peer = *peer;
     at.peer.total_ctas = max_splits * hkv * jobs;
@@ -1177,6 +1512,18 @@ int ql_attn_forward(ql_ctx* c, ql_kv* kv, const ql_attn_args* a) {
 
 int ql_attn_forward_appended(ql_ctx* c, ql_kv* kv, const ql_attn_args* a) {
   return attn_forward_impl(c, kv, a, nullptr, true);
+}
+
+int ql_attn_forward_sparse(ql_ctx* c, ql_kv* kv, const ql_attn_args* a, const ql_sparse_args* s) {
+  if (!c || !kv || !a || !s) return fail(QL_ERR_INVALID, "ql_attn_forward_sparse: NULL argument");
+  if (s->blocks < 1 || s->first < 0 || s->last < 1 || s->first > s->blocks - s->last)
+    return fail(QL_ERR_INVALID, "blocks %d must hold the first %d (>= 0) and the last %d (>= 1)",
+                s->blocks, s->first, s->last);
+  if (a->mem != QL_MEM_DEVICE)
+    return fail(QL_ERR_INVALID, "ql_attn_forward_sparse takes device buffers only");
+  if (s->selected && !aligned_to(s->selected, sizeof(int32_t)))
+    return fail(QL_ERR_INVALID, "selected is not aligned to its element size");
+  return attn_forward_impl(c, kv, a, nullptr, true, s);
 }
 
 }  // extern "C"
@@ -1209,9 +1556,9 @@ int ql_kv_append_prepare(ql_ctx* c, ql_kv* kv, const ql_attn_args* a, ql::CacheV
   if (hkv != kv->cfg.num_kv_heads || hd != kv->cfg.head_dim)
     return fail(QL_ERR_INVALID, "K shape [%d, %d, %d] does not match cache [_, %d, %d]",
                 a->new_len, hkv, hd, kv->cfg.num_kv_heads, kv->cfg.head_dim);
-  if (kv->cfg.dtype == QL_Q8_0)
+  if (block_dtype(kv->cfg.dtype))
     return fail(QL_ERR_UNSUPPORTED, "the fused projection appends f32, f16 or bf16 rows; a Q8_0 "
-                "cache takes ql_attn_forward");
+                "or Q4_0 cache takes ql_attn_forward");
   const int n = a->new_len;
   int32_t seqs[ql::kMaxBatch];
   int64_t ends[ql::kMaxBatch];

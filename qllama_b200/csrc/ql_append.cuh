@@ -21,6 +21,23 @@ __device__ __forceinline__ int64_t cache_row(const CacheView& c, int seq, int po
   return (static_cast<int64_t>(page) * c.hkv + h) * c.page + pos % c.page;
 }
 
+// The f32 value of column d of a cache row; base and scale: the K or the V planes.
+__device__ __forceinline__ float cache_value(const CacheView& c, const void* base,
+                                             const uint16_t* scale, int64_t row, int d) {
+  const size_t e = static_cast<size_t>(row) * c.hd + d;
+  if (c.dtype == kQ8_0) {
+    float s = __half2float(__ushort_as_half(scale[static_cast<size_t>(row) * (c.hd / 32) + d / 32]));
+    return s * static_cast<float>(static_cast<const int8_t*>(base)[e]);
+  }
+  if (c.dtype == kQ4_0) {
+    const int nb = c.hd / 32, byte = base == c.v ? q4_v_byte(d & ~1, nb) : q4_k_byte(d & ~1, nb);
+    const uint32_t w = static_cast<const uint8_t*>(base)[static_cast<size_t>(row) * (c.hd / 2) + byte];
+    const float s = __half2float(__ushort_as_half(scale[static_cast<size_t>(row) * nb + d / 32]));
+    return s * static_cast<float>(static_cast<int>((d & 1 ? w >> 4 : w) & 15u) - 8);
+  }
+  return load_elem(base, e, c.dtype);
+}
+
 // Source of the RoPE (cos, sin) pairs of one position: the host-built table
 // row, or (DEV) f64 pow/sincos evaluated on the device for callers that have
 // no table (the no-allocation decode entry point).
@@ -46,7 +63,7 @@ __device__ __forceinline__ double2 rope_cs(const RopeSrc& r, int p, int hd) {
 // by the table row when one is given, V as is, both converted to the cache
 // type.
 __device__ __forceinline__ void append_row(const void* kin, const void* vin, int in_dt,
-                                           size_t in_off, const double2* rope_row,
+                                           size_t k_off, size_t v_off, const double2* rope_row,
                                            const CacheView& c, int64_t dst, int lane) {
   const int hd = c.hd;
   const int pairs = hd / 2;
@@ -56,10 +73,10 @@ __device__ __forceinline__ void append_row(const void* kin, const void* vin, int
     const bool valid = p < pairs;
     float k0 = 0.f, k1 = 0.f, v0 = 0.f, v1 = 0.f;
     if (valid) {
-      k0 = load_elem(kin, in_off + 2 * p, in_dt);
-      k1 = load_elem(kin, in_off + 2 * p + 1, in_dt);
-      v0 = load_elem(vin, in_off + 2 * p, in_dt);
-      v1 = load_elem(vin, in_off + 2 * p + 1, in_dt);
+      k0 = load_elem(kin, k_off + 2 * p, in_dt);
+      k1 = load_elem(kin, k_off + 2 * p + 1, in_dt);
+      v0 = load_elem(vin, v_off + 2 * p, in_dt);
+      v1 = load_elem(vin, v_off + 2 * p + 1, in_dt);
       if (rope_row) rope_pair(k0, k1, rope_cs<false>(rope, p, hd), k0, k1);
     }
     const size_t e = static_cast<size_t>(dst) * hd + 2 * p;
@@ -75,6 +92,19 @@ __device__ __forceinline__ void append_row(const void* kin, const void* vin, int
           const size_t si = static_cast<size_t>(dst) * (hd / 32) + (2 * p) / 32;
           c.k_scale[si] = __half_as_ushort(sk);
           c.v_scale[si] = __half_as_ushort(sv);
+        }
+      }
+    } else if (c.dtype == kQ4_0) {  // head_dim is a multiple of 32: both halves are whole blocks
+      uint16_t sk, sv;
+      const uint32_t bk = q4_0_pair(k0, k1, sk), bv = q4_0_pair(v0, v1, sv);
+      if (valid) {
+        const size_t row = static_cast<size_t>(dst) * (hd / 2);
+        static_cast<uint8_t*>(c.k)[row + q4_k_byte(2 * p, hd / 32)] = static_cast<uint8_t>(bk);
+        static_cast<uint8_t*>(c.v)[row + q4_v_byte(2 * p, hd / 32)] = static_cast<uint8_t>(bv);
+        if ((lane & 15) == 0) {
+          const size_t si = static_cast<size_t>(dst) * (hd / 32) + (2 * p) / 32;
+          c.k_scale[si] = sk;
+          c.v_scale[si] = sv;
         }
       }
     } else if (valid) {
@@ -207,7 +237,7 @@ __device__ __forceinline__ void append_kv_row(const AppendArgs& a, int warp, int
   if (!ok) return;
   const size_t in_off = (static_cast<size_t>(b * a.new_len + t) * hkv + h) * a.cache.hd;
   const double2* rope = a.rope ? a.rope + static_cast<size_t>(pos) * (a.cache.hd / 2) : nullptr;
-  append_row(a.k, a.v, a.in_dtype, in_off, rope, a.cache, dst, lane);
+  append_row(a.k, a.v, a.in_dtype, in_off, in_off, rope, a.cache, dst, lane);
 }
 
 }  // namespace ql

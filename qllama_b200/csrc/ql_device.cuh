@@ -14,7 +14,7 @@
 
 namespace ql {
 
-enum : int { kF32 = 0, kF16 = 1, kBF16 = 2, kQ8_0 = 3 };
+enum : int { kF32 = 0, kF16 = 1, kBF16 = 2, kQ8_0 = 3, kQ4_0 = 4 };
 
 // Bits of the context status word that kernels raise instead of trapping.
 enum : uint32_t {
@@ -454,6 +454,62 @@ __device__ __forceinline__ void q8_0_pair(float x0, float x1, int8_t& q0, int8_t
   q0 = static_cast<int8_t>(r0 == r0 ? static_cast<int>(r0) : 0);
   q1 = static_cast<int8_t>(r1 == r1 ? static_cast<int>(r1) : 0);
   scale = __float2half_rn(d);
+}
+
+// Q4_0 cache blocks: 32 values as 4-bit codes c with one f16 scale d, each standing for
+// d * (c - 8).  The rule is the 4-bit weights': with m the block's value of largest
+// magnitude (the first of equals), d = f16(m / -8) and c = clamp(round(x / d) + 8, 0, 15),
+// ties to even; d == 0 gives code 8.  A block that holds a NaN or an infinity, or whose d
+// leaves f16's range, gets a NaN scale.
+constexpr uint16_t kHalfNan = 0x7fff;
+
+// The scale of a block from its signed largest value; `finite` is false if any value is not.
+__device__ __forceinline__ uint16_t q4_scale(float m, bool finite) {
+  const __half d = __float2half_rn(m * -0.125f);
+  return !finite || __hisinf(d) ? kHalfNan : __half_as_ushort(d);
+}
+
+// round(x / d) without a division: x * (1 / d) rounded is at most one off next to a tie,
+// and the remainder x - k d, exact in f32 (d has 11 bits, k five, |remainder| <= |x|),
+// says where the nearest multiple lies.
+__device__ __forceinline__ uint32_t q4_code(float x, float d, float inv) {
+  float k = rintf(x * inv);
+  const float e = fmaf(-k, d, x), half = 0.5f * fabsf(d);
+  const float up = (e < 0.f) == (d < 0.f) ? 1.f : -1.f;  // the direction of the remainder
+  const bool odd = (static_cast<int>(k) & 1) != 0;
+  if (fabsf(e) > half || (fabsf(e) == half && odd)) k += up;
+  return static_cast<uint32_t>(static_cast<int>(fminf(fmaxf(k, -8.f), 7.f)) + 8);
+}
+
+// One block held as 16 pairs by 16 consecutive lanes (the quantiser of q8_0_pair's layout):
+// the two codes of this lane's pair in one byte (the first in the low four bits).
+__device__ __forceinline__ uint32_t q4_0_pair(float x0, float x1, uint16_t& scale) {
+  const float m = fabsf(x1) > fabsf(x0) ? x1 : x0;
+  const bool finite = fabsf(x0) < __int_as_float(0x7f800000) && fabsf(x1) < __int_as_float(0x7f800000);
+  float amax = fabsf(m);
+#pragma unroll
+  for (int o = 8; o > 0; o >>= 1) amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, o));
+  const int lane = threadIdx.x & 31, half = lane & 16;
+  const uint32_t hit = __ballot_sync(0xffffffffu, fabsf(m) == amax) >> half & 0xffffu;
+  const uint32_t bad = __ballot_sync(0xffffffffu, !finite) >> half & 0xffffu;
+  const float top = __shfl_sync(0xffffffffu, m, half + (hit ? __ffs(hit) - 1 : 0));
+  scale = q4_scale(top, bad == 0);
+  const float d = __half2float(__ushort_as_half(scale));
+  if (bad || scale == kHalfNan || d == 0.f) return 0x88u;
+  const float inv = 1.f / d;
+  return q4_code(x0, d, inv) | q4_code(x1, d, inv) << 4;
+}
+
+// Byte of a Q4_0 cache row (head_dim / 2 bytes, NB = head_dim / 32 blocks) that holds the
+// codes of dims d, d + 1 (d even).  The order is the one in which the decode kernel's
+// tensor-core fragments take them, so that a lane's codes of a row are one load: of a K row
+// lane t of four takes dims 32 b + 8 t .. + 7 of every block b, of a V row lane g of eight
+// dims 32 b + 4 g .. + 3.
+__device__ __forceinline__ int q4_k_byte(int d, int nb) {
+  return (d & 31) / 8 * 4 * nb + d / 32 * 4 + (d & 7) / 2;
+}
+__device__ __forceinline__ int q4_v_byte(int d, int nb) {
+  return (d & 31) / 4 * 2 * nb + d / 32 * 2 + (d & 3) / 2;
 }
 
 }  // namespace ql

@@ -7,6 +7,7 @@
 #include <stdint.h>
 
 #include <atomic>
+#include <vector>
 
 struct ql_ctx {
   int device = 0;
@@ -16,8 +17,11 @@ struct ql_ctx {
   uint32_t* status = nullptr;  // device word raised by kernels
   void* ws = nullptr;          // workspace (staging, split partials, scratch)
   size_t ws_bytes = 0;
+  bool ws_captured = false;     // a captured graph uses the workspace
   int32_t* counters = nullptr;  // split-merge arrival counters, kept at zero
   size_t counters_n = 0;
+  bool counters_captured = false;  // a captured graph uses them
+  std::vector<void*> retired;   // outgrown workspaces and counters of captured graphs
   cudaEvent_t order[2] = {nullptr, nullptr};  // of ql_ctx_wait_stream and ql_ctx_join_stream
 };
 

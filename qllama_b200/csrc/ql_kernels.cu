@@ -34,16 +34,6 @@ namespace {
 
 constexpr float kLog2e = 1.4426950408889634f;
 
-__device__ __forceinline__ float cache_value(const CacheView& c, const void* base,
-                                             const uint16_t* scale, int64_t row, int d) {
-  const size_t e = static_cast<size_t>(row) * c.hd + d;
-  if (c.dtype == kQ8_0) {
-    float s = __half2float(__ushort_as_half(scale[static_cast<size_t>(row) * (c.hd / 32) + d / 32]));
-    return s * static_cast<float>(static_cast<const int8_t*>(base)[e]);
-  }
-  return load_elem(base, e, c.dtype);
-}
-
 }  // namespace
 
 // ---------------------------------------------------------------- append --
@@ -64,7 +54,7 @@ __global__ void __launch_bounds__(128) append_kernel(const __grid_constant__ App
 }
 
 cudaError_t launch_append(const AppendArgs& a, cudaStream_t s) {
-  const bool tokens = a.cache.dtype != kQ8_0 && (a.cache.hd == 64 || a.cache.hd == 128);
+  const bool tokens = a.cache.dtype <= kBF16 && (a.cache.hd == 64 || a.cache.hd == 128);
   const int warps = a.batch * a.new_len * (tokens ? 1 : a.cache.hkv);
   if (warps == 0) return cudaSuccess;
   const int blocks = (warps + 3) / 4;
@@ -112,6 +102,14 @@ cudaError_t launch_table_patch(const TablePatch& p, cudaStream_t s) {
 }
 
 // --------------------------------------------------------------- generic --
+namespace {
+
+__device__ __forceinline__ int sel_place(const int32_t* sel, int j) {
+  return sel[j / kTile] * kTile + j % kTile;
+}
+
+}  // namespace
+
 // One CTA per (query head, query token).  Bit-level restatement of the
 // reference's per-head loop (layers.rs:434-445) on the GPU.
 __global__ void __launch_bounds__(256) generic_kernel(const __grid_constant__ AttnArgs a,
@@ -122,7 +120,11 @@ __global__ void __launch_bounds__(256) generic_kernel(const __grid_constant__ At
   const int hd = a.cache.hd;
   const int kvh = h / a.group;
   const int qpos = a.seqs.start[b] + t;
-  const int L = qpos + 1;
+  // Key j of the row: position j, or, over selected blocks, place j % 64 of the list's block
+  // j / 64.  The newest block is always the list's last, so it alone ends early.
+  const int32_t* sel = a.sel ? a.sel + (static_cast<size_t>(job) * a.cache.hkv + kvh) * a.sel_max
+                             : nullptr;
+  const int L = sel ? sel_keys(qpos, a.sel_max) : qpos + 1;
   const int seq = a.seqs.seq[b];
   extern __shared__ float sh[];  // q [hd], reduction [32]
   float* q = sh;
@@ -144,7 +146,7 @@ __global__ void __launch_bounds__(256) generic_kernel(const __grid_constant__ At
   float mx = -CUDART_INF_F;
   for (int j = threadIdx.x; j < L; j += blockDim.x) {
     bool ok;
-    const int64_t row = cache_row(a.cache, seq, j, kvh, a.status, ok);
+    const int64_t row = cache_row(a.cache, seq, sel ? sel_place(sel, j) : j, kvh, a.status, ok);
     float acc = 0.f;
     for (int d = 0; d < hd; ++d)
       acc = __fadd_rn(acc, __fmul_rn(q[d], ok ? cache_value(a.cache, a.cache.k, a.cache.k_scale,
@@ -189,7 +191,7 @@ __global__ void __launch_bounds__(256) generic_kernel(const __grid_constant__ At
     float acc = 0.f;
     for (int j = 0; j < L; ++j) {
       bool ok;
-      const int64_t row = cache_row(a.cache, seq, j, kvh, nullptr, ok);
+      const int64_t row = cache_row(a.cache, seq, sel ? sel_place(sel, j) : j, kvh, nullptr, ok);
       const float vv = ok ? cache_value(a.cache, a.cache.v, a.cache.v_scale, row, d) : 0.f;
       acc = __fadd_rn(acc, __fmul_rn(sc[j], vv));
     }

@@ -54,9 +54,10 @@ struct SeqTable {
 
 // Geometry and storage of one layer of the paged KV cache.
 struct CacheView {
-  void* k;               // K values: [pages][hkv][page][hd] (int8 for Q8_0)
+  void* k;               // K values: [pages][hkv][page][hd] (int8 for Q8_0; Q4_0: hd/2 bytes a
+                         // row, in q4_k_byte's and q4_v_byte's order)
   void* v;               // V values, same geometry
-  uint16_t* k_scale;     // Q8_0 only: [pages][hkv][page][hd/32] f16 bits
+  uint16_t* k_scale;     // Q8_0 and Q4_0: [pages][hkv][page][hd/32] f16 bits
   uint16_t* v_scale;
   const int32_t* block_table;  // [max_batch][pages_per_seq]
   int32_t pages_per_seq;
@@ -64,8 +65,17 @@ struct CacheView {
   int32_t page;          // positions per page
   int32_t hkv;
   int32_t hd;
-  int32_t dtype;         // kF32 / kF16 / kBF16 / kQ8_0
+  int32_t dtype;         // kF32 / kF16 / kBF16 / kQ8_0 / kQ4_0
 };
+
+// Blocks in the list of a token at position qpos, and the keys in them: all of the newest
+// block's up to qpos, and whole blocks before it.
+__host__ __device__ constexpr int sel_blocks(int qpos, int sel_max) {
+  return qpos / kTile + 1 < sel_max ? qpos / kTile + 1 : sel_max;
+}
+__host__ __device__ constexpr int sel_keys(int qpos, int sel_max) {
+  return (sel_blocks(qpos, sel_max) - 1) * kTile + qpos % kTile + 1;
+}
 
 // Appends new K (rotated unless rope == nullptr) and V rows into the cache.
 struct AppendArgs {
@@ -110,6 +120,10 @@ struct AttnArgs {
   int32_t out_vec;   // `out` (and every peer output) is 16-byte aligned
   int32_t wide;      // split-KV kernel: the variant whose consumer groups share a split
   int32_t cluster;   // split-KV kernel: CTAs per cluster along the splits (0/1: none)
+  // attention over selected blocks of kTile positions: [jobs][hkv][sel_max] block ids in
+  // ascending order (sel_blocks of them live), or nullptr
+  const int32_t* sel;
+  int32_t sel_max;
   PeerOut peer;      // split-KV kernel: head-sharded output exchange
   uint32_t* status;
   SeqTable seqs;
@@ -143,6 +157,71 @@ struct PrefillArgs {
   __half* v_copy;
   int8_t* tile_exp;
   int32_t kv_rows;     // keys per (sequence, KV head) in the copies, a multiple of 128
+};
+
+// Rows of several sequences, packed one after the other: sequence b's are the tokens
+// first[b] .. first[b + 1].
+struct RaggedTable {
+  int32_t seq[kMaxBatch];
+  int32_t start[kMaxBatch];      // position of the sequence's first row
+  int32_t first[kMaxBatch + 1];  // its first token; first[batch] is their number
+};
+
+// Appends the rows of several sequences (K rotated), and rotates their queries.
+struct RaggedAppendArgs {
+  const void* q;  // [tokens][hq][hd] or nullptr
+  const void* k;  // [tokens][hkv][hd]
+  const void* v;
+  void* q_out;    // [tokens][hq][hd]
+  int64_t q_stride, k_stride, v_stride;  // elements from token to token
+  int32_t in_dtype;
+  int32_t q_out_dtype;
+  int32_t hq;
+  int32_t batch;
+  const double2* rope;  // [max_seq][hd/2] (cos, sin)
+  CacheView cache;
+  uint32_t* status;
+  RaggedTable rows;
+};
+
+// Rows of several sequences out of the cache.
+struct RaggedReadArgs {
+  void* k_out;  // [tokens][hkv][hd]
+  void* v_out;
+  int32_t out_dtype;
+  int32_t batch;
+  CacheView cache;
+  uint32_t* status;
+  RaggedTable rows;
+};
+
+// The least and largest key of each channel over whole blocks of kTile positions, by
+// physical page: [pages][page / kTile][hkv][2][hd] of f16 (f16 caches) or bf16 bits.
+struct BoundsArgs {
+  uint16_t* bounds;
+  CacheView cache;
+  int32_t batch;
+  uint32_t* status;
+  RaggedTable blocks;  // start: first block to summarise; first: prefix sums of their numbers
+};
+
+// Chooses each (token, KV head)'s blocks: the first `first`, the last `last` and the ones of
+// the largest scores, `take` in all.
+struct SelectArgs {
+  const void* q;   // rotated queries [batch, new_len, hq, hd]
+  int32_t in_dtype;
+  int32_t hq;
+  int32_t group;
+  int32_t batch;
+  int32_t new_len;
+  int32_t take, first, last;
+  int32_t max_blocks;   // row length of `score`
+  double* score;        // scratch [jobs][hkv][max_blocks]
+  const uint16_t* bounds;
+  int32_t* sel;         // [jobs][hkv][take], ascending, then -1
+  CacheView cache;
+  uint32_t* status;
+  SeqTable seqs;
 };
 
 struct GatherArgs {
@@ -198,6 +277,10 @@ cudaError_t launch_peer_push(const void* src, int64_t rows, int row_bytes, int h
 cudaError_t launch_rank_to_head_major(const void* src, void* dst, int nranks, int64_t rows,
                                       int row_bytes, cudaStream_t s);
 cudaError_t launch_gather(const GatherArgs& a, cudaStream_t s);
+cudaError_t launch_ragged_append(const RaggedAppendArgs& a, cudaStream_t s);
+cudaError_t launch_ragged_read(const RaggedReadArgs& a, cudaStream_t s);
+cudaError_t launch_bounds(const BoundsArgs& a, cudaStream_t s);
+cudaError_t launch_select(const SelectArgs& a, cudaStream_t s);
 // Writes the entries of `p` into the device block table, in stream order, as
 // an ordinary launch: a kernel queued after it sees the entries once its
 // stream dependency is met.  A split-KV launch that follows must not use

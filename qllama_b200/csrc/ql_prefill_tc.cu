@@ -755,22 +755,22 @@ __global__ void __launch_bounds__(128) prefill_prologue_kernel(const __grid_cons
 }
 
 // ------------------------------------------------- f16 copy of the keys --
-// bf16 and Q8_0 caches: one CTA per (128-key tile, K or V, KV head,
+// bf16, Q8_0 and Q4_0 caches: one CTA per (128-key tile, K or V, KV head,
 // sequence) copies the keys the call sees into the dense f16 scratch, two
-// threads per key row (each HD/2 values: bf16 as stored, Q8_0 dequantised
-// exactly in f32, int8 times its block's f16 scale).  The tile is divided by
+// threads per key row (each HD/2 values: bf16 as stored, Q8_0 and
+// Q4_0 dequantised exactly in f32, the integer times its block's f16 scale).  The tile is divided by
 // 2^e, e = f16_range_exp of its largest magnitude (0 for ordinary data;
 // otherwise the power of two that puts the tile into [2^14, 2^15)), and e goes
 // to tile_exp for the attention kernel to fold back.  bf16 values convert
 // exactly at that scale, apart from magnitudes under 2^(e-24); dequantised
-// Q8_0 values (up to 19 significant bits) round to f16's 11.  Keys past the
+// Q8_0 and Q4_0 values (up to 19 and 15 significant bits) round to f16's 11.  Keys past the
 // sequence's end (and rows of unallocated pages) are zeros.  Converting once
 // here, instead of in every attention CTA that reads the tile, costs one read
 // and one write of the keys (a few per cent of a long prefill) and keeps the
 // attention kernel's pipeline that of an f16 cache.
 template <int HD, int DT>
 __global__ void __launch_bounds__(256) tiles_to_f16_kernel(const __grid_constant__ PrefillArgs a) {
-  static_assert(DT == kBF16 || DT == kQ8_0, "bf16 or Q8_0 storage");
+  static_assert(DT == kBF16 || DT == kQ8_0 || DT == kQ4_0, "bf16, Q8_0 or Q4_0 storage");
   constexpr int kVals = HD / 2;    // values per thread
   constexpr int kPer = kVals / 8;  // 8-value groups per thread
   const int tile = blockIdx.x, kind = blockIdx.y & 1, kvh = blockIdx.y >> 1, b = blockIdx.z;
@@ -803,6 +803,18 @@ __global__ void __launch_bounds__(256) tiles_to_f16_kernel(const __grid_constant
         v[8 * g + 2 * k] = __uint_as_float(in[k] << 16);
         v[8 * g + 2 * k + 1] = __uint_as_float(in[k] & 0xffff0000u);
       }
+    }
+  } else if constexpr (DT == kQ4_0) {
+    constexpr int kNb = HD / 32;
+    const uint8_t* src = static_cast<const uint8_t*>(kind ? a.cache.v : a.cache.k) + row * (HD / 2);
+    const uint16_t* sc = (kind ? a.cache.v_scale : a.cache.k_scale) + row * kNb;
+#pragma unroll
+    for (int i = 0; i < kVals; i += 2) {
+      const int d = part * kVals + i;
+      const uint32_t w = src[kind ? q4_v_byte(d, kNb) : q4_k_byte(d, kNb)];
+      const float f = __half2float(__ushort_as_half(sc[d / 32]));
+      v[i] = f * static_cast<float>(static_cast<int>(w & 15u) - 8);
+      v[i + 1] = f * static_cast<float>(static_cast<int>(w >> 4) - 8);
     }
   } else {
     const uint4* src = reinterpret_cast<const uint4*>(
@@ -855,8 +867,7 @@ __global__ void __launch_bounds__(256) tiles_to_f16_kernel(const __grid_constant
 }
 
 bool prefill_tc_supported(int hd, int dtype, int new_len) {
-  return (hd == 64 || hd == 128) && (dtype == kF16 || dtype == kBF16 || dtype == kQ8_0) &&
-         new_len >= 64;
+  return (hd == 64 || hd == 128) && dtype != kF32 && new_len >= 64;
 }
 
 size_t prefill_q_rows(int new_len) { return static_cast<size_t>((new_len + kBM - 1) / kBM) * kBM; }
@@ -914,9 +925,9 @@ cudaError_t launch_prefill_tc(const PrefillArgs& a, const AppendArgs& ap, const 
   // append and the rotation as two ordinary launches (measured a few per cent
   // faster on 4 x 8192 tokens, where their traffic, not their latency, counts).
   const long long ctas = static_cast<long long>((a.new_len + kBM - 1) / kBM) * a.hq * a.batch;
-  // (append_token writes f32/f16/bf16 rows; a Q8_0 cache appends through
+  // (append_token writes f32/f16/bf16 rows; a Q8_0 or Q4_0 cache appends through
   // append_kernel, which quantises its blocks)
-  const bool fused = ctas < 8LL * a.num_sms && a.cache.dtype != kQ8_0;
+  const bool fused = ctas < 8LL * a.num_sms && a.cache.dtype <= kBF16;
   PrefillArgs qa = a;
   AppendArgs none = ap;
   none.new_len = 0;
@@ -936,7 +947,7 @@ cudaError_t launch_prefill_tc(const PrefillArgs& a, const AppendArgs& ap, const 
   cfg.numAttrs = fused ? 1 : 0;
   cudaError_t e = cudaLaunchKernelEx(&cfg, prefill_prologue_kernel, qa, fused ? ap : none);
   if (e != cudaSuccess) return e;
-  const bool bf = a.cache.dtype == kBF16 || a.cache.dtype == kQ8_0;  // reads the f16 copy
+  const bool bf = a.cache.dtype != kF16;  // reads the f16 copy
   if (bf) {  // the keys as f16 tiles, after the rows this call appends
     cudaLaunchConfig_t cc = {};
     cc.gridDim = dim3(static_cast<unsigned>(a.kv_rows / kBN), 2u * a.cache.hkv,
@@ -945,13 +956,15 @@ cudaError_t launch_prefill_tc(const PrefillArgs& a, const AppendArgs& ap, const 
     cc.stream = s;
     cc.attrs = attr;
     cc.numAttrs = 1;
-    const bool q8 = a.cache.dtype == kQ8_0;
+    const int dt = a.cache.dtype;
     if (a.cache.hd == 64)
-      e = q8 ? cudaLaunchKernelEx(&cc, tiles_to_f16_kernel<64, kQ8_0>, a)
-             : cudaLaunchKernelEx(&cc, tiles_to_f16_kernel<64, kBF16>, a);
+      e = dt == kQ8_0   ? cudaLaunchKernelEx(&cc, tiles_to_f16_kernel<64, kQ8_0>, a)
+          : dt == kQ4_0 ? cudaLaunchKernelEx(&cc, tiles_to_f16_kernel<64, kQ4_0>, a)
+                        : cudaLaunchKernelEx(&cc, tiles_to_f16_kernel<64, kBF16>, a);
     else
-      e = q8 ? cudaLaunchKernelEx(&cc, tiles_to_f16_kernel<128, kQ8_0>, a)
-             : cudaLaunchKernelEx(&cc, tiles_to_f16_kernel<128, kBF16>, a);
+      e = dt == kQ8_0   ? cudaLaunchKernelEx(&cc, tiles_to_f16_kernel<128, kQ8_0>, a)
+          : dt == kQ4_0 ? cudaLaunchKernelEx(&cc, tiles_to_f16_kernel<128, kQ4_0>, a)
+                        : cudaLaunchKernelEx(&cc, tiles_to_f16_kernel<128, kBF16>, a);
     if (e != cudaSuccess) return e;
   }
   if (a.cache.hd == 64)

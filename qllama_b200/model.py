@@ -58,6 +58,11 @@ class NormArgs(ctypes.Structure):
                 ("out", ctypes.c_void_p), ("out_scale", ctypes.c_void_p)]
 
 
+class SparseArgs(ctypes.Structure):
+    _fields_ = [("blocks", ctypes.c_int32), ("first", ctypes.c_int32),
+                ("last", ctypes.c_int32), ("selected", ctypes.c_void_p)]
+
+
 class LinearArgs(ctypes.Structure):
     _fields_ = [("rows", ctypes.c_int32), ("in_dtype", ctypes.c_int32),
                 ("out_dtype", ctypes.c_int32), ("x_stride", ctypes.c_int64),
@@ -93,6 +98,7 @@ def bind(L: ctypes.CDLL) -> None:
                             vp]
     L.ql_qkv_rope_append.argtypes = [vp, vp, ctypes.c_void_p, vp, i32, vp, vp]
     L.ql_attn_forward_appended.argtypes = [vp, vp, ctypes.c_void_p]
+    L.ql_attn_forward_sparse.argtypes = [vp, vp, ctypes.c_void_p, ctypes.POINTER(SparseArgs)]
     L.ql_llama_generate.argtypes = [vp, vp, i32, i32p, i32, i32, i32,
                                     ctypes.POINTER(SamplerConfig),
                                     ctypes.POINTER(ctypes.c_double), i32p, i32p]
@@ -236,27 +242,79 @@ def qkv_rope_append(kv, layer: int, x, wqkv_t, start_pos, num_heads: int, num_kv
     return q_rot
 
 
+def _appended_args(kv, layer, q_rot, start_pos, num_heads, num_kv_heads, head_dim, rope_theta,
+                   seq_ids, out, out_dtype):
+    """(AttnArgs, out, keep-alive) of attention over rows that are in the cache."""
+    qb = _qb()
+    if q_rot.dim() < 3:
+        raise _invalid(f"q_rot must be [batch, new_len, heads, head_dim], got {tuple(q_rot.shape)}")
+    batch, new_len = int(q_rot.shape[0]), int(q_rot.shape[1])
+    if q_rot.numel() != batch * new_len * num_heads * head_dim or not q_rot.is_contiguous():
+        raise _invalid(f"q_rot must be contiguous [batch, new_len, {num_heads}, {head_dim}], got "
+                       f"{tuple(q_rot.shape)}")
+    if out is not None:
+        t = out.dtype
+    else:
+        t = _named_type(out_dtype or "f32")
+    out = _output(kv.ctx, out, (batch, new_len, num_heads * head_dim), t, "out")
+    if np.ndim(start_pos) and len(start_pos) != batch or \
+            seq_ids is not None and len(seq_ids) != batch:
+        raise _invalid(f"one position and one sequence for each of {batch} rows of q_rot")
+    starts = (ctypes.c_int64 * batch)(*([start_pos] * batch if np.ndim(start_pos) == 0
+                                        else start_pos))
+    seqs = (ctypes.c_int32 * batch)(*(range(batch) if seq_ids is None else seq_ids))
+    dev = kv.ctx.device
+    args = qb.AttnArgs(layer, batch, new_len, seqs, starts, num_heads, num_kv_heads, head_dim,
+                       rope_theta, _float_code(q_rot, "q_rot"), _float_code(out, "out"),
+                       qb.MEM_DEVICE, _on(dev, q_rot, "q_rot"), None, None, _on(dev, out, "out"))
+    return args, out
+
+
 def attention_forward_appended(kv, layer: int, q_rot, start_pos, num_heads: int,
                                num_kv_heads: int, head_dim: int, rope_theta: float,
-                               seq_ids=None, out_dtype: str = "f32"):
-    """ql_attn_forward_appended over the rows qkv_rope_append wrote."""
+                               seq_ids=None, out_dtype: str | None = None, out=None):
+    """ql_attn_forward_appended over the rows that qkv_rope_append or KvCache.append
+    wrote: q_rot [batch, new_len, heads, head_dim] f32, f16 or bf16; returns
+    [batch, new_len, heads * head_dim] (`out`, or a new tensor of out_dtype, default f32)."""
+    L = _L or _start()
+    args, out = _appended_args(kv, layer, q_rot, start_pos, num_heads, num_kv_heads, head_dim,
+                               rope_theta, seq_ids, out, out_dtype)
+    side = _fork(kv.ctx)
+    rc = L.ql_attn_forward_appended(kv.ctx._h, kv._h, ctypes.byref(args))
+    if rc:
+        _raise(rc)
+    if side is not None:
+        _join(kv.ctx, side)
+    return out
+
+
+def attention_forward_sparse(kv, layer: int, q_rot, start_pos, num_heads: int,
+                             num_kv_heads: int, head_dim: int, blocks: int, first: int = 1,
+                             last: int = 1, seq_ids=None, out_dtype: str | None = None, out=None,
+                             selected=None):
+    """attention_forward_appended over `blocks` blocks of 64 positions for each token and
+    KV head: the first `first`, the newest `last` and those whose keys can score highest
+    (ql_attn_forward_sparse).  Returns (out, selected): selected, int32
+    [batch, new_len, num_kv_heads, blocks] or None, receives the blocks' numbers in
+    ascending order, -1 behind them."""
     import torch
 
-    qb = _qb()
-    batch, new_len = int(q_rot.shape[0]), int(q_rot.shape[1])
-    out = torch.empty(batch, new_len, num_heads * head_dim,
-                      dtype={"f32": torch.float32, "f16": torch.float16,
-                             "bf16": torch.bfloat16}[out_dtype], device=q_rot.device)
-    starts = np.atleast_1d(np.asarray(start_pos, dtype=np.int64))
-    if starts.size == 1 and batch > 1:
-        starts = np.repeat(starts, batch)
-    seqs = np.arange(batch, dtype=np.int32) if seq_ids is None else np.asarray(seq_ids, np.int32)
-    args = qb.AttnArgs(layer, batch, new_len, seqs.ctypes.data_as(ctypes.POINTER(ctypes.c_int32)),
-                       starts.ctypes.data_as(ctypes.POINTER(ctypes.c_int64)), num_heads,
-                       num_kv_heads, head_dim, rope_theta, qb.F32, qb.DTYPES[out_dtype],
-                       qb.MEM_DEVICE, q_rot.data_ptr(), None, None, out.data_ptr())
-    qb._check(qb.load().ql_attn_forward_appended(kv.ctx._h, kv._h, ctypes.byref(args)))
-    return out
+    L = _L or _start()
+    args, out = _appended_args(kv, layer, q_rot, start_pos, num_heads, num_kv_heads, head_dim,
+                               1.0, seq_ids, out, out_dtype)
+    sp = None
+    if selected is not None:
+        _output(kv.ctx, selected, (args.batch, args.new_len, num_kv_heads, blocks), torch.int32,
+                "selected")
+        sp = _on(kv.ctx.device, selected, "selected")
+    sparse = SparseArgs(blocks, first, last, sp)
+    side = _fork(kv.ctx)
+    rc = L.ql_attn_forward_sparse(kv.ctx._h, kv._h, ctypes.byref(args), ctypes.byref(sparse))
+    if rc:
+        _raise(rc)
+    if side is not None:
+        _join(kv.ctx, side)
+    return out, selected
 
 
 # ------------------------------------ 4-bit decode step and drafted tokens --
