@@ -59,10 +59,7 @@ int cuda_fail(cudaError_t e, const char* what) {
 
 size_t elem_bytes(int dt) { return dt == QL_F32 ? 4 : (dt == QL_Q8_0 ? 1 : 2); }
 
-// Bytes of `n` values in a cache's value plane (a whole number of rows).
-size_t plane_bytes(int dt, size_t n) { return dt == QL_Q4_0 ? n / 2 : n * elem_bytes(dt); }
-
-// Storage types whose blocks of 32 values have their scales in a plane of their own.
+// Storage types of blocks of 32 values.
 bool block_dtype(int dt) { return dt == QL_Q8_0 || dt == QL_Q4_0; }
 
 bool valid_io_dtype(int dt) { return dt == QL_F32 || dt == QL_F16 || dt == QL_BF16; }
@@ -112,8 +109,8 @@ struct ql_kv {
   ql_ctx* ctx = nullptr;
   ql_kv_config cfg{};
   int pages_per_seq = 0;
-  std::vector<void*> k, v;             // per layer
-  std::vector<uint16_t*> ks, vs;       // per layer, Q8_0 and Q4_0 scales
+  std::vector<void*> k, v;             // per layer (Q4_0: all in k)
+  std::vector<uint16_t*> ks, vs;       // per layer, Q8_0 scales
   std::vector<CUtensorMap> kmap, vmap;  // per layer, split-KV kernel descriptors
   bool have_maps = false;
   int32_t* d_table = nullptr;          // [max_batch][pages_per_seq]
@@ -203,8 +200,8 @@ ql::CacheView view_of(const ql_kv* kv, int layer) {
   ql::CacheView c;
   c.k = kv->k[layer];
   c.v = kv->v[layer];
-  c.k_scale = block_dtype(kv->cfg.dtype) ? kv->ks[layer] : nullptr;
-  c.v_scale = block_dtype(kv->cfg.dtype) ? kv->vs[layer] : nullptr;
+  c.k_scale = kv->cfg.dtype == QL_Q8_0 ? kv->ks[layer] : nullptr;
+  c.v_scale = kv->cfg.dtype == QL_Q8_0 ? kv->vs[layer] : nullptr;
   c.block_table = kv->d_table;
   c.pages_per_seq = kv->pages_per_seq;
   c.num_pages = kv->cfg.num_pages;
@@ -675,7 +672,9 @@ int ql_kv_create(ql_ctx* c, const ql_kv_config* cfg_in, ql_kv** out) {
   if (cfg.num_pages == 0) cfg.num_pages = cfg.max_batch * std::max(1, kv->pages_per_seq);
   kv->cfg = cfg;
   const size_t rows = static_cast<size_t>(cfg.num_pages) * cfg.num_kv_heads * cfg.page_size;
-  const size_t bytes = plane_bytes(cfg.dtype, rows * cfg.head_dim);
+  const bool q4 = cfg.dtype == QL_Q4_0;  // K, V and the scales in one plane
+  const size_t bytes = q4 ? rows / ql::kTile * ql::Q4Record{cfg.head_dim}.bytes()
+                          : rows * cfg.head_dim * elem_bytes(cfg.dtype);
   auto cleanup = [&](int code) {
     ql_kv_destroy(kv);
     return code;
@@ -683,13 +682,13 @@ int ql_kv_create(ql_ctx* c, const ql_kv_config* cfg_in, ql_kv** out) {
   for (int l = 0; l < cfg.num_layers; ++l) {
     void *kp = nullptr, *vp = nullptr;
     cudaError_t e = cudaMalloc(&kp, std::max<size_t>(bytes, 256));
-    if (e == cudaSuccess) e = cudaMalloc(&vp, std::max<size_t>(bytes, 256));
+    if (e == cudaSuccess && !q4) e = cudaMalloc(&vp, std::max<size_t>(bytes, 256));
     if (e == cudaSuccess) e = cudaMemset(kp, 0, std::max<size_t>(bytes, 256));
-    if (e == cudaSuccess) e = cudaMemset(vp, 0, std::max<size_t>(bytes, 256));
+    if (e == cudaSuccess && !q4) e = cudaMemset(vp, 0, std::max<size_t>(bytes, 256));
     kv->k.push_back(kp);
     kv->v.push_back(vp);
     if (e != cudaSuccess) return cleanup(cuda_fail(e, "allocate KV pool"));
-    if (block_dtype(cfg.dtype)) {
+    if (cfg.dtype == QL_Q8_0) {
       const size_t sb = std::max<size_t>(rows * (cfg.head_dim / 32) * 2, 256);
       uint16_t *a = nullptr, *b = nullptr;
       e = cudaMalloc(&a, sb);
@@ -698,7 +697,7 @@ int ql_kv_create(ql_ctx* c, const ql_kv_config* cfg_in, ql_kv** out) {
       if (e == cudaSuccess) e = cudaMemset(b, 0, sb);
       kv->ks.push_back(a);
       kv->vs.push_back(b);
-      if (e != cudaSuccess) return cleanup(cuda_fail(e, "allocate block scales"));
+      if (e != cudaSuccess) return cleanup(cuda_fail(e, "allocate Q8_0 scales"));
     }
   }
   kv->table.assign(static_cast<size_t>(cfg.max_batch) * std::max(1, kv->pages_per_seq), -1);
@@ -1264,6 +1263,23 @@ static int attn_forward_impl(ql_ctx* c, ql_kv* kv, const ql_attn_args* a,
   }
   // the lists' rows: as the caller asked for them, or as long as they can get
   const int sel_max = !sparse ? 0 : sparse->selected ? sparse->blocks : max_tiles;
+  // a few tokens over a Q4_0 cache: every job's tiles in one list
+  const bool q4_decode = kv->cfg.dtype == QL_Q4_0 && !tc_prefill &&
+                         ql::attn4_supported(hd, kv->cfg.page_size);
+  ql::Attn4Args a4{};
+  size_t a4_cta = 0, a4_warp = 0;
+  if (q4_decode) {
+    a4.units = sparse ? n * ((group + 7) / 8) : (n * group + 7) / 8;
+    int64_t total = 0;
+    for (int b = 0; b < a->batch; ++b) {
+      a4.first[b] = static_cast<int32_t>(total);
+      total += static_cast<int64_t>(row_tiles[b]) * hkv * a4.units;
+      if (total > (1 << 30))
+        return fail(QL_ERR_UNSUPPORTED, "more than %d tiles of keys in one call", 1 << 30);
+    }
+    a4.total = static_cast<int32_t>(total);
+    ql::attn4_plan(hd, c->num_sms, &a4, &a4_cta, &a4_warp);
+  }
   int tps = max_tiles, max_splits = 1;
   // Too few (token, KV head) jobs to fill half the SMs: the wide kernel, whose
   // consumer groups share each split's tiles, one CTA per SM (latency).
@@ -1333,9 +1349,12 @@ static int attn_forward_impl(ql_ctx* c, ql_kv* kv, const ql_attn_args* a,
   if (bf_copy) off += align256(2 * static_cast<size_t>(a->batch) * hkv * (kv_rows / 128));
   const int gjobs = std::min(jobs, 65535);
   const size_t o_gs = off;
-  if (!fast) off += align256(static_cast<size_t>(gjobs) * hq * max_len * sizeof(float));
+  const bool generic = !fast && !q4_decode && !tc_prefill;
+  if (generic) off += align256(static_cast<size_t>(gjobs) * hq * max_len * sizeof(float));
   const size_t o_gd = off;
-  if (!fast) off += align256(static_cast<size_t>(gjobs) * hq * max_len * sizeof(double));
+  if (generic) off += align256(static_cast<size_t>(gjobs) * hq * max_len * sizeof(double));
+  const size_t o_4c = off; off += align256(a4_cta);
+  const size_t o_4w = off; off += align256(a4_warp);
   const size_t o_sc = off;
   if (sparse) off += align256(static_cast<size_t>(jobs) * hkv * max_blocks * sizeof(double));
   const size_t o_sel = off;
@@ -1343,8 +1362,8 @@ static int attn_forward_impl(ql_ctx* c, ql_kv* kv, const ql_attn_args* a,
     off += align256(static_cast<size_t>(jobs) * hkv * sel_max * sizeof(int32_t));
   r = ensure_ws(c, off);
   if (r != QL_OK) return r;
-  if (fast && max_splits > 1) {
-    r = ensure_counters(c, static_cast<size_t>(jobs) * hkv);
+  if ((fast && max_splits > 1) || q4_decode) {
+    r = ensure_counters(c, static_cast<size_t>(q4_decode ? a->batch * a4.units : jobs) * hkv);
     if (r != QL_OK) return r;
   }
   char* w = static_cast<char*>(c->ws);
@@ -1491,7 +1510,30 @@ static int attn_forward_impl(ql_ctx* c, ql_kv* kv, const ql_attn_args* a,
     at.peer.total_ctas = max_splits * hkv * jobs;
     at.out_vec = 1;  // symmetric buffers are 256-byte aligned
   }
-  if (fast)
+  if (q4_decode) {
+    a4.q = q;
+    a4.in_dtype = a->in_dtype;
+    a4.q_vec = aligned_to(q, a->in_dtype == QL_F32 ? 16 : 8);
+    a4.out = out;
+    a4.out_dtype = a->out_dtype;
+    a4.out_vec = at.out_vec;
+    a4.rope = q_rope;
+    a4.rope_stride = q_rope_stride;
+    a4.cache = cv;
+    a4.hq = hq;
+    a4.group = group;
+    a4.batch = a->batch;
+    a4.new_len = n;
+    a4.scale = at.scale;
+    a4.sel = at.sel;
+    a4.sel_max = at.sel_max;
+    a4.cta_parts = reinterpret_cast<float*>(w + o_4c);
+    a4.warp_parts = reinterpret_cast<float*>(w + o_4w);
+    a4.counters = c->counters;
+    a4.status = c->status;
+    a4.seqs = st;
+    QL_CUDA(ql::launch_attn4(a4, c->stream), "launch Q4_0 attention");
+  } else if (fast)
     QL_CUDA(ql::launch_splitkv(at, &kv->kmap[layer], &kv->vmap[layer], jobs, c->stream,
                                /*pdl=*/!patched),
             "launch split-KV attention");

@@ -21,19 +21,34 @@ __device__ __forceinline__ int64_t cache_row(const CacheView& c, int seq, int po
   return (static_cast<int64_t>(page) * c.hkv + h) * c.page + pos % c.page;
 }
 
-// The f32 value of column d of a cache row; base and scale: the K or the V planes.
-__device__ __forceinline__ float cache_value(const CacheView& c, const void* base,
-                                             const uint16_t* scale, int64_t row, int d) {
+// Codes and scales of row `row` (cache_row) of a Q4_0 cache.
+__device__ __forceinline__ uint8_t* q4_codes(const CacheView& c, int64_t row, bool v) {
+  const Q4Record rec{c.hd};
+  return static_cast<uint8_t*>(c.k) + static_cast<size_t>(row / kTile) * rec.bytes() +
+         (v ? rec.v_codes() : 0) + static_cast<size_t>(row % kTile) * (c.hd / 2);
+}
+__device__ __forceinline__ uint16_t* q4_scales(const CacheView& c, int64_t row, bool v) {
+  const Q4Record rec{c.hd};
+  return reinterpret_cast<uint16_t*>(static_cast<uint8_t*>(c.k) +
+                                     static_cast<size_t>(row / kTile) * rec.bytes() +
+                                     (v ? rec.v_scales() : rec.k_scales())) +
+         static_cast<size_t>(row % kTile) * (c.hd / 32);
+}
+
+// The f32 value of column d of a cache row of K or V.
+__device__ __forceinline__ float cache_value(const CacheView& c, bool v, int64_t row, int d) {
+  if (c.dtype == kQ4_0) {
+    const int nb = c.hd / 32, byte = v ? q4_v_byte(d & ~1, nb) : q4_k_byte(d & ~1, nb);
+    const uint32_t w = q4_codes(c, row, v)[byte];
+    const float s = __half2float(__ushort_as_half(q4_scales(c, row, v)[d / 32]));
+    return s * static_cast<float>(static_cast<int>((d & 1 ? w >> 4 : w) & 15u) - 8);
+  }
+  const void* base = v ? c.v : c.k;
   const size_t e = static_cast<size_t>(row) * c.hd + d;
   if (c.dtype == kQ8_0) {
-    float s = __half2float(__ushort_as_half(scale[static_cast<size_t>(row) * (c.hd / 32) + d / 32]));
+    const float s = __half2float(__ushort_as_half(
+        (v ? c.v_scale : c.k_scale)[static_cast<size_t>(row) * (c.hd / 32) + d / 32]));
     return s * static_cast<float>(static_cast<const int8_t*>(base)[e]);
-  }
-  if (c.dtype == kQ4_0) {
-    const int nb = c.hd / 32, byte = base == c.v ? q4_v_byte(d & ~1, nb) : q4_k_byte(d & ~1, nb);
-    const uint32_t w = static_cast<const uint8_t*>(base)[static_cast<size_t>(row) * (c.hd / 2) + byte];
-    const float s = __half2float(__ushort_as_half(scale[static_cast<size_t>(row) * nb + d / 32]));
-    return s * static_cast<float>(static_cast<int>((d & 1 ? w >> 4 : w) & 15u) - 8);
   }
   return load_elem(base, e, c.dtype);
 }
@@ -98,13 +113,11 @@ __device__ __forceinline__ void append_row(const void* kin, const void* vin, int
       uint16_t sk, sv;
       const uint32_t bk = q4_0_pair(k0, k1, sk), bv = q4_0_pair(v0, v1, sv);
       if (valid) {
-        const size_t row = static_cast<size_t>(dst) * (hd / 2);
-        static_cast<uint8_t*>(c.k)[row + q4_k_byte(2 * p, hd / 32)] = static_cast<uint8_t>(bk);
-        static_cast<uint8_t*>(c.v)[row + q4_v_byte(2 * p, hd / 32)] = static_cast<uint8_t>(bv);
+        q4_codes(c, dst, false)[q4_k_byte(2 * p, hd / 32)] = static_cast<uint8_t>(bk);
+        q4_codes(c, dst, true)[q4_v_byte(2 * p, hd / 32)] = static_cast<uint8_t>(bv);
         if ((lane & 15) == 0) {
-          const size_t si = static_cast<size_t>(dst) * (hd / 32) + (2 * p) / 32;
-          c.k_scale[si] = sk;
-          c.v_scale[si] = sv;
+          q4_scales(c, dst, false)[(2 * p) / 32] = sk;
+          q4_scales(c, dst, true)[(2 * p) / 32] = sv;
         }
       }
     } else if (valid) {

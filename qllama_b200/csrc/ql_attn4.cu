@@ -1,0 +1,648 @@
+// ql_attn4.cu -- attention of a few query tokens over a Q4_0 cache for B200 (sm_100a).
+//
+// One KV head's 64 positions are one record of 72 hd bytes (Q4Record: codes of K and V, then
+// their scales), so a tile comes into shared memory as one bulk copy.  The work is the list of
+// all tiles of all jobs, a job being one (sequence, KV head, up to eight query rows: heads of
+// the group, of several tokens where they fit).  Every CTA takes an equal run of that list and
+// every warp of it an equal part, streaming its tiles through a ring of its own: no barrier
+// between warps until the run is done, whatever the sequences' lengths.  A job that lies inside
+// a warp's part is finished there; pieces of others are joined in the CTA, and across CTAs by
+// the last one to arrive.
+//
+// Per 16 positions, on the tensor cores (m16n8k16, positions and value columns as rows, query
+// rows as columns, so that no row of a fragment is idle):
+//   S = K q^T      A = the K codes, B = q
+//   O = V^T P      A = the V codes, B = P times the block's scale
+// A code c masked out of its word is the f16 number c 2^-24 (or, in the next nibble, c 2^-20):
+// f16's subnormals hold the codes exactly and the matrix instruction takes them as they are, so
+// that a fragment register costs one AND.  The powers of two are folded into q and the output;
+// the 8 that is subtracted from every code enters S as the accumulator's start (-8 sum q) and
+// leaves O with the product of P by a row of eights.  A K scale multiplies the block's partial
+// sums in f32, a V scale the probabilities in f16.
+//
+// Bound by HBM for long caches (2304 bytes of a head_dim 128 cache per 16 positions against
+// about 200 instructions of one warp).
+#include <math_constants.h>
+
+#include <algorithm>
+#include <atomic>
+
+#include "ql_append.cuh"
+#include "ql_device.cuh"
+#include "ql_internal.h"
+#include "ql_kernels.cuh"
+
+namespace ql {
+
+namespace {
+
+constexpr float kLog2e4 = 1.4426950408889634f;
+// A probability is 2^arg with arg at most kTop (less where scales reach 2): below f16's
+// overflow times a scale, and far above its subnormals.  The reference it is relative to moves
+// only when an arg exceeds that, by enough to leave kSlack free.
+constexpr float kTop = 14.f, kSlack = 4.f;
+
+template <int HD>
+struct Attn4Cfg {
+  static constexpr int kNb = HD / 32;
+  static constexpr int kWarps = 12;
+  static constexpr int kRecord = 72 * HD;
+  static constexpr int kStages = HD == 128 ? 2 : 4;
+  static constexpr int kRing = kStages * kRecord;  // of one warp
+  static constexpr int kPart = 8 * HD + 16;        // floats of a piece: rows, then (reference, sum)
+  static constexpr size_t kSmem = 128 + static_cast<size_t>(kWarps) * (kRing + kStages * 8) +
+                                  kWarps * 4 * 4 + 64;
+  static_assert(kPart * 4 <= kRing, "a warp's last piece takes its ring's place");
+};
+
+__device__ __forceinline__ void mma_f16(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2,
+                                        uint32_t a3, uint32_t b0, uint32_t b1) {
+  asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, "
+      "{%0,%1,%2,%3};"
+      : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+      : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
+
+// The transpose of an 8 x 8 matrix of f16 held as pairs along its rows.
+__device__ __forceinline__ uint32_t transpose8(uint32_t a) {
+  uint32_t d;
+  asm("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(d) : "r"(a));
+  return d;
+}
+
+__device__ __forceinline__ uint32_t halves(uint32_t a, uint32_t b, bool high) {
+  uint32_t d;  // the low (high) halves of a and b side by side
+  if (high)
+    asm("prmt.b32 %0, %1, %2, 0x7632;" : "=r"(d) : "r"(a), "r"(b));
+  else
+    asm("prmt.b32 %0, %1, %2, 0x5410;" : "=r"(d) : "r"(a), "r"(b));
+  return d;
+}
+
+__device__ __forceinline__ uint32_t mul2(uint32_t a, uint32_t b) {
+  const __half2 d = __hmul2(*reinterpret_cast<const __half2*>(&a), *reinterpret_cast<const __half2*>(&b));
+  return *reinterpret_cast<const uint32_t*>(&d);
+}
+
+__device__ __forceinline__ float ex2(float x) {  // 2^x; -inf -> +0
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+
+__device__ __forceinline__ float half_of(uint32_t w, bool high) {
+  return __half2float(__ushort_as_half(static_cast<uint16_t>(high ? w >> 16 : w & 0xffffu)));
+}
+
+// A job of the list: its sequence, KV head and query rows, and its tiles.
+struct Job {
+  int b, id, kvh, row0, rows;
+  int t0, tiles;  // its first place in the list of tiles, and their number
+};
+
+__device__ __forceinline__ Job job_at(const Attn4Args& a, int x) {
+  int lo = 0, hi = a.batch - 1;
+  while (lo < hi) {
+    const int mid = (lo + hi + 1) / 2;
+    if (a.first[mid] <= x) lo = mid;
+    else hi = mid - 1;
+  }
+  Job j;
+  j.b = lo;
+  const int end = a.seqs.start[lo] + a.new_len;
+  j.tiles = a.sel ? sel_blocks(end - 1, a.sel_max) : (end + kTile - 1) / kTile;
+  const int k = (x - a.first[lo]) / j.tiles;
+  j.t0 = a.first[lo] + k * j.tiles;
+  j.id = lo * a.cache.hkv * a.units + k;
+  j.kvh = k / a.units;
+  const int unit = k - j.kvh * a.units;
+  if (a.sel) {  // a list belongs to one token: chunks of its heads
+    const int per = (a.group + 7) / 8, t = unit / per, h0 = (unit - t * per) * 8;
+    j.row0 = t * a.group + h0;
+    j.rows = min(8, a.group - h0);
+  } else {
+    j.row0 = unit * 8;
+    j.rows = min(8, a.new_len * a.group - j.row0);
+  }
+  return j;
+}
+
+// The record that holds tile x of the list; -1 for a list's place behind its blocks.
+__device__ __forceinline__ int record_at(const Attn4Args& a, int x) {
+  const Job j = job_at(a, x);
+  const CacheView& c = a.cache;
+  int tile = x - j.t0;
+  if (a.sel) {
+    const int t = j.row0 / a.group;
+    if (tile >= sel_blocks(a.seqs.start[j.b] + t, a.sel_max)) return -1;
+    tile = a.sel[(static_cast<size_t>(j.b * a.new_len + t) * c.hkv + j.kvh) * a.sel_max + tile];
+  }
+  const int per = c.page / kTile;
+  int page = c.block_table[static_cast<size_t>(a.seqs.seq[j.b]) * c.pages_per_seq + tile / per];
+  if (page < 0 || page >= c.num_pages) {
+    atomicOr(a.status, kStatusBadPage);
+    page = 0;  // keep the pipeline consistent; the result is flagged
+  }
+  return (page * c.hkv + j.kvh) * per + tile % per;
+}
+
+// Element offset of query row `row` (token row / group, head row % group) in q and out.
+__device__ __forceinline__ size_t row_offset(const Attn4Args& a, const Job& j, int row, int hd) {
+  const int t = row / a.group, h = row - t * a.group;
+  return ((static_cast<size_t>(j.b) * a.new_len + t) * a.hq + j.kvh * a.group + h) * hd;
+}
+
+// Joins pieces of a job: part(i) for i < n gives one's floats.  Every thread of the CTA takes
+// columns; `emit` gets each (row, first column, four numerators, reference, sum).
+template <int HD, typename P, typename E>
+__device__ __forceinline__ void join_pieces(int n, int rows, int threads, P part, E emit) {
+  for (int c = threadIdx.x; c < rows * (HD / 4); c += threads) {
+    const int r = c / (HD / 4), d = c % (HD / 4) * 4;
+    float ref = -CUDART_INF_F, sum = 0.f;
+    float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
+    for (int i = 0; i < n; ++i) {
+      const float* p = part(i);
+      const float2 ml = *reinterpret_cast<const float2*>(p + 8 * HD + 2 * r);
+      const float4 v = *reinterpret_cast<const float4*>(p + r * HD + d);
+      const float top = fmaxf(ref, ml.x), base = top == -CUDART_INF_F ? 0.f : top;
+      const float w0 = exp2f(ref - base), w1 = exp2f(ml.x - base);
+      sum = sum * w0 + ml.y * w1;
+      acc.x = acc.x * w0 + v.x * w1;
+      acc.y = acc.y * w0 + v.y * w1;
+      acc.z = acc.z * w0 + v.z * w1;
+      acc.w = acc.w * w0 + v.w * w1;
+      ref = top;
+    }
+    emit(r, d, acc, ref, sum);
+  }
+}
+
+__device__ __forceinline__ float4 scaled(const float4& v, float f) {
+  return make_float4(v.x * f, v.y * f, v.z * f, v.w * f);
+}
+
+}  // namespace
+
+template <int HD>
+__global__ void __launch_bounds__(32 * Attn4Cfg<HD>::kWarps, 1)
+    attn4_kernel(const __grid_constant__ Attn4Args a) {
+  using C = Attn4Cfg<HD>;
+  constexpr int NB = C::kNb, W = C::kWarps, S = C::kStages;
+  constexpr Q4Record kRec{HD};
+  extern __shared__ uint8_t smem_raw[];
+  uint8_t* smem = reinterpret_cast<uint8_t*>(
+      (reinterpret_cast<uintptr_t>(smem_raw) + 127) & ~static_cast<uintptr_t>(127));
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int g = lane >> 2, tq = lane & 3;
+  uint8_t* ring = smem + warp * C::kRing;
+  uint64_t* full = reinterpret_cast<uint64_t*>(smem + W * C::kRing) + warp * S;
+  int* flag = reinterpret_cast<int*>(smem + W * C::kRing + W * S * 8);
+
+  const int c0 = blockIdx.x * a.per_cta, c1 = min(c0 + a.per_cta, a.total);
+  const int w0 = min(c0 + warp * a.per_warp, c1), w1 = min(w0 + a.per_warp, c1);
+  if (lane == 0) {
+    for (int s = 0; s < S; ++s) mbar_init(&full[s], 1);
+    fence_mbar_init();
+  }
+  __syncwarp();
+  griddep_wait();
+  griddep_launch_dependents();
+
+  // -------------------------------------------------------------- the ring --
+  // The lanes hold the records of 32 tiles at a time; lane 0 issues.
+  int lane_rec = 0;
+  auto issue = [&](int i) {
+    if ((i & 31) == 0) lane_rec = w0 + i + lane < w1 ? record_at(a, w0 + i + lane) : -1;
+    const int rec = __shfl_sync(0xffffffffu, lane_rec, i & 31);
+    if (lane != 0) return;
+    uint64_t* bar = &full[i % S];
+    if (rec < 0) {
+      mbar_arrive(bar);
+    } else {
+      mbar_arrive_expect_tx(bar, C::kRecord);
+      bulk_load(ring + (i % S) * C::kRecord,
+                static_cast<const uint8_t*>(a.cache.k) + static_cast<size_t>(rec) * kRec.bytes(),
+                C::kRecord, bar);
+    }
+  };
+  for (int i = 0; i < S && w0 + i < w1; ++i) issue(i);
+
+  uint32_t eights[NB];  // rows b, b + 4, ... of block b's matrix of eights
+#pragma unroll
+  for (int b = 0; b < NB; ++b) eights[b] = (g & 3) == b ? 0x00080008u : 0u;
+
+  bool alive = true;
+  int x = w0;
+  while (x < w1) {
+    const Job job = job_at(a, x);
+    const int seg1 = min(w1, job.t0 + job.tiles);
+    const int start = a.seqs.start[job.b];
+
+    // ------------------------------------------------------------- q --
+    // Lane (g, tq) holds dims 32 b + 8 tq .. + 7 of row g: the columns of B in the order in
+    // which the K words' nibbles come out (j and j + 4 together; odd ones, whose codes are
+    // 16 times as large, divided by 16).  Each row is scaled by a power of two to [2^14, 2^15).
+    uint32_t qh[NB][2][2], ql[NB][2][2];
+    float qo[NB][2], f[2];
+    bool has_lo;
+    {
+      float v[NB][8];
+      const bool live = g < job.rows;
+      const int row = job.row0 + (live ? g : 0), t = row / a.group;
+      const size_t off = row_offset(a, job, row, HD);
+      const double2* rope = a.rope + static_cast<size_t>(start + t) * a.rope_stride;
+      float mx = 0.f;
+#pragma unroll
+      for (int b = 0; b < NB; ++b) {
+        const int d = 32 * b + 8 * tq;
+        float lo4[4], hi4[4];
+        load_vec<4>(a.q, off + d, a.in_dtype, a.q_vec != 0, lo4);
+        load_vec<4>(a.q, off + d + 4, a.in_dtype, a.q_vec != 0, hi4);
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+          v[b][k] = live ? lo4[k] : 0.f;
+          v[b][k + 4] = live ? hi4[k] : 0.f;
+        }
+        if (a.rope_stride) {
+#pragma unroll
+          for (int k = 0; k < 8; k += 2)
+            rope_pair(v[b][k], v[b][k + 1], rope[(d + k) / 2], v[b][k], v[b][k + 1]);
+        }
+#pragma unroll
+        for (int k = 0; k < 8; ++k) mx = fmaxf(mx, fabsf(v[b][k]));
+      }
+      mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 1));
+      mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 2));
+      const uint32_t bits = __float_as_uint(mx);
+      int e = static_cast<int>(bits >> 23) - 127 - 14;
+      if (bits == 0 || bits >= 0x7f800000u) e = 0;
+      e = max(e, -100);
+      const float down = pow2f(-e);
+      float sums[NB];
+      bool lo_any = false;
+#pragma unroll
+      for (int b = 0; b < NB; ++b) {
+        float s = 0.f;
+#pragma unroll
+        for (int ks = 0; ks < 2; ++ks)
+#pragma unroll
+          for (int r = 0; r < 2; ++r) {
+            const float u = r ? down * 0.0625f : down;
+            const float y0 = v[b][2 * ks + r] * u, y1 = v[b][2 * ks + r + 4] * u;
+            float h0, l0, h1, l1;
+            split16<false>(y0, h0, l0);
+            split16<false>(y1, h1, l1);
+            qh[b][ks][r] = pack2<false>(h0, h1);
+            ql[b][ks][r] = pack2<false>(l0, l1);
+            lo_any |= (ql[b][ks][r] & 0x7fff7fffu) != 0;
+            s += (y0 + y1) * (r ? 16.f : 1.f);
+          }
+        s += __shfl_xor_sync(0xffffffffu, s, 1);
+        s += __shfl_xor_sync(0xffffffffu, s, 2);
+        sums[b] = s * (-8.f / 16777216.f);
+      }
+      has_lo = __any_sync(0xffffffffu, lo_any);
+      const float fr = a.scale * kLog2e4 * 16777216.f * pow2f(e);
+#pragma unroll
+      for (int k = 0; k < 2; ++k) {
+        f[k] = __shfl_sync(0xffffffffu, fr, (2 * tq + k) * 4);
+#pragma unroll
+        for (int b = 0; b < NB; ++b) qo[b][k] = __shfl_sync(0xffffffffu, sums[b], (2 * tq + k) * 4);
+      }
+    }
+    // The keys that this lane's two rows see: positions below lim (of a selection: places of
+    // its list), and those that all rows of the job see.
+    int lim[2], all;
+    if (a.sel) {
+      all = sel_keys(start + job.row0 / a.group, a.sel_max);
+      lim[0] = lim[1] = all;
+    } else {
+      all = start + job.row0 / a.group + 1;
+#pragma unroll
+      for (int k = 0; k < 2; ++k)
+        lim[k] = start + (job.row0 + min(2 * tq + k, job.rows - 1)) / a.group + 1;
+    }
+    const int most = a.sel ? all : start + (job.row0 + job.rows - 1) / a.group + 1;
+
+    float o[NB][2][4], off[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+    for (int b = 0; b < NB; ++b)
+#pragma unroll
+      for (int u = 0; u < 2; ++u) o[b][u][0] = o[b][u][1] = o[b][u][2] = o[b][u][3] = 0.f;
+    float ref[2] = {0.f, 0.f}, l[2] = {0.f, 0.f}, top = kTop;
+    bool fresh = true;
+    uint32_t nans = 0;  // of row 2 tq + k: bit 4 k + b, that it sees a value of block b that is NaN
+
+    // --------------------------------------------------------- the tiles --
+    for (; x < seg1; ++x) {
+      const int i = x - w0;
+      if (alive) alive = !__any_sync(0xffffffffu, !mbar_wait(&full[i % S], (i / S) & 1, a.status));
+      const uint8_t* st = ring + (i % S) * C::kRecord;
+      const int p0 = (x - job.t0) * kTile;
+      const bool tail = p0 + kTile > all;
+      const int slices = alive ? min(4, (most - p0 + 15) / 16) : 0;
+      for (int s = 0; s < slices; ++s) {
+        // ---- S = K q^T
+        uint32_t kw[2][NB], kd[2][(NB + 1) / 2];
+#pragma unroll
+        for (int r = 0; r < 2; ++r) {
+          const int row = 16 * s + g + 8 * r;
+          const uint8_t* kp = st + row * (HD / 2) + tq * (4 * NB);
+          const uint8_t* sp = st + kRec.k_scales() + row * (2 * NB);
+          if constexpr (NB == 4) {
+            const uint4 w = *reinterpret_cast<const uint4*>(kp);
+            kw[r][0] = w.x, kw[r][1] = w.y, kw[r][2] = w.z, kw[r][3] = w.w;
+            const uint2 d = *reinterpret_cast<const uint2*>(sp);
+            kd[r][0] = d.x, kd[r][1] = d.y;
+          } else {
+            const uint2 w = *reinterpret_cast<const uint2*>(kp);
+            kw[r][0] = w.x, kw[r][1] = w.y;
+            kd[r][0] = *reinterpret_cast<const uint32_t*>(sp);
+          }
+        }
+        float y[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+        for (int b = 0; b < NB; ++b) {
+          float c[4] = {qo[b][0], qo[b][1], qo[b][0], qo[b][1]};
+#pragma unroll
+          for (int ks = 0; ks < 2; ++ks) {
+            const uint32_t u0 = kw[0][b] >> (8 * ks), u1 = kw[1][b] >> (8 * ks);
+            const uint32_t a0 = u0 & 0x000f000fu, a1 = u1 & 0x000f000fu;
+            const uint32_t a2 = u0 & 0x00f000f0u, a3 = u1 & 0x00f000f0u;
+            mma_f16(c, a0, a1, a2, a3, qh[b][ks][0], qh[b][ks][1]);
+            if (has_lo) mma_f16(c, a0, a1, a2, a3, ql[b][ks][0], ql[b][ks][1]);
+          }
+          const float d0 = half_of(kd[0][b / 2], b & 1), d1 = half_of(kd[1][b / 2], b & 1);
+          y[0] = fmaf(c[0], d0, y[0]);
+          y[1] = fmaf(c[1], d0, y[1]);
+          y[2] = fmaf(c[2], d1, y[2]);
+          y[3] = fmaf(c[3], d1, y[3]);
+        }
+        // ---- V's scales of positions 2 tq, 2 tq + 1 and those plus 8
+        uint32_t vd[4][(NB + 1) / 2], any_d = 0;
+#pragma unroll
+        for (int r = 0; r < 4; ++r) {
+          const int row = 16 * s + 2 * tq + (r & 1) + 8 * (r >> 1);
+          const uint8_t* sp = st + kRec.v_scales() + row * (2 * NB);
+          if constexpr (NB == 4) {
+            const uint2 d = *reinterpret_cast<const uint2*>(sp);
+            vd[r][0] = d.x, vd[r][1] = d.y;
+            any_d |= d.x | d.y;
+          } else {
+            vd[r][0] = *reinterpret_cast<const uint32_t*>(sp);
+            any_d |= vd[r][0];
+          }
+        }
+        // ---- softmax: columns 2 tq, 2 tq + 1 of positions g and g + 8
+        if (tail) {
+#pragma unroll
+          for (int k = 0; k < 4; ++k)
+            if (p0 + 16 * s + g + 8 * (k >> 1) >= lim[k & 1]) y[k] = -CUDART_INF_F;
+        }
+        float arg[4];
+#pragma unroll
+        for (int k = 0; k < 4; ++k) arg[k] = fmaf(y[k], f[k & 1], -ref[k & 1]);
+        const bool over = fmaxf(fmaxf(arg[0], arg[1]), fmaxf(arg[2], arg[3])) > top;
+        // (a scale of 2 or more has the exponent's top bit)
+        if (__any_sync(0xffffffffu, over || (any_d & 0x40004000u)) || fresh) {
+          // NaN scales are taken out here and their columns remembered: in the product of P by
+          // a row of eights one would spread to the other blocks, and behind the end of the
+          // sequence, where P is 0, to everything.
+          uint32_t big = 0;  // the largest scale's bits
+#pragma unroll
+          for (int r = 0; r < 4; ++r)
+#pragma unroll
+            for (int b = 0; b < NB; ++b) {
+              const uint32_t h = (b & 1 ? vd[r][b / 2] >> 16 : vd[r][b / 2]) & 0x7fffu;
+              const bool bad = h > 0x7c00u;
+              if (!bad) big = max(big, h);
+              const uint32_t lanes = __ballot_sync(0xffffffffu, bad) & 15u;  // of tq 0..3
+              if (lanes) {
+                if (bad) vd[r][b / 2] &= b & 1 ? 0xffffu : 0xffff0000u;
+                const int place = p0 + 16 * s + 2 * (__ffs(lanes) - 1) + (r & 1) + 8 * (r >> 1);
+#pragma unroll
+                for (int k = 0; k < 2; ++k) nans |= (place < lim[k] ? 1u : 0u) << (4 * k + b);
+              }
+            }
+          big = __reduce_max_sync(0xffffffffu, big);
+          const float cap = fminf(top, kTop - fmaxf(0.f, static_cast<float>(static_cast<int>(big >> 10) - 15)));
+#pragma unroll
+          for (int k = 0; k < 2; ++k) {
+            float m = fmaxf(y[k] * f[k], y[k + 2] * f[k]);  // NaN does not count
+            m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, 4));
+            m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, 8));
+            m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, 16));
+            float next = ref[k] + (top - cap);
+            if ((fresh || m - next > cap) && m > -CUDART_INF_F) next = m - (cap - kSlack);
+            const float corr = fresh ? 0.f : ex2(ref[k] - next);
+            ref[k] = next;
+            l[k] *= corr;
+            off[k] *= corr;
+            off[k + 2] *= corr;
+#pragma unroll
+            for (int b = 0; b < NB; ++b)
+#pragma unroll
+              for (int u = 0; u < 2; ++u) {
+                o[b][u][k] *= corr;
+                o[b][u][k + 2] *= corr;
+              }
+          }
+          top = cap;
+          fresh = false;
+#pragma unroll
+          for (int k = 0; k < 4; ++k) arg[k] = fmaf(y[k], f[k & 1], -ref[k & 1]);
+        }
+        float p[4];
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+          p[k] = ex2(arg[k]);
+          l[k & 1] += p[k];
+        }
+        const uint32_t pt0 = transpose8(pack2<false>(p[0], p[1]));
+        const uint32_t pt1 = transpose8(pack2<false>(p[2], p[3]));
+        // ---- O += V^T (P d)
+        uint32_t vw[4][NB / 2];
+#pragma unroll
+        for (int r = 0; r < 4; ++r) {
+          const int row = 16 * s + 2 * tq + (r & 1) + 8 * (r >> 1);
+          const uint8_t* vp = st + kRec.v_codes() + row * (HD / 2) + g * (2 * NB);
+          if constexpr (NB == 4) {
+            const uint2 w = *reinterpret_cast<const uint2*>(vp);
+            vw[r][0] = w.x, vw[r][1] = w.y;
+          } else {
+            vw[r][0] = *reinterpret_cast<const uint32_t*>(vp);
+          }
+        }
+#pragma unroll
+        for (int b = 0; b < NB; ++b) {
+          const uint32_t b0 = mul2(pt0, halves(vd[0][b / 2], vd[1][b / 2], b & 1));
+          const uint32_t b1 = mul2(pt1, halves(vd[2][b / 2], vd[3][b / 2], b & 1));
+          mma_f16(off, eights[b], eights[b], eights[b], eights[b], b0, b1);
+          const uint32_t t0 = halves(vw[0][b / 2], vw[1][b / 2], b & 1);
+          const uint32_t t1 = halves(vw[2][b / 2], vw[3][b / 2], b & 1);
+#pragma unroll
+          for (int u = 0; u < 2; ++u) {
+            const uint32_t u0 = t0 >> (8 * u), u1 = t1 >> (8 * u);
+            mma_f16(o[b][u], u0 & 0x000f000fu, u0 & 0x00f000f0u, u1 & 0x000f000fu,
+                    u1 & 0x00f000f0u, b0, b1);
+          }
+        }
+      }
+      __syncwarp();  // the stage is free
+      if (alive && x + S < w1) issue(i + S);
+    }
+
+    // ------------------------------------------------- the end of a piece --
+#pragma unroll
+    for (int k = 0; k < 2; ++k) {
+      l[k] += __shfl_xor_sync(0xffffffffu, l[k], 4);
+      l[k] += __shfl_xor_sync(0xffffffffu, l[k], 8);
+      l[k] += __shfl_xor_sync(0xffffffffu, l[k], 16);
+    }
+    const bool whole = job.t0 >= w0 && job.t0 + job.tiles <= w1;
+    // A piece that ends the warp's part goes into its ring; an earlier one (of a job that
+    // other warps began) into memory: the CTA's own piece of it if no other warp here has one.
+    float* part = seg1 == w1 ? reinterpret_cast<float*>(ring)
+                  : warp == 0 ? a.cta_parts + static_cast<size_t>(2 * blockIdx.x) * C::kPart
+                              : a.warp_parts + static_cast<size_t>(blockIdx.x * W + warp) * C::kPart;
+#pragma unroll
+    for (int k = 0; k < 2; ++k) {
+      const int r = 2 * tq + k;
+      const bool live = r < job.rows;
+      const float f24 = 16777216.f * (whole ? 1.f / l[k] : 1.f);
+      const size_t base = whole && live ? row_offset(a, job, job.row0 + r, HD) : 0;
+      float eight[NB];
+#pragma unroll
+      for (int b = 0; b < NB; ++b) eight[b] = __shfl_sync(0xffffffffu, off[k], b * 4 + tq);
+      if (!live) continue;
+#pragma unroll
+      for (int b = 0; b < NB; ++b) {
+        float4 v = make_float4((o[b][0][k] - eight[b]) * f24,
+                               (o[b][0][k + 2] * 0.0625f - eight[b]) * f24,
+                               (o[b][1][k] - eight[b]) * f24,
+                               (o[b][1][k + 2] * 0.0625f - eight[b]) * f24);
+        if (nans >> (4 * k + b) & 1u) v.x = v.y = v.z = v.w = CUDART_NAN_F;
+        const int d = 32 * b + 4 * g;
+        if (whole)
+          store4(a.out, base + d, a.out_dtype, v, a.out_vec != 0);
+        else
+          *reinterpret_cast<float4*>(part + r * HD + d) = v;
+      }
+      if (!whole && g == 0) *reinterpret_cast<float2*>(part + 8 * HD + 2 * r) = make_float2(ref[k], l[k]);
+    }
+  }
+
+  // ------------------------------------------------------------ joining --
+  // (__syncthreads orders the pieces in memory as well, inside the CTA)
+  __syncthreads();
+  constexpr int T = 32 * W;
+  auto warp_begin = [&](int i) { return min(c0 + i * a.per_warp, c1); };
+  auto joined = [&](const Job& j, int i0, bool in_place) {
+    const int t1 = j.t0 + j.tiles, end = min(t1, c1);
+    const bool inside = j.t0 >= c0 && t1 <= c1;
+    const int slot = j.t0 > c0 ? 1 : 0;
+    float* mine = a.cta_parts + static_cast<size_t>(2 * blockIdx.x + slot) * C::kPart;
+    if (!in_place) {
+      int n = 1;
+      while (i0 + n < W && warp_begin(i0 + n) < end) ++n;
+      join_pieces<HD>(
+          n, j.rows, T,
+          [&](int k) -> const float* {
+            const int i = i0 + k;
+            return min(t1, c1) >= warp_begin(i + 1)
+                       ? reinterpret_cast<const float*>(smem + i * C::kRing)
+                       : a.warp_parts + static_cast<size_t>(blockIdx.x * W + i) * C::kPart;
+          },
+          [&](int r, int d, const float4& v, float ref, float sum) {
+            if (inside) {
+              store4(a.out, row_offset(a, j, j.row0 + r, HD) + d, a.out_dtype, scaled(v, 1.f / sum),
+                     a.out_vec != 0);
+            } else {
+              *reinterpret_cast<float4*>(mine + r * HD + d) = v;
+              if (d == 0) *reinterpret_cast<float2*>(mine + 8 * HD + 2 * r) = make_float2(ref, sum);
+            }
+          });
+    }
+    if (inside) return;
+    // The barrier orders every thread's part of the piece before thread 0's count, whose
+    // release makes it visible; the last CTA's acquire sees the others'.
+    const int first = j.t0 / a.per_cta, last = (t1 - 1) / a.per_cta;
+    __syncthreads();
+    if (threadIdx.x == 0) flag[0] = atom_add_acq_rel_gpu(&a.counters[j.id], 1) == last - first;
+    __syncthreads();
+    const bool merge = flag[0] != 0;
+    __syncthreads();
+    if (!merge) return;
+    if (threadIdx.x == 0) a.counters[j.id] = 0;
+    join_pieces<HD>(
+        last - first + 1, j.rows, T,
+        [&](int k) -> const float* {
+          const int c = first + k;
+          return a.cta_parts + static_cast<size_t>(2 * c + (j.t0 > c * a.per_cta ? 1 : 0)) * C::kPart;
+        },
+        [&](int r, int d, const float4& v, float, float sum) {
+          store4(a.out, row_offset(a, j, j.row0 + r, HD) + d, a.out_dtype, scaled(v, 1.f / sum),
+                 a.out_vec != 0);
+        });
+  };
+  for (int i = 0; i < W; ++i) {
+    const int b0 = warp_begin(i), b1 = warp_begin(i + 1);
+    if (b0 >= b1) break;
+    const Job lastj = job_at(a, b1 - 1);
+    const int t1 = lastj.t0 + lastj.tiles;
+    if (i == 0 && lastj.t0 > b0) {  // the first job of the run, if another CTA began it
+      const Job firstj = job_at(a, b0);
+      if (firstj.t0 < c0) joined(firstj, 0, true);
+    }
+    const bool whole = lastj.t0 >= b0 && t1 <= b1;
+    if (!whole && (lastj.t0 >= b0 || i == 0)) joined(lastj, i, false);
+  }
+}
+
+bool attn4_supported(int hd, int page) { return (hd == 64 || hd == 128) && page % kTile == 0; }
+
+namespace {
+
+template <int HD>
+cudaError_t launch_attn4_t(const Attn4Args& a, cudaStream_t s) {
+  using C = Attn4Cfg<HD>;
+  static std::atomic<uint64_t> done{0};
+  cudaError_t e = ql_once_per_device(done, [] {
+    return cudaFuncSetAttribute(attn4_kernel<HD>, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                static_cast<int>(C::kSmem));
+  });
+  if (e != cudaSuccess) return e;
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3((a.total + a.per_cta - 1) / a.per_cta);
+  cfg.blockDim = dim3(32 * C::kWarps);
+  cfg.dynamicSmemBytes = C::kSmem;
+  cfg.stream = s;
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = 1;
+  return cudaLaunchKernelEx(&cfg, attn4_kernel<HD>, a);
+}
+
+}  // namespace
+
+// The split of `total` tiles: CTAs, and tiles of a CTA and of a warp.  At least kMinTiles tiles
+// a CTA: fewer leave more pieces to join across CTAs than their streaming saves.
+void attn4_plan(int hd, int num_sms, Attn4Args* a, size_t* cta_bytes, size_t* warp_bytes) {
+  constexpr int kMinTiles = 4;
+  const int warps = hd == 128 ? Attn4Cfg<128>::kWarps : Attn4Cfg<64>::kWarps;
+  const int part = hd == 128 ? Attn4Cfg<128>::kPart : Attn4Cfg<64>::kPart;
+  const int want = std::max(1, std::min(num_sms, (a->total + kMinTiles - 1) / kMinTiles));
+  a->per_cta = (a->total + want - 1) / want;
+  a->per_warp = (a->per_cta + warps - 1) / warps;
+  const size_t ctas = (a->total + a->per_cta - 1) / a->per_cta;
+  *cta_bytes = ctas * 2 * part * sizeof(float);
+  *warp_bytes = ctas * warps * part * sizeof(float);
+}
+
+cudaError_t launch_attn4(const Attn4Args& a, cudaStream_t s) {
+  return a.cache.hd == 128 ? launch_attn4_t<128>(a, s) : launch_attn4_t<64>(a, s);
+}
+
+}  // namespace ql

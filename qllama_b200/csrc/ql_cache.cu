@@ -81,8 +81,8 @@ __global__ void __launch_bounds__(128) ragged_read_kernel(const __grid_constant_
                                 a.status, ok);
   const size_t o = static_cast<size_t>(warp) * c.hd;
   for (int d = lane; d < c.hd; d += 32) {
-    store_elem(a.k_out, o + d, a.out_dtype, ok ? cache_value(c, c.k, c.k_scale, row, d) : 0.f);
-    store_elem(a.v_out, o + d, a.out_dtype, ok ? cache_value(c, c.v, c.v_scale, row, d) : 0.f);
+    store_elem(a.k_out, o + d, a.out_dtype, ok ? cache_value(c, false, row, d) : 0.f);
+    store_elem(a.v_out, o + d, a.out_dtype, ok ? cache_value(c, true, row, d) : 0.f);
   }
 }
 
@@ -119,7 +119,7 @@ __global__ void __launch_bounds__(128) bounds_kernel(const __grid_constant__ Bou
     float lo = CUDART_INF_F, hi = -CUDART_INF_F;
     bool nan = false;
     for (int i = 0; i < kTile; ++i) {
-      const float x = cache_value(c, c.k, c.k_scale, row + i, d);
+      const float x = cache_value(c, false, row + i, d);
       nan |= x != x;
       lo = fminf(lo, x);
       hi = fmaxf(hi, x);

@@ -500,15 +500,15 @@ __device__ __forceinline__ uint32_t q4_0_pair(float x0, float x1, uint16_t& scal
   return q4_code(x0, d, inv) | q4_code(x1, d, inv) << 4;
 }
 
-// Byte of a Q4_0 cache row (head_dim / 2 bytes, NB = head_dim / 32 blocks) that holds the
-// codes of dims d, d + 1 (d even).  The order is the one in which the decode kernel's
-// tensor-core fragments take them, so that a lane's codes of a row are one load: of a K row
-// lane t of four takes dims 32 b + 8 t .. + 7 of every block b, of a V row lane g of eight
-// dims 32 b + 4 g .. + 3.
-__device__ __forceinline__ int q4_k_byte(int d, int nb) {
+// Byte of a row's codes (head_dim / 2 bytes, NB = head_dim / 32 blocks) that holds those of
+// dims d, d + 1 (d even).  The order is the one in which the decode kernel's tensor-core
+// fragments take them, so that a lane's codes of a row are one load: of a K row lane t of
+// four takes dims 32 b + 8 t .. + 7 of every block b, of a V row lane g of eight dims
+// 32 b + 4 g .. + 3.
+__host__ __device__ constexpr int q4_k_byte(int d, int nb) {
   return (d & 31) / 8 * 4 * nb + d / 32 * 4 + (d & 7) / 2;
 }
-__device__ __forceinline__ int q4_v_byte(int d, int nb) {
+__host__ __device__ constexpr int q4_v_byte(int d, int nb) {
   return (d & 31) / 4 * 2 * nb + d / 32 * 2 + (d & 3) / 2;
 }
 

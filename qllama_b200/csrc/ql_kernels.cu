@@ -78,8 +78,8 @@ __global__ void __launch_bounds__(128) gather_kernel(const __grid_constant__ Gat
   const int64_t row = cache_row(a.cache, a.seq, a.positions[i], h, nullptr, ok);
   const size_t o = (static_cast<size_t>(i) * hkv + h) * hd;
   for (int d = lane; d < hd; d += 32) {
-    a.k_out[o + d] = ok ? cache_value(a.cache, a.cache.k, a.cache.k_scale, row, d) : 0.f;
-    a.v_out[o + d] = ok ? cache_value(a.cache, a.cache.v, a.cache.v_scale, row, d) : 0.f;
+    a.k_out[o + d] = ok ? cache_value(a.cache, false, row, d) : 0.f;
+    a.v_out[o + d] = ok ? cache_value(a.cache, true, row, d) : 0.f;
   }
 }
 
@@ -149,8 +149,7 @@ __global__ void __launch_bounds__(256) generic_kernel(const __grid_constant__ At
     const int64_t row = cache_row(a.cache, seq, sel ? sel_place(sel, j) : j, kvh, a.status, ok);
     float acc = 0.f;
     for (int d = 0; d < hd; ++d)
-      acc = __fadd_rn(acc, __fmul_rn(q[d], ok ? cache_value(a.cache, a.cache.k, a.cache.k_scale,
-                                                               row, d)
+      acc = __fadd_rn(acc, __fmul_rn(q[d], ok ? cache_value(a.cache, false, row, d)
                                                : 0.f));
     acc = __fmul_rn(acc, a.scale);
     sc[j] = acc;
@@ -192,7 +191,7 @@ __global__ void __launch_bounds__(256) generic_kernel(const __grid_constant__ At
     for (int j = 0; j < L; ++j) {
       bool ok;
       const int64_t row = cache_row(a.cache, seq, sel ? sel_place(sel, j) : j, kvh, nullptr, ok);
-      const float vv = ok ? cache_value(a.cache, a.cache.v, a.cache.v_scale, row, d) : 0.f;
+      const float vv = ok ? cache_value(a.cache, true, row, d) : 0.f;
       acc = __fadd_rn(acc, __fmul_rn(sc[j], vv));
     }
     store_elem(a.out, (static_cast<size_t>(job) * a.hq + h) * hd + d, a.out_dtype, acc);

@@ -52,12 +52,23 @@ struct SeqTable {
   int32_t start[kMaxBatch];  // position of the first new token
 };
 
+// A Q4_0 cache keeps 64 positions of one KV head in one run of 72 hd bytes, so that a tile
+// with its scales is one bulk copy: the K codes [64][hd/2], the V codes [64][hd/2], the K
+// scales [64][hd/32] and the V scales, f16.
+struct Q4Record {
+  int hd;
+  __host__ __device__ constexpr size_t bytes() const { return 72 * static_cast<size_t>(hd); }
+  __host__ __device__ constexpr size_t v_codes() const { return 32 * static_cast<size_t>(hd); }
+  __host__ __device__ constexpr size_t k_scales() const { return 64 * static_cast<size_t>(hd); }
+  __host__ __device__ constexpr size_t v_scales() const { return 68 * static_cast<size_t>(hd); }
+};
+
 // Geometry and storage of one layer of the paged KV cache.
 struct CacheView {
-  void* k;               // K values: [pages][hkv][page][hd] (int8 for Q8_0; Q4_0: hd/2 bytes a
-                         // row, in q4_k_byte's and q4_v_byte's order)
-  void* v;               // V values, same geometry
-  uint16_t* k_scale;     // Q8_0 and Q4_0: [pages][hkv][page][hd/32] f16 bits
+  void* k;               // K values: [pages][hkv][page][hd] (int8 for Q8_0); Q4_0: the records
+                         // [pages][hkv][page/64] of Q4Record
+  void* v;               // V values, same geometry (Q4_0: null)
+  uint16_t* k_scale;     // Q8_0 only: [pages][hkv][page][hd/32] f16 bits
   uint16_t* v_scale;
   const int32_t* block_table;  // [max_batch][pages_per_seq]
   int32_t pages_per_seq;
@@ -127,6 +138,36 @@ struct AttnArgs {
   PeerOut peer;      // split-KV kernel: head-sharded output exchange
   uint32_t* status;
   SeqTable seqs;
+};
+
+// Attention of a few query tokens over a Q4_0 cache (ql_attn4.cu): jobs of up to eight query
+// rows (token, head of the group) of one KV head, their 64-position tiles in one list.
+struct Attn4Args {
+  const void* q;  // [batch, new_len, hq, hd]
+  int32_t in_dtype;
+  int32_t q_vec;  // q allows loads of four elements
+  void* out;      // [batch, new_len, hq*hd]
+  int32_t out_dtype;
+  int32_t out_vec;
+  const double2* rope;
+  int32_t rope_stride;  // as in AttnArgs; 0: q arrives rotated
+  CacheView cache;
+  int32_t hq;
+  int32_t group;
+  int32_t batch;
+  int32_t new_len;
+  int32_t units;        // jobs of one (sequence, KV head)
+  float scale;
+  const int32_t* sel;   // as in AttnArgs
+  int32_t sel_max;
+  int32_t total;        // tiles of all jobs
+  int32_t per_cta, per_warp;
+  float* cta_parts;     // [CTAs][2] pieces
+  float* warp_parts;    // [CTAs][warps] pieces
+  int32_t* counters;    // [jobs], zero between launches
+  uint32_t* status;
+  SeqTable seqs;
+  int32_t first[kMaxBatch];  // first tile of each sequence's jobs
 };
 
 // Multi-token causal attention on the tcgen05 tensor cores (f16 or bf16 cache, hd 64 or 128).
@@ -281,6 +322,11 @@ cudaError_t launch_ragged_append(const RaggedAppendArgs& a, cudaStream_t s);
 cudaError_t launch_ragged_read(const RaggedReadArgs& a, cudaStream_t s);
 cudaError_t launch_bounds(const BoundsArgs& a, cudaStream_t s);
 cudaError_t launch_select(const SelectArgs& a, cudaStream_t s);
+// Q4_0 decode: whether it applies, the split of a->total tiles (fills per_cta and per_warp,
+// reports the bytes of the pieces), and the launch.
+bool attn4_supported(int hd, int page);
+void attn4_plan(int hd, int num_sms, Attn4Args* a, size_t* cta_bytes, size_t* warp_bytes);
+cudaError_t launch_attn4(const Attn4Args& a, cudaStream_t s);
 // Writes the entries of `p` into the device block table, in stream order, as
 // an ordinary launch: a kernel queued after it sees the entries once its
 // stream dependency is met.  A split-KV launch that follows must not use

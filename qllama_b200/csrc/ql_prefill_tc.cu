@@ -806,8 +806,8 @@ __global__ void __launch_bounds__(256) tiles_to_f16_kernel(const __grid_constant
     }
   } else if constexpr (DT == kQ4_0) {
     constexpr int kNb = HD / 32;
-    const uint8_t* src = static_cast<const uint8_t*>(kind ? a.cache.v : a.cache.k) + row * (HD / 2);
-    const uint16_t* sc = (kind ? a.cache.v_scale : a.cache.k_scale) + row * kNb;
+    const uint8_t* src = q4_codes(a.cache, row, kind != 0);
+    const uint16_t* sc = q4_scales(a.cache, row, kind != 0);
 #pragma unroll
     for (int i = 0; i < kVals; i += 2) {
       const int d = part * kVals + i;
