@@ -21,26 +21,28 @@ __device__ __forceinline__ int64_t cache_row(const CacheView& c, int seq, int po
   return (static_cast<int64_t>(page) * c.hkv + h) * c.page + pos % c.page;
 }
 
-// Codes and scales of row `row` (cache_row) of a Q4_0 cache.
-__device__ __forceinline__ uint8_t* q4_codes(const CacheView& c, int64_t row, bool v) {
+// The byte with the codes of dims d, d + 1 (d even) of row `row` (cache_row) of a Q4_0 cache,
+// and the scale of its block b.
+__device__ __forceinline__ uint8_t* q4_code_at(const CacheView& c, int64_t row, int d, bool v) {
   const Q4Record rec{c.hd};
+  const int pos = static_cast<int>(row % kTile), nb = c.hd / 32;
   return static_cast<uint8_t*>(c.k) + static_cast<size_t>(row / kTile) * rec.bytes() +
-         (v ? rec.v_codes() : 0) + static_cast<size_t>(row % kTile) * (c.hd / 2);
+         (v ? rec.v_codes() + q4_v_byte(pos, d, nb) : q4_k_byte(pos, d, nb));
 }
-__device__ __forceinline__ uint16_t* q4_scales(const CacheView& c, int64_t row, bool v) {
+__device__ __forceinline__ uint16_t* q4_scale_at(const CacheView& c, int64_t row, int b, bool v) {
   const Q4Record rec{c.hd};
+  const int pos = static_cast<int>(row % kTile), nb = c.hd / 32;
   return reinterpret_cast<uint16_t*>(static_cast<uint8_t*>(c.k) +
                                      static_cast<size_t>(row / kTile) * rec.bytes() +
                                      (v ? rec.v_scales() : rec.k_scales())) +
-         static_cast<size_t>(row % kTile) * (c.hd / 32);
+         (v ? q4_v_scale(pos, b, nb) : q4_k_scale(pos, b, nb));
 }
 
 // The f32 value of column d of a cache row of K or V.
 __device__ __forceinline__ float cache_value(const CacheView& c, bool v, int64_t row, int d) {
   if (c.dtype == kQ4_0) {
-    const int nb = c.hd / 32, byte = v ? q4_v_byte(d & ~1, nb) : q4_k_byte(d & ~1, nb);
-    const uint32_t w = q4_codes(c, row, v)[byte];
-    const float s = __half2float(__ushort_as_half(q4_scales(c, row, v)[d / 32]));
+    const uint32_t w = *q4_code_at(c, row, d & ~1, v);
+    const float s = __half2float(__ushort_as_half(*q4_scale_at(c, row, d / 32, v)));
     return s * static_cast<float>(static_cast<int>((d & 1 ? w >> 4 : w) & 15u) - 8);
   }
   const void* base = v ? c.v : c.k;
@@ -113,11 +115,11 @@ __device__ __forceinline__ void append_row(const void* kin, const void* vin, int
       uint16_t sk, sv;
       const uint32_t bk = q4_0_pair(k0, k1, sk), bv = q4_0_pair(v0, v1, sv);
       if (valid) {
-        q4_codes(c, dst, false)[q4_k_byte(2 * p, hd / 32)] = static_cast<uint8_t>(bk);
-        q4_codes(c, dst, true)[q4_v_byte(2 * p, hd / 32)] = static_cast<uint8_t>(bv);
+        *q4_code_at(c, dst, 2 * p, false) = static_cast<uint8_t>(bk);
+        *q4_code_at(c, dst, 2 * p, true) = static_cast<uint8_t>(bv);
         if ((lane & 15) == 0) {
-          q4_scales(c, dst, false)[(2 * p) / 32] = sk;
-          q4_scales(c, dst, true)[(2 * p) / 32] = sv;
+          *q4_scale_at(c, dst, 2 * p / 32, false) = sk;
+          *q4_scale_at(c, dst, 2 * p / 32, true) = sv;
         }
       }
     } else if (valid) {

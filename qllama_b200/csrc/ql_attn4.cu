@@ -16,8 +16,8 @@
 // A code c masked out of its word is the f16 number c 2^-24 (or, in the next nibble, c 2^-20):
 // f16's subnormals hold the codes exactly and the matrix instruction takes them as they are, so
 // that a fragment register costs one AND.  The powers of two are folded into q and the output;
-// the 8 that is subtracted from every code enters S as the accumulator's start (-8 sum q) and
-// leaves O with the product of P by a row of eights.  A K scale multiplies the block's partial
+// the 8 that is subtracted from every code enters S as -8 sum q and leaves
+// O with the product of P by a row of eights.  A K scale multiplies the block's partial
 // sums in f32, a V scale the probabilities in f16.
 //
 // Bound by HBM for long caches (2304 bytes of a head_dim 128 cache per 16 positions against
@@ -55,6 +55,15 @@ struct Attn4Cfg {
   static_assert(kPart * 4 <= kRing, "a warp's last piece takes its ring's place");
 };
 
+// D = A B
+__device__ __forceinline__ void mma_f16_first(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2,
+                                              uint32_t a3, uint32_t b0, uint32_t b1) {
+  asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, "
+      "{%10,%10,%10,%10};"
+      : "=f"(d[0]), "=f"(d[1]), "=f"(d[2]), "=f"(d[3])
+      : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1), "f"(0.f));
+}
+
 __device__ __forceinline__ void mma_f16(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2,
                                         uint32_t a3, uint32_t b0, uint32_t b1) {
   asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, "
@@ -70,15 +79,6 @@ __device__ __forceinline__ uint32_t transpose8(uint32_t a) {
   return d;
 }
 
-__device__ __forceinline__ uint32_t halves(uint32_t a, uint32_t b, bool high) {
-  uint32_t d;  // the low (high) halves of a and b side by side
-  if (high)
-    asm("prmt.b32 %0, %1, %2, 0x7632;" : "=r"(d) : "r"(a), "r"(b));
-  else
-    asm("prmt.b32 %0, %1, %2, 0x5410;" : "=r"(d) : "r"(a), "r"(b));
-  return d;
-}
-
 __device__ __forceinline__ uint32_t mul2(uint32_t a, uint32_t b) {
   const __half2 d = __hmul2(*reinterpret_cast<const __half2*>(&a), *reinterpret_cast<const __half2*>(&b));
   return *reinterpret_cast<const uint32_t*>(&d);
@@ -90,8 +90,9 @@ __device__ __forceinline__ float ex2(float x) {  // 2^x; -inf -> +0
   return y;
 }
 
-__device__ __forceinline__ float half_of(uint32_t w, bool high) {
-  return __half2float(__ushort_as_half(static_cast<uint16_t>(high ? w >> 16 : w & 0xffffu)));
+__device__ __forceinline__ float half_of(const uint32_t& w, bool high) {
+  const __half2 h = *reinterpret_cast<const __half2*>(&w);
+  return high ? __high2float(h) : __low2float(h);
 }
 
 // A job of the list: its sequence, KV head and query rows, and its tiles.
@@ -183,7 +184,10 @@ __device__ __forceinline__ float4 scaled(const float4& v, float f) {
 
 }  // namespace
 
-template <int HD>
+// LO: q enters as two f16 parts; not needed where it is of 16 bits and arrives rotated (scaled
+// by its power of two, f16 holds all of a value's bits that are above 2^-38 of the row's
+// largest).
+template <int HD, bool LO>
 __global__ void __launch_bounds__(32 * Attn4Cfg<HD>::kWarps, 1)
     attn4_kernel(const __grid_constant__ Attn4Args a) {
   using C = Attn4Cfg<HD>;
@@ -244,7 +248,6 @@ __global__ void __launch_bounds__(32 * Attn4Cfg<HD>::kWarps, 1)
     // 16 times as large, divided by 16).  Each row is scaled by a power of two to [2^14, 2^15).
     uint32_t qh[NB][2][2], ql[NB][2][2];
     float qo[NB][2], f[2];
-    bool has_lo;
     {
       float v[NB][8];
       const bool live = g < job.rows;
@@ -279,7 +282,6 @@ __global__ void __launch_bounds__(32 * Attn4Cfg<HD>::kWarps, 1)
       e = max(e, -100);
       const float down = pow2f(-e);
       float sums[NB];
-      bool lo_any = false;
 #pragma unroll
       for (int b = 0; b < NB; ++b) {
         float s = 0.f;
@@ -294,14 +296,12 @@ __global__ void __launch_bounds__(32 * Attn4Cfg<HD>::kWarps, 1)
             split16<false>(y1, h1, l1);
             qh[b][ks][r] = pack2<false>(h0, h1);
             ql[b][ks][r] = pack2<false>(l0, l1);
-            lo_any |= (ql[b][ks][r] & 0x7fff7fffu) != 0;
-            s += (y0 + y1) * (r ? 16.f : 1.f);
+            s += (LO ? y0 + y1 : h0 + h1) * (r ? 16.f : 1.f);
           }
         s += __shfl_xor_sync(0xffffffffu, s, 1);
         s += __shfl_xor_sync(0xffffffffu, s, 2);
         sums[b] = s * (-8.f / 16777216.f);
       }
-      has_lo = __any_sync(0xffffffffu, lo_any);
       const float fr = a.scale * kLog2e4 * 16777216.f * pow2f(e);
 #pragma unroll
       for (int k = 0; k < 2; ++k) {
@@ -341,68 +341,86 @@ __global__ void __launch_bounds__(32 * Attn4Cfg<HD>::kWarps, 1)
       const int p0 = (x - job.t0) * kTile;
       const bool tail = p0 + kTile > all;
       const int slices = alive ? min(4, (most - p0 + 15) / 16) : 0;
-      for (int s = 0; s < slices; ++s) {
+      // Two times 16 positions at once: independent chains for the scheduler.
+      for (int s = 0; s < slices; s += 2) {
         // ---- S = K q^T
-        uint32_t kw[2][NB], kd[2][(NB + 1) / 2];
+        float y[2][4];
 #pragma unroll
-        for (int r = 0; r < 2; ++r) {
-          const int row = 16 * s + g + 8 * r;
-          const uint8_t* kp = st + row * (HD / 2) + tq * (4 * NB);
-          const uint8_t* sp = st + kRec.k_scales() + row * (2 * NB);
-          if constexpr (NB == 4) {
-            const uint4 w = *reinterpret_cast<const uint4*>(kp);
-            kw[r][0] = w.x, kw[r][1] = w.y, kw[r][2] = w.z, kw[r][3] = w.w;
-            const uint2 d = *reinterpret_cast<const uint2*>(sp);
-            kd[r][0] = d.x, kd[r][1] = d.y;
-          } else {
-            const uint2 w = *reinterpret_cast<const uint2*>(kp);
-            kw[r][0] = w.x, kw[r][1] = w.y;
-            kd[r][0] = *reinterpret_cast<const uint32_t*>(sp);
+        for (int e = 0; e < 2; ++e) {
+          uint32_t kw[2][NB], kd[2][NB / 2];
+#pragma unroll
+          for (int r = 0; r < 2; ++r) {
+            const int row = 16 * (s + e) + g + 8 * r;
+            const uint8_t* kp = st + q4_k_byte(row, 8 * tq, NB);
+            const uint8_t* sp = st + kRec.k_scales() + 2 * q4_k_scale(row, 0, NB);
+            if constexpr (NB == 4) {
+              const uint4 w = *reinterpret_cast<const uint4*>(kp);
+              kw[r][0] = w.x, kw[r][1] = w.y, kw[r][2] = w.z, kw[r][3] = w.w;
+              const uint2 d = *reinterpret_cast<const uint2*>(sp);
+              kd[r][0] = d.x, kd[r][1] = d.y;
+            } else {
+              const uint2 w = *reinterpret_cast<const uint2*>(kp);
+              kw[r][0] = w.x, kw[r][1] = w.y;
+              kd[r][0] = *reinterpret_cast<const uint32_t*>(sp);
+            }
           }
-        }
-        float y[4] = {0.f, 0.f, 0.f, 0.f};
+          y[e][0] = y[e][1] = y[e][2] = y[e][3] = 0.f;
 #pragma unroll
-        for (int b = 0; b < NB; ++b) {
-          float c[4] = {qo[b][0], qo[b][1], qo[b][0], qo[b][1]};
+          for (int b = 0; b < NB; ++b) {
+            float c[4];
 #pragma unroll
-          for (int ks = 0; ks < 2; ++ks) {
-            const uint32_t u0 = kw[0][b] >> (8 * ks), u1 = kw[1][b] >> (8 * ks);
-            const uint32_t a0 = u0 & 0x000f000fu, a1 = u1 & 0x000f000fu;
-            const uint32_t a2 = u0 & 0x00f000f0u, a3 = u1 & 0x00f000f0u;
-            mma_f16(c, a0, a1, a2, a3, qh[b][ks][0], qh[b][ks][1]);
-            if (has_lo) mma_f16(c, a0, a1, a2, a3, ql[b][ks][0], ql[b][ks][1]);
+            for (int ks = 0; ks < 2; ++ks) {
+              const uint32_t u0 = kw[0][b] >> (8 * ks), u1 = kw[1][b] >> (8 * ks);
+              const uint32_t a0 = u0 & 0x000f000fu, a1 = u1 & 0x000f000fu;
+              const uint32_t a2 = u0 & 0x00f000f0u, a3 = u1 & 0x00f000f0u;
+              if (ks == 0)
+                mma_f16_first(c, a0, a1, a2, a3, qh[b][0][0], qh[b][0][1]);
+              else
+                mma_f16(c, a0, a1, a2, a3, qh[b][1][0], qh[b][1][1]);
+              if constexpr (LO) mma_f16(c, a0, a1, a2, a3, ql[b][ks][0], ql[b][ks][1]);
+            }
+            const float d0 = half_of(kd[0][b / 2], b & 1), d1 = half_of(kd[1][b / 2], b & 1);
+            y[e][0] = fmaf(c[0] + qo[b][0], d0, y[e][0]);
+            y[e][1] = fmaf(c[1] + qo[b][1], d0, y[e][1]);
+            y[e][2] = fmaf(c[2] + qo[b][0], d1, y[e][2]);
+            y[e][3] = fmaf(c[3] + qo[b][1], d1, y[e][3]);
           }
-          const float d0 = half_of(kd[0][b / 2], b & 1), d1 = half_of(kd[1][b / 2], b & 1);
-          y[0] = fmaf(c[0], d0, y[0]);
-          y[1] = fmaf(c[1], d0, y[1]);
-          y[2] = fmaf(c[2], d1, y[2]);
-          y[3] = fmaf(c[3], d1, y[3]);
         }
         // ---- V's scales of positions 2 tq, 2 tq + 1 and those plus 8
-        uint32_t vd[4][(NB + 1) / 2], any_d = 0;
+        uint32_t vd[2][2][NB], any_d = 0;
 #pragma unroll
-        for (int r = 0; r < 4; ++r) {
-          const int row = 16 * s + 2 * tq + (r & 1) + 8 * (r >> 1);
-          const uint8_t* sp = st + kRec.v_scales() + row * (2 * NB);
-          if constexpr (NB == 4) {
-            const uint2 d = *reinterpret_cast<const uint2*>(sp);
-            vd[r][0] = d.x, vd[r][1] = d.y;
-            any_d |= d.x | d.y;
-          } else {
-            vd[r][0] = *reinterpret_cast<const uint32_t*>(sp);
-            any_d |= vd[r][0];
+        for (int e = 0; e < 2; ++e)
+#pragma unroll
+          for (int r = 0; r < 2; ++r) {
+            const uint8_t* sp =
+                st + kRec.v_scales() + 2 * q4_v_scale(16 * (s + e) + 2 * tq + 8 * r, 0, NB);
+            if constexpr (NB == 4) {
+              const uint4 d = *reinterpret_cast<const uint4*>(sp);
+              vd[e][r][0] = d.x, vd[e][r][1] = d.y, vd[e][r][2] = d.z, vd[e][r][3] = d.w;
+              any_d |= d.x | d.y | d.z | d.w;
+            } else {
+              const uint2 d = *reinterpret_cast<const uint2*>(sp);
+              vd[e][r][0] = d.x, vd[e][r][1] = d.y;
+              any_d |= d.x | d.y;
+            }
           }
-        }
         // ---- softmax: columns 2 tq, 2 tq + 1 of positions g and g + 8
         if (tail) {
 #pragma unroll
-          for (int k = 0; k < 4; ++k)
-            if (p0 + 16 * s + g + 8 * (k >> 1) >= lim[k & 1]) y[k] = -CUDART_INF_F;
-        }
-        float arg[4];
+          for (int e = 0; e < 2; ++e)
 #pragma unroll
-        for (int k = 0; k < 4; ++k) arg[k] = fmaf(y[k], f[k & 1], -ref[k & 1]);
-        const bool over = fmaxf(fmaxf(arg[0], arg[1]), fmaxf(arg[2], arg[3])) > top;
+            for (int k = 0; k < 4; ++k)
+              if (p0 + 16 * (s + e) + g + 8 * (k >> 1) >= lim[k & 1]) y[e][k] = -CUDART_INF_F;
+        }
+        float p[2][4];
+        bool over = false;
+#pragma unroll
+        for (int e = 0; e < 2; ++e)
+#pragma unroll
+          for (int k = 0; k < 4; ++k) {
+            p[e][k] = fmaf(y[e][k], f[k & 1], -ref[k & 1]);
+            over |= p[e][k] > top;
+          }
         // (a scale of 2 or more has the exponent's top bit)
         if (__any_sync(0xffffffffu, over || (any_d & 0x40004000u)) || fresh) {
           // NaN scales are taken out here and their columns remembered: in the product of P by
@@ -410,25 +428,30 @@ __global__ void __launch_bounds__(32 * Attn4Cfg<HD>::kWarps, 1)
           // sequence, where P is 0, to everything.
           uint32_t big = 0;  // the largest scale's bits
 #pragma unroll
-          for (int r = 0; r < 4; ++r)
+          for (int e = 0; e < 2; ++e)
 #pragma unroll
-            for (int b = 0; b < NB; ++b) {
-              const uint32_t h = (b & 1 ? vd[r][b / 2] >> 16 : vd[r][b / 2]) & 0x7fffu;
-              const bool bad = h > 0x7c00u;
-              if (!bad) big = max(big, h);
-              const uint32_t lanes = __ballot_sync(0xffffffffu, bad) & 15u;  // of tq 0..3
-              if (lanes) {
-                if (bad) vd[r][b / 2] &= b & 1 ? 0xffffu : 0xffff0000u;
-                const int place = p0 + 16 * s + 2 * (__ffs(lanes) - 1) + (r & 1) + 8 * (r >> 1);
+            for (int r = 0; r < 4; ++r)
 #pragma unroll
-                for (int k = 0; k < 2; ++k) nans |= (place < lim[k] ? 1u : 0u) << (4 * k + b);
+              for (int b = 0; b < NB; ++b) {
+                uint32_t& w = vd[e][r >> 1][b];
+                const uint32_t h = (r & 1 ? w >> 16 : w) & 0x7fffu;
+                const bool bad = h > 0x7c00u;
+                if (!bad) big = max(big, h);
+                const uint32_t lanes = __ballot_sync(0xffffffffu, bad) & 15u;  // of tq 0..3
+                if (lanes) {
+                  if (bad) w &= r & 1 ? 0xffffu : 0xffff0000u;
+                  const int place = p0 + 16 * (s + e) + 2 * (__ffs(lanes) - 1) + (r & 1) + 8 * (r >> 1);
+#pragma unroll
+                  for (int k = 0; k < 2; ++k) nans |= (place < lim[k] ? 1u : 0u) << (4 * k + b);
+                }
               }
-            }
           big = __reduce_max_sync(0xffffffffu, big);
           const float cap = fminf(top, kTop - fmaxf(0.f, static_cast<float>(static_cast<int>(big >> 10) - 15)));
 #pragma unroll
           for (int k = 0; k < 2; ++k) {
-            float m = fmaxf(y[k] * f[k], y[k + 2] * f[k]);  // NaN does not count
+            // NaN does not count
+            float m = fmaxf(fmaxf(y[0][k] * f[k], y[0][k + 2] * f[k]),
+                            fmaxf(y[1][k] * f[k], y[1][k + 2] * f[k]));
             m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, 4));
             m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, 8));
             m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, 16));
@@ -450,41 +473,43 @@ __global__ void __launch_bounds__(32 * Attn4Cfg<HD>::kWarps, 1)
           top = cap;
           fresh = false;
 #pragma unroll
-          for (int k = 0; k < 4; ++k) arg[k] = fmaf(y[k], f[k & 1], -ref[k & 1]);
-        }
-        float p[4];
+          for (int e = 0; e < 2; ++e)
 #pragma unroll
-        for (int k = 0; k < 4; ++k) {
-          p[k] = ex2(arg[k]);
-          l[k & 1] += p[k];
+            for (int k = 0; k < 4; ++k) p[e][k] = fmaf(y[e][k], f[k & 1], -ref[k & 1]);
         }
-        const uint32_t pt0 = transpose8(pack2<false>(p[0], p[1]));
-        const uint32_t pt1 = transpose8(pack2<false>(p[2], p[3]));
-        // ---- O += V^T (P d)
-        uint32_t vw[4][NB / 2];
 #pragma unroll
-        for (int r = 0; r < 4; ++r) {
-          const int row = 16 * s + 2 * tq + (r & 1) + 8 * (r >> 1);
-          const uint8_t* vp = st + kRec.v_codes() + row * (HD / 2) + g * (2 * NB);
-          if constexpr (NB == 4) {
-            const uint2 w = *reinterpret_cast<const uint2*>(vp);
-            vw[r][0] = w.x, vw[r][1] = w.y;
-          } else {
-            vw[r][0] = *reinterpret_cast<const uint32_t*>(vp);
+        for (int e = 0; e < 2; ++e) {
+#pragma unroll
+          for (int k = 0; k < 4; ++k) {
+            p[e][k] = ex2(p[e][k]);
+            l[k & 1] += p[e][k];
           }
-        }
+          const uint32_t pt0 = transpose8(pack2<false>(p[e][0], p[e][1]));
+          const uint32_t pt1 = transpose8(pack2<false>(p[e][2], p[e][3]));
+          // ---- O += V^T (P d)
+          uint32_t vw[2][NB];
 #pragma unroll
-        for (int b = 0; b < NB; ++b) {
-          const uint32_t b0 = mul2(pt0, halves(vd[0][b / 2], vd[1][b / 2], b & 1));
-          const uint32_t b1 = mul2(pt1, halves(vd[2][b / 2], vd[3][b / 2], b & 1));
-          mma_f16(off, eights[b], eights[b], eights[b], eights[b], b0, b1);
-          const uint32_t t0 = halves(vw[0][b / 2], vw[1][b / 2], b & 1);
-          const uint32_t t1 = halves(vw[2][b / 2], vw[3][b / 2], b & 1);
+          for (int r = 0; r < 2; ++r) {
+            const uint8_t* vp =
+                st + kRec.v_codes() + q4_v_byte(16 * (s + e) + 2 * tq + 8 * r, 4 * g, NB);
+            if constexpr (NB == 4) {
+              const uint4 w = *reinterpret_cast<const uint4*>(vp);
+              vw[r][0] = w.x, vw[r][1] = w.y, vw[r][2] = w.z, vw[r][3] = w.w;
+            } else {
+              const uint2 w = *reinterpret_cast<const uint2*>(vp);
+              vw[r][0] = w.x, vw[r][1] = w.y;
+            }
+          }
 #pragma unroll
-          for (int u = 0; u < 2; ++u) {
-            const uint32_t u0 = t0 >> (8 * u), u1 = t1 >> (8 * u);
-            mma_f16(o[b][u], u0 & 0x000f000fu, u0 & 0x00f000f0u, u1 & 0x000f000fu,
-                    u1 & 0x00f000f0u, b0, b1);
+          for (int b = 0; b < NB; ++b) {
+            const uint32_t b0 = mul2(pt0, vd[e][0][b]), b1 = mul2(pt1, vd[e][1][b]);
+            mma_f16(off, eights[b], eights[b], eights[b], eights[b], b0, b1);
+#pragma unroll
+            for (int u = 0; u < 2; ++u) {
+              const uint32_t u0 = vw[0][b] >> (8 * u), u1 = vw[1][b] >> (8 * u);
+              mma_f16(o[b][u], u0 & 0x000f000fu, u0 & 0x00f000f0u, u1 & 0x000f000fu,
+                      u1 & 0x00f000f0u, b0, b1);
+            }
           }
         }
       }
@@ -603,12 +628,12 @@ bool attn4_supported(int hd, int page) { return (hd == 64 || hd == 128) && page 
 
 namespace {
 
-template <int HD>
+template <int HD, bool LO>
 cudaError_t launch_attn4_t(const Attn4Args& a, cudaStream_t s) {
   using C = Attn4Cfg<HD>;
   static std::atomic<uint64_t> done{0};
   cudaError_t e = ql_once_per_device(done, [] {
-    return cudaFuncSetAttribute(attn4_kernel<HD>, cudaFuncAttributeMaxDynamicSharedMemorySize,
+    return cudaFuncSetAttribute(attn4_kernel<HD, LO>, cudaFuncAttributeMaxDynamicSharedMemorySize,
                                 static_cast<int>(C::kSmem));
   });
   if (e != cudaSuccess) return e;
@@ -622,7 +647,7 @@ cudaError_t launch_attn4_t(const Attn4Args& a, cudaStream_t s) {
   attr[0].val.programmaticStreamSerializationAllowed = 1;
   cfg.attrs = attr;
   cfg.numAttrs = 1;
-  return cudaLaunchKernelEx(&cfg, attn4_kernel<HD>, a);
+  return cudaLaunchKernelEx(&cfg, attn4_kernel<HD, LO>, a);
 }
 
 }  // namespace
@@ -642,7 +667,10 @@ void attn4_plan(int hd, int num_sms, Attn4Args* a, size_t* cta_bytes, size_t* wa
 }
 
 cudaError_t launch_attn4(const Attn4Args& a, cudaStream_t s) {
-  return a.cache.hd == 128 ? launch_attn4_t<128>(a, s) : launch_attn4_t<64>(a, s);
+  const bool lo = a.in_dtype == kF32 || a.rope_stride != 0;
+  if (a.cache.hd == 128)
+    return lo ? launch_attn4_t<128, true>(a, s) : launch_attn4_t<128, false>(a, s);
+  return lo ? launch_attn4_t<64, true>(a, s) : launch_attn4_t<64, false>(a, s);
 }
 
 }  // namespace ql

@@ -500,16 +500,27 @@ __device__ __forceinline__ uint32_t q4_0_pair(float x0, float x1, uint16_t& scal
   return q4_code(x0, d, inv) | q4_code(x1, d, inv) << 4;
 }
 
-// Byte of a row's codes (head_dim / 2 bytes, NB = head_dim / 32 blocks) that holds those of
-// dims d, d + 1 (d even).  The order is the one in which the decode kernel's tensor-core
-// fragments take them, so that a lane's codes of a row are one load: of a K row lane t of
-// four takes dims 32 b + 8 t .. + 7 of every block b, of a V row lane g of eight dims
-// 32 b + 4 g .. + 3.
-__host__ __device__ constexpr int q4_k_byte(int d, int nb) {
-  return (d & 31) / 8 * 4 * nb + d / 32 * 4 + (d & 7) / 2;
+// Where a Q4_0 record (64 positions) keeps the codes of dims d, d + 1 (d even) of a position:
+// the byte in its K or V codes, NB = head_dim / 32 blocks a row.  The order is the one in which
+// the decode kernel's tensor-core fragments take them.  Of a K row lane t of four takes dims
+// 32 b + 8 t .. + 7 of every block b, as one load.  Of V lane g of eight takes dims
+// 32 b + 4 g .. + 3 of two neighbouring positions, a block's in one word with the even position
+// in its low half; the lanes' places rotate from pair to pair so that the loads of a warp
+// spread over all banks of shared memory.
+__host__ __device__ constexpr int q4_k_byte(int pos, int d, int nb) {
+  return pos * 16 * nb + (d & 31) / 8 * 4 * nb + d / 32 * 4 + (d & 7) / 2;
 }
-__host__ __device__ constexpr int q4_v_byte(int d, int nb) {
-  return (d & 31) / 4 * 2 * nb + d / 32 * 2 + (d & 3) / 2;
+__host__ __device__ constexpr int q4_v_lane(int g, int pair, int nb) {
+  return nb == 4 ? g ^ 2 * (pair & 3) : nb == 2 ? g ^ 4 * (pair / 2 & 1) : g;
+}
+__host__ __device__ constexpr int q4_v_byte(int pos, int d, int nb) {
+  return pos / 2 * 32 * nb + q4_v_lane((d & 31) / 4, pos / 2, nb) * 4 * nb + d / 32 * 4 +
+         (pos & 1) * 2 + (d & 3) / 2;
+}
+// ... and a block's scale among its K or V scales.
+__host__ __device__ constexpr int q4_k_scale(int pos, int b, int nb) { return pos * nb + b; }
+__host__ __device__ constexpr int q4_v_scale(int pos, int b, int nb) {
+  return pos / 2 * 2 * nb + 2 * b + (pos & 1);
 }
 
 }  // namespace ql

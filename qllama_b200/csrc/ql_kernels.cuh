@@ -53,8 +53,8 @@ struct SeqTable {
 };
 
 // A Q4_0 cache keeps 64 positions of one KV head in one run of 72 hd bytes, so that a tile
-// with its scales is one bulk copy: the K codes [64][hd/2], the V codes [64][hd/2], the K
-// scales [64][hd/32] and the V scales, f16.
+// with its scales is one bulk copy: the K codes (64 hd/2 bytes), the V codes, the K scales
+// (64 hd/32 of f16) and the V scales, each in the order of q4_k_byte and its like.
 struct Q4Record {
   int hd;
   __host__ __device__ constexpr size_t bytes() const { return 72 * static_cast<size_t>(hd); }

@@ -805,14 +805,11 @@ __global__ void __launch_bounds__(256) tiles_to_f16_kernel(const __grid_constant
       }
     }
   } else if constexpr (DT == kQ4_0) {
-    constexpr int kNb = HD / 32;
-    const uint8_t* src = q4_codes(a.cache, row, kind != 0);
-    const uint16_t* sc = q4_scales(a.cache, row, kind != 0);
 #pragma unroll
     for (int i = 0; i < kVals; i += 2) {
       const int d = part * kVals + i;
-      const uint32_t w = src[kind ? q4_v_byte(d, kNb) : q4_k_byte(d, kNb)];
-      const float f = __half2float(__ushort_as_half(sc[d / 32]));
+      const uint32_t w = *q4_code_at(a.cache, row, d, kind != 0);
+      const float f = __half2float(__ushort_as_half(*q4_scale_at(a.cache, row, d / 32, kind != 0)));
       v[i] = f * static_cast<float>(static_cast<int>(w & 15u) - 8);
       v[i + 1] = f * static_cast<float>(static_cast<int>(w >> 4) - 8);
     }
