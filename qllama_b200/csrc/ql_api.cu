@@ -1241,7 +1241,7 @@ static int attn_forward_impl(ql_ctx* c, ql_kv* kv, const ql_attn_args* a,
   const int jobs = a->batch * n;
   const size_t qn = static_cast<size_t>(jobs) * hq * hd, kn = static_cast<size_t>(jobs) * hkv * hd;
   const size_t ib = elem_bytes(a->in_dtype), obb = elem_bytes(a->out_dtype);
-  const bool fast = !sparse && kv->have_maps &&
+  const bool fast = kv->have_maps &&
                     ql::splitkv_supported(hd, kv->cfg.dtype, group, kv->cfg.page_size);
   const bool tc_prefill = !sparse && (kv->have_maps || kv->cfg.dtype == QL_Q4_0) && n > 1 &&
                           ql::prefill_tc_supported(hd, kv->cfg.dtype, n);
@@ -1283,7 +1283,7 @@ static int attn_forward_impl(ql_ctx* c, ql_kv* kv, const ql_attn_args* a,
   int tps = max_tiles, max_splits = 1;
   // Too few (token, KV head) jobs to fill half the SMs: the wide kernel, whose
   // consumer groups share each split's tiles, one CTA per SM (latency).
-  const int wide_kg = fast ? ql::splitkv_wide_groups(hd, kv->cfg.dtype) : 0;
+  const int wide_kg = fast && !sparse ? ql::splitkv_wide_groups(hd, kv->cfg.dtype) : 0;
   const bool latency = fast && 2LL * jobs * hkv <= c->num_sms;
   // A short context in that regime: each job's tiles spread over up to
   // kMaxCluster CTAs (one tile each when every CTA of the launch then has an

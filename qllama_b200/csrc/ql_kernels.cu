@@ -497,7 +497,9 @@ __device__ __forceinline__ void emit_rows(const AttnArgs& a, const float* res, i
 // (0: read from the arguments).  Compile-time facts, so that each form holds
 // only its own merge, exchange and conversions: the code a launch runs is
 // fetched cold, and less of it is faster.
-template <int HD, int DT, bool DEVROPE, int KG, bool CL, bool PEER, int IO, int GRP>
+// SP: attention over selected blocks (a.sel; rows already appended, one token per job): tile i
+// of the job is block sel[i], and key positions are places in that list.
+template <int HD, int DT, bool DEVROPE, int KG, bool CL, bool PEER, int IO, int GRP, bool SP = false>
 __global__ void __launch_bounds__(SplitCfg<HD, DT, KG>::kThreads, SplitCfg<HD, DT, KG>::kMinCtas)
     splitkv_kernel(const __grid_constant__ AttnArgs a, const __grid_constant__ CUtensorMap kmap,
                    const __grid_constant__ CUtensorMap vmap, int job0) {
@@ -514,7 +516,7 @@ __global__ void __launch_bounds__(SplitCfg<HD, DT, KG>::kThreads, SplitCfg<HD, D
   const int b = job / a.new_len, t_tok = job % a.new_len;
   const int seq = a.seqs.seq[b];
   const int qpos = a.seqs.start[b] + t_tok;
-  const int L = qpos + 1;
+  const int L = SP ? sel_keys(qpos, a.sel_max) : qpos + 1;
   const int ntiles = (L + kTile - 1) / kTile;
   const int nsplit = (ntiles + a.tiles_per_split - 1) / a.tiles_per_split;
 
@@ -562,7 +564,7 @@ __global__ void __launch_bounds__(SplitCfg<HD, DT, KG>::kThreads, SplitCfg<HD, D
 
   uint64_t* appended = empty + C::kStages;  // the fused append is written and fenced
   uint8_t* newrow = reinterpret_cast<uint8_t*>(qs) + C::kRowOff;  // its converted K/V row
-  const bool appends = a.fuse_append && split == nsplit - 1;
+  const bool appends = !SP && a.fuse_append && split == nsplit - 1;
 
   if (threadIdx.x == 0) {
     for (int s = 0; s < C::kStages; ++s) {
@@ -582,8 +584,16 @@ __global__ void __launch_bounds__(SplitCfg<HD, DT, KG>::kThreads, SplitCfg<HD, D
   // patch kernel, and a launch that follows a patch is an ordinary one (no
   // programmatic dependency), so the entries are in place when this runs.
   const int* bt = a.cache.block_table + static_cast<size_t>(seq) * a.cache.pages_per_seq;
-  int lane_page = 0;
-  if (warp == NCW && lane < my_tiles) lane_page = __ldg(bt + (tile0 + lane) * kTile / a.cache.page);
+  // (A selection comes from the previous kernel: its blocks, and their pages, are read after
+  // the dependency.)
+  const int32_t* sel =
+      SP ? a.sel + (static_cast<size_t>(job) * hkv + kvh) * a.sel_max + tile0 : nullptr;
+  int lane_page = 0, lane_block = 0;
+  auto look_up = [&](int i) {  // the page of tile i of this split, and its block
+    lane_block = SP ? sel[i] : tile0 + i;
+    lane_page = __ldg(bt + lane_block * kTile / a.cache.page);
+  };
+  if (!SP && warp == NCW && lane < my_tiles) look_up(lane);
   // What the CTA reads first once the dependency is met is fetched into L2
   // now (prefetches read nothing into the CTA; lines written meanwhile are
   // updated in L2): the first stages' tiles, q of this KV head's group, the
@@ -593,7 +603,7 @@ __global__ void __launch_bounds__(SplitCfg<HD, DT, KG>::kThreads, SplitCfg<HD, D
   if (warp == NCW && appends)
     app_page = __ldg(bt + static_cast<size_t>(qpos) / a.cache.page);
   if (warp == NCW) {
-    if (lane < min(my_tiles, C::kStages) && lane_page >= 0 && lane_page < a.cache.num_pages) {
+    if (!SP && lane < min(my_tiles, C::kStages) && lane_page >= 0 && lane_page < a.cache.num_pages) {
       const int row =
           (lane_page * hkv + kvh) * a.cache.page + ((tile0 + lane) * kTile) % a.cache.page;
       if constexpr (Q8) {
@@ -651,9 +661,9 @@ __global__ void __launch_bounds__(SplitCfg<HD, DT, KG>::kThreads, SplitCfg<HD, D
   // the tile holding the new token waits until its K/V row has been appended.
   if (warp == NCW) {
     // Tile i of the split into stage i % kStages (lane 0).
-    auto issue = [&](int i, int page) {
+    auto issue = [&](int i, int page, int block) {
       const int st = i % C::kStages;
-      const int p0 = (tile0 + i) * kTile;
+      const int p0 = block * kTile;
       if (page < 0 || page >= a.cache.num_pages) {
         atomicOr(a.status, kStatusBadPage);
         page = 0;  // keep the pipeline consistent; the result is flagged
@@ -701,18 +711,17 @@ __global__ void __launch_bounds__(SplitCfg<HD, DT, KG>::kThreads, SplitCfg<HD, D
     bool alive = true, append_due = appends;
     const int burst = min(my_tiles, C::kStages);
     for (int i0 = 0; i0 < my_tiles && alive; i0 += 32) {
-      if (i0 > 0)
-        lane_page = i0 + lane < my_tiles ? __ldg(bt + (tile0 + i0 + lane) * kTile / a.cache.page)
-                                         : 0;
+      if ((SP || i0 > 0) && i0 + lane < my_tiles) look_up(i0 + lane);
       const int n = min(32, my_tiles - i0);
       for (int j = 0; j < n && alive; ++j) {
         const int page = __shfl_sync(0xffffffffu, lane_page, j);
+        const int block = SP ? __shfl_sync(0xffffffffu, lane_block, j) : tile0 + i0 + j;
         if (lane == 0) {
           const int i = i0 + j, st = i % C::kStages;
           if (i >= C::kStages && !mbar_wait(&empty[st], ((i / C::kStages) - 1) & 1, a.status))
             alive = false;
           else
-            issue(i, page);
+            issue(i, page, block);
         }
         alive = __shfl_sync(0xffffffffu, alive, 0);
         if (append_due && i0 + j + 1 == burst) {
@@ -1335,8 +1344,13 @@ using SplitKvFn = void (*)(const AttnArgs, const CUtensorMap, const CUtensorMap,
 // (single-GPU calls with the table's RoPE) I/O of the cache's own 16-bit type,
 // then also eight query heads per KV head when the call has that.
 template <int HD, int DT, bool DEVROPE, int KG>
-static SplitKvFn splitkv_form(bool clustered, bool peer, bool io, bool g8) {
+static SplitKvFn splitkv_form(bool clustered, bool peer, bool io, bool g8, bool sp = false) {
   constexpr int kIO = DT == kQ8_0 ? -1 : DT;
+  if constexpr (KG == 1 && !DEVROPE) {
+    if (sp)
+      return clustered ? splitkv_kernel<HD, DT, DEVROPE, KG, true, false, -1, 0, true>
+                       : splitkv_kernel<HD, DT, DEVROPE, KG, false, false, -1, 0, true>;
+  }
   if constexpr (KG == 1) {
     if (clustered) {
       if (peer) return splitkv_kernel<HD, DT, DEVROPE, KG, true, true, -1, 0>;
@@ -1369,10 +1383,10 @@ static cudaError_t configure_splitkv_t(int* ctas_per_sm) {
   }
   // every compiled form: shared memory (clustered forms add the gather area)
   // and, for clusters above 8 CTAs, the non-portable size
-  for (int form = 0; form < 16 && e == cudaSuccess; ++form) {
-    const bool clustered = form & 1, peer = form & 2, io = form & 4, g8 = form & 8;
-    if (clustered && KG != 1) continue;
-    SplitKvFn k = splitkv_form<HD, DT, DEVROPE, KG>(clustered, peer, io, g8);
+  for (int form = 0; form < 32 && e == cudaSuccess; ++form) {
+    const bool clustered = form & 1, peer = form & 2, io = form & 4, g8 = form & 8, sp = form & 16;
+    if ((clustered || sp) && KG != 1) continue;
+    SplitKvFn k = splitkv_form<HD, DT, DEVROPE, KG>(clustered, peer, io, g8, sp);
     e = cudaFuncSetAttribute(k, cudaFuncAttributeMaxDynamicSharedMemorySize,
                              static_cast<int>(clustered ? C::kSmemCluster : C::kSmem));
     if (e == cudaSuccess && clustered && C::kMaxCluster > 8)
@@ -1397,7 +1411,8 @@ static cudaError_t launch_splitkv_t(const AttnArgs& a, const CUtensorMap* kmap,
   if (e != cudaSuccess) return e;
   const bool io = DT != kQ8_0 && a.in_dtype == DT && a.out_dtype == DT;
   const SplitKvFn kernel = splitkv_form<HD, DT, DEVROPE, KG>(KG == 1 && a.cluster > 1,
-                                                             a.peer.nranks > 0, io, a.group == 8);
+                                                             a.peer.nranks > 0, io, a.group == 8,
+                                                             a.sel != nullptr);
   for (int j0 = 0; j0 < jobs; j0 += 65535) {
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = dim3(a.max_splits, a.cache.hkv, min(65535, jobs - j0));
