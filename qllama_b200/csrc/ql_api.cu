@@ -1261,6 +1261,9 @@ static int attn_forward_impl(ql_ctx* c, ql_kv* kv, const ql_attn_args* a,
     for (int b = 0; b < a->batch; ++b) row_tiles[b] = std::min(row_tiles[b], max_tiles);
     max_len = std::min<int64_t>(max_len, static_cast<int64_t>(max_tiles) * ql::kTile);
   }
+  if (sparse && max_blocks > (1 << 18))
+    return fail(QL_ERR_UNSUPPORTED, "attention over selected blocks takes sequences of up to %d "
+                "blocks", 1 << 18);
   // the lists' rows: as the caller asked for them, or as long as they can get
   const int sel_max = !sparse ? 0 : sparse->selected ? sparse->blocks : max_tiles;
   // a few tokens over a Q4_0 cache: every job's tiles in one list
@@ -1362,8 +1365,9 @@ static int attn_forward_impl(ql_ctx* c, ql_kv* kv, const ql_attn_args* a,
     off += align256(static_cast<size_t>(jobs) * hkv * sel_max * sizeof(int32_t));
   r = ensure_ws(c, off);
   if (r != QL_OK) return r;
-  if ((fast && max_splits > 1) || q4_decode) {
-    r = ensure_counters(c, static_cast<size_t>(q4_decode ? a->batch * a4.units : jobs) * hkv);
+  if ((fast && max_splits > 1) || q4_decode || sparse) {
+    r = ensure_counters(c, static_cast<size_t>(std::max(q4_decode ? a->batch * a4.units : 0, jobs)) *
+                               hkv);
     if (r != QL_OK) return r;
   }
   char* w = static_cast<char*>(c->ws);
@@ -1495,6 +1499,8 @@ static int attn_forward_impl(ql_ctx* c, ql_kv* kv, const ql_attn_args* a,
     se.first = sparse->first;
     se.last = sparse->last;
     se.max_blocks = max_blocks;
+    se.q_vec = aligned_to(q, a->in_dtype == QL_F32 ? 16 : 8);
+    se.counters = c->counters;  // zero again when the attention starts
     se.score = reinterpret_cast<double*>(w + o_sc);
     se.bounds = kv->bounds[layer];
     se.sel = sparse->selected ? sparse->selected : reinterpret_cast<int32_t*>(w + o_sel);

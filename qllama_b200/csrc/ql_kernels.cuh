@@ -257,6 +257,9 @@ struct SelectArgs {
   int32_t new_len;
   int32_t take, first, last;
   int32_t max_blocks;   // row length of `score`
+  int32_t smem_blocks;  // set by the launch: scores that shared memory holds
+  int32_t q_vec;        // q allows loads of four elements
+  int32_t* counters;    // [jobs][hkv], zero between launches
   double* score;        // scratch [jobs][hkv][max_blocks]
   const uint16_t* bounds;
   int32_t* sel;         // [jobs][hkv][take], ascending, then -1
