@@ -1519,7 +1519,7 @@ static int attn_forward_impl(ql_ctx* c, ql_kv* kv, const ql_attn_args* a,
   if (q4_decode) {
     a4.q = q;
     a4.in_dtype = a->in_dtype;
-    a4.q_vec = aligned_to(q, a->in_dtype == QL_F32 ? 16 : 8);
+    a4.q_vec = aligned_to(q, 16);
     a4.out = out;
     a4.out_dtype = a->out_dtype;
     a4.out_vec = at.out_vec;

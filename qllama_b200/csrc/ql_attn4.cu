@@ -51,7 +51,7 @@ struct Attn4Cfg {
   static constexpr int kRing = kStages * kRecord;  // of one warp
   static constexpr int kPart = 8 * HD + 16;        // floats of a piece: rows, then (reference, sum)
   static constexpr size_t kSmem = 128 + static_cast<size_t>(kWarps) * (kRing + kStages * 8) +
-                                  kWarps * 4 * 4 + 64;
+                                  kWarps * 32 + 16;
   static_assert(kPart * 4 <= kRing, "a warp's last piece takes its ring's place");
 };
 
@@ -101,24 +101,33 @@ struct Job {
   int t0, tiles;  // its first place in the list of tiles, and their number
 };
 
-__device__ __forceinline__ Job job_at(const Attn4Args& a, int x) {
-  int lo = 0, hi = a.batch - 1;
-  while (lo < hi) {
-    const int mid = (lo + hi + 1) / 2;
-    if (a.first[mid] <= x) lo = mid;
-    else hi = mid - 1;
-  }
+// a / b for 0 <= a < 2^30 and a quotient below 2^22, where the product with the reciprocal is at
+// most one off (an integer division takes several times as long, and these stand one behind
+// the other before the first key arrives).
+__device__ __forceinline__ int divide(int a, int b) {
+  int q = static_cast<int>(static_cast<float>(a) * __frcp_rn(static_cast<float>(b)));
+  const int r = a - q * b;
+  if (r < 0) --q;
+  if (r >= b) ++q;
+  return q;
+}
+
+__device__ __forceinline__ int seq_tiles(const Attn4Args& a, int b) {
+  const int end = a.seqs.start[b] + a.new_len;
+  return a.sel ? sel_blocks(end - 1, a.sel_max) : (end + kTile - 1) / kTile;
+}
+
+// Job k of sequence b.
+__device__ __forceinline__ Job job_of(const Attn4Args& a, int b, int k, int tiles) {
   Job j;
-  j.b = lo;
-  const int end = a.seqs.start[lo] + a.new_len;
-  j.tiles = a.sel ? sel_blocks(end - 1, a.sel_max) : (end + kTile - 1) / kTile;
-  const int k = (x - a.first[lo]) / j.tiles;
-  j.t0 = a.first[lo] + k * j.tiles;
-  j.id = lo * a.cache.hkv * a.units + k;
-  j.kvh = k / a.units;
+  j.b = b;
+  j.tiles = tiles;
+  j.t0 = a.first[b] + k * tiles;
+  j.id = b * a.cache.hkv * a.units + k;
+  j.kvh = divide(k, a.units);
   const int unit = k - j.kvh * a.units;
   if (a.sel) {  // a list belongs to one token: chunks of its heads
-    const int per = (a.group + 7) / 8, t = unit / per, h0 = (unit - t * per) * 8;
+    const int per = (a.group + 7) / 8, t = divide(unit, per), h0 = (unit - t * per) * 8;
     j.row0 = t * a.group + h0;
     j.rows = min(8, a.group - h0);
   } else {
@@ -128,28 +137,45 @@ __device__ __forceinline__ Job job_at(const Attn4Args& a, int x) {
   return j;
 }
 
-// The record that holds tile x of the list; -1 for a list's place behind its blocks.
-__device__ __forceinline__ int record_at(const Attn4Args& a, int x) {
-  const Job j = job_at(a, x);
+__device__ __forceinline__ Job job_at(const Attn4Args& a, int x) {
+  int lo = 0, hi = a.batch - 1;
+  while (lo < hi) {
+    const int mid = (lo + hi + 1) / 2;
+    if (a.first[mid] <= x) lo = mid;
+    else hi = mid - 1;
+  }
+  const int tiles = seq_tiles(a, lo);
+  return job_of(a, lo, divide(x - a.first[lo], tiles), tiles);
+}
+
+// The job behind j (which is not the last one).
+__device__ __forceinline__ Job next_job(const Attn4Args& a, const Job& j) {
+  const int per = a.cache.hkv * a.units, k = j.id - j.b * per + 1;
+  return k < per ? job_of(a, j.b, k, j.tiles) : job_of(a, j.b + 1, 0, seq_tiles(a, j.b + 1));
+}
+
+// The record that holds tile x of the list, of job j; -1 for a list's place behind its blocks.
+__device__ __forceinline__ int record_at(const Attn4Args& a, const Job& j, int x) {
   const CacheView& c = a.cache;
   int tile = x - j.t0;
   if (a.sel) {
-    const int t = j.row0 / a.group;
+    const int t = divide(j.row0, a.group);
     if (tile >= sel_blocks(a.seqs.start[j.b] + t, a.sel_max)) return -1;
     tile = a.sel[(static_cast<size_t>(j.b * a.new_len + t) * c.hkv + j.kvh) * a.sel_max + tile];
   }
   const int per = c.page / kTile;
-  int page = c.block_table[static_cast<size_t>(a.seqs.seq[j.b]) * c.pages_per_seq + tile / per];
+  const int in_seq = per == 1 ? tile : tile / per;
+  int page = c.block_table[static_cast<size_t>(a.seqs.seq[j.b]) * c.pages_per_seq + in_seq];
   if (page < 0 || page >= c.num_pages) {
     atomicOr(a.status, kStatusBadPage);
     page = 0;  // keep the pipeline consistent; the result is flagged
   }
-  return (page * c.hkv + j.kvh) * per + tile % per;
+  return (page * c.hkv + j.kvh) * per + tile - in_seq * per;
 }
 
 // Element offset of query row `row` (token row / group, head row % group) in q and out.
 __device__ __forceinline__ size_t row_offset(const Attn4Args& a, const Job& j, int row, int hd) {
-  const int t = row / a.group, h = row - t * a.group;
+  const int t = divide(row, a.group), h = row - t * a.group;
   return ((static_cast<size_t>(j.b) * a.new_len + t) * a.hq + j.kvh * a.group + h) * hd;
 }
 
@@ -200,7 +226,9 @@ __global__ void __launch_bounds__(32 * Attn4Cfg<HD>::kWarps, 1)
   const int g = lane >> 2, tq = lane & 3;
   uint8_t* ring = smem + warp * C::kRing;
   uint64_t* full = reinterpret_cast<uint64_t*>(smem + W * C::kRing) + warp * S;
-  int* flag = reinterpret_cast<int*>(smem + W * C::kRing + W * S * 8);
+  // the last job of every warp's part, for the joining
+  Job* last_job = reinterpret_cast<Job*>(smem + W * C::kRing + W * S * 8);
+  int* flag = reinterpret_cast<int*>(last_job + W);
 
   const int c0 = blockIdx.x * a.per_cta, c1 = min(c0 + a.per_cta, a.total);
   const int w0 = min(c0 + warp * a.per_warp, c1), w1 = min(w0 + a.per_warp, c1);
@@ -215,8 +243,22 @@ __global__ void __launch_bounds__(32 * Attn4Cfg<HD>::kWarps, 1)
   // -------------------------------------------------------------- the ring --
   // The lanes hold the records of 32 tiles at a time; lane 0 issues.
   int lane_rec = 0;
+  Job job{};  // of the part's first tile
   auto issue = [&](int i) {
-    if ((i & 31) == 0) lane_rec = w0 + i + lane < w1 ? record_at(a, w0 + i + lane) : -1;
+    if ((i & 31) == 0) {
+      const int x = min(w0 + i + lane, w1 - 1);
+      const Job j = job_at(a, x);
+      lane_rec = record_at(a, j, x);
+      if (i == 0) {
+        job.b = __shfl_sync(0xffffffffu, j.b, 0);
+        job.id = __shfl_sync(0xffffffffu, j.id, 0);
+        job.kvh = __shfl_sync(0xffffffffu, j.kvh, 0);
+        job.row0 = __shfl_sync(0xffffffffu, j.row0, 0);
+        job.rows = __shfl_sync(0xffffffffu, j.rows, 0);
+        job.t0 = __shfl_sync(0xffffffffu, j.t0, 0);
+        job.tiles = __shfl_sync(0xffffffffu, j.tiles, 0);
+      }
+    }
     const int rec = __shfl_sync(0xffffffffu, lane_rec, i & 31);
     if (lane != 0) return;
     uint64_t* bar = &full[i % S];
@@ -238,7 +280,7 @@ __global__ void __launch_bounds__(32 * Attn4Cfg<HD>::kWarps, 1)
   bool alive = true;
   int x = w0;
   while (x < w1) {
-    const Job job = job_at(a, x);
+    if (x > w0) job = next_job(a, job);
     const int seg1 = min(w1, job.t0 + job.tiles);
     const int start = a.seqs.start[job.b];
 
@@ -251,22 +293,52 @@ __global__ void __launch_bounds__(32 * Attn4Cfg<HD>::kWarps, 1)
     {
       float v[NB][8];
       const bool live = g < job.rows;
-      const int row = job.row0 + (live ? g : 0), t = row / a.group;
-      const size_t off = row_offset(a, job, row, HD);
-      const double2* rope = a.rope + static_cast<size_t>(start + t) * a.rope_stride;
+      const int row = job.row0 + (live ? g : 0);
+      const size_t off = row_offset(a, job, row, HD) + 8 * tq;
+      // the type is settled outside the loads, so that all are under way at once
+      if (a.in_dtype == kF32 && a.q_vec) {
+        const float4* p = reinterpret_cast<const float4*>(static_cast<const float*>(a.q) + off);
+        float4 w[NB][2];
+#pragma unroll
+        for (int b = 0; b < NB; ++b) w[b][0] = p[8 * b], w[b][1] = p[8 * b + 1];
+#pragma unroll
+        for (int b = 0; b < NB; ++b) {
+          v[b][0] = w[b][0].x, v[b][1] = w[b][0].y, v[b][2] = w[b][0].z, v[b][3] = w[b][0].w;
+          v[b][4] = w[b][1].x, v[b][5] = w[b][1].y, v[b][6] = w[b][1].z, v[b][7] = w[b][1].w;
+        }
+      } else if (a.in_dtype != kF32 && a.q_vec) {
+        const uint4* p = reinterpret_cast<const uint4*>(static_cast<const uint16_t*>(a.q) + off);
+        uint4 w[NB];
+#pragma unroll
+        for (int b = 0; b < NB; ++b) w[b] = p[4 * b];
+        const bool half = a.in_dtype == kF16;
+#pragma unroll
+        for (int b = 0; b < NB; ++b) {
+          const uint32_t in[4] = {w[b].x, w[b].y, w[b].z, w[b].w};
+#pragma unroll
+          for (int k = 0; k < 4; ++k) {
+            const float2 y = __half22float2(*reinterpret_cast<const __half2*>(&in[k]));
+            v[b][2 * k] = half ? y.x : __uint_as_float(in[k] << 16);
+            v[b][2 * k + 1] = half ? y.y : __uint_as_float(in[k] & 0xffff0000u);
+          }
+        }
+      } else {
+#pragma unroll
+        for (int b = 0; b < NB; ++b)
+#pragma unroll
+          for (int k = 0; k < 8; ++k) v[b][k] = load_elem(a.q, off + 32 * b + k, a.in_dtype);
+      }
+      const double2* rope =
+          a.rope_stride ? a.rope + static_cast<size_t>(start + divide(row, a.group)) * a.rope_stride
+                        : nullptr;
       float mx = 0.f;
 #pragma unroll
       for (int b = 0; b < NB; ++b) {
         const int d = 32 * b + 8 * tq;
-        float lo4[4], hi4[4];
-        load_vec<4>(a.q, off + d, a.in_dtype, a.q_vec != 0, lo4);
-        load_vec<4>(a.q, off + d + 4, a.in_dtype, a.q_vec != 0, hi4);
 #pragma unroll
-        for (int k = 0; k < 4; ++k) {
-          v[b][k] = live ? lo4[k] : 0.f;
-          v[b][k + 4] = live ? hi4[k] : 0.f;
-        }
-        if (a.rope_stride) {
+        for (int k = 0; k < 8; ++k)
+          if (!live) v[b][k] = 0.f;
+        if (rope) {
 #pragma unroll
           for (int k = 0; k < 8; k += 2)
             rope_pair(v[b][k], v[b][k + 1], rope[(d + k) / 2], v[b][k], v[b][k + 1]);
@@ -314,15 +386,15 @@ __global__ void __launch_bounds__(32 * Attn4Cfg<HD>::kWarps, 1)
     // its list), and those that all rows of the job see.
     int lim[2], all;
     if (a.sel) {
-      all = sel_keys(start + job.row0 / a.group, a.sel_max);
+      all = sel_keys(start + divide(job.row0, a.group), a.sel_max);
       lim[0] = lim[1] = all;
     } else {
-      all = start + job.row0 / a.group + 1;
+      all = start + divide(job.row0, a.group) + 1;
 #pragma unroll
       for (int k = 0; k < 2; ++k)
-        lim[k] = start + (job.row0 + min(2 * tq + k, job.rows - 1)) / a.group + 1;
+        lim[k] = start + divide(job.row0 + min(2 * tq + k, job.rows - 1), a.group) + 1;
     }
-    const int most = a.sel ? all : start + (job.row0 + job.rows - 1) / a.group + 1;
+    const int most = a.sel ? all : start + divide(job.row0 + job.rows - 1, a.group) + 1;
 
     float o[NB][2][4], off[4] = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
@@ -557,6 +629,8 @@ __global__ void __launch_bounds__(32 * Attn4Cfg<HD>::kWarps, 1)
     }
   }
 
+  if (lane == 0 && w0 < w1) last_job[warp] = job;
+
   // ------------------------------------------------------------ joining --
   // (__syncthreads orders the pieces in memory as well, inside the CTA)
   __syncthreads();
@@ -591,7 +665,7 @@ __global__ void __launch_bounds__(32 * Attn4Cfg<HD>::kWarps, 1)
     if (inside) return;
     // The barrier orders every thread's part of the piece before thread 0's count, whose
     // release makes it visible; the last CTA's acquire sees the others'.
-    const int first = j.t0 / a.per_cta, last = (t1 - 1) / a.per_cta;
+    const int first = divide(j.t0, a.per_cta), last = divide(t1 - 1, a.per_cta);
     __syncthreads();
     if (threadIdx.x == 0) flag[0] = atom_add_acq_rel_gpu(&a.counters[j.id], 1) == last - first;
     __syncthreads();
@@ -613,7 +687,7 @@ __global__ void __launch_bounds__(32 * Attn4Cfg<HD>::kWarps, 1)
   for (int i = 0; i < W; ++i) {
     const int b0 = warp_begin(i), b1 = warp_begin(i + 1);
     if (b0 >= b1) break;
-    const Job lastj = job_at(a, b1 - 1);
+    const Job lastj = last_job[i];
     const int t1 = lastj.t0 + lastj.tiles;
     if (i == 0 && lastj.t0 > b0) {  // the first job of the run, if another CTA began it
       const Job firstj = job_at(a, b0);

@@ -145,7 +145,7 @@ struct AttnArgs {
 struct Attn4Args {
   const void* q;  // [batch, new_len, hq, hd]
   int32_t in_dtype;
-  int32_t q_vec;  // q allows loads of four elements
+  int32_t q_vec;  // q is 16-byte aligned
   void* out;      // [batch, new_len, hq*hd]
   int32_t out_dtype;
   int32_t out_vec;
