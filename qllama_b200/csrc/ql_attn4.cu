@@ -179,35 +179,6 @@ __device__ __forceinline__ size_t row_offset(const Attn4Args& a, const Job& j, i
   return ((static_cast<size_t>(j.b) * a.new_len + t) * a.hq + j.kvh * a.group + h) * hd;
 }
 
-// Joins pieces of a job: part(i) for i < n gives one's floats.  Every thread of the CTA takes
-// columns; `emit` gets each (row, first column, four numerators, reference, sum).
-template <int HD, typename P, typename E>
-__device__ __forceinline__ void join_pieces(int n, int rows, int threads, P part, E emit) {
-  for (int c = threadIdx.x; c < rows * (HD / 4); c += threads) {
-    const int r = c / (HD / 4), d = c % (HD / 4) * 4;
-    float ref = -CUDART_INF_F, sum = 0.f;
-    float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
-    for (int i = 0; i < n; ++i) {
-      const float* p = part(i);
-      const float2 ml = *reinterpret_cast<const float2*>(p + 8 * HD + 2 * r);
-      const float4 v = *reinterpret_cast<const float4*>(p + r * HD + d);
-      const float top = fmaxf(ref, ml.x), base = top == -CUDART_INF_F ? 0.f : top;
-      const float w0 = exp2f(ref - base), w1 = exp2f(ml.x - base);
-      sum = sum * w0 + ml.y * w1;
-      acc.x = acc.x * w0 + v.x * w1;
-      acc.y = acc.y * w0 + v.y * w1;
-      acc.z = acc.z * w0 + v.z * w1;
-      acc.w = acc.w * w0 + v.w * w1;
-      ref = top;
-    }
-    emit(r, d, acc, ref, sum);
-  }
-}
-
-__device__ __forceinline__ float4 scaled(const float4& v, float f) {
-  return make_float4(v.x * f, v.y * f, v.z * f, v.w * f);
-}
-
 }  // namespace
 
 // LO: q enters as two f16 parts; not needed where it is of 16 bits and arrives rotated (scaled
@@ -237,27 +208,39 @@ __global__ void __launch_bounds__(32 * Attn4Cfg<HD>::kWarps, 1)
     fence_mbar_init();
   }
   __syncwarp();
+  // Before the previous kernel is waited for: the jobs of the first 32 tiles, and what is read
+  // first is fetched into L2 (prefetches read nothing into the CTA; lines written meanwhile
+  // are updated in L2).
+  Job lane_job = job_at(a, min(w0 + lane, a.total - 1));
+  Job job;  // of the part's first tile
+  job.b = __shfl_sync(0xffffffffu, lane_job.b, 0);
+  job.id = __shfl_sync(0xffffffffu, lane_job.id, 0);
+  job.kvh = __shfl_sync(0xffffffffu, lane_job.kvh, 0);
+  job.row0 = __shfl_sync(0xffffffffu, lane_job.row0, 0);
+  job.rows = __shfl_sync(0xffffffffu, lane_job.rows, 0);
+  job.t0 = __shfl_sync(0xffffffffu, lane_job.t0, 0);
+  job.tiles = __shfl_sync(0xffffffffu, lane_job.tiles, 0);
+  if (w0 < w1) {
+    if (!a.sel && w0 + lane < w1)
+      prefetch_l2(a.cache.block_table +
+                  static_cast<size_t>(a.seqs.seq[lane_job.b]) * a.cache.pages_per_seq +
+                  (w0 + lane - lane_job.t0) * kTile / a.cache.page);
+    const int esize = a.in_dtype == kF32 ? 4 : 2;
+    if (lane < job.rows * HD * esize / 128)
+      prefetch_l2(static_cast<const char*>(a.q) +
+                  (row_offset(a, job, job.row0 + lane * 128 / (HD * esize), HD) * esize +
+                   lane * 128 % (HD * esize)));
+  }
   griddep_wait();
   griddep_launch_dependents();
 
   // -------------------------------------------------------------- the ring --
   // The lanes hold the records of 32 tiles at a time; lane 0 issues.
-  int lane_rec = 0;
-  Job job{};  // of the part's first tile
+  int lane_rec = w0 < w1 ? record_at(a, lane_job, min(w0 + lane, a.total - 1)) : -1;
   auto issue = [&](int i) {
-    if ((i & 31) == 0) {
+    if ((i & 31) == 0 && i > 0) {
       const int x = min(w0 + i + lane, w1 - 1);
-      const Job j = job_at(a, x);
-      lane_rec = record_at(a, j, x);
-      if (i == 0) {
-        job.b = __shfl_sync(0xffffffffu, j.b, 0);
-        job.id = __shfl_sync(0xffffffffu, j.id, 0);
-        job.kvh = __shfl_sync(0xffffffffu, j.kvh, 0);
-        job.row0 = __shfl_sync(0xffffffffu, j.row0, 0);
-        job.rows = __shfl_sync(0xffffffffu, j.rows, 0);
-        job.t0 = __shfl_sync(0xffffffffu, j.t0, 0);
-        job.tiles = __shfl_sync(0xffffffffu, j.tiles, 0);
-      }
+      lane_rec = record_at(a, job_at(a, x), x);
     }
     const int rec = __shfl_sync(0xffffffffu, lane_rec, i & 31);
     if (lane != 0) return;
@@ -273,6 +256,11 @@ __global__ void __launch_bounds__(32 * Attn4Cfg<HD>::kWarps, 1)
   };
   for (int i = 0; i < S && w0 + i < w1; ++i) issue(i);
 
+  // This lane's places in a record: K codes and scales of position g, V's of the pair 2 tq.
+  const int k_at = q4_k_byte(g, 8 * tq, NB);
+  const int v_at = static_cast<int>(kRec.v_codes()) + q4_v_byte(2 * tq, 4 * g, NB);
+  const int ks_at = static_cast<int>(kRec.k_scales()) + 2 * q4_k_scale(g, 0, NB);
+  const int vs_at = static_cast<int>(kRec.v_scales()) + 2 * q4_v_scale(2 * tq, 0, NB);
   uint32_t eights[NB];  // rows b, b + 4, ... of block b's matrix of eights
 #pragma unroll
   for (int b = 0; b < NB; ++b) eights[b] = (g & 3) == b ? 0x00080008u : 0u;
@@ -415,6 +403,11 @@ __global__ void __launch_bounds__(32 * Attn4Cfg<HD>::kWarps, 1)
       const int slices = alive ? min(4, (most - p0 + 15) / 16) : 0;
       // Two times 16 positions at once: independent chains for the scheduler.
       for (int s = 0; s < slices; s += 2) {
+        // of positions 16 s on; 16 positions further lie 256 NB bytes of codes and 32 NB of scales
+        const uint8_t* sk = st + k_at + s * (256 * NB);
+        const uint8_t* sv = st + v_at + s * (256 * NB);
+        const uint8_t* sks = st + ks_at + s * (32 * NB);
+        const uint8_t* svs = st + vs_at + s * (32 * NB);
         // ---- S = K q^T
         float y[2][4];
 #pragma unroll
@@ -422,9 +415,8 @@ __global__ void __launch_bounds__(32 * Attn4Cfg<HD>::kWarps, 1)
           uint32_t kw[2][NB], kd[2][NB / 2];
 #pragma unroll
           for (int r = 0; r < 2; ++r) {
-            const int row = 16 * (s + e) + g + 8 * r;
-            const uint8_t* kp = st + q4_k_byte(row, 8 * tq, NB);
-            const uint8_t* sp = st + kRec.k_scales() + 2 * q4_k_scale(row, 0, NB);
+            const uint8_t* kp = sk + (256 * e + 128 * r) * NB;
+            const uint8_t* sp = sks + (32 * e + 16 * r) * NB;
             if constexpr (NB == 4) {
               const uint4 w = *reinterpret_cast<const uint4*>(kp);
               kw[r][0] = w.x, kw[r][1] = w.y, kw[r][2] = w.z, kw[r][3] = w.w;
@@ -464,8 +456,7 @@ __global__ void __launch_bounds__(32 * Attn4Cfg<HD>::kWarps, 1)
         for (int e = 0; e < 2; ++e)
 #pragma unroll
           for (int r = 0; r < 2; ++r) {
-            const uint8_t* sp =
-                st + kRec.v_scales() + 2 * q4_v_scale(16 * (s + e) + 2 * tq + 8 * r, 0, NB);
+            const uint8_t* sp = svs + (32 * e + 16 * r) * NB;
             if constexpr (NB == 4) {
               const uint4 d = *reinterpret_cast<const uint4*>(sp);
               vd[e][r][0] = d.x, vd[e][r][1] = d.y, vd[e][r][2] = d.z, vd[e][r][3] = d.w;
@@ -562,8 +553,7 @@ __global__ void __launch_bounds__(32 * Attn4Cfg<HD>::kWarps, 1)
           uint32_t vw[2][NB];
 #pragma unroll
           for (int r = 0; r < 2; ++r) {
-            const uint8_t* vp =
-                st + kRec.v_codes() + q4_v_byte(16 * (s + e) + 2 * tq + 8 * r, 4 * g, NB);
+            const uint8_t* vp = sv + (256 * e + 128 * r) * NB;
             if constexpr (NB == 4) {
               const uint4 w = *reinterpret_cast<const uint4*>(vp);
               vw[r][0] = w.x, vw[r][1] = w.y, vw[r][2] = w.z, vw[r][3] = w.w;
@@ -634,67 +624,88 @@ __global__ void __launch_bounds__(32 * Attn4Cfg<HD>::kWarps, 1)
   // ------------------------------------------------------------ joining --
   // (__syncthreads orders the pieces in memory as well, inside the CTA)
   __syncthreads();
-  constexpr int T = 32 * W;
+  // Candidates: the first job of the run, if another CTA began it and it ends in the first
+  // warp's part; then the last job of each warp's part, where its first tile here lies.  The
+  // code stands here once, in loops that are not unrolled: every launch runs it cold.
   auto warp_begin = [&](int i) { return min(c0 + i * a.per_warp, c1); };
-  auto joined = [&](const Job& j, int i0, bool in_place) {
+#pragma unroll 1
+  for (int i = -1; i < W; ++i) {
+    Job j;
+    if (i < 0) {
+      if (c0 >= c1 || last_job[0].t0 <= c0) continue;
+      j = job_at(a, c0);
+      if (j.t0 >= c0) continue;
+    } else {
+      const int b0 = warp_begin(i), b1 = warp_begin(i + 1);
+      if (b0 >= b1) break;
+      j = last_job[i];
+      if ((j.t0 >= b0 && j.t0 + j.tiles <= b1) || (j.t0 < b0 && i > 0)) continue;
+    }
     const int t1 = j.t0 + j.tiles, end = min(t1, c1);
     const bool inside = j.t0 >= c0 && t1 <= c1;
-    const int slot = j.t0 > c0 ? 1 : 0;
-    float* mine = a.cta_parts + static_cast<size_t>(2 * blockIdx.x + slot) * C::kPart;
-    if (!in_place) {
-      int n = 1;
-      while (i0 + n < W && warp_begin(i0 + n) < end) ++n;
-      join_pieces<HD>(
-          n, j.rows, T,
-          [&](int k) -> const float* {
-            const int i = i0 + k;
-            return min(t1, c1) >= warp_begin(i + 1)
-                       ? reinterpret_cast<const float*>(smem + i * C::kRing)
-                       : a.warp_parts + static_cast<size_t>(blockIdx.x * W + i) * C::kPart;
-          },
-          [&](int r, int d, const float4& v, float ref, float sum) {
-            if (inside) {
-              store4(a.out, row_offset(a, j, j.row0 + r, HD) + d, a.out_dtype, scaled(v, 1.f / sum),
-                     a.out_vec != 0);
-            } else {
-              *reinterpret_cast<float4*>(mine + r * HD + d) = v;
-              if (d == 0) *reinterpret_cast<float2*>(mine + 8 * HD + 2 * r) = make_float2(ref, sum);
-            }
-          });
-    }
-    if (inside) return;
-    // The barrier orders every thread's part of the piece before thread 0's count, whose
-    // release makes it visible; the last CTA's acquire sees the others'.
-    const int first = divide(j.t0, a.per_cta), last = divide(t1 - 1, a.per_cta);
-    __syncthreads();
-    if (threadIdx.x == 0) flag[0] = atom_add_acq_rel_gpu(&a.counters[j.id], 1) == last - first;
-    __syncthreads();
-    const bool merge = flag[0] != 0;
-    __syncthreads();
-    if (!merge) return;
-    if (threadIdx.x == 0) a.counters[j.id] = 0;
-    join_pieces<HD>(
-        last - first + 1, j.rows, T,
-        [&](int k) -> const float* {
+    const int first = inside ? 0 : divide(j.t0, a.per_cta);
+    const int last = inside ? 0 : divide(t1 - 1, a.per_cta);
+    float* mine = a.cta_parts + static_cast<size_t>(2 * blockIdx.x + (j.t0 > c0 ? 1 : 0)) * C::kPart;
+    int n = 1;
+    while (i >= 0 && i + n < W && warp_begin(i + n) < end) ++n;
+    // Pieces of the CTA's warps into the output or the CTA's own piece, then, by the last CTA
+    // to arrive, those of all CTAs.  (A job that ends in the first warp's part left its piece in
+    // the CTA's place already.)
+#pragma unroll 1
+    for (int phase = i < 0 ? 1 : 0; phase < 2; ++phase) {
+      if (phase == 1) {
+        // The barrier orders every thread's part of the piece before thread 0's count, whose
+        // release makes it visible; the last CTA's acquire sees the others'.
+        __syncthreads();
+        if (threadIdx.x == 0) {
+          flag[0] = atom_add_acq_rel_gpu(&a.counters[j.id], 1) == last - first;
+          if (flag[0]) a.counters[j.id] = 0;
+        }
+        __syncthreads();
+        const bool merge = flag[0] != 0;
+        __syncthreads();
+        if (!merge) break;
+        n = last - first + 1;
+      }
+      auto part = [&](int k) -> const float* {
+        if (phase == 1) {
           const int c = first + k;
           return a.cta_parts + static_cast<size_t>(2 * c + (j.t0 > c * a.per_cta ? 1 : 0)) * C::kPart;
-        },
-        [&](int r, int d, const float4& v, float, float sum) {
-          store4(a.out, row_offset(a, j, j.row0 + r, HD) + d, a.out_dtype, scaled(v, 1.f / sum),
-                 a.out_vec != 0);
-        });
-  };
-  for (int i = 0; i < W; ++i) {
-    const int b0 = warp_begin(i), b1 = warp_begin(i + 1);
-    if (b0 >= b1) break;
-    const Job lastj = last_job[i];
-    const int t1 = lastj.t0 + lastj.tiles;
-    if (i == 0 && lastj.t0 > b0) {  // the first job of the run, if another CTA began it
-      const Job firstj = job_at(a, b0);
-      if (firstj.t0 < c0) joined(firstj, 0, true);
+        }
+        return end >= warp_begin(i + k + 1)
+                   ? reinterpret_cast<const float*>(smem + (i + k) * C::kRing)
+                   : a.warp_parts + static_cast<size_t>(blockIdx.x * W + i + k) * C::kPart;
+      };
+#pragma unroll 1
+      for (int c = threadIdx.x; c < j.rows * (HD / 4); c += 32 * W) {
+        const int r = c / (HD / 4), d = c % (HD / 4) * 4;
+        float ref = -CUDART_INF_F, sum = 0.f;
+        float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll 4
+        for (int k = 0; k < n; ++k) {
+          const float* p = part(k);
+          const float2 ml = *reinterpret_cast<const float2*>(p + 8 * HD + 2 * r);
+          const float4 v = *reinterpret_cast<const float4*>(p + r * HD + d);
+          const float most = fmaxf(ref, ml.x), base = most == -CUDART_INF_F ? 0.f : most;
+          const float f0 = ex2(ref - base), f1 = ex2(ml.x - base);
+          sum = sum * f0 + ml.y * f1;
+          acc.x = acc.x * f0 + v.x * f1;
+          acc.y = acc.y * f0 + v.y * f1;
+          acc.z = acc.z * f0 + v.z * f1;
+          acc.w = acc.w * f0 + v.w * f1;
+          ref = most;
+        }
+        if (phase == 1 || inside) {
+          const float f = 1.f / sum;
+          store4(a.out, row_offset(a, j, j.row0 + r, HD) + d, a.out_dtype,
+                 make_float4(acc.x * f, acc.y * f, acc.z * f, acc.w * f), a.out_vec != 0);
+        } else {
+          *reinterpret_cast<float4*>(mine + r * HD + d) = acc;
+          if (d == 0) *reinterpret_cast<float2*>(mine + 8 * HD + 2 * r) = make_float2(ref, sum);
+        }
+      }
+      if (inside) break;
     }
-    const bool whole = lastj.t0 >= b0 && t1 <= b1;
-    if (!whole && (lastj.t0 >= b0 || i == 0)) joined(lastj, i, false);
   }
 }
 
