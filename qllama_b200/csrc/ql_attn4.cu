@@ -17,7 +17,7 @@
 // f16's subnormals hold the codes exactly and the matrix instruction takes them as they are, so
 // that a fragment register costs one AND.  The powers of two are folded into q and the output;
 // the 8 that is subtracted from every code enters S as -8 sum q and leaves
-// O with the product of P by a row of eights.  A K scale multiplies the block's partial
+// O with the product of P by rows of eights.  A K scale multiplies the block's partial
 // sums in f32, a V scale the probabilities in f16.
 //
 // Bound by HBM for long caches (2304 bytes of a head_dim 128 cache per 16 positions against
@@ -261,9 +261,7 @@ __global__ void __launch_bounds__(32 * Attn4Cfg<HD>::kWarps, 1)
   const int v_at = static_cast<int>(kRec.v_codes()) + q4_v_byte(2 * tq, 4 * g, NB);
   const int ks_at = static_cast<int>(kRec.k_scales()) + 2 * q4_k_scale(g, 0, NB);
   const int vs_at = static_cast<int>(kRec.v_scales()) + 2 * q4_v_scale(2 * tq, 0, NB);
-  uint32_t eights[NB];  // rows b, b + 4, ... of block b's matrix of eights
-#pragma unroll
-  for (int b = 0; b < NB; ++b) eights[b] = (g & 3) == b ? 0x00080008u : 0u;
+  constexpr uint32_t kEights = 0x00080008u;  // two codes of 8
 
   bool alive = true;
   int x = w0;
@@ -384,11 +382,13 @@ __global__ void __launch_bounds__(32 * Attn4Cfg<HD>::kWarps, 1)
     }
     const int most = a.sel ? all : start + divide(job.row0 + job.rows - 1, a.group) + 1;
 
-    float o[NB][2][4], off[4] = {0.f, 0.f, 0.f, 0.f};
+    float o[NB][2][4], off[NB][4];
 #pragma unroll
-    for (int b = 0; b < NB; ++b)
+    for (int b = 0; b < NB; ++b) {
+      off[b][0] = off[b][1] = off[b][2] = off[b][3] = 0.f;
 #pragma unroll
       for (int u = 0; u < 2; ++u) o[b][u][0] = o[b][u][1] = o[b][u][2] = o[b][u][3] = 0.f;
+    }
     float ref[2] = {0.f, 0.f}, l[2] = {0.f, 0.f}, top = kTop;
     bool fresh = true;
     uint32_t nans = 0;  // of row 2 tq + k: bit 4 k + b, that it sees a value of block b that is NaN
@@ -486,9 +486,8 @@ __global__ void __launch_bounds__(32 * Attn4Cfg<HD>::kWarps, 1)
           }
         // (a scale of 2 or more has the exponent's top bit)
         if (__any_sync(0xffffffffu, over || (any_d & 0x40004000u)) || fresh) {
-          // NaN scales are taken out here and their columns remembered: in the product of P by
-          // a row of eights one would spread to the other blocks, and behind the end of the
-          // sequence, where P is 0, to everything.
+          // NaN scales are taken out here and the blocks and rows that see them remembered:
+          // behind the end of a sequence, or of what a row sees, P is 0 and 0 times NaN is not.
           uint32_t big = 0;  // the largest scale's bits
 #pragma unroll
           for (int e = 0; e < 2; ++e)
@@ -523,15 +522,16 @@ __global__ void __launch_bounds__(32 * Attn4Cfg<HD>::kWarps, 1)
             const float corr = fresh ? 0.f : ex2(ref[k] - next);
             ref[k] = next;
             l[k] *= corr;
-            off[k] *= corr;
-            off[k + 2] *= corr;
 #pragma unroll
-            for (int b = 0; b < NB; ++b)
+            for (int b = 0; b < NB; ++b) {
+              off[b][k] *= corr;
+              off[b][k + 2] = 0.f;  // every row is alike: the lower eight stay unused
 #pragma unroll
               for (int u = 0; u < 2; ++u) {
                 o[b][u][k] *= corr;
                 o[b][u][k + 2] *= corr;
               }
+            }
           }
           top = cap;
           fresh = false;
@@ -565,7 +565,7 @@ __global__ void __launch_bounds__(32 * Attn4Cfg<HD>::kWarps, 1)
 #pragma unroll
           for (int b = 0; b < NB; ++b) {
             const uint32_t b0 = mul2(pt0, vd[e][0][b]), b1 = mul2(pt1, vd[e][1][b]);
-            mma_f16(off, eights[b], eights[b], eights[b], eights[b], b0, b1);
+            mma_f16(off[b], kEights, kEights, kEights, kEights, b0, b1);
 #pragma unroll
             for (int u = 0; u < 2; ++u) {
               const uint32_t u0 = vw[0][b] >> (8 * u), u1 = vw[1][b] >> (8 * u);
@@ -598,16 +598,13 @@ __global__ void __launch_bounds__(32 * Attn4Cfg<HD>::kWarps, 1)
       const bool live = r < job.rows;
       const float f24 = 16777216.f * (whole ? 1.f / l[k] : 1.f);
       const size_t base = whole && live ? row_offset(a, job, job.row0 + r, HD) : 0;
-      float eight[NB];
-#pragma unroll
-      for (int b = 0; b < NB; ++b) eight[b] = __shfl_sync(0xffffffffu, off[k], b * 4 + tq);
       if (!live) continue;
 #pragma unroll
       for (int b = 0; b < NB; ++b) {
-        float4 v = make_float4((o[b][0][k] - eight[b]) * f24,
-                               (o[b][0][k + 2] * 0.0625f - eight[b]) * f24,
-                               (o[b][1][k] - eight[b]) * f24,
-                               (o[b][1][k + 2] * 0.0625f - eight[b]) * f24);
+        float4 v = make_float4((o[b][0][k] - off[b][k]) * f24,
+                               (o[b][0][k + 2] * 0.0625f - off[b][k]) * f24,
+                               (o[b][1][k] - off[b][k]) * f24,
+                               (o[b][1][k + 2] * 0.0625f - off[b][k]) * f24);
         if (nans >> (4 * k + b) & 1u) v.x = v.y = v.z = v.w = CUDART_NAN_F;
         const int d = 32 * b + 4 * g;
         if (whole)
