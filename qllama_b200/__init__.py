@@ -189,6 +189,13 @@ def _buffer(x):
     return x.data_ptr(), (MEM_DEVICE if x.is_cuda else MEM_HOST), x
 
 
+def _positions(positions) -> np.ndarray:
+    """int32 positions; a range is not walked number by number."""
+    if isinstance(positions, range):
+        return np.arange(positions.start, positions.stop, positions.step, dtype=np.int32)
+    return np.ascontiguousarray(positions, dtype=np.int32)
+
+
 class Context:
     """One CUDA device and its stream/workspace (ql_ctx)."""
 
@@ -246,7 +253,7 @@ class KvCache:
             raise QllamaError(ERR_INVALID, "k and v must live in the same memory")
         kd = (ctypes.c_int64 * max(1, len(kk.shape)))(*kk.shape)
         vd = (ctypes.c_int64 * max(1, len(vv.shape)))(*vv.shape)
-        pos = np.ascontiguousarray(positions, dtype=np.int32)
+        pos = _positions(positions)
         _check(load().ql_kv_update(self.ctx._h, self._h, layer, seq, kp, kd, len(kk.shape), vp,
                                    vd, len(vv.shape), _dtype_code(kk),
                                    pos.ctypes.data_as(ctypes.POINTER(ctypes.c_int32)), pos.size,
@@ -254,7 +261,7 @@ class KvCache:
 
     def get(self, layer: int, positions, seq: int = 0):
         """cache.rs:185-229 -- returns f32 numpy arrays [n, num_kv_heads, head_dim]."""
-        pos = np.ascontiguousarray(positions, dtype=np.int32)
+        pos = _positions(positions)
         shape = (pos.size, self.num_kv_heads, self.head_dim)
         k = np.empty(shape, np.float32)
         v = np.empty(shape, np.float32)

@@ -24,72 +24,318 @@ __device__ __forceinline__ int ragged_seq(const RaggedTable& t, int batch, int r
   return lo;
 }
 
-}  // namespace
+// Eight consecutive values as they are in memory, and as f32.
+struct Raw8 {
+  uint4 w[2];  // the second for f32 only
+};
 
-// ---------------------------------------------------------------- append --
-// One warp per row: token r's query heads, then its KV heads.
-__global__ void __launch_bounds__(128) ragged_append_kernel(const __grid_constant__ RaggedAppendArgs a) {
-  const int64_t warp = (static_cast<int64_t>(blockIdx.x) * blockDim.x + threadIdx.x) >> 5;
+__device__ __forceinline__ Raw8 load_raw8(const void* base, size_t i, int dt, bool vec) {
+  Raw8 r;
+  if (vec && dt == kF32) {
+    const uint4* p = reinterpret_cast<const uint4*>(static_cast<const float*>(base) + i);
+    r.w[0] = p[0];
+    r.w[1] = p[1];
+  } else if (vec) {
+    r.w[0] = *reinterpret_cast<const uint4*>(static_cast<const uint16_t*>(base) + i);
+  } else if (dt == kF32) {
+    const uint32_t* p = static_cast<const uint32_t*>(base) + i;
+    r.w[0] = make_uint4(p[0], p[1], p[2], p[3]);
+    r.w[1] = make_uint4(p[4], p[5], p[6], p[7]);
+  } else {
+    const uint16_t* p = static_cast<const uint16_t*>(base) + i;
+    uint32_t x[4];
+#pragma unroll
+    for (int k = 0; k < 4; ++k) x[k] = p[2 * k] | static_cast<uint32_t>(p[2 * k + 1]) << 16;
+    r.w[0] = make_uint4(x[0], x[1], x[2], x[3]);
+  }
+  return r;
+}
+
+__device__ __forceinline__ void floats_of(const Raw8& r, int dt, float (&x)[8]) {
+  if (dt == kF32) {
+    const uint32_t in[8] = {r.w[0].x, r.w[0].y, r.w[0].z, r.w[0].w,
+                            r.w[1].x, r.w[1].y, r.w[1].z, r.w[1].w};
+#pragma unroll
+    for (int k = 0; k < 8; ++k) x[k] = __uint_as_float(in[k]);
+    return;
+  }
+  const uint32_t in[4] = {r.w[0].x, r.w[0].y, r.w[0].z, r.w[0].w};
+#pragma unroll
+  for (int k = 0; k < 4; ++k) {
+    const float2 f = dt == kF16 ? __half22float2(*reinterpret_cast<const __half2*>(&in[k]))
+                                : make_float2(__uint_as_float(in[k] << 16),
+                                              __uint_as_float(in[k] & 0xffff0000u));
+    x[2 * k] = f.x, x[2 * k + 1] = f.y;
+  }
+}
+
+// Eight values of a cache row at dims d .. d + 7; four neighbouring lanes hold a block of 32.
+__device__ __forceinline__ void store_cache8(const CacheView& c, int64_t row, int d, bool v,
+                                             const float (&x)[8], bool live, uint32_t lanes) {
+  if (c.dtype <= kBF16) {
+    if (live) store8(v ? c.v : c.k, static_cast<size_t>(row) * c.hd + d, c.dtype, x, true);
+    return;
+  }
   const int lane = threadIdx.x & 31;
-  const CacheView& c = a.cache;
-  const int heads = a.hq + c.hkv, hd = c.hd;
-  const int64_t r64 = warp / heads;
-  if (r64 >= a.rows.first[a.batch]) return;
-  const int r = static_cast<int>(r64), h = static_cast<int>(warp - r64 * heads);
-  const int b = ragged_seq(a.rows, a.batch, r);
-  const int pos = a.rows.start[b] + r - a.rows.first[b];
-  const double2* rope = a.rope + static_cast<size_t>(pos) * (hd / 2);
-  if (h < a.hq) {
-    const size_t in = static_cast<size_t>(r) * a.q_stride + static_cast<size_t>(h) * hd;
-    const size_t out = (static_cast<size_t>(r) * a.hq + h) * hd;
-    for (int p = lane; p < hd / 2; p += 32) {
-      float y0, y1;
-      rope_pair(load_elem(a.q, in + 2 * p, a.in_dtype), load_elem(a.q, in + 2 * p + 1, a.in_dtype),
-                rope[p], y0, y1);
-      store_elem(a.q_out, out + 2 * p, a.q_out_dtype, y0);
-      store_elem(a.q_out, out + 2 * p + 1, a.q_out_dtype, y1);
+  if (c.dtype == kQ8_0) {  // q8_0_pair's rule
+    float amax = 0.f;
+#pragma unroll
+    for (int k = 0; k < 8; ++k) amax = fmaxf(amax, fabsf(x[k]));
+    amax = fmaxf(amax, __shfl_xor_sync(lanes, amax, 1));
+    amax = fmaxf(amax, __shfl_xor_sync(lanes, amax, 2));
+    const float s = amax / 127.0f, id = s != 0.0f ? 1.0f / s : 0.0f;
+    uint32_t w[2] = {0, 0};
+#pragma unroll
+    for (int k = 0; k < 8; ++k) {
+      const float r = roundf(x[k] * id);
+      w[k / 4] |= (static_cast<uint32_t>(r == r ? static_cast<int>(r) : 0) & 0xffu) << (8 * (k & 3));
+    }
+    if (live) {
+      *reinterpret_cast<uint2*>(static_cast<int8_t*>(v ? c.v : c.k) +
+                                static_cast<size_t>(row) * c.hd + d) = make_uint2(w[0], w[1]);
+      if ((lane & 3) == 0)
+        (v ? c.v_scale : c.k_scale)[static_cast<size_t>(row) * (c.hd / 32) + d / 32] =
+            __half_as_ushort(__float2half_rn(s));
     }
     return;
   }
-  const int kvh = h - a.hq;
-  bool ok;
-  const int64_t dst = cache_row(c, a.rows.seq[b], pos, kvh, a.status, ok);
-  if (!ok) return;
-  append_row(a.k, a.v, a.in_dtype, static_cast<size_t>(r) * a.k_stride + static_cast<size_t>(kvh) * hd,
-             static_cast<size_t>(r) * a.v_stride + static_cast<size_t>(kvh) * hd, rope, c, dst, lane);
+  // Q4_0: the value of largest magnitude, of equal ones the first (in the lower lane)
+  float m = x[0];
+  bool finite = fabsf(x[0]) < CUDART_INF_F;
+#pragma unroll
+  for (int k = 1; k < 8; ++k) {
+    if (fabsf(x[k]) > fabsf(m)) m = x[k];
+    finite = finite && fabsf(x[k]) < CUDART_INF_F;
+  }
+#pragma unroll
+  for (int o = 1; o < 4; o <<= 1) {
+    const float w = __shfl_xor_sync(lanes, m, o);
+    if (fabsf(w) > fabsf(m) || (fabsf(w) == fabsf(m) && (lane & o))) m = w;
+  }
+  finite = (__ballot_sync(lanes, !finite) >> (lane & 28) & 15u) == 0;
+  const uint16_t scale = q4_scale(m, finite);
+  const float s = __half2float(__ushort_as_half(scale)), inv = 1.f / s;
+  uint32_t w = 0x88888888u;
+  if (scale != kHalfNan && s != 0.f) {
+    w = 0;
+#pragma unroll
+    for (int k = 0; k < 8; ++k) w |= q4_code(x[k], s, inv) << (4 * k);
+  }
+  if (!live) return;
+  uint8_t* at = q4_code_at(c, row, d, v);
+  if (v) {  // two lanes' places
+    *reinterpret_cast<uint16_t*>(at) = static_cast<uint16_t>(w);
+    *reinterpret_cast<uint16_t*>(q4_code_at(c, row, d + 4, true)) = static_cast<uint16_t>(w >> 16);
+  } else {
+    *reinterpret_cast<uint32_t*>(at) = w;
+  }
+  if ((lane & 3) == 0) *q4_scale_at(c, row, d / 32, v) = scale;
 }
 
-cudaError_t launch_ragged_append(const RaggedAppendArgs& a, cudaStream_t s) {
-  const int64_t warps = static_cast<int64_t>(a.rows.first[a.batch]) * (a.hq + a.cache.hkv);
-  if (warps == 0) return cudaSuccess;
-  ragged_append_kernel<<<static_cast<unsigned>((warps + 3) / 4), 128, 0, s>>>(a);
+// The converse: eight values of a cache row.
+__device__ __forceinline__ void load_cache8(const CacheView& c, int64_t row, int d, bool v,
+                                            float (&x)[8]) {
+  if (c.dtype <= kBF16) {
+    floats_of(load_raw8(v ? c.v : c.k, static_cast<size_t>(row) * c.hd + d, c.dtype, true), c.dtype, x);
+  } else if (c.dtype == kQ8_0) {
+    const uint2 w = *reinterpret_cast<const uint2*>(static_cast<const int8_t*>(v ? c.v : c.k) +
+                                                    static_cast<size_t>(row) * c.hd + d);
+    const float s = __half2float(__ushort_as_half(
+        (v ? c.v_scale : c.k_scale)[static_cast<size_t>(row) * (c.hd / 32) + d / 32]));
+#pragma unroll
+    for (int k = 0; k < 8; ++k)
+      x[k] = s * static_cast<float>(static_cast<int8_t>((k < 4 ? w.x : w.y) >> (8 * (k & 3))));
+  } else {
+    const uint8_t* at = q4_code_at(c, row, d, v);
+    const uint32_t w =
+        v ? *reinterpret_cast<const uint16_t*>(at) |
+                static_cast<uint32_t>(*reinterpret_cast<const uint16_t*>(q4_code_at(c, row, d + 4, true)))
+                    << 16
+          : *reinterpret_cast<const uint32_t*>(at);
+    const float s = __half2float(__ushort_as_half(*q4_scale_at(c, row, d / 32, v)));
+#pragma unroll
+    for (int k = 0; k < 8; ++k)
+      x[k] = s * static_cast<float>(static_cast<int>(w >> (4 * k) & 15u) - 8);
+  }
+}
+
+constexpr int kRowsPerGroup = 4;
+
+}  // namespace
+
+// ---------------------------------------------------------------- append --
+// A row of HD values takes HD / 8 lanes, eight values each: 16-byte loads, and four lanes a
+// block of 32.  A group of lanes takes up to kRowsPerGroup rows of one token (its query, key and
+// value heads in that order), loaded at once, and fetches the position's angles once for them.
+// HD 0: any head size, one warp per row (key and value rows of a head together).
+// Bound by the bytes for prompts: every row read once and written once.
+template <int HD>
+__global__ void __launch_bounds__(256) ragged_append_kernel(const __grid_constant__ RaggedAppendArgs a) {
+  const int64_t thread = static_cast<int64_t>(blockIdx.x) * blockDim.x + threadIdx.x;
+  const CacheView& c = a.cache;
+  if constexpr (HD == 0) {
+    const int64_t warp = thread >> 5;
+    const int lane = threadIdx.x & 31;
+    const int heads = a.hq + c.hkv, hd = c.hd;
+    const int64_t r64 = warp / heads;
+    if (r64 >= a.rows.first[a.batch]) return;
+    const int r = static_cast<int>(r64), h = static_cast<int>(warp - r64 * heads);
+    const int b = ragged_seq(a.rows, a.batch, r);
+    const int pos = a.rows.start[b] + r - a.rows.first[b];
+    const double2* rope = a.rope ? a.rope + static_cast<size_t>(pos) * (hd / 2) : nullptr;
+    if (h < a.hq) {
+      const size_t in = static_cast<size_t>(r) * a.q_stride + static_cast<size_t>(h) * hd;
+      const size_t out = (static_cast<size_t>(r) * a.hq + h) * hd;
+      for (int p = lane; p < hd / 2; p += 32) {
+        float y0 = load_elem(a.q, in + 2 * p, a.in_dtype);
+        float y1 = load_elem(a.q, in + 2 * p + 1, a.in_dtype);
+        if (rope) rope_pair(y0, y1, rope[p], y0, y1);
+        store_elem(a.q_out, out + 2 * p, a.q_out_dtype, y0);
+        store_elem(a.q_out, out + 2 * p + 1, a.q_out_dtype, y1);
+      }
+      return;
+    }
+    const int kvh = h - a.hq;
+    bool ok;
+    const int64_t dst = cache_row(c, a.rows.seq[b], pos, kvh, a.status, ok);
+    if (!ok) return;
+    append_row(a.k, a.v, a.in_dtype,
+               static_cast<size_t>(r) * a.k_stride + static_cast<size_t>(kvh) * hd,
+               static_cast<size_t>(r) * a.v_stride + static_cast<size_t>(kvh) * hd, rope, c, dst, lane);
+  } else {
+    constexpr int kLanes = HD / 8;
+    const uint32_t lanes =  // of this group, for its shuffles
+        (kLanes == 32 ? 0xffffffffu : (1u << kLanes) - 1) << (threadIdx.x & 31 & ~(kLanes - 1));
+    const int heads = a.hq + 2 * c.hkv;
+    const int chunks = (heads + kRowsPerGroup - 1) / kRowsPerGroup;
+    const int64_t group = thread / kLanes;
+    const int64_t r64 = group / chunks;
+    if (r64 >= a.rows.first[a.batch]) return;
+    const int r = static_cast<int>(r64);
+    const int h0 = static_cast<int>(group - r64 * chunks) * kRowsPerGroup;
+    const int d = static_cast<int>(thread % kLanes) * 8;
+    const int b = ragged_seq(a.rows, a.batch, r);
+    const int pos = a.rows.start[b] + r - a.rows.first[b];
+    Raw8 raw[kRowsPerGroup];
+#pragma unroll
+    for (int i = 0; i < kRowsPerGroup; ++i) {
+      const int h = h0 + i;
+      if (h < a.hq)
+        raw[i] = load_raw8(a.q, static_cast<size_t>(r) * a.q_stride + static_cast<size_t>(h) * HD + d,
+                           a.in_dtype, a.vec & 1);
+      else if (h < a.hq + c.hkv)
+        raw[i] = load_raw8(a.k, static_cast<size_t>(r) * a.k_stride +
+                                    static_cast<size_t>(h - a.hq) * HD + d,
+                           a.in_dtype, a.vec & 2);
+      else if (h < heads)
+        raw[i] = load_raw8(a.v, static_cast<size_t>(r) * a.v_stride +
+                                    static_cast<size_t>(h - a.hq - c.hkv) * HD + d,
+                           a.in_dtype, a.vec & 4);
+    }
+    double2 cs[4];
+    const bool turn = a.rope && h0 < a.hq + c.hkv;
+    if (turn) {
+      const double2* p = a.rope + static_cast<size_t>(pos) * (HD / 2) + d / 2;
+#pragma unroll
+      for (int k = 0; k < 4; ++k) cs[k] = p[k];
+    }
+    bool ok = true;
+    int64_t row0 = 0;
+    if (h0 + kRowsPerGroup > a.hq)
+      row0 = cache_row(c, a.rows.seq[b], pos, 0, a.status, ok);
+#pragma unroll
+    for (int i = 0; i < kRowsPerGroup; ++i) {
+      const int h = h0 + i;
+      if (h >= heads) break;
+      float x[8];
+      floats_of(raw[i], a.in_dtype, x);
+      if (turn && h < a.hq + c.hkv) {
+#pragma unroll
+        for (int k = 0; k < 4; ++k) rope_pair(x[2 * k], x[2 * k + 1], cs[k], x[2 * k], x[2 * k + 1]);
+      }
+      if (h < a.hq) {
+        store8(a.q_out, (static_cast<size_t>(r) * a.hq + h) * HD + d, a.q_out_dtype, x, a.vec & 8);
+      } else {
+        const bool v = h >= a.hq + c.hkv;
+        const int kvh = h - a.hq - (v ? c.hkv : 0);
+        store_cache8(c, row0 + static_cast<int64_t>(kvh) * c.page, d, v, x, ok, lanes);
+      }
+    }
+  }
+}
+
+cudaError_t launch_ragged_append(const RaggedAppendArgs& a_in, cudaStream_t s) {
+  RaggedAppendArgs a = a_in;
+  const int64_t tokens = a.rows.first[a.batch];
+  if (tokens == 0) return cudaSuccess;
+  const int hd = a.cache.hd;
+  // 16-byte accesses where the base and every row allow them
+  const int64_t per = a.in_dtype == kF32 ? 4 : 8;
+  auto fits = [](const void* p) { return reinterpret_cast<uintptr_t>(p) % 16 == 0; };
+  a.vec = (fits(a.q) && a.q_stride % per == 0 ? 1 : 0) | (fits(a.k) && a.k_stride % per == 0 ? 2 : 0) |
+          (fits(a.v) && a.v_stride % per == 0 ? 4 : 0) | (fits(a.q_out) ? 8 : 0);
+  if (hd != 64 && hd != 128) {
+    const int64_t threads = tokens * (a.hq + a.cache.hkv) * 32;
+    ragged_append_kernel<0><<<static_cast<unsigned>((threads + 255) / 256), 256, 0, s>>>(a);
+    return cudaGetLastError();
+  }
+  const int chunks = (a.hq + 2 * a.cache.hkv + kRowsPerGroup - 1) / kRowsPerGroup;
+  const int64_t threads = tokens * chunks * (hd / 8);
+  const unsigned blocks = static_cast<unsigned>((threads + 255) / 256);
+  if (hd == 64)
+    ragged_append_kernel<64><<<blocks, 256, 0, s>>>(a);
+  else
+    ragged_append_kernel<128><<<blocks, 256, 0, s>>>(a);
   return cudaGetLastError();
 }
 
 // ------------------------------------------------------------------ read --
-// One warp per (token, KV head).
-__global__ void __launch_bounds__(128) ragged_read_kernel(const __grid_constant__ RaggedReadArgs a) {
-  const int64_t warp = (static_cast<int64_t>(blockIdx.x) * blockDim.x + threadIdx.x) >> 5;
-  const int lane = threadIdx.x & 31;
+// As the append: a row's K and V by HD / 8 lanes; HD 0: one warp per (token, KV head).
+template <int HD>
+__global__ void __launch_bounds__(256) ragged_read_kernel(const __grid_constant__ RaggedReadArgs a) {
+  constexpr int kLanes = HD == 0 ? 32 : HD / 8;
+  const int64_t thread = static_cast<int64_t>(blockIdx.x) * blockDim.x + threadIdx.x;
   const CacheView& c = a.cache;
-  const int64_t r64 = warp / c.hkv;
+  const int64_t unit = thread / kLanes, r64 = unit / c.hkv;
   if (r64 >= a.rows.first[a.batch]) return;
-  const int r = static_cast<int>(r64), h = static_cast<int>(warp - r64 * c.hkv);
+  const int r = static_cast<int>(r64), h = static_cast<int>(unit - r64 * c.hkv);
   const int b = ragged_seq(a.rows, a.batch, r);
   bool ok;
   const int64_t row = cache_row(c, a.rows.seq[b], a.rows.start[b] + r - a.rows.first[b], h,
                                 a.status, ok);
-  const size_t o = static_cast<size_t>(warp) * c.hd;
-  for (int d = lane; d < c.hd; d += 32) {
-    store_elem(a.k_out, o + d, a.out_dtype, ok ? cache_value(c, false, row, d) : 0.f);
-    store_elem(a.v_out, o + d, a.out_dtype, ok ? cache_value(c, true, row, d) : 0.f);
+  const size_t o = static_cast<size_t>(unit) * c.hd;
+  if constexpr (HD == 0) {
+    for (int d = threadIdx.x & 31; d < c.hd; d += 32) {
+      store_elem(a.k_out, o + d, a.out_dtype, ok ? cache_value(c, false, row, d) : 0.f);
+      store_elem(a.v_out, o + d, a.out_dtype, ok ? cache_value(c, true, row, d) : 0.f);
+    }
+  } else {
+    const int d = static_cast<int>(thread % kLanes) * 8;
+    float k[8] = {}, v[8] = {};
+    if (ok) {
+      load_cache8(c, row, d, false, k);
+      load_cache8(c, row, d, true, v);
+    }
+    store8(a.k_out, o + d, a.out_dtype, k, a.vec & 1);
+    store8(a.v_out, o + d, a.out_dtype, v, a.vec & 2);
   }
 }
 
-cudaError_t launch_ragged_read(const RaggedReadArgs& a, cudaStream_t s) {
-  const int64_t warps = static_cast<int64_t>(a.rows.first[a.batch]) * a.cache.hkv;
-  if (warps == 0) return cudaSuccess;
-  ragged_read_kernel<<<static_cast<unsigned>((warps + 3) / 4), 128, 0, s>>>(a);
+cudaError_t launch_ragged_read(const RaggedReadArgs& a_in, cudaStream_t s) {
+  RaggedReadArgs a = a_in;
+  const int64_t rows = static_cast<int64_t>(a.rows.first[a.batch]) * a.cache.hkv;
+  if (rows == 0) return cudaSuccess;
+  a.vec = (reinterpret_cast<uintptr_t>(a.k_out) % 16 == 0 ? 1 : 0) |
+          (reinterpret_cast<uintptr_t>(a.v_out) % 16 == 0 ? 2 : 0);
+  const int hd = a.cache.hd;
+  const int64_t threads = rows * (hd == 64 || hd == 128 ? hd / 8 : 32);
+  const unsigned blocks = static_cast<unsigned>((threads + 255) / 256);
+  if (hd == 64)
+    ragged_read_kernel<64><<<blocks, 256, 0, s>>>(a);
+  else if (hd == 128)
+    ragged_read_kernel<128><<<blocks, 256, 0, s>>>(a);
+  else
+    ragged_read_kernel<0><<<blocks, 256, 0, s>>>(a);
   return cudaGetLastError();
 }
 

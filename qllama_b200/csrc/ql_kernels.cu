@@ -54,6 +54,24 @@ __global__ void __launch_bounds__(128) append_kernel(const __grid_constant__ App
 }
 
 cudaError_t launch_append(const AppendArgs& a, cudaStream_t s) {
+  if (a.cache.dtype == kQ4_0) {  // rows of one length for every sequence
+    RaggedAppendArgs r{};
+    r.k = a.k;
+    r.v = a.v;
+    r.k_stride = r.v_stride = static_cast<int64_t>(a.cache.hkv) * a.cache.hd;
+    r.in_dtype = a.in_dtype;
+    r.batch = a.batch;
+    r.rope = a.rope;
+    r.cache = a.cache;
+    r.status = a.status;
+    for (int b = 0; b < a.batch; ++b) {
+      r.rows.seq[b] = a.seqs.seq[b];
+      r.rows.start[b] = a.seqs.start[b];
+      r.rows.first[b] = b * a.new_len;
+    }
+    r.rows.first[a.batch] = a.batch * a.new_len;
+    return launch_ragged_append(r, s);
+  }
   const bool tokens = a.cache.dtype <= kBF16 && (a.cache.hd == 64 || a.cache.hd == 128);
   const int warps = a.batch * a.new_len * (tokens ? 1 : a.cache.hkv);
   if (warps == 0) return cudaSuccess;

@@ -215,11 +215,12 @@ struct RaggedAppendArgs {
   const void* v;
   void* q_out;    // [tokens][hq][hd]
   int64_t q_stride, k_stride, v_stride;  // elements from token to token
+  int32_t vec;    // set by the launch: which of q, k, v and q_out allow 16-byte accesses
   int32_t in_dtype;
   int32_t q_out_dtype;
   int32_t hq;
   int32_t batch;
-  const double2* rope;  // [max_seq][hd/2] (cos, sin)
+  const double2* rope;  // [max_seq][hd/2] (cos, sin) or nullptr
   CacheView cache;
   uint32_t* status;
   RaggedTable rows;
@@ -230,6 +231,7 @@ struct RaggedReadArgs {
   void* k_out;  // [tokens][hkv][hd]
   void* v_out;
   int32_t out_dtype;
+  int32_t vec;  // set by the launch: which of k_out and v_out allow 16-byte stores
   int32_t batch;
   CacheView cache;
   uint32_t* status;
