@@ -24,6 +24,7 @@ from __future__ import annotations
 
 import ctypes
 import os
+from array import array
 
 import numpy as np
 
@@ -86,9 +87,8 @@ class AttnArgs(ctypes.Structure):
 
 class AppendArgs(ctypes.Structure):
     _fields_ = [("layer_idx", ctypes.c_int32), ("batch", ctypes.c_int32),
-                ("seq_ids", ctypes.POINTER(ctypes.c_int32)),
-                ("start_pos", ctypes.POINTER(ctypes.c_int64)),
-                ("new_len", ctypes.POINTER(ctypes.c_int32)), ("num_heads", ctypes.c_int32),
+                ("seq_ids", ctypes.c_void_p), ("start_pos", ctypes.c_void_p),
+                ("new_len", ctypes.c_void_p), ("num_heads", ctypes.c_int32),
                 ("num_kv_heads", ctypes.c_int32), ("head_dim", ctypes.c_int32),
                 ("rope_theta", ctypes.c_float), ("in_dtype", ctypes.c_int32),
                 ("q_out_dtype", ctypes.c_int32), ("q_stride", ctypes.c_int64),
@@ -196,6 +196,26 @@ def _positions(positions) -> np.ndarray:
     return np.ascontiguousarray(positions, dtype=np.int32)
 
 
+_identity = {}  # batch -> the sequences 0 .. batch - 1
+
+
+def _ragged(seq_ids, start_pos, lens):
+    """(sequences, tokens, the addresses of seq_ids, start_pos and lens, what keeps them)."""
+    batch = len(lens)
+    if seq_ids is None:
+        seqs = _identity.get(batch)
+        if seqs is None:
+            seqs = _identity[batch] = array("i", range(batch))
+    else:
+        seqs = array("i", seq_ids)
+    starts, counts = array("q", start_pos), array("i", lens)
+    if len(starts) != batch or len(seqs) != batch:
+        raise QllamaError(ERR_INVALID, f"{batch} length(s) but {len(starts)} position(s) and "
+                                       f"{len(seqs)} sequence(s)")
+    return batch, sum(lens), (seqs.buffer_info()[0], starts.buffer_info()[0],
+                              counts.buffer_info()[0]), (seqs, starts, counts)
+
+
 class Context:
     """One CUDA device and its stream/workspace (ql_ctx)."""
 
@@ -285,8 +305,9 @@ class KvCache:
         n = len(seq)
         if len(new_len) != n:
             raise QllamaError(ERR_INVALID, f"{n} sequence(s) but {len(new_len)} length(s)")
-        _check(load().ql_kv_truncate_batch(self._h, n, (ctypes.c_int32 * n)(*seq),
-                                           (ctypes.c_int64 * n)(*new_len)))
+        seqs, lens = array("i", seq), array("q", new_len)
+        _check(load().ql_kv_truncate_batch(self._h, n, seqs.buffer_info()[0],
+                                           lens.buffer_info()[0]))
 
     def append(self, layer: int, k, v, start_pos, new_len, rope_theta: float, seq_ids=None,
                q=None, q_out=None):
@@ -301,37 +322,40 @@ class KvCache:
         from . import model as m
 
         L = m._L or m._start()
-        ctx, shape = self.ctx, (self.num_kv_heads, self.head_dim)
-        batch, total, rows = self._ragged(seq_ids, start_pos, new_len)
+        ctx, hkv, hd, dtype = self.ctx, self.num_kv_heads, self.head_dim, k.dtype
         dev = ctx.device
+        batch, total, rows, keep = _ragged(seq_ids, start_pos, new_len)
 
         def tokens(t, name, heads):
-            if t.dim() != 3 or t.shape[0] != total or t.shape[2] != shape[1] or \
-                    (heads and t.shape[1] != heads):
-                raise m._invalid(f"{name} has shape {tuple(t.shape)}, expected [{total}, "
-                                 f"{heads or 'heads'}, {shape[1]}]")
-            if t.dtype is not k.dtype:
+            """(stride, pointer) of a tensor of one row a token."""
+            shape = t.shape
+            if len(shape) != 3 or shape[0] != total or shape[1] != heads or shape[2] != hd:
+                raise m._invalid(f"{name} has shape {tuple(shape)}, expected [{total}, {heads}, "
+                                 f"{hd}]")
+            if t.dtype is not dtype:
                 raise m._invalid(f"{name} must have k's type")
-            width = t.shape[1] * t.shape[2]
-            if t.is_contiguous() or total < 2 and t[:1].is_contiguous():
+            if t.is_contiguous():
                 return 0, m._on(dev, t, name)
-            if t.stride(2) != 1 or t.stride(0) < width or \
-                    (t.shape[1] > 1 and t.stride(1) != t.shape[2]):
+            row, head, one = t.stride()
+            if (one != 1 and hd > 1) or (head != hd and heads > 1) or (
+                    total > 1 and row < heads * hd):
                 raise m._invalid(f"{name} must have a token's heads contiguous")
-            return t.stride(0), m._on(dev, t, name)
+            return row if total > 1 else 0, m._on(dev, t, name)
 
         dt = m._float_code(k, "k")
-        ks, kp = tokens(k, "k", shape[0])
-        vs, vp = tokens(v, "v", shape[0])
+        ks, kp = tokens(k, "k", hkv)
+        vs, vp = tokens(v, "v", hkv)
         hq, qs, qp, op, od = 0, 0, None, None, F32
         if q is not None:
-            qs, qp = tokens(q, "q", 0)
+            if q.dim() != 3:
+                raise m._invalid(f"q has shape {tuple(q.shape)}, expected [{total}, heads, {hd}]")
             hq = q.shape[1]
-            q_out = m._output(ctx, q_out, q.shape, q.dtype if q_out is None else q_out.dtype,
+            qs, qp = tokens(q, "q", hq)
+            q_out = m._output(ctx, q_out, q.shape, dtype if q_out is None else q_out.dtype,
                               "q_out")
             od, op = m._float_code(q_out, "q_out"), m._on(dev, q_out, "q_out")
-        args = AppendArgs(layer, batch, *rows, hq, *shape, rope_theta, dt, od, qs, ks, vs, qp, kp,
-                          vp, op)
+        args = AppendArgs(layer, batch, *rows, hq, hkv, hd, rope_theta, dt, od, qs, ks, vs, qp,
+                          kp, vp, op)
         side = m._fork(ctx)
         rc = L.ql_kv_append(ctx._h, self._h, ctypes.byref(args))
         if rc:
@@ -349,7 +373,7 @@ class KvCache:
 
         L = m._L or m._start()
         ctx = self.ctx
-        batch, total, rows = self._ragged(seq_ids, start_pos, lens)
+        batch, total, rows, keep = _ragged(seq_ids, start_pos, lens)
         shape = (total, self.num_kv_heads, self.head_dim)
         k, v = out if out is not None else (None, None)
         if out is None:
@@ -366,19 +390,6 @@ class KvCache:
         if side is not None:
             m._join(ctx, side)
         return k, v
-
-    @staticmethod
-    def _ragged(seq_ids, start_pos, lens):
-        """(sequences, tokens, (seq_ids, start_pos, lens) as C arrays)."""
-        batch = len(lens)
-        if seq_ids is None:
-            seq_ids = range(batch)
-        if len(start_pos) != batch or len(seq_ids) != batch:
-            raise QllamaError(ERR_INVALID, f"{batch} length(s) but {len(start_pos)} position(s) "
-                                           f"and {len(seq_ids)} sequence(s)")
-        return batch, int(sum(lens)), ((ctypes.c_int32 * batch)(*seq_ids),
-                                       (ctypes.c_int64 * batch)(*start_pos),
-                                       (ctypes.c_int32 * batch)(*lens))
 
     def seq_len(self, seq: int = 0) -> int:
         out = ctypes.c_int64()

@@ -1273,15 +1273,8 @@ static int attn_forward_impl(ql_ctx* c, ql_kv* kv, const ql_attn_args* a,
   size_t a4_cta = 0, a4_warp = 0;
   if (q4_decode) {
     a4.units = sparse ? n * ((group + 7) / 8) : (n * group + 7) / 8;
-    int64_t total = 0;
-    for (int b = 0; b < a->batch; ++b) {
-      a4.first[b] = static_cast<int32_t>(total);
-      total += static_cast<int64_t>(row_tiles[b]) * hkv * a4.units;
-      if (total > (1 << 30))
-        return fail(QL_ERR_UNSUPPORTED, "more than %d tiles of keys in one call", 1 << 30);
-    }
-    a4.total = static_cast<int32_t>(total);
-    ql::attn4_plan(hd, c->num_sms, &a4, &a4_cta, &a4_warp);
+    if (ql::attn4_plan(hd, c->num_sms, row_tiles, a->batch, hkv * a4.units, &a4, &a4_cta, &a4_warp))
+      return fail(QL_ERR_UNSUPPORTED, "more than %d tiles of keys in one call", 1 << 30);
   }
   int tps = max_tiles, max_splits = 1;
   // Too few (token, KV head) jobs to fill half the SMs: the wide kernel, whose
@@ -1499,7 +1492,8 @@ static int attn_forward_impl(ql_ctx* c, ql_kv* kv, const ql_attn_args* a,
     se.first = sparse->first;
     se.last = sparse->last;
     se.max_blocks = max_blocks;
-    se.q_vec = aligned_to(q, a->in_dtype == QL_F32 ? 16 : 8);
+    se.q_vec = aligned_to(q, 16);
+    se.num_sms = c->num_sms;
     se.counters = c->counters;  // zero again when the attention starts
     se.score = reinterpret_cast<double*>(w + o_sc);
     se.bounds = kv->bounds[layer];

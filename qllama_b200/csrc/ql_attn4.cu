@@ -47,12 +47,12 @@ struct Attn4Cfg {
   static constexpr int kNb = HD / 32;
   static constexpr int kWarps = 12;
   static constexpr int kRecord = 72 * HD;
-  static constexpr int kStages = HD == 128 ? 2 : 4;
-  static constexpr int kRing = kStages * kRecord;  // of one warp
-  static constexpr int kPart = 8 * HD + 16;        // floats of a piece: rows, then (reference, sum)
-  static constexpr size_t kSmem = 128 + static_cast<size_t>(kWarps) * (kRing + kStages * 8) +
-                                  kWarps * 32 + 16;
-  static_assert(kPart * 4 <= kRing, "a warp's last piece takes its ring's place");
+  static constexpr int kStages = HD == 128 ? 2 : 4;  // of a warp's ring, at most
+  static constexpr int kPart = 8 * HD + 16;  // floats of a piece: rows, then (reference, sum)
+  static constexpr size_t smem(int stages) {
+    return 128 + static_cast<size_t>(kWarps) * stages * (kRecord + 8) + kWarps * 32 + 16;
+  }
+  static_assert(kPart * 4 <= kRecord, "a warp's last piece takes its ring's place");
 };
 
 // D = A B
@@ -98,7 +98,7 @@ __device__ __forceinline__ float half_of(const uint32_t& w, bool high) {
 // A job of the list: its sequence, KV head and query rows, and its tiles.
 struct Job {
   int b, id, kvh, row0, rows;
-  int t0, tiles;  // its first place in the list of tiles, and their number
+  int t0, tiles;  // its first place in the list of tiles, and their number there
 };
 
 // a / b for 0 <= a < 2^30 and a quotient below 2^22, where the product with the reciprocal is at
@@ -112,9 +112,12 @@ __device__ __forceinline__ int divide(int a, int b) {
   return q;
 }
 
+// Places that a job of sequence b takes in the list: its tiles, or (aligned) as many as its CTAs
+// take, the last ones empty.
 __device__ __forceinline__ int seq_tiles(const Attn4Args& a, int b) {
   const int end = a.seqs.start[b] + a.new_len;
-  return a.sel ? sel_blocks(end - 1, a.sel_max) : (end + kTile - 1) / kTile;
+  const int n = a.sel ? sel_blocks(end - 1, a.sel_max) : (end + kTile - 1) / kTile;
+  return a.aligned ? divide(n + a.per_cta - 1, a.per_cta) * a.per_cta : n;
 }
 
 // Job k of sequence b.
@@ -154,7 +157,8 @@ __device__ __forceinline__ Job next_job(const Attn4Args& a, const Job& j) {
   return k < per ? job_of(a, j.b, k, j.tiles) : job_of(a, j.b + 1, 0, seq_tiles(a, j.b + 1));
 }
 
-// The record that holds tile x of the list, of job j; -1 for a list's place behind its blocks.
+// The record that holds tile x of the list, of job j; -1 for a place behind the job's tiles (or
+// behind a selection's blocks).
 __device__ __forceinline__ int record_at(const Attn4Args& a, const Job& j, int x) {
   const CacheView& c = a.cache;
   int tile = x - j.t0;
@@ -162,6 +166,8 @@ __device__ __forceinline__ int record_at(const Attn4Args& a, const Job& j, int x
     const int t = divide(j.row0, a.group);
     if (tile >= sel_blocks(a.seqs.start[j.b] + t, a.sel_max)) return -1;
     tile = a.sel[(static_cast<size_t>(j.b * a.new_len + t) * c.hkv + j.kvh) * a.sel_max + tile];
+  } else if (tile * kTile >= a.seqs.start[j.b] + a.new_len) {
+    return -1;
   }
   const int per = c.page / kTile;
   const int in_seq = per == 1 ? tile : tile / per;
@@ -188,17 +194,18 @@ template <int HD, bool LO>
 __global__ void __launch_bounds__(32 * Attn4Cfg<HD>::kWarps, 1)
     attn4_kernel(const __grid_constant__ Attn4Args a) {
   using C = Attn4Cfg<HD>;
-  constexpr int NB = C::kNb, W = C::kWarps, S = C::kStages;
+  constexpr int NB = C::kNb, W = C::kWarps;
+  const int S = a.stages, ring_bytes = S * C::kRecord;
   constexpr Q4Record kRec{HD};
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>(
       (reinterpret_cast<uintptr_t>(smem_raw) + 127) & ~static_cast<uintptr_t>(127));
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int g = lane >> 2, tq = lane & 3;
-  uint8_t* ring = smem + warp * C::kRing;
-  uint64_t* full = reinterpret_cast<uint64_t*>(smem + W * C::kRing) + warp * S;
+  uint8_t* ring = smem + warp * ring_bytes;
+  uint64_t* full = reinterpret_cast<uint64_t*>(smem + W * ring_bytes) + warp * S;
   // the last job of every warp's part, for the joining
-  Job* last_job = reinterpret_cast<Job*>(smem + W * C::kRing + W * S * 8);
+  Job* last_job = reinterpret_cast<Job*>(smem + W * ring_bytes + W * S * 8);
   int* flag = reinterpret_cast<int*>(last_job + W);
 
   const int c0 = blockIdx.x * a.per_cta, c1 = min(c0 + a.per_cta, a.total);
@@ -237,24 +244,24 @@ __global__ void __launch_bounds__(32 * Attn4Cfg<HD>::kWarps, 1)
   // -------------------------------------------------------------- the ring --
   // The lanes hold the records of 32 tiles at a time; lane 0 issues.
   int lane_rec = w0 < w1 ? record_at(a, lane_job, min(w0 + lane, a.total - 1)) : -1;
-  auto issue = [&](int i) {
+  auto issue = [&](int i, int stage) {
     if ((i & 31) == 0 && i > 0) {
       const int x = min(w0 + i + lane, w1 - 1);
       lane_rec = record_at(a, job_at(a, x), x);
     }
     const int rec = __shfl_sync(0xffffffffu, lane_rec, i & 31);
     if (lane != 0) return;
-    uint64_t* bar = &full[i % S];
+    uint64_t* bar = &full[stage];
     if (rec < 0) {
       mbar_arrive(bar);
     } else {
       mbar_arrive_expect_tx(bar, C::kRecord);
-      bulk_load(ring + (i % S) * C::kRecord,
+      bulk_load(ring + stage * C::kRecord,
                 static_cast<const uint8_t*>(a.cache.k) + static_cast<size_t>(rec) * kRec.bytes(),
                 C::kRecord, bar);
     }
   };
-  for (int i = 0; i < S && w0 + i < w1; ++i) issue(i);
+  for (int i = 0; i < S && w0 + i < w1; ++i) issue(i, i);
 
   // This lane's places in a record: K codes and scales of position g, V's of the pair 2 tq.
   const int k_at = q4_k_byte(g, 8 * tq, NB);
@@ -264,6 +271,7 @@ __global__ void __launch_bounds__(32 * Attn4Cfg<HD>::kWarps, 1)
   constexpr uint32_t kEights = 0x00080008u;  // two codes of 8
 
   bool alive = true;
+  int stage = 0, phase = 0;  // of the next tile
   int x = w0;
   while (x < w1) {
     if (x > w0) job = next_job(a, job);
@@ -395,9 +403,8 @@ __global__ void __launch_bounds__(32 * Attn4Cfg<HD>::kWarps, 1)
 
     // --------------------------------------------------------- the tiles --
     for (; x < seg1; ++x) {
-      const int i = x - w0;
-      if (alive) alive = !__any_sync(0xffffffffu, !mbar_wait(&full[i % S], (i / S) & 1, a.status));
-      const uint8_t* st = ring + (i % S) * C::kRecord;
+      if (alive) alive = !__any_sync(0xffffffffu, !mbar_wait(&full[stage], phase, a.status));
+      const uint8_t* st = ring + stage * C::kRecord;
       const int p0 = (x - job.t0) * kTile;
       const bool tail = p0 + kTile > all;
       const int slices = alive ? min(4, (most - p0 + 15) / 16) : 0;
@@ -576,7 +583,11 @@ __global__ void __launch_bounds__(32 * Attn4Cfg<HD>::kWarps, 1)
         }
       }
       __syncwarp();  // the stage is free
-      if (alive && x + S < w1) issue(i + S);
+      if (alive && x + S < w1) issue(x + S - w0, stage);
+      if (++stage == S) {
+        stage = 0;
+        phase ^= 1;
+      }
     }
 
     // ------------------------------------------------- the end of a piece --
@@ -586,6 +597,9 @@ __global__ void __launch_bounds__(32 * Attn4Cfg<HD>::kWarps, 1)
       l[k] += __shfl_xor_sync(0xffffffffu, l[k], 8);
       l[k] += __shfl_xor_sync(0xffffffffu, l[k], 16);
     }
+#pragma unroll
+    for (int k = 0; k < 2; ++k)
+      if (l[k] == 0.f) ref[k] = -CUDART_INF_F;  // the row sees none of these tiles
     const bool whole = job.t0 >= w0 && job.t0 + job.tiles <= w1;
     // A piece that ends the warp's part goes into its ring; an earlier one (of a job that
     // other warps began) into memory: the CTA's own piece of it if no other warp here has one.
@@ -621,88 +635,87 @@ __global__ void __launch_bounds__(32 * Attn4Cfg<HD>::kWarps, 1)
   // ------------------------------------------------------------ joining --
   // (__syncthreads orders the pieces in memory as well, inside the CTA)
   __syncthreads();
-  // Candidates: the first job of the run, if another CTA began it and it ends in the first
-  // warp's part; then the last job of each warp's part, where its first tile here lies.  The
-  // code stands here once, in loops that are not unrolled: every launch runs it cold.
+  // The first job of the run, if another CTA began it and it ends in the first warp's part; then
+  // the last job of each warp's part, where its first tile here lies.  (Loops that are not
+  // unrolled: every launch runs this code cold.)
   auto warp_begin = [&](int i) { return min(c0 + i * a.per_warp, c1); };
+  // Sums the n pieces part(0) .. of job j into the output, or into the piece `into`.
+  auto join = [&](const Job& j, int n, float* into, auto part) {
 #pragma unroll 1
-  for (int i = -1; i < W; ++i) {
-    Job j;
-    if (i < 0) {
-      if (c0 >= c1 || last_job[0].t0 <= c0) continue;
-      j = job_at(a, c0);
-      if (j.t0 >= c0) continue;
-    } else {
-      const int b0 = warp_begin(i), b1 = warp_begin(i + 1);
-      if (b0 >= b1) break;
-      j = last_job[i];
-      if ((j.t0 >= b0 && j.t0 + j.tiles <= b1) || (j.t0 < b0 && i > 0)) continue;
-    }
-    const int t1 = j.t0 + j.tiles, end = min(t1, c1);
-    const bool inside = j.t0 >= c0 && t1 <= c1;
-    const int first = inside ? 0 : divide(j.t0, a.per_cta);
-    const int last = inside ? 0 : divide(t1 - 1, a.per_cta);
-    float* mine = a.cta_parts + static_cast<size_t>(2 * blockIdx.x + (j.t0 > c0 ? 1 : 0)) * C::kPart;
-    int n = 1;
-    while (i >= 0 && i + n < W && warp_begin(i + n) < end) ++n;
-    // Pieces of the CTA's warps into the output or the CTA's own piece, then, by the last CTA
-    // to arrive, those of all CTAs.  (A job that ends in the first warp's part left its piece in
-    // the CTA's place already.)
-#pragma unroll 1
-    for (int phase = i < 0 ? 1 : 0; phase < 2; ++phase) {
-      if (phase == 1) {
-        // The barrier orders every thread's part of the piece before thread 0's count, whose
-        // release makes it visible; the last CTA's acquire sees the others'.
-        __syncthreads();
-        if (threadIdx.x == 0) {
-          flag[0] = atom_add_acq_rel_gpu(&a.counters[j.id], 1) == last - first;
-          if (flag[0]) a.counters[j.id] = 0;
-        }
-        __syncthreads();
-        const bool merge = flag[0] != 0;
-        __syncthreads();
-        if (!merge) break;
-        n = last - first + 1;
-      }
-      auto part = [&](int k) -> const float* {
-        if (phase == 1) {
-          const int c = first + k;
-          return a.cta_parts + static_cast<size_t>(2 * c + (j.t0 > c * a.per_cta ? 1 : 0)) * C::kPart;
-        }
-        return end >= warp_begin(i + k + 1)
-                   ? reinterpret_cast<const float*>(smem + (i + k) * C::kRing)
-                   : a.warp_parts + static_cast<size_t>(blockIdx.x * W + i + k) * C::kPart;
-      };
-#pragma unroll 1
-      for (int c = threadIdx.x; c < j.rows * (HD / 4); c += 32 * W) {
-        const int r = c / (HD / 4), d = c % (HD / 4) * 4;
-        float ref = -CUDART_INF_F, sum = 0.f;
-        float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
+    for (int c = threadIdx.x; c < j.rows * (HD / 4); c += 32 * W) {
+      const int r = c / (HD / 4), d = c % (HD / 4) * 4;
+      float ref = -CUDART_INF_F, sum = 0.f;
+      float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
 #pragma unroll 4
-        for (int k = 0; k < n; ++k) {
-          const float* p = part(k);
-          const float2 ml = *reinterpret_cast<const float2*>(p + 8 * HD + 2 * r);
-          const float4 v = *reinterpret_cast<const float4*>(p + r * HD + d);
-          const float most = fmaxf(ref, ml.x), base = most == -CUDART_INF_F ? 0.f : most;
-          const float f0 = ex2(ref - base), f1 = ex2(ml.x - base);
-          sum = sum * f0 + ml.y * f1;
-          acc.x = acc.x * f0 + v.x * f1;
-          acc.y = acc.y * f0 + v.y * f1;
-          acc.z = acc.z * f0 + v.z * f1;
-          acc.w = acc.w * f0 + v.w * f1;
-          ref = most;
-        }
-        if (phase == 1 || inside) {
-          const float f = 1.f / sum;
-          store4(a.out, row_offset(a, j, j.row0 + r, HD) + d, a.out_dtype,
-                 make_float4(acc.x * f, acc.y * f, acc.z * f, acc.w * f), a.out_vec != 0);
-        } else {
-          *reinterpret_cast<float4*>(mine + r * HD + d) = acc;
-          if (d == 0) *reinterpret_cast<float2*>(mine + 8 * HD + 2 * r) = make_float2(ref, sum);
-        }
+      for (int k = 0; k < n; ++k) {
+        const float* p = part(k);
+        const float2 ml = *reinterpret_cast<const float2*>(p + 8 * HD + 2 * r);
+        const float4 v = *reinterpret_cast<const float4*>(p + r * HD + d);
+        const float most = fmaxf(ref, ml.x), base = most == -CUDART_INF_F ? 0.f : most;
+        const float f0 = ex2(ref - base), f1 = ex2(ml.x - base);
+        sum = sum * f0 + ml.y * f1;
+        acc.x = acc.x * f0 + v.x * f1;
+        acc.y = acc.y * f0 + v.y * f1;
+        acc.z = acc.z * f0 + v.z * f1;
+        acc.w = acc.w * f0 + v.w * f1;
+        ref = most;
       }
-      if (inside) break;
+      if (into) {
+        *reinterpret_cast<float4*>(into + r * HD + d) = acc;
+        if (d == 0) *reinterpret_cast<float2*>(into + 8 * HD + 2 * r) = make_float2(ref, sum);
+      } else {
+        const float f = 1.f / sum;
+        store4(a.out, row_offset(a, j, j.row0 + r, HD) + d, a.out_dtype,
+               make_float4(acc.x * f, acc.y * f, acc.z * f, acc.w * f), a.out_vec != 0);
+      }
     }
+  };
+  Job open[2];  // jobs that other CTAs have pieces of: the run's first and its last
+  int opens = 0;
+  if (c0 < c1 && last_job[0].t0 > c0) {  // (its piece is in the CTA's place already)
+    open[0] = job_at(a, c0);
+    opens = open[0].t0 < c0;
+  }
+#pragma unroll 1
+  for (int i = 0; i < W; ++i) {
+    const int b0 = warp_begin(i), b1 = warp_begin(i + 1);
+    if (b0 >= b1) break;
+    const Job j = last_job[i];
+    const int t1 = j.t0 + j.tiles, end = min(t1, c1);
+    if ((j.t0 >= b0 && t1 <= b1) || (j.t0 < b0 && i > 0)) continue;
+    int n = 1;
+    while (i + n < W && warp_begin(i + n) < end) ++n;
+    const bool inside = j.t0 >= c0 && t1 <= c1;
+    join(j, n,
+         inside ? nullptr
+                : a.cta_parts + static_cast<size_t>(2 * blockIdx.x + (j.t0 > c0 ? 1 : 0)) * C::kPart,
+         [&](int k) -> const float* {
+           return end >= warp_begin(i + k + 1)
+                      ? reinterpret_cast<const float*>(smem + (i + k) * ring_bytes)
+                      : a.warp_parts + static_cast<size_t>(blockIdx.x * W + i + k) * C::kPart;
+         });
+    if (!inside) open[opens++] = j;
+  }
+  if (opens == 0) return;
+  // The barrier orders every thread's part of the pieces before the counts, whose release makes
+  // them visible; the last CTA's acquire sees the others'.
+  __syncthreads();
+  if (lane == 0 && warp < opens) {
+    const Job j = open[warp];
+    const int others = divide(j.t0 + j.tiles - 1, a.per_cta) - divide(j.t0, a.per_cta);
+    flag[warp] = atom_add_acq_rel_gpu(&a.counters[j.id], 1) == others;
+    if (flag[warp]) a.counters[j.id] = 0;
+  }
+  __syncthreads();
+#pragma unroll 1
+  for (int o = 0; o < opens; ++o) {
+    if (!flag[o]) continue;
+    const Job j = open[o];
+    const int first = divide(j.t0, a.per_cta), last = divide(j.t0 + j.tiles - 1, a.per_cta);
+    join(j, last - first + 1, nullptr, [&](int k) -> const float* {
+      const int c = first + k;
+      return a.cta_parts + static_cast<size_t>(2 * c + (j.t0 > c * a.per_cta ? 1 : 0)) * C::kPart;
+    });
   }
 }
 
@@ -716,13 +729,13 @@ cudaError_t launch_attn4_t(const Attn4Args& a, cudaStream_t s) {
   static std::atomic<uint64_t> done{0};
   cudaError_t e = ql_once_per_device(done, [] {
     return cudaFuncSetAttribute(attn4_kernel<HD, LO>, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                                static_cast<int>(C::kSmem));
+                                static_cast<int>(C::smem(C::kStages)));
   });
   if (e != cudaSuccess) return e;
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3((a.total + a.per_cta - 1) / a.per_cta);
   cfg.blockDim = dim3(32 * C::kWarps);
-  cfg.dynamicSmemBytes = C::kSmem;
+  cfg.dynamicSmemBytes = C::smem(a.stages);
   cfg.stream = s;
   cudaLaunchAttribute attr[1];
   attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
@@ -734,18 +747,57 @@ cudaError_t launch_attn4_t(const Attn4Args& a, cudaStream_t s) {
 
 }  // namespace
 
-// The split of `total` tiles: CTAs, and tiles of a CTA and of a warp.  At least kMinTiles tiles
-// a CTA: fewer leave more pieces to join across CTAs than their streaming saves.
-void attn4_plan(int hd, int num_sms, Attn4Args* a, size_t* cta_bytes, size_t* warp_bytes) {
-  constexpr int kMinTiles = 4;
+// The split of the tiles (tiles[b] of each of sequence b's `jobs` jobs) over CTAs and warps.
+// Each CTA takes an equal run of the list (one CTA an SM: a warp's ring fills its share of the
+// shared memory).  Where as many CTAs as there are SMs can be given whole shares of jobs with no
+// warp taking longer than in an equal split, the list is padded so that a CTA's run stays inside
+// one job: one piece a CTA to join instead of two.
+int attn4_plan(int hd, int num_sms, const int* tiles, int batch, int jobs, Attn4Args* a,
+               size_t* cta_bytes, size_t* warp_bytes) {
+  constexpr int kMinTiles = 4;  // of a CTA: fewer cost more in joining than they save
   const int warps = hd == 128 ? Attn4Cfg<128>::kWarps : Attn4Cfg<64>::kWarps;
   const int part = hd == 128 ? Attn4Cfg<128>::kPart : Attn4Cfg<64>::kPart;
-  const int want = std::max(1, std::min(num_sms, (a->total + kMinTiles - 1) / kMinTiles));
-  a->per_cta = (a->total + want - 1) / want;
+  const int most_stages = hd == 128 ? Attn4Cfg<128>::kStages : Attn4Cfg<64>::kStages;
+  int64_t total = 0;
+  int longest = 1;
+  for (int b = 0; b < batch; ++b) {
+    total += static_cast<int64_t>(tiles[b]) * jobs;
+    longest = std::max(longest, tiles[b]);
+  }
+  if (total > (1 << 30)) return 1;
+  const int ctas = static_cast<int>(
+      std::max<int64_t>(1, std::min<int64_t>(num_sms, (total + kMinTiles - 1) / kMinTiles)));
+  a->per_cta = static_cast<int>((total + ctas - 1) / ctas);
+  a->aligned = 0;
+  const int per_warp = (a->per_cta + warps - 1) / warps;
+  // the smallest share of a job that leaves no more CTAs than SMs
+  for (int splits = longest; splits >= 1; --splits) {
+    const int share = std::max((longest + splits - 1) / splits, std::min(longest, kMinTiles));
+    int64_t n = 0;
+    for (int b = 0; b < batch; ++b) n += static_cast<int64_t>((tiles[b] + share - 1) / share) * jobs;
+    if (n > num_sms) {
+      if (static_cast<int64_t>(batch) * jobs > num_sms) break;
+      continue;
+    }
+    if ((share + warps - 1) / warps <= per_warp) {
+      a->per_cta = share;
+      a->aligned = 1;
+    }
+    break;
+  }
   a->per_warp = (a->per_cta + warps - 1) / warps;
-  const size_t ctas = (a->total + a->per_cta - 1) / a->per_cta;
-  *cta_bytes = ctas * 2 * part * sizeof(float);
-  *warp_bytes = ctas * warps * part * sizeof(float);
+  a->stages = std::min(most_stages, a->per_warp);
+  total = 0;
+  for (int b = 0; b < batch; ++b) {
+    a->first[b] = static_cast<int32_t>(total);
+    const int t = a->aligned ? (tiles[b] + a->per_cta - 1) / a->per_cta * a->per_cta : tiles[b];
+    total += static_cast<int64_t>(t) * jobs;
+  }
+  a->total = static_cast<int32_t>(total);
+  const size_t n = static_cast<size_t>((total + a->per_cta - 1) / a->per_cta);
+  *cta_bytes = n * 2 * part * sizeof(float);
+  *warp_bytes = n * warps * part * sizeof(float);
+  return 0;
 }
 
 cudaError_t launch_attn4(const Attn4Args& a, cudaStream_t s) {

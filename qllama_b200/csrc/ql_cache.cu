@@ -387,7 +387,6 @@ cudaError_t launch_bounds(const BoundsArgs& a, cudaStream_t s) {
 namespace {
 
 constexpr int kChooseThreads = 256;
-constexpr int kChooseBlocks = 64;  // scored by one CTA
 constexpr int kBins = 2048;
 
 // Eight consecutive values of a bounds row.
@@ -423,8 +422,8 @@ __device__ __forceinline__ double block_extreme(double v, bool largest, double* 
 
 }  // namespace
 
-// Scores and choice in one launch.  The CTAs of a (token, KV head) score kChooseBlocks blocks
-// each; the last to arrive chooses.
+// Scores and choice in one launch.  The CTAs of a (token, KV head) score a.chunk blocks each;
+// the last to arrive chooses.
 //
 // Scores: the group's queries enter by the sums of their positive and of their negative parts,
 // because sum_h max(q_h lo, q_h hi) = (sum_h max(q_h, 0)) hi + (sum_h min(q_h, 0)) lo while
@@ -450,7 +449,7 @@ __global__ void __launch_bounds__(kChooseThreads)
     return;
   }
   const int lo_block = a.first, hi_block = count - a.last;  // the candidates
-  const int chunks = (hi_block + kChooseBlocks - 1) / kChooseBlocks;
+  const int chunks = (hi_block + a.chunk - 1) / a.chunk;
   if (static_cast<int>(blockIdx.x) >= chunks) return;
   const int free = a.take - a.first - a.last;
   double* score = a.score + pair * a.max_blocks;
@@ -468,7 +467,7 @@ __global__ void __launch_bounds__(kChooseThreads)
       }
       return a.bounds + bounds_row(c, page, block, kvh);
     };
-    const int block0 = blockIdx.x * kChooseBlocks, end = min(block0 + kChooseBlocks, hi_block);
+    const int block0 = blockIdx.x * a.chunk, end = min(block0 + a.chunk, hi_block);
     if constexpr (HD != 0) {
       constexpr int kPer = HD / 64;  // lane `sub` of eight: dims 64 j + 8 sub .. + 7
       const int sub = lane & 7;
@@ -477,19 +476,27 @@ __global__ void __launch_bounds__(kChooseThreads)
       for (int j = 0; j < kPer; ++j)
 #pragma unroll
         for (int k = 0; k < 8; ++k) up[j][k] = down[j][k] = 0.0;
-      for (int h = 0; h < a.group; ++h)
+      constexpr int kHeads = 4;  // loaded at once
+      for (int h0 = 0; h0 < a.group; h0 += kHeads) {
+        Raw8 raw[kHeads][kPer];
 #pragma unroll
-        for (int j = 0; j < kPer; ++j) {
-          float x[4], y[4];
-          const size_t at = q0 + static_cast<size_t>(h) * HD + 64 * j + 8 * sub;
-          load_vec<4>(a.q, at, a.in_dtype, a.q_vec != 0, x);
-          load_vec<4>(a.q, at + 4, a.in_dtype, a.q_vec != 0, y);
+        for (int h = 0; h < kHeads; ++h)
 #pragma unroll
-          for (int k = 0; k < 4; ++k) {
-            add_parts(x[k], up[j][k], down[j][k]);
-            add_parts(y[k], up[j][k + 4], down[j][k + 4]);
+          for (int j = 0; j < kPer; ++j)
+            raw[h][j] = load_raw8(a.q, q0 + static_cast<size_t>(min(h0 + h, a.group - 1)) * HD +
+                                           64 * j + 8 * sub, a.in_dtype, a.q_vec != 0);
+#pragma unroll
+        for (int h = 0; h < kHeads; ++h)
+#pragma unroll
+          for (int j = 0; j < kPer; ++j) {
+            float x[8];
+            floats_of(raw[h][j], a.in_dtype, x);
+            if (h0 + h < a.group) {
+#pragma unroll
+              for (int k = 0; k < 8; ++k) add_parts(x[k], up[j][k], down[j][k]);
+            }
           }
-        }
+      }
       for (int base = block0 + 4 * warp; base < end; base += kChooseThreads / 8) {
         const int block = base + (lane >> 3);
         const uint16_t* p = block < end && block >= lo_block ? bounds_of(block) : nullptr;
@@ -658,8 +665,13 @@ cudaError_t launch_select(const SelectArgs& a_in, cudaStream_t s) {
   constexpr size_t kLimit = 32 * 1024;
   a.smem_blocks = bits < kLimit ? static_cast<int32_t>((kLimit - bits) / sizeof(double)) : 0;
   const size_t smem = bits + (a.max_blocks <= a.smem_blocks ? a.max_blocks * sizeof(double) : 0);
+  // Blocks of a CTA: 32 in one go of its warps while the CTAs are few, more where they would
+  // come in several waves (a CTA begins with the queries, whatever it scores).
+  const int64_t pairs = static_cast<int64_t>(jobs) * a.cache.hkv;
+  a.chunk = 32;
+  while (a.chunk < 256 && pairs * ((a.max_blocks + a.chunk - 1) / a.chunk) > 2LL * a.num_sms) a.chunk *= 2;
   cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3((a.max_blocks + kChooseBlocks - 1) / kChooseBlocks, a.cache.hkv, jobs);
+  cfg.gridDim = dim3((a.max_blocks + a.chunk - 1) / a.chunk, a.cache.hkv, jobs);
   cfg.blockDim = dim3(kChooseThreads);
   cfg.dynamicSmemBytes = smem;
   cfg.stream = s;

@@ -160,8 +160,10 @@ struct Attn4Args {
   float scale;
   const int32_t* sel;   // as in AttnArgs
   int32_t sel_max;
-  int32_t total;        // tiles of all jobs
+  int32_t total;        // places in the list of all jobs' tiles
   int32_t per_cta, per_warp;
+  int32_t aligned;      // a job takes whole CTAs: its places are a multiple of per_cta
+  int32_t stages;       // records in a warp's ring
   float* cta_parts;     // [CTAs][2] pieces
   float* warp_parts;    // [CTAs][warps] pieces
   int32_t* counters;    // [jobs], zero between launches
@@ -260,7 +262,9 @@ struct SelectArgs {
   int32_t take, first, last;
   int32_t max_blocks;   // row length of `score`
   int32_t smem_blocks;  // set by the launch: scores that shared memory holds
-  int32_t q_vec;        // q allows loads of four elements
+  int32_t chunk;        // set by the launch: blocks that a CTA scores
+  int32_t num_sms;
+  int32_t q_vec;        // q is 16-byte aligned
   int32_t* counters;    // [jobs][hkv], zero between launches
   double* score;        // scratch [jobs][hkv][max_blocks]
   const uint16_t* bounds;
@@ -327,10 +331,11 @@ cudaError_t launch_ragged_append(const RaggedAppendArgs& a, cudaStream_t s);
 cudaError_t launch_ragged_read(const RaggedReadArgs& a, cudaStream_t s);
 cudaError_t launch_bounds(const BoundsArgs& a, cudaStream_t s);
 cudaError_t launch_select(const SelectArgs& a, cudaStream_t s);
-// Q4_0 decode: whether it applies, the split of a->total tiles (fills per_cta and per_warp,
-// reports the bytes of the pieces), and the launch.
+// Q4_0 decode: whether it applies; the split of the tiles (fills total, per_cta, per_warp,
+// aligned, stages and first, reports the bytes of the pieces; 1: too many tiles); the launch.
 bool attn4_supported(int hd, int page);
-void attn4_plan(int hd, int num_sms, Attn4Args* a, size_t* cta_bytes, size_t* warp_bytes);
+int attn4_plan(int hd, int num_sms, const int* tiles, int batch, int jobs, Attn4Args* a,
+               size_t* cta_bytes, size_t* warp_bytes);
 cudaError_t launch_attn4(const Attn4Args& a, cudaStream_t s);
 // Writes the entries of `p` into the device block table, in stream order, as
 // an ordinary launch: a kernel queued after it sees the entries once its

@@ -244,25 +244,23 @@ def qkv_rope_append(kv, layer: int, x, wqkv_t, start_pos, num_heads: int, num_kv
 
 def _appended_args(kv, layer, q_rot, start_pos, num_heads, num_kv_heads, head_dim, rope_theta,
                    seq_ids, out, out_dtype):
-    """(AttnArgs, out, keep-alive) of attention over rows that are in the cache."""
+    """(AttnArgs, out) of attention over rows that are in the cache."""
     qb = _qb()
-    if q_rot.dim() < 3:
-        raise _invalid(f"q_rot must be [batch, new_len, heads, head_dim], got {tuple(q_rot.shape)}")
-    batch, new_len = int(q_rot.shape[0]), int(q_rot.shape[1])
-    if q_rot.numel() != batch * new_len * num_heads * head_dim or not q_rot.is_contiguous():
+    shape = q_rot.shape
+    if len(shape) < 3 or not q_rot.is_contiguous() or \
+            q_rot.numel() != shape[0] * shape[1] * num_heads * head_dim:
         raise _invalid(f"q_rot must be contiguous [batch, new_len, {num_heads}, {head_dim}], got "
-                       f"{tuple(q_rot.shape)}")
-    if out is not None:
-        t = out.dtype
-    else:
-        t = _named_type(out_dtype or "f32")
+                       f"{tuple(shape)}")
+    batch, new_len = shape[0], shape[1]
+    t = out.dtype if out is not None else _named_type(out_dtype or "f32")
     out = _output(kv.ctx, out, (batch, new_len, num_heads * head_dim), t, "out")
-    if np.ndim(start_pos) and len(start_pos) != batch or \
-            seq_ids is not None and len(seq_ids) != batch:
+    if not hasattr(start_pos, "__len__"):
+        start_pos = [start_pos] * batch
+    if seq_ids is None:
+        seq_ids = range(batch)
+    if len(start_pos) != batch or len(seq_ids) != batch:
         raise _invalid(f"one position and one sequence for each of {batch} rows of q_rot")
-    starts = (ctypes.c_int64 * batch)(*([start_pos] * batch if np.ndim(start_pos) == 0
-                                        else start_pos))
-    seqs = (ctypes.c_int32 * batch)(*(range(batch) if seq_ids is None else seq_ids))
+    starts, seqs = (ctypes.c_int64 * batch)(*start_pos), (ctypes.c_int32 * batch)(*seq_ids)
     dev = kv.ctx.device
     args = qb.AttnArgs(layer, batch, new_len, seqs, starts, num_heads, num_kv_heads, head_dim,
                        rope_theta, _float_code(q_rot, "q_rot"), _float_code(out, "out"),

@@ -53,12 +53,22 @@ class Cache:
         return ctypes.byref(self.ctx), ctypes.byref(self.kv)
 
 
+KEEP = []  # arrays whose addresses are in structures
+
+
 def i32(*x):
     return (ctypes.c_int32 * len(x))(*x)
 
 
 def i64(*x):
     return (ctypes.c_int64 * len(x))(*x)
+
+
+def address(x):
+    if not isinstance(x, ctypes.Array):
+        return x
+    KEEP.append(x)
+    return ctypes.addressof(x)
 
 
 def refused(rc, text, code=qb.ERR_INVALID):
@@ -70,7 +80,7 @@ def append_args(**change):
     a = dict(layer_idx=0, batch=2, seq_ids=i32(0, 1), start_pos=i64(5, 0), new_len=i32(3, 4),
              num_heads=4, num_kv_heads=HKV, head_dim=HD, rope_theta=1e4, in_dtype=qb.F32,
              q_out_dtype=qb.F16, q=P, k=P + 8192, v=P + 16384, q_out=P + 32768)
-    return qb.AppendArgs(**{**a, **change})
+    return qb.AppendArgs(**{k: address(x) for k, x in {**a, **change}.items()})
 
 
 @pytest.mark.parametrize("change, text", [
@@ -208,9 +218,17 @@ def test_python_calls_check_their_lists():
     with pytest.raises(qb.QllamaError, match="length"):
         kv.truncate([0, 1], [3])
     with pytest.raises(qb.QllamaError, match="position"):
-        kv._ragged(None, [0], [1, 2])
+        qb._ragged(None, [0], [1, 2])
     with pytest.raises(qb.QllamaError, match="sequence"):
-        kv._ragged([0], [0, 0], [1, 2])
-    batch, total, rows = kv._ragged([3, 1], [10, 0], [2, 5])
+        qb._ragged([0], [0, 0], [1, 2])
+    batch, total, rows, keep = qb._ragged([3, 1], [10, 0], [2, 5])
     assert (batch, total) == (2, 7)
-    assert [list(x) for x in rows] == [[3, 1], [10, 0], [2, 5]]
+    assert [list(x) for x in keep] == [[3, 1], [10, 0], [2, 5]]
+    assert list(rows) == [x.buffer_info()[0] for x in keep]
+    assert list(qb._ragged(None, [0] * 3, [1] * 3)[3][0]) == [0, 1, 2]
+
+
+@pytest.mark.parametrize("positions", [range(3, 9), range(0), range(9, 3, -2), [4, 5, 7]])
+def test_positions(positions):
+    got = qb._positions(positions)
+    assert got.dtype == "int32" and got.flags.c_contiguous and list(got) == list(positions)

@@ -397,6 +397,24 @@ def test_4_bit_values_of_any_size(ctx, scale):
                  "prompt" if t >= 64 else "decode")
 
 
+@pytest.mark.parametrize("hd", [64, 128])
+def test_4_bit_scores_far_from_zero(ctx, hd):
+    """All scores near -400 (or, of the other heads, +400), over pieces of which some rows see
+    nothing."""
+    hq, hkv, n = 8, 2, 64 * 40 + 2
+    kv = qb.KvCache(ctx, 1, n, hkv, hd, "q4_0")
+    k = normal(1, n, hkv, hd, scale=0.1) + 1
+    v = normal(2, n, hkv, hd)
+    kv.update(0, k, v, range(n))
+    kc, vc = (x.double() for x in kv.read(0, [0], [n]))
+    for t in (1, 5):
+        q = normal(3, 1, t, hq, hd, scale=0.1) - 400 / math.sqrt(hd)
+        q[:, :, 1::2] *= -1
+        out = qm.attention_forward_appended(kv, 0, q, [n - t], hq, hkv, hd, THETA)
+        want, big = attention(q[0], kc, vc, n - t)
+        near(out[0].view(t, hq, hd), want, big, top(vc))
+
+
 def test_rows_behind_the_end_are_never_read(ctx):
     """A rolled-back sequence leaves NaN rows behind its end; other sequences' stay apart."""
     hq, hkv, hd = 8, 2, 128
