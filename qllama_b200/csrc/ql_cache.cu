@@ -389,9 +389,10 @@ namespace {
 constexpr int kChooseThreads = 256;
 constexpr int kBins = 2048;
 
+constexpr int kMaxChunk = 256;  // blocks that a CTA scores at most
+
 // Eight consecutive values of a bounds row.
-__device__ __forceinline__ void load_bounds(const uint16_t* p, bool half, float (&x)[8]) {
-  const uint4 w = *reinterpret_cast<const uint4*>(p);
+__device__ __forceinline__ void bounds_values(const uint4& w, bool half, float (&x)[8]) {
   const uint32_t in[4] = {w.x, w.y, w.z, w.w};
 #pragma unroll
   for (int k = 0; k < 4; ++k) {
@@ -497,24 +498,53 @@ __global__ void __launch_bounds__(kChooseThreads)
             }
           }
       }
-      for (int base = block0 + 4 * warp; base < end; base += kChooseThreads / 8) {
-        const int block = base + (lane >> 3);
-        const uint16_t* p = block < end && block >= lo_block ? bounds_of(block) : nullptr;
-        double s = 0.0;
-        if (p) {
+      // The blocks of all rounds are looked up at once, one by each of the eight lanes, and the
+      // next round's bounds are under way while one is summed.
+      constexpr int kRound = kChooseThreads / 8;
+      static_assert(kMaxChunk == 8 * kRound, "a lane a round");
+      const int base = block0 + 4 * warp + (lane >> 3);
+      const uint16_t* mine = nullptr;
+      if (base + sub * kRound < end && base + sub * kRound >= lo_block)
+        mine = bounds_of(base + sub * kRound);
+      struct Bounds {
+        uint4 lo[kPer], hi[kPer];
+        const uint16_t* p;
+      };
+      auto fetch = [&](int round) {
+        Bounds x;
+        x.p = reinterpret_cast<const uint16_t*>(__shfl_sync(
+            0xffffffffu, reinterpret_cast<unsigned long long>(mine), (lane & 24) + round));
+        if (x.p) {
+#pragma unroll
+          for (int j = 0; j < kPer; ++j) {
+            x.lo[j] = *reinterpret_cast<const uint4*>(x.p + 64 * j + 8 * sub);
+            x.hi[j] = *reinterpret_cast<const uint4*>(x.p + HD + 64 * j + 8 * sub);
+          }
+        }
+        return x;
+      };
+      const int rounds = (end - block0 + kRound - 1) / kRound;
+      Bounds next = fetch(0);
+      for (int round = 0; round < rounds; ++round) {
+        const Bounds x = next;
+        if (round + 1 < rounds) next = fetch(round + 1);
+        double s[kPer] = {};
+        if (x.p) {
 #pragma unroll
           for (int j = 0; j < kPer; ++j) {
             float lo[8], hi[8];
-            load_bounds(p + 64 * j + 8 * sub, half, lo);
-            load_bounds(p + HD + 64 * j + 8 * sub, half, hi);
+            bounds_values(x.lo[j], half, lo);
+            bounds_values(x.hi[j], half, hi);
 #pragma unroll
-            for (int k = 0; k < 8; ++k) s += up[j][k] * hi[k] + down[j][k] * lo[k];
+            for (int k = 0; k < 8; ++k) s[j] += up[j][k] * hi[k] + down[j][k] * lo[k];
           }
         }
+        double t = s[0];
+        if constexpr (kPer > 1) t += s[1];
 #pragma unroll
-        for (int o = 4; o > 0; o >>= 1) s += __shfl_xor_sync(0xffffffffu, s, o);
-        if (s != s) s = CUDART_INF;  // a NaN counts as the largest score
-        if (p && sub == 0) score[block] = s;
+        for (int o = 4; o > 0; o >>= 1) t += __shfl_xor_sync(0xffffffffu, t, o);
+        if (t != t) t = CUDART_INF;  // a NaN counts as the largest score
+        if (x.p && sub == 0) score[base + round * kRound] = t;
       }
     } else {
       const int bt = half ? kF16 : kBF16;
@@ -669,7 +699,7 @@ cudaError_t launch_select(const SelectArgs& a_in, cudaStream_t s) {
   // come in several waves (a CTA begins with the queries, whatever it scores).
   const int64_t pairs = static_cast<int64_t>(jobs) * a.cache.hkv;
   a.chunk = 32;
-  while (a.chunk < 256 && pairs * ((a.max_blocks + a.chunk - 1) / a.chunk) > 2LL * a.num_sms) a.chunk *= 2;
+  while (a.chunk < kMaxChunk && pairs * ((a.max_blocks + a.chunk - 1) / a.chunk) > 2LL * a.num_sms) a.chunk *= 2;
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3((a.max_blocks + a.chunk - 1) / a.chunk, a.cache.hkv, jobs);
   cfg.blockDim = dim3(kChooseThreads);
