@@ -15,10 +15,10 @@
 //   O = V^T P      A = the V codes, B = P times the block's scale
 // A code c masked out of its word is the f16 number c 2^-24 (or, in the next nibble, c 2^-20):
 // f16's subnormals hold the codes exactly and the matrix instruction takes them as they are, so
-// that a fragment register costs one AND.  The powers of two are folded into q and the output;
-// the 8 that is subtracted from every code enters S as -8 sum q and leaves
-// O with the product of P by rows of eights.  A K scale multiplies the block's partial
-// sums in f32, a V scale the probabilities in f16.
+// that a fragment register costs one AND.  The powers of two are folded into q and the output.
+// A K scale multiplies the block's partial sums in f32, a V scale the probabilities in f16.  The
+// 8 that is subtracted from every code enters S and leaves O as products of the scales: of K's
+// with -8 sum q of each block, of V's with P, where a row of ones beside them sums P itself.
 //
 // Bound by HBM for long caches (2304 bytes of a head_dim 128 cache per 16 positions against
 // about 200 instructions of one warp).
@@ -70,6 +70,14 @@ __device__ __forceinline__ void mma_f16(float (&d)[4], uint32_t a0, uint32_t a1,
       "{%0,%1,%2,%3};"
       : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
       : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
+
+// m16n8k8: D = A B.
+__device__ __forceinline__ void mma_f16_k8(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t b) {
+  asm("mma.sync.aligned.m16n8k8.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5}, {%6}, "
+      "{%7,%7,%7,%7};"
+      : "=f"(d[0]), "=f"(d[1]), "=f"(d[2]), "=f"(d[3])
+      : "r"(a0), "r"(a1), "r"(b), "f"(0.f));
 }
 
 // The transpose of an 8 x 8 matrix of f16 held as pairs along its rows.
@@ -268,7 +276,10 @@ __global__ void __launch_bounds__(32 * Attn4Cfg<HD>::kWarps, 1)
   const int v_at = static_cast<int>(kRec.v_codes()) + q4_v_byte(2 * tq, 4 * g, NB);
   const int ks_at = static_cast<int>(kRec.k_scales()) + 2 * q4_k_scale(g, 0, NB);
   const int vs_at = static_cast<int>(kRec.v_scales()) + 2 * q4_v_scale(2 * tq, 0, NB);
-  constexpr uint32_t kEights = 0x00080008u;  // two codes of 8
+  const int kw_at = ks_at + (NB == 4 ? (tq & 1) * 4 : 0);  // the scales of blocks 2 tq, 2 tq + 1
+  const int vw_at = vs_at + (g & (NB - 1)) * 4;            // V's of block g
+  // rows of V's scales, one a block, then a row of ones
+  const uint32_t aux_and = g < NB ? 0xffffffffu : 0u, aux_or = g == 4 ? 0x3c003c00u : 0u;
 
   bool alive = true;
   int stage = 0, phase = 0;  // of the next tile
@@ -281,9 +292,10 @@ __global__ void __launch_bounds__(32 * Attn4Cfg<HD>::kWarps, 1)
     // ------------------------------------------------------------- q --
     // Lane (g, tq) holds dims 32 b + 8 tq .. + 7 of row g: the columns of B in the order in
     // which the K words' nibbles come out (j and j + 4 together; odd ones, whose codes are
-    // 16 times as large, divided by 16).  Each row is scaled by a power of two to [2^14, 2^15).
-    uint32_t qh[NB][2][2], ql[NB][2][2];
-    float qo[NB][2], f[2];
+    // 16 times as large, divided by 16).  Each row is scaled by a power of two to [2^6, 2^7):
+    // -8 times a block's sum stays in f16's range.
+    uint32_t qh[NB][2][2], ql[NB][2][2], qo;
+    float f[2];
     {
       float v[NB][8];
       const bool live = g < job.rows;
@@ -343,7 +355,7 @@ __global__ void __launch_bounds__(32 * Attn4Cfg<HD>::kWarps, 1)
       mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 1));
       mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 2));
       const uint32_t bits = __float_as_uint(mx);
-      int e = static_cast<int>(bits >> 23) - 127 - 14;
+      int e = static_cast<int>(bits >> 23) - 127 - 6;
       if (bits == 0 || bits >= 0x7f800000u) e = 0;
       e = max(e, -100);
       const float down = pow2f(-e);
@@ -366,15 +378,23 @@ __global__ void __launch_bounds__(32 * Attn4Cfg<HD>::kWarps, 1)
           }
         s += __shfl_xor_sync(0xffffffffu, s, 1);
         s += __shfl_xor_sync(0xffffffffu, s, 2);
-        sums[b] = s * (-8.f / 16777216.f);
+        sums[b] = s * -8.f;
       }
-      const float fr = a.scale * kLog2e4 * 16777216.f * pow2f(e);
+      // B of the K scales' product: column g, the sums' high parts under blocks 2 tq, 2 tq + 1
+      // and what is left of them under the same scales again
+      const bool low = NB == 4 ? tq >= 2 : tq == 1;
+      float pair[2];
 #pragma unroll
       for (int k = 0; k < 2; ++k) {
-        f[k] = __shfl_sync(0xffffffffu, fr, (2 * tq + k) * 4);
-#pragma unroll
-        for (int b = 0; b < NB; ++b) qo[b][k] = __shfl_sync(0xffffffffu, sums[b], (2 * tq + k) * 4);
+        const float s = NB == 4 && (tq & 1) ? sums[NB - 2 + k] : sums[k];
+        float h, rest;
+        split16<false>(s, h, rest);
+        pair[k] = low ? rest : h;
       }
+      qo = NB == 2 && tq >= 2 ? 0u : pack2<false>(pair[0], pair[1]);
+      const float fr = a.scale * kLog2e4 * 16777216.f * pow2f(e);
+#pragma unroll
+      for (int k = 0; k < 2; ++k) f[k] = __shfl_sync(0xffffffffu, fr, (2 * tq + k) * 4);
     }
     // The keys that this lane's two rows see: positions below lim (of a selection: places of
     // its list), and those that all rows of the job see.
@@ -390,14 +410,12 @@ __global__ void __launch_bounds__(32 * Attn4Cfg<HD>::kWarps, 1)
     }
     const int most = a.sel ? all : start + divide(job.row0 + job.rows - 1, a.group) + 1;
 
-    float o[NB][2][4], off[NB][4];
+    float o[NB][2][4], aux[4] = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-    for (int b = 0; b < NB; ++b) {
-      off[b][0] = off[b][1] = off[b][2] = off[b][3] = 0.f;
+    for (int b = 0; b < NB; ++b)
 #pragma unroll
       for (int u = 0; u < 2; ++u) o[b][u][0] = o[b][u][1] = o[b][u][2] = o[b][u][3] = 0.f;
-    }
-    float ref[2] = {0.f, 0.f}, l[2] = {0.f, 0.f}, top = kTop;
+    float ref[2] = {0.f, 0.f}, top = kTop;
     bool fresh = true;
     uint32_t nans = 0;  // of row 2 tq + k: bit 4 k + b, that it sees a value of block b that is NaN
 
@@ -435,7 +453,10 @@ __global__ void __launch_bounds__(32 * Attn4Cfg<HD>::kWarps, 1)
               kd[r][0] = *reinterpret_cast<const uint32_t*>(sp);
             }
           }
-          y[e][0] = y[e][1] = y[e][2] = y[e][3] = 0.f;
+          const uint32_t* wp = reinterpret_cast<const uint32_t*>(st + kw_at + 32 * (s + e) * NB);
+          mma_f16_k8(y[e], wp[0], wp[4 * NB], qo);
+#pragma unroll
+          for (int k = 0; k < 4; ++k) y[e][k] *= 1.f / 16777216.f;
 #pragma unroll
           for (int b = 0; b < NB; ++b) {
             float c[4];
@@ -451,27 +472,29 @@ __global__ void __launch_bounds__(32 * Attn4Cfg<HD>::kWarps, 1)
               if constexpr (LO) mma_f16(c, a0, a1, a2, a3, ql[b][ks][0], ql[b][ks][1]);
             }
             const float d0 = half_of(kd[0][b / 2], b & 1), d1 = half_of(kd[1][b / 2], b & 1);
-            y[e][0] = fmaf(c[0] + qo[b][0], d0, y[e][0]);
-            y[e][1] = fmaf(c[1] + qo[b][1], d0, y[e][1]);
-            y[e][2] = fmaf(c[2] + qo[b][0], d1, y[e][2]);
-            y[e][3] = fmaf(c[3] + qo[b][1], d1, y[e][3]);
+            y[e][0] = fmaf(c[0], d0, y[e][0]);
+            y[e][1] = fmaf(c[1], d0, y[e][1]);
+            y[e][2] = fmaf(c[2], d1, y[e][2]);
+            y[e][3] = fmaf(c[3], d1, y[e][3]);
           }
         }
         // ---- V's scales of positions 2 tq, 2 tq + 1 and those plus 8
-        uint32_t vd[2][2][NB], any_d = 0;
+        uint32_t vd[2][2][NB], va[2][2], any_d = 0;
 #pragma unroll
         for (int e = 0; e < 2; ++e)
 #pragma unroll
           for (int r = 0; r < 2; ++r) {
+            const uint32_t w =
+                *reinterpret_cast<const uint32_t*>(st + vw_at + (32 * (s + e) + 16 * r) * NB);
+            any_d |= w;  // between them the lanes see every scale
+            va[e][r] = (w & aux_and) | aux_or;
             const uint8_t* sp = svs + (32 * e + 16 * r) * NB;
             if constexpr (NB == 4) {
               const uint4 d = *reinterpret_cast<const uint4*>(sp);
               vd[e][r][0] = d.x, vd[e][r][1] = d.y, vd[e][r][2] = d.z, vd[e][r][3] = d.w;
-              any_d |= d.x | d.y | d.z | d.w;
             } else {
               const uint2 d = *reinterpret_cast<const uint2*>(sp);
               vd[e][r][0] = d.x, vd[e][r][1] = d.y;
-              any_d |= d.x | d.y;
             }
           }
         // ---- softmax: columns 2 tq, 2 tq + 1 of positions g and g + 8
@@ -514,6 +537,13 @@ __global__ void __launch_bounds__(32 * Attn4Cfg<HD>::kWarps, 1)
                   for (int k = 0; k < 2; ++k) nans |= (place < lim[k] ? 1u : 0u) << (4 * k + b);
                 }
               }
+#pragma unroll
+          for (int e = 0; e < 2; ++e)
+#pragma unroll
+            for (int r = 0; r < 2; ++r) {
+              if ((va[e][r] & 0x7fffu) > 0x7c00u) va[e][r] &= 0xffff0000u;
+              if ((va[e][r] >> 16 & 0x7fffu) > 0x7c00u) va[e][r] &= 0xffffu;
+            }
           big = __reduce_max_sync(0xffffffffu, big);
           const float cap = fminf(top, kTop - fmaxf(0.f, static_cast<float>(static_cast<int>(big >> 10) - 15)));
 #pragma unroll
@@ -528,17 +558,14 @@ __global__ void __launch_bounds__(32 * Attn4Cfg<HD>::kWarps, 1)
             if ((fresh || m - next > cap) && m > -CUDART_INF_F) next = m - (cap - kSlack);
             const float corr = fresh ? 0.f : ex2(ref[k] - next);
             ref[k] = next;
-            l[k] *= corr;
+            aux[k] *= corr;
 #pragma unroll
-            for (int b = 0; b < NB; ++b) {
-              off[b][k] *= corr;
-              off[b][k + 2] = 0.f;  // every row is alike: the lower eight stay unused
+            for (int b = 0; b < NB; ++b)
 #pragma unroll
               for (int u = 0; u < 2; ++u) {
                 o[b][u][k] *= corr;
                 o[b][u][k + 2] *= corr;
               }
-            }
           }
           top = cap;
           fresh = false;
@@ -550,13 +577,11 @@ __global__ void __launch_bounds__(32 * Attn4Cfg<HD>::kWarps, 1)
 #pragma unroll
         for (int e = 0; e < 2; ++e) {
 #pragma unroll
-          for (int k = 0; k < 4; ++k) {
-            p[e][k] = ex2(p[e][k]);
-            l[k & 1] += p[e][k];
-          }
+          for (int k = 0; k < 4; ++k) p[e][k] = ex2(p[e][k]);
           const uint32_t pt0 = transpose8(pack2<false>(p[e][0], p[e][1]));
           const uint32_t pt1 = transpose8(pack2<false>(p[e][2], p[e][3]));
-          // ---- O += V^T (P d)
+          // ---- O += V^T (P d), and the sums of P d and P
+          mma_f16(aux, va[e][0], 0u, va[e][1], 0u, pt0, pt1);
           uint32_t vw[2][NB];
 #pragma unroll
           for (int r = 0; r < 2; ++r) {
@@ -572,7 +597,6 @@ __global__ void __launch_bounds__(32 * Attn4Cfg<HD>::kWarps, 1)
 #pragma unroll
           for (int b = 0; b < NB; ++b) {
             const uint32_t b0 = mul2(pt0, vd[e][0][b]), b1 = mul2(pt1, vd[e][1][b]);
-            mma_f16(off[b], kEights, kEights, kEights, kEights, b0, b1);
 #pragma unroll
             for (int u = 0; u < 2; ++u) {
               const uint32_t u0 = vw[0][b] >> (8 * u), u1 = vw[1][b] >> (8 * u);
@@ -591,15 +615,12 @@ __global__ void __launch_bounds__(32 * Attn4Cfg<HD>::kWarps, 1)
     }
 
     // ------------------------------------------------- the end of a piece --
+    float l[2];
 #pragma unroll
     for (int k = 0; k < 2; ++k) {
-      l[k] += __shfl_xor_sync(0xffffffffu, l[k], 4);
-      l[k] += __shfl_xor_sync(0xffffffffu, l[k], 8);
-      l[k] += __shfl_xor_sync(0xffffffffu, l[k], 16);
-    }
-#pragma unroll
-    for (int k = 0; k < 2; ++k)
+      l[k] = __shfl_sync(0xffffffffu, aux[k], 16 + tq);
       if (l[k] == 0.f) ref[k] = -CUDART_INF_F;  // the row sees none of these tiles
+    }
     const bool whole = job.t0 >= w0 && job.t0 + job.tiles <= w1;
     // A piece that ends the warp's part goes into its ring; an earlier one (of a job that
     // other warps began) into memory: the CTA's own piece of it if no other warp here has one.
@@ -612,13 +633,17 @@ __global__ void __launch_bounds__(32 * Attn4Cfg<HD>::kWarps, 1)
       const bool live = r < job.rows;
       const float f24 = 16777216.f * (whole ? 1.f / l[k] : 1.f);
       const size_t base = whole && live ? row_offset(a, job, job.row0 + r, HD) : 0;
+      float eight[NB];  // 8 sum P d of each block, in the units of O
+#pragma unroll
+      for (int b = 0; b < NB; ++b)
+        eight[b] = __shfl_sync(0xffffffffu, aux[k], 4 * b + tq) * (8.f / 16777216.f);
       if (!live) continue;
 #pragma unroll
       for (int b = 0; b < NB; ++b) {
-        float4 v = make_float4((o[b][0][k] - off[b][k]) * f24,
-                               (o[b][0][k + 2] * 0.0625f - off[b][k]) * f24,
-                               (o[b][1][k] - off[b][k]) * f24,
-                               (o[b][1][k + 2] * 0.0625f - off[b][k]) * f24);
+        float4 v = make_float4((o[b][0][k] - eight[b]) * f24,
+                               (o[b][0][k + 2] * 0.0625f - eight[b]) * f24,
+                               (o[b][1][k] - eight[b]) * f24,
+                               (o[b][1][k + 2] * 0.0625f - eight[b]) * f24);
         if (nans >> (4 * k + b) & 1u) v.x = v.y = v.z = v.w = CUDART_NAN_F;
         const int d = 32 * b + 4 * g;
         if (whole)

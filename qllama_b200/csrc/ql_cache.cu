@@ -429,7 +429,7 @@ __device__ __forceinline__ double block_extreme(double v, bool largest, double* 
 // Scores: the group's queries enter by the sums of their positive and of their negative parts,
 // because sum_h max(q_h lo, q_h hi) = (sum_h max(q_h, 0)) hi + (sum_h min(q_h, 0)) lo while
 // lo <= hi: two products a channel whatever the group.  In f64, so that only equal blocks tie.
-// Eight lanes a block (HD 64 or 128), else (HD 0) a warp.  Bound by the bounds' bytes.
+// HD / 8 lanes a block (HD 64 or 128), else (HD 0) a warp.  Bound by the bounds' bytes.
 //
 // Choice: a histogram over the range of the scores puts the border into one of kBins bins;
 // those above it are in, and the few in it are ranked among themselves by (score, block).
@@ -470,56 +470,47 @@ __global__ void __launch_bounds__(kChooseThreads)
     };
     const int block0 = blockIdx.x * a.chunk, end = min(block0 + a.chunk, hi_block);
     if constexpr (HD != 0) {
-      constexpr int kPer = HD / 64;  // lane `sub` of eight: dims 64 j + 8 sub .. + 7
-      const int sub = lane & 7;
-      double up[kPer][8], down[kPer][8];
+      constexpr int kLanes = HD / 8;  // of a block: lane `sub` has dims 8 sub .. + 7
+      const int sub = lane & (kLanes - 1);
+      double up[8], down[8];
 #pragma unroll
-      for (int j = 0; j < kPer; ++j)
-#pragma unroll
-        for (int k = 0; k < 8; ++k) up[j][k] = down[j][k] = 0.0;
+      for (int k = 0; k < 8; ++k) up[k] = down[k] = 0.0;
       constexpr int kHeads = 4;  // loaded at once
       for (int h0 = 0; h0 < a.group; h0 += kHeads) {
-        Raw8 raw[kHeads][kPer];
+        Raw8 raw[kHeads];
 #pragma unroll
         for (int h = 0; h < kHeads; ++h)
+          raw[h] = load_raw8(a.q, q0 + static_cast<size_t>(min(h0 + h, a.group - 1)) * HD + 8 * sub,
+                             a.in_dtype, a.q_vec != 0);
 #pragma unroll
-          for (int j = 0; j < kPer; ++j)
-            raw[h][j] = load_raw8(a.q, q0 + static_cast<size_t>(min(h0 + h, a.group - 1)) * HD +
-                                           64 * j + 8 * sub, a.in_dtype, a.q_vec != 0);
+        for (int h = 0; h < kHeads; ++h) {
+          float x[8];
+          floats_of(raw[h], a.in_dtype, x);
+          if (h0 + h < a.group) {
 #pragma unroll
-        for (int h = 0; h < kHeads; ++h)
-#pragma unroll
-          for (int j = 0; j < kPer; ++j) {
-            float x[8];
-            floats_of(raw[h][j], a.in_dtype, x);
-            if (h0 + h < a.group) {
-#pragma unroll
-              for (int k = 0; k < 8; ++k) add_parts(x[k], up[j][k], down[j][k]);
-            }
+            for (int k = 0; k < 8; ++k) add_parts(x[k], up[k], down[k]);
           }
+        }
       }
-      // The blocks of all rounds are looked up at once, one by each of the eight lanes, and the
+      // The blocks of all rounds are looked up at once, one by each lane of a group, and the
       // next round's bounds are under way while one is summed.
-      constexpr int kRound = kChooseThreads / 8;
-      static_assert(kMaxChunk == 8 * kRound, "a lane a round");
-      const int base = block0 + 4 * warp + (lane >> 3);
+      constexpr int kRound = kChooseThreads / kLanes;
+      static_assert(kMaxChunk <= kLanes * kRound, "a lane a round");
+      const int base = block0 + 32 / kLanes * warp + lane / kLanes;
       const uint16_t* mine = nullptr;
       if (base + sub * kRound < end && base + sub * kRound >= lo_block)
         mine = bounds_of(base + sub * kRound);
       struct Bounds {
-        uint4 lo[kPer], hi[kPer];
+        uint4 lo, hi;
         const uint16_t* p;
       };
       auto fetch = [&](int round) {
         Bounds x;
         x.p = reinterpret_cast<const uint16_t*>(__shfl_sync(
-            0xffffffffu, reinterpret_cast<unsigned long long>(mine), (lane & 24) + round));
+            0xffffffffu, reinterpret_cast<unsigned long long>(mine), (lane & ~(kLanes - 1)) + round));
         if (x.p) {
-#pragma unroll
-          for (int j = 0; j < kPer; ++j) {
-            x.lo[j] = *reinterpret_cast<const uint4*>(x.p + 64 * j + 8 * sub);
-            x.hi[j] = *reinterpret_cast<const uint4*>(x.p + HD + 64 * j + 8 * sub);
-          }
+          x.lo = *reinterpret_cast<const uint4*>(x.p + 8 * sub);
+          x.hi = *reinterpret_cast<const uint4*>(x.p + HD + 8 * sub);
         }
         return x;
       };
@@ -528,21 +519,17 @@ __global__ void __launch_bounds__(kChooseThreads)
       for (int round = 0; round < rounds; ++round) {
         const Bounds x = next;
         if (round + 1 < rounds) next = fetch(round + 1);
-        double s[kPer] = {};
+        double s[2] = {};
         if (x.p) {
+          float lo[8], hi[8];
+          bounds_values(x.lo, half, lo);
+          bounds_values(x.hi, half, hi);
 #pragma unroll
-          for (int j = 0; j < kPer; ++j) {
-            float lo[8], hi[8];
-            bounds_values(x.lo[j], half, lo);
-            bounds_values(x.hi[j], half, hi);
-#pragma unroll
-            for (int k = 0; k < 8; ++k) s[j] += up[j][k] * hi[k] + down[j][k] * lo[k];
-          }
+          for (int k = 0; k < 8; ++k) s[k & 1] += up[k] * hi[k] + down[k] * lo[k];
         }
-        double t = s[0];
-        if constexpr (kPer > 1) t += s[1];
+        double t = s[0] + s[1];
 #pragma unroll
-        for (int o = 4; o > 0; o >>= 1) t += __shfl_xor_sync(0xffffffffu, t, o);
+        for (int o = kLanes / 2; o > 0; o >>= 1) t += __shfl_xor_sync(0xffffffffu, t, o);
         if (t != t) t = CUDART_INF;  // a NaN counts as the largest score
         if (x.p && sub == 0) score[base + round * kRound] = t;
       }
@@ -595,6 +582,7 @@ __global__ void __launch_bounds__(kChooseThreads)
   if (threadIdx.x == 0) flag[3] = 0;
   if (free > 0) {
     double least = CUDART_INF, most = -CUDART_INF;
+#pragma unroll 4
     for (int j = lo_block + threadIdx.x; j < hi_block; j += kChooseThreads) {
       const double s = __ldcg(score + j);
       if (fits) dyn[j] = s;
@@ -695,8 +683,8 @@ cudaError_t launch_select(const SelectArgs& a_in, cudaStream_t s) {
   constexpr size_t kLimit = 32 * 1024;
   a.smem_blocks = bits < kLimit ? static_cast<int32_t>((kLimit - bits) / sizeof(double)) : 0;
   const size_t smem = bits + (a.max_blocks <= a.smem_blocks ? a.max_blocks * sizeof(double) : 0);
-  // Blocks of a CTA: 32 in one go of its warps while the CTAs are few, more where they would
-  // come in several waves (a CTA begins with the queries, whatever it scores).
+  // Blocks of a CTA: 32 while the CTAs are few, more where they would come in several waves (a
+  // CTA begins with the queries, whatever it scores).
   const int64_t pairs = static_cast<int64_t>(jobs) * a.cache.hkv;
   a.chunk = 32;
   while (a.chunk < kMaxChunk && pairs * ((a.max_blocks + a.chunk - 1) / a.chunk) > 2LL * a.num_sms) a.chunk *= 2;
