@@ -70,14 +70,16 @@ __device__ __forceinline__ void floats_of(const Raw8& r, int dt, float (&x)[8]) 
 }
 
 // Eight values of a cache row at dims d .. d + 7; four neighbouring lanes hold a block of 32.
+// KIND: kQ8_0, kQ4_0, or kF32 for the types that need no block.
+template <int KIND>
 __device__ __forceinline__ void store_cache8(const CacheView& c, int64_t row, int d, bool v,
                                              const float (&x)[8], bool live, uint32_t lanes) {
-  if (c.dtype <= kBF16) {
+  if constexpr (KIND == kF32) {
     if (live) store8(v ? c.v : c.k, static_cast<size_t>(row) * c.hd + d, c.dtype, x, true);
     return;
   }
   const int lane = threadIdx.x & 31;
-  if (c.dtype == kQ8_0) {  // q8_0_pair's rule
+  if constexpr (KIND == kQ8_0) {  // q8_0_pair's rule
     float amax = 0.f;
 #pragma unroll
     for (int k = 0; k < 8; ++k) amax = fmaxf(amax, fabsf(x[k]));
@@ -114,7 +116,7 @@ __device__ __forceinline__ void store_cache8(const CacheView& c, int64_t row, in
   }
   finite = (__ballot_sync(lanes, !finite) >> (lane & 28) & 15u) == 0;
   const uint16_t scale = q4_scale(m, finite);
-  const float s = __half2float(__ushort_as_half(scale)), inv = 1.f / s;
+  const float s = __half2float(__ushort_as_half(scale)), inv = q4_inverse(s);
   uint32_t w = 0x88888888u;
   if (scale != kHalfNan && s != 0.f) {
     w = 0;
@@ -159,116 +161,136 @@ __device__ __forceinline__ void load_cache8(const CacheView& c, int64_t row, int
   }
 }
 
-constexpr int kRowsPerGroup = 4;
+constexpr int kAtOnce = 4;  // rows whose loads a thread has under way together
 
 }  // namespace
 
 // ---------------------------------------------------------------- append --
 // A row of HD values takes HD / 8 lanes, eight values each: 16-byte loads, and four lanes a
-// block of 32.  A group of lanes takes up to kRowsPerGroup rows of one token (its query, key and
-// value heads in that order), loaded at once, and fetches the position's angles once for them.
-// HD 0: any head size, one warp per row (key and value rows of a head together).
-// Bound by the bytes for prompts: every row read once and written once.
-template <int HD>
-__global__ void __launch_bounds__(256) ragged_append_kernel(const __grid_constant__ RaggedAppendArgs a) {
-  const int64_t thread = static_cast<int64_t>(blockIdx.x) * blockDim.x + threadIdx.x;
+// block of 32.  The block's groups of lanes have a token each and take the same a.rows_each rows
+// of them (of the query, key and value heads in that order; blockIdx.y says which), kAtOnce at a
+// time; the position's angles are fetched once for all.  Neighbouring tokens stand in one warp,
+// whose stores of V codes then fill whole words.
+// IN: the input type, with every tensor 16-byte aligned; -1: read from the arguments, in any
+// place.  KIND: as store_cache8's.
+// Bound by the f64 rotation (reading the bits of f32 into f64 and back is done at a sixteenth
+// of the rate of f32 arithmetic) and the bytes, about alike.
+template <int HD, int IN, int KIND>
+__global__ void __launch_bounds__(256, 3) ragged_append_kernel(const __grid_constant__ RaggedAppendArgs a) {
+  constexpr int kLanes = HD / 8;
   const CacheView& c = a.cache;
-  if constexpr (HD == 0) {
-    const int64_t warp = thread >> 5;
-    const int lane = threadIdx.x & 31;
-    const int heads = a.hq + c.hkv, hd = c.hd;
-    const int64_t r64 = warp / heads;
-    if (r64 >= a.rows.first[a.batch]) return;
-    const int r = static_cast<int>(r64), h = static_cast<int>(warp - r64 * heads);
-    const int b = ragged_seq(a.rows, a.batch, r);
-    const int pos = a.rows.start[b] + r - a.rows.first[b];
-    const double2* rope = a.rope ? a.rope + static_cast<size_t>(pos) * (hd / 2) : nullptr;
-    if (h < a.hq) {
-      const size_t in = static_cast<size_t>(r) * a.q_stride + static_cast<size_t>(h) * hd;
-      const size_t out = (static_cast<size_t>(r) * a.hq + h) * hd;
-      for (int p = lane; p < hd / 2; p += 32) {
-        float y0 = load_elem(a.q, in + 2 * p, a.in_dtype);
-        float y1 = load_elem(a.q, in + 2 * p + 1, a.in_dtype);
-        if (rope) rope_pair(y0, y1, rope[p], y0, y1);
-        store_elem(a.q_out, out + 2 * p, a.q_out_dtype, y0);
-        store_elem(a.q_out, out + 2 * p + 1, a.q_out_dtype, y1);
-      }
-      return;
-    }
-    const int kvh = h - a.hq;
-    bool ok;
-    const int64_t dst = cache_row(c, a.rows.seq[b], pos, kvh, a.status, ok);
-    if (!ok) return;
-    append_row(a.k, a.v, a.in_dtype,
-               static_cast<size_t>(r) * a.k_stride + static_cast<size_t>(kvh) * hd,
-               static_cast<size_t>(r) * a.v_stride + static_cast<size_t>(kvh) * hd, rope, c, dst, lane);
-  } else {
-    constexpr int kLanes = HD / 8;
-    const uint32_t lanes =  // of this group, for its shuffles
-        (kLanes == 32 ? 0xffffffffu : (1u << kLanes) - 1) << (threadIdx.x & 31 & ~(kLanes - 1));
-    const int heads = a.hq + 2 * c.hkv;
-    const int chunks = (heads + kRowsPerGroup - 1) / kRowsPerGroup;
-    const int64_t group = thread / kLanes;
-    const int64_t r64 = group / chunks;
-    if (r64 >= a.rows.first[a.batch]) return;
-    const int r = static_cast<int>(r64);
-    const int h0 = static_cast<int>(group - r64 * chunks) * kRowsPerGroup;
-    const int d = static_cast<int>(thread % kLanes) * 8;
-    const int b = ragged_seq(a.rows, a.batch, r);
-    const int pos = a.rows.start[b] + r - a.rows.first[b];
-    Raw8 raw[kRowsPerGroup];
+  const int in_dt = IN >= 0 ? IN : a.in_dtype;
+  const int r = static_cast<int>(blockIdx.x) * (256 / kLanes) + threadIdx.x / kLanes;
+  if (r >= a.rows.first[a.batch]) return;
+  const uint32_t lanes =  // of this group, for its shuffles
+      ((1u << kLanes) - 1) << (threadIdx.x & 31 & ~(kLanes - 1));
+  const int heads = a.hq + 2 * c.hkv;
+  const int h0 = blockIdx.y * a.rows_each, h1 = min(h0 + a.rows_each, heads);
+  const int d = threadIdx.x % kLanes * 8;
+  const int b = ragged_seq(a.rows, a.batch, r);
+  const int pos = a.rows.start[b] + r - a.rows.first[b];
+  double2 cs[4];
+  const bool turn = a.rope && h0 < a.hq + c.hkv;
+  if (turn) {
+    const double2* p = a.rope + static_cast<size_t>(pos) * (HD / 2) + d / 2;
 #pragma unroll
-    for (int i = 0; i < kRowsPerGroup; ++i) {
-      const int h = h0 + i;
-      if (h < a.hq)
-        raw[i] = load_raw8(a.q, static_cast<size_t>(r) * a.q_stride + static_cast<size_t>(h) * HD + d,
-                           a.in_dtype, a.vec & 1);
-      else if (h < a.hq + c.hkv)
-        raw[i] = load_raw8(a.k, static_cast<size_t>(r) * a.k_stride +
-                                    static_cast<size_t>(h - a.hq) * HD + d,
-                           a.in_dtype, a.vec & 2);
-      else if (h < heads)
-        raw[i] = load_raw8(a.v, static_cast<size_t>(r) * a.v_stride +
-                                    static_cast<size_t>(h - a.hq - c.hkv) * HD + d,
-                           a.in_dtype, a.vec & 4);
-    }
-    double2 cs[4];
-    const bool turn = a.rope && h0 < a.hq + c.hkv;
-    if (turn) {
-      const double2* p = a.rope + static_cast<size_t>(pos) * (HD / 2) + d / 2;
+    for (int k = 0; k < 4; ++k) cs[k] = p[k];
+  }
+  bool ok = true;
+  int64_t row0 = 0;
+  if (h1 > a.hq) row0 = cache_row(c, a.rows.seq[b], pos, 0, a.status, ok);
+  for (int g0 = h0; g0 < h1; g0 += kAtOnce) {
+    Raw8 raw[kAtOnce];
 #pragma unroll
-      for (int k = 0; k < 4; ++k) cs[k] = p[k];
+    for (int i = 0; i < kAtOnce; ++i) {
+      const int h = min(g0 + i, h1 - 1);
+      const bool q = h < a.hq, k = h < a.hq + c.hkv;
+      const void* base = q ? a.q : k ? a.k : a.v;
+      const int64_t stride = q ? a.q_stride : k ? a.k_stride : a.v_stride;
+      const int in_row = h - (q ? 0 : k ? a.hq : a.hq + c.hkv);
+      raw[i] = load_raw8(base, static_cast<size_t>(r) * stride + static_cast<size_t>(in_row) * HD + d,
+                         in_dt, IN >= 0 || a.vec >> (q ? 0 : k ? 1 : 2) & 1);
     }
-    bool ok = true;
-    int64_t row0 = 0;
-    if (h0 + kRowsPerGroup > a.hq)
-      row0 = cache_row(c, a.rows.seq[b], pos, 0, a.status, ok);
 #pragma unroll
-    for (int i = 0; i < kRowsPerGroup; ++i) {
-      const int h = h0 + i;
-      if (h >= heads) break;
+    for (int i = 0; i < kAtOnce; ++i) {
+      const int h = g0 + i;
+      if (h >= h1) break;
       float x[8];
-      floats_of(raw[i], a.in_dtype, x);
+      floats_of(raw[i], in_dt, x);
       if (turn && h < a.hq + c.hkv) {
 #pragma unroll
         for (int k = 0; k < 4; ++k) rope_pair(x[2 * k], x[2 * k + 1], cs[k], x[2 * k], x[2 * k + 1]);
       }
       if (h < a.hq) {
-        store8(a.q_out, (static_cast<size_t>(r) * a.hq + h) * HD + d, a.q_out_dtype, x, a.vec & 8);
+        store8(a.q_out, (static_cast<size_t>(r) * a.hq + h) * HD + d, a.q_out_dtype, x,
+               IN >= 0 || (a.vec & 8) != 0);
       } else {
         const bool v = h >= a.hq + c.hkv;
         const int kvh = h - a.hq - (v ? c.hkv : 0);
-        store_cache8(c, row0 + static_cast<int64_t>(kvh) * c.page, d, v, x, ok, lanes);
+        store_cache8<KIND>(c, row0 + static_cast<int64_t>(kvh) * c.page, d, v, x, ok, lanes);
       }
     }
   }
 }
 
+// Any head size: one warp per query row, or per key and value row of a KV head.
+__global__ void __launch_bounds__(128) ragged_append_any_kernel(const __grid_constant__ RaggedAppendArgs a) {
+  const int64_t warp = (static_cast<int64_t>(blockIdx.x) * blockDim.x + threadIdx.x) >> 5;
+  const int lane = threadIdx.x & 31;
+  const CacheView& c = a.cache;
+  const int heads = a.hq + c.hkv, hd = c.hd;
+  const int64_t r64 = warp / heads;
+  if (r64 >= a.rows.first[a.batch]) return;
+  const int r = static_cast<int>(r64), h = static_cast<int>(warp - r64 * heads);
+  const int b = ragged_seq(a.rows, a.batch, r);
+  const int pos = a.rows.start[b] + r - a.rows.first[b];
+  const double2* rope = a.rope ? a.rope + static_cast<size_t>(pos) * (hd / 2) : nullptr;
+  if (h < a.hq) {
+    const size_t in = static_cast<size_t>(r) * a.q_stride + static_cast<size_t>(h) * hd;
+    const size_t out = (static_cast<size_t>(r) * a.hq + h) * hd;
+    for (int p = lane; p < hd / 2; p += 32) {
+      float y0 = load_elem(a.q, in + 2 * p, a.in_dtype);
+      float y1 = load_elem(a.q, in + 2 * p + 1, a.in_dtype);
+      if (rope) rope_pair(y0, y1, rope[p], y0, y1);
+      store_elem(a.q_out, out + 2 * p, a.q_out_dtype, y0);
+      store_elem(a.q_out, out + 2 * p + 1, a.q_out_dtype, y1);
+    }
+    return;
+  }
+  const int kvh = h - a.hq;
+  bool ok;
+  const int64_t dst = cache_row(c, a.rows.seq[b], pos, kvh, a.status, ok);
+  if (!ok) return;
+  append_row(a.k, a.v, a.in_dtype, static_cast<size_t>(r) * a.k_stride + static_cast<size_t>(kvh) * hd,
+             static_cast<size_t>(r) * a.v_stride + static_cast<size_t>(kvh) * hd, rope, c, dst, lane);
+}
+
+namespace {
+
+using AppendFn = void (*)(const RaggedAppendArgs);
+
+template <int HD, int IN>
+AppendFn append_form(int dtype) {
+  return dtype == kQ4_0   ? ragged_append_kernel<HD, IN, kQ4_0>
+         : dtype == kQ8_0 ? ragged_append_kernel<HD, IN, kQ8_0>
+                          : ragged_append_kernel<HD, IN, kF32>;
+}
+
+template <int HD>
+AppendFn append_form(int in_dt, int dtype) {
+  return in_dt == kF32    ? append_form<HD, kF32>(dtype)
+         : in_dt == kF16  ? append_form<HD, kF16>(dtype)
+         : in_dt == kBF16 ? append_form<HD, kBF16>(dtype)
+                          : append_form<HD, -1>(dtype);
+}
+
+}  // namespace
+
 cudaError_t launch_ragged_append(const RaggedAppendArgs& a_in, cudaStream_t s) {
   RaggedAppendArgs a = a_in;
   const int64_t tokens = a.rows.first[a.batch];
   if (tokens == 0) return cudaSuccess;
-  const int hd = a.cache.hd;
+  const int hd = a.cache.hd, heads = a.hq + 2 * a.cache.hkv;
   // 16-byte accesses where the base and every row allow them
   const int64_t per = a.in_dtype == kF32 ? 4 : 8;
   auto fits = [](const void* p) { return reinterpret_cast<uintptr_t>(p) % 16 == 0; };
@@ -276,16 +298,17 @@ cudaError_t launch_ragged_append(const RaggedAppendArgs& a_in, cudaStream_t s) {
           (fits(a.v) && a.v_stride % per == 0 ? 4 : 0) | (fits(a.q_out) ? 8 : 0);
   if (hd != 64 && hd != 128) {
     const int64_t threads = tokens * (a.hq + a.cache.hkv) * 32;
-    ragged_append_kernel<0><<<static_cast<unsigned>((threads + 255) / 256), 256, 0, s>>>(a);
+    ragged_append_any_kernel<<<static_cast<unsigned>((threads + 127) / 128), 128, 0, s>>>(a);
     return cudaGetLastError();
   }
-  const int chunks = (a.hq + 2 * a.cache.hkv + kRowsPerGroup - 1) / kRowsPerGroup;
-  const int64_t threads = tokens * chunks * (hd / 8);
-  const unsigned blocks = static_cast<unsigned>((threads + 255) / 256);
-  if (hd == 64)
-    ragged_append_kernel<64><<<blocks, 256, 0, s>>>(a);
-  else
-    ragged_append_kernel<128><<<blocks, 256, 0, s>>>(a);
+  // Rows of a thread: kAtOnce, or twice as many where the blocks are many waves anyway (the angles
+  // are then read half as often).
+  const int64_t blocks = (tokens * (hd / 8) + 255) / 256;
+  const int chunks = (heads + kAtOnce - 1) / kAtOnce;
+  a.rows_each = blocks * chunks > 4096 ? 2 * kAtOnce : kAtOnce;
+  const int in = a.vec == 15 ? a.in_dtype : -1;
+  const AppendFn k = hd == 64 ? append_form<64>(in, a.cache.dtype) : append_form<128>(in, a.cache.dtype);
+  k<<<dim3(static_cast<unsigned>(blocks), (heads + a.rows_each - 1) / a.rows_each), 256, 0, s>>>(a);
   return cudaGetLastError();
 }
 

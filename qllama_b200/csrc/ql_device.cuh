@@ -469,16 +469,22 @@ __device__ __forceinline__ uint16_t q4_scale(float m, bool finite) {
   return !finite || __hisinf(d) ? kHalfNan : __half_as_ushort(d);
 }
 
-// round(x / d) without a division: x * (1 / d) rounded is at most one off next to a tie,
-// and the remainder x - k d, exact in f32 (d has 11 bits, k five, |remainder| <= |x|),
-// says where the nearest multiple lies.
+// The code of x, round(x / d) + 8 clamped, without a division.  t = x / d + 1.5 2^23 rounds to a
+// whole number k in its last places; with a reciprocal that is one unit off k is at most one off,
+// next to a tie, and the remainder x - k d, exact in f32 (d has 11 bits, k five, and the
+// remainder is not above x), says so.
 __device__ __forceinline__ uint32_t q4_code(float x, float d, float inv) {
-  float k = rintf(x * inv);
+  constexpr float kMagic = 12582912.f;
+  const float t = fmaf(x, inv, kMagic), k = t - kMagic;
   const float e = fmaf(-k, d, x), half = 0.5f * fabsf(d);
-  const float up = (e < 0.f) == (d < 0.f) ? 1.f : -1.f;  // the direction of the remainder
-  const bool odd = (static_cast<int>(k) & 1) != 0;
-  if (fabsf(e) > half || (fabsf(e) == half && odd)) k += up;
-  return static_cast<uint32_t>(static_cast<int>(fminf(fmaxf(k, -8.f), 7.f)) + 8);
+  int c = __float_as_int(t) - (__float_as_int(kMagic) - 8);
+  if (fabsf(e) >= half && (fabsf(e) > half || (c & 1))) c += (e < 0.f) == (d < 0.f) ? 1 : -1;
+  return static_cast<uint32_t>(min(max(c, 0), 15));
+}
+__device__ __forceinline__ float q4_inverse(float d) {
+  float y;
+  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(d));
+  return y;
 }
 
 // One block held as 16 pairs by 16 consecutive lanes (the quantiser of q8_0_pair's layout):
@@ -496,7 +502,7 @@ __device__ __forceinline__ uint32_t q4_0_pair(float x0, float x1, uint16_t& scal
   scale = q4_scale(top, bad == 0);
   const float d = __half2float(__ushort_as_half(scale));
   if (bad || scale == kHalfNan || d == 0.f) return 0x88u;
-  const float inv = 1.f / d;
+  const float inv = q4_inverse(d);
   return q4_code(x0, d, inv) | q4_code(x1, d, inv) << 4;
 }
 

@@ -218,6 +218,7 @@ struct RaggedAppendArgs {
   void* q_out;    // [tokens][hq][hd]
   int64_t q_stride, k_stride, v_stride;  // elements from token to token
   int32_t vec;    // set by the launch: which of q, k, v and q_out allow 16-byte accesses
+  int32_t rows_each;  // set by the launch: rows of a token that a thread takes part in
   int32_t in_dtype;
   int32_t q_out_dtype;
   int32_t hq;
