@@ -69,16 +69,54 @@ __device__ __forceinline__ void floats_of(const Raw8& r, int dt, float (&x)[8]) 
   }
 }
 
-// Eight values of a cache row at dims d .. d + 7; four neighbouring lanes hold a block of 32.
-// KIND: kQ8_0, kQ4_0, or kF32 for the types that need no block.
+// Where one thread's dims d .. d + 7 of a position lie in the cache, for KV head 0, and the bytes
+// from head to head: computed once for all heads.
+struct RowPlace {
+  uint8_t *k, *v, *v2, *ks, *vs;  // v2: of dims d + 4 .. (Q4_0); ks, vs: the block's scale
+  size_t step, scale_step;
+};
+
 template <int KIND>
-__device__ __forceinline__ void store_cache8(const CacheView& c, int64_t row, int d, bool v,
+__device__ __forceinline__ RowPlace row_place(const CacheView& c, int page, int pos, int d) {
+  RowPlace p;
+  const int off = pos % c.page;
+  const size_t row = static_cast<size_t>(page) * c.hkv * c.page + off;
+  if constexpr (KIND == kQ4_0) {
+    const Q4Record rec{c.hd};
+    const int per = c.page / kTile, nb = c.hd / 32, at = off % kTile;
+    uint8_t* base = static_cast<uint8_t*>(c.k) +
+                    (static_cast<size_t>(page) * c.hkv * per + off / kTile) * rec.bytes();
+    p.k = base + q4_k_byte(at, d, nb);
+    p.v = base + rec.v_codes() + q4_v_byte(at, d, nb);
+    p.v2 = base + rec.v_codes() + q4_v_byte(at, d + 4, nb);
+    p.ks = base + rec.k_scales() + 2 * q4_k_scale(at, d / 32, nb);
+    p.vs = base + rec.v_scales() + 2 * q4_v_scale(at, d / 32, nb);
+    p.step = p.scale_step = per * rec.bytes();
+  } else {
+    const size_t size = KIND == kQ8_0 ? 1 : c.dtype == kF32 ? 4 : 2;
+    p.k = static_cast<uint8_t*>(c.k) + (row * c.hd + d) * size;
+    p.v = static_cast<uint8_t*>(c.v) + (row * c.hd + d) * size;
+    p.v2 = nullptr;
+    p.step = static_cast<size_t>(c.page) * c.hd * size;
+    p.ks = KIND == kQ8_0 ? reinterpret_cast<uint8_t*>(c.k_scale + row * (c.hd / 32) + d / 32) : nullptr;
+    p.vs = KIND == kQ8_0 ? reinterpret_cast<uint8_t*>(c.v_scale + row * (c.hd / 32) + d / 32) : nullptr;
+    p.scale_step = static_cast<size_t>(c.page) * (c.hd / 32) * 2;
+  }
+  return p;
+}
+
+// Writes eight values of KV head h; four neighbouring lanes hold a block of 32.  KIND: kQ8_0,
+// kQ4_0, or kF32 for the types that need no block.
+template <int KIND>
+__device__ __forceinline__ void store_cache8(const RowPlace& p, int dtype, int h, bool v,
                                              const float (&x)[8], bool live, uint32_t lanes) {
+  uint8_t* at = (v ? p.v : p.k) + h * p.step;
   if constexpr (KIND == kF32) {
-    if (live) store8(v ? c.v : c.k, static_cast<size_t>(row) * c.hd + d, c.dtype, x, true);
+    if (live) store8(at, 0, dtype, x, true);
     return;
   }
   const int lane = threadIdx.x & 31;
+  uint16_t* scale_at = reinterpret_cast<uint16_t*>((v ? p.vs : p.ks) + h * p.scale_step);
   if constexpr (KIND == kQ8_0) {  // q8_0_pair's rule
     float amax = 0.f;
 #pragma unroll
@@ -93,11 +131,8 @@ __device__ __forceinline__ void store_cache8(const CacheView& c, int64_t row, in
       w[k / 4] |= (static_cast<uint32_t>(r == r ? static_cast<int>(r) : 0) & 0xffu) << (8 * (k & 3));
     }
     if (live) {
-      *reinterpret_cast<uint2*>(static_cast<int8_t*>(v ? c.v : c.k) +
-                                static_cast<size_t>(row) * c.hd + d) = make_uint2(w[0], w[1]);
-      if ((lane & 3) == 0)
-        (v ? c.v_scale : c.k_scale)[static_cast<size_t>(row) * (c.hd / 32) + d / 32] =
-            __half_as_ushort(__float2half_rn(s));
+      *reinterpret_cast<uint2*>(at) = make_uint2(w[0], w[1]);
+      if ((lane & 3) == 0) *scale_at = __half_as_ushort(__float2half_rn(s));
     }
     return;
   }
@@ -116,49 +151,51 @@ __device__ __forceinline__ void store_cache8(const CacheView& c, int64_t row, in
   }
   finite = (__ballot_sync(lanes, !finite) >> (lane & 28) & 15u) == 0;
   const uint16_t scale = q4_scale(m, finite);
-  const float s = __half2float(__ushort_as_half(scale)), inv = q4_inverse(s);
-  uint32_t w = 0x88888888u;
-  if (scale != kHalfNan && s != 0.f) {
-    w = 0;
-#pragma unroll
-    for (int k = 0; k < 8; ++k) w |= q4_code(x[k], s, inv) << (4 * k);
-  }
+  const float s = __half2float(__ushort_as_half(scale));
+  const uint32_t w = scale == kHalfNan || s == 0.f ? 0x88888888u : q4_codes8(x, s, q4_inverse(s));
   if (!live) return;
-  uint8_t* at = q4_code_at(c, row, d, v);
   if (v) {  // two lanes' places
     *reinterpret_cast<uint16_t*>(at) = static_cast<uint16_t>(w);
-    *reinterpret_cast<uint16_t*>(q4_code_at(c, row, d + 4, true)) = static_cast<uint16_t>(w >> 16);
+    *reinterpret_cast<uint16_t*>(p.v2 + h * p.step) = static_cast<uint16_t>(w >> 16);
   } else {
     *reinterpret_cast<uint32_t*>(at) = w;
   }
-  if ((lane & 3) == 0) *q4_scale_at(c, row, d / 32, v) = scale;
+  if ((lane & 3) == 0) *scale_at = scale;
 }
 
-// The converse: eight values of a cache row.
-__device__ __forceinline__ void load_cache8(const CacheView& c, int64_t row, int d, bool v,
+// The converse: eight values of KV head h.
+template <int KIND>
+__device__ __forceinline__ void load_cache8(const RowPlace& p, int dtype, int h, bool v,
                                             float (&x)[8]) {
-  if (c.dtype <= kBF16) {
-    floats_of(load_raw8(v ? c.v : c.k, static_cast<size_t>(row) * c.hd + d, c.dtype, true), c.dtype, x);
-  } else if (c.dtype == kQ8_0) {
-    const uint2 w = *reinterpret_cast<const uint2*>(static_cast<const int8_t*>(v ? c.v : c.k) +
-                                                    static_cast<size_t>(row) * c.hd + d);
-    const float s = __half2float(__ushort_as_half(
-        (v ? c.v_scale : c.k_scale)[static_cast<size_t>(row) * (c.hd / 32) + d / 32]));
+  const uint8_t* at = (v ? p.v : p.k) + h * p.step;
+  if constexpr (KIND == kF32) {
+    floats_of(load_raw8(at, 0, dtype, true), dtype, x);
+    return;
+  }
+  const float s = __half2float(__ushort_as_half(
+      *reinterpret_cast<const uint16_t*>((v ? p.vs : p.ks) + h * p.scale_step)));
+  if constexpr (KIND == kQ8_0) {
+    const uint2 w = *reinterpret_cast<const uint2*>(at);
 #pragma unroll
     for (int k = 0; k < 8; ++k)
       x[k] = s * static_cast<float>(static_cast<int8_t>((k < 4 ? w.x : w.y) >> (8 * (k & 3))));
   } else {
-    const uint8_t* at = q4_code_at(c, row, d, v);
     const uint32_t w =
         v ? *reinterpret_cast<const uint16_t*>(at) |
-                static_cast<uint32_t>(*reinterpret_cast<const uint16_t*>(q4_code_at(c, row, d + 4, true)))
-                    << 16
+                static_cast<uint32_t>(*reinterpret_cast<const uint16_t*>(p.v2 + h * p.step)) << 16
           : *reinterpret_cast<const uint32_t*>(at);
-    const float s = __half2float(__ushort_as_half(*q4_scale_at(c, row, d / 32, v)));
 #pragma unroll
     for (int k = 0; k < 8; ++k)
       x[k] = s * static_cast<float>(static_cast<int>(w >> (4 * k) & 15u) - 8);
   }
+}
+
+// The page of a position, -1 (and the status raised) if the table's entry is outside the pool.
+__device__ __forceinline__ int page_of(const CacheView& c, int seq, int pos, uint32_t* status) {
+  const int page = c.block_table[static_cast<size_t>(seq) * c.pages_per_seq + pos / c.page];
+  if (page >= 0 && page < c.num_pages) return page;
+  if (status) atomicOr(status, kStatusBadPage);
+  return -1;
 }
 
 constexpr int kAtOnce = 4;  // rows whose loads a thread has under way together
@@ -196,20 +233,28 @@ __global__ void __launch_bounds__(256, 3) ragged_append_kernel(const __grid_cons
 #pragma unroll
     for (int k = 0; k < 4; ++k) cs[k] = p[k];
   }
-  bool ok = true;
-  int64_t row0 = 0;
-  if (h1 > a.hq) row0 = cache_row(c, a.rows.seq[b], pos, 0, a.status, ok);
+  int page = 0;
+  RowPlace place{};
+  if (h1 > a.hq) {
+    page = page_of(c, a.rows.seq[b], pos, a.status);
+    place = row_place<KIND>(c, max(page, 0), pos, d);
+  }
+  const int size = in_dt == kF32 ? 4 : 2, out_size = a.q_out_dtype == kF32 ? 4 : 2;
+  const size_t tok = static_cast<size_t>(r);
+  const uint8_t* q_at = static_cast<const uint8_t*>(a.q) + (tok * a.q_stride + d) * size;
+  const uint8_t* k_at = static_cast<const uint8_t*>(a.k) + (tok * a.k_stride + d) * size;
+  const uint8_t* v_at = static_cast<const uint8_t*>(a.v) + (tok * a.v_stride + d) * size;
+  uint8_t* out_at = static_cast<uint8_t*>(a.q_out) + (tok * a.hq * HD + d) * out_size;
   for (int g0 = h0; g0 < h1; g0 += kAtOnce) {
     Raw8 raw[kAtOnce];
 #pragma unroll
     for (int i = 0; i < kAtOnce; ++i) {
       const int h = min(g0 + i, h1 - 1);
       const bool q = h < a.hq, k = h < a.hq + c.hkv;
-      const void* base = q ? a.q : k ? a.k : a.v;
-      const int64_t stride = q ? a.q_stride : k ? a.k_stride : a.v_stride;
+      const uint8_t* at = q ? q_at : k ? k_at : v_at;
       const int in_row = h - (q ? 0 : k ? a.hq : a.hq + c.hkv);
-      raw[i] = load_raw8(base, static_cast<size_t>(r) * stride + static_cast<size_t>(in_row) * HD + d,
-                         in_dt, IN >= 0 || a.vec >> (q ? 0 : k ? 1 : 2) & 1);
+      raw[i] = load_raw8(at + in_row * HD * size, 0, in_dt,
+                         IN >= 0 || a.vec >> (q ? 0 : k ? 1 : 2) & 1);
     }
 #pragma unroll
     for (int i = 0; i < kAtOnce; ++i) {
@@ -222,12 +267,10 @@ __global__ void __launch_bounds__(256, 3) ragged_append_kernel(const __grid_cons
         for (int k = 0; k < 4; ++k) rope_pair(x[2 * k], x[2 * k + 1], cs[k], x[2 * k], x[2 * k + 1]);
       }
       if (h < a.hq) {
-        store8(a.q_out, (static_cast<size_t>(r) * a.hq + h) * HD + d, a.q_out_dtype, x,
-               IN >= 0 || (a.vec & 8) != 0);
+        store8(out_at + h * HD * out_size, 0, a.q_out_dtype, x, IN >= 0 || (a.vec & 8) != 0);
       } else {
         const bool v = h >= a.hq + c.hkv;
-        const int kvh = h - a.hq - (v ? c.hkv : 0);
-        store_cache8<KIND>(c, row0 + static_cast<int64_t>(kvh) * c.page, d, v, x, ok, lanes);
+        store_cache8<KIND>(place, c.dtype, h - a.hq - (v ? c.hkv : 0), v, x, page >= 0, lanes);
       }
     }
   }
@@ -313,52 +356,79 @@ cudaError_t launch_ragged_append(const RaggedAppendArgs& a_in, cudaStream_t s) {
 }
 
 // ------------------------------------------------------------------ read --
-// As the append: a row's K and V by HD / 8 lanes; HD 0: one warp per (token, KV head).
-template <int HD>
+// As the append: HD / 8 lanes have a token and read kAtOnce KV heads of it (blockIdx.y says
+// which), K and V.
+template <int HD, int KIND>
 __global__ void __launch_bounds__(256) ragged_read_kernel(const __grid_constant__ RaggedReadArgs a) {
-  constexpr int kLanes = HD == 0 ? 32 : HD / 8;
-  const int64_t thread = static_cast<int64_t>(blockIdx.x) * blockDim.x + threadIdx.x;
+  constexpr int kLanes = HD / 8;
   const CacheView& c = a.cache;
-  const int64_t unit = thread / kLanes, r64 = unit / c.hkv;
+  const int r = static_cast<int>(blockIdx.x) * (256 / kLanes) + threadIdx.x / kLanes;
+  if (r >= a.rows.first[a.batch]) return;
+  const int d = threadIdx.x % kLanes * 8;
+  const int b = ragged_seq(a.rows, a.batch, r);
+  const int pos = a.rows.start[b] + r - a.rows.first[b];
+  const int page = page_of(c, a.rows.seq[b], pos, a.status);
+  const RowPlace place = row_place<KIND>(c, max(page, 0), pos, d);
+  const int h0 = blockIdx.y * kAtOnce;
+  float k[kAtOnce][8], v[kAtOnce][8];
+#pragma unroll
+  for (int i = 0; i < kAtOnce; ++i) {
+    const int h = min(h0 + i, c.hkv - 1);
+    load_cache8<KIND>(place, c.dtype, h, false, k[i]);
+    load_cache8<KIND>(place, c.dtype, h, true, v[i]);
+  }
+#pragma unroll
+  for (int i = 0; i < kAtOnce; ++i) {
+    if (h0 + i >= c.hkv) break;
+    if (page < 0) {
+#pragma unroll
+      for (int e = 0; e < 8; ++e) k[i][e] = v[i][e] = 0.f;
+    }
+    const size_t o = (static_cast<size_t>(r) * c.hkv + h0 + i) * HD + d;
+    store8(a.k_out, o, a.out_dtype, k[i], a.vec & 1);
+    store8(a.v_out, o, a.out_dtype, v[i], a.vec & 2);
+  }
+}
+
+// Any head size: one warp per (token, KV head).
+__global__ void __launch_bounds__(128) ragged_read_any_kernel(const __grid_constant__ RaggedReadArgs a) {
+  const int64_t warp = (static_cast<int64_t>(blockIdx.x) * blockDim.x + threadIdx.x) >> 5;
+  const CacheView& c = a.cache;
+  const int64_t r64 = warp / c.hkv;
   if (r64 >= a.rows.first[a.batch]) return;
-  const int r = static_cast<int>(r64), h = static_cast<int>(unit - r64 * c.hkv);
+  const int r = static_cast<int>(r64), h = static_cast<int>(warp - r64 * c.hkv);
   const int b = ragged_seq(a.rows, a.batch, r);
   bool ok;
   const int64_t row = cache_row(c, a.rows.seq[b], a.rows.start[b] + r - a.rows.first[b], h,
                                 a.status, ok);
-  const size_t o = static_cast<size_t>(unit) * c.hd;
-  if constexpr (HD == 0) {
-    for (int d = threadIdx.x & 31; d < c.hd; d += 32) {
-      store_elem(a.k_out, o + d, a.out_dtype, ok ? cache_value(c, false, row, d) : 0.f);
-      store_elem(a.v_out, o + d, a.out_dtype, ok ? cache_value(c, true, row, d) : 0.f);
-    }
-  } else {
-    const int d = static_cast<int>(thread % kLanes) * 8;
-    float k[8] = {}, v[8] = {};
-    if (ok) {
-      load_cache8(c, row, d, false, k);
-      load_cache8(c, row, d, true, v);
-    }
-    store8(a.k_out, o + d, a.out_dtype, k, a.vec & 1);
-    store8(a.v_out, o + d, a.out_dtype, v, a.vec & 2);
+  const size_t o = static_cast<size_t>(warp) * c.hd;
+  for (int d = threadIdx.x & 31; d < c.hd; d += 32) {
+    store_elem(a.k_out, o + d, a.out_dtype, ok ? cache_value(c, false, row, d) : 0.f);
+    store_elem(a.v_out, o + d, a.out_dtype, ok ? cache_value(c, true, row, d) : 0.f);
   }
 }
 
 cudaError_t launch_ragged_read(const RaggedReadArgs& a_in, cudaStream_t s) {
   RaggedReadArgs a = a_in;
-  const int64_t rows = static_cast<int64_t>(a.rows.first[a.batch]) * a.cache.hkv;
-  if (rows == 0) return cudaSuccess;
+  const int64_t tokens = a.rows.first[a.batch];
+  if (tokens == 0) return cudaSuccess;
   a.vec = (reinterpret_cast<uintptr_t>(a.k_out) % 16 == 0 ? 1 : 0) |
           (reinterpret_cast<uintptr_t>(a.v_out) % 16 == 0 ? 2 : 0);
-  const int hd = a.cache.hd;
-  const int64_t threads = rows * (hd == 64 || hd == 128 ? hd / 8 : 32);
-  const unsigned blocks = static_cast<unsigned>((threads + 255) / 256);
-  if (hd == 64)
-    ragged_read_kernel<64><<<blocks, 256, 0, s>>>(a);
-  else if (hd == 128)
-    ragged_read_kernel<128><<<blocks, 256, 0, s>>>(a);
-  else
-    ragged_read_kernel<0><<<blocks, 256, 0, s>>>(a);
+  const int hd = a.cache.hd, dt = a.cache.dtype;
+  if (hd != 64 && hd != 128) {
+    const int64_t threads = tokens * a.cache.hkv * 32;
+    ragged_read_any_kernel<<<static_cast<unsigned>((threads + 127) / 128), 128, 0, s>>>(a);
+    return cudaGetLastError();
+  }
+  const dim3 grid(static_cast<unsigned>((tokens * (hd / 8) + 255) / 256),
+                  (a.cache.hkv + kAtOnce - 1) / kAtOnce);
+  const auto k = hd == 64 ? dt == kQ4_0   ? ragged_read_kernel<64, kQ4_0>
+                            : dt == kQ8_0 ? ragged_read_kernel<64, kQ8_0>
+                                          : ragged_read_kernel<64, kF32>
+                 : dt == kQ4_0 ? ragged_read_kernel<128, kQ4_0>
+                 : dt == kQ8_0 ? ragged_read_kernel<128, kQ8_0>
+                               : ragged_read_kernel<128, kF32>;
+  k<<<grid, 256, 0, s>>>(a);
   return cudaGetLastError();
 }
 

@@ -481,6 +481,27 @@ __device__ __forceinline__ uint32_t q4_code(float x, float d, float inv) {
   if (fabsf(e) >= half && (fabsf(e) > half || (c & 1))) c += (e < 0.f) == (d < 0.f) ? 1 : -1;
   return static_cast<uint32_t>(min(max(c, 0), 15));
 }
+// Eight codes in a word, the first in the low four bits.  Each rounded t is clamped as it is and
+// its low bits are the code; the words' sum, each shifted by a product, leaves the constant parts
+// to be taken off at once.  Where any remainder reaches half a step, all go by q4_code.
+__device__ __forceinline__ uint32_t q4_codes8(const float (&x)[8], float d, float inv) {
+  constexpr float kMagic = 12582912.f + 8.f;  // 0x4b400008
+  const float half = 0.5f * fabsf(d);
+  uint32_t w = 0u - 0x4b400000u * 0x11111111u;
+  bool near = false;
+#pragma unroll
+  for (int k = 0; k < 8; ++k) {
+    const float t = fmaf(x[k], inv, kMagic);
+    near |= fabsf(fmaf(kMagic - t, d, x[k])) >= half;
+    w += __float_as_uint(fminf(fmaxf(t, kMagic - 8.f), kMagic + 7.f)) * (1u << (4 * k));
+  }
+  if (near) {
+    w = 0;
+#pragma unroll
+    for (int k = 0; k < 8; ++k) w |= q4_code(x[k], d, inv) << (4 * k);
+  }
+  return w;
+}
 __device__ __forceinline__ float q4_inverse(float d) {
   float y;
   asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(d));
