@@ -196,6 +196,17 @@ def _positions(positions) -> np.ndarray:
     return np.ascontiguousarray(positions, dtype=np.int32)
 
 
+_model = None  # the module qllama_b200.model, at the first call that needs it
+
+
+def _import_model():
+    global _model
+    from . import model
+
+    _model = model
+    return model
+
+
 _identity = {}  # batch -> the sequences 0 .. batch - 1
 
 
@@ -319,8 +330,7 @@ class KvCache:
         position start_pos[b] on.  Returns the rotated queries (q_out, or a new tensor
         of q's type), None without q.
         """
-        from . import model as m
-
+        m = _model or _import_model()
         L = m._L or m._start()
         ctx, hkv, hd, dtype = self.ctx, self.num_kv_heads, self.head_dim, k.dtype
         dev = ctx.device
@@ -369,8 +379,7 @@ class KvCache:
         positions of sequence seq_ids[b] (default b) from start_pos[b] on, packed into
         (k, v), each [tokens, num_kv_heads, head_dim] of out_dtype (default: the cache's
         type, f32 for Q8_0 and Q4_0); `out`: the two tensors to write."""
-        from . import model as m
-
+        m = _model or _import_model()
         L = m._L or m._start()
         ctx = self.ctx
         batch, total, rows, keep = _ragged(seq_ids, start_pos, lens)
