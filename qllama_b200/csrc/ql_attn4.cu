@@ -40,7 +40,7 @@ constexpr float kLog2e4 = 1.4426950408889634f;
 // A probability is 2^arg with arg at most kTop (less where scales reach 2): below f16's
 // overflow times a scale, and far above its subnormals.  The reference it is relative to moves
 // only when an arg exceeds that, by enough to leave kSlack free.
-constexpr float kTop = 14.f, kSlack = 4.f;
+constexpr float kTop = 14.f, kSlack = 6.f;
 
 template <int HD>
 struct Attn4Cfg {
@@ -514,8 +514,9 @@ __global__ void __launch_bounds__(32 * Attn4Cfg<HD>::kWarps, 1)
             p[e][k] = fmaf(y[e][k], f[k & 1], -ref[k & 1]);
             over |= p[e][k] > top;
           }
-        // (a scale of 2 or more has the exponent's top bit)
-        if (__any_sync(0xffffffffu, over || (any_d & 0x40004000u)) || fresh) {
+        // (a scale of 2 or more, or a NaN, has the exponent's top bit)
+        float cap = top;
+        if (__any_sync(0xffffffffu, any_d & 0x40004000u)) {
           // NaN scales are taken out here and the blocks and rows that see them remembered:
           // behind the end of a sequence, or of what a row sees, P is 0 and 0 times NaN is not.
           uint32_t big = 0;  // the largest scale's bits
@@ -545,7 +546,9 @@ __global__ void __launch_bounds__(32 * Attn4Cfg<HD>::kWarps, 1)
               if ((va[e][r] >> 16 & 0x7fffu) > 0x7c00u) va[e][r] &= 0xffffu;
             }
           big = __reduce_max_sync(0xffffffffu, big);
-          const float cap = fminf(top, kTop - fmaxf(0.f, static_cast<float>(static_cast<int>(big >> 10) - 15)));
+          cap = fminf(top, kTop - fmaxf(0.f, static_cast<float>(static_cast<int>(big >> 10) - 15)));
+        }
+        if (__any_sync(0xffffffffu, over) || fresh || cap != top) {
 #pragma unroll
           for (int k = 0; k < 2; ++k) {
             // NaN does not count
