@@ -443,37 +443,94 @@ __device__ __forceinline__ size_t bounds_row(const CacheView& c, int page, int b
 }  // namespace
 
 // One CTA per (block, KV head): the least and largest key of each channel, rounded to f16 or
-// bf16.  A channel that holds a NaN gets NaN bounds.
+// bf16.  A channel that holds a NaN gets NaN bounds.  HD 64 or 128: HD / 8 lanes a position as in
+// the append, the block's positions in rounds, joined over the groups through shared memory;
+// HD 0: a thread a channel.
+template <int HD, int KIND>
 __global__ void __launch_bounds__(128) bounds_kernel(const __grid_constant__ BoundsArgs a) {
   const CacheView& c = a.cache;
   const int kvh = blockIdx.y;
   const int b = ragged_seq(a.blocks, a.batch, blockIdx.x);
   const int block = a.blocks.start[b] + static_cast<int>(blockIdx.x) - a.blocks.first[b];
-  bool ok;
-  const int64_t row = cache_row(c, a.blocks.seq[b], block * kTile, kvh, a.status, ok);
-  if (!ok) return;
-  const int page = static_cast<int>(row / c.page / c.hkv);
+  const int page = page_of(c, a.blocks.seq[b], block * kTile, a.status);
+  if (page < 0) return;
   uint16_t* out = a.bounds + bounds_row(c, page, block, kvh);
-  for (int d = threadIdx.x; d < c.hd; d += blockDim.x) {
-    float lo = CUDART_INF_F, hi = -CUDART_INF_F;
-    bool nan = false;
-    for (int i = 0; i < kTile; ++i) {
-      const float x = cache_value(c, false, row + i, d);
-      nan |= x != x;
-      lo = fminf(lo, x);
-      hi = fmaxf(hi, x);
-    }
+  const bool half = c.dtype == kF16;
+  auto write = [&](int d, float lo, float hi, bool nan) {
     if (nan) lo = hi = CUDART_NAN_F;
-    const bool half = c.dtype == kF16;
     out[d] = static_cast<uint16_t>(half ? pack2<false>(lo, lo) : pack2<true>(lo, lo));
     out[c.hd + d] = static_cast<uint16_t>(half ? pack2<false>(hi, hi) : pack2<true>(hi, hi));
+  };
+  if constexpr (HD != 0) {
+    constexpr int kLanes = HD / 8, kGroups = 128 / kLanes;
+    const int group = threadIdx.x / kLanes, d = threadIdx.x % kLanes * 8;
+    float lo[8], hi[8];
+    uint32_t nan = 0;
+#pragma unroll
+    for (int k = 0; k < 8; ++k) lo[k] = CUDART_INF_F, hi[k] = -CUDART_INF_F;
+#pragma unroll 4
+    for (int i = group; i < kTile; i += kGroups) {
+      float x[8];
+      load_cache8<KIND>(row_place<KIND>(c, page, block * kTile + i, d), c.dtype, kvh, false, x);
+#pragma unroll
+      for (int k = 0; k < 8; ++k) {
+        nan |= (x[k] != x[k] ? 1u : 0u) << k;
+        lo[k] = fminf(lo[k], x[k]);
+        hi[k] = fmaxf(hi[k], x[k]);
+      }
+    }
+    __shared__ float part[2][kGroups][HD];
+    __shared__ uint32_t nans[kGroups][kLanes];
+#pragma unroll
+    for (int k = 0; k < 8; ++k) {
+      part[0][group][d + k] = lo[k];
+      part[1][group][d + k] = hi[k];
+    }
+    nans[group][d / 8] = nan;
+    __syncthreads();
+    for (int e = threadIdx.x; e < HD; e += 128) {
+      float l = CUDART_INF_F, h = -CUDART_INF_F;
+      uint32_t bad = 0;
+      for (int g = 0; g < kGroups; ++g) {
+        l = fminf(l, part[0][g][e]);
+        h = fmaxf(h, part[1][g][e]);
+        bad |= nans[g][e / 8];
+      }
+      write(e, l, h, bad >> (e % 8) & 1u);
+    }
+  } else {
+    const int64_t row = (static_cast<int64_t>(page) * c.hkv + kvh) * c.page + block * kTile % c.page;
+    for (int d = threadIdx.x; d < c.hd; d += 128) {
+      float lo = CUDART_INF_F, hi = -CUDART_INF_F;
+      bool nan = false;
+      for (int i = 0; i < kTile; ++i) {
+        const float x = cache_value(c, false, row + i, d);
+        nan |= x != x;
+        lo = fminf(lo, x);
+        hi = fmaxf(hi, x);
+      }
+      write(d, lo, hi, nan);
+    }
   }
 }
+
+namespace {
+
+template <int HD>
+auto bounds_form(int dtype) {
+  return dtype == kQ4_0 ? bounds_kernel<HD, kQ4_0> : dtype == kQ8_0 ? bounds_kernel<HD, kQ8_0>
+                                                                    : bounds_kernel<HD, kF32>;
+}
+
+}  // namespace
 
 cudaError_t launch_bounds(const BoundsArgs& a, cudaStream_t s) {
   const int n = a.blocks.first[a.batch];
   if (n == 0) return cudaSuccess;
-  bounds_kernel<<<dim3(n, a.cache.hkv), 128, 0, s>>>(a);
+  const auto k = a.cache.hd == 128  ? bounds_form<128>(a.cache.dtype)
+                 : a.cache.hd == 64 ? bounds_form<64>(a.cache.dtype)
+                                    : bounds_kernel<0, kF32>;
+  k<<<dim3(n, a.cache.hkv), 128, 0, s>>>(a);
   return cudaGetLastError();
 }
 
@@ -502,16 +559,20 @@ __device__ __forceinline__ void add_parts(float x, double& up, double& down) {
   else down += x;  // a NaN lands here
 }
 
-__device__ __forceinline__ double block_extreme(double v, bool largest, double* red) {
+// The least and the largest over the block's threads.
+__device__ __forceinline__ void block_range(double& least, double& most, double2* red) {
+#pragma unroll
   for (int o = 16; o > 0; o >>= 1) {
-    const double w = __shfl_xor_sync(0xffffffffu, v, o);
-    v = largest ? fmax(v, w) : fmin(v, w);
+    least = fmin(least, __shfl_xor_sync(0xffffffffu, least, o));
+    most = fmax(most, __shfl_xor_sync(0xffffffffu, most, o));
   }
+  if ((threadIdx.x & 31) == 0) red[threadIdx.x >> 5] = make_double2(least, most);
   __syncthreads();
-  if ((threadIdx.x & 31) == 0) red[threadIdx.x >> 5] = v;
-  __syncthreads();
-  for (int i = 0; i < kChooseThreads / 32; ++i) v = largest ? fmax(v, red[i]) : fmin(v, red[i]);
-  return v;
+#pragma unroll
+  for (int i = 0; i < kChooseThreads / 32; ++i) {
+    least = fmin(least, red[i].x);
+    most = fmax(most, red[i].y);
+  }
 }
 
 }  // namespace
@@ -658,7 +719,7 @@ __global__ void __launch_bounds__(kChooseThreads)
   const bool fits = a.max_blocks <= a.smem_blocks;  // the scores, copied for the passes over them
   uint32_t* in = reinterpret_cast<uint32_t*>(dyn + (fits ? a.max_blocks : 0));  // a bit per block
   __shared__ int hist[kBins];
-  __shared__ double red[kChooseThreads / 32];
+  __shared__ double2 red[kChooseThreads / 32];
   __shared__ int scan[kChooseThreads / 32];
   constexpr int kList = 512;
   __shared__ int list[kList];
@@ -684,8 +745,7 @@ __global__ void __launch_bounds__(kChooseThreads)
         most = fmax(most, s);
       }
     }
-    least = block_extreme(least, false, red);
-    most = block_extreme(most, true, red);
+    block_range(least, most, red);
     const double scale = most > least ? (kBins - 3) / (most - least) : 0.0;
     // (rounded differences and products keep the order; infinities have bins of their own)
     auto bin = [&](double s) {
@@ -780,7 +840,7 @@ cudaError_t launch_select(const SelectArgs& a_in, cudaStream_t s) {
   // CTA begins with the queries, whatever it scores).
   const int64_t pairs = static_cast<int64_t>(jobs) * a.cache.hkv;
   a.chunk = 32;
-  while (a.chunk < kMaxChunk && pairs * ((a.max_blocks + a.chunk - 1) / a.chunk) > 2LL * a.num_sms) a.chunk *= 2;
+  while (a.chunk < kMaxChunk && pairs * ((a.max_blocks + a.chunk - 1) / a.chunk) > 4LL * a.num_sms) a.chunk *= 2;
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3((a.max_blocks + a.chunk - 1) / a.chunk, a.cache.hkv, jobs);
   cfg.blockDim = dim3(kChooseThreads);
