@@ -88,8 +88,9 @@ int ql_ctx_synchronize(ql_ctx* ctx);
  * Layout per layer: pages of `page_size` positions, each page holding
  * [num_kv_heads][page_size][head_dim] elements of K (post-RoPE, cache.rs:3-6)
  * and the same of V.  Q8_0 keeps the int8 values and the f16 block scales in
- * two planes with the same page geometry, Q4_0 the codes (half a byte each) and the
- * scales.  Sequence `s` owns pages through a block table shared by all layers.
+ * two planes with the same page geometry; Q4_0 keeps both, of K and of V, in one run per
+ * 64 positions of a KV head.  Sequence `s` owns pages through a block table shared by all
+ * layers.
  *
  * Q4_0: 32 values as codes 0..15 and a scale d, each standing for d * (code - 8): with m
  * the block's value of largest magnitude (the first of equals), d = f16(m / -8) and
@@ -158,7 +159,9 @@ int ql_kv_get(ql_ctx* ctx, const ql_kv* kv, int32_t layer, int32_t seq,
  * a fused projection can be given as they are.
  * start_pos[b] must equal the current length ("must continue"); new_len[b] may be 0.  The
  * rotation is ql_attn_forward's, in f64 and rounded once to f32, and the rows are then
- * converted to the cache's type; q_out gets the rotated queries rounded to q_out_dtype.
+ * converted to the cache's type (for Q8_0 with d = max|x| times the f32 nearest to 1/127: where
+ * x / d lies some units in f32's last place from a tie, the value may be the neighbour of the
+ * one that ql_kv_update stores, and likewise d); q_out gets the rotated queries rounded to q_out_dtype.
  * q_out [tokens, num_heads, head_dim] is contiguous and may be q itself (of the same type,
  * contiguous); any other overlap with an input is refused.  Device pointers, aligned to
  * their element size. */

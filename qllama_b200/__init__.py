@@ -310,7 +310,7 @@ class KvCache:
     def truncate(self, seq, new_len) -> None:
         """Roll sequence `seq` back to `new_len` positions in every layer (pages kept);
         lists of sequences and of their lengths roll back a batch at once."""
-        if np.ndim(seq) == 0:
+        if not hasattr(seq, "__len__"):
             _check(load().ql_kv_truncate(self._h, seq, new_len))
             return
         n = len(seq)

@@ -1026,9 +1026,12 @@ extern "C" {
 
 int ql_kv_append(ql_ctx* c, ql_kv* kv, const ql_append_args* a) {
   if (!c || !kv || !a) return fail(QL_ERR_INVALID, "ql_kv_append: NULL argument");
+  if (kv->ctx != c) return fail(QL_ERR_INVALID, "the cache belongs to another context");
   const int hq = a->num_heads, hkv = a->num_kv_heads, hd = a->head_dim;
   if (hq < 0 || hkv <= 0 || hd <= 0)
     return fail(QL_ERR_INVALID, "Attention head counts and head_dim must be positive");
+  if (hq > (1 << 16) || hkv > (1 << 16))
+    return fail(QL_ERR_UNSUPPORTED, "ql_kv_append takes up to %d heads", 1 << 16);
   if ((hd & 1) != 0)
     return fail(QL_ERR_INVALID,
                 "RoPE requires shape [seq_len, ..., head_dim] with a positive even head_dim");
@@ -1102,8 +1105,11 @@ int ql_kv_read(ql_ctx* c, const ql_kv* kv_in, int32_t layer, int32_t batch,
                const int32_t* seq_ids, const int64_t* start_pos, const int32_t* lens,
                int32_t out_dtype, void* k_out, void* v_out) {
   if (!c || !kv_in) return fail(QL_ERR_INVALID, "ql_kv_read: NULL argument");
+  if (kv_in->ctx != c) return fail(QL_ERR_INVALID, "the cache belongs to another context");
   ql_kv* kv = const_cast<ql_kv*>(kv_in);  // only the marks of the checks are written
   if (!valid_io_dtype(out_dtype)) return fail(QL_ERR_INVALID, "unknown output dtype %d", out_dtype);
+  if (kv->cfg.num_kv_heads > (1 << 16))
+    return fail(QL_ERR_UNSUPPORTED, "ql_kv_read takes up to %d KV heads", 1 << 16);
   ql::RaggedReadArgs k{};
   int64_t ends[ql::kMaxBatch];
   const int r = ragged_rows(kv, "ql_kv_read", layer, batch, seq_ids, start_pos, lens, false,
@@ -1558,6 +1564,7 @@ int ql_attn_forward_appended(ql_ctx* c, ql_kv* kv, const ql_attn_args* a) {
 
 int ql_attn_forward_sparse(ql_ctx* c, ql_kv* kv, const ql_attn_args* a, const ql_sparse_args* s) {
   if (!c || !kv || !a || !s) return fail(QL_ERR_INVALID, "ql_attn_forward_sparse: NULL argument");
+  if (kv->ctx != c) return fail(QL_ERR_INVALID, "the cache belongs to another context");
   if (s->blocks < 1 || s->first < 0 || s->last < 1 || s->first > s->blocks - s->last)
     return fail(QL_ERR_INVALID, "blocks %d must hold the first %d (>= 0) and the last %d (>= 1)",
                 s->blocks, s->first, s->last);

@@ -17,8 +17,9 @@
 // f16's subnormals hold the codes exactly and the matrix instruction takes them as they are, so
 // that a fragment register costs one AND.  The powers of two are folded into q and the output.
 // A K scale multiplies the block's partial sums in f32, a V scale the probabilities in f16.  The
-// 8 that is subtracted from every code enters S and leaves O as products of the scales: of K's
-// with -8 sum q of each block, of V's with P, where a row of ones beside them sums P itself.
+// 8 that is subtracted from every code enters S as the product of K's scales with -8 sum q of each
+// block, and leaves O with the product of ones and the same rounded P d that the codes met, so
+// that a rounding counts with the value and not with the code; ones and P give the sum of P.
 //
 // Bound by HBM for long caches (2304 bytes of a head_dim 128 cache per 16 positions against
 // about 200 instructions of one warp).
@@ -277,9 +278,7 @@ __global__ void __launch_bounds__(32 * Attn4Cfg<HD>::kWarps, 1)
   const int ks_at = static_cast<int>(kRec.k_scales()) + 2 * q4_k_scale(g, 0, NB);
   const int vs_at = static_cast<int>(kRec.v_scales()) + 2 * q4_v_scale(2 * tq, 0, NB);
   const int kw_at = ks_at + (NB == 4 ? (tq & 1) * 4 : 0);  // the scales of blocks 2 tq, 2 tq + 1
-  const int vw_at = vs_at + (g & (NB - 1)) * 4;            // V's of block g
-  // rows of V's scales, one a block, then a row of ones
-  const uint32_t aux_and = g < NB ? 0xffffffffu : 0u, aux_or = g == 4 ? 0x3c003c00u : 0u;
+  constexpr uint32_t kOnes = 0x3c003c00u;  // two f16
 
   bool alive = true;
   int stage = 0, phase = 0;  // of the next tile
@@ -410,7 +409,8 @@ __global__ void __launch_bounds__(32 * Attn4Cfg<HD>::kWarps, 1)
     }
     const int most = a.sel ? all : start + divide(job.row0 + job.rows - 1, a.group) + 1;
 
-    float o[NB][2][4], aux[4] = {0.f, 0.f, 0.f, 0.f};
+    // O, and (every row alike) the sums of P d of each block and of P
+    float o[NB][2][4], off[NB][4] = {}, sum[4] = {};
 #pragma unroll
     for (int b = 0; b < NB; ++b)
 #pragma unroll
@@ -479,22 +479,20 @@ __global__ void __launch_bounds__(32 * Attn4Cfg<HD>::kWarps, 1)
           }
         }
         // ---- V's scales of positions 2 tq, 2 tq + 1 and those plus 8
-        uint32_t vd[2][2][NB], va[2][2], any_d = 0;
+        uint32_t vd[2][2][NB], any_d = 0;
 #pragma unroll
         for (int e = 0; e < 2; ++e)
 #pragma unroll
           for (int r = 0; r < 2; ++r) {
-            const uint32_t w =
-                *reinterpret_cast<const uint32_t*>(st + vw_at + (32 * (s + e) + 16 * r) * NB);
-            any_d |= w;  // between them the lanes see every scale
-            va[e][r] = (w & aux_and) | aux_or;
             const uint8_t* sp = svs + (32 * e + 16 * r) * NB;
             if constexpr (NB == 4) {
               const uint4 d = *reinterpret_cast<const uint4*>(sp);
               vd[e][r][0] = d.x, vd[e][r][1] = d.y, vd[e][r][2] = d.z, vd[e][r][3] = d.w;
+              any_d |= d.x | d.y | d.z | d.w;
             } else {
               const uint2 d = *reinterpret_cast<const uint2*>(sp);
               vd[e][r][0] = d.x, vd[e][r][1] = d.y;
+              any_d |= d.x | d.y;
             }
           }
         // ---- softmax: columns 2 tq, 2 tq + 1 of positions g and g + 8
@@ -538,13 +536,6 @@ __global__ void __launch_bounds__(32 * Attn4Cfg<HD>::kWarps, 1)
                   for (int k = 0; k < 2; ++k) nans |= (place < lim[k] ? 1u : 0u) << (4 * k + b);
                 }
               }
-#pragma unroll
-          for (int e = 0; e < 2; ++e)
-#pragma unroll
-            for (int r = 0; r < 2; ++r) {
-              if ((va[e][r] & 0x7fffu) > 0x7c00u) va[e][r] &= 0xffff0000u;
-              if ((va[e][r] >> 16 & 0x7fffu) > 0x7c00u) va[e][r] &= 0xffffu;
-            }
           big = __reduce_max_sync(0xffffffffu, big);
           cap = fminf(top, kTop - fmaxf(0.f, static_cast<float>(static_cast<int>(big >> 10) - 15)));
         }
@@ -561,14 +552,16 @@ __global__ void __launch_bounds__(32 * Attn4Cfg<HD>::kWarps, 1)
             if ((fresh || m - next > cap) && m > -CUDART_INF_F) next = m - (cap - kSlack);
             const float corr = fresh ? 0.f : ex2(ref[k] - next);
             ref[k] = next;
-            aux[k] *= corr;
+            sum[k] *= corr;
 #pragma unroll
-            for (int b = 0; b < NB; ++b)
+            for (int b = 0; b < NB; ++b) {
+              off[b][k] *= corr;
 #pragma unroll
               for (int u = 0; u < 2; ++u) {
                 o[b][u][k] *= corr;
                 o[b][u][k + 2] *= corr;
               }
+            }
           }
           top = cap;
           fresh = false;
@@ -583,8 +576,8 @@ __global__ void __launch_bounds__(32 * Attn4Cfg<HD>::kWarps, 1)
           for (int k = 0; k < 4; ++k) p[e][k] = ex2(p[e][k]);
           const uint32_t pt0 = transpose8(pack2<false>(p[e][0], p[e][1]));
           const uint32_t pt1 = transpose8(pack2<false>(p[e][2], p[e][3]));
-          // ---- O += V^T (P d), and the sums of P d and P
-          mma_f16(aux, va[e][0], 0u, va[e][1], 0u, pt0, pt1);
+          // ---- O += V^T (P d), and the sums
+          mma_f16(sum, kOnes, kOnes, kOnes, kOnes, pt0, pt1);
           uint32_t vw[2][NB];
 #pragma unroll
           for (int r = 0; r < 2; ++r) {
@@ -600,6 +593,7 @@ __global__ void __launch_bounds__(32 * Attn4Cfg<HD>::kWarps, 1)
 #pragma unroll
           for (int b = 0; b < NB; ++b) {
             const uint32_t b0 = mul2(pt0, vd[e][0][b]), b1 = mul2(pt1, vd[e][1][b]);
+            mma_f16(off[b], kOnes, kOnes, kOnes, kOnes, b0, b1);
 #pragma unroll
             for (int u = 0; u < 2; ++u) {
               const uint32_t u0 = vw[0][b] >> (8 * u), u1 = vw[1][b] >> (8 * u);
@@ -621,7 +615,7 @@ __global__ void __launch_bounds__(32 * Attn4Cfg<HD>::kWarps, 1)
     float l[2];
 #pragma unroll
     for (int k = 0; k < 2; ++k) {
-      l[k] = __shfl_sync(0xffffffffu, aux[k], 16 + tq);
+      l[k] = sum[k];
       if (l[k] == 0.f) ref[k] = -CUDART_INF_F;  // the row sees none of these tiles
     }
     const bool whole = job.t0 >= w0 && job.t0 + job.tiles <= w1;
@@ -638,8 +632,7 @@ __global__ void __launch_bounds__(32 * Attn4Cfg<HD>::kWarps, 1)
       const size_t base = whole && live ? row_offset(a, job, job.row0 + r, HD) : 0;
       float eight[NB];  // 8 sum P d of each block, in the units of O
 #pragma unroll
-      for (int b = 0; b < NB; ++b)
-        eight[b] = __shfl_sync(0xffffffffu, aux[k], 4 * b + tq) * (8.f / 16777216.f);
+      for (int b = 0; b < NB; ++b) eight[b] = off[b][k] * (8.f / 16777216.f);
       if (!live) continue;
 #pragma unroll
       for (int b = 0; b < NB; ++b) {
@@ -798,15 +791,14 @@ int attn4_plan(int hd, int num_sms, const int* tiles, int batch, int jobs, Attn4
   a->per_cta = static_cast<int>((total + ctas - 1) / ctas);
   a->aligned = 0;
   const int per_warp = (a->per_cta + warps - 1) / warps;
-  // the smallest share of a job that leaves no more CTAs than SMs
-  for (int splits = longest; splits >= 1; --splits) {
+  // the smallest share of a job that leaves no more CTAs than SMs (the longest sequence's alone
+  // may not be more)
+  const bool room = static_cast<int64_t>(batch) * jobs <= num_sms;
+  for (int splits = room ? std::min(longest, num_sms / jobs) : 0; splits >= 1; --splits) {
     const int share = std::max((longest + splits - 1) / splits, std::min(longest, kMinTiles));
     int64_t n = 0;
     for (int b = 0; b < batch; ++b) n += static_cast<int64_t>((tiles[b] + share - 1) / share) * jobs;
-    if (n > num_sms) {
-      if (static_cast<int64_t>(batch) * jobs > num_sms) break;
-      continue;
-    }
+    if (n > num_sms) continue;
     if ((share + warps - 1) / warps <= per_warp) {
       a->per_cta = share;
       a->aligned = 1;

@@ -117,13 +117,14 @@ __device__ __forceinline__ void store_cache8(const RowPlace& p, int dtype, int h
   }
   const int lane = threadIdx.x & 31;
   uint16_t* scale_at = reinterpret_cast<uint16_t*>((v ? p.vs : p.ks) + h * p.scale_step);
-  if constexpr (KIND == kQ8_0) {  // q8_0_pair's rule
+  if constexpr (KIND == kQ8_0) {
+    // q8_0_pair's rule, but for the rounding of d: a product, not a division
     float amax = 0.f;
 #pragma unroll
     for (int k = 0; k < 8; ++k) amax = fmaxf(amax, fabsf(x[k]));
     amax = fmaxf(amax, __shfl_xor_sync(lanes, amax, 1));
     amax = fmaxf(amax, __shfl_xor_sync(lanes, amax, 2));
-    const float s = amax / 127.0f, id = s != 0.0f ? 1.0f / s : 0.0f;
+    const float s = amax * (1.0f / 127.0f), id = s != 0.0f ? 1.0f / s : 0.0f;
     uint32_t w[2] = {0, 0};
 #pragma unroll
     for (int k = 0; k < 8; ++k) {

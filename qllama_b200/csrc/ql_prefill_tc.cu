@@ -805,14 +805,31 @@ __global__ void __launch_bounds__(256) tiles_to_f16_kernel(const __grid_constant
       }
     }
   } else if constexpr (DT == kQ4_0) {
+    // a word of K holds eight dims' codes, two bytes of V four
+    constexpr int kEach = 8, kWords = kVals / kEach;
+    uint32_t w[kWords];
+    uint16_t sc[kVals / 32];
+    const uint8_t* codes = q4_code_at(a.cache, row, 0, kind != 0);
+    const int pos = static_cast<int>(row % kTile), d0 = part * kVals;
 #pragma unroll
-    for (int i = 0; i < kVals; i += 2) {
-      const int d = part * kVals + i;
-      const uint32_t w = *q4_code_at(a.cache, row, d, kind != 0);
-      const float f = __half2float(__ushort_as_half(*q4_scale_at(a.cache, row, d / 32, kind != 0)));
-      v[i] = f * static_cast<float>(static_cast<int>(w & 15u) - 8);
-      v[i + 1] = f * static_cast<float>(static_cast<int>(w >> 4) - 8);
+    for (int i = 0; i < kWords; ++i) {
+      const int d = d0 + kEach * i;
+      if (kind == 0) {
+        w[i] = *reinterpret_cast<const uint32_t*>(codes + q4_k_byte(pos, d, HD / 32) -
+                                                  q4_k_byte(pos, 0, HD / 32));
+      } else {
+        const int at = q4_v_byte(pos, 0, HD / 32);
+        w[i] = *reinterpret_cast<const uint16_t*>(codes + q4_v_byte(pos, d, HD / 32) - at) |
+               static_cast<uint32_t>(*reinterpret_cast<const uint16_t*>(
+                   codes + q4_v_byte(pos, d + 4, HD / 32) - at)) << 16;
+      }
     }
+#pragma unroll
+    for (int i = 0; i < kVals / 32; ++i) sc[i] = *q4_scale_at(a.cache, row, d0 / 32 + i, kind != 0);
+#pragma unroll
+    for (int i = 0; i < kVals; ++i)
+      v[i] = __half2float(__ushort_as_half(sc[i / 32])) *
+             static_cast<float>(static_cast<int>(w[i / kEach] >> (4 * (i % kEach)) & 15u) - 8);
   } else {
     const uint4* src = reinterpret_cast<const uint4*>(
         static_cast<const int8_t*>(kind ? a.cache.v : a.cache.k) + row * HD + part * kVals);

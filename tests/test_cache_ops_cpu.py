@@ -112,6 +112,22 @@ def test_append_refusals(change, text):
     assert list(c.lens[:SLOTS]) == [5, 0, 0, 0]
 
 
+def test_a_cache_of_another_context_is_refused():
+    c, other = Cache(lens=(100, 0, 0, 0)), Ctx()
+    L, x, kv = qb.load(), ctypes.byref(other), ctypes.byref(c.kv)
+    text = "belongs to another context"
+    refused(L.ql_kv_append(x, kv, ctypes.byref(append_args())), text)
+    refused(L.ql_kv_read(x, kv, 0, 1, i32(0), i64(0), i32(1), qb.F32, P, P + 8192), text)
+    refused(L.ql_attn_forward_sparse(x, kv, ctypes.byref(attn_args()),
+                                     ctypes.byref(qm.SparseArgs(4, 1, 1, None))), text)
+
+
+def test_too_many_heads_are_refused():
+    c = Cache()
+    refused(qb.load().ql_kv_append(*c.args(), ctypes.byref(append_args(num_heads=1 << 17))),
+            "heads", qb.ERR_UNSUPPORTED)
+
+
 def test_append_of_nothing_is_a_no_op():
     c = Cache(lens=(5, 0, 0, 0))
     for change in (dict(batch=0, seq_ids=None, start_pos=None, new_len=None),
