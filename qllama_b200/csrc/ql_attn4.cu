@@ -22,7 +22,12 @@
 // that a rounding counts with the value and not with the code; ones and P give the sum of P.
 //
 // Bound by HBM for long caches (2304 bytes of a head_dim 128 cache per 16 positions against
-// about 200 instructions of one warp).
+// about 200 instructions of one warp): 8 sequences of 32768 positions, 32/8 heads, 302 MB, take
+// 69 us, of which the stream of tiles is some 53 (5.7 TB/s) and the rest the beginning (look-ups
+// and queries, about 3 us), the joining (3 to 5 us) and the launch.  From L2, as with drafted
+// tokens whose jobs share the keys, it is bound by instruction issue: half of the ALU's slots.
+// Other shapes of the kernel measured the same or slower: sixteen warps of 128 registers, one
+// step of 16 positions, sixteen query rows a job.
 #include <math_constants.h>
 
 #include <algorithm>
