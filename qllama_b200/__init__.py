@@ -5,8 +5,11 @@ in-tree by qllama_b200.build).  The classes mirror the reference's interface
 for this path:
 
 * ``KvCache``  -- src/kv_cache/cache.rs (new / update / get / clear / seq_len),
-  device resident and paged, with f32, f16, bf16 or Q8_0 storage and several
-  sequence slots;
+  device resident and paged, with f32, f16, bf16, Q8_0 or Q4_0 storage and several
+  sequence slots; and, with no counterpart there, ``append`` (new rows of sequences of
+  different lengths, rotated on the way) and ``read`` (rows back on the device), which
+  take CUDA tensors and are ordered with torch's current stream as the calls of
+  ``qllama_b200.model`` are;
 * ``attention_forward`` -- steps 3-7 of ``Attention::forward_with_cache``
   (src/transformer/layers.rs:397-455) on already projected Q/K/V;
 * ``Comm`` / ``attention_forward_sharded`` -- the same operator with the KV

@@ -242,10 +242,10 @@ __global__ void __launch_bounds__(32 * Attn4Cfg<HD>::kWarps, 1)
   job.t0 = __shfl_sync(0xffffffffu, lane_job.t0, 0);
   job.tiles = __shfl_sync(0xffffffffu, lane_job.tiles, 0);
   if (w0 < w1) {
-    if (!a.sel && w0 + lane < w1)
+    const int entry = (w0 + lane - lane_job.t0) / (a.cache.page / kTile);
+    if (!a.sel && w0 + lane < w1 && entry < a.cache.pages_per_seq)  // (aligned: places without one)
       prefetch_l2(a.cache.block_table +
-                  static_cast<size_t>(a.seqs.seq[lane_job.b]) * a.cache.pages_per_seq +
-                  (w0 + lane - lane_job.t0) * kTile / a.cache.page);
+                  static_cast<size_t>(a.seqs.seq[lane_job.b]) * a.cache.pages_per_seq + entry);
     const int esize = a.in_dtype == kF32 ? 4 : 2;
     if (lane < job.rows * HD * esize / 128)
       prefetch_l2(static_cast<const char*>(a.q) +
@@ -617,12 +617,9 @@ __global__ void __launch_bounds__(32 * Attn4Cfg<HD>::kWarps, 1)
     }
 
     // ------------------------------------------------- the end of a piece --
-    float l[2];
 #pragma unroll
-    for (int k = 0; k < 2; ++k) {
-      l[k] = sum[k];
-      if (l[k] == 0.f) ref[k] = -CUDART_INF_F;  // the row sees none of these tiles
-    }
+    for (int k = 0; k < 2; ++k)
+      if (sum[k] == 0.f) ref[k] = -CUDART_INF_F;  // the row sees none of these tiles
     const bool whole = job.t0 >= w0 && job.t0 + job.tiles <= w1;
     // A piece that ends the warp's part goes into its ring; an earlier one (of a job that
     // other warps began) into memory: the CTA's own piece of it if no other warp here has one.
@@ -633,7 +630,7 @@ __global__ void __launch_bounds__(32 * Attn4Cfg<HD>::kWarps, 1)
     for (int k = 0; k < 2; ++k) {
       const int r = 2 * tq + k;
       const bool live = r < job.rows;
-      const float f24 = 16777216.f * (whole ? 1.f / l[k] : 1.f);
+      const float f24 = 16777216.f * (whole ? 1.f / sum[k] : 1.f);
       const size_t base = whole && live ? row_offset(a, job, job.row0 + r, HD) : 0;
       float eight[NB];  // 8 sum P d of each block, in the units of O
 #pragma unroll
@@ -652,7 +649,7 @@ __global__ void __launch_bounds__(32 * Attn4Cfg<HD>::kWarps, 1)
         else
           *reinterpret_cast<float4*>(part + r * HD + d) = v;
       }
-      if (!whole && g == 0) *reinterpret_cast<float2*>(part + 8 * HD + 2 * r) = make_float2(ref[k], l[k]);
+      if (!whole && g == 0) *reinterpret_cast<float2*>(part + 8 * HD + 2 * r) = make_float2(ref[k], sum[k]);
     }
   }
 

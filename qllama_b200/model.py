@@ -9,8 +9,10 @@ Mirrors the reference's interface for these pieces:
 * ``SamplerConfig`` / ``sample`` -- src/sampler/sampler.rs (the uniform draw
   is passed in: the reference draws it from its seeded generator).
 
-and, with no counterpart in the reference, the pieces of a decode step on 4-bit
-weights with drafted tokens:
+and, with no counterpart in the reference, attention over rows that are in the cache
+already, whole (``attention_forward_appended``) or over the blocks that a bound on
+their scores selects (``attention_forward_sparse``), and the pieces of a decode step
+on 4-bit weights with drafted tokens:
 
 * ``rms_norm``         -- RMSNorm with the residual's addition, plain or Q8_0 out;
 * ``Q4Weight`` / ``linear_q4`` -- 4-bit weight matrices and products of a few
