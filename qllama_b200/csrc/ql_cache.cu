@@ -164,30 +164,39 @@ __device__ __forceinline__ void store_cache8(const RowPlace& p, int dtype, int h
   if ((lane & 3) == 0) *scale_at = scale;
 }
 
-// The converse: eight values of KV head h.
+// The converse, in two steps so that several rows' loads are under way together: eight values of
+// KV head h as they lie there (a word or two of codes, the scale behind them), and as f32.
 template <int KIND>
-__device__ __forceinline__ void load_cache8(const RowPlace& p, int dtype, int h, bool v,
-                                            float (&x)[8]) {
+__device__ __forceinline__ Raw8 load_cache8(const RowPlace& p, int dtype, int h, bool v) {
   const uint8_t* at = (v ? p.v : p.k) + h * p.step;
-  if constexpr (KIND == kF32) {
-    floats_of(load_raw8(at, 0, dtype, true), dtype, x);
-    return;
-  }
-  const float s = __half2float(__ushort_as_half(
-      *reinterpret_cast<const uint16_t*>((v ? p.vs : p.ks) + h * p.scale_step)));
+  if constexpr (KIND == kF32) return load_raw8(at, 0, dtype, true);
+  Raw8 r;
+  r.w[0].z = *reinterpret_cast<const uint16_t*>((v ? p.vs : p.ks) + h * p.scale_step);
   if constexpr (KIND == kQ8_0) {
     const uint2 w = *reinterpret_cast<const uint2*>(at);
-#pragma unroll
-    for (int k = 0; k < 8; ++k)
-      x[k] = s * static_cast<float>(static_cast<int8_t>((k < 4 ? w.x : w.y) >> (8 * (k & 3))));
+    r.w[0].x = w.x, r.w[0].y = w.y;
   } else {
-    const uint32_t w =
-        v ? *reinterpret_cast<const uint16_t*>(at) |
-                static_cast<uint32_t>(*reinterpret_cast<const uint16_t*>(p.v2 + h * p.step)) << 16
-          : *reinterpret_cast<const uint32_t*>(at);
+    r.w[0].x = v ? *reinterpret_cast<const uint16_t*>(at) |
+                       static_cast<uint32_t>(*reinterpret_cast<const uint16_t*>(p.v2 + h * p.step)) << 16
+                 : *reinterpret_cast<const uint32_t*>(at);
+  }
+  return r;
+}
+
+template <int KIND>
+__device__ __forceinline__ void cache8_values(const Raw8& r, int dtype, float (&x)[8]) {
+  if constexpr (KIND == kF32) {
+    floats_of(r, dtype, x);
+    return;
+  }
+  const float s = __half2float(__ushort_as_half(static_cast<uint16_t>(r.w[0].z)));
 #pragma unroll
-    for (int k = 0; k < 8; ++k)
-      x[k] = s * static_cast<float>(static_cast<int>(w >> (4 * k) & 15u) - 8);
+  for (int k = 0; k < 8; ++k) {
+    if constexpr (KIND == kQ8_0)
+      x[k] = s * static_cast<float>(
+                     static_cast<int8_t>((k < 4 ? r.w[0].x : r.w[0].y) >> (8 * (k & 3))));
+    else
+      x[k] = s * static_cast<float>(static_cast<int>(r.w[0].x >> (4 * k) & 15u) - 8);
   }
 }
 
@@ -373,23 +382,26 @@ __global__ void __launch_bounds__(256) ragged_read_kernel(const __grid_constant_
   const int page = page_of(c, a.rows.seq[b], pos, a.status);
   const RowPlace place = row_place<KIND>(c, max(page, 0), pos, d);
   const int h0 = blockIdx.y * kAtOnce;
-  float k[kAtOnce][8], v[kAtOnce][8];
+  Raw8 raw[kAtOnce][2];
 #pragma unroll
-  for (int i = 0; i < kAtOnce; ++i) {
-    const int h = min(h0 + i, c.hkv - 1);
-    load_cache8<KIND>(place, c.dtype, h, false, k[i]);
-    load_cache8<KIND>(place, c.dtype, h, true, v[i]);
-  }
+  for (int i = 0; i < kAtOnce; ++i)
+#pragma unroll
+    for (int v = 0; v < 2; ++v)
+      raw[i][v] = load_cache8<KIND>(place, c.dtype, min(h0 + i, c.hkv - 1), v != 0);
 #pragma unroll
   for (int i = 0; i < kAtOnce; ++i) {
     if (h0 + i >= c.hkv) break;
-    if (page < 0) {
 #pragma unroll
-      for (int e = 0; e < 8; ++e) k[i][e] = v[i][e] = 0.f;
+    for (int v = 0; v < 2; ++v) {
+      float x[8];
+      cache8_values<KIND>(raw[i][v], c.dtype, x);
+      if (page < 0) {
+#pragma unroll
+        for (int e = 0; e < 8; ++e) x[e] = 0.f;
+      }
+      store8(v ? a.v_out : a.k_out, (static_cast<size_t>(r) * c.hkv + h0 + i) * HD + d, a.out_dtype,
+             x, a.vec >> v & 1);
     }
-    const size_t o = (static_cast<size_t>(r) * c.hkv + h0 + i) * HD + d;
-    store8(a.k_out, o, a.out_dtype, k[i], a.vec & 1);
-    store8(a.v_out, o, a.out_dtype, v[i], a.vec & 2);
   }
 }
 
@@ -474,7 +486,9 @@ __global__ void __launch_bounds__(128) bounds_kernel(const __grid_constant__ Bou
 #pragma unroll 4
     for (int i = group; i < kTile; i += kGroups) {
       float x[8];
-      load_cache8<KIND>(row_place<KIND>(c, page, block * kTile + i, d), c.dtype, kvh, false, x);
+      cache8_values<KIND>(
+          load_cache8<KIND>(row_place<KIND>(c, page, block * kTile + i, d), c.dtype, kvh, false),
+          c.dtype, x);
 #pragma unroll
       for (int k = 0; k < 8; ++k) {
         nan |= (x[k] != x[k] ? 1u : 0u) << k;

@@ -701,7 +701,8 @@ __device__ __forceinline__ void prologue_q(const PrefillArgs& a, int w, int lane
     float m = 0.f;
 #pragma unroll
     for (int i = 0; i < kN / 2; ++i) {
-      rope_pair(y[2 * i], y[2 * i + 1], cs[i], y[2 * i], y[2 * i + 1]);
+      // (queries that arrive rotated, stride 0, need not go through f64 and back)
+      if (a.rope_stride != 0) rope_pair(y[2 * i], y[2 * i + 1], cs[i], y[2 * i], y[2 * i + 1]);
       m = fmaxf(m, fmaxf(fabsf(y[2 * i]), fabsf(y[2 * i + 1])));
     }
     const int e = f16_range_exp(__reduce_max_sync(0xffffffffu, __float_as_uint(m)));
