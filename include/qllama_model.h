@@ -130,7 +130,11 @@ int ql_attn_forward_appended(ql_ctx* ctx, ql_kv* kv, const ql_attn_args* args);
  * that is NaN counts as the largest.
  * The bounds belong to the cache: a layer's first call allocates them (1/32 of an f16
  * cache's keys; make it before a capture), and a call adds those of the blocks that have
- * filled up since.  selected (may be NULL) receives each list in ascending order, -1 behind
+ * filled up since.  A captured call's replays take the bounds of the blocks that were whole
+ * and scored before the capture as they then are: when those rows have been replaced
+ * (truncated and appended anew), make an uncaptured call on the sequences before the replay,
+ * or capture again.  Rows that replays of captured appends rewrite are followed by the calls
+ * made or captured after the append's capture.  selected (may be NULL) receives each list in ascending order, -1 behind
  * its end.  args->mem must be QL_MEM_DEVICE; batch * new_len is at most 65535. */
 typedef struct {
   int32_t blocks;     /* >= first + last */

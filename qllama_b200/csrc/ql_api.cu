@@ -135,6 +135,12 @@ struct ql_kv {
   // (BoundsArgs::bounds), and how many leading blocks of each sequence have theirs.
   std::vector<uint16_t*> bounds;   // per layer, null until then
   std::vector<int32_t> bounded;    // [layer][seq]
+  // The blocks that appends recorded into graphs write, [layer][seq]: a replay changes them
+  // without a call here, so every call over selected blocks makes their bounds again.
+  struct Blocks {
+    int32_t begin = 0, end = 0;
+  };
+  std::vector<Blocks> replayed;
 };
 
 namespace {
@@ -249,6 +255,9 @@ int encode_q_map(CUtensorMap* m, void* base, int hd, uint64_t rows) {
 // rotated.
 int ensure_identity(ql_kv* kv) {
   if (kv->d_rope_id) return QL_OK;
+  if (is_capturing(kv->ctx->stream))
+    return fail(QL_ERR_INVALID, "a cache's first call uploads its rotations: make it before the "
+                "capture");
   std::vector<double2> id(std::max(1, kv->cfg.head_dim / 2), make_double2(1.0, 0.0));
   double2* p = nullptr;
   QL_CUDA(cudaMalloc(&p, id.size() * sizeof(double2)), "allocate rope table");
@@ -270,6 +279,9 @@ int ensure_rope(ql_kv* kv, float theta) {
   const int r = ensure_identity(kv);
   if (r != QL_OK) return r;
   if (kv->d_rope && kv->rope_theta == theta) return QL_OK;
+  if (is_capturing(kv->ctx->stream))
+    return fail(QL_ERR_INVALID, "a first call with a theta uploads its rotations: make it before "
+                "the capture");
   const int hd = kv->cfg.head_dim, pairs = hd / 2, n = kv->cfg.max_seq_len;
   std::vector<double> freq(pairs);
   for (int p = 0; p < pairs; ++p)
@@ -387,6 +399,26 @@ int32_t& bounded_at(ql_kv* kv, int layer, int seq) {
   return kv->bounded[static_cast<size_t>(layer) * kv->cfg.max_batch + seq];
 }
 
+ql_kv::Blocks& replayed_at(ql_kv* kv, int layer, int seq) {
+  return kv->replayed[static_cast<size_t>(layer) * kv->cfg.max_batch + seq];
+}
+
+// A call has appended positions up to `end` to each of the sequences.
+void lengthen(ql_kv* kv, int layer, const int32_t* seqs, const int64_t* ends, int batch) {
+  const bool capturing = is_capturing(kv->ctx->stream);
+  for (int b = 0; b < batch; ++b) {
+    int64_t& len = len_at(kv, layer, seqs[b]);
+    if (capturing && ends[b] > len) {
+      ql_kv::Blocks& r = replayed_at(kv, layer, seqs[b]);
+      const int32_t begin = static_cast<int32_t>(len / ql::kTile);
+      const int32_t end = static_cast<int32_t>((ends[b] + ql::kTile - 1) / ql::kTile);
+      r.begin = r.end ? std::min(r.begin, begin) : begin;
+      r.end = std::max(r.end, end);
+    }
+    len = ends[b];
+  }
+}
+
 // A sequence goes back to `len` positions: what later appends rewrite has no bounds.
 void shorten(ql_kv* kv, int layer, int seq, int64_t len) {
   len_at(kv, layer, seq) = len;
@@ -422,7 +454,9 @@ int ql_check_status(ql_ctx* c) {
 namespace {
 
 // Brings the bounds of a layer's whole blocks up to date for the listed sequences: the blocks
-// that have filled up since the last call (a launch for one call in 64 of a decode loop).
+// that have filled up since the last call (a launch for one call in 64 of a decode loop), and
+// those that replays of captured appends may have rewritten since.  A captured launch has not
+// run yet: it leaves the blocks to the next call as well.
 int ensure_bounds(ql_ctx* c, ql_kv* kv, int layer, const int32_t* seqs, int batch) {
   if (!kv->bounds[layer]) {
     if (is_capturing(c->stream))
@@ -432,24 +466,32 @@ int ensure_bounds(ql_ctx* c, ql_kv* kv, int layer, const int32_t* seqs, int batc
                          kv->cfg.num_kv_heads * 2 * kv->cfg.head_dim * sizeof(uint16_t);
     QL_CUDA(cudaMalloc(&kv->bounds[layer], std::max<size_t>(bytes, 256)), "allocate block bounds");
   }
-  ql::BoundsArgs a{};
-  int64_t total = 0;
-  for (int b = 0; b < batch; ++b) {
-    const int whole = static_cast<int>(len_at(kv, layer, seqs[b]) / ql::kTile);
-    a.blocks.seq[b] = seqs[b];
-    a.blocks.start[b] = bounded_at(kv, layer, seqs[b]);
-    a.blocks.first[b] = static_cast<int32_t>(total);
-    total += whole - a.blocks.start[b];
+  for (int pass = 0; pass < 2; ++pass) {
+    ql::BoundsArgs a{};
+    int64_t total = 0;
+    for (int b = 0; b < batch; ++b) {
+      const int whole = static_cast<int>(len_at(kv, layer, seqs[b]) / ql::kTile);
+      const int made = bounded_at(kv, layer, seqs[b]);
+      const ql_kv::Blocks& again = replayed_at(kv, layer, seqs[b]);
+      const int begin = pass == 0 ? again.begin : made;
+      const int end = pass == 0 ? std::min(again.end, made) : whole;
+      a.blocks.seq[b] = seqs[b];
+      a.blocks.start[b] = begin;
+      a.blocks.first[b] = static_cast<int32_t>(total);
+      total += std::max(0, end - begin);
+    }
+    a.blocks.first[batch] = static_cast<int32_t>(total);
+    if (total == 0) continue;
+    a.bounds = kv->bounds[layer];
+    a.cache = view_of(kv, layer);
+    a.batch = batch;
+    a.status = c->status;
+    QL_CUDA(ql::launch_bounds(a, c->stream), "launch block bounds");
   }
-  a.blocks.first[batch] = static_cast<int32_t>(total);
-  if (total == 0) return QL_OK;
-  a.bounds = kv->bounds[layer];
-  a.cache = view_of(kv, layer);
-  a.batch = batch;
-  a.status = c->status;
-  QL_CUDA(ql::launch_bounds(a, c->stream), "launch block bounds");
-  for (int b = 0; b < batch; ++b)
-    bounded_at(kv, layer, seqs[b]) = static_cast<int32_t>(len_at(kv, layer, seqs[b]) / ql::kTile);
+  if (!is_capturing(c->stream))
+    for (int b = 0; b < batch; ++b)
+      bounded_at(kv, layer, seqs[b]) =
+          static_cast<int32_t>(len_at(kv, layer, seqs[b]) / ql::kTile);
   return QL_OK;
 }
 
@@ -727,6 +769,7 @@ int ql_kv_create(ql_ctx* c, const ql_kv_config* cfg_in, ql_kv** out) {
   kv->len.assign(static_cast<size_t>(std::max(1, cfg.num_layers)) * cfg.max_batch, 0);
   kv->bounds.assign(cfg.num_layers, nullptr);
   kv->bounded.assign(kv->len.size(), 0);
+  kv->replayed.assign(kv->len.size(), {});
   cudaError_t e = cudaMalloc(&kv->d_table, kv->table.size() * sizeof(int32_t));
   // Every entry -1 (all bytes 0xff).  The pool memsets above ran on the legacy
   // stream, which the context's non-blocking stream does not wait for: the
@@ -922,7 +965,8 @@ int ql_kv_update(ql_ctx* c, ql_kv* kv, int32_t layer, int32_t seq, const void* k
   a.seqs.start[0] = static_cast<int32_t>(cur);
   QL_CUDA(ql::launch_append(a, c->stream), "launch append");
   if (mem == QL_MEM_HOST) QL_CUDA(cudaStreamSynchronize(c->stream), "synchronize update");
-  len_at(kv, layer, seq) = cur + n;
+  const int64_t end = cur + n;
+  lengthen(kv, layer, &seq, &end, 1);
   return QL_OK;
 }
 
@@ -1115,7 +1159,7 @@ int ql_kv_append(ql_ctx* c, ql_kv* kv, const ql_append_args* a) {
   k.cache = view_of(kv, a->layer_idx);
   k.status = c->status;
   QL_CUDA(ql::launch_ragged_append(k, c->stream), "launch append");
-  for (int b = 0; b < a->batch; ++b) len_at(kv, a->layer_idx, k.rows.seq[b]) = ends[b];
+  lengthen(kv, a->layer_idx, k.rows.seq, ends, a->batch);
   return QL_OK;
 }
 
@@ -1472,7 +1516,7 @@ static int attn_forward_impl(ql_ctx* c, ql_kv* kv, const ql_attn_args* a,
               "copy out");
       QL_CUDA(cudaStreamSynchronize(c->stream), "synchronize forward");
     }
-    for (int b = 0; b < a->batch; ++b) len_at(kv, layer, seqs[b]) = ends[b];
+    lengthen(kv, layer, seqs, ends, a->batch);
     return QL_OK;
   }
   ql::AttnArgs at{};
@@ -1568,7 +1612,7 @@ static int attn_forward_impl(ql_ctx* c, ql_kv* kv, const ql_attn_args* a,
             "copy out");
     QL_CUDA(cudaStreamSynchronize(c->stream), "synchronize forward");
   }
-  for (int b = 0; b < a->batch; ++b) len_at(kv, layer, seqs[b]) = ends[b];
+  lengthen(kv, layer, seqs, ends, a->batch);
   return QL_OK;
 }
 
@@ -1664,8 +1708,9 @@ int ql_kv_append_prepare(ql_ctx* c, ql_kv* kv, const ql_attn_args* a, ql::CacheV
 }
 
 void ql_kv_append_commit(ql_kv* kv, const ql_attn_args* a) {
-  for (int b = 0; b < a->batch; ++b)
-    len_at(kv, a->layer_idx, a->seq_ids[b]) = a->start_pos[b] + a->new_len;
+  int64_t ends[ql::kMaxBatch];
+  for (int b = 0; b < a->batch; ++b) ends[b] = a->start_pos[b] + a->new_len;
+  lengthen(kv, a->layer_idx, a->seq_ids, ends, a->batch);
 }
 
 extern "C" {
@@ -1797,7 +1842,7 @@ int ql_attn_decode_noalloc(ql_ctx* c, ql_kv* kv, const ql_attn_args* a) {
   }
   QL_CUDA(ql::launch_splitkv_device_rope(at, &kv->kmap[layer], &kv->vmap[layer], jobs, c->stream),
           "launch no-allocation decode");
-  for (int b = 0; b < a->batch; ++b) len_at(kv, layer, seqs[b]) = ends[b];
+  lengthen(kv, layer, seqs, ends, a->batch);
   return QL_OK;
 }
 

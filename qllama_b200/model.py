@@ -296,7 +296,9 @@ def attention_forward_sparse(kv, layer: int, q_rot, start_pos, num_heads: int,
     KV head: the first `first`, the newest `last` and those whose keys can score highest
     (ql_attn_forward_sparse).  Returns (out, selected): selected, int32
     [batch, new_len, num_kv_heads, blocks] or None, receives the blocks' numbers in
-    ascending order, -1 behind them."""
+    ascending order, -1 behind them.  A layer's first call allocates its blocks' bounds: make
+    it before a capture; after rows that a captured call has scored were truncated and
+    appended anew, make an uncaptured call before its replay."""
     import torch
 
     L = _L or _start()

@@ -746,6 +746,73 @@ def test_first_sparse_call_is_not_captured(ctx, stream):
     assert torch.equal(out, want)
 
 
+@pytest.mark.parametrize("cache", ["q4_0", "f16"])
+def test_blocks_around_captures(ctx, stream, cache):
+    """Blocks are chosen by the keys that the cache holds: after a call that has been captured
+    and not yet replayed, and after each replay of a captured append."""
+    hq, hkv, hd = 8, 2, 128
+    kv, _ = filled(ctx, cache, [130], hkv, hd, spare=400)
+    q = normal(1, 1, 1, hq, hd, dtype="f16")
+    out = torch.zeros(1, 1, hq * hd, dtype=torch.float16, device="cuda")
+    sel = torch.zeros(1, 1, hkv, 4, dtype=torch.int32, device="cuda")
+
+    def choose(m, kv=kv):
+        qm.attention_forward_sparse(kv, 0, q, [m - 1], hq, hkv, hd, 4, 1, 1, out=out, selected=sel)
+
+    def check(m):
+        k, v = (x.double() for x in kv.read(0, [0], [m], out_dtype="f32"))
+        pick = chosen(q[0], k, cache, m - 1, 4, 1, 1)
+        assert torch.equal(sel[0], pick)
+        want, big = attention(q[0], k, v, m - 1, keep_of(pick, m))
+        near(out.view(1, hq, hd), want, big, top(v))
+
+    def rows(seed, n):
+        return normal(seed, n, hkv, hd, dtype="f16"), normal(seed + 1, n, hkv, hd, dtype="f16")
+
+    choose(520, filled(ctx, cache, [520], hkv, hd)[0])  # the workspace is there
+    choose(130)
+    kv.append(0, *rows(3, 320), [130], [320], THETA)
+    choose_only, append_only = torch.cuda.CUDAGraph(), torch.cuda.CUDAGraph()
+    ctx.synchronize()
+    with torch.cuda.graph(choose_only, stream=stream):
+        choose(450)
+    choose(450)  # the captured call has not run
+    check(450)
+    out.zero_(), sel.zero_()
+    choose_only.replay()
+    check(450)
+    k, v = rows(5, 70)
+    kv.append(0, k, v, [450], [70], THETA)  # pages and tables are there
+    kv.truncate(0, 450)
+    ctx.synchronize()
+    with torch.cuda.graph(append_only, stream=stream):
+        kv.append(0, k, v, [450], [70], THETA)
+    for seed in (7, 9, 11):
+        for a, b, gain in zip((k, v), rows(seed, 70), (seed, 1)):
+            a.copy_(b * gain)
+        append_only.replay()
+        choose(520)
+        check(520)
+    del choose_only, append_only
+
+
+def test_first_call_with_a_theta_is_not_captured(ctx, stream):
+    """The upload of the rotations is refused under capture, and the capture goes on."""
+    kv, _ = filled(ctx, "f16", [70], 2, 64, spare=2)
+    row = normal(1, 1, 2, 64, dtype="f16")
+    kv.append(0, row, row, [70], [1], THETA)
+    kv.truncate(0, 70)
+    graph = torch.cuda.CUDAGraph()
+    ctx.synchronize()
+    with torch.cuda.graph(graph, stream=stream):
+        with pytest.raises(qb.QllamaError, match="before the capture"):
+            kv.append(0, row, row, [70], [1], 2 * THETA)
+        kv.append(0, row, row, [70], [1], THETA)
+    graph.replay()
+    assert kv.read(0, [70], [1])[1].float().equal(row.float())
+    del graph
+
+
 def test_tensors_of_another_stream(ctx):
     """Tensors of torch's current stream, while the context has its own: made late on a busy
     stream, used and dropped at once."""
