@@ -600,7 +600,9 @@ __device__ __forceinline__ void block_range(double& least, double& most, double2
 // Scores: the group's queries enter by the sums of their positive and of their negative parts,
 // because sum_h max(q_h lo, q_h hi) = (sum_h max(q_h, 0)) hi + (sum_h min(q_h, 0)) lo while
 // lo <= hi: two products a channel whatever the group.  In f64, so that only equal blocks tie.
-// HD / 8 lanes a block (HD 64 or 128), else (HD 0) a warp.
+// HD / 8 lanes a block (HD 64 or 128), else (HD 0) a warp.  A block whose table entry is
+// outside the pool raises the status and scores the least, so that every score is written and
+// none is a NaN: the ranks below are then those of distinct places.
 //
 // Choice: a histogram over the range of the scores puts the border into one of kBins bins;
 // those above it are in, and the few in it are ranked among themselves by (score, block).
@@ -706,7 +708,9 @@ __global__ void __launch_bounds__(kChooseThreads)
 #pragma unroll
         for (int o = kLanes / 2; o > 0; o >>= 1) t += __shfl_xor_sync(0xffffffffu, t, o);
         if (t != t) t = CUDART_INF;  // a NaN counts as the largest score
-        if (x.p && sub == 0) score[base + round * kRound] = t;
+        if (!x.p) t = -CUDART_INF;  // on no page: flagged, and chosen last
+        const int block = base + round * kRound;
+        if (sub == 0 && block >= lo_block && block < end) score[block] = t;
       }
     } else {
       const int bt = half ? kF16 : kBF16;
@@ -721,7 +725,7 @@ __global__ void __launch_bounds__(kChooseThreads)
         }
         for (int o = 16; o > 0; o >>= 1) s += __shfl_xor_sync(0xffffffffu, s, o);
         if (s != s) s = CUDART_INF;
-        if (lane == 0) score[block] = s;
+        if (lane == 0) score[block] = p ? s : -CUDART_INF;
       }
     }
   }
@@ -842,8 +846,8 @@ __global__ void __launch_bounds__(kChooseThreads)
       const int up = __shfl_up_sync(0xffffffffu, before, o);
       if (lane >= o) before += up;
     }
-    int32_t* out = sel + done + before - n;
-    for (; w; w &= w - 1) *out++ = 32 * (w0 + lane) + __ffs(w) - 1;
+    for (int i = done + before - n; w; w &= w - 1, ++i)
+      if (i < a.take) sel[i] = 32 * (w0 + lane) + __ffs(w) - 1;
     done += __shfl_sync(0xffffffffu, before, 31);
   }
 }

@@ -1,0 +1,60 @@
+"""Calls on the paged cache that its documentation allows at the edges of what
+tests/test_cache_ops_gpu.py covers: rows and blocks around captures, clears and other
+rotations, keys and values far from 1, and what Python callers may pass.
+
+Tolerances count roundings, as there: u(t) = eps(t) / 2 for one rounding to t.
+"""
+import math
+
+import numpy as np
+import pytest
+import torch
+
+import qllama_b200 as qb
+from qllama_b200 import model as qm
+from tests.test_cache_ops_gpu import (THETA, attention, chosen, ctx, filled, keep_of, near, normal,  # noqa: F401
+                                      on_stream, q4_plain, q8_plain, refuses, rotated, stored, stream,
+                                      top, u)
+
+pytestmark = pytest.mark.gpu
+
+
+@pytest.mark.parametrize("cache, hq, hkv, hd", [("f16", 8, 2, 128), ("q4_0", 8, 2, 64),
+                                                ("f32", 4, 2, 48)])
+def test_choice_over_blocks_without_pages(stream, cache, hq, hkv, hd):
+    """A captured selection replayed after its sequence has been cleared: the table holds no
+    pages.  The status says so, and nothing is written beside the lists, whatever the
+    workspace held (here NaNs)."""
+    c = qb.Context(0)
+    c.set_stream(stream.cuda_stream)
+    m, blocks = 1300, 4
+    kv, _ = filled(c, cache, [m], hkv, hd)
+    other = qb.KvCache(c, 1, 256, 2, 64, "f16")
+    q = normal(1, 1, 1, hq, hd, dtype="f16")
+    out = torch.zeros(1, 1, hq * hd, dtype=torch.float16, device="cuda")
+    room = torch.full((3 * hkv, blocks), -7, dtype=torch.int32, device="cuda")
+    sel = room[hkv:2 * hkv].view(1, 1, hkv, blocks)
+    call = lambda: qm.attention_forward_sparse(kv, 0, q, [m - 1], hq, hkv, hd, blocks, 1, 1,
+                                               out=out, selected=sel)
+    nan = np.full((128, 64, 64), 0xffffffff, np.uint32).view(np.float32)
+
+    def fill_workspace():  # host rows are staged at its beginning
+        qb.attention_forward(other, 0, nan, nan[:, :2], nan[:, :2], 0, 64, 2, 64, THETA)
+        other.clear()
+
+    fill_workspace()
+    call()
+    c.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph, stream=stream):
+        call()
+    kv.clear_seq(0)
+    fill_workspace()
+    graph.replay()
+    with pytest.raises(qb.QllamaError, match="block-table"):
+        c.synchronize()
+    assert (room[:hkv] == -7).all() and (room[2 * hkv:] == -7).all()
+    # the first and the newest block, and of equal scores the lower ones
+    assert sel.view(hkv, blocks).tolist() == [[0, 1, 2, (m - 1) // 64]] * hkv
+    c.synchronize()
+    del graph
