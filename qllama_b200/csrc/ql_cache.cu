@@ -576,6 +576,24 @@ __device__ __forceinline__ void add_parts(float x, double& up, double& down) {
   else down += x;  // a NaN lands here
 }
 
+// Channels d0, d0 + step .. below end of one block's score by its definition, head for head, a
+// NaN passed on.  For the blocks whose score by parts is a NaN: there 0 times an infinite bound
+// may stand for queries that the group does not have.
+__device__ __noinline__ double score_by_heads(const void* q, size_t q0, int in_dtype, int group,
+                                              int hd, const uint16_t* bounds, int bound_dtype,
+                                              int d0, int step, int end) {
+  double s = 0.0;
+  for (int d = d0; d < end; d += step) {
+    const double lo = load_elem(bounds, d, bound_dtype), hi = load_elem(bounds, hd + d, bound_dtype);
+    for (int h = 0; h < group; ++h) {
+      const double x = load_elem(q, q0 + static_cast<size_t>(h) * hd + d, in_dtype);
+      const double a = x * lo, b = x * hi;
+      s += a != a ? a : b != b ? b : fmax(a, b);
+    }
+  }
+  return s;
+}
+
 // The least and the largest over the block's threads.
 __device__ __forceinline__ void block_range(double& least, double& most, double2* red) {
 #pragma unroll
@@ -599,7 +617,9 @@ __device__ __forceinline__ void block_range(double& least, double& most, double2
 //
 // Scores: the group's queries enter by the sums of their positive and of their negative parts,
 // because sum_h max(q_h lo, q_h hi) = (sum_h max(q_h, 0)) hi + (sum_h min(q_h, 0)) lo while
-// lo <= hi: two products a channel whatever the group.  In f64, so that only equal blocks tie.
+// lo <= hi are finite: two products a channel whatever the group.  In f64, so that only equal
+// blocks tie.  An infinite bound times a sum that is 0 for want of queries gives a NaN, and any
+// NaN sends the block to score_by_heads.
 // HD / 8 lanes a block (HD 64 or 128), else (HD 0) a warp.  A block whose table entry is
 // outside the pool raises the status and scores the least, so that every score is written and
 // none is a NaN: the ranks below are then those of distinct places.
@@ -707,7 +727,15 @@ __global__ void __launch_bounds__(kChooseThreads)
         double t = s[0] + s[1];
 #pragma unroll
         for (int o = kLanes / 2; o > 0; o >>= 1) t += __shfl_xor_sync(0xffffffffu, t, o);
-        if (t != t) t = CUDART_INF;  // a NaN counts as the largest score
+        if (__any_sync(0xffffffffu, t != t)) {
+          double e = 0.0;
+          if (t != t)
+            e = score_by_heads(a.q, q0, a.in_dtype, a.group, HD, x.p, half ? kF16 : kBF16, 8 * sub,
+                               1, 8 * sub + 8);
+#pragma unroll
+          for (int o = kLanes / 2; o > 0; o >>= 1) e += __shfl_xor_sync(0xffffffffu, e, o);
+          if (t != t) t = e == e ? e : CUDART_INF;  // a NaN counts as the largest score
+        }
         if (!x.p) t = -CUDART_INF;  // on no page: flagged, and chosen last
         const int block = base + round * kRound;
         if (sub == 0 && block >= lo_block && block < end) score[block] = t;
@@ -724,7 +752,11 @@ __global__ void __launch_bounds__(kChooseThreads)
           s += up * load_elem(p, c.hd + d, bt) + down * load_elem(p, d, bt);
         }
         for (int o = 16; o > 0; o >>= 1) s += __shfl_xor_sync(0xffffffffu, s, o);
-        if (s != s) s = CUDART_INF;
+        if (s != s) {  // (every lane alike)
+          s = score_by_heads(a.q, q0, a.in_dtype, a.group, c.hd, p, bt, lane, 32, c.hd);
+          for (int o = 16; o > 0; o >>= 1) s += __shfl_xor_sync(0xffffffffu, s, o);
+          if (s != s) s = CUDART_INF;
+        }
         if (lane == 0) score[block] = p ? s : -CUDART_INF;
       }
     }

@@ -58,3 +58,30 @@ def test_choice_over_blocks_without_pages(stream, cache, hq, hkv, hd):
     assert sel.view(hkv, blocks).tolist() == [[0, 1, 2, (m - 1) // 64]] * hkv
     c.synchronize()
     del graph
+
+
+@pytest.mark.parametrize("cache, hq, hkv, hd", [("f16", 8, 2, 128), ("bf16", 6, 2, 64),
+                                                ("f32", 4, 2, 48), ("f16", 9, 1, 128)])
+@pytest.mark.parametrize("signs", ["positive", "negative", "mixed", "zeros"])
+def test_blocks_with_infinite_keys(ctx, cache, hq, hkv, hd, signs):
+    """A bound that is infinite counts by the score's definition: a key of -inf under
+    positive queries only adds what the block's largest key gives.  (The keys' own weight is 0
+    there, but 0 * inf in the sums over their products is not: outputs are not compared.)"""
+    m, blocks = 64 * 14, 5
+    kv = qb.KvCache(ctx, 1, m, hkv, hd, cache)
+    k = normal(1, m, hkv, hd)
+    k[64 * 3 + 5, 0, 7] = -math.inf
+    k[64 * 5 + 1, :, 2] = math.inf
+    k[64 * 7:64 * 8, 0, 9] = -math.inf    # both bounds
+    k[64 * 8 + 2, :, 11] = -math.inf
+    k[64 * 8 + 3, :, 12] = math.inf
+    k[64 * 9:64 * 10, :, 13] = math.inf
+    kv.update(0, k, normal(2, m, hkv, hd), range(m))
+    q = normal(3, 1, 1, hq, hd, dtype="bf16")
+    q = q.abs() if signs == "positive" else -q.abs() if signs == "negative" else q
+    if signs == "zeros":
+        q[..., [7, 13]] = 0
+    sel = torch.empty(1, 1, hkv, blocks, dtype=torch.int32, device="cuda")
+    qm.attention_forward_sparse(kv, 0, q, [m - 1], hq, hkv, hd, blocks, 1, 1, selected=sel)
+    rows = kv.read(0, [0], [m], out_dtype="f32")[0].double()
+    assert torch.equal(sel[0], chosen(q[0], rows, cache, m - 1, blocks, 1, 1))
