@@ -16,7 +16,9 @@
 // A code c masked out of its word is the f16 number c 2^-24 (or, in the next nibble, c 2^-20):
 // f16's subnormals hold the codes exactly and the matrix instruction takes them as they are, so
 // that a fragment register costs one AND.  The powers of two are folded into q and the output.
-// A K scale multiplies the block's partial sums in f32, a V scale the probabilities in f16.  The
+// A K scale multiplies the block's partial sums in f32, a V scale the probabilities in f16 (V's
+// scales as they are, or times a power of two that keeps small ones' products out of f16's
+// subnormals and large ones' below its overflow).  The
 // 8 that is subtracted from every code enters S as the product of K's scales with -8 sum q of each
 // block, and leaves O with the product of ones and the same rounded P d that the codes met, so
 // that a rounding counts with the value and not with the code; ones and P give the sum of P.
@@ -43,10 +45,13 @@ namespace ql {
 namespace {
 
 constexpr float kLog2e4 = 1.4426950408889634f;
-// A probability is 2^arg with arg at most kTop (less where scales reach 2): below f16's
-// overflow times a scale, and far above its subnormals.  The reference it is relative to moves
-// only when an arg exceeds that, by enough to leave kSlack free.
-constexpr float kTop = 14.f, kSlack = 6.f;
+// A probability is 2^arg with arg at most kTop: times a scale below 2 it is below f16's overflow.
+// The reference it is relative to moves only when an arg exceeds that, by enough to leave kSlack
+// free.  What is free is lost at the other end, where f16's subnormals begin 25 powers of two
+// below: outputs of positions that are e^18 times less likely than another one without a value
+// are 0.0005 of their norm off (with six bits free 0.003, and 8 x 32768 in 66.5 instead of 67.1
+// us; with one 0.0004 and 67.8 us).
+constexpr float kTop = 14.f, kSlack = 3.f;
 
 template <int HD>
 struct Attn4Cfg {
@@ -102,6 +107,11 @@ __device__ __forceinline__ float ex2(float x) {  // 2^x; -inf -> +0
   float y;
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
   return y;
+}
+
+// Orders this thread's stores to shared memory before later bulk copies into it.
+__device__ __forceinline__ void fence_proxy_async_shared() {
+  asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
 }
 
 __device__ __forceinline__ float half_of(const uint32_t& w, bool high) {
@@ -420,7 +430,11 @@ __global__ void __launch_bounds__(32 * Attn4Cfg<HD>::kWarps, 1)
     for (int b = 0; b < NB; ++b)
 #pragma unroll
       for (int u = 0; u < 2; ++u) o[b][u][0] = o[b][u][1] = o[b][u][2] = o[b][u][3] = 0.f;
-    float ref[2] = {0.f, 0.f}, top = kTop;
+    float ref[2] = {0.f, 0.f};
+    // V's scales enter times 2^vexp: as they are where the first tile's largest is of ordinary size,
+    // else by what takes it to [2^-2, 2^-1).  vexp only falls then, when a scale would reach 2.
+    constexpr int kUnset = 99;
+    int vexp = kUnset;
     bool fresh = true;
     uint32_t nans = 0;  // of row 2 tq + k: bit 4 k + b, that it sees a value of block b that is NaN
 
@@ -431,6 +445,78 @@ __global__ void __launch_bounds__(32 * Attn4Cfg<HD>::kWarps, 1)
       const int p0 = (x - job.t0) * kTile;
       const bool tail = p0 + kTile > all;
       const int slices = alive ? min(4, (most - p0 + 15) / 16) : 0;
+      // V's scales, those of positions 2 lane and 2 lane + 1 by each lane: where they cannot be
+      // taken as they are, they are written anew into the stage.  (2 or more and NaN ones have
+      // the exponent's top bit.)
+      uint32_t d2[NB], any_d = 0;
+      uint32_t* d2_at = reinterpret_cast<uint32_t*>(ring + stage * C::kRecord + kRec.v_scales()) + NB * lane;
+      if constexpr (NB == 4) {
+        const uint4 w = *reinterpret_cast<const uint4*>(d2_at);
+        d2[0] = w.x, d2[1] = w.y, d2[2] = w.z, d2[3] = w.w;
+      } else {
+        const uint2 w = *reinterpret_cast<const uint2*>(d2_at);
+        d2[0] = w.x, d2[1] = w.y;
+      }
+#pragma unroll
+      for (int b = 0; b < NB; ++b) any_d |= d2[b];
+      if (slices > 0 && __any_sync(0xffffffffu, any_d & (vexp == 0 ? 0x40004000u : ~0u))) {
+        // Behind the end, or behind what a row sees, P is 0, and 0 times NaN is not: scales behind
+        // the end are taken out, and NaN ones are, and the blocks and rows that see those remembered.
+        bool anew = p0 + kTile > most;
+        if (anew) {
+#pragma unroll
+          for (int b = 0; b < NB; ++b)
+            d2[b] &= (p0 + 2 * lane < most ? 0xffffu : 0u) | (p0 + 2 * lane + 1 < most ? 0xffff0000u : 0u);
+        }
+        auto largest = [&] {  // its bits
+          uint32_t m = 0;
+#pragma unroll
+          for (int b = 0; b < NB; ++b) m = __vmaxu2(m, d2[b] & 0x7fff7fffu);
+          return __reduce_max_sync(0xffffffffu, max(m & 0xffffu, m >> 16));
+        };
+        uint32_t big = largest();
+        if (big > 0x7c00u) {
+#pragma unroll
+          for (int b = 0; b < NB; ++b)
+#pragma unroll
+            for (int r = 0; r < 2; ++r) {
+              const bool bad = ((r ? d2[b] >> 16 : d2[b]) & 0x7fffu) > 0x7c00u;
+              if (bad) d2[b] &= r ? 0xffffu : 0xffff0000u;
+              for (uint32_t lanes = __ballot_sync(0xffffffffu, bad); lanes; lanes &= lanes - 1) {
+                const int place = p0 + 2 * (__ffs(lanes) - 1) + r;
+#pragma unroll
+                for (int k = 0; k < 2; ++k) nans |= (place < lim[k] ? 1u : 0u) << (4 * k + b);
+              }
+            }
+          big = largest();
+          anew = true;
+        }
+        const int large = big >= 0x400u ? static_cast<int>(big >> 10) - 15 : big ? 7 - __clz(big) : -24;
+        int next = vexp;
+        if (vexp == kUnset ? large < -4 || large > 0 : large + vexp > 0)
+          next = min(max(-2 - large, -15), 15);
+        else if (vexp == kUnset)
+          next = 0;
+        if (next != vexp && vexp != kUnset) {
+          const float corr = pow2f(next - vexp);
+#pragma unroll
+          for (int b = 0; b < NB; ++b)
+#pragma unroll
+            for (int k = 0; k < 4; ++k) {
+              off[b][k] *= corr;
+              o[b][0][k] *= corr;
+              o[b][1][k] *= corr;
+            }
+        }
+        vexp = next;
+        if (anew || vexp != 0) {
+          const uint32_t half = vexp > -15 ? (vexp + 15) << 10 : 0x200u;  // 2^vexp
+#pragma unroll
+          for (int b = 0; b < NB; ++b) d2_at[b] = mul2(d2[b], half << 16 | half);
+          fence_proxy_async_shared();  // before the next copy into the stage
+          __syncwarp();
+        }
+      }
       // Two times 16 positions at once: independent chains for the scheduler.
       for (int s = 0; s < slices; s += 2) {
         // of positions 16 s on; 16 positions further lie 256 NB bytes of codes and 32 NB of scales
@@ -484,7 +570,7 @@ __global__ void __launch_bounds__(32 * Attn4Cfg<HD>::kWarps, 1)
           }
         }
         // ---- V's scales of positions 2 tq, 2 tq + 1 and those plus 8
-        uint32_t vd[2][2][NB], any_d = 0;
+        uint32_t vd[2][2][NB];
 #pragma unroll
         for (int e = 0; e < 2; ++e)
 #pragma unroll
@@ -493,11 +579,9 @@ __global__ void __launch_bounds__(32 * Attn4Cfg<HD>::kWarps, 1)
             if constexpr (NB == 4) {
               const uint4 d = *reinterpret_cast<const uint4*>(sp);
               vd[e][r][0] = d.x, vd[e][r][1] = d.y, vd[e][r][2] = d.z, vd[e][r][3] = d.w;
-              any_d |= d.x | d.y | d.z | d.w;
             } else {
               const uint2 d = *reinterpret_cast<const uint2*>(sp);
               vd[e][r][0] = d.x, vd[e][r][1] = d.y;
-              any_d |= d.x | d.y;
             }
           }
         // ---- softmax: columns 2 tq, 2 tq + 1 of positions g and g + 8
@@ -515,36 +599,9 @@ __global__ void __launch_bounds__(32 * Attn4Cfg<HD>::kWarps, 1)
 #pragma unroll
           for (int k = 0; k < 4; ++k) {
             p[e][k] = fmaf(y[e][k], f[k & 1], -ref[k & 1]);
-            over |= p[e][k] > top;
+            over |= p[e][k] > kTop;
           }
-        // (a scale of 2 or more, or a NaN, has the exponent's top bit)
-        float cap = top;
-        if (__any_sync(0xffffffffu, any_d & 0x40004000u)) {
-          // NaN scales are taken out here and the blocks and rows that see them remembered:
-          // behind the end of a sequence, or of what a row sees, P is 0 and 0 times NaN is not.
-          uint32_t big = 0;  // the largest scale's bits
-#pragma unroll
-          for (int e = 0; e < 2; ++e)
-#pragma unroll
-            for (int r = 0; r < 4; ++r)
-#pragma unroll
-              for (int b = 0; b < NB; ++b) {
-                uint32_t& w = vd[e][r >> 1][b];
-                const uint32_t h = (r & 1 ? w >> 16 : w) & 0x7fffu;
-                const bool bad = h > 0x7c00u;
-                if (!bad) big = max(big, h);
-                const uint32_t lanes = __ballot_sync(0xffffffffu, bad) & 15u;  // of tq 0..3
-                if (lanes) {
-                  if (bad) w &= r & 1 ? 0xffffu : 0xffff0000u;
-                  const int place = p0 + 16 * (s + e) + 2 * (__ffs(lanes) - 1) + (r & 1) + 8 * (r >> 1);
-#pragma unroll
-                  for (int k = 0; k < 2; ++k) nans |= (place < lim[k] ? 1u : 0u) << (4 * k + b);
-                }
-              }
-          big = __reduce_max_sync(0xffffffffu, big);
-          cap = fminf(top, kTop - fmaxf(0.f, static_cast<float>(static_cast<int>(big >> 10) - 15)));
-        }
-        if (__any_sync(0xffffffffu, over) || fresh || cap != top) {
+        if (__any_sync(0xffffffffu, over) || fresh) {
 #pragma unroll
           for (int k = 0; k < 2; ++k) {
             // NaN does not count
@@ -553,8 +610,8 @@ __global__ void __launch_bounds__(32 * Attn4Cfg<HD>::kWarps, 1)
             m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, 4));
             m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, 8));
             m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, 16));
-            float next = ref[k] + (top - cap);
-            if ((fresh || m - next > cap) && m > -CUDART_INF_F) next = m - (cap - kSlack);
+            float next = ref[k];
+            if ((fresh || m - next > kTop) && m > -CUDART_INF_F) next = m - (kTop - kSlack);
             const float corr = fresh ? 0.f : ex2(ref[k] - next);
             ref[k] = next;
             sum[k] *= corr;
@@ -568,7 +625,6 @@ __global__ void __launch_bounds__(32 * Attn4Cfg<HD>::kWarps, 1)
               }
             }
           }
-          top = cap;
           fresh = false;
 #pragma unroll
           for (int e = 0; e < 2; ++e)
@@ -630,7 +686,7 @@ __global__ void __launch_bounds__(32 * Attn4Cfg<HD>::kWarps, 1)
     for (int k = 0; k < 2; ++k) {
       const int r = 2 * tq + k;
       const bool live = r < job.rows;
-      const float f24 = 16777216.f * (whole ? 1.f / sum[k] : 1.f);
+      const float f24 = 16777216.f * pow2f(vexp == kUnset ? 0 : -vexp) * (whole ? 1.f / sum[k] : 1.f);
       const size_t base = whole && live ? row_offset(a, job, job.row0 + r, HD) : 0;
       float eight[NB];  // 8 sum P d of each block, in the units of O
 #pragma unroll

@@ -85,3 +85,66 @@ def test_blocks_with_infinite_keys(ctx, cache, hq, hkv, hd, signs):
     qm.attention_forward_sparse(kv, 0, q, [m - 1], hq, hkv, hd, blocks, 1, 1, selected=sel)
     rows = kv.read(0, [0], [m], out_dtype="f32")[0].double()
     assert torch.equal(sel[0], chosen(q[0], rows, cache, m - 1, blocks, 1, 1))
+
+
+def off_by(got, want):
+    """The largest distance of a head's output, relative to its norm."""
+    return float(((got.double() - want).norm(dim=-1) / want.norm(dim=-1)).max())
+
+
+# Of outputs that are sums of many independent values of mean 0, each times a probability that
+# has been rounded to f16 alone and once more with V's scale: 2 * 2^-11 of each at most, and the
+# sums' norms are in the same proportion.  (Scores add 2^-18 of their sum of magnitudes.)
+NORM = 1e-3
+
+
+@pytest.mark.parametrize("size", [1.0, 1e-2, 1e-3, 1e-4, 300.0])
+@pytest.mark.parametrize("gap", [0, 10, 14])
+def test_small_values_beside_a_position_without_any(ctx, size, gap):
+    """Values far from 1, and a first position that takes nearly all of the weight, `gap` above
+    the others' scores, but has no value (an attention sink)."""
+    B, hq, hkv, hd, m = 20, 8, 2, 128, 2050
+    kv = qb.KvCache(ctx, 1, m, hkv, hd, "q4_0", 64, B)
+    for b in range(B):
+        k, v = normal(b, m, hkv, hd), normal(b + 100, m, hkv, hd, scale=size)
+        k[0], v[0] = 0, 0
+        k[:, :, 0] = 0
+        k[0, :, 0] = 8
+        kv.update(0, k, v, range(m), seq=b)
+    q = normal(200, B, 1, hq, hd)
+    q[..., 0] = gap * math.sqrt(hd) / 8
+    out = qm.attention_forward_appended(kv, 0, q, [m - 1] * B, hq, hkv, hd, THETA)
+    for b in range(B):
+        kc, vc = (x.double() for x in kv.read(0, [0], [m], [b]))
+        want, _ = attention(q[b], kc, vc, m - 1)
+        assert off_by(out[b].view(1, hq, hd), want) <= NORM
+
+
+@pytest.mark.parametrize("hd", [64, 128])
+@pytest.mark.parametrize("n", [1, 4])
+@pytest.mark.parametrize("order", ["rising", "falling", "behind the end"])
+def test_values_of_changing_size(ctx, hd, n, order):
+    """Values whose size doubles (or halves) from tile to tile, over f16's range and more; and
+    large and NaN rows behind the end of a sequence of small ones."""
+    hq, hkv, m = 8, 2, 64 * 24 + 37
+    kv = qb.KvCache(ctx, 1, 64 * 27, hkv, hd, "q4_0", 128, 2)
+    k, v = normal(1, m, hkv, hd), normal(2, m, hkv, hd)
+    if order == "behind the end":
+        bad = torch.full((64 * 27, hkv, hd), 3e4, device="cuda")
+        bad[1::2] = math.nan
+        kv.update(0, bad, bad, range(64 * 27), seq=0)
+        kv.update(0, bad, bad, range(64 * 27), seq=1)
+        kv.truncate([0, 1], [0, 0])
+        v *= 1e-3
+    else:
+        tile = torch.arange(m, device="cuda") // 64
+        v *= 2.0 ** (tile - 13 if order == "rising" else 11 - tile)[:, None, None]
+    for s in (0, 1):
+        kv.update(0, k[:m - 900 * s], v[:m - 900 * s], range(m - 900 * s), seq=s)
+    q = normal(3, 2, n, hq, hd)
+    start = [m - n, m - 900 - n]
+    out = qm.attention_forward_appended(kv, 0, q, start, hq, hkv, hd, THETA)
+    for s in (0, 1):
+        kc, vc = (x.double() for x in kv.read(0, [0], [m - 900 * s], [s]))
+        want, _ = attention(q[s], kc, vc, start[s])
+        assert off_by(out[s].view(n, hq, hd), want) <= NORM
