@@ -164,7 +164,10 @@ int ql_kv_get(ql_ctx* ctx, const ql_kv* kv, int32_t layer, int32_t seq,
  * one that ql_kv_update stores, and likewise d); q_out gets the rotated queries rounded to q_out_dtype.
  * q_out [tokens, num_heads, head_dim] is contiguous and may be q itself (of the same type,
  * contiguous); any other overlap with an input is refused.  Device pointers, aligned to
- * their element size. */
+ * their element size.
+ * A cache's first call with a theta, of this function or of ql_attn_forward, makes a table of
+ * its rotations on the host and waits for the upload: make it before a capture.  Up to four
+ * tables are kept, and beside them those that captured calls read. */
 typedef struct {
   int32_t layer_idx;
   int32_t batch;             /* sequences, each slot once (0 is a no-op) */

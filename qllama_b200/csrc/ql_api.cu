@@ -141,6 +141,16 @@ struct ql_kv {
     int32_t begin = 0, end = 0;
   };
   std::vector<Blocks> replayed;
+  // The rotations of the thetas that calls have come with; d_rope and rope_theta are the last
+  // call's.  A captured graph goes on reading its table, so that one is never rewritten.
+  struct Rope {
+    float theta = 0.f;
+    double2* table = nullptr;
+    bool captured = false;
+    uint64_t used = 0;  // the call that used it last
+  };
+  std::vector<Rope> ropes;
+  uint64_t rope_calls = 0;
 };
 
 namespace {
@@ -272,14 +282,31 @@ int ensure_identity(ql_kv* kv) {
   return QL_OK;
 }
 
-// Builds (once per theta) the f64 (cos, sin) table of every position with the
-// reference formula: freq_i = theta^(-2i/hd) via pow, angle = pos * freq_i
-// (src/tensor/ops.rs:193-207), evaluated by the host libm as the reference does.
+// Makes d_rope the f64 (cos, sin) table of every position for a theta, with the reference
+// formula: freq_i = theta^(-2i/hd) via pow, angle = pos * freq_i
+// (src/tensor/ops.rs:193-207), evaluated by the host libm as the reference does.  A cache keeps
+// the tables of its last kRopes thetas, and beside them those that captured graphs read.
 int ensure_rope(ql_kv* kv, float theta) {
   const int r = ensure_identity(kv);
   if (r != QL_OK) return r;
-  if (kv->d_rope && kv->rope_theta == theta) return QL_OK;
-  if (is_capturing(kv->ctx->stream))
+  constexpr size_t kRopes = 4;
+  const bool capturing = is_capturing(kv->ctx->stream);
+  ++kv->rope_calls;
+  size_t free_ones = 0;
+  ql_kv::Rope* oldest = nullptr;
+  for (ql_kv::Rope& t : kv->ropes) {
+    if (t.theta == theta) {
+      t.captured |= capturing;
+      t.used = kv->rope_calls;
+      kv->d_rope = t.table;
+      kv->rope_theta = theta;
+      return QL_OK;
+    }
+    if (t.captured) continue;
+    ++free_ones;
+    if (!oldest || t.used < oldest->used) oldest = &t;
+  }
+  if (capturing)
     return fail(QL_ERR_INVALID, "a first call with a theta uploads its rotations: make it before "
                 "the capture");
   const int hd = kv->cfg.head_dim, pairs = hd / 2, n = kv->cfg.max_seq_len;
@@ -309,16 +336,30 @@ int ensure_rope(ql_kv* kv, float theta) {
   }
   fill(done, n);
   for (std::thread& t : threads) t.join();
-  if (!kv->d_rope) {
-    QL_CUDA(cudaMalloc(&kv->d_rope, std::max<size_t>(1, tab.size()) * sizeof(double2)),
-            "allocate rope table");
+  if (free_ones < kRopes) {
+    double2* table = nullptr;
+    const cudaError_t e = cudaMalloc(&table, std::max<size_t>(1, tab.size()) * sizeof(double2));
+    if (e == cudaSuccess) {
+      kv->ropes.push_back({theta, table});
+      oldest = &kv->ropes.back();
+    } else if (oldest) {
+      cudaGetLastError();  // no room for one more: the oldest makes way
+    } else {
+      return cuda_fail(e, "allocate rope table");
+    }
   }
+  ql_kv::Rope& t = *oldest;
+  t.theta = 0.f;  // of no call until the upload is done
+  t.used = kv->rope_calls;
+  kv->d_rope = nullptr;
   // On the context's stream (the kernels that read the table run there), and
   // waited for before the host vector goes away.
-  QL_CUDA(cudaMemcpyAsync(kv->d_rope, tab.data(), tab.size() * sizeof(double2),
+  QL_CUDA(cudaMemcpyAsync(t.table, tab.data(), tab.size() * sizeof(double2),
                           cudaMemcpyHostToDevice, kv->ctx->stream),
           "upload rope table");
   QL_CUDA(cudaStreamSynchronize(kv->ctx->stream), "wait for the rope table upload");
+  t.theta = theta;
+  kv->d_rope = t.table;
   kv->rope_theta = theta;
   return QL_OK;
 }
@@ -801,7 +842,7 @@ int ql_kv_destroy(ql_kv* kv) {
   for (void* p : kv->vs) cudaFree(p);
   for (void* p : kv->bounds) cudaFree(p);
   if (kv->d_table) cudaFree(kv->d_table);
-  if (kv->d_rope) cudaFree(kv->d_rope);
+  for (const ql_kv::Rope& t : kv->ropes) cudaFree(t.table);
   if (kv->d_rope_id) cudaFree(kv->d_rope_id);
   delete kv;
   return QL_OK;

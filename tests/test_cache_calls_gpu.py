@@ -148,3 +148,59 @@ def test_values_of_changing_size(ctx, hd, n, order):
         kc, vc = (x.double() for x in kv.read(0, [0], [m - 900 * s], [s]))
         want, _ = attention(q[s], kc, vc, start[s])
         assert off_by(out[s].view(n, hq, hd), want) <= NORM
+
+
+@pytest.mark.parametrize("call", ["append", "forward", "appended rows of a projection"])
+def test_captured_rotations_stay_those_of_their_theta(ctx, stream, call):
+    """A captured call replays with its own theta, whatever other calls on the cache rotate by
+    in between; calls of several thetas alternate, also inside one graph."""
+    hq, hkv, hd, n = 4, 2, 64, 3
+    thetas = [1e4, 5e5, 1e6, 1e3, 2e4, 3e4]
+    kv = qb.KvCache(ctx, 1, 128, hkv, hd, "f32")
+    q, k, v = (normal(i, n, h, hd) for i, h in ((1, hq), (2, hkv), (3, hkv)))
+    x, w = normal(4, 1, n, 32), normal(5, 32, (hq + 2 * hkv) * hd)
+
+    def run(theta, start=40):
+        """(the rotated keys' positions, the keys before the rotation)"""
+        if call == "append":
+            kv.append(0, k, v, [start], [n], theta)
+            return k
+        if call == "forward":
+            qb.attention_forward(kv, 0, q, k, v, start, hq, hkv, hd, theta)
+            return k
+        qm.qkv_rope_append(kv, 0, x, w, start, hq, hkv, hd, theta)
+        return (x[0].double() @ w.double())[:, hq * hd:(hq + hkv) * hd].float().view(n, hkv, hd)
+
+    def check(theta, start=40):
+        got, want = kv.read(0, [start], [n])[0], rotated(keys, range(start, start + n), theta)
+        # (a projection's products are summed in f32: 32 terms of up to 4 * 4)
+        off = 0 if call != "appended rows of a projection" else 32 * 32 * 16 * 2.0 ** -24
+        torch.testing.assert_close(got, want, rtol=0, atol=off)
+
+    zeros = torch.zeros(40, hkv, hd, device="cuda")
+    kv.update(0, zeros, zeros, range(40))
+    for t in thetas[:2]:
+        keys = run(t)
+        check(t)
+        kv.truncate(0, 40)
+    ctx.synchronize()
+    graph, both = torch.cuda.CUDAGraph(), torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph, stream=stream):
+        run(thetas[0])
+    kv.truncate(0, 40)
+    with torch.cuda.graph(both, stream=stream):
+        run(thetas[1])
+        run(thetas[0], 40 + n)
+    for t in thetas[1:]:
+        kv.truncate(0, 40)
+        run(t)
+        check(t)
+        graph.replay()
+        check(thetas[0])
+    kv.truncate(0, 40)
+    run(thetas[2])
+    run(thetas[2], 40 + n)
+    both.replay()
+    check(thetas[1])
+    check(thetas[0], 40 + n)
+    del graph, both
