@@ -365,9 +365,9 @@ int ensure_rope(ql_kv* kv, float theta) {
 }
 
 // Queues the upload of the block-table entries listed in idx[0..n) (their
-// values taken from the host mirror) as table patch launches on the
-// context's stream: stream-ordered, with no host synchronisation.
-int upload_table_entries(ql_kv* kv, const int32_t* idx, size_t n) {
+// values taken from the host mirror) as table patch launches on stream s, the
+// context's: stream-ordered, with no host synchronisation.
+int upload_table_entries(ql_kv* kv, const int32_t* idx, size_t n, cudaStream_t s) {
   ql::TablePatch p;
   p.table = kv->d_table;
   for (size_t i0 = 0; i0 < n; i0 += ql::kTablePatchMax) {
@@ -377,10 +377,17 @@ int upload_table_entries(ql_kv* kv, const int32_t* idx, size_t n) {
       p.idx[i] = idx[i0 + i];
       p.val[i] = kv->table[static_cast<size_t>(idx[i0 + i])];
     }
-    QL_CUDA(ql::launch_table_patch(p, kv->ctx->stream), "launch block-table patch");
+    QL_CUDA(ql::launch_table_patch(p, s), "launch block-table patch");
   }
   return QL_OK;
 }
+
+// Lets this thread wait for a stream that is not being captured while another one is.
+struct CaptureAside {
+  cudaStreamCaptureMode mode = cudaStreamCaptureModeRelaxed;
+  CaptureAside() { cudaThreadExchangeStreamCaptureMode(&mode); }
+  ~CaptureAside() { cudaThreadExchangeStreamCaptureMode(&mode); }
+};
 
 // Gives every listed sequence the pages its new length needs; rolls back on
 // exhaustion so that the call stays transactional.  New entries reach the
@@ -388,6 +395,10 @@ int upload_table_entries(ql_kv* kv, const int32_t* idx, size_t n) {
 // host synchronisation, no per-call allocation); *patched tells the caller
 // that a split-KV launch following it must not use programmatic dependent
 // launch (that kernel reads the table before its grid dependency wait).
+// While that stream is being captured the entries are written at once, by another stream, and
+// waited for: the host's table says from here on that the pages are the sequence's, whether or
+// not, and when, the graph is launched.  (They were no sequence's, and nothing in flight reads
+// or writes their entries: ql_kv_clear_seq waits for its own.)
 int reserve_pages(ql_kv* kv, const int32_t* seqs, const int64_t* ends, int count, bool* patched) {
   const int P = kv->cfg.page_size, pps = kv->pages_per_seq;
   *patched = false;
@@ -415,7 +426,16 @@ int reserve_pages(ql_kv* kv, const int32_t* seqs, const int64_t* ends, int count
     }
   }
   if (!kv->patch_idx.empty()) {
-    const int r = upload_table_entries(kv, kv->patch_idx.data(), kv->patch_idx.size());
+    const int32_t* idx = kv->patch_idx.data();
+    const size_t n = kv->patch_idx.size();
+    if (is_capturing(kv->ctx->stream)) {
+      const CaptureAside mode;
+      const int r = upload_table_entries(kv, idx, n, kv->ctx->aside);
+      if (r != QL_OK) return r;
+      QL_CUDA(cudaStreamSynchronize(kv->ctx->aside), "wait for the block-table patch");
+      return QL_OK;
+    }
+    const int r = upload_table_entries(kv, idx, n, kv->ctx->stream);
     if (r != QL_OK) return r;
     *patched = true;
   }
@@ -680,6 +700,7 @@ int ql_ctx_create(int device, ql_ctx** out) {
   c->device = device;
   c->num_sms = prop.multiProcessorCount;
   e = cudaStreamCreateWithFlags(&c->own, cudaStreamNonBlocking);
+  if (e == cudaSuccess) e = cudaStreamCreateWithFlags(&c->aside, cudaStreamNonBlocking);
   if (e == cudaSuccess) e = cudaMalloc(&c->status, sizeof(uint32_t));
   if (e == cudaSuccess) e = cudaMemsetAsync(c->status, 0, sizeof(uint32_t), c->own);
   if (e == cudaSuccess) e = cudaStreamSynchronize(c->own);
@@ -703,6 +724,7 @@ int ql_ctx_destroy(ql_ctx* c) {
   for (cudaEvent_t e : c->order)
     if (e) cudaEventDestroy(e);
   if (c->own) cudaStreamDestroy(c->own);
+  if (c->aside) cudaStreamDestroy(c->aside);
   delete c;
   return QL_OK;
 }
@@ -876,9 +898,11 @@ int ql_kv_clear_seq(ql_kv* kv, int32_t seq) {
     }
     kv->seq_pages[seq] = 0;
     // the device table follows the mirror (-1: the slot owns no page)
-    const int r = upload_table_entries(kv, kv->patch_idx.data(), kv->patch_idx.size());
+    const int r = upload_table_entries(kv, kv->patch_idx.data(), kv->patch_idx.size(),
+                                       kv->ctx->stream);
     kv->patch_idx.clear();
     if (r != QL_OK) return r;
+    QL_CUDA(cudaStreamSynchronize(kv->ctx->stream), "wait for the released pages");
   }
   return QL_OK;
 }
@@ -1185,8 +1209,8 @@ int ql_kv_append(ql_ctx* c, ql_kv* kv, const ql_append_args* a) {
   ql_device_guard dev(c->device);
   QL_CUDA(dev.error(), "set device");
   bool patched = false;  // the append is an ordinary launch: it sees the patch
-  r = reserve_pages(kv, k.rows.seq, ends, a->batch, &patched);
-  if (r == QL_OK) r = ensure_rope(kv, a->rope_theta);
+  r = ensure_rope(kv, a->rope_theta);
+  if (r == QL_OK) r = reserve_pages(kv, k.rows.seq, ends, a->batch, &patched);
   if (r != QL_OK) return r;
   k.q = hq > 0 ? a->q : nullptr;
   k.k = a->k;
@@ -1337,10 +1361,9 @@ static int attn_forward_impl(ql_ctx* c, ql_kv* kv, const ql_attn_args* a,
                 "decode on the split-KV kernel");
   QL_CUDA(cudaSetDevice(c->device), "set device");
   bool patched = false;
-  int r = appended ? QL_OK : reserve_pages(kv, seqs, ends, a->batch, &patched);
-  if (r != QL_OK) return r;
   // rows that are in the cache were rotated when they were appended
-  r = appended ? ensure_identity(kv) : ensure_rope(kv, a->rope_theta);
+  int r = appended ? ensure_identity(kv) : ensure_rope(kv, a->rope_theta);
+  if (r == QL_OK && !appended) r = reserve_pages(kv, seqs, ends, a->batch, &patched);
   if (r != QL_OK) return r;
   if (sparse) {
     r = ensure_bounds(c, kv, layer, seqs, a->batch);
@@ -1740,8 +1763,8 @@ int ql_kv_append_prepare(ql_ctx* c, ql_kv* kv, const ql_attn_args* a, ql::CacheV
   }
   QL_CUDA(cudaSetDevice(c->device), "set device");
   bool patched = false;
-  int r = n > 0 ? reserve_pages(kv, seqs, ends, a->batch, &patched) : QL_OK;
-  if (r == QL_OK) r = ensure_rope(kv, a->rope_theta);
+  int r = ensure_rope(kv, a->rope_theta);
+  if (r == QL_OK && n > 0) r = reserve_pages(kv, seqs, ends, a->batch, &patched);
   if (r != QL_OK) return r;
   *view = view_of(kv, layer);
   *rope = kv->d_rope;

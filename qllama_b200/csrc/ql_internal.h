@@ -23,6 +23,7 @@ struct ql_ctx {
   bool counters_captured = false;  // a captured graph uses them
   std::vector<void*> retired;   // outgrown workspaces and counters of captured graphs
   cudaEvent_t order[2] = {nullptr, nullptr};  // of ql_ctx_wait_stream and ql_ctx_join_stream
+  cudaStream_t aside = nullptr;  // for what has to happen at once while `stream` is captured
 };
 
 // Records the message of a failed call (ql_last_error) and returns `code`.

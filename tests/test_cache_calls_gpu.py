@@ -204,3 +204,49 @@ def test_captured_rotations_stay_those_of_their_theta(ctx, stream, call):
     check(thetas[1])
     check(thetas[0], 40 + n)
     del graph, both
+
+
+@pytest.mark.parametrize("cache", ["f16", "q4_0"])
+@pytest.mark.parametrize("then", ["discarded", "refused", "replayed late"])
+def test_pages_taken_under_capture(ctx, stream, cache, then):
+    """Pages that a captured call takes are the sequence's for later calls too: where the
+    capture is thrown away, where a part of it is refused, and before its first replay."""
+    hq, hkv, hd, m, n = 4, 2, 64, 60, 70
+    kv = qb.KvCache(ctx, 1, 256, hkv, hd, cache, 64, 2)
+    old, k, v = (normal(i, r, hkv, hd, dtype="f16") for i, r in ((1, m), (2, n), (3, n)))
+    q = normal(4, n, hq, hd, dtype="f16")
+    kv.append(0, old, old, [m - 60], [60], THETA)
+    first = normal(5, 200, hkv, hd, dtype="f16")
+    kv.append(0, first, first, [0], [200], THETA, seq_ids=[1])
+    kv.clear_seq(1)  # its pages are handed out anew
+    q_out = torch.empty_like(q)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph, stream=stream):
+        if then == "refused":
+            with pytest.raises(qb.QllamaError, match="before the capture"):
+                kv.append(0, k, v, [m], [n], 3 * THETA, q=q, q_out=q_out)
+        kv.append(0, k, v, [m], [n], THETA, q=q, q_out=q_out)
+    kv.truncate(0, m)
+    if then == "discarded":
+        graph.reset()
+    places = range(m, m + n)
+
+    def check(k, v):
+        got = kv.read(0, [m], [n])
+        for x, y in zip(got, (rotated(k, places), v.float())):
+            torch.testing.assert_close(x.double(), stored(y, cache), rtol=0, atol=0)
+        out = qm.attention_forward_appended(kv, 0, normal(6, 1, 1, hq, hd), [m + n - 1], hq, hkv,
+                                            hd, THETA)
+        kc, vc = (x.double() for x in kv.read(0, [0], [m + n], out_dtype="f32"))
+        want, big = attention(normal(6, 1, hq, hd), kc, vc, m + n - 1)
+        near(out.view(1, hq, hd), want, big, top(vc))
+        ctx.synchronize()  # no kernel met an entry outside the pool
+
+    other = normal(7, n, hkv, hd, dtype="f16")
+    kv.append(0, other, k, [m], [n], THETA, q=q)
+    check(other, k)
+    if then != "discarded":
+        graph.replay()
+        check(k, v)
+        assert torch.equal(q_out, rotated(q, places).half())
+    del graph
