@@ -78,7 +78,8 @@ __device__ __forceinline__ double2 rope_cs(const RopeSrc& r, int p, int hd) {
 
 // One warp writes one cache row (one position of one KV head): K rotated
 // by the table row when one is given, V as is, both converted to the cache
-// type.
+// type.  PRODUCT: as q8_0_pair's.
+template <bool PRODUCT = false>
 __device__ __forceinline__ void append_row(const void* kin, const void* vin, int in_dt,
                                            size_t k_off, size_t v_off, const double2* rope_row,
                                            const CacheView& c, int64_t dst, int lane) {
@@ -100,8 +101,8 @@ __device__ __forceinline__ void append_row(const void* kin, const void* vin, int
     if (c.dtype == kQ8_0) {
       int8_t qk0, qk1, qv0, qv1;
       __half sk, sv;
-      q8_0_pair(k0, k1, qk0, qk1, sk);
-      q8_0_pair(v0, v1, qv0, qv1, sv);
+      q8_0_pair<PRODUCT>(k0, k1, qk0, qk1, sk);
+      q8_0_pair<PRODUCT>(v0, v1, qv0, qv1, sv);
       if (valid) {
         *reinterpret_cast<char2*>(static_cast<int8_t*>(c.k) + e) = make_char2(qk0, qk1);
         *reinterpret_cast<char2*>(static_cast<int8_t*>(c.v) + e) = make_char2(qv0, qv1);

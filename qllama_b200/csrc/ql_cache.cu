@@ -316,8 +316,8 @@ __global__ void __launch_bounds__(128) ragged_append_any_kernel(const __grid_con
   bool ok;
   const int64_t dst = cache_row(c, a.rows.seq[b], pos, kvh, a.status, ok);
   if (!ok) return;
-  append_row(a.k, a.v, a.in_dtype, static_cast<size_t>(r) * a.k_stride + static_cast<size_t>(kvh) * hd,
-             static_cast<size_t>(r) * a.v_stride + static_cast<size_t>(kvh) * hd, rope, c, dst, lane);
+  append_row<true>(a.k, a.v, a.in_dtype, static_cast<size_t>(r) * a.k_stride + static_cast<size_t>(kvh) * hd,
+                   static_cast<size_t>(r) * a.v_stride + static_cast<size_t>(kvh) * hd, rope, c, dst, lane);
 }
 
 namespace {

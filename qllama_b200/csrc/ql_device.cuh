@@ -442,13 +442,15 @@ __device__ __forceinline__ void rope_pair(float x0, float x1, double2 cs, float&
 // Q8_0 quantisation of one 32-value block held as 16 pairs by 16 consecutive
 // lanes (lane & 15 = pair index within the block).  Same rule as the GGUF
 // reference quantiser: d = amax/127, id = 1/d (0 if d == 0), q = round(x*id)
-// with ties away from zero, scale stored as f16(d).
+// with ties away from zero, scale stored as f16(d).  PRODUCT: d = amax times the f32 nearest to
+// 1/127 instead, the rule of ql_kv_append at every head size.
+template <bool PRODUCT = false>
 __device__ __forceinline__ void q8_0_pair(float x0, float x1, int8_t& q0, int8_t& q1,
                                           __half& scale) {
   float amax = fmaxf(fabsf(x0), fabsf(x1));
 #pragma unroll
   for (int o = 8; o > 0; o >>= 1) amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, o));
-  float d = amax / 127.0f;
+  float d = PRODUCT ? amax * (1.0f / 127.0f) : amax / 127.0f;
   float id = d != 0.0f ? 1.0f / d : 0.0f;
   float r0 = roundf(x0 * id), r1 = roundf(x1 * id);
   q0 = static_cast<int8_t>(r0 == r0 ? static_cast<int>(r0) : 0);

@@ -250,3 +250,19 @@ def test_pages_taken_under_capture(ctx, stream, cache, then):
         check(k, v)
         assert torch.equal(q_out, rotated(q, places).half())
     del graph
+
+
+@pytest.mark.parametrize("hd", [32, 64, 96, 128, 256])
+def test_q8_appends_have_one_rule(ctx, hd):
+    """ql_kv_append takes a Q8_0 block's d as max|x| times the f32 nearest to 1/127 whatever the
+    head size: for these maxima half of them then lies on the other side of a tie."""
+    hkv, n = 3, 66
+    v = normal(1, n, hkv, hd, dtype="bf16") * 0.2
+    b = v.view(-1, 32)
+    for i, m in enumerate((1.1171875, 1.6171875, 1.8671875)):
+        b[i::4, 5], b[i::4, 20], b[i::4, 31] = m, m / 2, -m / 2
+    kv = qb.KvCache(ctx, 1, 128, hkv, hd, "q8_0")
+    kv.append(0, v, v, [0], [n], THETA)
+    k, got = kv.read(0, [0], [n])
+    torch.testing.assert_close(got.double(), q8_plain(v.float()), rtol=0, atol=0)
+    torch.testing.assert_close(k.double(), q8_plain(rotated(v, range(n))), rtol=0, atol=0)
