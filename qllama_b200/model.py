@@ -244,6 +244,22 @@ def qkv_rope_append(kv, layer: int, x, wqkv_t, start_pos, num_heads: int, num_kv
     return q_rot
 
 
+def _numbers(x, batch, kind):
+    """A C array of `batch` numbers: that many, or one for all, in any form that numpy takes;
+    None if there are others."""
+    if type(x) is int:
+        return (kind * batch)(*((x,) * batch))
+    if type(x) in (list, tuple, range) and len(x) == batch:
+        try:
+            return (kind * batch)(*x)
+        except TypeError:  # not whole numbers
+            pass
+    x = np.asarray(x, dtype=np.int64).ravel()
+    if x.size not in (1, batch):
+        return None
+    return (kind * batch)(*np.broadcast_to(x, batch).tolist())
+
+
 def _appended_args(kv, layer, q_rot, start_pos, num_heads, num_kv_heads, head_dim, rope_theta,
                    seq_ids, out, out_dtype):
     """(AttnArgs, out) of attention over rows that are in the cache."""
@@ -256,13 +272,10 @@ def _appended_args(kv, layer, q_rot, start_pos, num_heads, num_kv_heads, head_di
     batch, new_len = shape[0], shape[1]
     t = out.dtype if out is not None else _named_type(out_dtype or "f32")
     out = _output(kv.ctx, out, (batch, new_len, num_heads * head_dim), t, "out")
-    if not hasattr(start_pos, "__len__"):
-        start_pos = [start_pos] * batch
-    if seq_ids is None:
-        seq_ids = range(batch)
-    if len(start_pos) != batch or len(seq_ids) != batch:
+    starts = _numbers(start_pos, batch, ctypes.c_int64)
+    seqs = _numbers(range(batch) if seq_ids is None else seq_ids, batch, ctypes.c_int32)
+    if starts is None or seqs is None:
         raise _invalid(f"one position and one sequence for each of {batch} rows of q_rot")
-    starts, seqs = (ctypes.c_int64 * batch)(*start_pos), (ctypes.c_int32 * batch)(*seq_ids)
     dev = kv.ctx.device
     args = qb.AttnArgs(layer, batch, new_len, seqs, starts, num_heads, num_kv_heads, head_dim,
                        rope_theta, _float_code(q_rot, "q_rot"), _float_code(out, "out"),
