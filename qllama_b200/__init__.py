@@ -7,9 +7,11 @@ for this path:
 * ``KvCache``  -- src/kv_cache/cache.rs (new / update / get / clear / seq_len),
   device resident and paged, with f32, f16, bf16, Q8_0 or Q4_0 storage and several
   sequence slots; and, with no counterpart there, ``append`` (new rows of sequences of
-  different lengths, rotated on the way) and ``read`` (rows back on the device), which
-  take CUDA tensors and are ordered with torch's current stream as the calls of
-  ``qllama_b200.model`` are;
+  different lengths, rotated on the way) and ``read`` (rows back on the device).  CUDA
+  tensors given to ``update``, ``append`` and ``read`` are ordered with torch's current
+  stream as in the calls of ``qllama_b200.model``; ``attention_forward`` and
+  ``attention_forward_sharded`` run on the context's stream and order nothing by
+  themselves;
 * ``attention_forward`` -- steps 3-7 of ``Attention::forward_with_cache``
   (src/transformer/layers.rs:397-455) on already projected Q/K/V;
 * ``Comm`` / ``attention_forward_sharded`` -- the same operator with the KV
@@ -280,7 +282,8 @@ class KvCache:
         self._h = h
 
     def update(self, layer: int, k, v, positions, seq: int = 0) -> None:
-        """cache.rs:83-170 -- k already rotated; shapes are checked as the reference does."""
+        """cache.rs:83-170 -- k already rotated; shapes are checked as the reference does.
+        CUDA tensors are ordered with torch's current stream, as in ``append``."""
         kp, mem, kk = _buffer(k)
         vp, mem2, vv = _buffer(v)
         if mem != mem2:
@@ -288,10 +291,17 @@ class KvCache:
         kd = (ctypes.c_int64 * max(1, len(kk.shape)))(*kk.shape)
         vd = (ctypes.c_int64 * max(1, len(vv.shape)))(*vv.shape)
         pos = _positions(positions)
+        side = None
+        if mem == MEM_DEVICE:
+            m = _model or _import_model()
+            m._L or m._start()
+            side = m._fork(self.ctx)
         _check(load().ql_kv_update(self.ctx._h, self._h, layer, seq, kp, kd, len(kk.shape), vp,
                                    vd, len(vv.shape), _dtype_code(kk),
                                    pos.ctypes.data_as(ctypes.POINTER(ctypes.c_int32)), pos.size,
                                    mem))
+        if side is not None:
+            m._join(self.ctx, side)
 
     def get(self, layer: int, positions, seq: int = 0):
         """cache.rs:185-229 -- returns f32 numpy arrays [n, num_kv_heads, head_dim]."""

@@ -266,3 +266,29 @@ def test_q8_appends_have_one_rule(ctx, hd):
     k, got = kv.read(0, [0], [n])
     torch.testing.assert_close(got.double(), q8_plain(v.float()), rtol=0, atol=0)
     torch.testing.assert_close(k.double(), q8_plain(rotated(v, range(n))), rtol=0, atol=0)
+
+
+@pytest.mark.parametrize("contiguous", [True, False])
+def test_update_with_tensors_of_another_stream(contiguous):
+    """KvCache.update of tensors that torch's current stream has yet to write, while the context
+    has a stream of its own; they are dropped, and their memory written to, right after it."""
+    hkv, hd, n = 2, 64, 100
+    c = qb.Context(0)
+    kv = qb.KvCache(c, 1, 128, hkv, hd, "f32")
+    side = torch.cuda.Stream()
+    rows = [normal(i, n, hkv, hd) for i in range(3)]
+    torch.cuda.synchronize()
+    for i in range(3):
+        with torch.cuda.stream(side):
+            torch.cuda._sleep(20_000_000)
+            k, v = rows[i] + 1, rows[i] - 1
+            if not contiguous:
+                k, v = (x.transpose(0, 1).contiguous().transpose(0, 1) for x in (k, v))
+            kv.update(0, k, v, range(n))
+            del k, v
+            junk = [torch.full((n, hkv, hd), 7.0, device="cuda") for _ in range(4)]
+            got = kv.read(0, [0], [n])
+        side.synchronize()
+        assert torch.equal(got[0], rows[i] + 1) and torch.equal(got[1], rows[i] - 1)
+        kv.truncate(0, 0)
+        del junk
