@@ -66,6 +66,8 @@ const char* ql_last_error(void);
 
 /* ---- context: one CUDA device, one stream, a reusable workspace ---- */
 int ql_ctx_create(int device, ql_ctx** out);
+/* No call takes the context after this; what has been made with it (caches, weights, models,
+ * communicators) may be destroyed before or after it. */
 int ql_ctx_destroy(ql_ctx* ctx);
 /* Use `stream` (a cudaStream_t; NULL = the context's own stream) for later calls. */
 int ql_ctx_set_stream(ql_ctx* ctx, void* stream);

@@ -107,7 +107,7 @@ int ql_fail(int code, const char* fmt, ...) {
 }
 
 struct ql_kv {
-  ql_ctx* ctx = nullptr;
+  ql_ctx_ref ctx;
   ql_kv_config cfg{};
   int pages_per_seq = 0;
   std::vector<void*> k, v;             // per layer (Q4_0: all in k)
@@ -489,6 +489,20 @@ void shorten(ql_kv* kv, int layer, int seq, int64_t len) {
 
 }  // namespace
 
+void ql_ctx_release(ql_ctx* c) {
+  if (c->users.fetch_sub(1, std::memory_order_acq_rel) != 1) return;
+  if (c->own) cudaStreamSynchronize(c->own);
+  if (c->ws) cudaFree(c->ws);
+  for (void* p : c->retired) cudaFree(p);
+  if (c->counters) cudaFree(c->counters);
+  if (c->status) cudaFree(c->status);
+  for (cudaEvent_t e : c->order)
+    if (e) cudaEventDestroy(e);
+  if (c->own) cudaStreamDestroy(c->own);
+  if (c->aside) cudaStreamDestroy(c->aside);
+  delete c;
+}
+
 int ql_ctx_workspace(ql_ctx* c, size_t bytes, void** out) {
   const int r = ensure_ws(c, bytes);
   if (r != QL_OK) return r;
@@ -716,16 +730,9 @@ int ql_ctx_create(int device, ql_ctx** out) {
 int ql_ctx_destroy(ql_ctx* c) {
   if (!c) return QL_OK;
   cudaSetDevice(c->device);
+  c->stream = c->own;  // the caller's may go now; caches that are left are destroyed on this one
   if (c->own) cudaStreamSynchronize(c->own);
-  if (c->ws) cudaFree(c->ws);
-  for (void* p : c->retired) cudaFree(p);
-  if (c->counters) cudaFree(c->counters);
-  if (c->status) cudaFree(c->status);
-  for (cudaEvent_t e : c->order)
-    if (e) cudaEventDestroy(e);
-  if (c->own) cudaStreamDestroy(c->own);
-  if (c->aside) cudaStreamDestroy(c->aside);
-  delete c;
+  ql_ctx_release(c);
   return QL_OK;
 }
 
@@ -1962,7 +1969,7 @@ static_assert(QL_COMM_MAX_RANKS == ql::kMaxRanks, "rank limit");
 }  // namespace
 
 struct ql_comm {
-  ql_ctx* ctx = nullptr;
+  ql_ctx_ref ctx;
   int nranks = 1;
   int rank = 0;
   int mode = QL_COMM_P2P;

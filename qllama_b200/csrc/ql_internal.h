@@ -24,6 +24,33 @@ struct ql_ctx {
   std::vector<void*> retired;   // outgrown workspaces and counters of captured graphs
   cudaEvent_t order[2] = {nullptr, nullptr};  // of ql_ctx_wait_stream and ql_ctx_join_stream
   cudaStream_t aside = nullptr;  // for what has to happen at once while `stream` is captured
+  std::atomic<int> users{1};     // its handle, and what has been made with it
+};
+
+// One user less; the last one's going frees the context.
+void ql_ctx_release(ql_ctx* c);
+
+// The context of a cache, a weight, a model or a communicator: it stays until the last of them
+// has gone, in whatever order a caller (or Python's collector) destroys them and the context.
+class ql_ctx_ref {
+ public:
+  ql_ctx_ref() = default;
+  ql_ctx_ref(const ql_ctx_ref&) = delete;
+  ql_ctx_ref& operator=(const ql_ctx_ref&) = delete;
+  ~ql_ctx_ref() {
+    if (c_) ql_ctx_release(c_);
+  }
+  ql_ctx_ref& operator=(ql_ctx* c) {
+    if (c) c->users.fetch_add(1, std::memory_order_relaxed);
+    if (c_) ql_ctx_release(c_);
+    c_ = c;
+    return *this;
+  }
+  operator ql_ctx*() const { return c_; }
+  ql_ctx* operator->() const { return c_; }
+
+ private:
+  ql_ctx* c_ = nullptr;
 };
 
 // Records the message of a failed call (ql_last_error) and returns `code`.

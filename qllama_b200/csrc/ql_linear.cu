@@ -440,7 +440,7 @@ cudaError_t launch_norm(const NormArgs& a, int num_sms, cudaStream_t s) {
 // 64 (32 bytes a tile, [g][h]) or of 128 (32 bytes for two tiles along the columns);
 // the four lanes of a quad read the same.
 struct ql_q4 {
-  ql_ctx* ctx = nullptr;
+  ql_ctx_ref ctx;
   int n = 0, k = 0, group = 0;
   int tiles = 0, chunks = 0;
   uint32_t* codes = nullptr;   // [tiles][chunks][32][4]

@@ -801,7 +801,7 @@ cudaError_t launch_sample(const ql_sampler_config& c, const float* logits, int v
 
 // -------------------------------------------------------------------- model --
 struct ql_llama {
-  ql_ctx* ctx = nullptr;
+  ql_ctx_ref ctx;
   ql_llama_config cfg{};
   int hd = 0, kvd = 0, qkv_cols = 0;
   float* embd = nullptr;      // [V, E]

@@ -292,3 +292,45 @@ def test_update_with_tensors_of_another_stream(contiguous):
         assert torch.equal(got[0], rows[i] + 1) and torch.equal(got[1], rows[i] - 1)
         kv.truncate(0, 0)
         del junk
+
+
+def test_a_context_may_go_first():
+    """Caches and weights outlive their context's handle, also in a cycle that the collector
+    takes apart in an order of its own; with the last of them the context's memory goes."""
+    import gc
+
+    def free():
+        gc.collect()
+        torch.cuda.synchronize()
+        torch.cuda.empty_cache()
+        return torch.cuda.mem_get_info()[0]
+
+    def use(c, kv):
+        q, k, v = (normal(i, 1, 300, h, 64) for i, h in ((1, 8), (2, 2), (3, 2)))
+        kv.truncate(0, 0)
+        return qb.attention_forward(kv, 0, q, k, v, 0, 8, 2, 64, THETA)
+
+    c = qb.Context(0)
+    use(c, qb.KvCache(c, 1, 1 << 14, 2, 64, "f32"))  # what is loaded once is loaded
+    del c
+    before = free()
+    for way in ("closed", "cycle"):
+        stream = torch.cuda.Stream()
+        c = qb.Context(0)
+        c.set_stream(stream.cuda_stream)
+        kv = qb.KvCache(c, 1, 1 << 16, 2, 64, "f32")
+        w = qm.Q4Weight(c, np.zeros((1 << 14, 1 << 11), np.uint8), np.zeros((1 << 14, 1 << 7), np.float16))
+        with torch.cuda.stream(stream):
+            use(c, kv)
+        assert free() < before - (64 << 20)
+        if way == "closed":
+            c.close()
+            c.close()
+            del stream
+            kv.close()
+            w.close()
+        else:
+            c.others, kv.others = [kv, w, c], [c, w]
+        del c, kv, w
+        stream = None
+        assert free() >= before - (8 << 20)
