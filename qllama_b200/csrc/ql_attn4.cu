@@ -211,9 +211,10 @@ __device__ __forceinline__ size_t row_offset(const Attn4Args& a, const Job& j, i
 
 }  // namespace
 
-// LO: q enters as two f16 parts; not needed where it is of 16 bits and arrives rotated (scaled
-// by its power of two, f16 holds all of a value's bits that are above 2^-38 of the row's
-// largest).
+// LO: q enters as two f16 parts; not needed where it is of 16 bits and arrives rotated: scaled by
+// its power of two it is left in steps of at most 2^-38 of the row's largest (of 2^-34 in the odd
+// places, which enter divided by 16), and those of bf16's eight bits that lie above them, or of
+// f16's eleven, are all there.
 template <int HD, bool LO>
 __global__ void __launch_bounds__(32 * Attn4Cfg<HD>::kWarps, 1)
     attn4_kernel(const __grid_constant__ Attn4Args a) {
@@ -306,8 +307,8 @@ __global__ void __launch_bounds__(32 * Attn4Cfg<HD>::kWarps, 1)
     // ------------------------------------------------------------- q --
     // Lane (g, tq) holds dims 32 b + 8 tq .. + 7 of row g: the columns of B in the order in
     // which the K words' nibbles come out (j and j + 4 together; odd ones, whose codes are
-    // 16 times as large, divided by 16).  Each row is scaled by a power of two to [2^6, 2^7):
-    // -8 times a block's sum stays in f16's range.
+    // 16 times as large, divided by 16).  Each row is scaled by a power of two to [2^14, 2^15):
+    // far from f16's subnormals, and a 32nd of a block's sum stays in f16's range.
     uint32_t qh[NB][2][2], ql[NB][2][2], qo;
     float f[2];
     {
@@ -369,7 +370,7 @@ __global__ void __launch_bounds__(32 * Attn4Cfg<HD>::kWarps, 1)
       mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 1));
       mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 2));
       const uint32_t bits = __float_as_uint(mx);
-      int e = static_cast<int>(bits >> 23) - 127 - 6;
+      int e = static_cast<int>(bits >> 23) - 127 - 14;
       if (bits == 0 || bits >= 0x7f800000u) e = 0;
       e = max(e, -100);
       const float down = pow2f(-e);
@@ -392,7 +393,7 @@ __global__ void __launch_bounds__(32 * Attn4Cfg<HD>::kWarps, 1)
           }
         s += __shfl_xor_sync(0xffffffffu, s, 1);
         s += __shfl_xor_sync(0xffffffffu, s, 2);
-        sums[b] = s * -8.f;
+        sums[b] = s * -0.03125f;  // -8 times it, by 2^8
       }
       // B of the K scales' product: column g, the sums' high parts under blocks 2 tq, 2 tq + 1
       // and what is left of them under the same scales again
@@ -547,7 +548,7 @@ __global__ void __launch_bounds__(32 * Attn4Cfg<HD>::kWarps, 1)
           const uint32_t* wp = reinterpret_cast<const uint32_t*>(st + kw_at + 32 * (s + e) * NB);
           mma_f16_k8(y[e], wp[0], wp[4 * NB], qo);
 #pragma unroll
-          for (int k = 0; k < 4; ++k) y[e][k] *= 1.f / 16777216.f;
+          for (int k = 0; k < 4; ++k) y[e][k] *= 256.f / 16777216.f;
 #pragma unroll
           for (int b = 0; b < NB; ++b) {
             float c[4];

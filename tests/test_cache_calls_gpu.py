@@ -334,3 +334,31 @@ def test_a_context_may_go_first():
         del c, kv, w
         stream = None
         assert free() >= before - (8 << 20)
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "f16"])
+@pytest.mark.parametrize("places", ["even", "odd", "all"])
+@pytest.mark.parametrize("hd", [64, 128])
+def test_queries_far_below_their_largest(ctx, dtype, places, hd):
+    """Rotated 16-bit queries with values 2^-22 of the row's largest and less, in either nibble
+    of the codes' words, on keys that are as much larger there."""
+    hq, hkv, m = 8, 2, 1000
+    k = normal(1, m, hkv, hd)
+    k[..., 32:] *= 2.0 ** 15
+    q = normal(2, 1, 1, hq, hd)
+    if dtype == "f16":  # 2^-24 is the least of its values
+        q[..., :32] *= 2.0 ** 8
+        k[..., :32] *= 2.0 ** -8
+    q[..., 32:] *= 2.0 ** (-22 if dtype == "bf16" else -14)
+    if places != "all":
+        q[..., 32 + (places == "even")::2] = 0
+    k[..., 32:] *= 2.0 ** (2 if dtype == "bf16" else -4)  # a 32nd of what the others give
+    k.clamp_(-5e5, 5e5)  # what a block of the cache can hold
+    q = q.to(torch.bfloat16 if dtype == "bf16" else torch.float16)
+    kv = qb.KvCache(ctx, 1, m, hkv, hd, "q4_0")
+    kv.update(0, k, normal(3, m, hkv, hd), range(m))
+    kc, vc = (x.double() for x in kv.read(0, [0], [m]))
+    assert torch.isfinite(kc).all()
+    out = qm.attention_forward_appended(kv, 0, q, [m - 1], hq, hkv, hd, THETA)
+    want, _ = attention(q[0], kc, vc, m - 1)
+    assert off_by(out.view(1, hq, hd), want) <= NORM
