@@ -52,6 +52,7 @@ constexpr float kLog2e4 = 1.4426950408889634f;
 // are 0.0005 of their norm off (with six bits free 0.003, and 8 x 32768 in 66.5 instead of 67.1
 // us; with one 0.0004 and 67.8 us).
 constexpr float kTop = 14.f, kSlack = 3.f;
+constexpr float kFused = 1 << 20;
 
 template <int HD>
 struct Attn4Cfg {
@@ -112,6 +113,12 @@ __device__ __forceinline__ float ex2(float x) {  // 2^x; -inf -> +0
 // Orders this thread's stores to shared memory before later bulk copies into it.
 __device__ __forceinline__ void fence_proxy_async_shared() {
   asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+}
+
+// A probability's exponent, not fused: the reference was taken from a rounded product, and where
+// that is above kFused, what the rounding left off would show.
+__device__ __forceinline__ float exponent(float y, float f, float ref) {
+  return __fsub_rn(__fmul_rn(y, f), ref);
 }
 
 __device__ __forceinline__ float half_of(const uint32_t& w, bool high) {
@@ -407,7 +414,10 @@ __global__ void __launch_bounds__(32 * Attn4Cfg<HD>::kWarps, 1)
         pair[k] = low ? rest : h;
       }
       qo = NB == 2 && tq >= 2 ? 0u : pack2<false>(pair[0], pair[1]);
-      const float fr = a.scale * kLog2e4 * 16777216.f * pow2f(e);
+      // (at most 2^100, for queries beyond 2^90: scores that differ at all, by 2^-72 before this
+      // factor, then leave one another no probability, with this factor as with the true one,
+      // which could leave f32's range)
+      const float fr = fminf(a.scale * kLog2e4 * 16777216.f * pow2f(e), 0x1p100f);
 #pragma unroll
       for (int k = 0; k < 2; ++k) f[k] = __shfl_sync(0xffffffffu, fr, (2 * tq + k) * 4);
     }
@@ -436,7 +446,9 @@ __global__ void __launch_bounds__(32 * Attn4Cfg<HD>::kWarps, 1)
     // else by what takes it to [2^-2, 2^-1).  vexp only falls then, when a scale would reach 2.
     constexpr int kUnset = 99;
     int vexp = kUnset;
-    bool fresh = true;
+    // of the references: not yet set, or beyond kFused, where each step computes its exponents anew
+    enum : int { kSet, kFar, kNone };
+    int state = kNone;
     uint32_t nans = 0;  // of row 2 tq + k: bit 4 k + b, that it sees a value of block b that is NaN
 
     // --------------------------------------------------------- the tiles --
@@ -602,7 +614,8 @@ __global__ void __launch_bounds__(32 * Attn4Cfg<HD>::kWarps, 1)
             p[e][k] = fmaf(y[e][k], f[k & 1], -ref[k & 1]);
             over |= p[e][k] > kTop;
           }
-        if (__any_sync(0xffffffffu, over) || fresh) {
+        if (__any_sync(0xffffffffu, over) || state != kSet) {
+          const bool fresh = state == kNone;
 #pragma unroll
           for (int k = 0; k < 2; ++k) {
             // NaN does not count
@@ -626,11 +639,11 @@ __global__ void __launch_bounds__(32 * Attn4Cfg<HD>::kWarps, 1)
               }
             }
           }
-          fresh = false;
+          state = __any_sync(0xffffffffu, fabsf(ref[0]) > kFused || fabsf(ref[1]) > kFused) ? kFar : kSet;
 #pragma unroll
           for (int e = 0; e < 2; ++e)
 #pragma unroll
-            for (int k = 0; k < 4; ++k) p[e][k] = fmaf(y[e][k], f[k & 1], -ref[k & 1]);
+            for (int k = 0; k < 4; ++k) p[e][k] = exponent(y[e][k], f[k & 1], ref[k & 1]);
         }
 #pragma unroll
         for (int e = 0; e < 2; ++e) {

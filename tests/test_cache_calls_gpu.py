@@ -12,7 +12,7 @@ import torch
 
 import qllama_b200 as qb
 from qllama_b200 import model as qm
-from tests.test_cache_ops_gpu import (THETA, attention, chosen, ctx, filled, keep_of, near, normal,  # noqa: F401
+from tests.test_cache_ops_gpu import (DT, THETA, attention, chosen, ctx, filled, keep_of, near, normal,  # noqa: F401
                                       on_stream, q4_plain, q8_plain, refuses, rotated, stored, stream,
                                       top, u)
 
@@ -362,3 +362,44 @@ def test_queries_far_below_their_largest(ctx, dtype, places, hd):
     out = qm.attention_forward_appended(kv, 0, q, [m - 1], hq, hkv, hd, THETA)
     want, _ = attention(q[0], kc, vc, m - 1)
     assert off_by(out.view(1, hq, hd), want) <= NORM
+
+
+@pytest.mark.parametrize("size", [1e25, 1e33, 1e36, 3e38])
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+@pytest.mark.parametrize("call", ["appended", "forward"])
+def test_queries_up_to_the_types_largest(ctx, size, dtype, call):
+    """The largest score takes all of the weight, and the output is its position's row."""
+    hq, hkv, hd, m = 8, 2, 128, 300
+    kv = qb.KvCache(ctx, 1, m + 1, hkv, hd, "q4_0")
+    kv.update(0, normal(1, m, hkv, hd, scale=1e-3), normal(2, m, hkv, hd), range(m))
+    q = (torch.rand(1, 1, hq, hd, device="cuda") * 2 - 1).mul_(0.7)
+    q[..., 64:] = 0
+    q = (q * size).to(DT[dtype])
+    if call == "forward":
+        row = normal(3, 1, 1, hkv, hd, scale=1e-3)
+        out = qb.attention_forward(kv, 0, q, row.to(q.dtype), row.to(q.dtype), [m], hq, hkv, hd, THETA)
+        q, n = rotated(q[0].float(), [m])[None], m + 1
+    else:
+        out, n = qm.attention_forward_appended(kv, 0, q, [m - 1], hq, hkv, hd, THETA), m
+    kc, vc = (x.double() for x in kv.read(0, [0], [n]))
+    x = torch.einsum("hgd,lhd->hgl", q[0, 0].double().view(hkv, -1, hd), kc)
+    best = x.argmax(-1)
+    want = torch.stack([vc[best[h], h] for h in range(hkv)])
+    # a probability of 1, rounded to f16 with its scale
+    torch.testing.assert_close(out.view(hkv, -1, hd).double(), want, rtol=2.0 ** -10, atol=1e-30)
+
+
+@pytest.mark.parametrize("size", [1.0, 1e9, 1e30, 3e38])
+@pytest.mark.parametrize("sign", [1, -1])
+def test_equal_scores_share_the_weight(ctx, size, sign):
+    """However large the scores: the output of equal keys is the mean of the values."""
+    B, hq, hkv, hd, m = 3, 8, 2, 128, 2000
+    kv = qb.KvCache(ctx, 1, m, hkv, hd, "q4_0", 64, B)
+    for b in range(B):
+        kv.update(0, normal(b, 1, hkv, hd, scale=1e-2).expand(m - b, -1, -1).contiguous(),
+                  normal(b + 9, m - b, hkv, hd), range(m - b), seq=b)
+    q = torch.full((B, 1, hq, hd), sign * size, device="cuda")
+    out = qm.attention_forward_appended(kv, 0, q, [m - 1 - b for b in range(B)], hq, hkv, hd, THETA)
+    for b in range(B):
+        mean = kv.read(0, [0], [m - b], [b])[1].double().mean(0).repeat_interleave(hq // hkv, 0)
+        assert off_by(out[b].view(hq, hd), mean) <= NORM
