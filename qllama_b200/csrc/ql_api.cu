@@ -1411,9 +1411,13 @@ static int attn_forward_impl(ql_ctx* c, ql_kv* kv, const ql_attn_args* a,
   ql::Attn4Args a4{};
   size_t a4_cta = 0, a4_warp = 0;
   if (q4_decode) {
-    a4.units = sparse ? n * ((group + 7) / 8) : (n * group + 7) / 8;
-    if (ql::attn4_plan(hd, c->num_sms, row_tiles, a->batch, hkv * a4.units, &a4, &a4_cta, &a4_warp))
-      return fail(QL_ERR_UNSUPPORTED, "more than %d tiles of keys in one call", 1 << 30);
+    const int64_t units = sparse ? 1LL * n * ((group + 7) / 8) : (1LL * n * group + 7) / 8;
+    const int64_t each = hkv * units;  // jobs of a sequence
+    a4.units = static_cast<int32_t>(units);
+    if (each > INT32_MAX || ql::attn4_plan(hd, c->num_sms, row_tiles, a->batch,
+                                           static_cast<int>(each), &a4, &a4_cta, &a4_warp))
+      return fail(QL_ERR_UNSUPPORTED, "more than %d tiles of keys, or %d groups of eight query "
+                  "rows of a sequence, in one call", 1 << 30, 1 << 22);
   }
   int tps = max_tiles, max_splits = 1;
   // Too few (token, KV head) jobs to fill half the SMs: the wide kernel, whose

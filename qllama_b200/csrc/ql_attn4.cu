@@ -857,7 +857,8 @@ int attn4_plan(int hd, int num_sms, const int* tiles, int batch, int jobs, Attn4
     total += static_cast<int64_t>(tiles[b]) * jobs;
     longest = std::max(longest, tiles[b]);
   }
-  if (total > (1 << 30)) return 1;
+  // (what the kernel's divide() takes; padding below adds no more than a share of each job)
+  if (total > (1 << 30) || jobs >= (1 << 22)) return 1;
   const int ctas = static_cast<int>(
       std::max<int64_t>(1, std::min<int64_t>(num_sms, (total + kMinTiles - 1) / kMinTiles)));
   a->per_cta = static_cast<int>((total + ctas - 1) / ctas);

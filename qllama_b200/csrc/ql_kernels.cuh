@@ -333,7 +333,8 @@ cudaError_t launch_ragged_read(const RaggedReadArgs& a, cudaStream_t s);
 cudaError_t launch_bounds(const BoundsArgs& a, cudaStream_t s);
 cudaError_t launch_select(const SelectArgs& a, cudaStream_t s);
 // Q4_0 decode: whether it applies; the split of the tiles (fills total, per_cta, per_warp,
-// aligned, stages and first, reports the bytes of the pieces; 1: too many tiles); the launch.
+// aligned, stages and first, reports the bytes of the pieces; 1: too many tiles or jobs); the
+// launch.
 bool attn4_supported(int hd, int page);
 int attn4_plan(int hd, int num_sms, const int* tiles, int batch, int jobs, Attn4Args* a,
                size_t* cta_bytes, size_t* warp_bytes);

@@ -44,3 +44,20 @@ def test_one_sequence_may_be_a_number():
 def test_other_numbers_of_them_are_refused(start_pos, seq_ids):
     with pytest.raises(qb.QllamaError, match="one position and one sequence"):
         args(start_pos, seq_ids)
+
+
+def test_plan_of_too_many_tiles_or_jobs():
+    """The Q4_0 kernel's quotients stay below 2^22 and its list below 2^30 places."""
+    plan = getattr(qb.load(), "_ZN2ql10attn4_planEiiPKiiiPNS_9Attn4ArgsEPmS4_")
+    args = ctypes.create_string_buffer(1 << 14)
+    a, b = ctypes.c_size_t(), ctypes.c_size_t()
+
+    def run(tiles, jobs, hd=128):
+        t = (ctypes.c_int32 * len(tiles))(*tiles)
+        return plan(hd, 148, t, len(tiles), jobs, args, ctypes.byref(a), ctypes.byref(b))
+
+    for hd in (64, 128):
+        assert run([1], (1 << 22) - 1, hd) == 0 and a.value > 0 and b.value > 0
+        assert run([1, 1], 1 << 22, hd) == 1
+        assert run([1 << 20], 1 << 10, hd) == 0
+        assert run([1 << 20], (1 << 10) + 1, hd) == 1
