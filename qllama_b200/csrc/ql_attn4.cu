@@ -239,6 +239,8 @@ __global__ void __launch_bounds__(32 * Attn4Cfg<HD>::kWarps, 1)
   // the last job of every warp's part, for the joining
   Job* last_job = reinterpret_cast<Job*>(smem + W * ring_bytes + W * S * 8);
   int* flag = reinterpret_cast<int*>(last_job + W);
+  int* died = flag + 2;  // of a warp whose copy did not come in time: that tile
+  static_assert(W * sizeof(Job) + (2 + W) * sizeof(int) <= W * 32 + 16, "smem()'s last part");
 
   const int c0 = blockIdx.x * a.per_cta, c1 = min(c0 + a.per_cta, a.total);
   const int w0 = min(c0 + warp * a.per_warp, c1), w1 = min(w0 + a.per_warp, c1);
@@ -453,7 +455,10 @@ __global__ void __launch_bounds__(32 * Attn4Cfg<HD>::kWarps, 1)
 
     // --------------------------------------------------------- the tiles --
     for (; x < seg1; ++x) {
-      if (alive) alive = !__any_sync(0xffffffffu, !mbar_wait(&full[stage], phase, a.status));
+      if (alive && __any_sync(0xffffffffu, !mbar_wait(&full[stage], phase, a.status))) {
+        alive = false;
+        died[warp] = x - w0;
+      }
       const uint8_t* st = ring + stage * C::kRecord;
       const int p0 = (x - job.t0) * kTile;
       const bool tail = p0 + kTile > all;
@@ -723,6 +728,12 @@ __global__ void __launch_bounds__(32 * Attn4Cfg<HD>::kWarps, 1)
     }
   }
 
+  // (the status says so; the warp's other copies in flight are waited for, as long again)
+  if (!alive) {
+#pragma unroll 1
+    for (int i = died[warp], n = min(i + S, w1 - w0); i < n; ++i)
+      mbar_wait(&full[i % S], i / S & 1, a.status);
+  }
   if (lane == 0 && w0 < w1) last_job[warp] = job;
 
   // ------------------------------------------------------------ joining --
