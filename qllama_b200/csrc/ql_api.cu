@@ -456,6 +456,10 @@ int64_t& len_at(ql_kv* kv, int layer, int seq) {
   return kv->len[static_cast<size_t>(layer) * kv->cfg.max_batch + seq];
 }
 
+int64_t len_at(const ql_kv* kv, int layer, int seq) {
+  return kv->len[static_cast<size_t>(layer) * kv->cfg.max_batch + seq];
+}
+
 int32_t& bounded_at(ql_kv* kv, int layer, int seq) {
   return kv->bounded[static_cast<size_t>(layer) * kv->cfg.max_batch + seq];
 }
@@ -1090,11 +1094,11 @@ int ql_kv_get(ql_ctx* c, const ql_kv* kv, int32_t layer, int32_t seq, const int3
 
 namespace {
 
-// The sequences of a call on rows packed one after the other: each slot once, its rows
-// [start, start + n) inside the cache's capacity (appended ones continue its prefix, read ones
-// lie in it).  Fills the launch's table and, per sequence, where its rows end.
-int ragged_rows(ql_kv* kv, const char* who, int layer, int batch, const int32_t* seq_ids,
-                const int64_t* start_pos, const int32_t* lens, bool append, ql::RaggedTable* t,
+// The sequences of a call on rows packed one after the other, their rows [start, start + n) inside
+// the cache's capacity: appended ones continue the prefix of a slot that is listed once, read ones
+// (append null) lie in it.  Fills the launch's table and, per sequence, where its rows end.
+int ragged_rows(const ql_kv* kv, const char* who, int layer, int batch, const int32_t* seq_ids,
+                const int64_t* start_pos, const int32_t* lens, ql_kv* append, ql::RaggedTable* t,
                 int64_t* ends) {
   if (layer < 0 || layer >= kv->cfg.num_layers)
     return fail(QL_ERR_INVALID, "KV cache layer index %d out of range (cache has %d layers)",
@@ -1103,16 +1107,16 @@ int ragged_rows(ql_kv* kv, const char* who, int layer, int batch, const int32_t*
     return fail(QL_ERR_INVALID, "batch %d is outside 0..%d", batch, ql::kMaxBatch);
   if (batch > 0 && (!seq_ids || !start_pos || !lens))
     return fail(QL_ERR_INVALID, "%s: seq_ids, start_pos or the lengths are NULL", who);
-  const uint32_t mark = next_seen_epoch(kv);
+  const uint32_t mark = append ? next_seen_epoch(append) : 0;
   int64_t total = 0;
   for (int b = 0; b < batch; ++b) {
     const int s = seq_ids[b];
     if (s < 0 || s >= kv->cfg.max_batch)
       return fail(QL_ERR_INVALID, "sequence %d out of range (cache has %d slots)", s,
                   kv->cfg.max_batch);
-    if (append && kv->seen_mark[s] == mark)
+    if (append && append->seen_mark[s] == mark)
       return fail(QL_ERR_INVALID, "sequence %d appears twice in one call", s);
-    kv->seen_mark[s] = mark;
+    if (append) append->seen_mark[s] = mark;
     const int64_t start = start_pos[b], n = lens[b], cur = len_at(kv, layer, s);
     if (n < 0) return fail(QL_ERR_INVALID, "sequence %d has %lld rows", s, (long long)n);
     if (start < 0) return fail(QL_ERR_INVALID, "start_pos %lld is negative", (long long)start);
@@ -1188,7 +1192,7 @@ int ql_kv_append(ql_ctx* c, ql_kv* kv, const ql_append_args* a) {
                 (long long)a->q_stride, (long long)a->k_stride, (long long)a->v_stride);
   int64_t ends[ql::kMaxBatch];
   int r = ragged_rows(kv, "ql_kv_append", a->layer_idx, a->batch, a->seq_ids, a->start_pos,
-                      a->new_len, true, &k.rows, ends);
+                      a->new_len, kv, &k.rows, ends);
   if (r != QL_OK) return r;
   const int64_t total = k.rows.first[a->batch];
   if (total == 0) return QL_OK;
@@ -1235,18 +1239,17 @@ int ql_kv_append(ql_ctx* c, ql_kv* kv, const ql_append_args* a) {
   return QL_OK;
 }
 
-int ql_kv_read(ql_ctx* c, const ql_kv* kv_in, int32_t layer, int32_t batch,
+int ql_kv_read(ql_ctx* c, const ql_kv* kv, int32_t layer, int32_t batch,
                const int32_t* seq_ids, const int64_t* start_pos, const int32_t* lens,
                int32_t out_dtype, void* k_out, void* v_out) {
-  if (!c || !kv_in) return fail(QL_ERR_INVALID, "ql_kv_read: NULL argument");
-  if (kv_in->ctx != c) return fail(QL_ERR_INVALID, "the cache belongs to another context");
-  ql_kv* kv = const_cast<ql_kv*>(kv_in);  // only the marks of the checks are written
+  if (!c || !kv) return fail(QL_ERR_INVALID, "ql_kv_read: NULL argument");
+  if (kv->ctx != c) return fail(QL_ERR_INVALID, "the cache belongs to another context");
   if (!valid_io_dtype(out_dtype)) return fail(QL_ERR_INVALID, "unknown output dtype %d", out_dtype);
   if (kv->cfg.num_kv_heads > (1 << 16))
     return fail(QL_ERR_UNSUPPORTED, "ql_kv_read takes up to %d KV heads", 1 << 16);
   ql::RaggedReadArgs k{};
   int64_t ends[ql::kMaxBatch];
-  const int r = ragged_rows(kv, "ql_kv_read", layer, batch, seq_ids, start_pos, lens, false,
+  const int r = ragged_rows(kv, "ql_kv_read", layer, batch, seq_ids, start_pos, lens, nullptr,
                             &k.rows, ends);
   if (r != QL_OK) return r;
   if (k.rows.first[batch] == 0) return QL_OK;

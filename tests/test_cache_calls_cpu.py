@@ -61,3 +61,17 @@ def test_plan_of_too_many_tiles_or_jobs():
         assert run([1, 1], 1 << 22, hd) == 1
         assert run([1 << 20], 1 << 10, hd) == 0
         assert run([1 << 20], (1 << 10) + 1, hd) == 1
+
+
+def test_reading_changes_nothing_of_the_cache():
+    """ql_kv_read takes the cache as const: two threads may read it at once."""
+    from tests.test_cache_ops_cpu import P, Cache, i32, i64, refused
+
+    c = Cache(lens=(100, 50, 0, 0))
+    before = ctypes.string_at(ctypes.addressof(c.kv), ctypes.sizeof(c.kv))
+    L = qb.load()
+    assert L.ql_kv_read(*c.args(), 0, 2, i32(0, 1), i64(100, 50), i32(0, 0), qb.F32, None, None) == qb.OK
+    refused(L.ql_kv_read(*c.args(), 0, 2, i32(0, 0), i64(0, 99), i32(9, 2), qb.F32, P, P + 32768),
+            "beyond the written prefix")
+    assert list(c.marks) == [0] * 4
+    assert ctypes.string_at(ctypes.addressof(c.kv), ctypes.sizeof(c.kv)) == before
