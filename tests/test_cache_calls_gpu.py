@@ -403,3 +403,71 @@ def test_equal_scores_share_the_weight(ctx, size, sign):
     for b in range(B):
         mean = kv.read(0, [0], [m - b], [b])[1].double().mean(0).repeat_interleave(hq // hkv, 0)
         assert off_by(out[b].view(hq, hd), mean) <= NORM
+
+
+# What the kernels' outputs may be off by relative to their norm, by the cache's type.  f16 and
+# bf16: queries and probabilities enter as two 16-bit parts (bf16: what is left is below 2^-17 of
+# them; scores are sums of up to 16 in magnitude here); Q8_0: queries as two 8-bit parts, 2^-16 of
+# the row's largest, which 128 channels add up to 2^-12.  A key left out of 20000 is 2^-7.1 off.
+NORMS = {"f32": 2.0 ** -12, "f16": 2.0 ** -12, "bf16": 2.0 ** -12, "q8_0": NORM, "q4_0": NORM}
+
+
+@pytest.mark.parametrize("cache", ["f16", "bf16", "q8_0", "q4_0"])
+@pytest.mark.parametrize("n", [1, 3])
+def test_no_key_of_a_long_cache_is_left_out(ctx, cache, n):
+    """Distances by norm, dense and over chosen blocks: a mean over many keys is small beside
+    its largest value, and so is what one of them adds."""
+    hq, hkv, hd, lens = 8, 2, 128, [4097, 20000, 130]
+    kv, rows = filled(ctx, cache, lens, hkv, hd)
+    q = normal(50, 3, n, hq, hd)
+    start = [m - n for m in lens]
+    out = qm.attention_forward_appended(kv, 0, q, start, hq, hkv, hd, THETA)
+    sel = torch.empty(3, n, hkv, 60, dtype=torch.int32, device="cuda")
+    part, _ = qm.attention_forward_sparse(kv, 0, q, start, hq, hkv, hd, 60, 1, 2, selected=sel)
+    for b, (k, v) in enumerate(rows):
+        want, _ = attention(q[b], k, v, start[b])
+        assert off_by(out[b].view(n, hq, hd), want) <= NORMS[cache]
+        pick = chosen(q[b], k, cache, start[b], 60, 1, 2)
+        assert torch.equal(sel[b], pick)
+        want, _ = attention(q[b], k, v, start[b], keep_of(pick, lens[b]))
+        assert off_by(part[b].view(n, hq, hd), want) <= NORMS[cache]
+
+
+@pytest.mark.parametrize("cache, hq, hkv, hd, n", [("f16", 24, 2, 128, 1), ("bf16", 16, 1, 64, 3),
+                                                   ("q8_0", 20, 2, 128, 1), ("f32", 12, 1, 128, 2),
+                                                   ("q4_0", 24, 2, 128, 2), ("q8_0", 8, 2, 64, 1)])
+def test_blocks_with_more_heads_on_a_kv_head(ctx, cache, hq, hkv, hd, n):
+    lens = [1500, 64, 700]
+    kv, rows = filled(ctx, cache, lens, hkv, hd)
+    q = normal(60, 3, n, hq, hd, dtype="bf16")
+    start = [m - n for m in lens]
+    sel = torch.empty(3, n, hkv, 5, dtype=torch.int32, device="cuda")
+    out, _ = qm.attention_forward_sparse(kv, 0, q, start, hq, hkv, hd, 5, 1, 1, selected=sel)
+    for b, (k, v) in enumerate(rows):
+        pick = chosen(q[b], k, cache, start[b], 5, 1, 1)
+        assert torch.equal(sel[b], pick)
+        want, _ = attention(q[b], k, v, start[b], keep_of(pick, lens[b]))
+        assert off_by(out[b].view(n, hq, hd), want) <= NORMS[cache]
+
+
+@pytest.mark.parametrize("cache", ["q4_0", "f16"])
+def test_a_sequence_alone_and_in_a_batch(ctx, cache):
+    """The split of the work goes by the whole batch, so a sequence's bits may differ with its
+    company, by roundings only; the blocks chosen do not."""
+    hq, hkv, hd, lens = 32, 8, 128, [3000, 100, 1700, 9000]
+    kv, _ = filled(ctx, cache, lens, hkv, hd)
+    q = normal(5, 4, 1, hq, hd, dtype="bf16")
+    start = [m - 1 for m in lens]
+
+    def run(seqs):
+        sel = torch.empty(len(seqs), 1, hkv, 9, dtype=torch.int32, device="cuda")
+        args = (q[seqs], [start[s] for s in seqs], hq, hkv, hd)
+        a = qm.attention_forward_appended(kv, 0, *args, THETA, seq_ids=seqs)
+        b, _ = qm.attention_forward_sparse(kv, 0, *args, 9, seq_ids=seqs, selected=sel)
+        return a.view(-1, hq, hd), b.view(-1, hq, hd), sel
+
+    a, b, sel = run([0, 1, 2, 3])
+    for s in range(4):
+        x, y, z = run([s])
+        assert torch.equal(z[0], sel[s])
+        assert off_by(x[0], a[s].double()) <= NORMS[cache] and off_by(y[0], b[s].double()) <= NORMS[cache]
