@@ -419,8 +419,12 @@ __device__ __forceinline__ void load_q_pairs(const AttnArgs& a, size_t row0, int
 }
 
 // Decode softmax: the running maximum used as reference lags the true one by
-// at most this much (log2 units), so probabilities stay below 2^8.
-constexpr float kLazyLog2 = 8.f;
+// at most kLazyLog2 (log2 units), and stands kLiftLog2 below the maximum it was
+// taken from, so probabilities stay below 2^15 and the smallest ones above
+// f16's subnormals as far as that allows: beside a position without a value
+// that is e^18 times as likely, the others' outputs are 0.0007 of their norm
+// off (0.074 with no lift).
+constexpr float kLazyLog2 = 8.f, kLiftLog2 = 7.f;
 
 __device__ __forceinline__ uint32_t swz128(int row, int chunk) {
   // byte offset of 16-byte chunk `chunk` (0..7) of row `row` in a 128B-swizzled box
@@ -954,13 +958,13 @@ __global__ void __launch_bounds__(SplitCfg<HD, DT, KG>::kThreads, SplitCfg<HD, D
       mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 1));
       mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 2));
       // The reference maximum moves only when the tile's maximum exceeds it
-      // by more than 2^kLazyLog2, so P stays below 2^kLazyLog2 and (m, l, O)
-      // stay consistent; the rescale of O then happens a few times per split
+      // by more than 2^kLazyLog2, so P stays below 2^(kLazyLog2 + kLiftLog2) and
+      // (m, l, O) stay consistent; the rescale of O then happens a few times per split
       // instead of whenever one of the eight heads sees a new maximum.
       const bool bump = mx > m + kLazyLog2;  // always taken while m is -inf and mx is not
       const float corr = bump ? exp2f(m - mx) : 1.f;  // 0 when m was -inf
       if (bump) m = mx;
-      const float base = m == -CUDART_INF_F ? 0.f : m;
+      const float base = m == -CUDART_INF_F ? 0.f : m - kLiftLog2;
       float p[4], psum = 0.f;
 #pragma unroll
       for (int e = 0; e < 4; ++e) {

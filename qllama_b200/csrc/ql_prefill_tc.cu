@@ -51,6 +51,10 @@ constexpr int kBM = 128;  // query rows per CTA
 constexpr int kBN = 128;  // keys per KV tile
 constexpr float kLog2eP = 1.4426950408889634f;
 constexpr float kRescaleLog2 = 8.f;  // rescale O only when the max grows by more than 2^8
+// The reference stands this far below the maximum: P, below 2^15, keeps the most of f16's range
+// for positions that are much less likely than another one (e^18 times: outputs 0.006 of their
+// norm off, with no lift 0.62).
+constexpr float kLiftLog2 = 7.f;
 
 // ------------------------------------------------------------ tcgen05 PTX --
 __device__ __forceinline__ void tmem_alloc(uint32_t* dst_smem, uint32_t ncols) {
@@ -512,8 +516,8 @@ __global__ void __launch_bounds__(PrefillCfg<HD, NQ>::kThreads, 1)
       mx = __fmul_rn(mx, sl2);
       float corr = 1.f;
       bool rescale = false;
-      if (mx > m_used + kRescaleLog2 || m_used == -CUDART_INF_F) {
-        const float m_new = mx == -CUDART_INF_F ? 0.f : mx;
+      if (mx > m_used + (kRescaleLog2 + kLiftLog2) || m_used == -CUDART_INF_F) {
+        const float m_new = mx == -CUDART_INF_F ? 0.f : mx - kLiftLog2;
         corr = ex2_approx(m_used - m_new);  // 0 while nothing has been accumulated
         rescale = j > 0 && m_used != -CUDART_INF_F;
         m_used = m_new;
@@ -522,11 +526,11 @@ __global__ void __launch_bounds__(PrefillCfg<HD, NQ>::kThreads, 1)
       // multiply by exactly 1.
       rescale = __any_sync(0xffffffffu, rescale);
       // p = 2^(s*scale*log2e - m), packed f16 pairs over S's first 64 columns.
-      // m_used is the rounded product max(s)*scale*log2e; a fused multiply-add
-      // against it is off by up to half an ulp of that product, harmless
+      // m_used is the rounded product max(s)*scale*log2e less the lift; a fused
+      // multiply-add against it is off by up to half an ulp of that product, harmless
       // below 2^20 but an overflow of 2^(...) for scores far above any
       // attention's usual range, where the rounded products are subtracted
-      // instead (the largest then gives exactly 2^0).
+      // instead (the largest then gives 2^7, or 2^0 where the lift is below an ulp).
       float ps[4] = {0.f, 0.f, 0.f, 0.f};
       auto emit_p = [&](auto exact) {
 #pragma unroll

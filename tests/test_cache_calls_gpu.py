@@ -471,3 +471,38 @@ def test_a_sequence_alone_and_in_a_batch(ctx, cache):
         x, y, z = run([s])
         assert torch.equal(z[0], sel[s])
         assert off_by(x[0], a[s].double()) <= NORMS[cache] and off_by(y[0], b[s].double()) <= NORMS[cache]
+
+
+@pytest.mark.parametrize("cache", ["f16", "bf16", "q8_0", "q4_0"])
+@pytest.mark.parametrize("n, gap", [(1, 10), (1, 14), (1, 18), (64, 10), (64, 14)])
+def test_every_kernel_beside_a_position_without_a_value(ctx, cache, n, gap):
+    """As test_small_values_beside_a_position_without_any, for every storage type and for
+    prompts, dense and over chosen blocks.
+
+    Prompts round queries, keys and values to f16, 2^-11 of each at most: of independent errors
+    less than NORM comes of it, but the first position's score is one product, whose error of
+    2^-11 * gap is in every output's sum of weights.
+    Beside a gap of 18, decode over f16 and Q8_0 has probabilities that are e^-18 of 2^7: they
+    lose up to half of f16's smallest step, 2^-25, and their root mean square is
+    2^(7 - 18 * 1.4427) * e = 2^-17.5 (scores are normal with a variance of 1): 2^-7.5."""
+    B, hq, hkv, hd, m = 3, 8, 2, 128, 2050
+    kv = qb.KvCache(ctx, 1, m, hkv, hd, cache, 64, B)
+    for b in range(B):
+        k, v = normal(b, m, hkv, hd), normal(b + 100, m, hkv, hd, scale=0.01)
+        k[0], v[0] = 0, 0
+        k[:, :, 0] = 0
+        k[0, :, 0] = 8
+        kv.update(0, k, v, range(m), seq=b)
+    q = normal(200, B, n, hq, hd)
+    q[..., 0] = gap * math.sqrt(hd) / 8
+    start = [m - n] * B
+    few = 2.0 ** -7.5 if gap == 18 else NORM
+    out = qm.attention_forward_appended(kv, 0, q, start, hq, hkv, hd, THETA)
+    sel = torch.empty(B, n, hkv, 20, dtype=torch.int32, device="cuda")
+    part, _ = qm.attention_forward_sparse(kv, 0, q, start, hq, hkv, hd, 20, 1, 1, selected=sel)
+    for b in range(B):
+        kc, vc = (x.double() for x in kv.read(0, [0], [m], [b], out_dtype="f32"))
+        want, _ = attention(q[b], kc, vc, start[b])
+        assert off_by(out[b].view(n, hq, hd), want) <= (NORM + gap * 2.0 ** -11 if n >= 64 else few)
+        want, _ = attention(q[b], kc, vc, start[b], keep_of(sel[b], m))
+        assert off_by(part[b].view(n, hq, hd), want) <= few
