@@ -122,8 +122,9 @@ int ql_attn_forward_appended(ql_ctx* ctx, ql_kv* kv, const ql_attn_args* args);
  * own: the first `first`, the newest `last`, and of the others those of the largest scores,
  * the lower block of equal ones.  A token that sees no more than `blocks` blocks attends to
  * all of them, as ql_attn_forward_appended does.
- * Block j's score for a KV head bounds from above what any of its keys can score, summed
- * over the head's group of queries:
+ * Block j's score for a KV head stands for the most that any of its keys can score, summed
+ * over the head's group of queries (a bound from above for f16 and bf16 caches, whose keys lo and
+ * hi hold exactly; of other types a term may be 2^-9 of itself short of it, by the rounding):
  *   sum_h sum_d max(q_hd * lo_jd, q_hd * hi_jd),
  * with lo and hi the least and the largest value of channel d among the block's stored keys
  * (dequantised; rounded to f16 for an f16 cache, else to bf16), evaluated in f64.  A score
@@ -134,8 +135,11 @@ int ql_attn_forward_appended(ql_ctx* ctx, ql_kv* kv, const ql_attn_args* args);
  * and scored before the capture as they then are: when those rows have been replaced
  * (truncated and appended anew), make an uncaptured call on the sequences before the replay,
  * or capture again.  Rows that replays of captured appends rewrite are followed by the calls
- * made or captured after the append's capture.  selected (may be NULL) receives each list in ascending order, -1 behind
- * its end.  args->mem must be QL_MEM_DEVICE; batch * new_len is at most 65535. */
+ * made or captured after the append's capture: each such call scores again the blocks between
+ * the first and the last that captured appends have written in the slot, for the cache's whole
+ * life, so captures of long appends are best made on slots of their own.
+ * selected (may be NULL) receives each list in ascending order, -1 behind its end.  args->mem
+ * must be QL_MEM_DEVICE; batch * new_len is at most 65535. */
 typedef struct {
   int32_t blocks;     /* >= first + last */
   int32_t first;      /* >= 0 */
