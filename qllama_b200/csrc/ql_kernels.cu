@@ -957,14 +957,15 @@ __global__ void __launch_bounds__(SplitCfg<HD, DT, KG>::kThreads, SplitCfg<HD, D
       }
       mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 1));
       mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 2));
-      // The reference maximum moves only when the tile's maximum exceeds it
-      // by more than 2^kLazyLog2, so P stays below 2^(kLazyLog2 + kLiftLog2) and
+      // The reference m moves only when the tile's maximum exceeds the one it was
+      // taken from by more than 2^kLazyLog2, so P stays below 2^(kLazyLog2 + kLiftLog2) and
       // (m, l, O) stay consistent; the rescale of O then happens a few times per split
       // instead of whenever one of the eight heads sees a new maximum.
-      const bool bump = mx > m + kLazyLog2;  // always taken while m is -inf and mx is not
-      const float corr = bump ? exp2f(m - mx) : 1.f;  // 0 when m was -inf
-      if (bump) m = mx;
-      const float base = m == -CUDART_INF_F ? 0.f : m - kLiftLog2;
+      const bool bump = mx > m + (kLazyLog2 + kLiftLog2);  // always taken while m is -inf and mx is not
+      const float next = mx - kLiftLog2;
+      const float corr = bump ? exp2f(m - next) : 1.f;  // 0 when m was -inf
+      if (bump) m = next;
+      const float base = m == -CUDART_INF_F ? 0.f : m;
       float p[4], psum = 0.f;
 #pragma unroll
       for (int e = 0; e < 4; ++e) {
