@@ -568,12 +568,12 @@ __global__ void __launch_bounds__(PrefillCfg<HD, NQ>::kThreads, 1)
         const int ev = tile_exp[v_exp_off + j];
         if (ev > ev_used) {
           if (j > 0) {
-            ocorr *= pow2f(ev_used - ev);
+            ocorr *= pow2f(max(ev_used - ev, -126));
             rescale = true;
           }
           ev_used = ev;
         } else if (ev < ev_used) {
-          const float pf = pow2f(ev - ev_used);
+          const float pf = pow2f(max(ev - ev_used, -126));
           tmem_wait_st();
 #pragma unroll
           for (int c = 0; c < kBN / 64; ++c) {
@@ -765,8 +765,9 @@ __global__ void __launch_bounds__(128) prefill_prologue_kernel(const __grid_cons
 // threads per key row (each HD/2 values: bf16 as stored, Q8_0 and
 // Q4_0 dequantised exactly in f32, the integer times its block's f16 scale).  The tile is divided by
 // 2^e, e = f16_range_exp of its largest magnitude (0 for ordinary data;
-// otherwise the power of two that puts the tile into [2^14, 2^15)), and e goes
-// to tile_exp for the attention kernel to fold back.  bf16 values convert
+// otherwise the power of two that puts the tile into [2^14, 2^15), small tiles
+// of V into [2^-2, 2^6)), and e goes to tile_exp for the attention kernel to
+// fold back.  bf16 values convert
 // exactly at that scale, apart from magnitudes under 2^(e-24); dequantised
 // Q8_0 and Q4_0 values (up to 19 and 15 significant bits) round to f16's 11.  Keys past the
 // sequence's end (and rows of unallocated pages) are zeros.  Converting once
@@ -863,7 +864,15 @@ __global__ void __launch_bounds__(256) tiles_to_f16_kernel(const __grid_constant
   uint32_t tb = wmax[0];
 #pragma unroll
   for (int i = 1; i < 8; ++i) tb = max(tb, wmax[i]);
-  const int e = f16_range_exp(tb);
+  int e = f16_range_exp(tb);
+  if (kind) {
+    // V: from 2^-2 on left alone, smaller ones times 2^8, 2^16, ..: 12 powers of two below the
+    // largest are in f16's normal range, and tiles of like values mostly have one exponent.  (P
+    // takes what neighbours differ by, and keeps its bits over some 2^20: see the attention
+    // kernel.)
+    const int top = static_cast<int>(tb >> 23) - 127;
+    if (top < -2) e = -8 * min((-2 - top + 7) / 8, 15);
+  }
   const float f = pow2f(-e);
   const int kv_tiles = a.kv_rows / kBN;
   if (threadIdx.x == 0)

@@ -506,3 +506,49 @@ def test_every_kernel_beside_a_position_without_a_value(ctx, cache, n, gap):
         assert off_by(out[b].view(n, hq, hd), want) <= (NORM + gap * 2.0 ** -11 if n >= 64 else few)
         want, _ = attention(q[b], kc, vc, start[b], keep_of(sel[b], m))
         assert off_by(part[b].view(n, hq, hd), want) <= few
+
+
+@pytest.mark.parametrize("cache", ["bf16", "q8_0", "q4_0", "f16"])
+@pytest.mark.parametrize("hd", [64, 128])
+@pytest.mark.parametrize("size", [1e-4, 2e-4, 2.4e-4, 3e-4, 1e-3, 0.06, 1e-6, 1.0, 6e3])
+@pytest.mark.parametrize("tiles", ["alike", "apart"])
+def test_prompts_over_values_of_any_size(ctx, cache, hd, size, tiles):
+    """Values around the sizes at which tiles of an f16 copy begin to be scaled, and far from
+    them; tiles of like values, and of values up to 2^10 apart.
+
+    Queries, keys, values and probabilities are rounded to f16: independent errors of 2^-11 at
+    most, of which scores collect theirs over hd products (variance 1): 4 * 2^-11."""
+    B, hq, hkv, n, m = 2, 6, 3, 70, 1000
+    kv = qb.KvCache(ctx, 1, m, hkv, hd, cache, 64, B)
+    for b in range(B):
+        v = normal(b + 100, m, hkv, hd, scale=size)
+        if tiles == "apart":
+            v *= 2.0 ** (((torch.arange(m, device="cuda") // 64) * 7 + b) % 11 - 10)[:, None, None]
+        if cache == "f16" and size < 1e-2:
+            v *= 1e2 if size > 1e-5 else 1e4  # such a cache's own steps
+        kv.update(0, normal(b, m, hkv, hd), v, range(m), seq=b)
+    q = normal(200, B, n, hq, hd)
+    out = qm.attention_forward_appended(kv, 0, q, [m - n] * B, hq, hkv, hd, THETA)
+    for b in range(B):
+        kc, vc = (x.double() for x in kv.read(0, [0], [m], [b], out_dtype="f32"))
+        want, _ = attention(q[b], kc, vc, m - n)
+        off = (out[b].view(n, hq, hd).double() - want).norm(dim=-1)
+        assert (off <= 4 * 2.0 ** -11 * want.norm(dim=-1)).all()  # (0: what a Q8_0 scale rounds off)
+
+
+def test_small_rows_in_front_of_large_ones(ctx):
+    """The first rows of a prompt see only values that are 2^-8 of those further on in their
+    tile: as exact as the others."""
+    B, hq, hkv, hd, n = 3, 4, 2, 128, 130
+    kv = qb.KvCache(ctx, 1, n, hkv, hd, "bf16", 64, B)
+    for b, size in enumerate((1e-4, 2.0, 1e-7)):
+        v = normal(b + 10, n, hkv, hd, scale=size)
+        v[:64] *= 2.0 ** -8
+        kv.update(0, normal(b, n, hkv, hd), v, range(n), seq=b)
+    q = normal(200, B, n, hq, hd)
+    out = qm.attention_forward_appended(kv, 0, q, [0] * B, hq, hkv, hd, THETA)
+    for b in range(B):
+        kc, vc = (x.double() for x in kv.read(0, [0], [n], [b], out_dtype="f32"))
+        want, _ = attention(q[b], kc, vc, 0)
+        # (rounding of values and scores as above)
+        assert off_by(out[b].view(n, hq, hd), want) <= 4 * 2.0 ** -11
