@@ -244,6 +244,9 @@ def qkv_rope_append(kv, layer: int, x, wqkv_t, start_pos, num_heads: int, num_kv
     return q_rot
 
 
+_first = {}  # batch -> the sequences 0 .. batch - 1 (the library only reads them)
+
+
 def _numbers(x, batch, kind):
     """A C array of `batch` numbers: that many, or one for all, in any form that numpy takes;
     None if there are others."""
@@ -273,7 +276,10 @@ def _appended_args(kv, layer, q_rot, start_pos, num_heads, num_kv_heads, head_di
     t = out.dtype if out is not None else _named_type(out_dtype or "f32")
     out = _output(kv.ctx, out, (batch, new_len, num_heads * head_dim), t, "out")
     starts = _numbers(start_pos, batch, ctypes.c_int64)
-    seqs = _numbers(range(batch) if seq_ids is None else seq_ids, batch, ctypes.c_int32)
+    if seq_ids is not None:
+        seqs = _numbers(seq_ids, batch, ctypes.c_int32)
+    elif (seqs := _first.get(batch)) is None:
+        seqs = _first[batch] = (ctypes.c_int32 * batch)(*range(batch))
     if starts is None or seqs is None:
         raise _invalid(f"one position and one sequence for each of {batch} rows of q_rot")
     dev = kv.ctx.device
